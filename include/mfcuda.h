@@ -3,7 +3,8 @@
  * data-parallel hot path: dtype conversion, packed Int4 group dequant,
  * axpy / scalar-broadcast vector loops, fused elementwise chains and
  * per-tensor amax-scaled FP8 quantisation (single tensor and whole
- * checkpoints sharded over several GPUs).
+ * checkpoints sharded over several GPUs), and a decoding step over a paged
+ * key-value cache (page tables, rotary positions, cache writes, attention).
  *
  * Conventions
  *   - Plain C types only: pointers, int32_t/int64_t/size_t, float.
@@ -18,7 +19,7 @@
  *   - No entry point synchronises the host with the device except the ones
  *     whose name says so (mf_stream_sync, mf_event_sync, mf_device_sync) and
  *     the set-up calls (mf_init, mf_alloc, mf_free, mf_fused_compile,
- *     mf_comm_init). Scalar results such as amax are written to device
+ *     mf_comm_init, mf_paged_attn_create). Scalar results such as amax are written to device
  *     memory, never returned to the host (manifesto
  *     scripts/check_banned.sh:28-40 forbids host syncs on the launch path).
  *   - Arithmetic follows manifesto's Go scalar code bit for bit, including
@@ -100,6 +101,7 @@ typedef void* mf_event;  /* cudaEvent_t */
 typedef struct mf_fused_kernel_s* mf_fused_kernel;
 typedef struct mf_comm_s* mf_comm;
 typedef struct mf_ckpt_plan_s* mf_ckpt_plan;
+typedef struct mf_paged_attn_s* mf_paged_attn;
 
 /* ---------------------------------------------------------------------
  * Lifecycle and errors
@@ -127,6 +129,9 @@ int mf_device_status(int* device_code);
 /* Device status code of a bounded wait that gave up (a bulk-copy stage that
  * never landed, or mf_wait_flag's flag that was never set). */
 #define MF_DEVICE_TIMEOUT 0x7100
+/* Device status code of a page number or slot outside its cache: nothing was
+ * read or written there (the token counts as masked). */
+#define MF_DEVICE_BAD_PAGE 0x7200
 /* Make `stream` wait until the int at device address `flag` equals `expect`
  * (acquire load, polled with a short sleep), for at most `max_polls` polls;
  * if it never does, record MF_DEVICE_TIMEOUT in the sticky status and let the
@@ -432,6 +437,161 @@ int mf_ckpt_plan_run(mf_ckpt_plan plan, float* d_amax, float* d_scale_inv, mf_st
 int mf_ckpt_plan_run_passes(mf_ckpt_plan plan, int passes, float* d_amax, float* d_scale_inv, mf_stream stream);
 int mf_ckpt_plan_info(mf_ckpt_plan plan, int32_t* n_groups, int32_t* grid, int64_t* elements);
 int mf_ckpt_plan_destroy(mf_ckpt_plan plan);
+
+/* ---------------------------------------------------------------------
+ * K10: a decoding step over a paged key-value cache.  The reference declares
+ * the state (page_table: Int32 [capacity], paged_tensor: zeroed storage,
+ * runtime/session.go:160-205) and keeps its books on the host
+ * (runtime/paged_plan.go:14-177); it has no device code for it, so the
+ * formulas below are the definition.
+ *
+ * A cache is n_pages pages of page_size tokens; token `off` of page `page`
+ * has, for each of kv_heads heads, head_dim contiguous elements at
+ *   page * page_stride + off * token_stride + head * head_stride   (elements)
+ * for the keys and again, in another buffer, for the values: both orders of
+ * heads and tokens inside a page, and padded ones, are strides.  Slot s is
+ * token s % page_size of page s / page_size.  Elements are F32, BF16 or F16,
+ * or FP8 codes; the value of a code of head h is decode(code) * scale_inv[h]
+ * (float32 per head on the device; NULL = 1), as mf_fp8_quantize's scale_inv.
+ * ------------------------------------------------------------------- */
+typedef struct mf_cache_layout {
+    int32_t dtype;
+    int32_t kv_heads;
+    int32_t head_dim;
+    int32_t page_size;
+    int64_t n_pages;
+    int64_t page_stride; /* elements */
+    int64_t token_stride;
+    int64_t head_stride;
+} mf_cache_layout;
+
+/* Page tables and slots of a step's new tokens, from the requests' lengths.
+ * Request r holds lens[r] tokens and gets new_tokens[r] more (negative counts
+ * as 0).  With page size P, held = ceil(lens / P), need = ceil((lens + new) / P)
+ * - held and before = the sum of need over the requests in front of r:
+ *   a request fits when ceil((lens + new) / P) <= max_pages and (need == 0 or
+ *   before + need <= pool[1]); one without room in its table needs no pages;
+ *   table[r][held + j] = free_pages[pool[0] + before + j],  j < need, if it fits;
+ *   starts[r] = sum of new in front of r, starts[n_requests] = their total;
+ *   token i = starts[r] + t: positions[i] = lens[r] + t, owner[i] = r,
+ *   slots[i] = table[r][positions[i] / P] * P + positions[i] % P, or -1 if r
+ *   does not fit; lens_after[r] = lens[r] + new[r] if it fits, else lens[r];
+ *   pool_after = {pool[0] + taken, pool[1] - taken, total of new, requests
+ *   that do not fit}, taken = the largest before + need that fits.
+ * pool is {index of the first free page in free_pages, number of free pages};
+ * free_pages holds at least pool[0] + pool[1] page numbers.  slots, positions
+ * and owner have `tokens` entries: those past the total get -1, 0, -1, and
+ * tokens past `tokens` have no entry (the table is complete all the same).
+ * Inputs are not changed (lens_after and pool_after are other buffers than
+ * lens and pool), so a step can be planned again.  One launch. */
+typedef struct mf_page_config {
+    int32_t page_size;
+    int32_t max_pages;    /* entries of a request's table row */
+    int64_t table_stride; /* int32 entries from one row to the next, >= max_pages */
+} mf_page_config;
+int mf_page_assign(const mf_page_config* config, const int32_t* lens, const int32_t* new_tokens,
+                   int32_t n_requests, int32_t* table, const int32_t* free_pages, const int32_t* pool,
+                   int64_t tokens, int64_t* slots, int32_t* positions, int32_t* owner, int32_t* starts,
+                   int32_t* lens_after, int32_t* pool_after, mf_stream stream);
+
+/* Rotary positions.  The first rot_dim elements of a head are rot_dim / 2
+ * pairs (a, b): (x[i], x[i + rot_dim/2]) in the HALF layout, (x[2i], x[2i+1])
+ * in the INTERLEAVED one.  With angle = position * inv_freq[i]:
+ *   a' = magnitude * (a cos - b sin),  b' = magnitude * (b cos + a sin);
+ * the elements past rot_dim pass through.  inverse != 0 turns by -angle, which
+ * is the gradient: dx = rope(dy, inverse).  The angle is formed and reduced in
+ * float64 (a float32 product loses the phase of far positions), the rest is
+ * float32, rounded once to the dtype (F32, BF16 or F16).  Positions are any
+ * int32.  src and dst are [tokens, heads, head_dim] with head_dim contiguous
+ * and strides in elements; dst may be src with the same strides. */
+enum mf_rope_layout { MF_ROPE_HALF = 0, MF_ROPE_INTERLEAVED = 1 };
+typedef struct mf_rope_config {
+    int32_t dtype;
+    int32_t head_dim;
+    int32_t rot_dim; /* even, <= head_dim, <= 1024 */
+    int32_t layout;  /* mf_rope_layout */
+    float magnitude;
+    const float* inv_freq; /* device, rot_dim / 2 */
+} mf_rope_config;
+int mf_rope(const mf_rope_config* config, int inverse, const void* src, int64_t src_token_stride,
+            int64_t src_head_stride, void* dst, int64_t dst_token_stride, int64_t dst_head_stride,
+            const int32_t* positions, int64_t tokens, int32_t heads, mf_stream stream);
+/* The frequencies, computed in float64 and rounded to float32 once (host only):
+ * base^(-2i/rot_dim), then
+ *   LINEAR  divided by factor;
+ *   BASE    with the base times factor^(rot_dim / (rot_dim - 2));
+ *   BANDS   with turns = original_length * f / 2 pi and ramp = clamp((turns -
+ *           low_turns) / (high_turns - low_turns), 0, 1):
+ *           (1 - ramp) * f / factor + ramp * f. */
+enum mf_rope_scaling { MF_ROPE_NONE = 0, MF_ROPE_LINEAR = 1, MF_ROPE_BASE = 2, MF_ROPE_BANDS = 3 };
+int mf_rope_frequencies(int32_t rot_dim, double base, int scaling, double factor, double original_length,
+                        double low_turns, double high_turns, float* inv_freq);
+
+/* A step's queries and keys rotated (as mf_rope), keys and values written to
+ * their slots: q_out[t][h] = rope(q[t][h]); cache_k at slots[t] =
+ * encode(rope(k[t][h])), cache_v = encode(v[t][h]).  An FP8 cache stores
+ * encode(x * (1 / scale_inv[head])) with the encoder of `compat`; any other
+ * cache has the inputs' dtype.  A slot of -1 (any negative) writes no key or
+ * value; one past the cache neither, and records MF_DEVICE_BAD_PAGE.  Two
+ * tokens of a call must not share a slot.  q_out may be q with the same
+ * strides.  Strides in elements; inputs BF16, F16 or F32. */
+typedef struct mf_rope_append_config {
+    mf_rope_config rope;
+    mf_cache_layout cache;
+    int32_t q_heads;
+    int32_t compat;
+    const float* k_scale_inv; /* [kv_heads] on the device, or NULL */
+    const float* v_scale_inv;
+    int64_t q_token_stride, q_head_stride;
+    int64_t k_token_stride, k_head_stride;
+    int64_t v_token_stride, v_head_stride;
+    int64_t out_token_stride, out_head_stride;
+} mf_rope_append_config;
+int mf_rope_append(const mf_rope_append_config* config, const void* q, const void* k, const void* v, void* q_out,
+                   void* k_cache, void* v_cache, const int32_t* positions, const int64_t* slots, int64_t tokens,
+                   mf_stream stream);
+
+/* Attention of one new token per request over the paged cache.  Query head h
+ * reads key-value head h / (q_heads / kv_heads).  Request r sees the tokens
+ * n of [first, len), len = lens[r] (clamped to the table's reach) and first =
+ * max(0, len - window) (window 0 = all), token n in page table[r][n / page_size]:
+ *   s_n = scale * (q . k_n)            then, if softcap > 0, softcap * tanh(s_n / softcap)
+ *         + slopes[h] * (n - (len - 1))
+ *   out = sum_n exp(s_n) v_n / sum_n exp(s_n),  lse = log(sum_n exp(s_n))
+ * A request that sees nothing gets out = 0 and lse = -inf.  A page number
+ * outside the cache masks its tokens and records MF_DEVICE_BAD_PAGE; table
+ * entries past the last page are not read.
+ * q and out: [n_requests, q_heads, head_dim] of q_dtype (BF16 or F16) with
+ * head_dim contiguous; lse (may be NULL): float32 [n_requests, q_heads].  The
+ * cache's dtype is q_dtype, F8E4M3 or F8E5M2; head_dim is a multiple of 8 (of
+ * 16 for FP8) up to 256; cache buffers and strides are multiples of 16 bytes.
+ * Products and sums are float32, the weights exp(s - max) enter the product
+ * with the values as two 16-bit terms (their sum has 16 bits or more).
+ *
+ * A handle holds the description and the workspace of the split (about 10 MB):
+ * create it once, run it for every step and layer.  A handle is not shared
+ * between streams that run at once.  One launch per run, no host sync; results
+ * do not depend on the order in which the parts finish. */
+typedef struct mf_paged_attn_config {
+    mf_cache_layout cache;
+    int32_t q_dtype;
+    int32_t q_heads;
+    int32_t max_pages;    /* entries of a request's table row */
+    int32_t window;       /* 0: all tokens */
+    int64_t table_stride; /* int32 entries */
+    float scale;
+    float softcap;            /* 0: none */
+    const float* slopes;      /* [q_heads] on the device, or NULL */
+    const float* k_scale_inv; /* [kv_heads] on the device, or NULL */
+    const float* v_scale_inv;
+    int64_t q_token_stride, q_head_stride;
+    int64_t out_token_stride, out_head_stride;
+} mf_paged_attn_config;
+int mf_paged_attn_create(const mf_paged_attn_config* config, mf_paged_attn* handle);
+int mf_paged_attn_run(mf_paged_attn handle, const void* q, const void* k_cache, const void* v_cache,
+                      const int32_t* table, const int32_t* lens, int32_t n_requests, void* out, float* lse,
+                      mf_stream stream);
+int mf_paged_attn_destroy(mf_paged_attn handle);
 
 /* ---------------------------------------------------------------------
  * Measurement.  No counterpart in the reference (it has no device code).

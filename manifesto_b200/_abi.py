@@ -42,11 +42,89 @@ class FusedProgram(ctypes.Structure):
     ]
 
 
+class CacheLayout(ctypes.Structure):
+    """mf_cache_layout: dtype, shape and strides (elements) of a paged key or value cache."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("n_pages", ctypes.c_int64),
+        ("page_stride", ctypes.c_int64),
+        ("token_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+    ]
+
+
+class PageConfig(ctypes.Structure):
+    """mf_page_config."""
+
+    _fields_ = [("page_size", ctypes.c_int32), ("max_pages", ctypes.c_int32), ("table_stride", ctypes.c_int64)]
+
+
+class RopeConfig(ctypes.Structure):
+    """mf_rope_config."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("rot_dim", ctypes.c_int32),
+        ("layout", ctypes.c_int32),
+        ("magnitude", ctypes.c_float),
+        ("inv_freq", ctypes.c_void_p),
+    ]
+
+
+class RopeAppendConfig(ctypes.Structure):
+    """mf_rope_append_config."""
+
+    _fields_ = [
+        ("rope", RopeConfig),
+        ("cache", CacheLayout),
+        ("q_heads", ctypes.c_int32),
+        ("compat", ctypes.c_int32),
+        ("k_scale_inv", ctypes.c_void_p),
+        ("v_scale_inv", ctypes.c_void_p),
+        ("q_token_stride", ctypes.c_int64),
+        ("q_head_stride", ctypes.c_int64),
+        ("k_token_stride", ctypes.c_int64),
+        ("k_head_stride", ctypes.c_int64),
+        ("v_token_stride", ctypes.c_int64),
+        ("v_head_stride", ctypes.c_int64),
+        ("out_token_stride", ctypes.c_int64),
+        ("out_head_stride", ctypes.c_int64),
+    ]
+
+
+class PagedAttnConfig(ctypes.Structure):
+    """mf_paged_attn_config."""
+
+    _fields_ = [
+        ("cache", CacheLayout),
+        ("q_dtype", ctypes.c_int32),
+        ("q_heads", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("window", ctypes.c_int32),
+        ("table_stride", ctypes.c_int64),
+        ("scale", ctypes.c_float),
+        ("softcap", ctypes.c_float),
+        ("slopes", ctypes.c_void_p),
+        ("k_scale_inv", ctypes.c_void_p),
+        ("v_scale_inv", ctypes.c_void_p),
+        ("q_token_stride", ctypes.c_int64),
+        ("q_head_stride", ctypes.c_int64),
+        ("out_token_stride", ctypes.c_int64),
+        ("out_head_stride", ctypes.c_int64),
+    ]
+
+
 _vp = ctypes.c_void_p
 _i32 = ctypes.c_int32
 _i64 = ctypes.c_int64
 _int = ctypes.c_int
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 _sz = ctypes.c_size_t
 
 # name -> argtypes (every function returns int status except where noted)
@@ -107,6 +185,13 @@ SIGNATURES: dict[str, list] = {
     "mf_ckpt_plan_run_passes": [_vp, _int, _vp, _vp, _vp],
     "mf_ckpt_plan_info": [_vp, ctypes.POINTER(_i32), ctypes.POINTER(_i32), ctypes.POINTER(_i64)],
     "mf_ckpt_plan_destroy": [_vp],
+    "mf_page_assign": [ctypes.POINTER(PageConfig), _vp, _vp, _i32, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    "mf_rope": [ctypes.POINTER(RopeConfig), _int, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i32, _vp],
+    "mf_rope_frequencies": [_i32, _f64, _int, _f64, _f64, _f64, _f64, ctypes.POINTER(_f32)],
+    "mf_rope_append": [ctypes.POINTER(RopeAppendConfig), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp],
+    "mf_paged_attn_create": [ctypes.POINTER(PagedAttnConfig), ctypes.POINTER(_vp)],
+    "mf_paged_attn_run": [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp],
+    "mf_paged_attn_destroy": [_vp],
 }
 
 _lib: ctypes.CDLL | None = None

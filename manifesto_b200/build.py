@@ -32,6 +32,9 @@ SOURCES = [
     "ckpt.cu",
     "fused.cu",
     "fused_jit.cu",
+    "pages.cu",
+    "rope.cu",
+    "paged_attn.cu",
     "comm.cu",
     "probe.cu",
 ]

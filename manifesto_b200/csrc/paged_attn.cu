@@ -1,0 +1,967 @@
+// paged_attn.cu -- attention of one new token per request over a paged
+// key-value cache (mf_paged_attn_*).
+//
+// For request r and query head h over its tokens n:
+//   s_n = scale * q.k_n  (capped, biased),  out = sum exp(s_n) v_n / sum exp(s_n).
+// One pass over the cache with a running maximum m and sum l: a new maximum
+// multiplies what is summed so far by exp(m_old - m_new).  Parts of a request
+// summed apart join the same way, from their (m, l, unnormalised out).
+//
+// Bound: HBM.  Each key and value byte is used for the query heads of its
+// key-value head only (4 operations per element and query head: 8 heads on
+// BF16 are 32 operations for 2 bytes), far below what tensor cores need to
+// be the limit, so the design is about keeping loads in flight:
+//   * The work is cut into tiles of 16 tokens of one (request, key-value head,
+//     block of 8 * NT query heads) item, laid end to end over all requests;
+//     every warp of the grid takes an equal run of tiles, whatever the lengths.
+//   * A warp works alone: its own ring of stages in shared memory filled by
+//     16-byte cp.async (rows of masked tokens are zero-filled, not read), no
+//     CTA barrier inside the loop.  Page numbers are read one tile ahead.
+//   * Products run on mma.m16n8k16 with tokens (then head_dim) on the long side
+//     and query heads on the side of 8: S^T = K Q^T and O^T = V^T P^T, so one
+//     key-value head with up to 8 query heads wastes nothing more; the weights
+//     move from the first product's result layout to the second's operand
+//     layout by movmatrix, in registers.  The wide tensor-core form
+//     (tcgen05) needs 64 or more rows of queries to be fed: there are 1 to 16.
+//   * exp(s - m) is rounded to two 16-bit terms (high and low), so the weights
+//     carry 16 bits (BF16) or more and the result's only 16-bit rounding that
+//     counts is the final one.
+//   * FP8 codes become f16 in registers (exact); the queries are then f16 too,
+//     scaled by a power of two per head so that none overflows.
+// Where a run of tiles ends inside an item, the warps of a CTA join their
+// parts in shared memory, CTAs through the workspace: the last of an item's
+// CTAs to arrive (a ticket) joins them in the order of the tokens, so the
+// result does not depend on who was last.
+#include <new>
+
+#include "mf_runtime.h"
+#include "mf_vec.cuh"
+
+namespace mf {
+namespace {
+
+constexpr int kTile = 16;          // tokens of a tile
+constexpr float kLog2e = 1.44269504088896341f;
+constexpr float kLn2 = 0.693147180559945309f;
+
+struct AttnArgs {
+    const void* q;
+    const void* k;
+    const void* v;
+    const int32_t* table;
+    const int32_t* lens;
+    void* out;
+    float* lse;
+    const float* slopes;
+    const float* k_scale;
+    const float* v_scale;
+    float* warp_part;     // [workers][NT * 8 * (DP + 2)]: parts that end inside a warp's run
+    float* cta_part;      // [CTAs][2][NT * 8 * (DP + 2)]: parts that leave the CTA
+    int32_t* tickets;     // [CTAs], zero between runs
+    int32_t* status;
+    int64_t q_req, q_head, out_req, out_head;
+    int64_t page_stride, token_stride, head_stride, table_stride;
+    int64_t n_pages;
+    int32_t n_requests, q_heads, kv_heads, group, blocks;  // blocks of query heads per key-value head
+    int32_t head_dim, page, max_pages, window, q_f16;
+    float scale, softcap;
+};
+
+// ------------------------------------------------------------------ pieces
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+template <bool BF16>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (BF16)
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    uint32_t r;
+    if constexpr (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+template <bool BF16>
+__device__ __forceinline__ void unpack2(uint32_t v, float& lo, float& hi) {
+    if constexpr (BF16) {
+        lo = __uint_as_float(v << 16);
+        hi = __uint_as_float(v & 0xffff0000u);
+    } else {
+        f16x2_to_f32x2(v, lo, hi);
+    }
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// Two FP8 codes -> f16x2, exact.
+template <int DT>
+__device__ __forceinline__ uint32_t fp8x2_to_f16x2(uint32_t two) {
+    if constexpr (DT == MF_DT_F8E4M3) return e4m3x2_to_f16x2(two);
+    else return __byte_perm(two, 0u, 0x1404u);
+}
+// exp2(m_old - m_new) for m_old <= m_new, 1 where both are the same infinity.
+__device__ __forceinline__ float rescale(float m_old, float m_new) {
+    return m_old == m_new ? 1.0f : exp2_fast(m_old - m_new);
+}
+
+// Tokens that request r sees, and the first of them.
+__device__ __forceinline__ int32_t seen_tokens(const AttnArgs& a, int32_t r, int32_t& first) {
+    const int64_t reach = static_cast<int64_t>(a.max_pages) * a.page;
+    int32_t len = max(__ldg(a.lens + r), 0);
+    if (len > reach) len = static_cast<int32_t>(reach);
+    const int32_t n = a.window > 0 ? min(len, a.window) : len;
+    first = len - n;
+    return n;
+}
+__device__ __forceinline__ int64_t tiles_of(int32_t tokens) { return (static_cast<int64_t>(tokens) + kTile - 1) / kTile; }
+
+// A place in the row of all tiles: request, item of the request, tile of the item.
+struct Place {
+    int32_t r, item, t, nt;   // nt: tiles of the request's items
+    int32_t n, first;         // tokens it sees
+    __device__ __forceinline__ void next(const AttnArgs& a, int32_t items) {
+        if (++t < nt) return;
+        t = 0;
+        if (++item < items) return;
+        item = 0;
+        while (++r < a.n_requests) {
+            n = seen_tokens(a, r, first);
+            nt = static_cast<int32_t>(tiles_of(n));
+            if (nt > 0) return;
+        }
+        nt = 0;
+    }
+};
+
+// What is known of one part of an item that a warp or CTA summed.
+struct Part {
+    int64_t start;   // first tile of the item in the row of all tiles; -1: no part
+    int32_t r, item, nt;
+    int32_t ta, tb;  // its tiles of the item
+};
+
+// MODE: dtype of the cache; DP: head_dim padded to 64, 128 or 256; NT: blocks
+// of 8 query heads a warp holds; W: warps; S: stages of a warp's ring.
+template <int MODE, int DP, int NT, int W, int S>
+struct Attn {
+    static constexpr bool kFp8 = MODE == MF_DT_F8E4M3 || MODE == MF_DT_F8E5M2;
+    static constexpr bool kBf16 = MODE == MF_DT_BF16;
+    static constexpr int kBytes = kFp8 ? 1 : 2;
+    static constexpr int kRow = DP * kBytes;          // bytes of a token's row
+    static constexpr int kChunks = kRow / 16;         // 16-byte pieces of a row
+    static constexpr int kStage = 2 * kTile * kRow;   // keys, then values
+    static constexpr int kSteps = DP / 16;            // products of 16 along head_dim
+    static constexpr int kHeads = 8 * NT;
+    static constexpr int kLd = DP + 4;                // floats of a staged head's row (spread over the banks)
+    static constexpr int kPart = kHeads * (DP + 2);   // floats of a part in the workspace: out, then m, l
+    static constexpr int kThreads = 32 * W;
+    static constexpr int kRing = W * S * kStage;
+    static constexpr int kStaged = W * kHeads * kLd * 4;
+    static constexpr int kBuffer = kRing > kStaged ? kRing : kStaged;
+
+    struct Shared {
+        int64_t prefix[kThreads + 1];   // tiles of the requests in front of each thread's
+        int64_t warp_sum[W];
+        Part part[2 * W];               // first and last part of each warp
+        float m[2 * W][kHeads], l[2 * W][kHeads];
+        int32_t mask[W][S];             // tokens of each stage that are there
+        int32_t joins[2];               // whether this CTA joins the item of its slot
+    };
+    static constexpr int kSharedBytes = kBuffer + static_cast<int>(sizeof(Shared));
+};
+
+// Piece `c` of row `row` of a tile: the pieces of a row are exchanged so that
+// eight rows of one column fall on different banks.
+template <int CHUNKS>
+__device__ __forceinline__ uint32_t swizzled(int row, int c) {
+    if constexpr (CHUNKS >= 8) return static_cast<uint32_t>(row * CHUNKS + (c ^ (row & 7))) * 16u;
+    else return static_cast<uint32_t>(row * CHUNKS + (c ^ ((row >> 1) & (CHUNKS - 1)))) * 16u;
+}
+
+// Write `f` (4 floats of head h, elements d..d+3, normalised) to the output.
+__device__ __forceinline__ void store_out4(const AttnArgs& a, int32_t r, int32_t head, int d, float4 f) {
+    if (d >= a.head_dim) return;
+    char* p = static_cast<char*>(a.out) + 2 * (r * a.out_req + head * a.out_head + d);
+    const float v[4] = {f.x, f.y, f.z, f.w};
+    uint32_t w[2];
+    if (a.q_f16) encode4<MF_DT_F16>(v, w, 0);
+    else encode4<MF_DT_BF16>(v, w, 0);
+    *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+}
+
+__device__ __forceinline__ void store_lse(const AttnArgs& a, int32_t r, int32_t head, float m, float l) {
+    if (a.lse) a.lse[static_cast<int64_t>(r) * a.q_heads + head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+template <int MODE, int DP, int NT, int W, int S>
+__global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a) {
+    using K = Attn<MODE, DP, NT, W, S>;
+    extern __shared__ __align__(128) unsigned char smem[];
+    auto& sh = *reinterpret_cast<typename K::Shared*>(smem + K::kBuffer);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int g = lane >> 2, j = lane & 3;  // row and column pair of a product's fragment
+    const int32_t items = a.kv_heads * a.blocks;
+
+    // requests that see nothing
+    for (int32_t r = blockIdx.x; r < a.n_requests; r += gridDim.x) {
+        int32_t first;
+        if (seen_tokens(a, r, first) > 0) continue;
+        for (int i = tid; i < a.q_heads * (a.head_dim / 4); i += K::kThreads)
+            store_out4(a, r, i / (a.head_dim / 4), i % (a.head_dim / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f));
+        for (int i = tid; i < a.q_heads; i += K::kThreads) store_lse(a, r, i, 0.0f, 0.0f);
+    }
+
+    // prefix of the tiles: thread i sums `per` consecutive requests
+    const int32_t per = (a.n_requests + K::kThreads - 1) / K::kThreads;
+    int64_t sum = 0;
+    for (int32_t i = 0; i < per; ++i) {
+        const int32_t r = tid * per + i;
+        int32_t first;
+        if (r < a.n_requests) sum += tiles_of(seen_tokens(a, r, first)) * items;
+    }
+    int64_t inc = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int64_t x = __shfl_up_sync(0xffffffffu, inc, d);
+        if (lane >= d) inc += x;
+    }
+    if (lane == 31) sh.warp_sum[warp] = inc;
+    if (lane < 2) sh.part[2 * warp + lane].start = -1;
+    __syncthreads();
+    int64_t total = 0, base = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+        if (w == warp) base = total;
+        total += sh.warp_sum[w];
+    }
+    sh.prefix[tid] = base + inc - sum;
+    if (tid == 0) sh.prefix[K::kThreads] = total;
+    __syncthreads();
+    if (total == 0) return;
+    const int64_t want = (total + W - 1) / W;
+    const int64_t ctas = want < gridDim.x ? want : gridDim.x;
+    if (blockIdx.x >= ctas) return;
+    const int64_t workers = ctas * W;
+    const int64_t id = static_cast<int64_t>(blockIdx.x) * W + warp;
+    const int64_t x0 = total * id / workers, x1 = total * (id + 1) / workers;
+    const int64_t my_tiles = x1 - x0;
+
+    uint32_t qf[NT][K::kSteps][2];
+    float o[NT][K::kSteps][4];
+    float m[NT][2], l[NT][2], scale[NT][2], slope[NT][2];
+    if (my_tiles > 0) {
+        // the place of tile x0: the thread whose requests hold it, then the request among them
+        int lo = 0, hi = K::kThreads;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (sh.prefix[mid] <= x0) lo = mid;
+            else hi = mid;
+        }
+        Place at{};
+        int64_t before = sh.prefix[lo];
+        for (int32_t r0 = lo * per;; r0 += 32) {
+            int32_t first = 0, n = 0;
+            if (r0 + lane < a.n_requests) n = seen_tokens(a, r0 + lane, first);
+            const int64_t mine = tiles_of(n) * items;
+            int64_t upto = mine;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int64_t x = __shfl_up_sync(0xffffffffu, upto, d);
+                if (lane >= d) upto += x;
+            }
+            const uint32_t past = __ballot_sync(0xffffffffu, before + upto > x0);
+            if (past || r0 + 32 >= a.n_requests) {
+                const int src = past ? __ffs(past) - 1 : 0;
+                at.r = r0 + src;
+                at.n = __shfl_sync(0xffffffffu, n, src);
+                at.first = __shfl_sync(0xffffffffu, first, src);
+                before += __shfl_sync(0xffffffffu, upto - mine, src);
+                break;
+            }
+            before += __shfl_sync(0xffffffffu, upto, 31);
+        }
+        at.nt = static_cast<int32_t>(tiles_of(at.n));
+        const int64_t in_request = x0 - before;
+        at.item = static_cast<int32_t>(in_request / at.nt);
+        at.t = static_cast<int32_t>(in_request % at.nt);
+
+        const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * (S * K::kStage);
+        Place load = at;
+        int64_t to_load = my_tiles;
+        int32_t page_no = -1, page_off = 0;
+        bool there = false;
+        const int row = lane & 15;
+        // the page of this lane's row of the tile at `load`
+        auto look_up = [&]() {
+            const int32_t p = load.t * kTile + row;
+            there = to_load > 0 && p < load.n;
+            if (there) {
+                const int32_t tok = load.first + p;
+                page_off = tok % a.page;
+                page_no = __ldg(a.table + load.r * a.table_stride + tok / a.page);
+            }
+        };
+        auto issue = [&](int stage) {
+            if (to_load > 0) {
+                bool ok = there;
+                if (ok && (page_no < 0 || page_no >= a.n_pages)) {
+                    ok = false;
+                    atomicExch(a.status, MF_DEVICE_BAD_PAGE);
+                }
+                const int32_t kv = load.item / a.blocks;
+                int64_t off = ok ? page_no * a.page_stride + page_off * a.token_stride + kv * a.head_stride : -1;
+                const uint32_t mask = __ballot_sync(0xffffffffu, ok) & 0xffffu;
+                if (lane == 0) sh.mask[warp][stage] = static_cast<int32_t>(mask);
+                const uint32_t dst = ring + stage * K::kStage;
+#pragma unroll
+                for (int i = 0; i < kTile * K::kChunks / 32; ++i) {
+                    const int piece = i * 32 + lane, rw = piece / K::kChunks, c = piece % K::kChunks;
+                    const int64_t o = __shfl_sync(0xffffffffu, off, rw);
+                    const bool get = o >= 0 && c * (16 / K::kBytes) < a.head_dim;
+                    const int64_t byte = get ? o * K::kBytes + c * 16 : 0;
+                    const uint32_t to = dst + swizzled<K::kChunks>(rw, c);
+                    cp_async16(to, static_cast<const char*>(a.k) + byte, get ? 16u : 0u);
+                    cp_async16(to + kTile * K::kRow, static_cast<const char*>(a.v) + byte, get ? 16u : 0u);
+                }
+                load.next(a, items);
+                --to_load;
+                look_up();
+            }
+            cp_async_commit();
+        };
+        look_up();
+#pragma unroll
+        for (int s = 0; s < S - 1; ++s) issue(s);
+
+        int32_t ta = at.t, kv = 0, head0 = 0;
+        int stage = 0;
+        for (int64_t i = 0; i < my_tiles; ++i) {
+            cp_async_wait<S - 2>();
+            __syncwarp();
+            issue(stage == 0 ? S - 1 : stage - 1);
+            if (i == 0 || at.t == 0) {
+                // a new item: its queries
+                ta = at.t;
+                kv = at.item / a.blocks;
+                head0 = kv * a.group + at.item % a.blocks * K::kHeads;
+                const int32_t heads = min(K::kHeads, (kv + 1) * a.group - head0);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const int h = n * 8 + g;
+                    const char* q = static_cast<const char*>(a.q) + 2 * (at.r * a.q_req + (head0 + h) * a.q_head);
+                    float top = 0.0f;
+#pragma unroll
+                    for (int c = 0; c < K::kSteps; ++c) {
+                        uint32_t w0 = 0, w1 = 0;
+                        if (h < heads) {
+                            const int d0 = K::kFp8 ? c * 16 + 4 * j : c * 16 + 2 * j;
+                            const int d1 = K::kFp8 ? d0 + 2 : d0 + 8;
+                            if (d0 < a.head_dim) w0 = __ldg(reinterpret_cast<const uint32_t*>(q + 2 * d0));
+                            if (d1 < a.head_dim) w1 = __ldg(reinterpret_cast<const uint32_t*>(q + 2 * d1));
+                        }
+                        qf[n][c][0] = w0;
+                        qf[n][c][1] = w1;
+                        if constexpr (K::kFp8) {
+                            float f[4];
+                            if (a.q_f16) {
+                                unpack2<false>(w0, f[0], f[1]);
+                                unpack2<false>(w1, f[2], f[3]);
+                            } else {
+                                unpack2<true>(w0, f[0], f[1]);
+                                unpack2<true>(w1, f[2], f[3]);
+                            }
+                            top = fmaxf(top, fmaxf(fmaxf(fabsf(f[0]), fabsf(f[1])), fmaxf(fabsf(f[2]), fabsf(f[3]))));
+                        }
+                    }
+                    float back = 1.0f;
+                    if constexpr (K::kFp8) {
+                        // f16 queries, scaled by a power of two to a largest magnitude in [1, 2)
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                        const uint32_t field = __float_as_uint(top) >> 23;  // biased exponent
+                        const bool scales = field >= 1 && field <= 254;
+                        const uint32_t e = min(field, 253u);
+                        const float fit = scales ? __uint_as_float((254u - e) << 23) : 1.0f;
+                        back = scales ? __uint_as_float(e << 23) : 1.0f;
+#pragma unroll
+                        for (int c = 0; c < K::kSteps; ++c)
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) {
+                                float f0, f1;
+                                if (a.q_f16) unpack2<false>(qf[n][c][x], f0, f1);
+                                else unpack2<true>(qf[n][c][x], f0, f1);
+                                qf[n][c][x] = pack2<false>(f0 * fit, f1 * fit);
+                            }
+                    }
+                    const float ks = a.k_scale ? __ldg(a.k_scale + kv) : 1.0f;
+                    // head 2j + x of this lane's columns: its scale is with the lanes of row 2j + x
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const float b = __shfl_sync(0xffffffffu, back, (2 * j + x) * 4);
+                        scale[n][x] = a.scale * ks * b;
+                        const int hx = n * 8 + 2 * j + x;
+                        slope[n][x] = a.slopes && hx < heads ? __ldg(a.slopes + head0 + hx) * kLog2e : 0.0f;
+                        if (!(a.softcap > 0.0f)) scale[n][x] *= kLog2e;
+                        m[n][x] = -INFINITY;
+                        l[n][x] = 0.0f;
+                    }
+#pragma unroll
+                    for (int c = 0; c < K::kSteps; ++c)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) o[n][c][x] = 0.0f;
+                }
+            }
+
+            // S^T = K Q^T, two chains of sums
+            const uint32_t keys = ring + stage * K::kStage, values = keys + kTile * K::kRow;
+            float s[NT][2][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) s[n][0][x] = s[n][1][x] = 0.0f;
+            {
+                const int rw = (lane & 7) + ((lane >> 3) & 1) * 8, ch = lane >> 4;
+                if constexpr (!K::kFp8) {
+#pragma unroll
+                    for (int c = 0; c < K::kSteps; ++c) {
+                        uint32_t f[4];
+                        ldsm4(f, keys + swizzled<K::kChunks>(rw, 2 * c + ch));
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) mma16816<K::kBf16>(s[n][c & 1], f, qf[n][c][0], qf[n][c][1]);
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < K::kSteps; c += 2) {
+                        uint32_t f[4];
+                        ldsm4(f, keys + swizzled<K::kChunks>(rw, c + ch));
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            // four codes of a row: elements 4j, 4j+1 take the place of the product's 2j, 2j+1,
+                            // elements 4j+2, 4j+3 that of 2j+8, 2j+9 (the queries are laid out alike)
+                            const uint32_t f16[4] = {
+                                fp8x2_to_f16x2<MODE>(f[2 * x]), fp8x2_to_f16x2<MODE>(f[2 * x + 1]),
+                                fp8x2_to_f16x2<MODE>(f[2 * x] >> 16), fp8x2_to_f16x2<MODE>(f[2 * x + 1] >> 16)};
+#pragma unroll
+                            for (int n = 0; n < NT; ++n)
+                                mma16816<false>(s[n][x], f16, qf[n][c + x][0], qf[n][c + x][1]);
+                        }
+                    }
+                }
+            }
+
+            // scores of tokens g and g + 8, heads 2j and 2j + 1
+            const uint32_t mask = static_cast<uint32_t>(sh.mask[warp][stage]);
+            const bool in0 = (mask >> g) & 1u, in1 = (mask >> (g + 8)) & 1u;
+            const float away = static_cast<float>(at.t * kTile + g - (at.n - 1));  // distance to the newest token, <= 0
+            uint32_t ph[NT][2], pl[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float p[4];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    float f = (s[n][0][x] + s[n][1][x]) * scale[n][x & 1];
+                    if (a.softcap > 0.0f) f = a.softcap * kLog2e * tanhf(f / a.softcap);
+                    f = __fmaf_rn(slope[n][x & 1], away + (x & 2 ? 8.0f : 0.0f), f);
+                    p[x] = (x & 2 ? in1 : in0) ? f : -INFINITY;
+                }
+                const float t0 = fmaxf(p[0], p[2]), t1 = fmaxf(p[1], p[3]);
+                if (__any_sync(0xffffffffu, t0 > m[n][0] || t1 > m[n][1])) {
+                    float top[2] = {t0, t1};
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 4));
+                        top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 8));
+                        top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 16));
+                        top[x] = fmaxf(top[x], m[n][x]);
+                        const float r = rescale(m[n][x], top[x]);
+                        m[n][x] = top[x];
+                        l[n][x] *= r;
+#pragma unroll
+                        for (int c = 0; c < K::kSteps; ++c) {
+                            o[n][c][x] *= r;
+                            o[n][c][x + 2] *= r;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const float mx = m[n][x & 1] == -INFINITY ? 0.0f : m[n][x & 1];
+                    p[x] = exp2_fast(p[x] - mx);
+                    l[n][x & 1] += p[x];
+                }
+                // high and low terms, tokens x heads -> heads x tokens
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const uint32_t high = pack2<K::kBf16>(p[2 * x], p[2 * x + 1]);
+                    float f0, f1;
+                    unpack2<K::kBf16>(high, f0, f1);
+                    const uint32_t low = pack2<K::kBf16>(p[2 * x] - f0, p[2 * x + 1] - f1);
+                    ph[n][x] = transpose8x8(high);
+                    pl[n][x] = transpose8x8(low);
+                }
+            }
+
+            // O^T += V^T P^T
+            if constexpr (!K::kFp8) {
+                const int rw = (lane & 7) + (lane >> 4) * 8, ch = (lane >> 3) & 1;
+#pragma unroll
+                for (int c = 0; c < K::kSteps; ++c) {
+                    uint32_t f[4];
+                    ldsm4_t(f, values + swizzled<K::kChunks>(rw, 2 * c + ch));
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        mma16816<K::kBf16>(o[n][c], f, ph[n][0], ph[n][1]);
+                        mma16816<K::kBf16>(o[n][c], f, pl[n][0], pl[n][1]);
+                    }
+                }
+            } else {
+                const int rw = (lane & 7) + ((lane >> 3) & 1) * 8, ch = lane >> 4;
+#pragma unroll
+                for (int c = 0; c < K::kSteps; c += 2) {
+                    uint32_t f[4];
+                    ldsm4_t(f, values + swizzled<K::kChunks>(rw, c + ch));
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        // a transposed pair of bytes holds elements 2g, 2g+1 of two tokens: row g of the product
+                        // is element 2g, row g + 8 element 2g + 1
+                        const uint32_t u = f[2 * x], w = f[2 * x + 1];
+                        const uint32_t f16[4] = {
+                            fp8x2_to_f16x2<MODE>(__byte_perm(u, 0u, 0x4420u)), fp8x2_to_f16x2<MODE>(__byte_perm(u, 0u, 0x4431u)),
+                            fp8x2_to_f16x2<MODE>(__byte_perm(w, 0u, 0x4420u)), fp8x2_to_f16x2<MODE>(__byte_perm(w, 0u, 0x4431u))};
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            mma16816<false>(o[n][c + x], f16, ph[n][0], ph[n][1]);
+                            mma16816<false>(o[n][c + x], f16, pl[n][0], pl[n][1]);
+                        }
+                    }
+                }
+            }
+
+            // the item's last tile, or this warp's
+            const bool ends = at.t + 1 == at.nt, stops = i + 1 == my_tiles;
+            if (ends || stops) {
+                const bool whole = ends && ta == 0;
+                const int32_t heads = min(K::kHeads, (kv + 1) * a.group - head0);
+                const int which = stops ? 1 : 0;
+                const float vs = a.v_scale ? __ldg(a.v_scale + kv) : 1.0f;
+                float* part = whole ? nullptr : a.warp_part + id * K::kPart;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        l[n][x] += __shfl_xor_sync(0xffffffffu, l[n][x], 4);
+                        l[n][x] += __shfl_xor_sync(0xffffffffu, l[n][x], 8);
+                        l[n][x] += __shfl_xor_sync(0xffffffffu, l[n][x], 16);
+                    }
+                    if (whole) {
+                        float f[2];
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const int h = n * 8 + 2 * j + x;
+                            f[x] = l[n][x] == 0.0f ? 0.0f : __fdiv_rn(vs, l[n][x]);
+                            if (g == 0 && h < heads) store_lse(a, at.r, head0 + h, m[n][x], l[n][x]);
+                        }
+#pragma unroll
+                        for (int c = 0; c < K::kSteps; ++c) {
+                            char* out = static_cast<char*>(a.out);
+                            if constexpr (!K::kFp8) {
+                                // elements x heads -> heads x elements
+                                const uint32_t u = transpose8x8(pack2<K::kBf16>(o[n][c][0] * f[0], o[n][c][1] * f[1]));
+                                const uint32_t w = transpose8x8(pack2<K::kBf16>(o[n][c][2] * f[0], o[n][c][3] * f[1]));
+                                const int h = n * 8 + g, d = c * 16 + 2 * j;
+                                char* at_out = out + 2 * (at.r * a.out_req + (head0 + h) * a.out_head + d);
+                                if (h < heads && d < a.head_dim) *reinterpret_cast<uint32_t*>(at_out) = u;
+                                if (h < heads && d + 8 < a.head_dim) *reinterpret_cast<uint32_t*>(at_out + 16) = w;
+                            } else {
+#pragma unroll
+                                for (int x = 0; x < 2; ++x) {
+                                    const int h = n * 8 + 2 * j + x, d = c * 16 + 2 * g;
+                                    const float u = o[n][c][x] * f[x], w = o[n][c][x + 2] * f[x];
+                                    const uint32_t two = a.q_f16 ? pack2<false>(u, w) : pack2<true>(u, w);
+                                    if (h < heads && d < a.head_dim)
+                                        *reinterpret_cast<uint32_t*>(out + 2 * (at.r * a.out_req + (head0 + h) * a.out_head + d)) = two;
+                                }
+                            }
+                        }
+                    } else if (!stops) {
+                        // the item began in another warp: its end waits in the workspace
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const int h = n * 8 + 2 * j + x;
+                            if (g == 0) {
+                                sh.m[2 * warp][h] = m[n][x];
+                                sh.l[2 * warp][h] = l[n][x];
+                            }
+#pragma unroll
+                            for (int c = 0; c < K::kSteps; ++c) {
+                                const int d0 = K::kFp8 ? c * 16 + 2 * g : c * 16 + g, d1 = K::kFp8 ? d0 + 1 : d0 + 8;
+                                part[h * DP + d0] = o[n][c][x];
+                                part[h * DP + d1] = o[n][c][x + 2];
+                            }
+                        }
+                    }
+                }
+                if (!whole && lane == 0) {
+                    Part& p = sh.part[2 * warp + which];
+                    p.start = x0 + i - at.t;
+                    p.r = at.r;
+                    p.item = at.item;
+                    p.nt = at.nt;
+                    p.ta = ta;
+                    p.tb = at.t + 1;
+                }
+            }
+            at.next(a, items);
+            stage = stage + 1 == S ? 0 : stage + 1;
+        }
+        cp_async_wait<0>();
+    }
+    __syncthreads();  // every ring is done with: the last parts are staged there
+    if (sh.part[2 * warp + 1].start >= 0) {
+        float* mine = reinterpret_cast<float*>(smem) + warp * (K::kHeads * K::kLd);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int h = n * 8 + 2 * j + x;
+                if (g == 0) {
+                    sh.m[2 * warp + 1][h] = m[n][x];
+                    sh.l[2 * warp + 1][h] = l[n][x];
+                }
+#pragma unroll
+                for (int c = 0; c < K::kSteps; ++c) {
+                    const int d0 = K::kFp8 ? c * 16 + 2 * g : c * 16 + g, d1 = K::kFp8 ? d0 + 1 : d0 + 8;
+                    mine[h * K::kLd + d0] = o[n][c][x];
+                    mine[h * K::kLd + d1] = o[n][c][x + 2];
+                }
+            }
+    }
+    __syncthreads();
+
+    // join the parts of each item inside the CTA: runs of consecutive parts with one start
+    constexpr int kFour = DP / 4;
+    if (tid < 2) sh.joins[tid] = 0;
+    bool open[2] = {false, false};
+    int32_t open_first[2] = {0, 0}, open_last[2] = {0, 0};
+    Part open_part[2];
+    for (int e = 0; e < 2 * W;) {
+        const Part p = sh.part[e];
+        if (p.start < 0) {
+            ++e;
+            continue;
+        }
+        int last = e;
+        for (int k = e + 1; k < 2 * W; ++k) {
+            if (sh.part[k].start < 0) continue;
+            if (sh.part[k].start != p.start) break;
+            last = k;
+        }
+        const int32_t tb = sh.part[last].tb;
+        const bool whole = p.ta == 0 && tb == p.nt;
+        const int32_t kv = p.item / a.blocks, head0 = kv * a.group + p.item % a.blocks * K::kHeads;
+        const int32_t heads = min(K::kHeads, (kv + 1) * a.group - head0);
+        const float vs = a.v_scale ? __ldg(a.v_scale + kv) : 1.0f;
+        const int slot = p.ta > 0 ? 0 : 1;
+        float* to = a.cta_part + (static_cast<int64_t>(blockIdx.x) * 2 + slot) * K::kPart;
+        for (int i = tid; i < heads * kFour; i += K::kThreads) {
+            const int h = i / kFour, d = i % kFour * 4;
+            float top = -INFINITY;
+            for (int k = e; k <= last; ++k)
+                if (sh.part[k].start >= 0) top = fmaxf(top, sh.m[k][h]);
+            float sum_l = 0.0f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int k = e; k <= last; ++k) {
+                if (sh.part[k].start < 0) continue;
+                const float r = rescale(sh.m[k][h], top);
+                const float* from = (k & 1) ? reinterpret_cast<const float*>(smem) + ((k >> 1) * K::kHeads + h) * K::kLd + d
+                                            : a.warp_part + (static_cast<int64_t>(blockIdx.x) * W + (k >> 1)) * K::kPart + h * DP + d;
+                const float4 f = *reinterpret_cast<const float4*>(from);
+                sum_l = __fmaf_rn(sh.l[k][h], r, sum_l);
+                acc.x = __fmaf_rn(f.x, r, acc.x);
+                acc.y = __fmaf_rn(f.y, r, acc.y);
+                acc.z = __fmaf_rn(f.z, r, acc.z);
+                acc.w = __fmaf_rn(f.w, r, acc.w);
+            }
+            if (whole) {
+                const float f = sum_l == 0.0f ? 0.0f : __fdiv_rn(vs, sum_l);
+                store_out4(a, p.r, head0 + h, d, make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
+                if (d == 0) store_lse(a, p.r, head0 + h, top, sum_l);
+            } else {
+                *reinterpret_cast<float4*>(to + h * DP + d) = acc;
+                if (d == 0) {
+                    to[K::kHeads * DP + h] = top;
+                    to[K::kHeads * DP + K::kHeads + h] = sum_l;
+                }
+            }
+        }
+        if (!whole) {
+            // the CTAs that hold the item's first and last tile
+            const int64_t end = p.start + p.nt - 1;
+            open[slot] = true;
+            open_part[slot] = p;
+            open_first[slot] = static_cast<int32_t>(((p.start + 1) * workers - 1) / total / W);
+            open_last[slot] = static_cast<int32_t>(((end + 1) * workers - 1) / total / W);
+        }
+        e = last + 1;
+    }
+    if (!open[0] && !open[1]) return;
+
+    // join between CTAs: the last one to arrive does it, and leaves the ticket at zero
+    __threadfence();
+    __syncthreads();
+    if (tid < 2 && (tid == 0 ? open[0] : open[1])) {
+        const int32_t first = tid == 0 ? open_first[0] : open_first[1], last = tid == 0 ? open_last[0] : open_last[1];
+        const int32_t n = last - first + 1;
+        if (atomicAdd(a.tickets + first, 1) == n - 1) {
+            a.tickets[first] = 0;
+            sh.joins[tid] = 1;
+        }
+        __threadfence();
+    }
+    __syncthreads();
+#pragma unroll
+    for (int slot = 0; slot < 2; ++slot) {
+        if (!open[slot] || !sh.joins[slot]) continue;
+        const Part& p = open_part[slot];
+        const int32_t kv = p.item / a.blocks, head0 = kv * a.group + p.item % a.blocks * K::kHeads;
+        const int32_t heads = min(K::kHeads, (kv + 1) * a.group - head0);
+        const float vs = a.v_scale ? __ldg(a.v_scale + kv) : 1.0f;
+        const int32_t first = open_first[slot], last = open_last[slot];
+        for (int i = tid; i < heads * kFour; i += K::kThreads) {
+            const int h = i / kFour, d = i % kFour * 4;
+            float top = -INFINITY;
+            for (int32_t c = first; c <= last; ++c) {
+                const float* from = a.cta_part + (static_cast<int64_t>(c) * 2 + (c == first)) * K::kPart;
+                top = fmaxf(top, __ldcg(from + K::kHeads * DP + h));
+            }
+            float sum_l = 0.0f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int32_t c = first; c <= last; ++c) {
+                const float* from = a.cta_part + (static_cast<int64_t>(c) * 2 + (c == first)) * K::kPart;
+                const float r = rescale(__ldcg(from + K::kHeads * DP + h), top);
+                const float4 f = __ldcg(reinterpret_cast<const float4*>(from + h * DP + d));
+                sum_l = __fmaf_rn(__ldcg(from + K::kHeads * DP + K::kHeads + h), r, sum_l);
+                acc.x = __fmaf_rn(f.x, r, acc.x);
+                acc.y = __fmaf_rn(f.y, r, acc.y);
+                acc.z = __fmaf_rn(f.z, r, acc.z);
+                acc.w = __fmaf_rn(f.w, r, acc.w);
+            }
+            const float f = sum_l == 0.0f ? 0.0f : __fdiv_rn(vs, sum_l);
+            store_out4(a, p.r, head0 + h, d, make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
+            if (d == 0) store_lse(a, p.r, head0 + h, top, sum_l);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ host
+
+struct Kernel {
+    void (*fn)(AttnArgs);
+    int threads, shared, part_floats, warps;
+};
+
+template <int MODE, int DP, int NT, int W, int S>
+Kernel kernel_of() {
+    using K = Attn<MODE, DP, NT, W, S>;
+    static_assert(K::kSharedBytes <= 232448, "shared memory of one CTA");
+    return Kernel{paged_attn_kernel<MODE, DP, NT, W, S>, K::kThreads, K::kSharedBytes, K::kPart, W};
+}
+
+// Warps and stages: about 192 KB of ring per SM, the bytes in flight that keep HBM busy.
+template <int MODE, int NT>
+Kernel pick_dim(int head_dim) {
+    constexpr bool fp8 = MODE == MF_DT_F8E4M3 || MODE == MF_DT_F8E5M2;
+    if (head_dim <= 64) return kernel_of<MODE, 64, NT, 8, fp8 ? 8 : 6>();
+    if (head_dim <= 128) return kernel_of<MODE, 128, NT, 8, fp8 ? 6 : 3>();
+    return kernel_of<MODE, 256, NT, fp8 ? 8 : 4, 3>();
+}
+template <int MODE>
+Kernel pick_heads(int group, int head_dim) {
+    return group <= 8 ? pick_dim<MODE, 1>(head_dim) : pick_dim<MODE, 2>(head_dim);
+}
+Kernel pick(int cache_dtype, int group, int head_dim) {
+    switch (cache_dtype) {
+    case MF_DT_BF16: return pick_heads<MF_DT_BF16>(group, head_dim);
+    case MF_DT_F16: return pick_heads<MF_DT_F16>(group, head_dim);
+    case MF_DT_F8E4M3: return pick_heads<MF_DT_F8E4M3>(group, head_dim);
+    default: return pick_heads<MF_DT_F8E5M2>(group, head_dim);
+    }
+}
+
+}  // namespace
+}  // namespace mf
+
+using namespace mf;
+
+struct mf_paged_attn_s {
+    mf_paged_attn_config config;
+    Kernel kernel;
+    AttnArgs args;
+    void* workspace;
+    int device, ctas;
+};
+
+extern "C" int mf_paged_attn_create(const mf_paged_attn_config* config, mf_paged_attn* handle) {
+    MF_ENTER();
+    if (!config || !handle) return fail(MF_ERR_INVALID_ARGUMENT, "mf_paged_attn_create: NULL argument");
+    *handle = nullptr;
+    const mf_paged_attn_config& c = *config;
+    const mf_cache_layout& k = c.cache;
+    if (c.q_dtype != MF_DT_BF16 && c.q_dtype != MF_DT_F16)
+        return fail(MF_ERR_DTYPE_UNSUPPORTED, "mf_paged_attn_create: queries of dtype %d (BF16 and F16 are supported)", c.q_dtype);
+    if (!is_fp8(k.dtype) && k.dtype != c.q_dtype)
+        return fail(MF_ERR_DTYPE_MISMATCH, "mf_paged_attn_create: cache dtype %d is neither FP8 nor the queries' %d", k.dtype,
+                    c.q_dtype);
+    if (k.kv_heads <= 0 || c.q_heads <= 0 || c.q_heads % k.kv_heads || c.q_heads > 65536)
+        return fail(MF_ERR_SHAPE_INVALID, "mf_paged_attn_create: %d query heads over %d key-value heads", c.q_heads, k.kv_heads);
+    const int step = is_fp8(k.dtype) ? 16 : 8;
+    if (k.head_dim <= 0 || k.head_dim > 256 || k.head_dim % step)
+        return fail(MF_ERR_SHAPE_INVALID, "mf_paged_attn_create: head_dim %d must be a multiple of %d up to 256", k.head_dim, step);
+    if (k.page_size <= 0 || k.n_pages < 0 || c.max_pages <= 0 || c.table_stride < c.max_pages)
+        return fail(MF_ERR_SHAPE_INVALID, "mf_paged_attn_create: %lld pages of %d, table rows of %d (stride %lld)",
+                    (long long)k.n_pages, k.page_size, c.max_pages, (long long)c.table_stride);
+    if (k.page_stride % step || k.token_stride % step || k.head_stride % step)
+        return fail(MF_ERR_LAYOUT_UNSUPPORTED, "mf_paged_attn_create: cache strides must be multiples of 16 bytes");
+    if (c.q_token_stride % 2 || c.q_head_stride % 2 || c.out_token_stride % 4 || c.out_head_stride % 4)
+        return fail(MF_ERR_LAYOUT_UNSUPPORTED, "mf_paged_attn_create: query strides must be even, output strides multiples of 4");
+    if (c.window < 0 || !(c.softcap >= 0.0f))
+        return fail(MF_ERR_INVALID_ARGUMENT, "mf_paged_attn_create: window %d, softcap %g", c.window, c.softcap);
+    const int group = c.q_heads / k.kv_heads;
+    Kernel kernel = pick(k.dtype, group, k.head_dim);
+    MF_CUDA_CHECK(cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel.fn), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       kernel.shared));
+    const int ctas = state().sm_count;
+    const size_t warp_part = static_cast<size_t>(ctas) * kernel.warps * kernel.part_floats * 4;
+    const size_t cta_part = static_cast<size_t>(ctas) * 2 * kernel.part_floats * 4;
+    const size_t bytes = warp_part + cta_part + static_cast<size_t>(ctas) * 4;
+    mf_paged_attn_s* h = new (std::nothrow) mf_paged_attn_s{};
+    if (!h) return fail(MF_ERR_ALLOCATOR_EXHAUSTED, "mf_paged_attn_create: out of host memory");
+    cudaError_t err = cudaMalloc(&h->workspace, bytes);
+    if (err != cudaSuccess) {
+        cudaGetLastError();
+        delete h;
+        if (err == cudaErrorMemoryAllocation)
+            return fail(MF_ERR_ALLOCATOR_EXHAUSTED, "mf_paged_attn_create: %zu bytes: out of device memory", bytes);
+        return cuda_fail(err, "mf_paged_attn_create: cudaMalloc");
+    }
+    char* w = static_cast<char*>(h->workspace);
+    err = cudaMemset(w + warp_part + cta_part, 0, static_cast<size_t>(ctas) * 4);
+    if (err == cudaSuccess) err = cudaStreamSynchronize(nullptr);  // streams that do not wait for the default one may run it
+    if (err != cudaSuccess) {
+        cudaFree(h->workspace);
+        delete h;
+        return cuda_fail(err, "mf_paged_attn_create: cudaMemset");
+    }
+    h->config = c;
+    h->kernel = kernel;
+    h->device = state().device;
+    h->ctas = ctas;
+    AttnArgs& a = h->args;
+    a.slopes = c.slopes;
+    a.k_scale = is_fp8(k.dtype) ? c.k_scale_inv : nullptr;
+    a.v_scale = is_fp8(k.dtype) ? c.v_scale_inv : nullptr;
+    a.warp_part = reinterpret_cast<float*>(w);
+    a.cta_part = reinterpret_cast<float*>(w + warp_part);
+    a.tickets = reinterpret_cast<int32_t*>(w + warp_part + cta_part);
+    a.status = sticky_status_ptr();
+    a.q_req = c.q_token_stride;
+    a.q_head = c.q_head_stride;
+    a.out_req = c.out_token_stride;
+    a.out_head = c.out_head_stride;
+    a.page_stride = k.page_stride;
+    a.token_stride = k.token_stride;
+    a.head_stride = k.head_stride;
+    a.table_stride = c.table_stride;
+    a.n_pages = k.n_pages;
+    a.q_heads = c.q_heads;
+    a.kv_heads = k.kv_heads;
+    a.group = group;
+    a.blocks = (group + (group <= 8 ? 7 : 15)) / (group <= 8 ? 8 : 16);
+    a.head_dim = k.head_dim;
+    a.page = k.page_size;
+    a.max_pages = c.max_pages;
+    a.window = c.window;
+    a.q_f16 = c.q_dtype == MF_DT_F16;
+    a.scale = c.scale;
+    a.softcap = c.softcap;
+    if (!a.status) {
+        cudaFree(h->workspace);
+        delete h;
+        return fail(MF_ERR_CUDA, "mf_paged_attn_create: sticky status word unavailable");
+    }
+    *handle = h;
+    return MF_OK;
+}
+
+extern "C" int mf_paged_attn_run(mf_paged_attn handle, const void* q, const void* k_cache, const void* v_cache,
+                                 const int32_t* table, const int32_t* lens, int32_t n_requests, void* out, float* lse,
+                                 mf_stream stream) {
+    MF_ENTER();
+    if (!handle) return fail(MF_ERR_INVALID_ARGUMENT, "mf_paged_attn_run: handle is NULL");
+    if (handle->device != state().device)
+        return fail(MF_ERR_INVALID_ARGUMENT, "mf_paged_attn_run: the handle belongs to device %d", handle->device);
+    if (n_requests < 0) return fail(MF_ERR_SHAPE_INVALID, "mf_paged_attn_run: %d requests", n_requests);
+    if (n_requests == 0) return MF_OK;
+    if (!q || !k_cache || !v_cache || !table || !lens || !out)
+        return fail(MF_ERR_INVALID_ARGUMENT, "mf_paged_attn_run: NULL buffer");
+    if (!aligned16(k_cache) || !aligned16(v_cache))
+        return fail(MF_ERR_LAYOUT_UNSUPPORTED, "mf_paged_attn_run: cache buffers must be 16-byte aligned");
+    if (reinterpret_cast<uintptr_t>(q) % 4 || reinterpret_cast<uintptr_t>(out) % 8)
+        return fail(MF_ERR_LAYOUT_UNSUPPORTED, "mf_paged_attn_run: q must be 4-byte and out 8-byte aligned");
+    AttnArgs a = handle->args;
+    a.q = q;
+    a.k = k_cache;
+    a.v = v_cache;
+    a.table = table;
+    a.lens = lens;
+    a.n_requests = n_requests;
+    a.out = out;
+    a.lse = lse;
+    handle->kernel.fn<<<static_cast<unsigned>(handle->ctas), handle->kernel.threads, handle->kernel.shared,
+                        static_cast<cudaStream_t>(stream)>>>(a);
+    MF_LAUNCH_CHECK("mf_paged_attn_run");
+    return MF_OK;
+}
+
+extern "C" int mf_paged_attn_destroy(mf_paged_attn handle) {
+    if (!handle) return MF_OK;
+    MF_ENTER();
+    MF_CUDA_CHECK(cudaFree(handle->workspace));
+    delete handle;
+    return MF_OK;
+}
