@@ -56,8 +56,8 @@ struct AttnArgs {
     const float* k_scale;
     const float* v_scale;
     float* warp_part;     // [workers][NT * 8 * (DP + 2)]: parts that end inside a warp's run
-    float* cta_part;      // [CTAs][2][NT * 8 * (DP + 2)]: parts that leave the CTA
-    int32_t* tickets;     // [CTAs], zero between runs
+    float* cta_part;      // [CTAs][3][NT * 8 * (DP + 2)]: parts that leave the CTA, and joined groups of them
+    int32_t* tickets;     // [2][CTAs], zero between runs
     int32_t* status;
     int64_t q_req, q_head, out_req, out_head;
     int64_t page_stride, token_stride, head_stride, table_stride;
@@ -139,32 +139,46 @@ __device__ __forceinline__ float rescale(float m_old, float m_new) {
     return m_old == m_new ? 1.0f : exp2_fast(m_old - m_new);
 }
 
-// Tokens that request r sees, and the first of them.
-__device__ __forceinline__ int32_t seen_tokens(const AttnArgs& a, int32_t r, int32_t& first) {
-    const int64_t reach = static_cast<int64_t>(a.max_pages) * a.page;
-    int32_t len = max(__ldg(a.lens + r), 0);
-    if (len > reach) len = static_cast<int32_t>(reach);
-    const int32_t n = a.window > 0 ? min(len, a.window) : len;
-    first = len - n;
-    return n;
+// tanh(x) = 1 - 2 / (1 + exp(2x)): 2^-22 of 1, the limits at both ends.
+__device__ __forceinline__ float tanh_fast(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + exp2_fast(2.0f * kLog2e * x)));
+    return __fmaf_rn(-2.0f, r, 1.0f);
 }
-__device__ __forceinline__ int64_t tiles_of(int32_t tokens) { return (static_cast<int64_t>(tokens) + kTile - 1) / kTile; }
+
+// A request's tokens: [first, len) are seen, from the tile that starts at `base`
+// (a multiple of the tile, so that a tile never crosses a page of whole tiles).
+struct Span {
+    int32_t len, first, base;
+};
+__device__ __forceinline__ Span span_of(const AttnArgs& a, int32_t r) {
+    const int64_t reach = static_cast<int64_t>(a.max_pages) * a.page;
+    Span s;
+    s.len = max(__ldg(a.lens + r), 0);
+    if (s.len > reach) s.len = static_cast<int32_t>(reach);
+    s.first = a.window > 0 && s.len > a.window ? s.len - a.window : 0;
+    s.base = s.first & ~(kTile - 1);
+    return s;
+}
+__device__ __forceinline__ int32_t tiles_of(const Span& s) {
+    return static_cast<int32_t>((static_cast<uint32_t>(s.len - s.base) + (kTile - 1)) / kTile);
+}
 
 // A place in the row of all tiles: request, item of the request, tile of the item.
 struct Place {
     int32_t r, item, t, nt;   // nt: tiles of the request's items
-    int32_t n, first;         // tokens it sees
+    Span span;
     __device__ __forceinline__ void next(const AttnArgs& a, int32_t items) {
         if (++t < nt) return;
         t = 0;
         if (++item < items) return;
         item = 0;
+        nt = 0;
         while (++r < a.n_requests) {
-            n = seen_tokens(a, r, first);
-            nt = static_cast<int32_t>(tiles_of(n));
+            span = span_of(a, r);
+            nt = tiles_of(span);
             if (nt > 0) return;
         }
-        nt = 0;
     }
 };
 
@@ -174,6 +188,8 @@ struct Part {
     int32_t r, item, nt;
     int32_t ta, tb;  // its tiles of the item
 };
+
+constexpr int kJoin = 16;  // most parts that one step of a join between CTAs takes
 
 // MODE: dtype of the cache; DP: head_dim padded to 64, 128 or 256; NT: blocks
 // of 8 query heads a warp holds; W: warps; S: stages of a warp's ring.
@@ -187,20 +203,25 @@ struct Attn {
     static constexpr int kStage = 2 * kTile * kRow;   // keys, then values
     static constexpr int kSteps = DP / 16;            // products of 16 along head_dim
     static constexpr int kHeads = 8 * NT;
+    static constexpr int kFour = DP / 4;
     static constexpr int kLd = DP + 4;                // floats of a staged head's row (spread over the banks)
     static constexpr int kPart = kHeads * (DP + 2);   // floats of a part in the workspace: out, then m, l
     static constexpr int kThreads = 32 * W;
     static constexpr int kRing = W * S * kStage;
     static constexpr int kStaged = W * kHeads * kLd * 4;
     static constexpr int kBuffer = kRing > kStaged ? kRing : kStaged;
+    static_assert(2 * W <= 32, "a lane for each part of a CTA");
 
     struct Shared {
         int64_t prefix[kThreads + 1];   // tiles of the requests in front of each thread's
         int64_t warp_sum[W];
         Part part[2 * W];               // first and last part of each warp
         float m[2 * W][kHeads], l[2 * W][kHeads];
+        float weight[kJoin][kHeads], top[kHeads], sum[kHeads];
         int32_t mask[W][S];             // tokens of each stage that are there
-        int32_t joins[2];               // whether this CTA joins the item of its slot
+        int32_t lead[2 * W + 1];        // first part of each joined item, then 2 * W
+        int32_t items;                  // joined items
+        int32_t won[2];                 // whether this CTA joins the item of its slot
     };
     static constexpr int kSharedBytes = kBuffer + static_cast<int>(sizeof(Shared));
 };
@@ -228,6 +249,99 @@ __device__ __forceinline__ void store_lse(const AttnArgs& a, int32_t r, int32_t 
     if (a.lse) a.lse[static_cast<int64_t>(r) * a.q_heads + head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
+__device__ __forceinline__ float4 fma4(float4 f, float r, float4 acc) {
+    return make_float4(__fmaf_rn(f.x, r, acc.x), __fmaf_rn(f.y, r, acc.y), __fmaf_rn(f.z, r, acc.z), __fmaf_rn(f.w, r, acc.w));
+}
+__device__ __forceinline__ float4 scale4(float4 f, float r) { return make_float4(f.x * r, f.y * r, f.z * r, f.w * r); }
+
+// Query heads of an item: the first of them, how many, and their key-value head.
+template <int HEADS>
+struct Heads {
+    int32_t kv, head0, count;
+    __device__ __forceinline__ Heads(const AttnArgs& a, int32_t item) {
+        kv = item / a.blocks;
+        head0 = kv * a.group + item % a.blocks * HEADS;
+        count = min(HEADS, (kv + 1) * a.group - head0);
+    }
+};
+
+// One more arrival at a ticket that `count` CTAs share; true for the last one,
+// which leaves the ticket at zero.  What every thread of the CTA wrote before
+// the last barrier is visible to whoever arrives later.
+__device__ __forceinline__ bool arrive_last(int32_t* ticket, int32_t count) {
+    int32_t old;
+    asm volatile("fence.acq_rel.gpu;" ::: "memory");
+    asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(old) : "l"(ticket) : "memory");
+    if (old != count - 1) return false;
+    *ticket = 0;
+    asm volatile("fence.acq_rel.gpu;" ::: "memory");
+    return true;
+}
+
+// Joins parts 0 .. n-1 (n <= kJoin) at first + k * stride floats: to the
+// output if `to` is NULL, else to a part there.  All threads of the CTA.
+template <class K>
+__device__ __forceinline__ void join_parts(const AttnArgs& a, typename K::Shared& sh, const float* first, int64_t stride,
+                                           const float* at0, int32_t n, int32_t r, int32_t item, float* to, int dp) {
+    const int tid = threadIdx.x;
+    const Heads<K::kHeads> hd(a, item);
+    auto part = [&](int k) { return k == 0 ? at0 : first + k * stride; };
+    constexpr int kAhead = 8;
+    float4 f[kAhead];
+    int i = tid;
+    // the first element's loads travel together with those of the weights
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+        if (i < hd.count * K::kFour && k < n) f[k] = __ldcg(reinterpret_cast<const float4*>(part(k) + i * 4));
+    if (tid < hd.count) {
+        float top = -INFINITY, sum = 0.0f, m[kJoin], l[kJoin];
+#pragma unroll
+        for (int k = 0; k < kJoin; ++k) {
+            m[k] = k < n ? __ldcg(part(k) + K::kHeads * dp + tid) : -INFINITY;
+            l[k] = k < n ? __ldcg(part(k) + K::kHeads * dp + K::kHeads + tid) : 0.0f;
+        }
+#pragma unroll
+        for (int k = 0; k < kJoin; ++k) top = fmaxf(top, m[k]);
+#pragma unroll
+        for (int k = 0; k < kJoin; ++k) {
+            if (k >= n) break;
+            const float w = rescale(m[k], top);
+            sh.weight[k][tid] = w;
+            sum = __fmaf_rn(l[k], w, sum);
+        }
+        sh.top[tid] = top;
+        sh.sum[tid] = sum;
+    }
+    __syncthreads();
+    const float vs = a.v_scale ? __ldg(a.v_scale + hd.kv) : 1.0f;
+    for (; i < hd.count * K::kFour; i += K::kThreads) {
+        const int h = i / K::kFour, d = i % K::kFour * 4;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k0 = 0; k0 < n; k0 += kAhead) {
+            if (k0 > 0 || i != tid) {
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k)
+                    if (k0 + k < n) f[k] = __ldcg(reinterpret_cast<const float4*>(part(k0 + k) + i * 4));
+            }
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k)
+                if (k0 + k < n) acc = fma4(f[k], sh.weight[k0 + k][h], acc);
+        }
+        const float sum = sh.sum[h];
+        if (to) {
+            *reinterpret_cast<float4*>(to + i * 4) = acc;
+            if (d == 0) {
+                to[K::kHeads * dp + h] = sh.top[h];
+                to[K::kHeads * dp + K::kHeads + h] = sum;
+            }
+        } else {
+            store_out4(a, r, hd.head0 + h, d, scale4(acc, sum == 0.0f ? 0.0f : __fdiv_rn(vs, sum)));
+            if (d == 0) store_lse(a, r, hd.head0 + h, sh.top[h], sum);
+        }
+    }
+    __syncthreads();
+}
+
 template <int MODE, int DP, int NT, int W, int S>
 __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a) {
     using K = Attn<MODE, DP, NT, W, S>;
@@ -237,22 +351,16 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
     const int g = lane >> 2, j = lane & 3;  // row and column pair of a product's fragment
     const int32_t items = a.kv_heads * a.blocks;
 
-    // requests that see nothing
-    for (int32_t r = blockIdx.x; r < a.n_requests; r += gridDim.x) {
-        int32_t first;
-        if (seen_tokens(a, r, first) > 0) continue;
-        for (int i = tid; i < a.q_heads * (a.head_dim / 4); i += K::kThreads)
-            store_out4(a, r, i / (a.head_dim / 4), i % (a.head_dim / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f));
-        for (int i = tid; i < a.q_heads; i += K::kThreads) store_lse(a, r, i, 0.0f, 0.0f);
-    }
-
     // prefix of the tiles: thread i sums `per` consecutive requests
     const int32_t per = (a.n_requests + K::kThreads - 1) / K::kThreads;
     int64_t sum = 0;
+    bool empty = false;
     for (int32_t i = 0; i < per; ++i) {
         const int32_t r = tid * per + i;
-        int32_t first;
-        if (r < a.n_requests) sum += tiles_of(seen_tokens(a, r, first)) * items;
+        if (r >= a.n_requests) break;
+        const int32_t nt = tiles_of(span_of(a, r));
+        sum += static_cast<int64_t>(nt) * items;
+        empty |= nt == 0 && r % gridDim.x == blockIdx.x;
     }
     int64_t inc = sum;
 #pragma unroll
@@ -262,7 +370,15 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
     }
     if (lane == 31) sh.warp_sum[warp] = inc;
     if (lane < 2) sh.part[2 * warp + lane].start = -1;
-    __syncthreads();
+    if (__syncthreads_or(empty)) {
+        // requests that see nothing
+        for (int32_t r = blockIdx.x; r < a.n_requests; r += gridDim.x) {
+            if (tiles_of(span_of(a, r)) > 0) continue;
+            for (int i = tid; i < a.q_heads * (a.head_dim / 4); i += K::kThreads)
+                store_out4(a, r, i / (a.head_dim / 4), i % (a.head_dim / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f));
+            for (int i = tid; i < a.q_heads; i += K::kThreads) store_lse(a, r, i, 0.0f, 0.0f);
+        }
+    }
     int64_t total = 0, base = 0;
 #pragma unroll
     for (int w = 0; w < W; ++w) {
@@ -274,16 +390,17 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
     __syncthreads();
     if (total == 0) return;
     const int64_t want = (total + W - 1) / W;
-    const int64_t ctas = want < gridDim.x ? want : gridDim.x;
+    int32_t ctas = static_cast<int32_t>(want < gridDim.x ? want : gridDim.x);
+    if (a.n_requests == 1 && items <= gridDim.x) ctas = max(ctas / items, 1) * items;  // no CTA has parts of two items
     if (blockIdx.x >= ctas) return;
-    const int64_t workers = ctas * W;
-    const int64_t id = static_cast<int64_t>(blockIdx.x) * W + warp;
+    const int32_t workers = ctas * W;
+    const int32_t id = blockIdx.x * W + warp;
     const int64_t x0 = total * id / workers, x1 = total * (id + 1) / workers;
-    const int64_t my_tiles = x1 - x0;
+    const int32_t my_tiles = static_cast<int32_t>(x1 - x0);
 
     uint32_t qf[NT][K::kSteps][2];
     float o[NT][K::kSteps][4];
-    float m[NT][2], l[NT][2], scale[NT][2], slope[NT][2];
+    float m[NT][2], mu[NT][2], l[NT][2], scale[NT][2], slope[NT][2];  // mu: m, or 0 while m is -inf
     if (my_tiles > 0) {
         // the place of tile x0: the thread whose requests hold it, then the request among them
         int lo = 0, hi = K::kThreads;
@@ -295,9 +412,8 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
         Place at{};
         int64_t before = sh.prefix[lo];
         for (int32_t r0 = lo * per;; r0 += 32) {
-            int32_t first = 0, n = 0;
-            if (r0 + lane < a.n_requests) n = seen_tokens(a, r0 + lane, first);
-            const int64_t mine = tiles_of(n) * items;
+            const int32_t nt = r0 + lane < a.n_requests ? tiles_of(span_of(a, r0 + lane)) : 0;
+            const int64_t mine = static_cast<int64_t>(nt) * items;
             int64_t upto = mine;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
@@ -308,55 +424,82 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
             if (past || r0 + 32 >= a.n_requests) {
                 const int src = past ? __ffs(past) - 1 : 0;
                 at.r = r0 + src;
-                at.n = __shfl_sync(0xffffffffu, n, src);
-                at.first = __shfl_sync(0xffffffffu, first, src);
                 before += __shfl_sync(0xffffffffu, upto - mine, src);
                 break;
             }
             before += __shfl_sync(0xffffffffu, upto, 31);
         }
-        at.nt = static_cast<int32_t>(tiles_of(at.n));
+        at.span = span_of(a, at.r);
+        at.nt = tiles_of(at.span);
         const int64_t in_request = x0 - before;
         at.item = static_cast<int32_t>(in_request / at.nt);
         at.t = static_cast<int32_t>(in_request % at.nt);
 
         const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * (S * K::kStage);
         Place load = at;
-        int64_t to_load = my_tiles;
-        int32_t page_no = -1, page_off = 0;
-        bool there = false;
-        const int row = lane & 15;
-        // the page of this lane's row of the tile at `load`
+        int32_t to_load = my_tiles;
+        const bool whole_tiles = a.page % kTile == 0;  // a tile lies in one page
+        const int lane_row = whole_tiles ? 0 : lane & 15;
+        // place of this lane's piece in the first rows that one instruction copies, and of the next rows
+        constexpr int kRows = 32 / K::kChunks > 0 ? 32 / K::kChunks : 1;  // rows of one instruction
+        constexpr int kCopies = kTile * K::kChunks / 32;
+        const int piece_row = lane / K::kChunks, piece = lane % K::kChunks;
+        const int64_t row_bytes = a.token_stride * K::kBytes;
+        const int64_t lane_bytes = piece_row * row_bytes + piece * 16;
+        const bool piece_in = piece * (16 / K::kBytes) < a.head_dim;
+        int32_t page_no = -1;
+        // the page of the tile at `load`, or of this lane's row of it
         auto look_up = [&]() {
-            const int32_t p = load.t * kTile + row;
-            there = to_load > 0 && p < load.n;
-            if (there) {
-                const int32_t tok = load.first + p;
-                page_off = tok % a.page;
-                page_no = __ldg(a.table + load.r * a.table_stride + tok / a.page);
-            }
+            const int32_t tok = load.span.base + load.t * kTile + lane_row;
+            if (to_load > 0 && tok < load.span.len)
+                page_no = __ldg(a.table + load.r * a.table_stride + static_cast<uint32_t>(tok) / static_cast<uint32_t>(a.page));
         };
         auto issue = [&](int stage) {
             if (to_load > 0) {
-                bool ok = there;
+                const int32_t tok0 = load.span.base + load.t * kTile, tok = tok0 + (lane & 15);
+                const bool seen = tok >= load.span.first && tok < load.span.len;
+                bool ok = seen;
                 if (ok && (page_no < 0 || page_no >= a.n_pages)) {
                     ok = false;
                     atomicExch(a.status, MF_DEVICE_BAD_PAGE);
                 }
-                const int32_t kv = load.item / a.blocks;
-                int64_t off = ok ? page_no * a.page_stride + page_off * a.token_stride + kv * a.head_stride : -1;
                 const uint32_t mask = __ballot_sync(0xffffffffu, ok) & 0xffffu;
                 if (lane == 0) sh.mask[warp][stage] = static_cast<int32_t>(mask);
+                const int32_t kv = load.item / a.blocks;
                 const uint32_t dst = ring + stage * K::kStage;
+                const int32_t off_page = static_cast<int32_t>(static_cast<uint32_t>(tok0 + lane_row) % static_cast<uint32_t>(a.page));
+                const int64_t at_row = (page_no * a.page_stride + off_page * a.token_stride + kv * a.head_stride) * K::kBytes;
+                if (whole_tiles) {
+                    const char* kp = static_cast<const char*>(a.k) + at_row + lane_bytes;
+                    const int64_t kv_gap = static_cast<const char*>(a.v) - static_cast<const char*>(a.k);
+                    if (mask == 0xffffu && a.head_dim == DP) {
 #pragma unroll
-                for (int i = 0; i < kTile * K::kChunks / 32; ++i) {
-                    const int piece = i * 32 + lane, rw = piece / K::kChunks, c = piece % K::kChunks;
-                    const int64_t o = __shfl_sync(0xffffffffu, off, rw);
-                    const bool get = o >= 0 && c * (16 / K::kBytes) < a.head_dim;
-                    const int64_t byte = get ? o * K::kBytes + c * 16 : 0;
-                    const uint32_t to = dst + swizzled<K::kChunks>(rw, c);
-                    cp_async16(to, static_cast<const char*>(a.k) + byte, get ? 16u : 0u);
-                    cp_async16(to + kTile * K::kRow, static_cast<const char*>(a.v) + byte, get ? 16u : 0u);
+                        for (int i = 0; i < kCopies; ++i, kp += kRows * row_bytes) {
+                            const uint32_t to = dst + swizzled<K::kChunks>(i * kRows + piece_row, piece);
+                            cp_async16(to, kp, 16u);
+                            cp_async16(to + kTile * K::kRow, kp + kv_gap, 16u);
+                        }
+                    } else {
+#pragma unroll 1
+                        for (int i = 0; i < kCopies; ++i, kp += kRows * row_bytes) {
+                            const int rw = i * kRows + piece_row;
+                            const bool get = piece_in && ((mask >> rw) & 1u);
+                            const uint32_t to = dst + swizzled<K::kChunks>(rw, piece);
+                            cp_async16(to, get ? kp : static_cast<const char*>(a.k), get ? 16u : 0u);
+                            cp_async16(to + kTile * K::kRow, get ? kp + kv_gap : static_cast<const char*>(a.v), get ? 16u : 0u);
+                        }
+                    }
+                } else {
+#pragma unroll 1
+                    for (int i = 0; i < kCopies; ++i) {
+                        const int rw = i * kRows + piece_row;
+                        const int64_t row_at = __shfl_sync(0xffffffffu, at_row, rw);
+                        const bool get = piece_in && ((mask >> rw) & 1u);
+                        const int64_t byte = get ? row_at + piece * 16 : 0;
+                        const uint32_t to = dst + swizzled<K::kChunks>(rw, piece);
+                        cp_async16(to, static_cast<const char*>(a.k) + byte, get ? 16u : 0u);
+                        cp_async16(to + kTile * K::kRow, static_cast<const char*>(a.v) + byte, get ? 16u : 0u);
+                    }
                 }
                 load.next(a, items);
                 --to_load;
@@ -365,30 +508,33 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
             cp_async_commit();
         };
         look_up();
-#pragma unroll
+#pragma unroll 1
         for (int s = 0; s < S - 1; ++s) issue(s);
 
-        int32_t ta = at.t, kv = 0, head0 = 0;
+        // rows of this lane in the loads of a product's operands
+        const int k_row = (lane & 7) + ((lane >> 3) & 1) * 8, k_piece = lane >> 4;
+        const int v_row = K::kFp8 ? k_row : (lane & 7) + (lane >> 4) * 8, v_piece = K::kFp8 ? k_piece : (lane >> 3) & 1;
+        const bool rules = a.softcap > 0.0f || a.slopes;
+        int32_t ta = at.t;
         int stage = 0;
-        for (int64_t i = 0; i < my_tiles; ++i) {
+#pragma unroll 1
+        for (int32_t i = 0; i < my_tiles; ++i) {
             cp_async_wait<S - 2>();
             __syncwarp();
             issue(stage == 0 ? S - 1 : stage - 1);
             if (i == 0 || at.t == 0) {
                 // a new item: its queries
                 ta = at.t;
-                kv = at.item / a.blocks;
-                head0 = kv * a.group + at.item % a.blocks * K::kHeads;
-                const int32_t heads = min(K::kHeads, (kv + 1) * a.group - head0);
+                const Heads<K::kHeads> hd(a, at.item);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     const int h = n * 8 + g;
-                    const char* q = static_cast<const char*>(a.q) + 2 * (at.r * a.q_req + (head0 + h) * a.q_head);
+                    const char* q = static_cast<const char*>(a.q) + 2 * (at.r * a.q_req + (hd.head0 + h) * a.q_head);
                     float top = 0.0f;
 #pragma unroll
                     for (int c = 0; c < K::kSteps; ++c) {
                         uint32_t w0 = 0, w1 = 0;
-                        if (h < heads) {
+                        if (h < hd.count) {
                             const int d0 = K::kFp8 ? c * 16 + 4 * j : c * 16 + 2 * j;
                             const int d1 = K::kFp8 ? d0 + 2 : d0 + 8;
                             if (d0 < a.head_dim) w0 = __ldg(reinterpret_cast<const uint32_t*>(q + 2 * d0));
@@ -428,16 +574,17 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                                 qf[n][c][x] = pack2<false>(f0 * fit, f1 * fit);
                             }
                     }
-                    const float ks = a.k_scale ? __ldg(a.k_scale + kv) : 1.0f;
+                    const float ks = a.k_scale ? __ldg(a.k_scale + hd.kv) : 1.0f;
                     // head 2j + x of this lane's columns: its scale is with the lanes of row 2j + x
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
                         const float b = __shfl_sync(0xffffffffu, back, (2 * j + x) * 4);
                         scale[n][x] = a.scale * ks * b;
                         const int hx = n * 8 + 2 * j + x;
-                        slope[n][x] = a.slopes && hx < heads ? __ldg(a.slopes + head0 + hx) * kLog2e : 0.0f;
-                        if (!(a.softcap > 0.0f)) scale[n][x] *= kLog2e;
+                        slope[n][x] = a.slopes && hx < hd.count ? __ldg(a.slopes + hd.head0 + hx) * kLog2e : 0.0f;
+                        scale[n][x] = a.softcap > 0.0f ? __fdiv_rn(scale[n][x], a.softcap) : scale[n][x] * kLog2e;
                         m[n][x] = -INFINITY;
+                        mu[n][x] = 0.0f;
                         l[n][x] = 0.0f;
                     }
 #pragma unroll
@@ -449,55 +596,57 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
 
             // S^T = K Q^T, two chains of sums
             const uint32_t keys = ring + stage * K::kStage, values = keys + kTile * K::kRow;
+            const uint32_t mask = static_cast<uint32_t>(sh.mask[warp][stage]);
             float s[NT][2][4];
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int x = 0; x < 4; ++x) s[n][0][x] = s[n][1][x] = 0.0f;
-            {
-                const int rw = (lane & 7) + ((lane >> 3) & 1) * 8, ch = lane >> 4;
-                if constexpr (!K::kFp8) {
+            if constexpr (!K::kFp8) {
 #pragma unroll
-                    for (int c = 0; c < K::kSteps; ++c) {
-                        uint32_t f[4];
-                        ldsm4(f, keys + swizzled<K::kChunks>(rw, 2 * c + ch));
+                for (int c = 0; c < K::kSteps; ++c) {
+                    uint32_t f[4];
+                    ldsm4(f, keys + swizzled<K::kChunks>(k_row, 2 * c + k_piece));
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) mma16816<K::kBf16>(s[n][c & 1], f, qf[n][c][0], qf[n][c][1]);
-                    }
-                } else {
+                    for (int n = 0; n < NT; ++n) mma16816<K::kBf16>(s[n][c & 1], f, qf[n][c][0], qf[n][c][1]);
+                }
+            } else {
 #pragma unroll
-                    for (int c = 0; c < K::kSteps; c += 2) {
-                        uint32_t f[4];
-                        ldsm4(f, keys + swizzled<K::kChunks>(rw, c + ch));
+                for (int c = 0; c < K::kSteps; c += 2) {
+                    uint32_t f[4];
+                    ldsm4(f, keys + swizzled<K::kChunks>(k_row, c + k_piece));
 #pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            // four codes of a row: elements 4j, 4j+1 take the place of the product's 2j, 2j+1,
-                            // elements 4j+2, 4j+3 that of 2j+8, 2j+9 (the queries are laid out alike)
-                            const uint32_t f16[4] = {
-                                fp8x2_to_f16x2<MODE>(f[2 * x]), fp8x2_to_f16x2<MODE>(f[2 * x + 1]),
-                                fp8x2_to_f16x2<MODE>(f[2 * x] >> 16), fp8x2_to_f16x2<MODE>(f[2 * x + 1] >> 16)};
+                    for (int x = 0; x < 2; ++x) {
+                        // four codes of a row: elements 4j, 4j+1 take the place of the product's 2j, 2j+1,
+                        // elements 4j+2, 4j+3 that of 2j+8, 2j+9 (the queries are laid out alike)
+                        const uint32_t f16[4] = {
+                            fp8x2_to_f16x2<MODE>(f[2 * x]), fp8x2_to_f16x2<MODE>(f[2 * x + 1]),
+                            fp8x2_to_f16x2<MODE>(f[2 * x] >> 16), fp8x2_to_f16x2<MODE>(f[2 * x + 1] >> 16)};
 #pragma unroll
-                            for (int n = 0; n < NT; ++n)
-                                mma16816<false>(s[n][x], f16, qf[n][c + x][0], qf[n][c + x][1]);
-                        }
+                        for (int n = 0; n < NT; ++n) mma16816<false>(s[n][x], f16, qf[n][c + x][0], qf[n][c + x][1]);
                     }
                 }
             }
 
-            // scores of tokens g and g + 8, heads 2j and 2j + 1
-            const uint32_t mask = static_cast<uint32_t>(sh.mask[warp][stage]);
-            const bool in0 = (mask >> g) & 1u, in1 = (mask >> (g + 8)) & 1u;
-            const float away = static_cast<float>(at.t * kTile + g - (at.n - 1));  // distance to the newest token, <= 0
+            // scores of tokens g and g + 8, heads 2j and 2j + 1, times log2(e)
             uint32_t ph[NT][2], pl[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 float p[4];
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    float f = (s[n][0][x] + s[n][1][x]) * scale[n][x & 1];
-                    if (a.softcap > 0.0f) f = a.softcap * kLog2e * tanhf(f / a.softcap);
-                    f = __fmaf_rn(slope[n][x & 1], away + (x & 2 ? 8.0f : 0.0f), f);
-                    p[x] = (x & 2 ? in1 : in0) ? f : -INFINITY;
+                for (int x = 0; x < 4; ++x) p[x] = (s[n][0][x] + s[n][1][x]) * scale[n][x & 1];
+                if (rules) {
+                    // distance to the newest token, <= 0
+                    const float away = static_cast<float>(at.span.base + at.t * kTile + g - (at.span.len - 1));
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        if (a.softcap > 0.0f) p[x] = a.softcap * kLog2e * tanh_fast(p[x]);
+                        p[x] = __fmaf_rn(slope[n][x & 1], away + (x & 2 ? 8.0f : 0.0f), p[x]);
+                    }
+                }
+                if (mask != 0xffffu) {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) p[x] = (mask >> (x & 2 ? g + 8 : g)) & 1u ? p[x] : -INFINITY;
                 }
                 const float t0 = fmaxf(p[0], p[2]), t1 = fmaxf(p[1], p[3]);
                 if (__any_sync(0xffffffffu, t0 > m[n][0] || t1 > m[n][1])) {
@@ -510,6 +659,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                         top[x] = fmaxf(top[x], m[n][x]);
                         const float r = rescale(m[n][x], top[x]);
                         m[n][x] = top[x];
+                        mu[n][x] = top[x] == -INFINITY ? 0.0f : top[x];
                         l[n][x] *= r;
 #pragma unroll
                         for (int c = 0; c < K::kSteps; ++c) {
@@ -520,8 +670,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                 }
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
-                    const float mx = m[n][x & 1] == -INFINITY ? 0.0f : m[n][x & 1];
-                    p[x] = exp2_fast(p[x] - mx);
+                    p[x] = exp2_fast(p[x] - mu[n][x & 1]);
                     l[n][x & 1] += p[x];
                 }
                 // high and low terms, tokens x heads -> heads x tokens
@@ -530,19 +679,17 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                     const uint32_t high = pack2<K::kBf16>(p[2 * x], p[2 * x + 1]);
                     float f0, f1;
                     unpack2<K::kBf16>(high, f0, f1);
-                    const uint32_t low = pack2<K::kBf16>(p[2 * x] - f0, p[2 * x + 1] - f1);
                     ph[n][x] = transpose8x8(high);
-                    pl[n][x] = transpose8x8(low);
+                    pl[n][x] = transpose8x8(pack2<K::kBf16>(p[2 * x] - f0, p[2 * x + 1] - f1));
                 }
             }
 
             // O^T += V^T P^T
             if constexpr (!K::kFp8) {
-                const int rw = (lane & 7) + (lane >> 4) * 8, ch = (lane >> 3) & 1;
 #pragma unroll
                 for (int c = 0; c < K::kSteps; ++c) {
                     uint32_t f[4];
-                    ldsm4_t(f, values + swizzled<K::kChunks>(rw, 2 * c + ch));
+                    ldsm4_t(f, values + swizzled<K::kChunks>(v_row, 2 * c + v_piece));
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         mma16816<K::kBf16>(o[n][c], f, ph[n][0], ph[n][1]);
@@ -550,11 +697,10 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                     }
                 }
             } else {
-                const int rw = (lane & 7) + ((lane >> 3) & 1) * 8, ch = lane >> 4;
 #pragma unroll
                 for (int c = 0; c < K::kSteps; c += 2) {
                     uint32_t f[4];
-                    ldsm4_t(f, values + swizzled<K::kChunks>(rw, c + ch));
+                    ldsm4_t(f, values + swizzled<K::kChunks>(v_row, c + v_piece));
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
                         // a transposed pair of bytes holds elements 2g, 2g+1 of two tokens: row g of the product
@@ -576,10 +722,9 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
             const bool ends = at.t + 1 == at.nt, stops = i + 1 == my_tiles;
             if (ends || stops) {
                 const bool whole = ends && ta == 0;
-                const int32_t heads = min(K::kHeads, (kv + 1) * a.group - head0);
-                const int which = stops ? 1 : 0;
-                const float vs = a.v_scale ? __ldg(a.v_scale + kv) : 1.0f;
-                float* part = whole ? nullptr : a.warp_part + id * K::kPart;
+                const Heads<K::kHeads> hd(a, at.item);
+                const float vs = a.v_scale ? __ldg(a.v_scale + hd.kv) : 1.0f;
+                float* part = a.warp_part + static_cast<int64_t>(id) * K::kPart;
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -594,7 +739,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                         for (int x = 0; x < 2; ++x) {
                             const int h = n * 8 + 2 * j + x;
                             f[x] = l[n][x] == 0.0f ? 0.0f : __fdiv_rn(vs, l[n][x]);
-                            if (g == 0 && h < heads) store_lse(a, at.r, head0 + h, m[n][x], l[n][x]);
+                            if (g == 0 && h < hd.count) store_lse(a, at.r, hd.head0 + h, m[n][x], l[n][x]);
                         }
 #pragma unroll
                         for (int c = 0; c < K::kSteps; ++c) {
@@ -604,17 +749,17 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                                 const uint32_t u = transpose8x8(pack2<K::kBf16>(o[n][c][0] * f[0], o[n][c][1] * f[1]));
                                 const uint32_t w = transpose8x8(pack2<K::kBf16>(o[n][c][2] * f[0], o[n][c][3] * f[1]));
                                 const int h = n * 8 + g, d = c * 16 + 2 * j;
-                                char* at_out = out + 2 * (at.r * a.out_req + (head0 + h) * a.out_head + d);
-                                if (h < heads && d < a.head_dim) *reinterpret_cast<uint32_t*>(at_out) = u;
-                                if (h < heads && d + 8 < a.head_dim) *reinterpret_cast<uint32_t*>(at_out + 16) = w;
+                                char* at_out = out + 2 * (at.r * a.out_req + (hd.head0 + h) * a.out_head + d);
+                                if (h < hd.count && d < a.head_dim) *reinterpret_cast<uint32_t*>(at_out) = u;
+                                if (h < hd.count && d + 8 < a.head_dim) *reinterpret_cast<uint32_t*>(at_out + 16) = w;
                             } else {
 #pragma unroll
                                 for (int x = 0; x < 2; ++x) {
                                     const int h = n * 8 + 2 * j + x, d = c * 16 + 2 * g;
                                     const float u = o[n][c][x] * f[x], w = o[n][c][x + 2] * f[x];
                                     const uint32_t two = a.q_f16 ? pack2<false>(u, w) : pack2<true>(u, w);
-                                    if (h < heads && d < a.head_dim)
-                                        *reinterpret_cast<uint32_t*>(out + 2 * (at.r * a.out_req + (head0 + h) * a.out_head + d)) = two;
+                                    if (h < hd.count && d < a.head_dim)
+                                        *reinterpret_cast<uint32_t*>(out + 2 * (at.r * a.out_req + (hd.head0 + h) * a.out_head + d)) = two;
                                 }
                             }
                         }
@@ -637,7 +782,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                     }
                 }
                 if (!whole && lane == 0) {
-                    Part& p = sh.part[2 * warp + which];
+                    Part& p = sh.part[2 * warp + (stops ? 1 : 0)];
                     p.start = x0 + i - at.t;
                     p.r = at.r;
                     p.item = at.item;
@@ -652,8 +797,9 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
         cp_async_wait<0>();
     }
     __syncthreads();  // every ring is done with: the last parts are staged there
+    float* staged = reinterpret_cast<float*>(smem);
     if (sh.part[2 * warp + 1].start >= 0) {
-        float* mine = reinterpret_cast<float*>(smem) + warp * (K::kHeads * K::kLd);
+        float* mine = staged + warp * (K::kHeads * K::kLd);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -671,120 +817,108 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                 }
             }
     }
-    __syncthreads();
-
-    // join the parts of each item inside the CTA: runs of consecutive parts with one start
-    constexpr int kFour = DP / 4;
-    if (tid < 2) sh.joins[tid] = 0;
-    bool open[2] = {false, false};
-    int32_t open_first[2] = {0, 0}, open_last[2] = {0, 0};
-    Part open_part[2];
-    for (int e = 0; e < 2 * W;) {
-        const Part p = sh.part[e];
-        if (p.start < 0) {
-            ++e;
-            continue;
+    if (warp == 0) {
+        // the joined items: runs of consecutive parts with one start
+        const int64_t start = lane < 2 * W ? sh.part[lane].start : -1;
+        const uint32_t have = __ballot_sync(0xffffffffu, start >= 0), lower = have & ((1u << lane) - 1u);
+        const int64_t left = __shfl_sync(0xffffffffu, start, lower ? 31 - __clz(lower) : lane);
+        const uint32_t leads = __ballot_sync(0xffffffffu, start >= 0 && (!lower || left != start));
+        if ((leads >> lane) & 1u) sh.lead[__popc(leads & ((1u << lane) - 1u))] = lane;
+        if (lane == 0) {
+            sh.items = __popc(leads);
+            sh.lead[__popc(leads)] = 2 * W;
         }
-        int last = e;
-        for (int k = e + 1; k < 2 * W; ++k) {
-            if (sh.part[k].start < 0) continue;
-            if (sh.part[k].start != p.start) break;
-            last = k;
-        }
-        const int32_t tb = sh.part[last].tb;
-        const bool whole = p.ta == 0 && tb == p.nt;
-        const int32_t kv = p.item / a.blocks, head0 = kv * a.group + p.item % a.blocks * K::kHeads;
-        const int32_t heads = min(K::kHeads, (kv + 1) * a.group - head0);
-        const float vs = a.v_scale ? __ldg(a.v_scale + kv) : 1.0f;
-        const int slot = p.ta > 0 ? 0 : 1;
-        float* to = a.cta_part + (static_cast<int64_t>(blockIdx.x) * 2 + slot) * K::kPart;
-        for (int i = tid; i < heads * kFour; i += K::kThreads) {
-            const int h = i / kFour, d = i % kFour * 4;
-            float top = -INFINITY;
-            for (int k = e; k <= last; ++k)
-                if (sh.part[k].start >= 0) top = fmaxf(top, sh.m[k][h]);
-            float sum_l = 0.0f;
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int k = e; k <= last; ++k) {
-                if (sh.part[k].start < 0) continue;
-                const float r = rescale(sh.m[k][h], top);
-                const float* from = (k & 1) ? reinterpret_cast<const float*>(smem) + ((k >> 1) * K::kHeads + h) * K::kLd + d
-                                            : a.warp_part + (static_cast<int64_t>(blockIdx.x) * W + (k >> 1)) * K::kPart + h * DP + d;
-                const float4 f = *reinterpret_cast<const float4*>(from);
-                sum_l = __fmaf_rn(sh.l[k][h], r, sum_l);
-                acc.x = __fmaf_rn(f.x, r, acc.x);
-                acc.y = __fmaf_rn(f.y, r, acc.y);
-                acc.z = __fmaf_rn(f.z, r, acc.z);
-                acc.w = __fmaf_rn(f.w, r, acc.w);
-            }
-            if (whole) {
-                const float f = sum_l == 0.0f ? 0.0f : __fdiv_rn(vs, sum_l);
-                store_out4(a, p.r, head0 + h, d, make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
-                if (d == 0) store_lse(a, p.r, head0 + h, top, sum_l);
-            } else {
-                *reinterpret_cast<float4*>(to + h * DP + d) = acc;
-                if (d == 0) {
-                    to[K::kHeads * DP + h] = top;
-                    to[K::kHeads * DP + K::kHeads + h] = sum_l;
-                }
-            }
-        }
-        if (!whole) {
-            // the CTAs that hold the item's first and last tile
-            const int64_t end = p.start + p.nt - 1;
-            open[slot] = true;
-            open_part[slot] = p;
-            open_first[slot] = static_cast<int32_t>(((p.start + 1) * workers - 1) / total / W);
-            open_last[slot] = static_cast<int32_t>(((end + 1) * workers - 1) / total / W);
-        }
-        e = last + 1;
     }
-    if (!open[0] && !open[1]) return;
-
-    // join between CTAs: the last one to arrive does it, and leaves the ticket at zero
-    __threadfence();
     __syncthreads();
-    if (tid < 2 && (tid == 0 ? open[0] : open[1])) {
-        const int32_t first = tid == 0 ? open_first[0] : open_first[1], last = tid == 0 ? open_last[0] : open_last[1];
-        const int32_t n = last - first + 1;
-        if (atomicAdd(a.tickets + first, 1) == n - 1) {
-            a.tickets[first] = 0;
-            sh.joins[tid] = 1;
+
+    // join the parts of each item inside the CTA
+    const int32_t joined = sh.items;
+    if (joined == 0) return;
+    for (int i = tid; i < joined * K::kHeads * K::kFour; i += K::kThreads) {
+        const int grp = i / (K::kHeads * K::kFour), h = i / K::kFour % K::kHeads, d = i % K::kFour * 4;
+        const int e = sh.lead[grp], end = sh.lead[grp + 1];
+        const Part& p = sh.part[e];
+        const Heads<K::kHeads> hd(a, p.item);
+        if (h >= hd.count) continue;
+        float top = -INFINITY;
+        int32_t tb = 0;
+        for (int k = e; k < end; ++k)
+            if (sh.part[k].start >= 0) {
+                top = fmaxf(top, sh.m[k][h]);
+                tb = sh.part[k].tb;
+            }
+        float sum_l = 0.0f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k = e; k < end; ++k) {
+            if (sh.part[k].start < 0) continue;
+            const float r = rescale(sh.m[k][h], top);
+            const float* from = (k & 1) ? staged + ((k >> 1) * K::kHeads + h) * K::kLd + d
+                                        : a.warp_part + (static_cast<int64_t>(blockIdx.x) * W + (k >> 1)) * K::kPart + h * DP + d;
+            sum_l = __fmaf_rn(sh.l[k][h], r, sum_l);
+            acc = fma4(*reinterpret_cast<const float4*>(from), r, acc);
         }
-        __threadfence();
+        if (p.ta == 0 && tb == p.nt) {
+            const float vs = a.v_scale ? __ldg(a.v_scale + hd.kv) : 1.0f;
+            store_out4(a, p.r, hd.head0 + h, d, scale4(acc, sum_l == 0.0f ? 0.0f : __fdiv_rn(vs, sum_l)));
+            if (d == 0) store_lse(a, p.r, hd.head0 + h, top, sum_l);
+        } else {
+            float* to = a.cta_part + (static_cast<int64_t>(blockIdx.x) * 3 + (p.ta > 0 ? 0 : 1)) * K::kPart;
+            *reinterpret_cast<float4*>(to + h * DP + d) = acc;
+            if (d == 0) {
+                to[K::kHeads * DP + h] = top;
+                to[K::kHeads * DP + K::kHeads + h] = sum_l;
+            }
+        }
+    }
+
+    // Join between CTAs.  Slot 0 is the end (or middle) of an item that began in an earlier CTA, slot 1 the start of one
+    // that ends in a later CTA; an item's CTAs are first .. last.  More than kJoin of them join in groups, then the groups.
+    Part open[2] = {sh.part[sh.lead[0]], sh.part[sh.lead[joined - 1]]};
+    bool is_open[2] = {open[0].ta > 0, false};
+    {
+        int k = 2 * W - 1;
+        while (sh.part[k].start < 0) --k;
+        is_open[1] = open[1].ta == 0 && sh.part[k].tb < open[1].nt;
+    }
+    if (!is_open[0] && !is_open[1]) return;
+    int32_t first[2], last[2], size[2];
+#pragma unroll
+    for (int slot = 0; slot < 2; ++slot) {
+        if (!is_open[slot]) continue;
+        const int64_t tile = open[slot].start;
+        first[slot] = static_cast<int32_t>(((tile + 1) * workers - 1) / total / W);
+        last[slot] = static_cast<int32_t>(((tile + open[slot].nt) * workers - 1) / total / W);
+        const int32_t n = last[slot] - first[slot] + 1;
+        size[slot] = n <= kJoin ? n : max(12, (n + kJoin - 1) / kJoin);
     }
     __syncthreads();
 #pragma unroll
     for (int slot = 0; slot < 2; ++slot) {
-        if (!open[slot] || !sh.joins[slot]) continue;
-        const Part& p = open_part[slot];
-        const int32_t kv = p.item / a.blocks, head0 = kv * a.group + p.item % a.blocks * K::kHeads;
-        const int32_t heads = min(K::kHeads, (kv + 1) * a.group - head0);
-        const float vs = a.v_scale ? __ldg(a.v_scale + kv) : 1.0f;
-        const int32_t first = open_first[slot], last = open_last[slot];
-        for (int i = tid; i < heads * kFour; i += K::kThreads) {
-            const int h = i / kFour, d = i % kFour * 4;
-            float top = -INFINITY;
-            for (int32_t c = first; c <= last; ++c) {
-                const float* from = a.cta_part + (static_cast<int64_t>(c) * 2 + (c == first)) * K::kPart;
-                top = fmaxf(top, __ldcg(from + K::kHeads * DP + h));
-            }
-            float sum_l = 0.0f;
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int32_t c = first; c <= last; ++c) {
-                const float* from = a.cta_part + (static_cast<int64_t>(c) * 2 + (c == first)) * K::kPart;
-                const float r = rescale(__ldcg(from + K::kHeads * DP + h), top);
-                const float4 f = __ldcg(reinterpret_cast<const float4*>(from + h * DP + d));
-                sum_l = __fmaf_rn(__ldcg(from + K::kHeads * DP + K::kHeads + h), r, sum_l);
-                acc.x = __fmaf_rn(f.x, r, acc.x);
-                acc.y = __fmaf_rn(f.y, r, acc.y);
-                acc.z = __fmaf_rn(f.z, r, acc.z);
-                acc.w = __fmaf_rn(f.w, r, acc.w);
-            }
-            const float f = sum_l == 0.0f ? 0.0f : __fdiv_rn(vs, sum_l);
-            store_out4(a, p.r, head0 + h, d, make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
-            if (d == 0) store_lse(a, p.r, head0 + h, top, sum_l);
-        }
+        if (tid != 32 * slot || !is_open[slot]) continue;
+        const int32_t lo = first[slot] + (static_cast<int32_t>(blockIdx.x) - first[slot]) / size[slot] * size[slot];
+        const int32_t n = min(size[slot], last[slot] - lo + 1);
+        // a group of one has no ticket: that CTA's may be the next item's
+        sh.won[slot] = n == 1 || arrive_last(a.tickets + lo, n);
+    }
+    __syncthreads();
+    const int64_t kCta = 3 * K::kPart;
+#pragma unroll
+    for (int slot = 0; slot < 2; ++slot) {
+        if (!is_open[slot] || !sh.won[slot]) continue;
+        const Part& p = open[slot];
+        const int32_t at = (static_cast<int32_t>(blockIdx.x) - first[slot]) / size[slot];
+        const int32_t lo = first[slot] + at * size[slot], n = min(size[slot], last[slot] - lo + 1);
+        const int32_t groups = (last[slot] - first[slot]) / size[slot] + 1;
+        const float* parts = a.cta_part + lo * kCta;
+        float* group = a.cta_part + lo * kCta + 2 * K::kPart;
+        join_parts<K>(a, sh, parts, kCta, parts + (lo == first[slot] ? K::kPart : 0), n, p.r, p.item,
+                      groups == 1 ? nullptr : group, DP);
+        if (groups == 1) continue;
+        if (tid == 0) sh.won[slot] = arrive_last(a.tickets + gridDim.x + first[slot], groups);
+        __syncthreads();
+        if (!sh.won[slot]) continue;
+        const float* heads = a.cta_part + first[slot] * kCta + 2 * K::kPart;
+        join_parts<K>(a, sh, heads, kCta * size[slot], heads, groups, p.r, p.item, nullptr, DP);
     }
 }
 
@@ -867,8 +1001,8 @@ extern "C" int mf_paged_attn_create(const mf_paged_attn_config* config, mf_paged
                                        kernel.shared));
     const int ctas = state().sm_count;
     const size_t warp_part = static_cast<size_t>(ctas) * kernel.warps * kernel.part_floats * 4;
-    const size_t cta_part = static_cast<size_t>(ctas) * 2 * kernel.part_floats * 4;
-    const size_t bytes = warp_part + cta_part + static_cast<size_t>(ctas) * 4;
+    const size_t cta_part = static_cast<size_t>(ctas) * 3 * kernel.part_floats * 4;
+    const size_t bytes = warp_part + cta_part + static_cast<size_t>(ctas) * 8;
     mf_paged_attn_s* h = new (std::nothrow) mf_paged_attn_s{};
     if (!h) return fail(MF_ERR_ALLOCATOR_EXHAUSTED, "mf_paged_attn_create: out of host memory");
     cudaError_t err = cudaMalloc(&h->workspace, bytes);
@@ -880,7 +1014,7 @@ extern "C" int mf_paged_attn_create(const mf_paged_attn_config* config, mf_paged
         return cuda_fail(err, "mf_paged_attn_create: cudaMalloc");
     }
     char* w = static_cast<char*>(h->workspace);
-    err = cudaMemset(w + warp_part + cta_part, 0, static_cast<size_t>(ctas) * 4);
+    err = cudaMemset(w + warp_part + cta_part, 0, static_cast<size_t>(ctas) * 8);
     if (err == cudaSuccess) err = cudaStreamSynchronize(nullptr);  // streams that do not wait for the default one may run it
     if (err != cudaSuccess) {
         cudaFree(h->workspace);
