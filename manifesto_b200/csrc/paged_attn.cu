@@ -182,6 +182,13 @@ struct Place {
     }
 };
 
+// x * y / z, in 32 bits where they hold it (a 64-bit division is a long call).
+__device__ __forceinline__ int64_t mul_div(int64_t x, int32_t y, int64_t z) {
+    const int64_t p = x * y;
+    if (((p | z) >> 32) == 0) return static_cast<uint32_t>(p) / static_cast<uint32_t>(z);
+    return p / z;
+}
+
 // What is known of one part of an item that a warp or CTA summed.
 struct Part {
     int64_t start;   // first tile of the item in the row of all tiles; -1: no part
@@ -190,6 +197,9 @@ struct Part {
 };
 
 constexpr int kJoin = 16;  // most parts that one step of a join between CTAs takes
+// A maximum is only replaced by one that is this much larger (in powers of two): until then the weights grow up to
+// 2^8, which float32 sums and both terms of a weight hold as well, and what is summed is not rescaled.
+constexpr float kLazy = 8.0f;
 
 // MODE: dtype of the cache; DP: head_dim padded to 64, 128 or 256; NT: blocks
 // of 8 query heads a warp holds; W: warps; S: stages of a warp's ring.
@@ -232,6 +242,13 @@ template <int CHUNKS>
 __device__ __forceinline__ uint32_t swizzled(int row, int c) {
     if constexpr (CHUNKS >= 8) return static_cast<uint32_t>(row * CHUNKS + (c ^ (row & 7))) * 16u;
     else return static_cast<uint32_t>(row * CHUNKS + (c ^ ((row >> 1) & (CHUNKS - 1)))) * 16u;
+}
+
+// The same for an even piece c more, from the place of a row's piece 0 or 1 (stages start at multiples of 128).
+template <int CHUNKS>
+__device__ __forceinline__ uint32_t pieces_on(uint32_t at, int c) {
+    if constexpr (CHUNKS >= 8) return (at ^ static_cast<uint32_t>((c & 7) * 16)) + static_cast<uint32_t>((c >> 3) * 128);
+    else return at ^ static_cast<uint32_t>(c * 16);
 }
 
 // Write `f` (4 floats of head h, elements d..d+3, normalised) to the output.
@@ -278,14 +295,16 @@ __device__ __forceinline__ bool arrive_last(int32_t* ticket, int32_t count) {
     return true;
 }
 
-// Joins parts 0 .. n-1 (n <= kJoin) at first + k * stride floats: to the
-// output if `to` is NULL, else to a part there.  All threads of the CTA.
+// Joins parts 0 .. n-1 (n <= kJoin) at first + k * stride floats, but the first
+// at at0 and the last at at_end: to the output if `to` is NULL, else to a part
+// there.  All threads of the CTA.
 template <class K>
 __device__ __forceinline__ void join_parts(const AttnArgs& a, typename K::Shared& sh, const float* first, int64_t stride,
-                                           const float* at0, int32_t n, int32_t r, int32_t item, float* to, int dp) {
+                                           const float* at0, const float* at_end, int32_t n, int32_t r, int32_t item, float* to,
+                                           int dp) {
     const int tid = threadIdx.x;
     const Heads<K::kHeads> hd(a, item);
-    auto part = [&](int k) { return k == 0 ? at0 : first + k * stride; };
+    auto part = [&](int k) { return k == 0 ? at0 : k == n - 1 ? at_end : first + k * stride; };
     constexpr int kAhead = 8;
     float4 f[kAhead];
     int i = tid;
@@ -395,125 +414,157 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
     if (blockIdx.x >= ctas) return;
     const int32_t workers = ctas * W;
     const int32_t id = blockIdx.x * W + warp;
-    const int64_t x0 = total * id / workers, x1 = total * (id + 1) / workers;
+    const int64_t x0 = mul_div(total, id, workers), x1 = mul_div(total, id + 1, workers);
     const int32_t my_tiles = static_cast<int32_t>(x1 - x0);
 
     uint32_t qf[NT][K::kSteps][2];
     float o[NT][K::kSteps][4];
-    float m[NT][2], mu[NT][2], l[NT][2], scale[NT][2], slope[NT][2];  // mu: m, or 0 while m is -inf
+    float m[NT][2], l[NT][2], scale[NT][2], slope[NT][2];
     if (my_tiles > 0) {
-        // the place of tile x0: the thread whose requests hold it, then the request among them
-        int lo = 0, hi = K::kThreads;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (sh.prefix[mid] <= x0) lo = mid;
-            else hi = mid;
-        }
-        Place at{};
-        int64_t before = sh.prefix[lo];
-        for (int32_t r0 = lo * per;; r0 += 32) {
-            const int32_t nt = r0 + lane < a.n_requests ? tiles_of(span_of(a, r0 + lane)) : 0;
-            const int64_t mine = static_cast<int64_t>(nt) * items;
-            int64_t upto = mine;
+        // the place of tile x0: the warp, then the thread whose requests hold it, then the request among them
+        int64_t before = 0;
+        int lo = 0;
 #pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const int64_t x = __shfl_up_sync(0xffffffffu, upto, d);
-                if (lane >= d) upto += x;
+        for (int w = 1; w < W; ++w)
+            if (sh.prefix[32 * w] <= x0) lo = 32 * w;
+        lo += 31 - __clz(__ballot_sync(0xffffffffu, sh.prefix[lo + lane] <= x0));
+        before = sh.prefix[lo];
+        Place at{};
+        at.r = lo;
+        if (per > 1) {
+            for (int32_t r0 = lo * per;; r0 += 32) {
+                const int32_t nt = r0 + lane < a.n_requests ? tiles_of(span_of(a, r0 + lane)) : 0;
+                const int64_t mine = static_cast<int64_t>(nt) * items;
+                int64_t upto = mine;
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                    const int64_t x = __shfl_up_sync(0xffffffffu, upto, d);
+                    if (lane >= d) upto += x;
+                }
+                const uint32_t past = __ballot_sync(0xffffffffu, before + upto > x0);
+                if (past || r0 + 32 >= a.n_requests) {
+                    const int src = past ? __ffs(past) - 1 : 0;
+                    at.r = r0 + src;
+                    before += __shfl_sync(0xffffffffu, upto - mine, src);
+                    break;
+                }
+                before += __shfl_sync(0xffffffffu, upto, 31);
             }
-            const uint32_t past = __ballot_sync(0xffffffffu, before + upto > x0);
-            if (past || r0 + 32 >= a.n_requests) {
-                const int src = past ? __ffs(past) - 1 : 0;
-                at.r = r0 + src;
-                before += __shfl_sync(0xffffffffu, upto - mine, src);
-                break;
-            }
-            before += __shfl_sync(0xffffffffu, upto, 31);
         }
         at.span = span_of(a, at.r);
         at.nt = tiles_of(at.span);
         const int64_t in_request = x0 - before;
-        at.item = static_cast<int32_t>(in_request / at.nt);
-        at.t = static_cast<int32_t>(in_request % at.nt);
+        at.item = static_cast<int32_t>(mul_div(in_request, 1, at.nt));
+        at.t = static_cast<int32_t>(in_request - static_cast<int64_t>(at.item) * at.nt);
 
         const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * (S * K::kStage);
         Place load = at;
         int32_t to_load = my_tiles;
         const bool whole_tiles = a.page % kTile == 0;  // a tile lies in one page
-        const int lane_row = whole_tiles ? 0 : lane & 15;
-        // place of this lane's piece in the first rows that one instruction copies, and of the next rows
-        constexpr int kRows = 32 / K::kChunks > 0 ? 32 / K::kChunks : 1;  // rows of one instruction
+        constexpr int kRows = 32 / K::kChunks > 0 ? 32 / K::kChunks : 1;  // rows that one instruction copies
         constexpr int kCopies = kTile * K::kChunks / 32;
         const int piece_row = lane / K::kChunks, piece = lane % K::kChunks;
-        const int64_t row_bytes = a.token_stride * K::kBytes;
+        const int64_t row_bytes = a.token_stride * K::kBytes, page_bytes = a.page_stride * K::kBytes;
         const int64_t lane_bytes = piece_row * row_bytes + piece * 16;
         const bool piece_in = piece * (16 / K::kBytes) < a.head_dim;
-        int32_t page_no = -1;
-        // the page of the tile at `load`, or of this lane's row of it
-        auto look_up = [&]() {
+        const int64_t kv_gap = static_cast<const char*>(a.v) - static_cast<const char*>(a.k);
+        const int32_t lane_row = whole_tiles ? 0 : lane & 15;
+        // of the tile at `load`: the page (or that of this lane's row), its place in the table's row and the tile's in it
+        const int32_t* table_row = nullptr;
+        const char* head_at = nullptr;
+        int32_t page_no = -1, page_idx = 0, page_off = 0;
+        auto look_up = [&](bool new_item) {
+            if (to_load == 0) return;
             const int32_t tok = load.span.base + load.t * kTile + lane_row;
-            if (to_load > 0 && tok < load.span.len)
-                page_no = __ldg(a.table + load.r * a.table_stride + static_cast<uint32_t>(tok) / static_cast<uint32_t>(a.page));
+            if (new_item) {
+                table_row = a.table + load.r * a.table_stride;
+                head_at = static_cast<const char*>(a.k) + load.item / a.blocks * a.head_stride * K::kBytes + lane_bytes;
+            }
+            if (new_item || !whole_tiles) {
+                page_idx = static_cast<int32_t>(static_cast<uint32_t>(tok) / static_cast<uint32_t>(a.page));
+                page_off = tok - page_idx * a.page;
+            } else if ((page_off += kTile) >= a.page) {
+                page_off = 0;
+                ++page_idx;
+            }
+            if (tok < load.span.len) page_no = __ldg(table_row + page_idx);
         };
+        uint32_t partial = 0;  // stages that lack some of their tokens: those have a mask
         auto issue = [&](int stage) {
             if (to_load > 0) {
-                const int32_t tok0 = load.span.base + load.t * kTile, tok = tok0 + (lane & 15);
-                const bool seen = tok >= load.span.first && tok < load.span.len;
-                bool ok = seen;
-                if (ok && (page_no < 0 || page_no >= a.n_pages)) {
-                    ok = false;
-                    atomicExch(a.status, MF_DEVICE_BAD_PAGE);
-                }
-                const uint32_t mask = __ballot_sync(0xffffffffu, ok) & 0xffffu;
-                if (lane == 0) sh.mask[warp][stage] = static_cast<int32_t>(mask);
-                const int32_t kv = load.item / a.blocks;
+                const int32_t tok0 = load.span.base + load.t * kTile;
                 const uint32_t dst = ring + stage * K::kStage;
-                const int32_t off_page = static_cast<int32_t>(static_cast<uint32_t>(tok0 + lane_row) % static_cast<uint32_t>(a.page));
-                const int64_t at_row = (page_no * a.page_stride + off_page * a.token_stride + kv * a.head_stride) * K::kBytes;
-                if (whole_tiles) {
-                    const char* kp = static_cast<const char*>(a.k) + at_row + lane_bytes;
-                    const int64_t kv_gap = static_cast<const char*>(a.v) - static_cast<const char*>(a.k);
-                    if (mask == 0xffffu && a.head_dim == DP) {
+                const bool page_ok = page_no >= 0 && page_no < a.n_pages;
+                if (whole_tiles && page_ok && tok0 >= load.span.first && tok0 + kTile <= load.span.len) {
+                    partial &= ~(1u << stage);
+                    const char* kp = head_at + (page_no * page_bytes + page_off * row_bytes);
 #pragma unroll
-                        for (int i = 0; i < kCopies; ++i, kp += kRows * row_bytes) {
-                            const uint32_t to = dst + swizzled<K::kChunks>(i * kRows + piece_row, piece);
+                    for (int i = 0; i < kCopies; ++i, kp += kRows * row_bytes) {
+                        const uint32_t to = dst + swizzled<K::kChunks>(i * kRows + piece_row, piece);
+                        if (piece_in) {
                             cp_async16(to, kp, 16u);
                             cp_async16(to + kTile * K::kRow, kp + kv_gap, 16u);
                         }
-                    } else {
-#pragma unroll 1
-                        for (int i = 0; i < kCopies; ++i, kp += kRows * row_bytes) {
-                            const int rw = i * kRows + piece_row;
-                            const bool get = piece_in && ((mask >> rw) & 1u);
-                            const uint32_t to = dst + swizzled<K::kChunks>(rw, piece);
-                            cp_async16(to, get ? kp : static_cast<const char*>(a.k), get ? 16u : 0u);
-                            cp_async16(to + kTile * K::kRow, get ? kp + kv_gap : static_cast<const char*>(a.v), get ? 16u : 0u);
-                        }
                     }
                 } else {
+                    const int32_t tok = tok0 + (lane & 15);
+                    const bool seen = tok >= load.span.first && tok < load.span.len;
+                    if (seen && !page_ok) atomicExch(a.status, MF_DEVICE_BAD_PAGE);
+                    const uint32_t mask = __ballot_sync(0xffffffffu, seen && page_ok) & 0xffffu;
+                    partial = (partial & ~(1u << stage)) | (mask != 0xffffu ? 1u << stage : 0u);
+                    if (lane == 0) sh.mask[warp][stage] = static_cast<int32_t>(mask);
+                    const int64_t at_row = page_no * page_bytes + page_off * row_bytes;
 #pragma unroll 1
                     for (int i = 0; i < kCopies; ++i) {
                         const int rw = i * kRows + piece_row;
-                        const int64_t row_at = __shfl_sync(0xffffffffu, at_row, rw);
+                        // one page: rows follow the tile's first; else each row's place is with the lane of its number
+                        const int64_t row_at = whole_tiles ? at_row + i * kRows * row_bytes
+                                                           : __shfl_sync(0xffffffffu, at_row, rw) - piece_row * row_bytes;
                         const bool get = piece_in && ((mask >> rw) & 1u);
-                        const int64_t byte = get ? row_at + piece * 16 : 0;
+                        const char* kp = get ? head_at + row_at : static_cast<const char*>(a.k);
                         const uint32_t to = dst + swizzled<K::kChunks>(rw, piece);
-                        cp_async16(to, static_cast<const char*>(a.k) + byte, get ? 16u : 0u);
-                        cp_async16(to + kTile * K::kRow, static_cast<const char*>(a.v) + byte, get ? 16u : 0u);
+                        cp_async16(to, kp, get ? 16u : 0u);
+                        cp_async16(to + kTile * K::kRow, kp + kv_gap, get ? 16u : 0u);
                     }
                 }
                 load.next(a, items);
                 --to_load;
-                look_up();
+                look_up(load.t == 0);
             }
             cp_async_commit();
         };
-        look_up();
+        look_up(true);
+        if (a.head_dim < DP) {  // what is past the head is never copied: zeros
+            for (int i = lane; i < S * K::kStage / 16; i += 32)
+                reinterpret_cast<uint4*>(smem + warp * (S * K::kStage))[i] = make_uint4(0, 0, 0, 0);
+            __syncwarp();
+        }
 #pragma unroll 1
         for (int s = 0; s < S - 1; ++s) issue(s);
+
+        // the queries of the item at `p`, as they are
+        auto load_queries = [&](const Place& p) {
+            const Heads<K::kHeads> hd(a, p.item);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const int h = n * 8 + g;
+                const char* q = static_cast<const char*>(a.q) + 2 * (p.r * a.q_req + (hd.head0 + h) * a.q_head);
+#pragma unroll
+                for (int c = 0; c < K::kSteps; ++c) {
+                    const int d0 = K::kFp8 ? c * 16 + 4 * j : c * 16 + 2 * j;
+                    const int d1 = K::kFp8 ? d0 + 2 : d0 + 8;
+                    qf[n][c][0] = h < hd.count && d0 < a.head_dim ? __ldg(reinterpret_cast<const uint32_t*>(q + 2 * d0)) : 0u;
+                    qf[n][c][1] = h < hd.count && d1 < a.head_dim ? __ldg(reinterpret_cast<const uint32_t*>(q + 2 * d1)) : 0u;
+                }
+            }
+        };
+        load_queries(at);
 
         // rows of this lane in the loads of a product's operands
         const int k_row = (lane & 7) + ((lane >> 3) & 1) * 8, k_piece = lane >> 4;
         const int v_row = K::kFp8 ? k_row : (lane & 7) + (lane >> 4) * 8, v_piece = K::kFp8 ? k_piece : (lane >> 3) & 1;
+        const uint32_t k_at = swizzled<K::kChunks>(k_row, k_piece);
+        const uint32_t v_at = swizzled<K::kChunks>(v_row, v_piece) + kTile * K::kRow;
         const bool rules = a.softcap > 0.0f || a.slopes;
         int32_t ta = at.t;
         int stage = 0;
@@ -523,40 +574,24 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
             __syncwarp();
             issue(stage == 0 ? S - 1 : stage - 1);
             if (i == 0 || at.t == 0) {
-                // a new item: its queries
+                // a new item; its queries were loaded while the one before it ended
                 ta = at.t;
                 const Heads<K::kHeads> hd(a, at.item);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const int h = n * 8 + g;
-                    const char* q = static_cast<const char*>(a.q) + 2 * (at.r * a.q_req + (hd.head0 + h) * a.q_head);
-                    float top = 0.0f;
-#pragma unroll
-                    for (int c = 0; c < K::kSteps; ++c) {
-                        uint32_t w0 = 0, w1 = 0;
-                        if (h < hd.count) {
-                            const int d0 = K::kFp8 ? c * 16 + 4 * j : c * 16 + 2 * j;
-                            const int d1 = K::kFp8 ? d0 + 2 : d0 + 8;
-                            if (d0 < a.head_dim) w0 = __ldg(reinterpret_cast<const uint32_t*>(q + 2 * d0));
-                            if (d1 < a.head_dim) w1 = __ldg(reinterpret_cast<const uint32_t*>(q + 2 * d1));
-                        }
-                        qf[n][c][0] = w0;
-                        qf[n][c][1] = w1;
-                        if constexpr (K::kFp8) {
-                            float f[4];
-                            if (a.q_f16) {
-                                unpack2<false>(w0, f[0], f[1]);
-                                unpack2<false>(w1, f[2], f[3]);
-                            } else {
-                                unpack2<true>(w0, f[0], f[1]);
-                                unpack2<true>(w1, f[2], f[3]);
-                            }
-                            top = fmaxf(top, fmaxf(fmaxf(fabsf(f[0]), fabsf(f[1])), fmaxf(fabsf(f[2]), fabsf(f[3]))));
-                        }
-                    }
                     float back = 1.0f;
                     if constexpr (K::kFp8) {
                         // f16 queries, scaled by a power of two to a largest magnitude in [1, 2)
+                        float top = 0.0f;
+#pragma unroll
+                        for (int c = 0; c < K::kSteps; ++c)
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) {
+                                float f0, f1;
+                                if (a.q_f16) unpack2<false>(qf[n][c][x], f0, f1);
+                                else unpack2<true>(qf[n][c][x], f0, f1);
+                                top = fmaxf(top, fmaxf(fabsf(f0), fabsf(f1)));
+                            }
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                         const uint32_t field = __float_as_uint(top) >> 23;  // biased exponent
@@ -584,7 +619,6 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                         slope[n][x] = a.slopes && hx < hd.count ? __ldg(a.slopes + hd.head0 + hx) * kLog2e : 0.0f;
                         scale[n][x] = a.softcap > 0.0f ? __fdiv_rn(scale[n][x], a.softcap) : scale[n][x] * kLog2e;
                         m[n][x] = -INFINITY;
-                        mu[n][x] = 0.0f;
                         l[n][x] = 0.0f;
                     }
 #pragma unroll
@@ -595,8 +629,9 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
             }
 
             // S^T = K Q^T, two chains of sums
-            const uint32_t keys = ring + stage * K::kStage, values = keys + kTile * K::kRow;
-            const uint32_t mask = static_cast<uint32_t>(sh.mask[warp][stage]);
+            const uint32_t keys = ring + stage * K::kStage + k_at, values = ring + stage * K::kStage + v_at;
+            const uint32_t mask = (partial >> stage) & 1u ? static_cast<uint32_t>(sh.mask[warp][stage]) : 0xffffu;
+            const bool ends = at.t + 1 == at.nt, stops = i + 1 == my_tiles;  // the item's last tile, or this warp's
             float s[NT][2][4];
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -606,7 +641,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
 #pragma unroll
                 for (int c = 0; c < K::kSteps; ++c) {
                     uint32_t f[4];
-                    ldsm4(f, keys + swizzled<K::kChunks>(k_row, 2 * c + k_piece));
+                    ldsm4(f, pieces_on<K::kChunks>(keys, 2 * c));
 #pragma unroll
                     for (int n = 0; n < NT; ++n) mma16816<K::kBf16>(s[n][c & 1], f, qf[n][c][0], qf[n][c][1]);
                 }
@@ -614,7 +649,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
 #pragma unroll
                 for (int c = 0; c < K::kSteps; c += 2) {
                     uint32_t f[4];
-                    ldsm4(f, keys + swizzled<K::kChunks>(k_row, c + k_piece));
+                    ldsm4(f, pieces_on<K::kChunks>(keys, c));
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
                         // four codes of a row: elements 4j, 4j+1 take the place of the product's 2j, 2j+1,
@@ -627,6 +662,10 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                     }
                 }
             }
+
+            Place following = at;
+            following.next(a, items);
+            if (ends && !stops) load_queries(following);
 
             // scores of tokens g and g + 8, heads 2j and 2j + 1, times log2(e)
             uint32_t ph[NT][2], pl[NT][2];
@@ -649,7 +688,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                     for (int x = 0; x < 4; ++x) p[x] = (mask >> (x & 2 ? g + 8 : g)) & 1u ? p[x] : -INFINITY;
                 }
                 const float t0 = fmaxf(p[0], p[2]), t1 = fmaxf(p[1], p[3]);
-                if (__any_sync(0xffffffffu, t0 > m[n][0] || t1 > m[n][1])) {
+                if (__any_sync(0xffffffffu, t0 > m[n][0] + kLazy || t1 > m[n][1] + kLazy)) {
                     float top[2] = {t0, t1};
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
@@ -659,7 +698,6 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                         top[x] = fmaxf(top[x], m[n][x]);
                         const float r = rescale(m[n][x], top[x]);
                         m[n][x] = top[x];
-                        mu[n][x] = top[x] == -INFINITY ? 0.0f : top[x];
                         l[n][x] *= r;
 #pragma unroll
                         for (int c = 0; c < K::kSteps; ++c) {
@@ -668,9 +706,11 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                         }
                     }
                 }
+                // while nothing is seen, the maximum is -inf and so are the scores: weights of 0
+                const float less[2] = {m[n][0] == -INFINITY ? 0.0f : m[n][0], m[n][1] == -INFINITY ? 0.0f : m[n][1]};
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
-                    p[x] = exp2_fast(p[x] - mu[n][x & 1]);
+                    p[x] = exp2_fast(p[x] - less[x & 1]);
                     l[n][x & 1] += p[x];
                 }
                 // high and low terms, tokens x heads -> heads x tokens
@@ -689,7 +729,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
 #pragma unroll
                 for (int c = 0; c < K::kSteps; ++c) {
                     uint32_t f[4];
-                    ldsm4_t(f, values + swizzled<K::kChunks>(v_row, 2 * c + v_piece));
+                    ldsm4_t(f, pieces_on<K::kChunks>(values, 2 * c));
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         mma16816<K::kBf16>(o[n][c], f, ph[n][0], ph[n][1]);
@@ -700,7 +740,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
 #pragma unroll
                 for (int c = 0; c < K::kSteps; c += 2) {
                     uint32_t f[4];
-                    ldsm4_t(f, values + swizzled<K::kChunks>(v_row, c + v_piece));
+                    ldsm4_t(f, pieces_on<K::kChunks>(values, c));
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
                         // a transposed pair of bytes holds elements 2g, 2g+1 of two tokens: row g of the product
@@ -718,8 +758,6 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                 }
             }
 
-            // the item's last tile, or this warp's
-            const bool ends = at.t + 1 == at.nt, stops = i + 1 == my_tiles;
             if (ends || stops) {
                 const bool whole = ends && ta == 0;
                 const Heads<K::kHeads> hd(a, at.item);
@@ -791,7 +829,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                     p.tb = at.t + 1;
                 }
             }
-            at.next(a, items);
+            at = following;
             stage = stage + 1 == S ? 0 : stage + 1;
         }
         cp_async_wait<0>();
@@ -886,8 +924,8 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
     for (int slot = 0; slot < 2; ++slot) {
         if (!is_open[slot]) continue;
         const int64_t tile = open[slot].start;
-        first[slot] = static_cast<int32_t>(((tile + 1) * workers - 1) / total / W);
-        last[slot] = static_cast<int32_t>(((tile + open[slot].nt) * workers - 1) / total / W);
+        first[slot] = static_cast<int32_t>(((tile + 1) * workers - 1) / total) / W;
+        last[slot] = static_cast<int32_t>(((tile + open[slot].nt) * workers - 1) / total) / W;
         const int32_t n = last[slot] - first[slot] + 1;
         size[slot] = n <= kJoin ? n : max(12, (n + kJoin - 1) / kJoin);
     }
@@ -909,16 +947,21 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
         const int32_t at = (static_cast<int32_t>(blockIdx.x) - first[slot]) / size[slot];
         const int32_t lo = first[slot] + at * size[slot], n = min(size[slot], last[slot] - lo + 1);
         const int32_t groups = (last[slot] - first[slot]) / size[slot] + 1;
-        const float* parts = a.cta_part + lo * kCta;
-        float* group = a.cta_part + lo * kCta + 2 * K::kPart;
-        join_parts<K>(a, sh, parts, kCta, parts + (lo == first[slot] ? K::kPart : 0), n, p.r, p.item,
-                      groups == 1 ? nullptr : group, DP);
+        // a group's result goes to slot 2 of its first CTA; a group of one, an item's last CTA (where the next item may
+        // have its first group), is its own result
+        if (groups == 1 || n > 1) {
+            const float* parts = a.cta_part + lo * kCta;
+            join_parts<K>(a, sh, parts, kCta, parts + (lo == first[slot] ? K::kPart : 0), parts + (n - 1) * kCta, n, p.r,
+                          p.item, groups == 1 ? nullptr : a.cta_part + lo * kCta + 2 * K::kPart, DP);
+        }
         if (groups == 1) continue;
         if (tid == 0) sh.won[slot] = arrive_last(a.tickets + gridDim.x + first[slot], groups);
         __syncthreads();
         if (!sh.won[slot]) continue;
         const float* heads = a.cta_part + first[slot] * kCta + 2 * K::kPart;
-        join_parts<K>(a, sh, heads, kCta * size[slot], heads, groups, p.r, p.item, nullptr, DP);
+        const int32_t in_last = (last[slot] - first[slot]) % size[slot] + 1;
+        const float* end = a.cta_part + (last[slot] - in_last + 1) * kCta + (in_last == 1 ? 0 : 2 * K::kPart);
+        join_parts<K>(a, sh, heads, kCta * size[slot], heads, end, groups, p.r, p.item, nullptr, DP);
     }
 }
 
@@ -940,9 +983,9 @@ Kernel kernel_of() {
 template <int MODE, int NT>
 Kernel pick_dim(int head_dim) {
     constexpr bool fp8 = MODE == MF_DT_F8E4M3 || MODE == MF_DT_F8E5M2;
-    if (head_dim <= 64) return kernel_of<MODE, 64, NT, 8, fp8 ? 8 : 6>();
-    if (head_dim <= 128) return kernel_of<MODE, 128, NT, 8, fp8 ? 6 : 3>();
-    return kernel_of<MODE, 256, NT, fp8 ? 8 : 4, 3>();
+    if (head_dim <= 64) return kernel_of<MODE, 64, NT, 12, fp8 ? 6 : 4>();
+    if (head_dim <= 128) return kernel_of<MODE, 128, NT, 12, fp8 ? 4 : 2>();
+    return kernel_of<MODE, 256, NT, fp8 ? 8 : 6, fp8 ? 3 : 2>();
 }
 template <int MODE>
 Kernel pick_heads(int group, int head_dim) {
