@@ -40,7 +40,7 @@
 namespace mf {
 namespace {
 
-constexpr int kTile = 16;          // tokens of a tile
+constexpr int kBlock = 16;         // tokens of one product; a tile is one or two blocks
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kLn2 = 0.693147180559945309f;
 
@@ -55,13 +55,14 @@ struct AttnArgs {
     const float* slopes;
     const float* k_scale;
     const float* v_scale;
-    float* warp_part;     // [workers][NT * 8 * (DP + 2)]: parts that end inside a warp's run
-    float* cta_part;      // [CTAs][3][NT * 8 * (DP + 2)]: parts that leave the CTA, and joined groups of them
+    float* team_part;     // [teams][heads * (DP + 2)]: parts that end inside a team's run
+    float* cta_part;      // [CTAs][3][heads * (DP + 2)]: parts that leave the CTA, and joined groups of them
     int32_t* tickets;     // [2][CTAs], zero between runs
     int32_t* status;
     int64_t q_req, q_head, out_req, out_head;
-    int64_t page_stride, token_stride, head_stride, table_stride;
-    int64_t n_pages;
+    int64_t head_bytes, table_stride;
+    int32_t page_bytes, row_bytes;
+    uint32_t n_pages;
     int32_t n_requests, q_heads, kv_heads, group, blocks;  // blocks of query heads per key-value head
     int32_t head_dim, page, max_pages, window, q_f16;
     float scale, softcap;
@@ -128,6 +129,12 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+// Barrier of a team's warps.
+template <int TM>
+__device__ __forceinline__ void team_sync(int team) {
+    if constexpr (TM == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(32 * TM) : "memory");
+}
 // Two FP8 codes -> f16x2, exact.
 template <int DT>
 __device__ __forceinline__ uint32_t fp8x2_to_f16x2(uint32_t two) {
@@ -146,8 +153,8 @@ __device__ __forceinline__ float tanh_fast(float x) {
     return __fmaf_rn(-2.0f, r, 1.0f);
 }
 
-// A request's tokens: [first, len) are seen, from the tile that starts at `base`
-// (a multiple of the tile, so that a tile never crosses a page of whole tiles).
+// A request's tokens: [first, len) are seen, in tiles from `base` on (a multiple
+// of the block, so that a block never crosses a page of whole blocks).
 struct Span {
     int32_t len, first, base;
 };
@@ -157,14 +164,16 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, int32_t r) {
     s.len = max(__ldg(a.lens + r), 0);
     if (s.len > reach) s.len = static_cast<int32_t>(reach);
     s.first = a.window > 0 && s.len > a.window ? s.len - a.window : 0;
-    s.base = s.first & ~(kTile - 1);
+    s.base = s.first & ~(kBlock - 1);
     return s;
 }
+template <int T>
 __device__ __forceinline__ int32_t tiles_of(const Span& s) {
-    return static_cast<int32_t>((static_cast<uint32_t>(s.len - s.base) + (kTile - 1)) / kTile);
+    return static_cast<int32_t>((static_cast<uint32_t>(s.len - s.base) + (T - 1)) / T);
 }
 
 // A place in the row of all tiles: request, item of the request, tile of the item.
+template <int T>
 struct Place {
     int32_t r, item, t, nt;   // nt: tiles of the request's items
     Span span;
@@ -176,7 +185,7 @@ struct Place {
         nt = 0;
         while (++r < a.n_requests) {
             span = span_of(a, r);
-            nt = tiles_of(span);
+            nt = tiles_of<T>(span);
             if (nt > 0) return;
         }
     }
@@ -201,35 +210,40 @@ constexpr int kJoin = 16;  // most parts that one step of a join between CTAs ta
 // 2^8, which float32 sums and both terms of a weight hold as well, and what is summed is not rescaled.
 constexpr float kLazy = 8.0f;
 
-// MODE: dtype of the cache; DP: head_dim padded to 64, 128 or 256; NT: blocks
-// of 8 query heads a warp holds; W: warps; S: stages of a warp's ring.
-template <int MODE, int DP, int NT, int W, int S>
+// MODE: dtype of the cache; DP: head_dim padded to 64, 128 or 256; TM: warps of a team; W: warps; T: tokens of a
+// tile; S: stages of a team's ring.  A team works on one item at a time, each of its warps for 8 query heads.
+template <int MODE, int DP, int TM, int W, int T, int S>
 struct Attn {
     static constexpr bool kFp8 = MODE == MF_DT_F8E4M3 || MODE == MF_DT_F8E5M2;
     static constexpr bool kBf16 = MODE == MF_DT_BF16;
     static constexpr int kBytes = kFp8 ? 1 : 2;
     static constexpr int kRow = DP * kBytes;          // bytes of a token's row
     static constexpr int kChunks = kRow / 16;         // 16-byte pieces of a row
-    static constexpr int kStage = 2 * kTile * kRow;   // keys, then values
+    static constexpr int kStage = 2 * T * kRow;       // keys, then values
+    static constexpr int kBlocks = T / kBlock;
+    static constexpr uint32_t kAll = T == 32 ? 0xffffffffu : 0xffffu;  // every token of a tile
     static constexpr int kSteps = DP / 16;            // products of 16 along head_dim
-    static constexpr int kHeads = 8 * NT;
+    static constexpr int kTeams = W / TM;
+    static constexpr int kHeads = 8 * TM;             // query heads of an item, at most
     static constexpr int kFour = DP / 4;
     static constexpr int kLd = DP + 4;                // floats of a staged head's row (spread over the banks)
     static constexpr int kPart = kHeads * (DP + 2);   // floats of a part in the workspace: out, then m, l
     static constexpr int kThreads = 32 * W;
-    static constexpr int kRing = W * S * kStage;
-    static constexpr int kStaged = W * kHeads * kLd * 4;
+    static constexpr int kRing = kTeams * S * kStage;
+    static constexpr int kStaged = kTeams * kHeads * kLd * 4;
     static constexpr int kBuffer = kRing > kStaged ? kRing : kStaged;
-    static_assert(2 * W <= 32, "a lane for each part of a CTA");
+    static_assert(2 * kTeams <= 32, "a lane for each part of a CTA");
+    static_assert(TM == 1 || kTeams < 16, "a barrier for each team");
+    static_assert(W >= 2 && (T == kBlock || T == 2 * kBlock), "");
 
     struct Shared {
         int64_t prefix[kThreads + 1];   // tiles of the requests in front of each thread's
         int64_t warp_sum[W];
-        Part part[2 * W];               // first and last part of each warp
-        float m[2 * W][kHeads], l[2 * W][kHeads];
+        Part part[2 * kTeams];          // first and last part of each team
+        float m[2 * kTeams][kHeads], l[2 * kTeams][kHeads];
         float weight[kJoin][kHeads], top[kHeads], sum[kHeads];
-        int32_t mask[W][S];             // tokens of each stage that are there
-        int32_t lead[2 * W + 1];        // first part of each joined item, then 2 * W
+        uint32_t mask[kTeams][S];       // tokens of each stage that are there
+        int32_t lead[2 * kTeams + 1];   // first part of each joined item, then 2 * kTeams
         int32_t items;                  // joined items
         int32_t won[2];                 // whether this CTA joins the item of its slot
     };
@@ -361,12 +375,13 @@ __device__ __forceinline__ void join_parts(const AttnArgs& a, typename K::Shared
     __syncthreads();
 }
 
-template <int MODE, int DP, int NT, int W, int S>
+template <int MODE, int DP, int TM, int W, int T, int S>
 __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a) {
-    using K = Attn<MODE, DP, NT, W, S>;
+    using K = Attn<MODE, DP, TM, W, T, S>;
     extern __shared__ __align__(128) unsigned char smem[];
     auto& sh = *reinterpret_cast<typename K::Shared*>(smem + K::kBuffer);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int team = warp / TM, member = warp % TM;
     const int g = lane >> 2, j = lane & 3;  // row and column pair of a product's fragment
     const int32_t items = a.kv_heads * a.blocks;
 
@@ -377,7 +392,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
     for (int32_t i = 0; i < per; ++i) {
         const int32_t r = tid * per + i;
         if (r >= a.n_requests) break;
-        const int32_t nt = tiles_of(span_of(a, r));
+        const int32_t nt = tiles_of<T>(span_of(a, r));
         sum += static_cast<int64_t>(nt) * items;
         empty |= nt == 0 && r % gridDim.x == blockIdx.x;
     }
@@ -388,11 +403,11 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
         if (lane >= d) inc += x;
     }
     if (lane == 31) sh.warp_sum[warp] = inc;
-    if (lane < 2) sh.part[2 * warp + lane].start = -1;
+    if (tid < 2 * K::kTeams) sh.part[tid].start = -1;
     if (__syncthreads_or(empty)) {
         // requests that see nothing
         for (int32_t r = blockIdx.x; r < a.n_requests; r += gridDim.x) {
-            if (tiles_of(span_of(a, r)) > 0) continue;
+            if (tiles_of<T>(span_of(a, r)) > 0) continue;
             for (int i = tid; i < a.q_heads * (a.head_dim / 4); i += K::kThreads)
                 store_out4(a, r, i / (a.head_dim / 4), i % (a.head_dim / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f));
             for (int i = tid; i < a.q_heads; i += K::kThreads) store_lse(a, r, i, 0.0f, 0.0f);
@@ -408,18 +423,18 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
     if (tid == 0) sh.prefix[K::kThreads] = total;
     __syncthreads();
     if (total == 0) return;
-    const int64_t want = (total + W - 1) / W;
+    const int64_t want = (total + K::kTeams - 1) / K::kTeams;
     int32_t ctas = static_cast<int32_t>(want < gridDim.x ? want : gridDim.x);
     if (a.n_requests == 1 && items <= gridDim.x) ctas = max(ctas / items, 1) * items;  // no CTA has parts of two items
     if (blockIdx.x >= ctas) return;
-    const int32_t workers = ctas * W;
-    const int32_t id = blockIdx.x * W + warp;
+    const int32_t workers = ctas * K::kTeams;
+    const int32_t id = blockIdx.x * K::kTeams + team;
     const int64_t x0 = mul_div(total, id, workers), x1 = mul_div(total, id + 1, workers);
     const int32_t my_tiles = static_cast<int32_t>(x1 - x0);
 
-    uint32_t qf[NT][K::kSteps][2];
-    float o[NT][K::kSteps][4];
-    float m[NT][2], l[NT][2], scale[NT][2], slope[NT][2];
+    uint32_t qf[K::kSteps][2];
+    float o[K::kSteps][4];
+    float m[2], l[2];
     if (my_tiles > 0) {
         // the place of tile x0: the warp, then the thread whose requests hold it, then the request among them
         int64_t before = 0;
@@ -429,11 +444,11 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
             if (sh.prefix[32 * w] <= x0) lo = 32 * w;
         lo += 31 - __clz(__ballot_sync(0xffffffffu, sh.prefix[lo + lane] <= x0));
         before = sh.prefix[lo];
-        Place at{};
+        Place<T> at{};
         at.r = lo;
         if (per > 1) {
             for (int32_t r0 = lo * per;; r0 += 32) {
-                const int32_t nt = r0 + lane < a.n_requests ? tiles_of(span_of(a, r0 + lane)) : 0;
+                const int32_t nt = r0 + lane < a.n_requests ? tiles_of<T>(span_of(a, r0 + lane)) : 0;
                 const int64_t mine = static_cast<int64_t>(nt) * items;
                 int64_t upto = mine;
 #pragma unroll
@@ -452,79 +467,99 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
             }
         }
         at.span = span_of(a, at.r);
-        at.nt = tiles_of(at.span);
+        at.nt = tiles_of<T>(at.span);
         const int64_t in_request = x0 - before;
         at.item = static_cast<int32_t>(mul_div(in_request, 1, at.nt));
         at.t = static_cast<int32_t>(in_request - static_cast<int64_t>(at.item) * at.nt);
 
-        const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * (S * K::kStage);
-        Place load = at;
+        unsigned char* my_ring = smem + team * (S * K::kStage);
+        const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(my_ring));
+        Place<T> load = at;
         int32_t to_load = my_tiles;
-        const bool whole_tiles = a.page % kTile == 0;  // a tile lies in one page
+        const bool whole = a.page % kBlock == 0;  // a block lies in one page
         constexpr int kRows = 32 / K::kChunks > 0 ? 32 / K::kChunks : 1;  // rows that one instruction copies
-        constexpr int kCopies = kTile * K::kChunks / 32;
-        const int piece_row = lane / K::kChunks, piece = lane % K::kChunks;
-        const int64_t row_bytes = a.token_stride * K::kBytes, page_bytes = a.page_stride * K::kBytes;
-        const int64_t lane_bytes = piece_row * row_bytes + piece * 16;
+        constexpr int kCopies = kBlock * K::kChunks / 32 / TM;            // of a block, by one warp
+        static_assert(kCopies > 0, "");
+        const int piece_row = lane / K::kChunks + member * (kCopies * kRows), piece = lane % K::kChunks;
+        const int64_t lane_bytes = static_cast<int64_t>(piece_row) * a.row_bytes + piece * 16;
         const bool piece_in = piece * (16 / K::kBytes) < a.head_dim;
         const int64_t kv_gap = static_cast<const char*>(a.v) - static_cast<const char*>(a.k);
-        const int32_t lane_row = whole_tiles ? 0 : lane & 15;
-        // of the tile at `load`: the page (or that of this lane's row), its place in the table's row and the tile's in it
+        // of the blocks of the tile at `load` (or, blocks not being whole, of this lane's row): their pages, the pages'
+        // places in the table's row and the blocks' in the pages
         const int32_t* table_row = nullptr;
         const char* head_at = nullptr;
-        int32_t page_no = -1, page_idx = 0, page_off = 0;
+        int32_t page_no[K::kBlocks], page_idx[K::kBlocks], page_off[K::kBlocks];
         auto look_up = [&](bool new_item) {
             if (to_load == 0) return;
-            const int32_t tok = load.span.base + load.t * kTile + lane_row;
             if (new_item) {
                 table_row = a.table + load.r * a.table_stride;
-                head_at = static_cast<const char*>(a.k) + load.item / a.blocks * a.head_stride * K::kBytes + lane_bytes;
+                head_at = static_cast<const char*>(a.k) + load.item / a.blocks * a.head_bytes + lane_bytes;
             }
-            if (new_item || !whole_tiles) {
-                page_idx = static_cast<int32_t>(static_cast<uint32_t>(tok) / static_cast<uint32_t>(a.page));
-                page_off = tok - page_idx * a.page;
-            } else if ((page_off += kTile) >= a.page) {
-                page_off = 0;
-                ++page_idx;
+#pragma unroll
+            for (int b = 0; b < K::kBlocks; ++b) {
+                const int32_t tok = load.span.base + load.t * T + (whole ? b * kBlock : lane & (T - 1));
+                if (new_item || !whole) {
+                    page_idx[b] = static_cast<int32_t>(static_cast<uint32_t>(tok) / static_cast<uint32_t>(a.page));
+                    page_off[b] = tok - page_idx[b] * a.page;
+                } else {
+                    page_off[b] += T;
+#pragma unroll
+                    for (int x = 0; x < K::kBlocks; ++x)
+                        if (page_off[b] >= a.page) {
+                            page_off[b] -= a.page;
+                            ++page_idx[b];
+                        }
+                }
+                if (tok < load.span.len) page_no[b] = __ldg(table_row + page_idx[b]);
             }
-            if (tok < load.span.len) page_no = __ldg(table_row + page_idx);
         };
         uint32_t partial = 0;  // stages that lack some of their tokens: those have a mask
         auto issue = [&](int stage) {
             if (to_load > 0) {
-                const int32_t tok0 = load.span.base + load.t * kTile;
+                const int32_t tok0 = load.span.base + load.t * T;
                 const uint32_t dst = ring + stage * K::kStage;
-                const bool page_ok = page_no >= 0 && page_no < a.n_pages;
-                if (whole_tiles && page_ok && tok0 >= load.span.first && tok0 + kTile <= load.span.len) {
-                    partial &= ~(1u << stage);
-                    const char* kp = head_at + (page_no * page_bytes + page_off * row_bytes);
+                bool ok[K::kBlocks], all = whole && tok0 >= load.span.first && tok0 + T <= load.span.len;
+                int64_t at_block[K::kBlocks];
 #pragma unroll
-                    for (int i = 0; i < kCopies; ++i, kp += kRows * row_bytes) {
-                        const uint32_t to = dst + swizzled<K::kChunks>(i * kRows + piece_row, piece);
-                        if (piece_in) {
-                            cp_async16(to, kp, 16u);
-                            cp_async16(to + kTile * K::kRow, kp + kv_gap, 16u);
+                for (int b = 0; b < K::kBlocks; ++b) {
+                    ok[b] = static_cast<uint32_t>(page_no[b]) < a.n_pages;
+                    all &= ok[b];
+                    at_block[b] = static_cast<int64_t>(page_no[b]) * a.page_bytes + page_off[b] * a.row_bytes;
+                }
+                if (all) {
+                    partial &= ~(1u << stage);
+#pragma unroll
+                    for (int b = 0; b < K::kBlocks; ++b) {
+                        const char* kp = head_at + at_block[b];
+#pragma unroll
+                        for (int i = 0; i < kCopies; ++i, kp += kRows * a.row_bytes) {
+                            const uint32_t to = dst + b * kBlock * K::kRow + swizzled<K::kChunks>(i * kRows + piece_row, piece);
+                            if (piece_in) {
+                                cp_async16(to, kp, 16u);
+                                cp_async16(to + T * K::kRow, kp + kv_gap, 16u);
+                            }
                         }
                     }
                 } else {
-                    const int32_t tok = tok0 + (lane & 15);
+                    // the row of this lane: whether it is there, and where
+                    const int mine = whole ? (lane & (T - 1)) / kBlock : 0;
+                    const int32_t tok = tok0 + (lane & (T - 1));
                     const bool seen = tok >= load.span.first && tok < load.span.len;
-                    if (seen && !page_ok) atomicExch(a.status, MF_DEVICE_BAD_PAGE);
-                    const uint32_t mask = __ballot_sync(0xffffffffu, seen && page_ok) & 0xffffu;
-                    partial = (partial & ~(1u << stage)) | (mask != 0xffffu ? 1u << stage : 0u);
-                    if (lane == 0) sh.mask[warp][stage] = static_cast<int32_t>(mask);
-                    const int64_t at_row = page_no * page_bytes + page_off * row_bytes;
+                    const bool mine_ok = mine == 0 ? ok[0] : ok[K::kBlocks - 1];
+                    if (seen && !mine_ok) atomicExch(a.status, MF_DEVICE_BAD_PAGE);
+                    const uint32_t mask = __ballot_sync(0xffffffffu, seen && mine_ok) & K::kAll;
+                    partial = (partial & ~(1u << stage)) | (mask != K::kAll ? 1u << stage : 0u);
+                    if (lane == 0) sh.mask[team][stage] = mask;
+                    const int64_t row = (mine == 0 ? at_block[0] : at_block[K::kBlocks - 1]) + (whole ? (lane & (kBlock - 1)) * a.row_bytes : 0);
 #pragma unroll 1
-                    for (int i = 0; i < kCopies; ++i) {
-                        const int rw = i * kRows + piece_row;
-                        // one page: rows follow the tile's first; else each row's place is with the lane of its number
-                        const int64_t row_at = whole_tiles ? at_row + i * kRows * row_bytes
-                                                           : __shfl_sync(0xffffffffu, at_row, rw) - piece_row * row_bytes;
+                    for (int i = 0; i < K::kBlocks * kCopies; ++i) {
+                        const int rw = i / kCopies * kBlock + i % kCopies * kRows + piece_row;
+                        const int64_t row_at = __shfl_sync(0xffffffffu, row, rw) - static_cast<int64_t>(piece_row) * a.row_bytes;
                         const bool get = piece_in && ((mask >> rw) & 1u);
                         const char* kp = get ? head_at + row_at : static_cast<const char*>(a.k);
                         const uint32_t to = dst + swizzled<K::kChunks>(rw, piece);
                         cp_async16(to, kp, get ? 16u : 0u);
-                        cp_async16(to + kTile * K::kRow, kp + kv_gap, get ? 16u : 0u);
+                        cp_async16(to + T * K::kRow, kp + kv_gap, get ? 16u : 0u);
                     }
                 }
                 load.next(a, items);
@@ -535,27 +570,24 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
         };
         look_up(true);
         if (a.head_dim < DP) {  // what is past the head is never copied: zeros
-            for (int i = lane; i < S * K::kStage / 16; i += 32)
-                reinterpret_cast<uint4*>(smem + warp * (S * K::kStage))[i] = make_uint4(0, 0, 0, 0);
-            __syncwarp();
+            for (int i = member * 32 + lane; i < S * K::kStage / 16; i += 32 * TM)
+                reinterpret_cast<uint4*>(my_ring)[i] = make_uint4(0, 0, 0, 0);
+            team_sync<TM>(team);
         }
 #pragma unroll 1
         for (int s = 0; s < S - 1; ++s) issue(s);
 
         // the queries of the item at `p`, as they are
-        auto load_queries = [&](const Place& p) {
+        auto load_queries = [&](const Place<T>& p) {
             const Heads<K::kHeads> hd(a, p.item);
+            const int h = member * 8 + g;
+            const char* q = static_cast<const char*>(a.q) + 2 * (p.r * a.q_req + (hd.head0 + h) * a.q_head);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const int h = n * 8 + g;
-                const char* q = static_cast<const char*>(a.q) + 2 * (p.r * a.q_req + (hd.head0 + h) * a.q_head);
-#pragma unroll
-                for (int c = 0; c < K::kSteps; ++c) {
-                    const int d0 = K::kFp8 ? c * 16 + 4 * j : c * 16 + 2 * j;
-                    const int d1 = K::kFp8 ? d0 + 2 : d0 + 8;
-                    qf[n][c][0] = h < hd.count && d0 < a.head_dim ? __ldg(reinterpret_cast<const uint32_t*>(q + 2 * d0)) : 0u;
-                    qf[n][c][1] = h < hd.count && d1 < a.head_dim ? __ldg(reinterpret_cast<const uint32_t*>(q + 2 * d1)) : 0u;
-                }
+            for (int c = 0; c < K::kSteps; ++c) {
+                const int d0 = K::kFp8 ? c * 16 + 4 * j : c * 16 + 2 * j;
+                const int d1 = K::kFp8 ? d0 + 2 : d0 + 8;
+                qf[c][0] = h < hd.count && d0 < a.head_dim ? __ldg(reinterpret_cast<const uint32_t*>(q + 2 * d0)) : 0u;
+                qf[c][1] = h < hd.count && d1 < a.head_dim ? __ldg(reinterpret_cast<const uint32_t*>(q + 2 * d1)) : 0u;
             }
         };
         load_queries(at);
@@ -564,263 +596,258 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
         const int k_row = (lane & 7) + ((lane >> 3) & 1) * 8, k_piece = lane >> 4;
         const int v_row = K::kFp8 ? k_row : (lane & 7) + (lane >> 4) * 8, v_piece = K::kFp8 ? k_piece : (lane >> 3) & 1;
         const uint32_t k_at = swizzled<K::kChunks>(k_row, k_piece);
-        const uint32_t v_at = swizzled<K::kChunks>(v_row, v_piece) + kTile * K::kRow;
+        const uint32_t v_at = swizzled<K::kChunks>(v_row, v_piece) + T * K::kRow;
         const bool rules = a.softcap > 0.0f || a.slopes;
+        float scale[2] = {0.0f, 0.0f}, slope[2] = {0.0f, 0.0f};
         int32_t ta = at.t;
         int stage = 0;
 #pragma unroll 1
         for (int32_t i = 0; i < my_tiles; ++i) {
             cp_async_wait<S - 2>();
-            __syncwarp();
+            team_sync<TM>(team);
             issue(stage == 0 ? S - 1 : stage - 1);
             if (i == 0 || at.t == 0) {
                 // a new item; its queries were loaded while the one before it ended
                 ta = at.t;
                 const Heads<K::kHeads> hd(a, at.item);
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    float back = 1.0f;
-                    if constexpr (K::kFp8) {
-                        // f16 queries, scaled by a power of two to a largest magnitude in [1, 2)
-                        float top = 0.0f;
-#pragma unroll
-                        for (int c = 0; c < K::kSteps; ++c)
-#pragma unroll
-                            for (int x = 0; x < 2; ++x) {
-                                float f0, f1;
-                                if (a.q_f16) unpack2<false>(qf[n][c][x], f0, f1);
-                                else unpack2<true>(qf[n][c][x], f0, f1);
-                                top = fmaxf(top, fmaxf(fabsf(f0), fabsf(f1)));
-                            }
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                        const uint32_t field = __float_as_uint(top) >> 23;  // biased exponent
-                        const bool scales = field >= 1 && field <= 254;
-                        const uint32_t e = min(field, 253u);
-                        const float fit = scales ? __uint_as_float((254u - e) << 23) : 1.0f;
-                        back = scales ? __uint_as_float(e << 23) : 1.0f;
-#pragma unroll
-                        for (int c = 0; c < K::kSteps; ++c)
-#pragma unroll
-                            for (int x = 0; x < 2; ++x) {
-                                float f0, f1;
-                                if (a.q_f16) unpack2<false>(qf[n][c][x], f0, f1);
-                                else unpack2<true>(qf[n][c][x], f0, f1);
-                                qf[n][c][x] = pack2<false>(f0 * fit, f1 * fit);
-                            }
-                    }
-                    const float ks = a.k_scale ? __ldg(a.k_scale + hd.kv) : 1.0f;
-                    // head 2j + x of this lane's columns: its scale is with the lanes of row 2j + x
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const float b = __shfl_sync(0xffffffffu, back, (2 * j + x) * 4);
-                        scale[n][x] = a.scale * ks * b;
-                        const int hx = n * 8 + 2 * j + x;
-                        slope[n][x] = a.slopes && hx < hd.count ? __ldg(a.slopes + hd.head0 + hx) * kLog2e : 0.0f;
-                        scale[n][x] = a.softcap > 0.0f ? __fdiv_rn(scale[n][x], a.softcap) : scale[n][x] * kLog2e;
-                        m[n][x] = -INFINITY;
-                        l[n][x] = 0.0f;
-                    }
+                float back = 1.0f;
+                if constexpr (K::kFp8) {
+                    // f16 queries, scaled by a power of two to a largest magnitude in [1, 2)
+                    float top = 0.0f;
 #pragma unroll
                     for (int c = 0; c < K::kSteps; ++c)
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) o[n][c][x] = 0.0f;
+                        for (int x = 0; x < 2; ++x) {
+                            float f0, f1;
+                            if (a.q_f16) unpack2<false>(qf[c][x], f0, f1);
+                            else unpack2<true>(qf[c][x], f0, f1);
+                            top = fmaxf(top, fmaxf(fabsf(f0), fabsf(f1)));
+                        }
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    const uint32_t field = __float_as_uint(top) >> 23;  // biased exponent
+                    const bool scales = field >= 1 && field <= 254;
+                    const uint32_t e = min(field, 253u);
+                    const float fit = scales ? __uint_as_float((254u - e) << 23) : 1.0f;
+                    back = scales ? __uint_as_float(e << 23) : 1.0f;
+#pragma unroll
+                    for (int c = 0; c < K::kSteps; ++c)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            float f0, f1;
+                            if (a.q_f16) unpack2<false>(qf[c][x], f0, f1);
+                            else unpack2<true>(qf[c][x], f0, f1);
+                            qf[c][x] = pack2<false>(f0 * fit, f1 * fit);
+                        }
                 }
+                const float ks = a.k_scale ? __ldg(a.k_scale + hd.kv) : 1.0f;
+                // head 2j + x of this lane's columns: its scale is with the lanes of row 2j + x
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const float b = __shfl_sync(0xffffffffu, back, (2 * j + x) * 4);
+                    const int hx = member * 8 + 2 * j + x;
+                    scale[x] = a.scale * ks * b;
+                    scale[x] = a.softcap > 0.0f ? __fdiv_rn(scale[x], a.softcap) : scale[x] * kLog2e;
+                    slope[x] = a.slopes && hx < hd.count ? __ldg(a.slopes + hd.head0 + hx) * kLog2e : 0.0f;
+                    m[x] = -INFINITY;
+                    l[x] = 0.0f;
+                }
+#pragma unroll
+                for (int c = 0; c < K::kSteps; ++c)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) o[c][x] = 0.0f;
             }
 
             // S^T = K Q^T, two chains of sums
             const uint32_t keys = ring + stage * K::kStage + k_at, values = ring + stage * K::kStage + v_at;
-            const uint32_t mask = (partial >> stage) & 1u ? static_cast<uint32_t>(sh.mask[warp][stage]) : 0xffffu;
-            const bool ends = at.t + 1 == at.nt, stops = i + 1 == my_tiles;  // the item's last tile, or this warp's
-            float s[NT][2][4];
+            const uint32_t mask = (partial >> stage) & 1u ? sh.mask[team][stage] : K::kAll;
+            const bool ends = at.t + 1 == at.nt, stops = i + 1 == my_tiles;  // the item's last tile, or this team's
+            float s[K::kBlocks][2][4];
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+            for (int b = 0; b < K::kBlocks; ++b) {
 #pragma unroll
-                for (int x = 0; x < 4; ++x) s[n][0][x] = s[n][1][x] = 0.0f;
-            if constexpr (!K::kFp8) {
+                for (int x = 0; x < 4; ++x) s[b][0][x] = s[b][1][x] = 0.0f;
+                const uint32_t rows = keys + b * kBlock * K::kRow;
+                if constexpr (!K::kFp8) {
 #pragma unroll
-                for (int c = 0; c < K::kSteps; ++c) {
-                    uint32_t f[4];
-                    ldsm4(f, pieces_on<K::kChunks>(keys, 2 * c));
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) mma16816<K::kBf16>(s[n][c & 1], f, qf[n][c][0], qf[n][c][1]);
-                }
-            } else {
-#pragma unroll
-                for (int c = 0; c < K::kSteps; c += 2) {
-                    uint32_t f[4];
-                    ldsm4(f, pieces_on<K::kChunks>(keys, c));
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        // four codes of a row: elements 4j, 4j+1 take the place of the product's 2j, 2j+1,
-                        // elements 4j+2, 4j+3 that of 2j+8, 2j+9 (the queries are laid out alike)
-                        const uint32_t f16[4] = {
-                            fp8x2_to_f16x2<MODE>(f[2 * x]), fp8x2_to_f16x2<MODE>(f[2 * x + 1]),
-                            fp8x2_to_f16x2<MODE>(f[2 * x] >> 16), fp8x2_to_f16x2<MODE>(f[2 * x + 1] >> 16)};
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) mma16816<false>(s[n][x], f16, qf[n][c + x][0], qf[n][c + x][1]);
+                    for (int c = 0; c < K::kSteps; ++c) {
+                        uint32_t f[4];
+                        ldsm4(f, pieces_on<K::kChunks>(rows, 2 * c));
+                        mma16816<K::kBf16>(s[b][c & 1], f, qf[c][0], qf[c][1]);
                     }
-                }
-            }
-
-            Place following = at;
-            following.next(a, items);
-            if (ends && !stops) load_queries(following);
-
-            // scores of tokens g and g + 8, heads 2j and 2j + 1, times log2(e)
-            uint32_t ph[NT][2], pl[NT][2];
+                } else {
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                float p[4];
+                    for (int c = 0; c < K::kSteps; c += 2) {
+                        uint32_t f[4];
+                        ldsm4(f, pieces_on<K::kChunks>(rows, c));
 #pragma unroll
-                for (int x = 0; x < 4; ++x) p[x] = (s[n][0][x] + s[n][1][x]) * scale[n][x & 1];
-                if (rules) {
-                    // distance to the newest token, <= 0
-                    const float away = static_cast<float>(at.span.base + at.t * kTile + g - (at.span.len - 1));
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        if (a.softcap > 0.0f) p[x] = a.softcap * kLog2e * tanh_fast(p[x]);
-                        p[x] = __fmaf_rn(slope[n][x & 1], away + (x & 2 ? 8.0f : 0.0f), p[x]);
-                    }
-                }
-                if (mask != 0xffffu) {
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) p[x] = (mask >> (x & 2 ? g + 8 : g)) & 1u ? p[x] : -INFINITY;
-                }
-                const float t0 = fmaxf(p[0], p[2]), t1 = fmaxf(p[1], p[3]);
-                if (__any_sync(0xffffffffu, t0 > m[n][0] + kLazy || t1 > m[n][1] + kLazy)) {
-                    float top[2] = {t0, t1};
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 4));
-                        top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 8));
-                        top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 16));
-                        top[x] = fmaxf(top[x], m[n][x]);
-                        const float r = rescale(m[n][x], top[x]);
-                        m[n][x] = top[x];
-                        l[n][x] *= r;
-#pragma unroll
-                        for (int c = 0; c < K::kSteps; ++c) {
-                            o[n][c][x] *= r;
-                            o[n][c][x + 2] *= r;
+                        for (int x = 0; x < 2; ++x) {
+                            // four codes of a row: elements 4j, 4j+1 take the place of the product's 2j, 2j+1,
+                            // elements 4j+2, 4j+3 that of 2j+8, 2j+9 (the queries are laid out alike)
+                            const uint32_t f16[4] = {
+                                fp8x2_to_f16x2<MODE>(f[2 * x]), fp8x2_to_f16x2<MODE>(f[2 * x + 1]),
+                                fp8x2_to_f16x2<MODE>(f[2 * x] >> 16), fp8x2_to_f16x2<MODE>(f[2 * x + 1] >> 16)};
+                            mma16816<false>(s[b][x], f16, qf[c + x][0], qf[c + x][1]);
                         }
                     }
                 }
-                // while nothing is seen, the maximum is -inf and so are the scores: weights of 0
-                const float less[2] = {m[n][0] == -INFINITY ? 0.0f : m[n][0], m[n][1] == -INFINITY ? 0.0f : m[n][1]};
+            }
+            Place<T> following = at;
+            following.next(a, items);
+            if (ends && !stops) load_queries(following);
+
+            // scores of tokens g and g + 8 of each block, heads 2j and 2j + 1, times log2(e)
+            float p[K::kBlocks][4], top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int b = 0; b < K::kBlocks; ++b) {
+#pragma unroll
+                for (int x = 0; x < 4; ++x) p[b][x] = (s[b][0][x] + s[b][1][x]) * scale[x & 1];
+                if (rules) {
+                    // distance to the newest token, <= 0
+                    const float away = static_cast<float>(at.span.base + at.t * T + b * kBlock + g - (at.span.len - 1));
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        if (a.softcap > 0.0f) p[b][x] = a.softcap * kLog2e * tanh_fast(p[b][x]);
+                        p[b][x] = __fmaf_rn(slope[x & 1], away + (x & 2 ? 8.0f : 0.0f), p[b][x]);
+                    }
+                }
+                if (mask != K::kAll) {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        p[b][x] = (mask >> (b * kBlock + (x & 2 ? g + 8 : g))) & 1u ? p[b][x] : -INFINITY;
+                }
+                top[0] = fmaxf(top[0], fmaxf(p[b][0], p[b][2]));
+                top[1] = fmaxf(top[1], fmaxf(p[b][1], p[b][3]));
+            }
+            if (__any_sync(0xffffffffu, top[0] > m[0] + kLazy || top[1] > m[1] + kLazy)) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 4));
+                    top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 8));
+                    top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 16));
+                    top[x] = fmaxf(top[x], m[x]);
+                    const float r = rescale(m[x], top[x]);
+                    m[x] = top[x];
+                    l[x] *= r;
+#pragma unroll
+                    for (int c = 0; c < K::kSteps; ++c) {
+                        o[c][x] *= r;
+                        o[c][x + 2] *= r;
+                    }
+                }
+            }
+            // weights; while nothing is seen, the maximum is -inf and so are the scores: weights of 0
+            const float less[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+            uint32_t ph[K::kBlocks][2], pl[K::kBlocks][2];
+#pragma unroll
+            for (int b = 0; b < K::kBlocks; ++b) {
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
-                    p[x] = exp2_fast(p[x] - less[x & 1]);
-                    l[n][x & 1] += p[x];
+                    p[b][x] = exp2_fast(p[b][x] - less[x & 1]);
+                    l[x & 1] += p[b][x];
                 }
                 // high and low terms, tokens x heads -> heads x tokens
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    const uint32_t high = pack2<K::kBf16>(p[2 * x], p[2 * x + 1]);
+                    const uint32_t high = pack2<K::kBf16>(p[b][2 * x], p[b][2 * x + 1]);
                     float f0, f1;
                     unpack2<K::kBf16>(high, f0, f1);
-                    ph[n][x] = transpose8x8(high);
-                    pl[n][x] = transpose8x8(pack2<K::kBf16>(p[2 * x] - f0, p[2 * x + 1] - f1));
+                    ph[b][x] = transpose8x8(high);
+                    pl[b][x] = transpose8x8(pack2<K::kBf16>(p[b][2 * x] - f0, p[b][2 * x + 1] - f1));
                 }
             }
 
             // O^T += V^T P^T
-            if constexpr (!K::kFp8) {
 #pragma unroll
-                for (int c = 0; c < K::kSteps; ++c) {
-                    uint32_t f[4];
-                    ldsm4_t(f, pieces_on<K::kChunks>(values, 2 * c));
+            for (int b = 0; b < K::kBlocks; ++b) {
+                const uint32_t rows = values + b * kBlock * K::kRow;
+                if constexpr (!K::kFp8) {
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        mma16816<K::kBf16>(o[n][c], f, ph[n][0], ph[n][1]);
-                        mma16816<K::kBf16>(o[n][c], f, pl[n][0], pl[n][1]);
+                    for (int c = 0; c < K::kSteps; ++c) {
+                        uint32_t f[4];
+                        ldsm4_t(f, pieces_on<K::kChunks>(rows, 2 * c));
+                        mma16816<K::kBf16>(o[c], f, ph[b][0], ph[b][1]);
+                        mma16816<K::kBf16>(o[c], f, pl[b][0], pl[b][1]);
                     }
-                }
-            } else {
+                } else {
 #pragma unroll
-                for (int c = 0; c < K::kSteps; c += 2) {
-                    uint32_t f[4];
-                    ldsm4_t(f, pieces_on<K::kChunks>(values, c));
+                    for (int c = 0; c < K::kSteps; c += 2) {
+                        uint32_t f[4];
+                        ldsm4_t(f, pieces_on<K::kChunks>(rows, c));
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        // a transposed pair of bytes holds elements 2g, 2g+1 of two tokens: row g of the product
-                        // is element 2g, row g + 8 element 2g + 1
-                        const uint32_t u = f[2 * x], w = f[2 * x + 1];
-                        const uint32_t f16[4] = {
-                            fp8x2_to_f16x2<MODE>(__byte_perm(u, 0u, 0x4420u)), fp8x2_to_f16x2<MODE>(__byte_perm(u, 0u, 0x4431u)),
-                            fp8x2_to_f16x2<MODE>(__byte_perm(w, 0u, 0x4420u)), fp8x2_to_f16x2<MODE>(__byte_perm(w, 0u, 0x4431u))};
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            mma16816<false>(o[n][c + x], f16, ph[n][0], ph[n][1]);
-                            mma16816<false>(o[n][c + x], f16, pl[n][0], pl[n][1]);
+                        for (int x = 0; x < 2; ++x) {
+                            // a transposed pair of bytes holds elements 2g, 2g+1 of two tokens: row g of the product
+                            // is element 2g, row g + 8 element 2g + 1
+                            const uint32_t u = f[2 * x], w = f[2 * x + 1];
+                            const uint32_t f16[4] = {
+                                fp8x2_to_f16x2<MODE>(__byte_perm(u, 0u, 0x4420u)), fp8x2_to_f16x2<MODE>(__byte_perm(u, 0u, 0x4431u)),
+                                fp8x2_to_f16x2<MODE>(__byte_perm(w, 0u, 0x4420u)), fp8x2_to_f16x2<MODE>(__byte_perm(w, 0u, 0x4431u))};
+                            mma16816<false>(o[c + x], f16, ph[b][0], ph[b][1]);
+                            mma16816<false>(o[c + x], f16, pl[b][0], pl[b][1]);
                         }
                     }
                 }
             }
 
             if (ends || stops) {
-                const bool whole = ends && ta == 0;
+                const bool all_of_it = ends && ta == 0;
                 const Heads<K::kHeads> hd(a, at.item);
-                const float vs = a.v_scale ? __ldg(a.v_scale + hd.kv) : 1.0f;
-                float* part = a.warp_part + static_cast<int64_t>(id) * K::kPart;
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
+                for (int x = 0; x < 2; ++x) {
+                    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 4);
+                    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 8);
+                    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 16);
+                }
+                if (all_of_it) {
+                    const float vs = a.v_scale ? __ldg(a.v_scale + hd.kv) : 1.0f;
+                    float f[2];
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        l[n][x] += __shfl_xor_sync(0xffffffffu, l[n][x], 4);
-                        l[n][x] += __shfl_xor_sync(0xffffffffu, l[n][x], 8);
-                        l[n][x] += __shfl_xor_sync(0xffffffffu, l[n][x], 16);
+                        const int h = member * 8 + 2 * j + x;
+                        f[x] = l[x] == 0.0f ? 0.0f : __fdiv_rn(vs, l[x]);
+                        if (g == 0 && h < hd.count) store_lse(a, at.r, hd.head0 + h, m[x], l[x]);
                     }
-                    if (whole) {
-                        float f[2];
+                    char* out = static_cast<char*>(a.out) + 2 * (at.r * a.out_req + hd.head0 * a.out_head);
 #pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            const int h = n * 8 + 2 * j + x;
-                            f[x] = l[n][x] == 0.0f ? 0.0f : __fdiv_rn(vs, l[n][x]);
-                            if (g == 0 && h < hd.count) store_lse(a, at.r, hd.head0 + h, m[n][x], l[n][x]);
+                    for (int c = 0; c < K::kSteps; ++c) {
+                        if constexpr (!K::kFp8) {
+                            // elements x heads -> heads x elements
+                            const uint32_t u = transpose8x8(pack2<K::kBf16>(o[c][0] * f[0], o[c][1] * f[1]));
+                            const uint32_t w = transpose8x8(pack2<K::kBf16>(o[c][2] * f[0], o[c][3] * f[1]));
+                            const int h = member * 8 + g, d = c * 16 + 2 * j;
+                            char* to = out + 2 * (h * a.out_head + d);
+                            if (h < hd.count && d < a.head_dim) *reinterpret_cast<uint32_t*>(to) = u;
+                            if (h < hd.count && d + 8 < a.head_dim) *reinterpret_cast<uint32_t*>(to + 16) = w;
+                        } else {
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) {
+                                const int h = member * 8 + 2 * j + x, d = c * 16 + 2 * g;
+                                const float u = o[c][x] * f[x], w = o[c][x + 2] * f[x];
+                                const uint32_t two = a.q_f16 ? pack2<false>(u, w) : pack2<true>(u, w);
+                                if (h < hd.count && d < a.head_dim) *reinterpret_cast<uint32_t*>(out + 2 * (h * a.out_head + d)) = two;
+                            }
+                        }
+                    }
+                } else if (!stops) {
+                    // the item began in another team: its end waits in the workspace
+                    float* part = a.team_part + static_cast<int64_t>(id) * K::kPart;
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const int h = member * 8 + 2 * j + x;
+                        if (g == 0) {
+                            sh.m[2 * team][h] = m[x];
+                            sh.l[2 * team][h] = l[x];
                         }
 #pragma unroll
                         for (int c = 0; c < K::kSteps; ++c) {
-                            char* out = static_cast<char*>(a.out);
-                            if constexpr (!K::kFp8) {
-                                // elements x heads -> heads x elements
-                                const uint32_t u = transpose8x8(pack2<K::kBf16>(o[n][c][0] * f[0], o[n][c][1] * f[1]));
-                                const uint32_t w = transpose8x8(pack2<K::kBf16>(o[n][c][2] * f[0], o[n][c][3] * f[1]));
-                                const int h = n * 8 + g, d = c * 16 + 2 * j;
-                                char* at_out = out + 2 * (at.r * a.out_req + (hd.head0 + h) * a.out_head + d);
-                                if (h < hd.count && d < a.head_dim) *reinterpret_cast<uint32_t*>(at_out) = u;
-                                if (h < hd.count && d + 8 < a.head_dim) *reinterpret_cast<uint32_t*>(at_out + 16) = w;
-                            } else {
-#pragma unroll
-                                for (int x = 0; x < 2; ++x) {
-                                    const int h = n * 8 + 2 * j + x, d = c * 16 + 2 * g;
-                                    const float u = o[n][c][x] * f[x], w = o[n][c][x + 2] * f[x];
-                                    const uint32_t two = a.q_f16 ? pack2<false>(u, w) : pack2<true>(u, w);
-                                    if (h < hd.count && d < a.head_dim)
-                                        *reinterpret_cast<uint32_t*>(out + 2 * (at.r * a.out_req + (hd.head0 + h) * a.out_head + d)) = two;
-                                }
-                            }
-                        }
-                    } else if (!stops) {
-                        // the item began in another warp: its end waits in the workspace
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            const int h = n * 8 + 2 * j + x;
-                            if (g == 0) {
-                                sh.m[2 * warp][h] = m[n][x];
-                                sh.l[2 * warp][h] = l[n][x];
-                            }
-#pragma unroll
-                            for (int c = 0; c < K::kSteps; ++c) {
-                                const int d0 = K::kFp8 ? c * 16 + 2 * g : c * 16 + g, d1 = K::kFp8 ? d0 + 1 : d0 + 8;
-                                part[h * DP + d0] = o[n][c][x];
-                                part[h * DP + d1] = o[n][c][x + 2];
-                            }
+                            const int d0 = K::kFp8 ? c * 16 + 2 * g : c * 16 + g, d1 = K::kFp8 ? d0 + 1 : d0 + 8;
+                            part[h * DP + d0] = o[c][x];
+                            part[h * DP + d1] = o[c][x + 2];
                         }
                     }
                 }
-                if (!whole && lane == 0) {
-                    Part& p = sh.part[2 * warp + (stops ? 1 : 0)];
+                if (!all_of_it && lane == 0 && member == 0) {
+                    Part& p = sh.part[2 * team + (stops ? 1 : 0)];
                     p.start = x0 + i - at.t;
                     p.r = at.r;
                     p.item = at.item;
@@ -836,35 +863,34 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
     }
     __syncthreads();  // every ring is done with: the last parts are staged there
     float* staged = reinterpret_cast<float*>(smem);
-    if (sh.part[2 * warp + 1].start >= 0) {
-        float* mine = staged + warp * (K::kHeads * K::kLd);
+    if (sh.part[2 * team + 1].start >= 0) {
+        float* mine = staged + team * (K::kHeads * K::kLd);
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const int h = n * 8 + 2 * j + x;
-                if (g == 0) {
-                    sh.m[2 * warp + 1][h] = m[n][x];
-                    sh.l[2 * warp + 1][h] = l[n][x];
-                }
-#pragma unroll
-                for (int c = 0; c < K::kSteps; ++c) {
-                    const int d0 = K::kFp8 ? c * 16 + 2 * g : c * 16 + g, d1 = K::kFp8 ? d0 + 1 : d0 + 8;
-                    mine[h * K::kLd + d0] = o[n][c][x];
-                    mine[h * K::kLd + d1] = o[n][c][x + 2];
-                }
+        for (int x = 0; x < 2; ++x) {
+            const int h = member * 8 + 2 * j + x;
+            if (g == 0) {
+                sh.m[2 * team + 1][h] = m[x];
+                sh.l[2 * team + 1][h] = l[x];
             }
+#pragma unroll
+            for (int c = 0; c < K::kSteps; ++c) {
+                const int d0 = K::kFp8 ? c * 16 + 2 * g : c * 16 + g, d1 = K::kFp8 ? d0 + 1 : d0 + 8;
+                mine[h * K::kLd + d0] = o[c][x];
+                mine[h * K::kLd + d1] = o[c][x + 2];
+            }
+        }
     }
+    constexpr int kParts = 2 * K::kTeams;
     if (warp == 0) {
         // the joined items: runs of consecutive parts with one start
-        const int64_t start = lane < 2 * W ? sh.part[lane].start : -1;
+        const int64_t start = lane < kParts ? sh.part[lane].start : -1;
         const uint32_t have = __ballot_sync(0xffffffffu, start >= 0), lower = have & ((1u << lane) - 1u);
         const int64_t left = __shfl_sync(0xffffffffu, start, lower ? 31 - __clz(lower) : lane);
         const uint32_t leads = __ballot_sync(0xffffffffu, start >= 0 && (!lower || left != start));
         if ((leads >> lane) & 1u) sh.lead[__popc(leads & ((1u << lane) - 1u))] = lane;
         if (lane == 0) {
             sh.items = __popc(leads);
-            sh.lead[__popc(leads)] = 2 * W;
+            sh.lead[__popc(leads)] = kParts;
         }
     }
     __syncthreads();
@@ -891,7 +917,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
             if (sh.part[k].start < 0) continue;
             const float r = rescale(sh.m[k][h], top);
             const float* from = (k & 1) ? staged + ((k >> 1) * K::kHeads + h) * K::kLd + d
-                                        : a.warp_part + (static_cast<int64_t>(blockIdx.x) * W + (k >> 1)) * K::kPart + h * DP + d;
+                                        : a.team_part + (static_cast<int64_t>(blockIdx.x) * K::kTeams + (k >> 1)) * K::kPart + h * DP + d;
             sum_l = __fmaf_rn(sh.l[k][h], r, sum_l);
             acc = fma4(*reinterpret_cast<const float4*>(from), r, acc);
         }
@@ -914,7 +940,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
     Part open[2] = {sh.part[sh.lead[0]], sh.part[sh.lead[joined - 1]]};
     bool is_open[2] = {open[0].ta > 0, false};
     {
-        int k = 2 * W - 1;
+        int k = kParts - 1;
         while (sh.part[k].start < 0) --k;
         is_open[1] = open[1].ta == 0 && sh.part[k].tb < open[1].nt;
     }
@@ -924,8 +950,8 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
     for (int slot = 0; slot < 2; ++slot) {
         if (!is_open[slot]) continue;
         const int64_t tile = open[slot].start;
-        first[slot] = static_cast<int32_t>(((tile + 1) * workers - 1) / total) / W;
-        last[slot] = static_cast<int32_t>(((tile + open[slot].nt) * workers - 1) / total) / W;
+        first[slot] = static_cast<int32_t>(((tile + 1) * workers - 1) / total) / K::kTeams;
+        last[slot] = static_cast<int32_t>(((tile + open[slot].nt) * workers - 1) / total) / K::kTeams;
         const int32_t n = last[slot] - first[slot] + 1;
         size[slot] = n <= kJoin ? n : max(12, (n + kJoin - 1) / kJoin);
     }
@@ -969,34 +995,35 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
 
 struct Kernel {
     void (*fn)(AttnArgs);
-    int threads, shared, part_floats, warps;
+    int threads, shared, part_floats, teams;
 };
 
-template <int MODE, int DP, int NT, int W, int S>
+template <int MODE, int DP, int TM, int W, int T, int S>
 Kernel kernel_of() {
-    using K = Attn<MODE, DP, NT, W, S>;
+    using K = Attn<MODE, DP, TM, W, T, S>;
     static_assert(K::kSharedBytes <= 232448, "shared memory of one CTA");
-    return Kernel{paged_attn_kernel<MODE, DP, NT, W, S>, K::kThreads, K::kSharedBytes, K::kPart, W};
+    return Kernel{paged_attn_kernel<MODE, DP, TM, W, T, S>, K::kThreads, K::kSharedBytes, K::kPart, K::kTeams};
 }
 
-// Warps and stages: about 192 KB of ring per SM, the bytes in flight that keep HBM busy.
-template <int MODE, int NT>
-Kernel pick_dim(int head_dim) {
-    constexpr bool fp8 = MODE == MF_DT_F8E4M3 || MODE == MF_DT_F8E5M2;
-    if (head_dim <= 64) return kernel_of<MODE, 64, NT, 12, fp8 ? 6 : 4>();
-    if (head_dim <= 128) return kernel_of<MODE, 128, NT, 12, fp8 ? 4 : 2>();
-    return kernel_of<MODE, 256, NT, fp8 ? 8 : 6, fp8 ? 3 : 2>();
-}
+// Warps, tokens of a tile and stages: about 192 KB of ring per SM, the bytes in flight that keep HBM busy.
 template <int MODE>
-Kernel pick_heads(int group, int head_dim) {
-    return group <= 8 ? pick_dim<MODE, 1>(head_dim) : pick_dim<MODE, 2>(head_dim);
+Kernel pick_shape(int group, int head_dim) {
+    constexpr bool fp8 = MODE == MF_DT_F8E4M3 || MODE == MF_DT_F8E5M2;
+    if (group <= 8) {
+        if (head_dim <= 64) return kernel_of<MODE, 64, 1, 12, 32, fp8 ? 4 : 2>();
+        if (head_dim <= 128) return kernel_of<MODE, 128, 1, 12, fp8 ? 32 : 16, 2>();
+        return kernel_of<MODE, 256, 1, fp8 ? 8 : 6, 16, fp8 ? 3 : 2>();
+    }
+    if (head_dim <= 64) return kernel_of<MODE, 64, 2, 12, 32, 4>();
+    if (head_dim <= 128) return kernel_of<MODE, 128, 2, 12, fp8 ? 32 : 16, 4>();
+    return kernel_of<MODE, 256, 2, 12, 16, fp8 ? 4 : 2>();
 }
 Kernel pick(int cache_dtype, int group, int head_dim) {
     switch (cache_dtype) {
-    case MF_DT_BF16: return pick_heads<MF_DT_BF16>(group, head_dim);
-    case MF_DT_F16: return pick_heads<MF_DT_F16>(group, head_dim);
-    case MF_DT_F8E4M3: return pick_heads<MF_DT_F8E4M3>(group, head_dim);
-    default: return pick_heads<MF_DT_F8E5M2>(group, head_dim);
+    case MF_DT_BF16: return pick_shape<MF_DT_BF16>(group, head_dim);
+    case MF_DT_F16: return pick_shape<MF_DT_F16>(group, head_dim);
+    case MF_DT_F8E4M3: return pick_shape<MF_DT_F8E4M3>(group, head_dim);
+    default: return pick_shape<MF_DT_F8E5M2>(group, head_dim);
     }
 }
 
@@ -1034,6 +1061,10 @@ extern "C" int mf_paged_attn_create(const mf_paged_attn_config* config, mf_paged
                     (long long)k.n_pages, k.page_size, c.max_pages, (long long)c.table_stride);
     if (k.page_stride % step || k.token_stride % step || k.head_stride % step)
         return fail(MF_ERR_LAYOUT_UNSUPPORTED, "mf_paged_attn_create: cache strides must be multiples of 16 bytes");
+    const int code = is_fp8(k.dtype) ? 1 : 2;
+    if (k.page_stride < 0 || k.token_stride < 0 || k.head_stride < 0 || k.page_stride > 0x7fffffffll / code ||
+        k.token_stride > 0x7fffffffll / code / k.page_size)
+        return fail(MF_ERR_LAYOUT_UNSUPPORTED, "mf_paged_attn_create: cache strides may not be negative, a page is below 2 GB");
     if (c.q_token_stride % 2 || c.q_head_stride % 2 || c.out_token_stride % 4 || c.out_head_stride % 4)
         return fail(MF_ERR_LAYOUT_UNSUPPORTED, "mf_paged_attn_create: query strides must be even, output strides multiples of 4");
     if (c.window < 0 || !(c.softcap >= 0.0f))
@@ -1043,9 +1074,9 @@ extern "C" int mf_paged_attn_create(const mf_paged_attn_config* config, mf_paged
     MF_CUDA_CHECK(cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel.fn), cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        kernel.shared));
     const int ctas = state().sm_count;
-    const size_t warp_part = static_cast<size_t>(ctas) * kernel.warps * kernel.part_floats * 4;
+    const size_t team_part = static_cast<size_t>(ctas) * kernel.teams * kernel.part_floats * 4;
     const size_t cta_part = static_cast<size_t>(ctas) * 3 * kernel.part_floats * 4;
-    const size_t bytes = warp_part + cta_part + static_cast<size_t>(ctas) * 8;
+    const size_t bytes = team_part + cta_part + static_cast<size_t>(ctas) * 8;
     mf_paged_attn_s* h = new (std::nothrow) mf_paged_attn_s{};
     if (!h) return fail(MF_ERR_ALLOCATOR_EXHAUSTED, "mf_paged_attn_create: out of host memory");
     cudaError_t err = cudaMalloc(&h->workspace, bytes);
@@ -1057,7 +1088,7 @@ extern "C" int mf_paged_attn_create(const mf_paged_attn_config* config, mf_paged
         return cuda_fail(err, "mf_paged_attn_create: cudaMalloc");
     }
     char* w = static_cast<char*>(h->workspace);
-    err = cudaMemset(w + warp_part + cta_part, 0, static_cast<size_t>(ctas) * 8);
+    err = cudaMemset(w + team_part + cta_part, 0, static_cast<size_t>(ctas) * 8);
     if (err == cudaSuccess) err = cudaStreamSynchronize(nullptr);  // streams that do not wait for the default one may run it
     if (err != cudaSuccess) {
         cudaFree(h->workspace);
@@ -1072,19 +1103,19 @@ extern "C" int mf_paged_attn_create(const mf_paged_attn_config* config, mf_paged
     a.slopes = c.slopes;
     a.k_scale = is_fp8(k.dtype) ? c.k_scale_inv : nullptr;
     a.v_scale = is_fp8(k.dtype) ? c.v_scale_inv : nullptr;
-    a.warp_part = reinterpret_cast<float*>(w);
-    a.cta_part = reinterpret_cast<float*>(w + warp_part);
-    a.tickets = reinterpret_cast<int32_t*>(w + warp_part + cta_part);
+    a.team_part = reinterpret_cast<float*>(w);
+    a.cta_part = reinterpret_cast<float*>(w + team_part);
+    a.tickets = reinterpret_cast<int32_t*>(w + team_part + cta_part);
     a.status = sticky_status_ptr();
     a.q_req = c.q_token_stride;
     a.q_head = c.q_head_stride;
     a.out_req = c.out_token_stride;
     a.out_head = c.out_head_stride;
-    a.page_stride = k.page_stride;
-    a.token_stride = k.token_stride;
-    a.head_stride = k.head_stride;
+    a.page_bytes = static_cast<int32_t>(k.page_stride * code);
+    a.row_bytes = static_cast<int32_t>(k.token_stride * code);
+    a.head_bytes = k.head_stride * code;
     a.table_stride = c.table_stride;
-    a.n_pages = k.n_pages;
+    a.n_pages = static_cast<uint32_t>(k.n_pages < 0x7fffffff ? k.n_pages : 0x7fffffff);
     a.q_heads = c.q_heads;
     a.kv_heads = k.kv_heads;
     a.group = group;
