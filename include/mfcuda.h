@@ -132,6 +132,9 @@ int mf_device_status(int* device_code);
 /* Device status code of a page number or slot outside its cache: nothing was
  * read or written there (the token counts as masked). */
 #define MF_DEVICE_BAD_PAGE 0x7200
+/* Device status code of a call whose device-side lengths ask for more than it
+ * can index: nothing was computed. */
+#define MF_DEVICE_TOO_LARGE 0x7300
 /* Make `stream` wait until the int at device address `flag` equals `expect`
  * (acquire load, polled with a short sleep), for at most `max_polls` polls;
  * if it never does, record MF_DEVICE_TIMEOUT in the sticky status and let the
@@ -568,6 +571,8 @@ int mf_rope_append(const mf_rope_append_config* config, const void* q, const voi
  * Products and sums are float32, the weights exp(s - max) enter the product
  * with the values as two 16-bit terms (their sum has 16 bits or more).
  *
+ * One run covers up to 2^31 - 1 tiles (16 tokens of one key-value head, for up
+ * to 16 query heads); lengths that ask for more record MF_DEVICE_TOO_LARGE.
  * A handle holds the description and the workspace of the split (about 10 MB):
  * create it once, run it for every step and layer.  A handle is not shared
  * between streams that run at once.  One launch per run, no host sync; results

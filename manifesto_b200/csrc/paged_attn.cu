@@ -34,6 +34,7 @@
 // result does not depend on who was last.
 #include <new>
 
+#include "mf_async.cuh"
 #include "mf_runtime.h"
 #include "mf_vec.cuh"
 
@@ -44,28 +45,32 @@ constexpr int kBlock = 16;         // tokens of one product; a tile is one or tw
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kLn2 = 0.693147180559945309f;
 
+// Ordered by first use: the start of a run waits for a line of parameters only once or twice.
 struct AttnArgs {
-    const void* q;
-    const void* k;
-    const void* v;
-    const int32_t* table;
     const int32_t* lens;
-    void* out;
-    float* lse;
+    const int32_t* table;
+    int32_t n_requests, items;  // items: kv_heads * blocks
+    int32_t max_pages, page, window, blocks;  // blocks of query heads per key-value head
+    const char* k;
+    const char* v;
+    int32_t page_bytes, row_bytes;
+    int64_t head_bytes, table_stride;
+    uint32_t n_pages;
+    int32_t head_dim;
+    const char* q;
+    int64_t q_req, q_head;
+    int32_t q_heads, group, q_f16;
+    float scale, softcap;
     const float* slopes;
     const float* k_scale;
     const float* v_scale;
+    char* out;
+    int64_t out_req, out_head;
+    float* lse;
     float* team_part;     // [teams][heads * (DP + 2)]: parts that end inside a team's run
     float* cta_part;      // [CTAs][3][heads * (DP + 2)]: parts that leave the CTA, and joined groups of them
     int32_t* tickets;     // [2][CTAs], zero between runs
     int32_t* status;
-    int64_t q_req, q_head, out_req, out_head;
-    int64_t head_bytes, table_stride;
-    int32_t page_bytes, row_bytes;
-    uint32_t n_pages;
-    int32_t n_requests, q_heads, kv_heads, group, blocks;  // blocks of query heads per key-value head
-    int32_t head_dim, page, max_pages, window, q_f16;
-    float scale, softcap;
 };
 
 // ------------------------------------------------------------------ pieces
@@ -191,24 +196,43 @@ struct Place {
     }
 };
 
-// x * y / z, in 32 bits where they hold it (a 64-bit division is a long call).
-__device__ __forceinline__ int64_t mul_div(int64_t x, int32_t y, int64_t z) {
-    const int64_t p = x * y;
-    if (((p | z) >> 32) == 0) return static_cast<uint32_t>(p) / static_cast<uint32_t>(z);
-    return p / z;
-}
+// An even cut of `total` into `parts`: part i starts at total * i / parts, in 32 bits for parts below 2^16.
+struct Cut {
+    int32_t total, parts, q, rem;
+    __device__ __forceinline__ Cut(int32_t total_, int32_t parts_)
+        : total(total_), parts(parts_), q(total_ / parts_), rem(total_ % parts_) {}
+    __device__ __forceinline__ int32_t start(int32_t i) const { return q * i + rem * i / parts; }
+    // the part that x is in, of a cut without empty parts
+    __device__ __forceinline__ int32_t part_of(int32_t x) const {
+        int32_t i = min(parts - 1, static_cast<int32_t>((static_cast<float>(x) + 0.5f) * static_cast<float>(parts) / static_cast<float>(total)));
+        while (start(i) > x) --i;
+        while (i + 1 < parts && start(i + 1) <= x) ++i;
+        return i;
+    }
+};
 
 // What is known of one part of an item that a warp or CTA summed.
 struct Part {
-    int64_t start;   // first tile of the item in the row of all tiles; -1: no part
+    int32_t start;   // first tile of the item in the row of all tiles; -1: no part
     int32_t r, item, nt;
     int32_t ta, tb;  // its tiles of the item
+};
+
+// An item of which this CTA has parts: the parts, where it belongs, and whether it is whole (slot -1) or other CTAs have
+// parts of it, too.  Slot 0 is the end or middle of an item that began in an earlier CTA, slot 1 the start of one that ends
+// in a later CTA.
+struct Joined {
+    uint32_t parts;
+    int32_t r, kv, head0, heads, slot, start, nt;
 };
 
 constexpr int kJoin = 16;  // most parts that one step of a join between CTAs takes
 // A maximum is only replaced by one that is this much larger (in powers of two): until then the weights grow up to
 // 2^8, which float32 sums and both terms of a weight hold as well, and what is summed is not rescaled.
 constexpr float kLazy = 8.0f;
+// A warp waits for the others of its CTA when it is this many tiles ahead.  Their loads queue for the same HBM, so
+// those that lag get what the waiting one leaves, and all end together: without it the warps of a CTA ended 12% apart.
+constexpr int kAhead = 2;
 
 // MODE: dtype of the cache; DP: head_dim padded to 64, 128 or 256; TM: warps of a team; W: warps; T: tokens of a
 // tile; S: stages of a team's ring.  A team works on one item at a time, each of its warps for 8 query heads.
@@ -226,24 +250,27 @@ struct Attn {
     static constexpr int kTeams = W / TM;
     static constexpr int kHeads = 8 * TM;             // query heads of an item, at most
     static constexpr int kFour = DP / 4;
-    static constexpr int kLd = DP + 4;                // floats of a staged head's row (spread over the banks)
     static constexpr int kPart = kHeads * (DP + 2);   // floats of a part in the workspace: out, then m, l
     static constexpr int kThreads = 32 * W;
     static constexpr int kRing = kTeams * S * kStage;
-    static constexpr int kStaged = kTeams * kHeads * kLd * 4;
+    // floats of a staged head's row: spread over the banks where there is room for two parts of each team
+    static constexpr int kLd = 2 * kTeams * kHeads * (DP + 4) * 4 <= kRing ? DP + 4 : DP;
+    static constexpr int kStaged = 2 * kTeams * kHeads * kLd * 4;
     static constexpr int kBuffer = kRing > kStaged ? kRing : kStaged;
     static_assert(2 * kTeams <= 32, "a lane for each part of a CTA");
     static_assert(TM == 1 || kTeams < 16, "a barrier for each team");
     static_assert(W >= 2 && (T == kBlock || T == 2 * kBlock), "");
 
     struct Shared {
-        int64_t prefix[kThreads + 1];   // tiles of the requests in front of each thread's
-        int64_t warp_sum[W];
+        uint64_t step[4];               // all warps are done with a tile
+        int64_t warp_sum[32];           // tiles of the requests of each warp's threads
+        int32_t thread_sum[kThreads];   // and of each thread's
         Part part[2 * kTeams];          // first and last part of each team
-        float m[2 * kTeams][kHeads], l[2 * kTeams][kHeads];
+        float m[2 * kTeams][kHeads], l[2 * kTeams][kHeads];  // of the parts; m becomes their weight
+        Joined joined[2 * kTeams];
+        float joined_m[2 * kTeams][kHeads], joined_l[2 * kTeams][kHeads];
         float weight[kJoin][kHeads], top[kHeads], sum[kHeads];
         uint32_t mask[kTeams][S];       // tokens of each stage that are there
-        int32_t lead[2 * kTeams + 1];   // first part of each joined item, then 2 * kTeams
         int32_t items;                  // joined items
         int32_t won[2];                 // whether this CTA joins the item of its slot
     };
@@ -268,7 +295,7 @@ __device__ __forceinline__ uint32_t pieces_on(uint32_t at, int c) {
 // Write `f` (4 floats of head h, elements d..d+3, normalised) to the output.
 __device__ __forceinline__ void store_out4(const AttnArgs& a, int32_t r, int32_t head, int d, float4 f) {
     if (d >= a.head_dim) return;
-    char* p = static_cast<char*>(a.out) + 2 * (r * a.out_req + head * a.out_head + d);
+    char* p = a.out + 2 * (r * a.out_req + head * a.out_head + d);
     const float v[4] = {f.x, f.y, f.z, f.w};
     uint32_t w[2];
     if (a.q_f16) encode4<MF_DT_F16>(v, w, 0);
@@ -290,86 +317,95 @@ template <int HEADS>
 struct Heads {
     int32_t kv, head0, count;
     __device__ __forceinline__ Heads(const AttnArgs& a, int32_t item) {
-        kv = item / a.blocks;
-        head0 = kv * a.group + item % a.blocks * HEADS;
+        kv = a.blocks == 1 ? item : item / a.blocks;
+        head0 = kv * a.group + (item - kv * a.blocks) * HEADS;
         count = min(HEADS, (kv + 1) * a.group - head0);
     }
 };
 
 // One more arrival at a ticket that `count` CTAs share; true for the last one,
 // which leaves the ticket at zero.  What every thread of the CTA wrote before
-// the last barrier is visible to whoever arrives later.
+// the last barrier is visible to whoever arrives later (the release is
+// cumulative over what the barrier ordered before it).
 __device__ __forceinline__ bool arrive_last(int32_t* ticket, int32_t count) {
     int32_t old;
-    asm volatile("fence.acq_rel.gpu;" ::: "memory");
     asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(old) : "l"(ticket) : "memory");
     if (old != count - 1) return false;
     *ticket = 0;
-    asm volatile("fence.acq_rel.gpu;" ::: "memory");
     return true;
 }
 
 // Joins parts 0 .. n-1 (n <= kJoin) at first + k * stride floats, but the first
 // at at0 and the last at at_end: to the output if `to` is NULL, else to a part
-// there.  All threads of the CTA.
-template <class K>
-__device__ __forceinline__ void join_parts(const AttnArgs& a, typename K::Shared& sh, const float* first, int64_t stride,
-                                           const float* at0, const float* at_end, int32_t n, int32_t r, int32_t item, float* to,
-                                           int dp) {
+// there.  All threads of the CTA; the parts pass through shared memory, as many
+// at a time as it holds.
+template <class K, int DP>
+__device__ __forceinline__ void join_parts(const AttnArgs& a, typename K::Shared& sh, unsigned char* smem, const float* first,
+                                           int64_t stride, const float* at0, const float* at_end, int32_t n, const Joined& w,
+                                           float* to) {
+    constexpr int kFloats = K::kHeads * DP, kRound = K::kBuffer / (kFloats * 4);
+    constexpr int kEach = (K::kHeads * K::kFour + K::kThreads - 1) / K::kThreads;
+    static_assert(kRound >= 1, "");
     const int tid = threadIdx.x;
-    const Heads<K::kHeads> hd(a, item);
+    const float* in = reinterpret_cast<const float*>(smem);
+    const uint32_t buffer = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
     auto part = [&](int k) { return k == 0 ? at0 : k == n - 1 ? at_end : first + k * stride; };
-    constexpr int kAhead = 8;
-    float4 f[kAhead];
-    int i = tid;
-    // the first element's loads travel together with those of the weights
+    float4 acc[kEach];
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k)
-        if (i < hd.count * K::kFour && k < n) f[k] = __ldcg(reinterpret_cast<const float4*>(part(k) + i * 4));
-    if (tid < hd.count) {
-        float top = -INFINITY, sum = 0.0f, m[kJoin], l[kJoin];
-#pragma unroll
-        for (int k = 0; k < kJoin; ++k) {
-            m[k] = k < n ? __ldcg(part(k) + K::kHeads * dp + tid) : -INFINITY;
-            l[k] = k < n ? __ldcg(part(k) + K::kHeads * dp + K::kHeads + tid) : 0.0f;
+    for (int e = 0; e < kEach; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k0 = 0; k0 < n; k0 += kRound) {
+        const int k1 = min(k0 + kRound, n);
+#pragma unroll 1
+        for (int k = k0; k < k1; ++k) {
+            const float* from = part(k);
+            for (int i = tid; i < w.heads * K::kFour; i += K::kThreads)
+                cp_async16(buffer + ((k - k0) * kFloats + i * 4) * 4, from + i * 4, 16u);
         }
+        cp_async_commit();
+        if (k0 == 0 && tid < w.heads) {
+            float top = -INFINITY, sum = 0.0f, m[kJoin], l[kJoin];
 #pragma unroll
-        for (int k = 0; k < kJoin; ++k) top = fmaxf(top, m[k]);
-#pragma unroll
-        for (int k = 0; k < kJoin; ++k) {
-            if (k >= n) break;
-            const float w = rescale(m[k], top);
-            sh.weight[k][tid] = w;
-            sum = __fmaf_rn(l[k], w, sum);
-        }
-        sh.top[tid] = top;
-        sh.sum[tid] = sum;
-    }
-    __syncthreads();
-    const float vs = a.v_scale ? __ldg(a.v_scale + hd.kv) : 1.0f;
-    for (; i < hd.count * K::kFour; i += K::kThreads) {
-        const int h = i / K::kFour, d = i % K::kFour * 4;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int k0 = 0; k0 < n; k0 += kAhead) {
-            if (k0 > 0 || i != tid) {
-#pragma unroll
-                for (int k = 0; k < kAhead; ++k)
-                    if (k0 + k < n) f[k] = __ldcg(reinterpret_cast<const float4*>(part(k0 + k) + i * 4));
+            for (int k = 0; k < kJoin; ++k) {
+                m[k] = k < n ? __ldcg(part(k) + kFloats + tid) : -INFINITY;
+                l[k] = k < n ? __ldcg(part(k) + kFloats + K::kHeads + tid) : 0.0f;
+                top = fmaxf(top, m[k]);
             }
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k)
-                if (k0 + k < n) acc = fma4(f[k], sh.weight[k0 + k][h], acc);
+            for (int k = 0; k < kJoin; ++k) {
+                const float by = rescale(m[k], top);
+                sh.weight[k][tid] = by;
+                sum = k < n ? __fmaf_rn(l[k], by, sum) : sum;
+            }
+            sh.top[tid] = top;
+            sh.sum[tid] = sum;
         }
+        cp_async_wait<0>();
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            const int i = tid + e * K::kThreads, h = i / K::kFour;
+            if (i >= w.heads * K::kFour) break;
+#pragma unroll 4
+            for (int k = k0; k < k1; ++k)
+                acc[e] = fma4(*reinterpret_cast<const float4*>(in + (k - k0) * kFloats + i * 4), sh.weight[k][h], acc[e]);
+        }
+        __syncthreads();
+    }
+    const float vs = a.v_scale ? __ldg(a.v_scale + w.kv) : 1.0f;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        const int i = tid + e * K::kThreads, h = i / K::kFour, d = i % K::kFour * 4;
+        if (i >= w.heads * K::kFour) break;
         const float sum = sh.sum[h];
         if (to) {
-            *reinterpret_cast<float4*>(to + i * 4) = acc;
+            *reinterpret_cast<float4*>(to + i * 4) = acc[e];
             if (d == 0) {
-                to[K::kHeads * dp + h] = sh.top[h];
-                to[K::kHeads * dp + K::kHeads + h] = sum;
+                to[kFloats + h] = sh.top[h];
+                to[kFloats + K::kHeads + h] = sum;
             }
         } else {
-            store_out4(a, r, hd.head0 + h, d, scale4(acc, sum == 0.0f ? 0.0f : __fdiv_rn(vs, sum)));
-            if (d == 0) store_lse(a, r, hd.head0 + h, sh.top[h], sum);
+            store_out4(a, w.r, w.head0 + h, d, scale4(acc[e], sum == 0.0f ? 0.0f : __fdiv_rn(vs, sum)));
+            if (d == 0) store_lse(a, w.r, w.head0 + h, sh.top[h], sum);
         }
     }
     __syncthreads();
@@ -383,9 +419,9 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int team = warp / TM, member = warp % TM;
     const int g = lane >> 2, j = lane & 3;  // row and column pair of a product's fragment
-    const int32_t items = a.kv_heads * a.blocks;
+    const int32_t items = a.items;
 
-    // prefix of the tiles: thread i sums `per` consecutive requests
+    // the tiles of thread i's `per` consecutive requests
     const int32_t per = (a.n_requests + K::kThreads - 1) / K::kThreads;
     int64_t sum = 0;
     bool empty = false;
@@ -396,14 +432,14 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
         sum += static_cast<int64_t>(nt) * items;
         empty |= nt == 0 && r % gridDim.x == blockIdx.x;
     }
-    int64_t inc = sum;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const int64_t x = __shfl_up_sync(0xffffffffu, inc, d);
-        if (lane >= d) inc += x;
+    sh.thread_sum[tid] = static_cast<int32_t>(sum);
+    {
+        const int64_t low = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(sum & 0xffff));
+        const int64_t high = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(sum >> 16 < (1 << 26) ? sum >> 16 : 1 << 26));
+        if (lane == 0) sh.warp_sum[warp] = (high << 16) + low;
     }
-    if (lane == 31) sh.warp_sum[warp] = inc;
     if (tid < 2 * K::kTeams) sh.part[tid].start = -1;
+    if (tid < 4) mbar_init(&sh.step[tid], W);
     if (__syncthreads_or(empty)) {
         // requests that see nothing
         for (int32_t r = blockIdx.x; r < a.n_requests; r += gridDim.x) {
@@ -413,47 +449,57 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
             for (int i = tid; i < a.q_heads; i += K::kThreads) store_lse(a, r, i, 0.0f, 0.0f);
         }
     }
-    int64_t total = 0, base = 0;
+    // the row of all tiles: this CTA's run of them, and this team's of those
+    const int64_t of_warp = lane < W ? sh.warp_sum[lane] : 0;
+    int64_t in_front = of_warp;
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-        if (w == warp) base = total;
-        total += sh.warp_sum[w];
+    for (int d = 1; d < 16; d <<= 1) {
+        const int64_t x = __shfl_up_sync(0xffffffffu, in_front, d);
+        if (lane >= d) in_front += x;
     }
-    sh.prefix[tid] = base + inc - sum;
-    if (tid == 0) sh.prefix[K::kThreads] = total;
-    __syncthreads();
-    if (total == 0) return;
-    const int64_t want = (total + K::kTeams - 1) / K::kTeams;
-    int32_t ctas = static_cast<int32_t>(want < gridDim.x ? want : gridDim.x);
+    const int64_t total64 = __shfl_sync(0xffffffffu, in_front, W - 1);
+    if (total64 == 0) return;
+    if (total64 > 0x7fffffff) {
+        if (tid == 0) atomicExch(a.status, MF_DEVICE_TOO_LARGE);
+        return;
+    }
+    const int32_t total = static_cast<int32_t>(total64), want = (total - 1) / K::kTeams + 1;
+    int32_t ctas = min(want, static_cast<int32_t>(gridDim.x));
     if (a.n_requests == 1 && items <= gridDim.x) ctas = max(ctas / items, 1) * items;  // no CTA has parts of two items
     if (blockIdx.x >= ctas) return;
-    const int32_t workers = ctas * K::kTeams;
+    const Cut by_cta(total, ctas);
+    const int32_t cta_tile = by_cta.start(blockIdx.x), cta_tiles = by_cta.start(blockIdx.x + 1) - cta_tile;
+    const Cut by_team(cta_tiles, K::kTeams);
+    const int32_t x0 = cta_tile + by_team.start(team), my_tiles = cta_tile + by_team.start(team + 1) - x0;
     const int32_t id = blockIdx.x * K::kTeams + team;
-    const int64_t x0 = mul_div(total, id, workers), x1 = mul_div(total, id + 1, workers);
-    const int32_t my_tiles = static_cast<int32_t>(x1 - x0);
 
     uint32_t qf[K::kSteps][2];
     float o[K::kSteps][4];
     float m[2], l[2];
     if (my_tiles > 0) {
         // the place of tile x0: the warp, then the thread whose requests hold it, then the request among them
-        int64_t before = 0;
-        int lo = 0;
+        in_front -= of_warp;
+        const int in_warp = 31 - __clz(__ballot_sync(0xffffffffu, lane < W && in_front <= x0));
+        int32_t before = static_cast<int32_t>(__shfl_sync(0xffffffffu, in_front, in_warp));
+        const int32_t of_thread = sh.thread_sum[32 * in_warp + lane];
+        int32_t ahead = of_thread;
 #pragma unroll
-        for (int w = 1; w < W; ++w)
-            if (sh.prefix[32 * w] <= x0) lo = 32 * w;
-        lo += 31 - __clz(__ballot_sync(0xffffffffu, sh.prefix[lo + lane] <= x0));
-        before = sh.prefix[lo];
+        for (int d = 1; d < 32; d <<= 1) {
+            const int32_t x = __shfl_up_sync(0xffffffffu, ahead, d);
+            if (lane >= d) ahead += x;
+        }
+        ahead -= of_thread;
+        const int in_lane = 31 - __clz(__ballot_sync(0xffffffffu, before + ahead <= x0));
+        before += __shfl_sync(0xffffffffu, ahead, in_lane);
         Place<T> at{};
-        at.r = lo;
+        at.r = 32 * in_warp + in_lane;
         if (per > 1) {
-            for (int32_t r0 = lo * per;; r0 += 32) {
-                const int32_t nt = r0 + lane < a.n_requests ? tiles_of<T>(span_of(a, r0 + lane)) : 0;
-                const int64_t mine = static_cast<int64_t>(nt) * items;
-                int64_t upto = mine;
-#pragma unroll
+            for (int32_t r0 = at.r * per;; r0 += 32) {
+                const int32_t mine = r0 + lane < a.n_requests ? tiles_of<T>(span_of(a, r0 + lane)) * items : 0;
+                int32_t upto = mine;
+#pragma unroll 1
                 for (int d = 1; d < 32; d <<= 1) {
-                    const int64_t x = __shfl_up_sync(0xffffffffu, upto, d);
+                    const int32_t x = __shfl_up_sync(0xffffffffu, upto, d);
                     if (lane >= d) upto += x;
                 }
                 const uint32_t past = __ballot_sync(0xffffffffu, before + upto > x0);
@@ -468,9 +514,9 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
         }
         at.span = span_of(a, at.r);
         at.nt = tiles_of<T>(at.span);
-        const int64_t in_request = x0 - before;
-        at.item = static_cast<int32_t>(mul_div(in_request, 1, at.nt));
-        at.t = static_cast<int32_t>(in_request - static_cast<int64_t>(at.item) * at.nt);
+        const int32_t in_request = x0 - before;
+        at.item = in_request / at.nt;
+        at.t = in_request - at.item * at.nt;
 
         unsigned char* my_ring = smem + team * (S * K::kStage);
         const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(my_ring));
@@ -483,7 +529,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
         const int piece_row = lane / K::kChunks + member * (kCopies * kRows), piece = lane % K::kChunks;
         const int64_t lane_bytes = static_cast<int64_t>(piece_row) * a.row_bytes + piece * 16;
         const bool piece_in = piece * (16 / K::kBytes) < a.head_dim;
-        const int64_t kv_gap = static_cast<const char*>(a.v) - static_cast<const char*>(a.k);
+        const int64_t kv_gap = a.v - a.k;
         // of the blocks of the tile at `load` (or, blocks not being whole, of this lane's row): their pages, the pages'
         // places in the table's row and the blocks' in the pages
         const int32_t* table_row = nullptr;
@@ -493,7 +539,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
             if (to_load == 0) return;
             if (new_item) {
                 table_row = a.table + load.r * a.table_stride;
-                head_at = static_cast<const char*>(a.k) + load.item / a.blocks * a.head_bytes + lane_bytes;
+                head_at = a.k + (a.blocks == 1 ? load.item : load.item / a.blocks) * a.head_bytes + lane_bytes;
             }
 #pragma unroll
             for (int b = 0; b < K::kBlocks; ++b) {
@@ -556,7 +602,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                         const int rw = i / kCopies * kBlock + i % kCopies * kRows + piece_row;
                         const int64_t row_at = __shfl_sync(0xffffffffu, row, rw) - static_cast<int64_t>(piece_row) * a.row_bytes;
                         const bool get = piece_in && ((mask >> rw) & 1u);
-                        const char* kp = get ? head_at + row_at : static_cast<const char*>(a.k);
+                        const char* kp = get ? head_at + row_at : a.k;
                         const uint32_t to = dst + swizzled<K::kChunks>(rw, piece);
                         cp_async16(to, kp, get ? 16u : 0u);
                         cp_async16(to + T * K::kRow, kp + kv_gap, get ? 16u : 0u);
@@ -581,7 +627,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
         auto load_queries = [&](const Place<T>& p) {
             const Heads<K::kHeads> hd(a, p.item);
             const int h = member * 8 + g;
-            const char* q = static_cast<const char*>(a.q) + 2 * (p.r * a.q_req + (hd.head0 + h) * a.q_head);
+            const char* q = a.q + 2 * (p.r * a.q_req + (hd.head0 + h) * a.q_head);
 #pragma unroll
             for (int c = 0; c < K::kSteps; ++c) {
                 const int d0 = K::kFp8 ? c * 16 + 4 * j : c * 16 + 2 * j;
@@ -601,8 +647,11 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
         float scale[2] = {0.0f, 0.0f}, slope[2] = {0.0f, 0.0f};
         int32_t ta = at.t;
         int stage = 0;
+        const int32_t common = by_team.q;  // tiles that every team of the CTA has
 #pragma unroll 1
         for (int32_t i = 0; i < my_tiles; ++i) {
+            if (i >= kAhead && i - kAhead < common && !mbar_wait(&sh.step[(i - kAhead) & 3], ((i - kAhead) >> 2) & 1))
+                atomicExch(a.status, MF_DEVICE_TIMEOUT);  // the results do not depend on it
             cp_async_wait<S - 2>();
             team_sync<TM>(team);
             issue(stage == 0 ? S - 1 : stage - 1);
@@ -807,7 +856,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                         f[x] = l[x] == 0.0f ? 0.0f : __fdiv_rn(vs, l[x]);
                         if (g == 0 && h < hd.count) store_lse(a, at.r, hd.head0 + h, m[x], l[x]);
                     }
-                    char* out = static_cast<char*>(a.out) + 2 * (at.r * a.out_req + hd.head0 * a.out_head);
+                    char* out = a.out + 2 * (at.r * a.out_req + hd.head0 * a.out_head);
 #pragma unroll
                     for (int c = 0; c < K::kSteps; ++c) {
                         if constexpr (!K::kFp8) {
@@ -856,15 +905,25 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                     p.tb = at.t + 1;
                 }
             }
+            if (lane == 0 && i < common) mbar_arrive(&sh.step[i & 3]);
             at = following;
             stage = stage + 1 == S ? 0 : stage + 1;
         }
         cp_async_wait<0>();
     }
     __syncthreads();  // every ring is done with: the last parts are staged there
-    float* staged = reinterpret_cast<float*>(smem);
+    float* staged = reinterpret_cast<float*>(smem);  // [parts][heads][kLd]
+    if (sh.part[2 * team].start >= 0) {
+        // the first part comes back from the workspace
+        const float* from = a.team_part + static_cast<int64_t>(id) * K::kPart + member * 8 * DP;
+        const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(staged + (2 * team * K::kHeads + member * 8) * K::kLd));
+#pragma unroll 1
+        for (int i = lane; i < 8 * K::kFour; i += 32)
+            cp_async16(to + (i / K::kFour * K::kLd + i % K::kFour * 4) * 4, from + i * 4, 16u);
+    }
+    cp_async_commit();
     if (sh.part[2 * team + 1].start >= 0) {
-        float* mine = staged + team * (K::kHeads * K::kLd);
+        float* mine = staged + (2 * team + 1) * (K::kHeads * K::kLd);
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
             const int h = member * 8 + 2 * j + x;
@@ -881,52 +940,85 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
         }
     }
     constexpr int kParts = 2 * K::kTeams;
+    // the joined items: runs of consecutive parts with one start
+    const int32_t start = lane < kParts ? sh.part[lane].start : -1;
+    const uint32_t have = __ballot_sync(0xffffffffu, start >= 0), lower = have & ((1u << lane) - 1u);
+    const int32_t left = __shfl_sync(0xffffffffu, start, lower ? 31 - __clz(lower) : lane);
+    const uint32_t leads = __ballot_sync(0xffffffffu, start >= 0 && (!lower || left != start));
+    if (leads == 0) return;
+    const uint32_t up_to = leads & (0xffffffffu >> (31 - lane));   // leads at or before this lane
+    const uint32_t after = leads & ~(0xffffffffu >> (31 - lane));  // and behind it
+    const int lead = up_to ? 31 - __clz(up_to) : lane, end = after ? __ffs(after) - 2 : 31;  // this lane's run of parts
+    const int grp = __popc(up_to) - 1;
     if (warp == 0) {
-        // the joined items: runs of consecutive parts with one start
-        const int64_t start = lane < kParts ? sh.part[lane].start : -1;
-        const uint32_t have = __ballot_sync(0xffffffffu, start >= 0), lower = have & ((1u << lane) - 1u);
-        const int64_t left = __shfl_sync(0xffffffffu, start, lower ? 31 - __clz(lower) : lane);
-        const uint32_t leads = __ballot_sync(0xffffffffu, start >= 0 && (!lower || left != start));
-        if ((leads >> lane) & 1u) sh.lead[__popc(leads & ((1u << lane) - 1u))] = lane;
-        if (lane == 0) {
-            sh.items = __popc(leads);
-            sh.lead[__popc(leads)] = kParts;
+        const uint32_t parts = have & (0xffffffffu << lead) & (0xffffffffu >> (31 - end));
+        if (lane == lead && start >= 0) {
+            const Part& p = sh.part[lane];
+            const Heads<K::kHeads> hd(a, p.item);
+            const bool whole = p.ta == 0 && sh.part[31 - __clz(parts)].tb == p.nt;
+            sh.joined[grp] = Joined{parts, p.r, hd.kv, hd.head0, hd.count, whole ? -1 : p.ta > 0 ? 0 : 1, p.start, p.nt};
         }
+        if (lane == 0) sh.items = __popc(leads);
     }
     __syncthreads();
 
-    // join the parts of each item inside the CTA
-    const int32_t joined = sh.items;
-    if (joined == 0) return;
-    for (int i = tid; i < joined * K::kHeads * K::kFour; i += K::kThreads) {
-        const int grp = i / (K::kHeads * K::kFour), h = i / K::kFour % K::kHeads, d = i % K::kFour * 4;
-        const int e = sh.lead[grp], end = sh.lead[grp + 1];
-        const Part& p = sh.part[e];
-        const Heads<K::kHeads> hd(a, p.item);
-        if (h >= hd.count) continue;
-        float top = -INFINITY;
-        int32_t tb = 0;
-        for (int k = e; k < end; ++k)
-            if (sh.part[k].start >= 0) {
-                top = fmaxf(top, sh.m[k][h]);
-                tb = sh.part[k].tb;
-            }
-        float sum_l = 0.0f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int k = e; k < end; ++k) {
-            if (sh.part[k].start < 0) continue;
-            const float r = rescale(sh.m[k][h], top);
-            const float* from = (k & 1) ? staged + ((k >> 1) * K::kHeads + h) * K::kLd + d
-                                        : a.team_part + (static_cast<int64_t>(blockIdx.x) * K::kTeams + (k >> 1)) * K::kPart + h * DP + d;
-            sum_l = __fmaf_rn(sh.l[k][h], r, sum_l);
-            acc = fma4(*reinterpret_cast<const float4*>(from), r, acc);
+    // Join the parts of each item inside the CTA.  First the parts' weights: a warp for each head, a lane for each part.
+    for (int h = warp; h < K::kHeads; h += W) {
+        const bool is = start >= 0;
+        const float mine = is ? sh.m[lane][h] : -INFINITY;
+        float top = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const float x = __shfl_up_sync(0xffffffffu, top, d);
+            if (lane - d >= lead) top = fmaxf(top, x);
         }
-        if (p.ta == 0 && tb == p.nt) {
-            const float vs = a.v_scale ? __ldg(a.v_scale + hd.kv) : 1.0f;
-            store_out4(a, p.r, hd.head0 + h, d, scale4(acc, sum_l == 0.0f ? 0.0f : __fdiv_rn(vs, sum_l)));
-            if (d == 0) store_lse(a, p.r, hd.head0 + h, top, sum_l);
+        top = __shfl_sync(0xffffffffu, top, end);
+        const float w = rescale(mine, top);
+        float sum_l = is ? sh.l[lane][h] * w : 0.0f;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const float x = __shfl_up_sync(0xffffffffu, sum_l, d);
+            if (lane - d >= lead) sum_l += x;
+        }
+        sum_l = __shfl_sync(0xffffffffu, sum_l, end);
+        if (is) sh.m[lane][h] = w;
+        if (is && lane == lead) {
+            sh.joined_m[grp][h] = top;
+            sh.joined_l[grp][h] = sum_l;
+        }
+    }
+    cp_async_wait<0>();
+    __syncthreads();
+    const int32_t joined = sh.items;
+    for (int i = tid; i < joined * K::kHeads * K::kFour; i += K::kThreads) {
+        const int which = i / (K::kHeads * K::kFour), h = i / K::kFour % K::kHeads, d = i % K::kFour * 4;
+        const Joined& w = sh.joined[which];
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (uint32_t parts = w.parts; parts;) {
+            float4 f[4];
+            float by[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int k = parts ? __ffs(parts) - 1 : -1;
+                parts &= parts - 1;
+                by[x] = 0.0f;
+                f[x] = acc;
+                if (k >= 0) {
+                    by[x] = sh.m[k][h];
+                    f[x] = *reinterpret_cast<const float4*>(staged + (k * K::kHeads + h) * K::kLd + d);
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < 4; ++x) acc = x > 0 && by[x] == 0.0f ? acc : fma4(f[x], by[x], acc);
+        }
+        const float top = sh.joined_m[which][h], sum_l = sh.joined_l[which][h];
+        if (h >= w.heads) continue;
+        if (w.slot < 0) {
+            const float vs = a.v_scale ? __ldg(a.v_scale + w.kv) : 1.0f;
+            store_out4(a, w.r, w.head0 + h, d, scale4(acc, sum_l == 0.0f ? 0.0f : __fdiv_rn(vs, sum_l)));
+            if (d == 0) store_lse(a, w.r, w.head0 + h, top, sum_l);
         } else {
-            float* to = a.cta_part + (static_cast<int64_t>(blockIdx.x) * 3 + (p.ta > 0 ? 0 : 1)) * K::kPart;
+            float* to = a.cta_part + (static_cast<int64_t>(blockIdx.x) * 3 + w.slot) * K::kPart;
             *reinterpret_cast<float4*>(to + h * DP + d) = acc;
             if (d == 0) {
                 to[K::kHeads * DP + h] = top;
@@ -935,23 +1027,16 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
         }
     }
 
-    // Join between CTAs.  Slot 0 is the end (or middle) of an item that began in an earlier CTA, slot 1 the start of one
-    // that ends in a later CTA; an item's CTAs are first .. last.  More than kJoin of them join in groups, then the groups.
-    Part open[2] = {sh.part[sh.lead[0]], sh.part[sh.lead[joined - 1]]};
-    bool is_open[2] = {open[0].ta > 0, false};
-    {
-        int k = kParts - 1;
-        while (sh.part[k].start < 0) --k;
-        is_open[1] = open[1].ta == 0 && sh.part[k].tb < open[1].nt;
-    }
+    // Join between CTAs: the last of an item's CTAs to arrive does it.  More than kJoin join in groups, then the groups.
+    const Joined open[2] = {sh.joined[0], sh.joined[joined - 1]};
+    const bool is_open[2] = {open[0].slot == 0, open[1].slot == 1};
     if (!is_open[0] && !is_open[1]) return;
     int32_t first[2], last[2], size[2];
 #pragma unroll
     for (int slot = 0; slot < 2; ++slot) {
         if (!is_open[slot]) continue;
-        const int64_t tile = open[slot].start;
-        first[slot] = static_cast<int32_t>(((tile + 1) * workers - 1) / total) / K::kTeams;
-        last[slot] = static_cast<int32_t>(((tile + open[slot].nt) * workers - 1) / total) / K::kTeams;
+        first[slot] = by_cta.part_of(open[slot].start);
+        last[slot] = by_cta.part_of(open[slot].start + open[slot].nt - 1);
         const int32_t n = last[slot] - first[slot] + 1;
         size[slot] = n <= kJoin ? n : max(12, (n + kJoin - 1) / kJoin);
     }
@@ -969,7 +1054,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
 #pragma unroll
     for (int slot = 0; slot < 2; ++slot) {
         if (!is_open[slot] || !sh.won[slot]) continue;
-        const Part& p = open[slot];
+        const Joined& p = open[slot];
         const int32_t at = (static_cast<int32_t>(blockIdx.x) - first[slot]) / size[slot];
         const int32_t lo = first[slot] + at * size[slot], n = min(size[slot], last[slot] - lo + 1);
         const int32_t groups = (last[slot] - first[slot]) / size[slot] + 1;
@@ -977,8 +1062,8 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
         // have its first group), is its own result
         if (groups == 1 || n > 1) {
             const float* parts = a.cta_part + lo * kCta;
-            join_parts<K>(a, sh, parts, kCta, parts + (lo == first[slot] ? K::kPart : 0), parts + (n - 1) * kCta, n, p.r,
-                          p.item, groups == 1 ? nullptr : a.cta_part + lo * kCta + 2 * K::kPart, DP);
+            join_parts<K, DP>(a, sh, smem, parts, kCta, parts + (lo == first[slot] ? K::kPart : 0), parts + (n - 1) * kCta, n, p,
+                              groups == 1 ? nullptr : a.cta_part + lo * kCta + 2 * K::kPart);
         }
         if (groups == 1) continue;
         if (tid == 0) sh.won[slot] = arrive_last(a.tickets + gridDim.x + first[slot], groups);
@@ -986,8 +1071,8 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
         if (!sh.won[slot]) continue;
         const float* heads = a.cta_part + first[slot] * kCta + 2 * K::kPart;
         const int32_t in_last = (last[slot] - first[slot]) % size[slot] + 1;
-        const float* end = a.cta_part + (last[slot] - in_last + 1) * kCta + (in_last == 1 ? 0 : 2 * K::kPart);
-        join_parts<K>(a, sh, heads, kCta * size[slot], heads, end, groups, p.r, p.item, nullptr, DP);
+        const float* tail = a.cta_part + (last[slot] - in_last + 1) * kCta + (in_last == 1 ? 0 : 2 * K::kPart);
+        join_parts<K, DP>(a, sh, smem, heads, kCta * size[slot], heads, tail, groups, p, nullptr);
     }
 }
 
@@ -1117,9 +1202,9 @@ extern "C" int mf_paged_attn_create(const mf_paged_attn_config* config, mf_paged
     a.table_stride = c.table_stride;
     a.n_pages = static_cast<uint32_t>(k.n_pages < 0x7fffffff ? k.n_pages : 0x7fffffff);
     a.q_heads = c.q_heads;
-    a.kv_heads = k.kv_heads;
     a.group = group;
-    a.blocks = (group + (group <= 8 ? 7 : 15)) / (group <= 8 ? 8 : 16);
+    a.blocks = group <= 8 ? 1 : (group + 15) / 16;
+    a.items = k.kv_heads * a.blocks;
     a.head_dim = k.head_dim;
     a.page = k.page_size;
     a.max_pages = c.max_pages;
@@ -1152,13 +1237,13 @@ extern "C" int mf_paged_attn_run(mf_paged_attn handle, const void* q, const void
     if (reinterpret_cast<uintptr_t>(q) % 4 || reinterpret_cast<uintptr_t>(out) % 8)
         return fail(MF_ERR_LAYOUT_UNSUPPORTED, "mf_paged_attn_run: q must be 4-byte and out 8-byte aligned");
     AttnArgs a = handle->args;
-    a.q = q;
-    a.k = k_cache;
-    a.v = v_cache;
+    a.q = static_cast<const char*>(q);
+    a.k = static_cast<const char*>(k_cache);
+    a.v = static_cast<const char*>(v_cache);
     a.table = table;
     a.lens = lens;
     a.n_requests = n_requests;
-    a.out = out;
+    a.out = static_cast<char*>(out);
     a.lse = lse;
     handle->kernel.fn<<<static_cast<unsigned>(handle->ctas), handle->kernel.threads, handle->kernel.shared,
                         static_cast<cudaStream_t>(stream)>>>(a);
