@@ -34,7 +34,6 @@
 // result does not depend on who was last.
 #include <new>
 
-#include "mf_async.cuh"
 #include "mf_runtime.h"
 #include "mf_vec.cuh"
 
@@ -56,6 +55,7 @@ struct AttnArgs {
     int32_t page_bytes, row_bytes;
     int64_t head_bytes, table_stride;
     uint32_t n_pages;
+    uint32_t page_mul, page_shift;  // x / page = (mulhi(x, page_mul) + x) >> page_shift for x below 2^31
     int32_t head_dim;
     const char* q;
     int64_t q_req, q_head;
@@ -100,9 +100,20 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
-template <bool BF16>
+// c = a b (FIRST) or c += a b, 16 x 16 by 16 x 8.
+template <bool BF16, bool FIRST = false>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    if constexpr (BF16)
+    if constexpr (FIRST && BF16)
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+    else if constexpr (FIRST)
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+    else if constexpr (BF16)
         asm volatile(
             "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -140,11 +151,27 @@ __device__ __forceinline__ void team_sync(int team) {
     if constexpr (TM == 1) __syncwarp();
     else asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(32 * TM) : "memory");
 }
-// Two FP8 codes -> f16x2, exact.
+// Four FP8 codes -> two f16x2, exact: codes 0, 1 and codes 2, 3.
 template <int DT>
-__device__ __forceinline__ uint32_t fp8x2_to_f16x2(uint32_t two) {
-    if constexpr (DT == MF_DT_F8E4M3) return e4m3x2_to_f16x2(two);
-    else return __byte_perm(two, 0u, 0x1404u);
+__device__ __forceinline__ void fp8x4_to_f16(uint32_t four, uint32_t& low, uint32_t& high) {
+    if constexpr (DT == MF_DT_F8E4M3) {
+        asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+            : "=r"(low), "=r"(high)
+            : "r"(four));
+    } else {
+        low = __byte_perm(four, 0u, 0x1404u);
+        high = __byte_perm(four, 0u, 0x3424u);
+    }
+}
+// The same for codes 0, 2 and codes 1, 3.
+template <int DT>
+__device__ __forceinline__ void fp8x4_to_f16_strided(uint32_t four, uint32_t& even, uint32_t& odd) {
+    if constexpr (DT == MF_DT_F8E4M3) {
+        fp8x4_to_f16<DT>(__byte_perm(four, 0u, 0x3120u), even, odd);
+    } else {
+        even = __byte_perm(four, 0u, 0x2404u);
+        odd = __byte_perm(four, 0u, 0x3414u);
+    }
 }
 // exp2(m_old - m_new) for m_old <= m_new, 1 where both are the same infinity.
 __device__ __forceinline__ float rescale(float m_old, float m_new) {
@@ -230,10 +257,6 @@ constexpr int kJoin = 16;  // most parts that one step of a join between CTAs ta
 // A maximum is only replaced by one that is this much larger (in powers of two): until then the weights grow up to
 // 2^8, which float32 sums and both terms of a weight hold as well, and what is summed is not rescaled.
 constexpr float kLazy = 8.0f;
-// A warp waits for the others of its CTA when it is this many tiles ahead.  Their loads queue for the same HBM, so
-// those that lag get what the waiting one leaves, and all end together: without it the warps of a CTA ended 12% apart.
-constexpr int kAhead = 2;
-
 // MODE: dtype of the cache; DP: head_dim padded to 64, 128 or 256; TM: warps of a team; W: warps; T: tokens of a
 // tile; S: stages of a team's ring.  A team works on one item at a time, each of its warps for 8 query heads.
 template <int MODE, int DP, int TM, int W, int T, int S>
@@ -242,7 +265,7 @@ struct Attn {
     static constexpr bool kBf16 = MODE == MF_DT_BF16;
     static constexpr int kBytes = kFp8 ? 1 : 2;
     static constexpr int kRow = DP * kBytes;          // bytes of a token's row
-    static constexpr int kChunks = kRow / 16;         // 16-byte pieces of a row
+    static constexpr int kChunks = kRow / 16;         // 16-byte pieces of it
     static constexpr int kStage = 2 * T * kRow;       // keys, then values
     static constexpr int kBlocks = T / kBlock;
     static constexpr uint32_t kAll = T == 32 ? 0xffffffffu : 0xffffu;  // every token of a tile
@@ -262,7 +285,6 @@ struct Attn {
     static_assert(W >= 2 && (T == kBlock || T == 2 * kBlock), "");
 
     struct Shared {
-        uint64_t step[4];               // all warps are done with a tile
         int64_t warp_sum[32];           // tiles of the requests of each warp's threads
         int32_t thread_sum[kThreads];   // and of each thread's
         Part part[2 * kTeams];          // first and last part of each team
@@ -278,7 +300,10 @@ struct Attn {
 };
 
 // Piece `c` of row `row` of a tile: the pieces of a row are exchanged so that
-// eight rows of one column fall on different banks.
+// eight rows of one column fall on different banks.  (Rows 16 bytes longer
+// than they are do that too, and need no exclusive-or, but then the 32-byte
+// sectors of a copy cross those of shared memory: 102 instead of 92 us for 64
+// requests of 2048 tokens, 32/8 heads of 128.)
 template <int CHUNKS>
 __device__ __forceinline__ uint32_t swizzled(int row, int c) {
     if constexpr (CHUNKS >= 8) return static_cast<uint32_t>(row * CHUNKS + (c ^ (row & 7))) * 16u;
@@ -439,7 +464,6 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
         if (lane == 0) sh.warp_sum[warp] = (high << 16) + low;
     }
     if (tid < 2 * K::kTeams) sh.part[tid].start = -1;
-    if (tid < 4) mbar_init(&sh.step[tid], W);
     if (__syncthreads_or(empty)) {
         // requests that see nothing
         for (int32_t r = blockIdx.x; r < a.n_requests; r += gridDim.x) {
@@ -522,7 +546,8 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
         const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(my_ring));
         Place<T> load = at;
         int32_t to_load = my_tiles;
-        const bool whole = a.page % kBlock == 0;  // a block lies in one page
+        const bool whole = a.page % kBlock == 0;         // a block lies in one page
+        const bool dense = a.row_bytes == DP * K::kBytes;  // rows follow one another
         constexpr int kRows = 32 / K::kChunks > 0 ? 32 / K::kChunks : 1;  // rows that one instruction copies
         constexpr int kCopies = kBlock * K::kChunks / 32 / TM;            // of a block, by one warp
         static_assert(kCopies > 0, "");
@@ -530,40 +555,43 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
         const int64_t lane_bytes = static_cast<int64_t>(piece_row) * a.row_bytes + piece * 16;
         const bool piece_in = piece * (16 / K::kBytes) < a.head_dim;
         const int64_t kv_gap = a.v - a.k;
+        const int32_t lane_tok = whole ? 0 : lane & (T - 1);
         // of the blocks of the tile at `load` (or, blocks not being whole, of this lane's row): their pages, the pages'
-        // places in the table's row and the blocks' in the pages
-        const int32_t* table_row = nullptr;
+        // entries in the table and the blocks' places in the pages
         const char* head_at = nullptr;
-        int32_t page_no[K::kBlocks], page_idx[K::kBlocks], page_off[K::kBlocks];
+        const int32_t* entry[K::kBlocks];
+        int32_t page_no[K::kBlocks], page_off[K::kBlocks], tok0 = 0;
         auto look_up = [&](bool new_item) {
-            if (to_load == 0) return;
             if (new_item) {
-                table_row = a.table + load.r * a.table_stride;
+                tok0 = load.span.base + load.t * T;
                 head_at = a.k + (a.blocks == 1 ? load.item : load.item / a.blocks) * a.head_bytes + lane_bytes;
+            } else {
+                tok0 += T;
             }
 #pragma unroll
             for (int b = 0; b < K::kBlocks; ++b) {
-                const int32_t tok = load.span.base + load.t * T + (whole ? b * kBlock : lane & (T - 1));
+                const int32_t tok = tok0 + lane_tok + (whole ? b * kBlock : 0);
                 if (new_item || !whole) {
-                    page_idx[b] = static_cast<int32_t>(static_cast<uint32_t>(tok) / static_cast<uint32_t>(a.page));
-                    page_off[b] = tok - page_idx[b] * a.page;
+                    const uint32_t x = static_cast<uint32_t>(tok);
+                    const int32_t idx = static_cast<int32_t>((__umulhi(x, a.page_mul) + x) >> a.page_shift);
+                    page_off[b] = tok - idx * a.page;
+                    entry[b] = a.table + load.r * a.table_stride + idx;
                 } else {
                     page_off[b] += T;
 #pragma unroll
                     for (int x = 0; x < K::kBlocks; ++x)
                         if (page_off[b] >= a.page) {
                             page_off[b] -= a.page;
-                            ++page_idx[b];
+                            ++entry[b];
                         }
                 }
-                if (tok < load.span.len) page_no[b] = __ldg(table_row + page_idx[b]);
+                if (tok < load.span.len) page_no[b] = __ldg(entry[b]);
             }
         };
         uint32_t partial = 0;  // stages that lack some of their tokens: those have a mask
         auto issue = [&](int stage) {
             if (to_load > 0) {
-                const int32_t tok0 = load.span.base + load.t * T;
-                const uint32_t dst = ring + stage * K::kStage;
+                const uint32_t to = ring + stage * K::kStage;
                 bool ok[K::kBlocks], all = whole && tok0 >= load.span.first && tok0 + T <= load.span.len;
                 int64_t at_block[K::kBlocks];
 #pragma unroll
@@ -577,12 +605,20 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
 #pragma unroll
                     for (int b = 0; b < K::kBlocks; ++b) {
                         const char* kp = head_at + at_block[b];
+                        const char* vp = kp + kv_gap;
+                        if (piece_in && dense) {
 #pragma unroll
-                        for (int i = 0; i < kCopies; ++i, kp += kRows * a.row_bytes) {
-                            const uint32_t to = dst + b * kBlock * K::kRow + swizzled<K::kChunks>(i * kRows + piece_row, piece);
-                            if (piece_in) {
-                                cp_async16(to, kp, 16u);
-                                cp_async16(to + T * K::kRow, kp + kv_gap, 16u);
+                            for (int i = 0; i < kCopies; ++i) {
+                                const uint32_t dst = to + b * kBlock * K::kRow + swizzled<K::kChunks>(i * kRows + piece_row, piece);
+                                cp_async16(dst, kp + i * (kRows * DP * K::kBytes), 16u);
+                                cp_async16(dst + T * K::kRow, vp + i * (kRows * DP * K::kBytes), 16u);
+                            }
+                        } else if (piece_in) {
+#pragma unroll
+                            for (int i = 0; i < kCopies; ++i) {
+                                const uint32_t dst = to + b * kBlock * K::kRow + swizzled<K::kChunks>(i * kRows + piece_row, piece);
+                                cp_async16(dst, kp + i * kRows * a.row_bytes, 16u);
+                                cp_async16(dst + T * K::kRow, vp + i * kRows * a.row_bytes, 16u);
                             }
                         }
                     }
@@ -597,20 +633,23 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                     partial = (partial & ~(1u << stage)) | (mask != K::kAll ? 1u << stage : 0u);
                     if (lane == 0) sh.mask[team][stage] = mask;
                     const int64_t row = (mine == 0 ? at_block[0] : at_block[K::kBlocks - 1]) + (whole ? (lane & (kBlock - 1)) * a.row_bytes : 0);
-#pragma unroll 1
+                    const char* base = head_at - static_cast<int64_t>(piece_row) * a.row_bytes;
+#pragma unroll 2
                     for (int i = 0; i < K::kBlocks * kCopies; ++i) {
-                        const int rw = i / kCopies * kBlock + i % kCopies * kRows + piece_row;
-                        const int64_t row_at = __shfl_sync(0xffffffffu, row, rw) - static_cast<int64_t>(piece_row) * a.row_bytes;
-                        const bool get = piece_in && ((mask >> rw) & 1u);
-                        const char* kp = get ? head_at + row_at : a.k;
-                        const uint32_t to = dst + swizzled<K::kChunks>(rw, piece);
-                        cp_async16(to, kp, get ? 16u : 0u);
-                        cp_async16(to + T * K::kRow, kp + kv_gap, get ? 16u : 0u);
+                        const int at_row = i / kCopies * kBlock + i % kCopies * kRows, rw = at_row + piece_row;
+                        const char* kp = base + __shfl_sync(0xffffffffu, row, rw);
+                        const bool get = (mask >> rw) & 1u;
+                        if (piece_in) {
+                            const uint32_t dst = to + swizzled<K::kChunks>(rw, piece);
+                            cp_async16(dst, get ? kp : a.k, get ? 16u : 0u);
+                            cp_async16(dst + T * K::kRow, get ? kp + kv_gap : a.k, get ? 16u : 0u);
+                        }
                     }
                 }
-                load.next(a, items);
-                --to_load;
-                look_up(load.t == 0);
+                if (--to_load > 0) {
+                    load.next(a, items);
+                    look_up(load.t == 0);
+                }
             }
             cp_async_commit();
         };
@@ -641,23 +680,16 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
         // rows of this lane in the loads of a product's operands
         const int k_row = (lane & 7) + ((lane >> 3) & 1) * 8, k_piece = lane >> 4;
         const int v_row = K::kFp8 ? k_row : (lane & 7) + (lane >> 4) * 8, v_piece = K::kFp8 ? k_piece : (lane >> 3) & 1;
-        const uint32_t k_at = swizzled<K::kChunks>(k_row, k_piece);
-        const uint32_t v_at = swizzled<K::kChunks>(v_row, v_piece) + T * K::kRow;
+        const uint32_t k_at = ring + swizzled<K::kChunks>(k_row, k_piece);
+        const uint32_t v_at = ring + T * K::kRow + swizzled<K::kChunks>(v_row, v_piece);
         const bool rules = a.softcap > 0.0f || a.slopes;
-        float scale[2] = {0.0f, 0.0f}, slope[2] = {0.0f, 0.0f};
-        int32_t ta = at.t;
         int stage = 0;
-        const int32_t common = by_team.q;  // tiles that every team of the CTA has
-#pragma unroll 1
-        for (int32_t i = 0; i < my_tiles; ++i) {
-            if (i >= kAhead && i - kAhead < common && !mbar_wait(&sh.step[(i - kAhead) & 3], ((i - kAhead) >> 2) & 1))
-                atomicExch(a.status, MF_DEVICE_TIMEOUT);  // the results do not depend on it
-            cp_async_wait<S - 2>();
-            team_sync<TM>(team);
-            issue(stage == 0 ? S - 1 : stage - 1);
-            if (i == 0 || at.t == 0) {
+        int32_t done = 0;
+        while (done < my_tiles) {
+            const int32_t ta = at.t, tb = min(at.nt, ta + my_tiles - done);
+            float scale[2], slope[2], less[2], high[2];  // less: m, or 0 while it is -inf; high: what raises the maximum
+            {
                 // a new item; its queries were loaded while the one before it ended
-                ta = at.t;
                 const Heads<K::kHeads> hd(a, at.item);
                 float back = 1.0f;
                 if constexpr (K::kFp8) {
@@ -698,8 +730,8 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                     scale[x] = a.scale * ks * b;
                     scale[x] = a.softcap > 0.0f ? __fdiv_rn(scale[x], a.softcap) : scale[x] * kLog2e;
                     slope[x] = a.slopes && hx < hd.count ? __ldg(a.slopes + hd.head0 + hx) * kLog2e : 0.0f;
-                    m[x] = -INFINITY;
-                    l[x] = 0.0f;
+                    m[x] = high[x] = -INFINITY;
+                    less[x] = l[x] = 0.0f;
                 }
 #pragma unroll
                 for (int c = 0; c < K::kSteps; ++c)
@@ -707,138 +739,149 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                     for (int x = 0; x < 4; ++x) o[c][x] = 0.0f;
             }
 
-            // S^T = K Q^T, two chains of sums
-            const uint32_t keys = ring + stage * K::kStage + k_at, values = ring + stage * K::kStage + v_at;
-            const uint32_t mask = (partial >> stage) & 1u ? sh.mask[team][stage] : K::kAll;
-            const bool ends = at.t + 1 == at.nt, stops = i + 1 == my_tiles;  // the item's last tile, or this team's
-            float s[K::kBlocks][2][4];
+#pragma unroll 1
+            for (int32_t t = ta; t < tb; ++t) {
+                cp_async_wait<S - 2>();
+                team_sync<TM>(team);
+                issue(stage == 0 ? S - 1 : stage - 1);
+
+                // S^T = K Q^T, two chains of sums
+                const uint32_t keys = k_at + stage * K::kStage, values = v_at + stage * K::kStage;
+                const uint32_t mask = (partial >> stage) & 1u ? sh.mask[team][stage] : K::kAll;
+                float s[K::kBlocks][2][4];
 #pragma unroll
-            for (int b = 0; b < K::kBlocks; ++b) {
+                for (int b = 0; b < K::kBlocks; ++b) {
+                    const uint32_t rows = keys + b * kBlock * K::kRow;
+                    if constexpr (!K::kFp8) {
 #pragma unroll
-                for (int x = 0; x < 4; ++x) s[b][0][x] = s[b][1][x] = 0.0f;
-                const uint32_t rows = keys + b * kBlock * K::kRow;
-                if constexpr (!K::kFp8) {
+                        for (int c = 0; c < K::kSteps; ++c) {
+                            uint32_t f[4];
+                            ldsm4(f, pieces_on<K::kChunks>(rows, 2 * c));
+                            if (c < 2) mma16816<K::kBf16, true>(s[b][c & 1], f, qf[c][0], qf[c][1]);
+                            else mma16816<K::kBf16>(s[b][c & 1], f, qf[c][0], qf[c][1]);
+                        }
+                    } else {
 #pragma unroll
-                    for (int c = 0; c < K::kSteps; ++c) {
-                        uint32_t f[4];
-                        ldsm4(f, pieces_on<K::kChunks>(rows, 2 * c));
-                        mma16816<K::kBf16>(s[b][c & 1], f, qf[c][0], qf[c][1]);
-                    }
-                } else {
+                        for (int c = 0; c < K::kSteps; c += 2) {
+                            uint32_t f[4];
+                            ldsm4(f, pieces_on<K::kChunks>(rows, c));
 #pragma unroll
-                    for (int c = 0; c < K::kSteps; c += 2) {
-                        uint32_t f[4];
-                        ldsm4(f, pieces_on<K::kChunks>(rows, c));
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            // four codes of a row: elements 4j, 4j+1 take the place of the product's 2j, 2j+1,
-                            // elements 4j+2, 4j+3 that of 2j+8, 2j+9 (the queries are laid out alike)
-                            const uint32_t f16[4] = {
-                                fp8x2_to_f16x2<MODE>(f[2 * x]), fp8x2_to_f16x2<MODE>(f[2 * x + 1]),
-                                fp8x2_to_f16x2<MODE>(f[2 * x] >> 16), fp8x2_to_f16x2<MODE>(f[2 * x + 1] >> 16)};
-                            mma16816<false>(s[b][x], f16, qf[c + x][0], qf[c + x][1]);
+                            for (int x = 0; x < 2; ++x) {
+                                // four codes of a row: elements 4j, 4j+1 take the place of the product's 2j, 2j+1,
+                                // elements 4j+2, 4j+3 that of 2j+8, 2j+9 (the queries are laid out alike)
+                                uint32_t f16[4];
+                                fp8x4_to_f16<MODE>(f[2 * x], f16[0], f16[2]);
+                                fp8x4_to_f16<MODE>(f[2 * x + 1], f16[1], f16[3]);
+                                if (c == 0) mma16816<false, true>(s[b][x], f16, qf[c + x][0], qf[c + x][1]);
+                                else mma16816<false>(s[b][x], f16, qf[c + x][0], qf[c + x][1]);
+                            }
                         }
                     }
                 }
-            }
-            Place<T> following = at;
-            following.next(a, items);
-            if (ends && !stops) load_queries(following);
-
-            // scores of tokens g and g + 8 of each block, heads 2j and 2j + 1, times log2(e)
-            float p[K::kBlocks][4], top[2] = {-INFINITY, -INFINITY};
+                // scores of tokens g and g + 8 of each block, heads 2j and 2j + 1, times log2(e)
+                float p[K::kBlocks][4], top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-            for (int b = 0; b < K::kBlocks; ++b) {
+                for (int b = 0; b < K::kBlocks; ++b) {
 #pragma unroll
-                for (int x = 0; x < 4; ++x) p[b][x] = (s[b][0][x] + s[b][1][x]) * scale[x & 1];
-                if (rules) {
-                    // distance to the newest token, <= 0
-                    const float away = static_cast<float>(at.span.base + at.t * T + b * kBlock + g - (at.span.len - 1));
+                    for (int x = 0; x < 4; ++x) p[b][x] = (s[b][0][x] + s[b][1][x]) * scale[x & 1];
+                    if (rules) {
+                        // distance to the newest token, <= 0
+                        const float away = static_cast<float>(at.span.base + t * T + b * kBlock + g - (at.span.len - 1));
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            if (a.softcap > 0.0f) p[b][x] = a.softcap * kLog2e * tanh_fast(p[b][x]);
+                            p[b][x] = __fmaf_rn(slope[x & 1], away + (x & 2 ? 8.0f : 0.0f), p[b][x]);
+                        }
+                    }
+                    if (mask != K::kAll) {
+#pragma unroll
+                        for (int x = 0; x < 4; ++x)
+                            p[b][x] = (mask >> (b * kBlock + (x & 2 ? g + 8 : g))) & 1u ? p[b][x] : -INFINITY;
+                    }
+                    top[0] = fmaxf(top[0], fmaxf(p[b][0], p[b][2]));
+                    top[1] = fmaxf(top[1], fmaxf(p[b][1], p[b][3]));
+                }
+                if (__any_sync(0xffffffffu, top[0] > high[0] || top[1] > high[1])) {
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 4));
+                        top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 8));
+                        top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 16));
+                        top[x] = fmaxf(top[x], m[x]);
+                        const float r = rescale(m[x], top[x]);
+                        m[x] = top[x];
+                        high[x] = top[x] + kLazy;
+                        less[x] = top[x] == -INFINITY ? 0.0f : top[x];
+                        l[x] *= r;
+#pragma unroll
+                        for (int c = 0; c < K::kSteps; ++c) {
+                            o[c][x] *= r;
+                            o[c][x + 2] *= r;
+                        }
+                    }
+                }
+                // weights; while nothing is seen, the maximum is -inf and so are the scores: weights of 0
+                uint32_t ph[K::kBlocks][2], pl[K::kBlocks][2];
+#pragma unroll
+                for (int b = 0; b < K::kBlocks; ++b) {
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
-                        if (a.softcap > 0.0f) p[b][x] = a.softcap * kLog2e * tanh_fast(p[b][x]);
-                        p[b][x] = __fmaf_rn(slope[x & 1], away + (x & 2 ? 8.0f : 0.0f), p[b][x]);
+                        p[b][x] = exp2_fast(p[b][x] - less[x & 1]);
+                        l[x & 1] += p[b][x];
+                    }
+                    // high and low terms, tokens x heads -> heads x tokens
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const uint32_t high = pack2<K::kBf16>(p[b][2 * x], p[b][2 * x + 1]);
+                        float f0, f1;
+                        unpack2<K::kBf16>(high, f0, f1);
+                        ph[b][x] = transpose8x8(high);
+                        pl[b][x] = transpose8x8(pack2<K::kBf16>(p[b][2 * x] - f0, p[b][2 * x + 1] - f1));
                     }
                 }
-                if (mask != K::kAll) {
-#pragma unroll
-                    for (int x = 0; x < 4; ++x)
-                        p[b][x] = (mask >> (b * kBlock + (x & 2 ? g + 8 : g))) & 1u ? p[b][x] : -INFINITY;
-                }
-                top[0] = fmaxf(top[0], fmaxf(p[b][0], p[b][2]));
-                top[1] = fmaxf(top[1], fmaxf(p[b][1], p[b][3]));
-            }
-            if (__any_sync(0xffffffffu, top[0] > m[0] + kLazy || top[1] > m[1] + kLazy)) {
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 4));
-                    top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 8));
-                    top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 16));
-                    top[x] = fmaxf(top[x], m[x]);
-                    const float r = rescale(m[x], top[x]);
-                    m[x] = top[x];
-                    l[x] *= r;
-#pragma unroll
-                    for (int c = 0; c < K::kSteps; ++c) {
-                        o[c][x] *= r;
-                        o[c][x + 2] *= r;
-                    }
-                }
-            }
-            // weights; while nothing is seen, the maximum is -inf and so are the scores: weights of 0
-            const float less[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
-            uint32_t ph[K::kBlocks][2], pl[K::kBlocks][2];
-#pragma unroll
-            for (int b = 0; b < K::kBlocks; ++b) {
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    p[b][x] = exp2_fast(p[b][x] - less[x & 1]);
-                    l[x & 1] += p[b][x];
-                }
-                // high and low terms, tokens x heads -> heads x tokens
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const uint32_t high = pack2<K::kBf16>(p[b][2 * x], p[b][2 * x + 1]);
-                    float f0, f1;
-                    unpack2<K::kBf16>(high, f0, f1);
-                    ph[b][x] = transpose8x8(high);
-                    pl[b][x] = transpose8x8(pack2<K::kBf16>(p[b][2 * x] - f0, p[b][2 * x + 1] - f1));
-                }
-            }
 
-            // O^T += V^T P^T
+                // O^T += V^T P^T
 #pragma unroll
-            for (int b = 0; b < K::kBlocks; ++b) {
-                const uint32_t rows = values + b * kBlock * K::kRow;
-                if constexpr (!K::kFp8) {
+                for (int b = 0; b < K::kBlocks; ++b) {
+                    const uint32_t rows = values + b * kBlock * K::kRow;
+                    if constexpr (!K::kFp8) {
 #pragma unroll
-                    for (int c = 0; c < K::kSteps; ++c) {
-                        uint32_t f[4];
-                        ldsm4_t(f, pieces_on<K::kChunks>(rows, 2 * c));
-                        mma16816<K::kBf16>(o[c], f, ph[b][0], ph[b][1]);
-                        mma16816<K::kBf16>(o[c], f, pl[b][0], pl[b][1]);
-                    }
-                } else {
+                        for (int c = 0; c < K::kSteps; ++c) {
+                            uint32_t f[4];
+                            ldsm4_t(f, pieces_on<K::kChunks>(rows, 2 * c));
+                            mma16816<K::kBf16>(o[c], f, ph[b][0], ph[b][1]);
+                            mma16816<K::kBf16>(o[c], f, pl[b][0], pl[b][1]);
+                        }
+                    } else {
 #pragma unroll
-                    for (int c = 0; c < K::kSteps; c += 2) {
-                        uint32_t f[4];
-                        ldsm4_t(f, pieces_on<K::kChunks>(rows, c));
+                        for (int c = 0; c < K::kSteps; c += 2) {
+                            uint32_t f[4];
+                            ldsm4_t(f, pieces_on<K::kChunks>(rows, c));
 #pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            // a transposed pair of bytes holds elements 2g, 2g+1 of two tokens: row g of the product
-                            // is element 2g, row g + 8 element 2g + 1
-                            const uint32_t u = f[2 * x], w = f[2 * x + 1];
-                            const uint32_t f16[4] = {
-                                fp8x2_to_f16x2<MODE>(__byte_perm(u, 0u, 0x4420u)), fp8x2_to_f16x2<MODE>(__byte_perm(u, 0u, 0x4431u)),
-                                fp8x2_to_f16x2<MODE>(__byte_perm(w, 0u, 0x4420u)), fp8x2_to_f16x2<MODE>(__byte_perm(w, 0u, 0x4431u))};
-                            mma16816<false>(o[c + x], f16, ph[b][0], ph[b][1]);
-                            mma16816<false>(o[c + x], f16, pl[b][0], pl[b][1]);
+                            for (int x = 0; x < 2; ++x) {
+                                // a transposed pair of bytes holds elements 2g, 2g+1 of two tokens: row g of the product
+                                // is element 2g, row g + 8 element 2g + 1
+                                uint32_t f16[4];
+                                fp8x4_to_f16_strided<MODE>(f[2 * x], f16[0], f16[1]);
+                                fp8x4_to_f16_strided<MODE>(f[2 * x + 1], f16[2], f16[3]);
+                                mma16816<false>(o[c + x], f16, ph[b][0], ph[b][1]);
+                                mma16816<false>(o[c + x], f16, pl[b][0], pl[b][1]);
+                            }
                         }
                     }
                 }
-            }
 
-            if (ends || stops) {
+                stage = stage + 1 == S ? 0 : stage + 1;
+            }
+            done += tb - ta;
+            Place<T> following = at;
+            following.t = tb - 1;
+            const bool ends = tb == at.nt, stops = done == my_tiles;  // the item, this team's run
+            if (!stops) {
+                following.next(a, items);
+                load_queries(following);
+            }
+            {
                 const bool all_of_it = ends && ta == 0;
                 const Heads<K::kHeads> hd(a, at.item);
 #pragma unroll
@@ -897,17 +940,15 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                 }
                 if (!all_of_it && lane == 0 && member == 0) {
                     Part& p = sh.part[2 * team + (stops ? 1 : 0)];
-                    p.start = x0 + i - at.t;
+                    p.start = x0 + done - tb;
                     p.r = at.r;
                     p.item = at.item;
                     p.nt = at.nt;
                     p.ta = ta;
-                    p.tb = at.t + 1;
+                    p.tb = tb;
                 }
             }
-            if (lane == 0 && i < common) mbar_arrive(&sh.step[i & 3]);
             at = following;
-            stage = stage + 1 == S ? 0 : stage + 1;
         }
         cp_async_wait<0>();
     }
@@ -1208,6 +1249,8 @@ extern "C" int mf_paged_attn_create(const mf_paged_attn_config* config, mf_paged
     a.head_dim = k.head_dim;
     a.page = k.page_size;
     a.max_pages = c.max_pages;
+    while ((1ull << a.page_shift) < static_cast<uint64_t>(a.page)) ++a.page_shift;
+    a.page_mul = static_cast<uint32_t>((((1ull << a.page_shift) - a.page) << 32) / a.page + 1);
     a.window = c.window;
     a.q_f16 = c.q_dtype == MF_DT_F16;
     a.scale = c.scale;
