@@ -10,6 +10,7 @@
 // units of 2 * VEC elements with all threads.  Bound: HBM, every element read
 // and written once; for the few tokens of a decoding step, the launch.
 #include <cmath>
+#include <initializer_list>
 
 #include "mf_runtime.h"
 #include "mf_vec.cuh"
@@ -24,23 +25,36 @@ constexpr int kRopeTableFloats = 2048;  // cosines and sines of a CTA's tokens: 
 struct RopeSegment {
     const void* src;
     void* dst;
-    int64_t src_token, src_head;
-    int64_t dst_token, dst_head;  // an array's strides; a cache's are in RopeArgs
+    int32_t src_token, src_head;
+    int32_t dst_token, dst_head;  // an array's strides; a cache's are in RopeArgs
     const float* scale_inv;
     int32_t heads;
     int32_t first;                // heads in front of this segment
     bool turns, cached;
 };
 
+// x / d = (mulhi(x, mul) + x) >> shift for x below 2^31: a division by a number
+// that only the host knows takes three instructions instead of twenty.
+struct Divisor {
+    uint32_t d, mul, shift;
+};
+Divisor divisor(int32_t d) {
+    Divisor v{static_cast<uint32_t>(d), 0, 0};
+    while ((1ull << v.shift) < v.d) ++v.shift;
+    v.mul = static_cast<uint32_t>((((1ull << v.shift) - v.d) << 32) / v.d + 1);
+    return v;
+}
+__device__ __forceinline__ uint32_t operator/(uint32_t x, const Divisor& v) { return (__umulhi(x, v.mul) + x) >> v.shift; }
+
 struct RopeArgs {
     RopeSegment seg[3];
+    Divisor per_token, units, half;  // units of a token and of a head, rotated pairs
     const float* inv_freq;
     const int32_t* positions;
     const int64_t* slots;
-    int64_t tokens;
     int64_t cache_slots, page_stride, token_stride, head_stride;
     int32_t* status;
-    int32_t n_seg, heads, head_dim, rot, page_size, tokens_per_cta;
+    int32_t tokens, n_seg, heads, head_dim, rot, page_size, tokens_per_cta;
     int32_t interleaved, inverse, compat;
     float magnitude;
 };
@@ -74,6 +88,29 @@ __device__ __forceinline__ void load_n(const void* p, int64_t i, float (&v)[N]) 
     }
 }
 
+// N elements of v as stored in DT.  A sum of all of them is not a number when
+// one of them is not (or when infinities meet): only then does each element
+// take the encoder's rule for NaN.
+template <int DT, int N>
+__device__ __forceinline__ void encode_n(const float (&v)[N], uint32_t* w, int compat) {
+    if constexpr (DT == MF_DT_BF16 || DT == MF_DT_F16) {
+        float all = v[0];
+#pragma unroll
+        for (int k = 1; k < N; ++k) all += v[k];
+        if (all == all) {
+#pragma unroll
+            for (int k = 0; k < N; k += 2)
+                w[k / 2] = DT == MF_DT_BF16 ? f32x2_to_bf16x2_nonan(v[k], v[k + 1]) : f32x2_to_f16x2_nonan(v[k], v[k + 1]);
+            return;
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < N / 4; ++q) {
+        const float f[4] = {v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+        encode4<DT>(f, w + q * dtype_bytes(DT), compat);
+    }
+}
+
 template <int DT, int N>
 __device__ __forceinline__ void store_n(void* p, int64_t i, const float (&v)[N], int compat) {
     char* at = static_cast<char*>(p) + i * dtype_bytes(DT);
@@ -82,11 +119,7 @@ __device__ __forceinline__ void store_n(void* p, int64_t i, const float (&v)[N],
     } else {
         constexpr int kWords = N * dtype_bytes(DT) / 4;
         uint32_t w[kWords];
-#pragma unroll
-        for (int q = 0; q < N / 4; ++q) {
-            const float f[4] = {v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
-            encode4<DT>(f, w + q * dtype_bytes(DT), compat);
-        }
+        encode_n<DT, N>(v, w, compat);
         if constexpr (kWords % 4 == 0) {
 #pragma unroll
             for (int k = 0; k < kWords / 4; ++k)
@@ -118,25 +151,26 @@ template <int IN, int CACHE, int VEC>
 __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a) {
     __shared__ __align__(16) float s_cos[kRopeTableFloats / 2];
     __shared__ __align__(16) float s_sin[kRopeTableFloats / 2];
-    const int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.tokens_per_cta;
-    const int n_tok = static_cast<int>(min(static_cast<int64_t>(a.tokens_per_cta), a.tokens - t0));
+    const int32_t t0 = static_cast<int32_t>(blockIdx.x * a.tokens_per_cta);
+    const int n_tok = min(a.tokens_per_cta, a.tokens - t0);
     const int half = a.rot >> 1;
     for (int i = threadIdx.x; i < n_tok * half; i += kRopeThreads) {
-        const float2 cs = turn_of(a.positions[t0 + i / half], a.inv_freq[i % half], a.magnitude, a.inverse);
+        const int tok = static_cast<uint32_t>(i) / a.half;
+        const float2 cs = turn_of(a.positions[t0 + tok], a.inv_freq[i - tok * half], a.magnitude, a.inverse);
         s_cos[i] = cs.x;
         s_sin[i] = cs.y;
     }
     __syncthreads();
-    const int units = (a.head_dim + 2 * VEC - 1) / (2 * VEC);  // per head; the last may be one element short (VEC 1)
-    const int per_token = a.heads * units;
+    // per head; the last may be one element short (VEC 1)
+    const int units = a.units.d, per_token = a.per_token.d;
     const int step = kRopeThreads * gridDim.y;
     for (int i = blockIdx.y * kRopeThreads + threadIdx.x; i < n_tok * per_token; i += step) {
-        const int tok = i / per_token, in_tok = i - tok * per_token;
-        int h = in_tok / units;
+        const int tok = static_cast<uint32_t>(i) / a.per_token, in_tok = i - tok * per_token;
+        int h = static_cast<uint32_t>(in_tok) / a.units;
         const int u = in_tok - h * units;
         const RopeSegment& g = a.seg[(a.n_seg > 1 && h >= a.seg[1].first) + (a.n_seg > 2 && h >= a.seg[2].first)];
         h -= g.first;
-        const int64_t t = t0 + tok;
+        const int32_t t = t0 + tok;
         // the two places of the unit
         const int e = u * 2 * VEC;
         const bool turning = g.turns && e < a.rot;
@@ -149,7 +183,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a) {
             eb = e + VEC;
         }
         const bool second = VEC > 1 || eb < a.head_dim;
-        const int64_t from = t * g.src_token + h * g.src_head;
+        const int64_t from = static_cast<int64_t>(t) * g.src_token + static_cast<int64_t>(h) * g.src_head;
         float x[VEC], y[VEC];
         load_n<IN, VEC>(g.src, from + ea, x);
         if (second) load_n<IN, VEC>(g.src, from + eb, y);
@@ -177,7 +211,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a) {
             }
         }
         if (!g.cached) {
-            const int64_t to = t * g.dst_token + h * g.dst_head;
+            const int64_t to = static_cast<int64_t>(t) * g.dst_token + static_cast<int64_t>(h) * g.dst_head;
             store_n<IN, VEC>(g.dst, to + ea, x, 0);
             if (second) store_n<IN, VEC>(g.dst, to + eb, y, 0);
             continue;
@@ -228,7 +262,8 @@ int check_rope(const char* name, const mf_rope_config* c, int64_t tokens) {
     if (c->layout != MF_ROPE_HALF && c->layout != MF_ROPE_INTERLEAVED)
         return fail(MF_ERR_INVALID_ARGUMENT, "%s: unknown layout %d", name, c->layout);
     if (c->rot_dim > 0 && !c->inv_freq) return fail(MF_ERR_INVALID_ARGUMENT, "%s: inv_freq is NULL", name);
-    if (tokens < 0) return fail(MF_ERR_SHAPE_INVALID, "%s: negative token count %lld", name, (long long)tokens);
+    if (tokens < 0 || tokens > 0x7fffffffll)
+        return fail(MF_ERR_SHAPE_INVALID, "%s: %lld tokens (0 to 2^31 - 1)", name, (long long)tokens);
     return MF_OK;
 }
 
@@ -240,20 +275,23 @@ int finish_and_launch(const char* name, RopeArgs& a, const mf_rope_config* c, in
     a.rot = c->rot_dim;
     a.interleaved = c->layout == MF_ROPE_INTERLEAVED;
     a.magnitude = c->magnitude;
-    const int64_t units = static_cast<int64_t>(a.heads) * ((a.head_dim + 2 * vec - 1) / (2 * vec));
+    const int per_head = (a.head_dim + 2 * vec - 1) / (2 * vec);
+    const int64_t units = static_cast<int64_t>(a.heads) * per_head;
+    a.per_token = divisor(static_cast<int32_t>(units));
+    a.units = divisor(per_head);
+    a.half = divisor(a.rot > 1 ? a.rot / 2 : 1);
     const int sms = state().sm_count;
     const int room = a.rot ? kRopeTableFloats / a.rot : 16;  // tokens whose cosines fit
     int per = 1;
     while (per * 2 <= room && per < 16 && a.tokens / (per * 2) >= 8ll * sms && per * units < 8 * kRopeThreads) per *= 2;
     a.tokens_per_cta = per;
-    const int64_t blocks = (a.tokens + per - 1) / per;
+    const int64_t blocks = (static_cast<int64_t>(a.tokens) + per - 1) / per;
     int64_t split = 1;
     if (blocks < sms) {
         split = (units + kRopeThreads - 1) / kRopeThreads;
         if (split > sms / blocks) split = sms / blocks;
         if (split < 1) split = 1;
     }
-    if (blocks > 0x7fffffffll) return fail(MF_ERR_SHAPE_INVALID, "%s: too many tokens (%lld)", name, (long long)a.tokens);
     const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(split));
     switch (c->dtype) {
     case MF_DT_F32:
@@ -276,6 +314,12 @@ int finish_and_launch(const char* name, RopeArgs& a, const mf_rope_config* c, in
     }
     MF_LAUNCH_CHECK(name);
     return MF_OK;
+}
+
+bool fits_int(std::initializer_list<int64_t> strides) {
+    for (int64_t s : strides)
+        if (s < -0x7fffffffll || s > 0x7fffffffll) return false;
+    return true;
 }
 
 // The widest access that the head's split allows (both parts whole units).
@@ -301,6 +345,8 @@ extern "C" int mf_rope(const mf_rope_config* config, int inverse, const void* sr
         return fail(MF_ERR_SHAPE_INVALID, "mf_rope: %d heads of %d elements", heads, config->head_dim);
     if (src == dst && (src_token_stride != dst_token_stride || src_head_stride != dst_head_stride))
         return fail(MF_ERR_LAYOUT_UNSUPPORTED, "mf_rope: in place needs equal strides");
+    if (!fits_int({src_token_stride, src_head_stride, dst_token_stride, dst_head_stride}))
+        return fail(MF_ERR_LAYOUT_UNSUPPORTED, "mf_rope: a stride is over 2^31 - 1 elements");
     const int bytes = dtype_bytes(config->dtype);
     int vec = 1;
     for (int v : {8, 4})
@@ -308,12 +354,13 @@ extern "C" int mf_rope(const mf_rope_config* config, int inverse, const void* sr
             fits_vec(v, bytes, dst, dst_token_stride, dst_head_stride))
             vec = v;
     RopeArgs a{};
-    a.seg[0] = RopeSegment{src, dst, src_token_stride, src_head_stride, dst_token_stride, dst_head_stride, nullptr,
-                           heads, 0, true, false};
+    auto stride = [](int64_t s) { return static_cast<int32_t>(s); };
+    a.seg[0] = RopeSegment{src, dst, stride(src_token_stride), stride(src_head_stride), stride(dst_token_stride),
+                           stride(dst_head_stride), nullptr, heads, 0, true, false};
     a.n_seg = 1;
     a.heads = heads;
     a.positions = positions;
-    a.tokens = tokens;
+    a.tokens = static_cast<int32_t>(tokens);
     a.inverse = inverse != 0;
     return finish_and_launch("mf_rope", a, config, MF_DT_INVALID, vec, static_cast<cudaStream_t>(stream));
 }
@@ -345,6 +392,9 @@ extern "C" int mf_rope_append(const mf_rope_append_config* config, const void* q
         return fail(MF_ERR_INVALID_ARGUMENT, "mf_rope_append: NULL buffer");
     if (q == q_out && c.q_heads > 0 && (c.q_token_stride != c.out_token_stride || c.q_head_stride != c.out_head_stride))
         return fail(MF_ERR_LAYOUT_UNSUPPORTED, "mf_rope_append: in place needs equal strides");
+    if (!fits_int({c.q_token_stride, c.q_head_stride, c.k_token_stride, c.k_head_stride, c.v_token_stride, c.v_head_stride,
+                   c.out_token_stride, c.out_head_stride}))
+        return fail(MF_ERR_LAYOUT_UNSUPPORTED, "mf_rope_append: a stride is over 2^31 - 1 elements");
     const int bytes = dtype_bytes(c.rope.dtype), code = dtype_bytes(cache.dtype);
     int vec = 1;
     for (int w : {8, 4})
@@ -357,17 +407,18 @@ extern "C" int mf_rope_append(const mf_rope_append_config* config, const void* q
             fits_vec(w, code, v_cache, cache.page_stride, cache.token_stride, cache.head_stride))
             vec = w;
     RopeArgs a{};
-    a.seg[0] = RopeSegment{q, q_out, c.q_token_stride, c.q_head_stride, c.out_token_stride, c.out_head_stride, nullptr,
-                           c.q_heads, 0, true, false};
-    a.seg[1] = RopeSegment{k, k_cache, c.k_token_stride, c.k_head_stride, 0, 0, c.k_scale_inv, cache.kv_heads, c.q_heads,
-                           true, true};
-    a.seg[2] = RopeSegment{v, v_cache, c.v_token_stride, c.v_head_stride, 0, 0, c.v_scale_inv, cache.kv_heads,
-                           c.q_heads + cache.kv_heads, false, true};
+    auto stride = [](int64_t s) { return static_cast<int32_t>(s); };
+    a.seg[0] = RopeSegment{q, q_out, stride(c.q_token_stride), stride(c.q_head_stride), stride(c.out_token_stride),
+                           stride(c.out_head_stride), nullptr, c.q_heads, 0, true, false};
+    a.seg[1] = RopeSegment{k, k_cache, stride(c.k_token_stride), stride(c.k_head_stride), 0, 0, c.k_scale_inv,
+                           cache.kv_heads, c.q_heads, true, true};
+    a.seg[2] = RopeSegment{v, v_cache, stride(c.v_token_stride), stride(c.v_head_stride), 0, 0, c.v_scale_inv,
+                           cache.kv_heads, c.q_heads + cache.kv_heads, false, true};
     a.n_seg = 3;
     a.heads = static_cast<int32_t>(heads);
     a.positions = positions;
     a.slots = slots;
-    a.tokens = tokens;
+    a.tokens = static_cast<int32_t>(tokens);
     a.cache_slots = cache.n_pages * cache.page_size;
     a.page_size = cache.page_size;
     a.page_stride = cache.page_stride;
