@@ -276,8 +276,7 @@ struct Attn {
     static constexpr int kPart = kHeads * (DP + 2);   // floats of a part in the workspace: out, then m, l
     static constexpr int kThreads = 32 * W;
     static constexpr int kRing = kTeams * S * kStage;
-    // floats of a staged head's row: spread over the banks where there is room for two parts of each team
-    static constexpr int kLd = 2 * kTeams * kHeads * (DP + 4) * 4 <= kRing ? DP + 4 : DP;
+    static constexpr int kLd = DP + 4;                // floats of a staged head's row (spread over the banks)
     static constexpr int kStaged = 2 * kTeams * kHeads * kLd * 4;
     static constexpr int kBuffer = kRing > kStaged ? kRing : kStaged;
     static_assert(2 * kTeams <= 32, "a lane for each part of a CTA");
@@ -295,6 +294,7 @@ struct Attn {
         uint32_t mask[kTeams][S];       // tokens of each stage that are there
         int32_t items;                  // joined items
         int32_t won[2];                 // whether this CTA joins the item of its slot
+        int32_t first[2], last[2], size[2];  // that item's CTAs, and how many join at a time
     };
     static constexpr int kSharedBytes = kBuffer + static_cast<int>(sizeof(Shared));
 };
@@ -371,48 +371,57 @@ __device__ __forceinline__ void join_parts(const AttnArgs& a, typename K::Shared
     constexpr int kFloats = K::kHeads * DP, kRound = K::kBuffer / (kFloats * 4);
     constexpr int kEach = (K::kHeads * K::kFour + K::kThreads - 1) / K::kThreads;
     static_assert(kRound >= 1, "");
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, lane = tid & 31, used = w.heads * K::kFour;
     const float* in = reinterpret_cast<const float*>(smem);
     const uint32_t buffer = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
     auto part = [&](int k) { return k == 0 ? at0 : k == n - 1 ? at_end : first + k * stride; };
     float4 acc[kEach];
 #pragma unroll
     for (int e = 0; e < kEach; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
     for (int k0 = 0; k0 < n; k0 += kRound) {
         const int k1 = min(k0 + kRound, n);
 #pragma unroll 1
         for (int k = k0; k < k1; ++k) {
             const float* from = part(k);
-            for (int i = tid; i < w.heads * K::kFour; i += K::kThreads)
-                cp_async16(buffer + ((k - k0) * kFloats + i * 4) * 4, from + i * 4, 16u);
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) {
+                const int i = tid + e * K::kThreads;
+                if (i < used) cp_async16(buffer + ((k - k0) * kFloats + i * 4) * 4, from + i * 4, 16u);
+            }
         }
         cp_async_commit();
-        if (k0 == 0 && tid < w.heads) {
-            float top = -INFINITY, sum = 0.0f, m[kJoin], l[kJoin];
+        if (k0 == 0) {
+            // the weights meanwhile: a warp for each head, a lane for each part
+#pragma unroll 1
+            for (int h = tid >> 5; h < w.heads; h += K::kThreads / 32) {
+                const float* of = part(lane < n ? lane : 0) + kFloats + h;
+                const float m = lane < n ? __ldcg(of) : -INFINITY, l = lane < n ? __ldcg(of + K::kHeads) : 0.0f;
+                float top = m;
 #pragma unroll
-            for (int k = 0; k < kJoin; ++k) {
-                m[k] = k < n ? __ldcg(part(k) + kFloats + tid) : -INFINITY;
-                l[k] = k < n ? __ldcg(part(k) + kFloats + K::kHeads + tid) : 0.0f;
-                top = fmaxf(top, m[k]);
-            }
+                for (int d = 1; d < kJoin; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                top = __shfl_sync(0xffffffffu, top, 0);
+                const float by = rescale(m, top);
+                float sum = l * by;
 #pragma unroll
-            for (int k = 0; k < kJoin; ++k) {
-                const float by = rescale(m[k], top);
-                sh.weight[k][tid] = by;
-                sum = k < n ? __fmaf_rn(l[k], by, sum) : sum;
+                for (int d = 1; d < kJoin; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                if (lane < kJoin) sh.weight[lane][h] = by;
+                if (lane == 0) {
+                    sh.top[h] = top;
+                    sh.sum[h] = sum;
+                }
             }
-            sh.top[tid] = top;
-            sh.sum[tid] = sum;
         }
         cp_async_wait<0>();
         __syncthreads();
+#pragma unroll 1
+        for (int k = k0; k < k1; ++k) {
 #pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-            const int i = tid + e * K::kThreads, h = i / K::kFour;
-            if (i >= w.heads * K::kFour) break;
-#pragma unroll 4
-            for (int k = k0; k < k1; ++k)
-                acc[e] = fma4(*reinterpret_cast<const float4*>(in + (k - k0) * kFloats + i * 4), sh.weight[k][h], acc[e]);
+            for (int e = 0; e < kEach; ++e) {
+                const int i = tid + e * K::kThreads;
+                if (i < used)
+                    acc[e] = fma4(*reinterpret_cast<const float4*>(in + (k - k0) * kFloats + i * 4), sh.weight[k][i / K::kFour], acc[e]);
+            }
         }
         __syncthreads();
     }
@@ -420,7 +429,7 @@ __device__ __forceinline__ void join_parts(const AttnArgs& a, typename K::Shared
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
         const int i = tid + e * K::kThreads, h = i / K::kFour, d = i % K::kFour * 4;
-        if (i >= w.heads * K::kFour) break;
+        if (i >= used) break;
         const float sum = sh.sum[h];
         if (to) {
             *reinterpret_cast<float4*>(to + i * 4) = acc[e];
@@ -659,9 +668,6 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                 reinterpret_cast<uint4*>(my_ring)[i] = make_uint4(0, 0, 0, 0);
             team_sync<TM>(team);
         }
-#pragma unroll 1
-        for (int s = 0; s < S - 1; ++s) issue(s);
-
         // the queries of the item at `p`, as they are
         auto load_queries = [&](const Place<T>& p) {
             const Heads<K::kHeads> hd(a, p.item);
@@ -683,7 +689,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
         const uint32_t k_at = ring + swizzled<K::kChunks>(k_row, k_piece);
         const uint32_t v_at = ring + T * K::kRow + swizzled<K::kChunks>(v_row, v_piece);
         const bool rules = a.softcap > 0.0f || a.slopes;
-        int stage = 0;
+        int stage = 0, fill = 0;  // the stages of the tile at hand and of the next to be copied
         int32_t done = 0;
         while (done < my_tiles) {
             const int32_t ta = at.t, tb = min(at.nt, ta + my_tiles - done);
@@ -740,10 +746,12 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
             }
 
 #pragma unroll 1
-            for (int32_t t = ta; t < tb; ++t) {
+            for (int32_t t = done == 0 ? ta - (S - 1) : ta; t < tb; ++t) {  // the first S - 1 rounds only fill the ring
                 cp_async_wait<S - 2>();
                 team_sync<TM>(team);
-                issue(stage == 0 ? S - 1 : stage - 1);
+                issue(fill);
+                fill = fill + 1 == S ? 0 : fill + 1;
+                if (t < ta) continue;
 
                 // S^T = K Q^T, two chains of sums
                 const uint32_t keys = k_at + stage * K::kStage, values = v_at + stage * K::kStage;
@@ -1069,51 +1077,55 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
     }
 
     // Join between CTAs: the last of an item's CTAs to arrive does it.  More than kJoin join in groups, then the groups.
-    const Joined open[2] = {sh.joined[0], sh.joined[joined - 1]};
-    const bool is_open[2] = {open[0].slot == 0, open[1].slot == 1};
-    if (!is_open[0] && !is_open[1]) return;
-    int32_t first[2], last[2], size[2];
-#pragma unroll
-    for (int slot = 0; slot < 2; ++slot) {
-        if (!is_open[slot]) continue;
-        first[slot] = by_cta.part_of(open[slot].start);
-        last[slot] = by_cta.part_of(open[slot].start + open[slot].nt - 1);
-        const int32_t n = last[slot] - first[slot] + 1;
-        size[slot] = n <= kJoin ? n : max(12, (n + kJoin - 1) / kJoin);
+    if (sh.joined[0].slot != 0 && sh.joined[joined - 1].slot != 1) return;
+    __syncthreads();
+    if (tid < 64 && lane == 0) {
+        const Joined& w = sh.joined[warp == 0 ? 0 : joined - 1];
+        if (w.slot == warp) {
+            const int32_t first = by_cta.part_of(w.start), last = by_cta.part_of(w.start + w.nt - 1), n = last - first + 1;
+            const int32_t size = n <= kJoin ? n : max(12, (n + kJoin - 1) / kJoin);
+            const int32_t lo = first + (static_cast<int32_t>(blockIdx.x) - first) / size * size;
+            const int32_t here = min(size, last - lo + 1);
+            sh.first[warp] = first;
+            sh.last[warp] = last;
+            sh.size[warp] = size;
+            // a group of one has no ticket: that CTA's may be the next item's
+            sh.won[warp] = here == 1 || arrive_last(a.tickets + lo, here);
+        } else {
+            sh.won[warp] = 0;
+        }
     }
     __syncthreads();
-#pragma unroll
+    constexpr int64_t kCta = 3 * K::kPart;
+#pragma unroll 1
     for (int slot = 0; slot < 2; ++slot) {
-        if (tid != 32 * slot || !is_open[slot]) continue;
-        const int32_t lo = first[slot] + (static_cast<int32_t>(blockIdx.x) - first[slot]) / size[slot] * size[slot];
-        const int32_t n = min(size[slot], last[slot] - lo + 1);
-        // a group of one has no ticket: that CTA's may be the next item's
-        sh.won[slot] = n == 1 || arrive_last(a.tickets + lo, n);
-    }
-    __syncthreads();
-    const int64_t kCta = 3 * K::kPart;
-#pragma unroll
-    for (int slot = 0; slot < 2; ++slot) {
-        if (!is_open[slot] || !sh.won[slot]) continue;
-        const Joined& p = open[slot];
-        const int32_t at = (static_cast<int32_t>(blockIdx.x) - first[slot]) / size[slot];
-        const int32_t lo = first[slot] + at * size[slot], n = min(size[slot], last[slot] - lo + 1);
-        const int32_t groups = (last[slot] - first[slot]) / size[slot] + 1;
+        if (!sh.won[slot]) continue;
+        const Joined w = sh.joined[slot == 0 ? 0 : joined - 1];
+        const int32_t first = sh.first[slot], last = sh.last[slot], size = sh.size[slot];
+        const int32_t groups = (last - first) / size + 1, lo = first + (static_cast<int32_t>(blockIdx.x) - first) / size * size;
         // a group's result goes to slot 2 of its first CTA; a group of one, an item's last CTA (where the next item may
         // have its first group), is its own result
-        if (groups == 1 || n > 1) {
-            const float* parts = a.cta_part + lo * kCta;
-            join_parts<K, DP>(a, sh, smem, parts, kCta, parts + (lo == first[slot] ? K::kPart : 0), parts + (n - 1) * kCta, n, p,
-                              groups == 1 ? nullptr : a.cta_part + lo * kCta + 2 * K::kPart);
+        int32_t n = min(size, last - lo + 1);
+        const float* parts = a.cta_part + lo * kCta;
+        const float *at0 = parts + (lo == first ? K::kPart : 0), *at_end = parts + (n - 1) * kCta;
+        int64_t stride = kCta;
+        float* to = groups == 1 ? nullptr : a.cta_part + lo * kCta + 2 * K::kPart;
+#pragma unroll 1
+        for (int level = 0; level < 2; ++level) {
+            if (level == 1) {
+                if (groups == 1) break;
+                if (tid == 0) sh.won[slot] = arrive_last(a.tickets + gridDim.x + first, groups);
+                __syncthreads();
+                if (!sh.won[slot]) break;
+                const int32_t in_last = (last - first) % size + 1;
+                parts = at0 = a.cta_part + first * kCta + 2 * K::kPart;
+                at_end = a.cta_part + (last - in_last + 1) * kCta + (in_last == 1 ? 0 : 2 * K::kPart);
+                stride = kCta * size;
+                n = groups;
+                to = nullptr;
+            }
+            if (to == nullptr || n > 1) join_parts<K, DP>(a, sh, smem, parts, stride, at0, at_end, n, w, to);
         }
-        if (groups == 1) continue;
-        if (tid == 0) sh.won[slot] = arrive_last(a.tickets + gridDim.x + first[slot], groups);
-        __syncthreads();
-        if (!sh.won[slot]) continue;
-        const float* heads = a.cta_part + first[slot] * kCta + 2 * K::kPart;
-        const int32_t in_last = (last[slot] - first[slot]) % size[slot] + 1;
-        const float* tail = a.cta_part + (last[slot] - in_last + 1) * kCta + (in_last == 1 ? 0 : 2 * K::kPart);
-        join_parts<K, DP>(a, sh, smem, heads, kCta * size[slot], heads, tail, groups, p, nullptr);
     }
 }
 

@@ -30,16 +30,8 @@ ROPE_LAYOUTS = {"half": 0, "interleaved": 1}
 ROPE_SCALINGS = {"none": 0, "linear": 1, "base": 2, "bands": 3}
 
 
-def _bound(name: str):
-    """The C entry point, looked up once: these calls are on a decoding step's critical path."""
-    fn = getattr(_abi.lib(), name)
-
-    def invoke(*args) -> None:
-        rc = fn(*args)
-        if rc != 0:
-            raise_for_status(rc, f"{name}: {_abi.last_error()}")
-
-    return invoke
+def _raise(name: str, rc: int) -> None:
+    raise_for_status(rc, f"{name}: {_abi.last_error()}")
 
 
 def rope_frequencies(rot_dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
@@ -83,14 +75,16 @@ class PageAssigner:
         self.config = _abi.PageConfig(int(page_size), int(max_pages),
                                       int(max_pages if table_stride is None else table_stride))
         self._config = ctypes.byref(self.config)
-        self._call = _bound("mf_page_assign")
+        self._assign = _abi.lib().mf_page_assign  # looked up once: the calls are on a decoding step's critical path
 
     def assign(self, lens: int, new_tokens: int, n_requests: int, table: int, free_pages: int, pool: int, tokens: int,
                slots: int, positions: int, owner: int, starts: int, lens_after: int, pool_after: int, stream=None) -> None:
         """Extend the tables in place and write the tokens' slots, positions and owners, the requests' starts and
         lengths after the step, and what is left of the pool."""
-        self._call(self._config, lens, new_tokens, n_requests, table, free_pages, pool, tokens, slots, positions, owner,
-                   starts, lens_after, pool_after, stream_handle(stream))
+        rc = self._assign(self._config, lens, new_tokens, n_requests, table, free_pages, pool, tokens, slots, positions,
+                          owner, starts, lens_after, pool_after, stream if stream is None else stream_handle(stream))
+        if rc:
+            _raise("mf_page_assign", rc)
 
 
 class Rope:
@@ -103,13 +97,16 @@ class Rope:
         self.config = _abi.RopeConfig(int(dtype), int(head_dim), int(head_dim if rot_dim is None else rot_dim),
                                       ROPE_LAYOUTS[layout], float(magnitude), int(inv_freq))
         self._config = ctypes.byref(self.config)
-        self._call = _bound("mf_rope")
+        self._rope = _abi.lib().mf_rope
 
     def _run(self, inverse, src, dst, positions, tokens, heads, src_strides, dst_strides, stream) -> None:
         dim = self.config.head_dim
         st, sh = src_strides or (heads * dim, dim)
         dt, dh = dst_strides or (heads * dim, dim)
-        self._call(self._config, inverse, src, st, sh, dst, dt, dh, positions, tokens, heads, stream_handle(stream))
+        rc = self._rope(self._config, inverse, src, st, sh, dst, dt, dh, positions, tokens, heads,
+                        stream if stream is None else stream_handle(stream))
+        if rc:
+            _raise("mf_rope", rc)
 
     def forward(self, src: int, dst: int, positions: int, tokens: int, heads: int, src_strides=None, dst_strides=None,
                 stream=None) -> None:
@@ -135,11 +132,14 @@ class RopeAppend:
         self.config = _abi.RopeAppendConfig(rope.config, cache.struct, int(q_heads), int(compat), int(k_scale_inv) or None,
                                             int(v_scale_inv) or None, qs, dim, ks, dim, ks, dim, q_heads * dim, dim)
         self._config = ctypes.byref(self.config)
-        self._call = _bound("mf_rope_append")
+        self._append = _abi.lib().mf_rope_append
 
     def run(self, q: int, k: int, v: int, q_out: int, k_cache: int, v_cache: int, positions: int, slots: int, tokens: int,
             stream=None) -> None:
-        self._call(self._config, q, k, v, q_out, k_cache, v_cache, positions, slots, tokens, stream_handle(stream))
+        rc = self._append(self._config, q, k, v, q_out, k_cache, v_cache, positions, slots, tokens,
+                          stream if stream is None else stream_handle(stream))
+        if rc:
+            _raise("mf_rope_append", rc)
 
 
 class PagedAttention:
@@ -163,13 +163,16 @@ class PagedAttention:
         handle = ctypes.c_void_p()
         _abi.call("mf_paged_attn_create", ctypes.byref(self.config), ctypes.byref(handle))
         self._handle = handle.value
-        self._call = _bound("mf_paged_attn_run")
+        self._attend = _abi.lib().mf_paged_attn_run
 
     def run(self, q: int, k_cache: int, v_cache: int, table: int, lens: int, n_requests: int, out: int, lse: int = 0,
             stream=None) -> None:
         if self._handle is None:
             raise TensorClosed("paged attention: closed")
-        self._call(self._handle, q, k_cache, v_cache, table, lens, n_requests, out, lse, stream_handle(stream))
+        rc = self._attend(self._handle, q, k_cache, v_cache, table, lens, n_requests, out, lse,
+                          stream if stream is None else stream_handle(stream))
+        if rc:
+            _raise("mf_paged_attn_run", rc)
 
     def close(self) -> None:
         """Free the workspace; the object's last run has to be over."""
