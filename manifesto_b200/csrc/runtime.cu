@@ -98,6 +98,12 @@ int mf_device_count(int* count) {
 
 int mf_init(int device) {
     std::lock_guard<std::mutex> lock(g_init_mutex);
+    if (g_state.open && g_state.device == device) {
+        // again: the properties are known, and reading them takes a millisecond
+        MF_CUDA_CHECK(cudaSetDevice(device));
+        MF_CUDA_CHECK(cudaFree(nullptr));
+        return MF_OK;
+    }
     int count = 0;
     cudaError_t err = cudaGetDeviceCount(&count);
     if (err != cudaSuccess || count == 0) {

@@ -736,3 +736,21 @@ def test_attn_refusals(backend):
     a.run(0, 0, 0, 0, 0, 0, 0)
     a.close()
     b.free()
+
+
+# ------------------------------------------------------------------ together
+
+@pytest.mark.parametrize("cache,most", [("bf16", 0.05), ("f8_e4m3", 0.35), ("f8_e5m2", 0.7)])
+def test_decoding_steps_of_the_example(backend, cache, most):
+    """Prompts, then a token at a time, against float64 attention over what the requests hold.
+
+    A BF16 cache rounds values and rotated keys and queries (2^-9 of themselves on average, |v| up to 4, scores off by
+    2^-8 of 3 at most): 0.05.  FP8 keys and values are off by up to 2^-4 (E4M3) or 2^-3 (E5M2) of themselves: a value of 4
+    by 0.25 or 0.5, more than what its token's weight changes."""
+    import importlib.util
+    from pathlib import Path
+    spec = importlib.util.spec_from_file_location("paged_decode", Path(__file__).parents[1] / "examples" / "paged_decode.py")
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    worst = example.run(cache_dtype=cache)
+    assert len(worst) == 5 and max(worst) <= most
