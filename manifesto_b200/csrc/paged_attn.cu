@@ -253,6 +253,7 @@ struct Joined {
     int32_t r, kv, head0, heads, slot, start, nt;
 };
 
+constexpr int kFills = 3;  // ways to give each item CTAs of its own
 constexpr int kJoin = 16;  // most parts that one step of a join between CTAs takes
 // A maximum is only replaced by one that is this much larger (in powers of two): until then the weights grow up to
 // 2^8, which float32 sums and both terms of a weight hold as well, and what is summed is not rescaled.
@@ -284,8 +285,10 @@ struct Attn {
     static_assert(W >= 2 && (T == kBlock || T == 2 * kBlock), "");
 
     struct Shared {
-        int64_t warp_sum[32];           // tiles of the requests of each warp's threads
+        int64_t warp_sum[W];            // tiles of the requests of each warp's threads
         int32_t thread_sum[kThreads];   // and of each thread's
+        int32_t thread_nt[kThreads];    // tiles of an item of each thread's last request
+        uint32_t warp_ctas[kFills][W];  // the CTAs that the requests of each warp get where each item has its own
         Part part[2 * kTeams];          // first and last part of each team
         float m[2 * kTeams][kHeads], l[2 * kTeams][kHeads];  // of the parts; m becomes their weight
         Joined joined[2 * kTeams];
@@ -445,6 +448,19 @@ __device__ __forceinline__ void join_parts(const AttnArgs& a, typename K::Shared
     __syncthreads();
 }
 
+// CTAs of an item of nt tiles where each item has its own, so that a team has up to kOwnTiles[fill] tiles.  A handful
+// of tiles takes no longer than the join between two CTAs; the first limit whose CTAs are all there is taken, and a
+// request alone gets all there are when it has more than one CTA's.  8 requests of 1000 tokens, 32/8 heads of 128:
+// 16.1 us with the row of tiles cut evenly, 12.7 so; 8 of 2000: 22.8 and 19.5.
+__device__ constexpr int kOwnTiles[kFills] = {3, 6, 12};
+template <class K>
+__device__ __forceinline__ int32_t ctas_of(const AttnArgs& a, int32_t nt, int fill) {
+    if (nt == 0) return 0;
+    const int32_t n = (nt - 1) / (K::kTeams * kOwnTiles[fill]) + 1;
+    if (n == 1 || a.n_requests > 1) return n;
+    return max(min(static_cast<int32_t>(gridDim.x) / a.items, (nt - 1) / K::kTeams + 1), 1);
+}
+
 template <int MODE, int DP, int TM, int W, int T, int S>
 __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a) {
     using K = Attn<MODE, DP, TM, W, T, S>;
@@ -459,14 +475,26 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
     const int32_t per = (a.n_requests + K::kThreads - 1) / K::kThreads;
     int64_t sum = 0;
     bool empty = false;
+    int32_t nt_of = 0;
     for (int32_t i = 0; i < per; ++i) {
         const int32_t r = tid * per + i;
         if (r >= a.n_requests) break;
         const int32_t nt = tiles_of<T>(span_of(a, r));
         sum += static_cast<int64_t>(nt) * items;
+        nt_of = nt;
         empty |= nt == 0 && r % gridDim.x == blockIdx.x;
     }
     sh.thread_sum[tid] = static_cast<int32_t>(sum);
+    const bool few = static_cast<int64_t>(a.n_requests) * items <= gridDim.x;  // there may be CTAs for each item
+    if (few) {
+        sh.thread_nt[tid] = nt_of;
+#pragma unroll 1
+        for (int f = 0; f < kFills; ++f) {
+            const int64_t mine = static_cast<int64_t>(ctas_of<K>(a, nt_of, f)) * items;
+            const uint32_t all = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(mine < (1 << 20) ? mine : 1 << 20));
+            if (lane == 0) sh.warp_ctas[f][warp] = all;
+        }
+    }
     {
         const int64_t low = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(sum & 0xffff));
         const int64_t high = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(sum >> 16 < (1 << 26) ? sum >> 16 : 1 << 26));
@@ -482,39 +510,18 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
             for (int i = tid; i < a.q_heads; i += K::kThreads) store_lse(a, r, i, 0.0f, 0.0f);
         }
     }
-    // the row of all tiles: this CTA's run of them, and this team's of those
-    const int64_t of_warp = lane < W ? sh.warp_sum[lane] : 0;
-    int64_t in_front = of_warp;
+    // Of W values of warps and the values of their threads, in a row: the thread that place `key` is at, and how far into it.
+    auto locate = [&](int64_t of_warp, auto of_threads, int32_t key, int32_t& into) {
+        int64_t in_front = of_warp;
 #pragma unroll
-    for (int d = 1; d < 16; d <<= 1) {
-        const int64_t x = __shfl_up_sync(0xffffffffu, in_front, d);
-        if (lane >= d) in_front += x;
-    }
-    const int64_t total64 = __shfl_sync(0xffffffffu, in_front, W - 1);
-    if (total64 == 0) return;
-    if (total64 > 0x7fffffff) {
-        if (tid == 0) atomicExch(a.status, MF_DEVICE_TOO_LARGE);
-        return;
-    }
-    const int32_t total = static_cast<int32_t>(total64), want = (total - 1) / K::kTeams + 1;
-    int32_t ctas = min(want, static_cast<int32_t>(gridDim.x));
-    if (a.n_requests == 1 && items <= gridDim.x) ctas = max(ctas / items, 1) * items;  // no CTA has parts of two items
-    if (blockIdx.x >= ctas) return;
-    const Cut by_cta(total, ctas);
-    const int32_t cta_tile = by_cta.start(blockIdx.x), cta_tiles = by_cta.start(blockIdx.x + 1) - cta_tile;
-    const Cut by_team(cta_tiles, K::kTeams);
-    const int32_t x0 = cta_tile + by_team.start(team), my_tiles = cta_tile + by_team.start(team + 1) - x0;
-    const int32_t id = blockIdx.x * K::kTeams + team;
-
-    uint32_t qf[K::kSteps][2];
-    float o[K::kSteps][4];
-    float m[2], l[2];
-    if (my_tiles > 0) {
-        // the place of tile x0: the warp, then the thread whose requests hold it, then the request among them
+        for (int d = 1; d < 16; d <<= 1) {
+            const int64_t x = __shfl_up_sync(0xffffffffu, in_front, d);
+            if (lane >= d) in_front += x;
+        }
         in_front -= of_warp;
-        const int in_warp = 31 - __clz(__ballot_sync(0xffffffffu, lane < W && in_front <= x0));
-        int32_t before = static_cast<int32_t>(__shfl_sync(0xffffffffu, in_front, in_warp));
-        const int32_t of_thread = sh.thread_sum[32 * in_warp + lane];
+        const int in_warp = 31 - __clz(__ballot_sync(0xffffffffu, lane < W && in_front <= key));
+        const int32_t before = static_cast<int32_t>(__shfl_sync(0xffffffffu, in_front, in_warp));
+        const int32_t of_thread = of_threads(32 * in_warp + lane);
         int32_t ahead = of_thread;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -522,35 +529,87 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
             if (lane >= d) ahead += x;
         }
         ahead -= of_thread;
-        const int in_lane = 31 - __clz(__ballot_sync(0xffffffffu, before + ahead <= x0));
-        before += __shfl_sync(0xffffffffu, ahead, in_lane);
-        Place<T> at{};
-        at.r = 32 * in_warp + in_lane;
-        if (per > 1) {
-            for (int32_t r0 = at.r * per;; r0 += 32) {
-                const int32_t mine = r0 + lane < a.n_requests ? tiles_of<T>(span_of(a, r0 + lane)) * items : 0;
-                int32_t upto = mine;
-#pragma unroll 1
-                for (int d = 1; d < 32; d <<= 1) {
-                    const int32_t x = __shfl_up_sync(0xffffffffu, upto, d);
-                    if (lane >= d) upto += x;
-                }
-                const uint32_t past = __ballot_sync(0xffffffffu, before + upto > x0);
-                if (past || r0 + 32 >= a.n_requests) {
-                    const int src = past ? __ffs(past) - 1 : 0;
-                    at.r = r0 + src;
-                    before += __shfl_sync(0xffffffffu, upto - mine, src);
-                    break;
-                }
-                before += __shfl_sync(0xffffffffu, upto, 31);
-            }
-        }
+        const int in_lane = 31 - __clz(__ballot_sync(0xffffffffu, before + ahead <= key));
+        into = key - before - __shfl_sync(0xffffffffu, ahead, in_lane);
+        return 32 * in_warp + in_lane;
+    };
+    // Each item has CTAs of its own where those suffice; else the row of all tiles is cut evenly.
+    const int64_t tiles_of_warp = lane < W ? sh.warp_sum[lane] : 0;
+    int64_t total64 = tiles_of_warp;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) total64 += __shfl_xor_sync(0xffffffffu, total64, d);
+    uint32_t ctas_of_warp = 0, all_ctas = 0xffffffffu;
+    int fill = -1;
+    while (few && all_ctas > gridDim.x && ++fill < kFills) {
+        ctas_of_warp = lane < W ? sh.warp_ctas[fill][lane] : 0;
+        all_ctas = __reduce_add_sync(0xffffffffu, ctas_of_warp);
+    }
+    if (total64 == 0) return;
+    if (total64 > 0x7fffffff) {
+        if (tid == 0) atomicExch(a.status, MF_DEVICE_TOO_LARGE);
+        return;
+    }
+    const bool own = all_ctas <= gridDim.x;
+    const int32_t total = static_cast<int32_t>(total64), want = (total - 1) / K::kTeams + 1;
+    const int32_t ctas = own ? static_cast<int32_t>(all_ctas) : min(want, static_cast<int32_t>(gridDim.x));
+    if (blockIdx.x >= ctas) return;
+    const Cut by_cta(total, ctas);
+    const int32_t id = blockIdx.x * K::kTeams + team;
+    Place<T> at{};
+    int32_t x0, my_tiles, own_first = 0, own_last = 0;  // first tile in the row (of the item, if it has its own CTAs), tiles
+    if (own) {
+        int32_t into;
+        at.r = locate(ctas_of_warp, [&](int t) { return ctas_of<K>(a, sh.thread_nt[t], fill) * items; }, blockIdx.x, into);
         at.span = span_of(a, at.r);
         at.nt = tiles_of<T>(at.span);
-        const int32_t in_request = x0 - before;
-        at.item = in_request / at.nt;
-        at.t = in_request - at.item * at.nt;
+        const int32_t each = ctas_of<K>(a, at.nt, fill);
+        at.item = into / each;
+        const int32_t nth = into - at.item * each;
+        const Cut of_item(at.nt, each);
+        const int32_t from = of_item.start(nth);
+        const Cut by_team(of_item.start(nth + 1) - from, K::kTeams);
+        x0 = at.t = from + by_team.start(team);
+        my_tiles = from + by_team.start(team + 1) - x0;
+        own_first = blockIdx.x - nth;
+        own_last = own_first + each - 1;
+    } else {
+        const int32_t cta_tile = by_cta.start(blockIdx.x);
+        const Cut by_team(by_cta.start(blockIdx.x + 1) - cta_tile, K::kTeams);
+        x0 = cta_tile + by_team.start(team);
+        my_tiles = cta_tile + by_team.start(team + 1) - x0;
+        if (my_tiles > 0) {
+            int32_t into;
+            at.r = locate(tiles_of_warp, [&](int t) { return sh.thread_sum[t]; }, x0, into);
+            if (per > 1) {
+                for (int32_t r0 = at.r * per;; r0 += 32) {
+                    const int32_t mine = r0 + lane < a.n_requests ? tiles_of<T>(span_of(a, r0 + lane)) * items : 0;
+                    int32_t upto = mine;
+#pragma unroll 1
+                    for (int d = 1; d < 32; d <<= 1) {
+                        const int32_t x = __shfl_up_sync(0xffffffffu, upto, d);
+                        if (lane >= d) upto += x;
+                    }
+                    const uint32_t past = __ballot_sync(0xffffffffu, upto > into);
+                    if (past || r0 + 32 >= a.n_requests) {
+                        const int src = past ? __ffs(past) - 1 : 0;
+                        at.r = r0 + src;
+                        into -= __shfl_sync(0xffffffffu, upto - mine, src);
+                        break;
+                    }
+                    into -= __shfl_sync(0xffffffffu, upto, 31);
+                }
+            }
+            at.span = span_of(a, at.r);
+            at.nt = tiles_of<T>(at.span);
+            at.item = into / at.nt;
+            at.t = into - at.item * at.nt;
+        }
+    }
 
+    uint32_t qf[K::kSteps][2];
+    float o[K::kSteps][4];
+    float m[2], l[2];
+    if (my_tiles > 0) {
         unsigned char* my_ring = smem + team * (S * K::kStage);
         const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(my_ring));
         Place<T> load = at;
@@ -1082,7 +1141,8 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
     if (tid < 64 && lane == 0) {
         const Joined& w = sh.joined[warp == 0 ? 0 : joined - 1];
         if (w.slot == warp) {
-            const int32_t first = by_cta.part_of(w.start), last = by_cta.part_of(w.start + w.nt - 1), n = last - first + 1;
+            const int32_t first = own ? own_first : by_cta.part_of(w.start);
+            const int32_t last = own ? own_last : by_cta.part_of(w.start + w.nt - 1), n = last - first + 1;
             const int32_t size = n <= kJoin ? n : max(12, (n + kJoin - 1) / kJoin);
             const int32_t lo = first + (static_cast<int32_t>(blockIdx.x) - first) / size * size;
             const int32_t here = min(size, last - lo + 1);
