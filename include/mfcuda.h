@@ -472,8 +472,9 @@ typedef struct mf_cache_layout {
  * Request r holds lens[r] tokens and gets new_tokens[r] more (negative counts
  * as 0).  With page size P, held = ceil(lens / P), need = ceil((lens + new) / P)
  * - held and before = the sum of need over the requests in front of r:
- *   a request fits when ceil((lens + new) / P) <= max_pages and (need == 0 or
- *   before + need <= pool[1]); one without room in its table needs no pages;
+ *   a request fits when ceil((lens + new) / P) <= max_pages, (need == 0 or
+ *   before + need <= pool[1]) and its last token's number and position are
+ *   31-bit; one without room in its table needs no pages;
  *   table[r][held + j] = free_pages[pool[0] + before + j],  j < need, if it fits;
  *   starts[r] = sum of new in front of r, starts[n_requests] = their total;
  *   token i = starts[r] + t: positions[i] = lens[r] + t, owner[i] = r,

@@ -32,8 +32,11 @@
 // parts in shared memory, CTAs through the workspace: the last of an item's
 // CTAs to arrive (a ticket) joins them in the order of the tokens, so the
 // result does not depend on who was last.
+#include <mutex>
 #include <new>
 
+#include "mf_divisor.cuh"
+#include "mf_internal.h"
 #include "mf_runtime.h"
 #include "mf_vec.cuh"
 
@@ -55,7 +58,7 @@ struct AttnArgs {
     int32_t page_bytes, row_bytes;
     int64_t head_bytes, table_stride;
     uint32_t n_pages;
-    uint32_t page_mul, page_shift;  // x / page = (mulhi(x, page_mul) + x) >> page_shift for x below 2^31
+    Divisor by_page;
     int32_t head_dim;
     const char* q;
     int64_t q_req, q_head;
@@ -223,7 +226,7 @@ struct Place {
     }
 };
 
-// An even cut of `total` into `parts`: part i starts at total * i / parts, in 32 bits for parts below 2^16.
+// An even cut of `total` into `parts`: part i starts at total * i / parts, in 32 bits (parts are below 2^15).
 struct Cut {
     int32_t total, parts, q, rem;
     __device__ __forceinline__ Cut(int32_t total_, int32_t parts_)
@@ -640,8 +643,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
             for (int b = 0; b < K::kBlocks; ++b) {
                 const int32_t tok = tok0 + lane_tok + (whole ? b * kBlock : 0);
                 if (new_item || !whole) {
-                    const uint32_t x = static_cast<uint32_t>(tok);
-                    const int32_t idx = static_cast<int32_t>((__umulhi(x, a.page_mul) + x) >> a.page_shift);
+                    const int32_t idx = static_cast<uint32_t>(tok) / a.by_page;
                     page_off[b] = tok - idx * a.page;
                     entry[b] = a.table + load.r * a.table_stride + idx;
                 } else {
@@ -1230,11 +1232,67 @@ Kernel pick(int cache_dtype, int group, int head_dim) {
 
 using namespace mf;
 
+namespace mf {
+namespace {
+
+// Workspaces of destroyed handles, for the next ones: allocating one takes
+// from half a millisecond to three.  Their tickets are zero, as every run leaves them.
+constexpr int kKept = 8;
+struct Kept {
+    void* p;
+    size_t bytes;
+    int device;
+};
+Kept g_kept[kKept];
+std::mutex g_kept_mutex;
+
+// The smallest kept workspace of `bytes` to four times that, or NULL.
+void* take_kept(size_t bytes, int device, size_t* got) {
+    std::lock_guard<std::mutex> lock(g_kept_mutex);
+    Kept* best = nullptr;
+    for (Kept& k : g_kept)
+        if (k.p && k.device == device && k.bytes >= bytes && k.bytes <= 4 * bytes && (!best || k.bytes < best->bytes)) best = &k;
+    if (!best) return nullptr;
+    void* p = best->p;
+    *got = best->bytes;
+    best->p = nullptr;
+    // a host that reset the device took it along
+    cudaPointerAttributes at;
+    if (cudaPointerGetAttributes(&at, p) != cudaSuccess || at.type != cudaMemoryTypeDevice || at.device != device) {
+        cudaGetLastError();
+        return nullptr;
+    }
+    return p;
+}
+
+bool keep(void* p, size_t bytes, int device) {
+    std::lock_guard<std::mutex> lock(g_kept_mutex);
+    for (Kept& k : g_kept)
+        if (!k.p) {
+            k = Kept{p, bytes, device};
+            return true;
+        }
+    return false;
+}
+
+}  // namespace
+
+void release_attn_workspaces() {
+    std::lock_guard<std::mutex> lock(g_kept_mutex);
+    for (Kept& k : g_kept) {
+        if (k.p) cudaFree(k.p);
+        k.p = nullptr;
+    }
+}
+
+}  // namespace mf
+
 struct mf_paged_attn_s {
     mf_paged_attn_config config;
     Kernel kernel;
     AttnArgs args;
     void* workspace;
+    size_t bytes;
     int device, ctas;
 };
 
@@ -1274,25 +1332,31 @@ extern "C" int mf_paged_attn_create(const mf_paged_attn_config* config, mf_paged
     const int ctas = state().sm_count;
     const size_t team_part = static_cast<size_t>(ctas) * kernel.teams * kernel.part_floats * 4;
     const size_t cta_part = static_cast<size_t>(ctas) * 3 * kernel.part_floats * 4;
-    const size_t bytes = team_part + cta_part + static_cast<size_t>(ctas) * 8;
+    const size_t bytes = (static_cast<size_t>(ctas) * 8 + 255) / 256 * 256 + team_part + cta_part;
     mf_paged_attn_s* h = new (std::nothrow) mf_paged_attn_s{};
     if (!h) return fail(MF_ERR_ALLOCATOR_EXHAUSTED, "mf_paged_attn_create: out of host memory");
-    cudaError_t err = cudaMalloc(&h->workspace, bytes);
-    if (err != cudaSuccess) {
-        cudaGetLastError();
-        delete h;
-        if (err == cudaErrorMemoryAllocation)
-            return fail(MF_ERR_ALLOCATOR_EXHAUSTED, "mf_paged_attn_create: %zu bytes: out of device memory", bytes);
-        return cuda_fail(err, "mf_paged_attn_create: cudaMalloc");
+    // tickets first: they stay in their place, whatever shape uses the workspace next
+    const size_t tickets = (static_cast<size_t>(ctas) * 8 + 255) / 256 * 256;
+    h->bytes = bytes;
+    h->workspace = take_kept(bytes, state().device, &h->bytes);
+    if (!h->workspace) {
+        cudaError_t err = cudaMalloc(&h->workspace, bytes);
+        if (err != cudaSuccess) {
+            cudaGetLastError();
+            delete h;
+            if (err == cudaErrorMemoryAllocation)
+                return fail(MF_ERR_ALLOCATOR_EXHAUSTED, "mf_paged_attn_create: %zu bytes: out of device memory", bytes);
+            return cuda_fail(err, "mf_paged_attn_create: cudaMalloc");
+        }
+        err = cudaMemset(h->workspace, 0, tickets);
+        if (err == cudaSuccess) err = cudaStreamSynchronize(nullptr);  // streams that do not wait for the default one may run it
+        if (err != cudaSuccess) {
+            cudaFree(h->workspace);
+            delete h;
+            return cuda_fail(err, "mf_paged_attn_create: cudaMemset");
+        }
     }
     char* w = static_cast<char*>(h->workspace);
-    err = cudaMemset(w + team_part + cta_part, 0, static_cast<size_t>(ctas) * 8);
-    if (err == cudaSuccess) err = cudaStreamSynchronize(nullptr);  // streams that do not wait for the default one may run it
-    if (err != cudaSuccess) {
-        cudaFree(h->workspace);
-        delete h;
-        return cuda_fail(err, "mf_paged_attn_create: cudaMemset");
-    }
     h->config = c;
     h->kernel = kernel;
     h->device = state().device;
@@ -1301,9 +1365,9 @@ extern "C" int mf_paged_attn_create(const mf_paged_attn_config* config, mf_paged
     a.slopes = c.slopes;
     a.k_scale = is_fp8(k.dtype) ? c.k_scale_inv : nullptr;
     a.v_scale = is_fp8(k.dtype) ? c.v_scale_inv : nullptr;
-    a.team_part = reinterpret_cast<float*>(w);
-    a.cta_part = reinterpret_cast<float*>(w + team_part);
-    a.tickets = reinterpret_cast<int32_t*>(w + team_part + cta_part);
+    a.tickets = reinterpret_cast<int32_t*>(w);
+    a.team_part = reinterpret_cast<float*>(w + tickets);
+    a.cta_part = reinterpret_cast<float*>(w + tickets + team_part);
     a.status = sticky_status_ptr();
     a.q_req = c.q_token_stride;
     a.q_head = c.q_head_stride;
@@ -1321,8 +1385,7 @@ extern "C" int mf_paged_attn_create(const mf_paged_attn_config* config, mf_paged
     a.head_dim = k.head_dim;
     a.page = k.page_size;
     a.max_pages = c.max_pages;
-    while ((1ull << a.page_shift) < static_cast<uint64_t>(a.page)) ++a.page_shift;
-    a.page_mul = static_cast<uint32_t>((((1ull << a.page_shift) - a.page) << 32) / a.page + 1);
+    a.by_page = divisor(a.page);
     a.window = c.window;
     a.q_f16 = c.q_dtype == MF_DT_F16;
     a.scale = c.scale;
@@ -1369,7 +1432,8 @@ extern "C" int mf_paged_attn_run(mf_paged_attn handle, const void* q, const void
 extern "C" int mf_paged_attn_destroy(mf_paged_attn handle) {
     if (!handle) return MF_OK;
     MF_ENTER();
-    MF_CUDA_CHECK(cudaFree(handle->workspace));
+    MF_CUDA_CHECK(cudaDeviceSynchronize());  // as freeing it would: no run of the handle goes on
+    if (!keep(handle->workspace, handle->bytes, handle->device)) MF_CUDA_CHECK(cudaFree(handle->workspace));
     delete handle;
     return MF_OK;
 }

@@ -12,6 +12,7 @@
 // every gridDim-th run of 512 tokens and of 512 requests.  Bound: the launch
 // and one chain of dependent loads for a decoding step; the 16 bytes written
 // per token for a long prompt.
+#include "mf_divisor.cuh"
 #include "mf_runtime.h"
 
 namespace mf {
@@ -36,8 +37,9 @@ struct AssignArgs {
     int64_t tokens;
     int64_t table_stride;
     int32_t n_requests;
-    int32_t page;
     int32_t max_pages;
+    Divisor page;
+    bool wide;  // lens and new_tokens are 16-byte aligned
 };
 
 struct Sums {
@@ -61,24 +63,39 @@ __device__ __forceinline__ int32_t clamp_i32(int64_t v) {
     return static_cast<int32_t>(v > 0x7fffffffll ? 0x7fffffffll : v);
 }
 
+// Pages of n tokens (n below 2^32, the one past 2^31 - 1 never asked for).
+__device__ __forceinline__ uint32_t pages_of(uint32_t n, const Divisor& page) {
+    const uint32_t q = n / page;
+    return q + (q * page.d != n);
+}
+
 // A request's need of pages; `room`: whether its table row reaches that far.
-__device__ __forceinline__ int64_t pages_needed(uint32_t len, uint32_t fresh, uint32_t page, uint32_t max_pages,
-                                                bool& room) {
-    const uint32_t held = len / page + (len % page != 0);
+__device__ __forceinline__ uint32_t pages_needed(uint32_t len, uint32_t fresh, const Divisor& page, uint32_t max_pages,
+                                                 bool& room) {
     const uint32_t sum = len + fresh;  // both below 2^31: it fits
-    const uint32_t after = sum / page + (sum % page != 0);
-    room = after <= max_pages && sum <= 0x7fffffffu;
-    return room ? after - held : 0;
+    room = sum <= 0x7fffffffu;
+    if (!room) return 0;
+    const uint32_t after = pages_of(sum, page);
+    room = after <= max_pages;
+    return room ? after - pages_of(len, page) : 0;
+}
+
+// Whether a request fits that needs `need` pages behind `before` others, its
+// tokens numbered from `start` on (in 31 bits).
+__device__ __forceinline__ bool fits_in(bool room, int64_t need, int64_t before, int64_t count, int64_t start, uint32_t fresh) {
+    return room && (need == 0 || before + need <= count) && start + fresh <= 0x7fffffffll;
 }
 
 __global__ void __launch_bounds__(kAssignThreads) page_assign_kernel(const AssignArgs a) {
-    __shared__ int64_t s_tok[kAssignTile + 1];   // token prefix of the tile's requests
-    __shared__ int64_t s_page[kAssignTile];      // page prefix, over all requests
+    __shared__ int32_t s_tok[kAssignTile];        // token prefix of the tile's requests, inside the tile
+    __shared__ int32_t s_page[kAssignTile];       // page prefix, over all requests
+    __shared__ uint32_t s_len[kAssignTile], s_new[kAssignTile];
     __shared__ Sums s_warp[kAssignThreads / 32];
     __shared__ long long s_taken;
     __shared__ int s_refused;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const uint32_t page = static_cast<uint32_t>(a.page), max_pages = static_cast<uint32_t>(a.max_pages);
+    const Divisor page = a.page;
+    const uint32_t max_pages = static_cast<uint32_t>(a.max_pages);
     const int32_t head = a.pool[0] < 0 ? 0 : a.pool[0];
     const int64_t count = a.pool[0] < 0 || a.pool[1] < 0 ? 0 : a.pool[1];
     if (tid == 0) {
@@ -93,14 +110,20 @@ __global__ void __launch_bounds__(kAssignThreads) page_assign_kernel(const Assig
         Sums mine{0, 0}, at[kAssignItems];
         bool room[kAssignItems];
         int64_t need[kAssignItems];
-#pragma unroll
-        for (int i = 0; i < kAssignItems; ++i) {
-            const int32_t r = r0 + tid * kAssignItems + i;
-            const bool in = r < a.n_requests;
-            const int32_t l = in ? a.lens[r] : 0, f = in ? a.fresh[r] : 0;
-            len[i] = l < 0 ? 0u : static_cast<uint32_t>(l);
-            fresh[i] = f < 0 ? 0u : static_cast<uint32_t>(f);
+        const int32_t mine_at = r0 + tid * kAssignItems;
+        int4 l4 = make_int4(0, 0, 0, 0), f4 = l4;
+        static_assert(kAssignItems == 4, "");
+        if (a.wide && mine_at + kAssignItems <= a.n_requests) {
+            l4 = *reinterpret_cast<const int4*>(a.lens + mine_at);
+            f4 = *reinterpret_cast<const int4*>(a.fresh + mine_at);
+        } else {
+            if (mine_at < a.n_requests) l4.x = a.lens[mine_at], f4.x = a.fresh[mine_at];
+            if (mine_at + 1 < a.n_requests) l4.y = a.lens[mine_at + 1], f4.y = a.fresh[mine_at + 1];
+            if (mine_at + 2 < a.n_requests) l4.z = a.lens[mine_at + 2], f4.z = a.fresh[mine_at + 2];
+            if (mine_at + 3 < a.n_requests) l4.w = a.lens[mine_at + 3], f4.w = a.fresh[mine_at + 3];
         }
+        len[0] = max(l4.x, 0), len[1] = max(l4.y, 0), len[2] = max(l4.z, 0), len[3] = max(l4.w, 0);
+        fresh[0] = max(f4.x, 0), fresh[1] = max(f4.y, 0), fresh[2] = max(f4.z, 0), fresh[3] = max(f4.w, 0);
 #pragma unroll
         for (int i = 0; i < kAssignItems; ++i) {
             need[i] = pages_needed(len[i], fresh[i], page, max_pages, room[i]);
@@ -125,10 +148,13 @@ __global__ void __launch_bounds__(kAssignThreads) page_assign_kernel(const Assig
         for (int i = 0; i < kAssignItems; ++i) {
             const int32_t k = tid * kAssignItems + i, r = r0 + k;
             const int64_t tok = before.tokens + at[i].tokens, pg = page_base + before.pages + at[i].pages;
-            s_tok[k] = tok;
-            s_page[k] = pg;
+            // what is past 31 bits is past what fits
+            s_tok[k] = clamp_i32(tok);
+            s_page[k] = clamp_i32(pg);
+            s_len[k] = len[i];
+            s_new[k] = fresh[i];
             if (r >= a.n_requests) continue;
-            const bool fits = room[i] && (need[i] == 0 || pg + need[i] <= count);
+            const bool fits = fits_in(room[i], need[i], pg, count, tok_base + tok, fresh[i]);
             refused += !fits;
             if (fits && need[i] > 0) taken = max(taken, static_cast<long long>(pg + need[i]));
             if ((r / kAssignThreads) % gridDim.x == blockIdx.x) {
@@ -136,41 +162,41 @@ __global__ void __launch_bounds__(kAssignThreads) page_assign_kernel(const Assig
                 a.lens_after[r] = static_cast<int32_t>(fits ? len[i] + fresh[i] : len[i]);
             }
         }
-        if (tid == 0) s_tok[kAssignTile] = all.tokens;
         __syncthreads();
 
         const int32_t in_tile = min(kAssignTile, a.n_requests - r0);
         // this CTA's runs of 512 tokens that meet the tile's
-        const int64_t end = tok_base + all.tokens;
+        const int64_t end = tok_base + all.tokens, reach = end < 0x7fffffffll ? end : 0x7fffffffll;
         int64_t run = tok_base / kAssignThreads;
         run += (static_cast<int64_t>(blockIdx.x) - run % gridDim.x + gridDim.x) % gridDim.x;
-        for (; run * kAssignThreads < end; run += gridDim.x) {
+        for (; run * kAssignThreads < reach; run += gridDim.x) {
             const int64_t i = run * kAssignThreads + tid;
-            if (i < tok_base || i >= end) continue;
+            if (i < tok_base || i >= reach) continue;
+            const int32_t in_tokens = static_cast<int32_t>(i - tok_base);
             int lo = 0, hi = in_tile;  // the last request whose prefix is at or below the token
             while (hi - lo > 1) {
                 const int mid = (lo + hi) >> 1;
-                if (s_tok[mid] <= i - tok_base) lo = mid;
+                if (s_tok[mid] <= in_tokens) lo = mid;
                 else hi = mid;
             }
             const int32_t r = r0 + lo;
-            const uint32_t l = static_cast<uint32_t>(max(a.lens[r], 0)), f = static_cast<uint32_t>(max(a.fresh[r], 0));
+            const uint32_t l = s_len[lo], f = s_new[lo];
             bool has_room;
             const int64_t n = pages_needed(l, f, page, max_pages, has_room);
-            const bool fits = has_room && (n == 0 || s_page[lo] + n <= count);
-            const uint32_t pos = l + static_cast<uint32_t>(i - tok_base - s_tok[lo]);
+            const bool fits = fits_in(has_room, n, s_page[lo], count, tok_base + s_tok[lo], f);
+            const uint32_t pos = l + static_cast<uint32_t>(in_tokens - s_tok[lo]);
             int64_t slot = -1;
             if (fits) {
-                const uint32_t col = pos / page, off = pos % page, held = l / page + (l % page != 0);
+                const uint32_t col = pos / page, off = pos - col * page.d, held = pages_of(l, page);
                 int32_t* entry = a.table + static_cast<int64_t>(r) * a.table_stride + col;
                 int32_t number;
                 if (col >= held) {
-                    number = a.free_pages[head + s_page[lo] + (col - held)];
+                    number = a.free_pages[static_cast<int64_t>(head) + s_page[lo] + (col - held)];
                     if (off == 0) *entry = number;
                 } else {
                     number = *entry;
                 }
-                slot = static_cast<int64_t>(number) * page + off;
+                slot = static_cast<int64_t>(number) * page.d + off;
             }
             if (i < a.tokens) {
                 a.slots[i] = slot;
@@ -229,7 +255,8 @@ extern "C" int mf_page_assign(const mf_page_config* config, const int32_t* lens,
     if (lens_after == lens || lens_after == new_tokens || pool_after == pool)
         return fail(MF_ERR_INVALID_ARGUMENT, "mf_page_assign: outputs may not be the inputs (lens_after, pool_after)");
     AssignArgs a{lens, new_tokens, free_pages, pool, table, slots, positions, owner, starts, lens_after, pool_after,
-                 tokens, config->table_stride, n_requests, config->page_size, config->max_pages};
+                 tokens, config->table_stride, n_requests, config->max_pages, divisor(config->page_size),
+                 aligned16(lens) && aligned16(new_tokens)};
     const int64_t work = tokens > n_requests ? tokens : n_requests;
     const int64_t grid = stream_grid(work, kAssignThreads, 1);
     page_assign_kernel<<<static_cast<unsigned>(grid), kAssignThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);

@@ -12,6 +12,7 @@
 #include <cmath>
 #include <initializer_list>
 
+#include "mf_divisor.cuh"
 #include "mf_runtime.h"
 #include "mf_vec.cuh"
 
@@ -32,19 +33,6 @@ struct RopeSegment {
     int32_t first;                // heads in front of this segment
     bool turns, cached;
 };
-
-// x / d = (mulhi(x, mul) + x) >> shift for x below 2^31: a division by a number
-// that only the host knows takes three instructions instead of twenty.
-struct Divisor {
-    uint32_t d, mul, shift;
-};
-Divisor divisor(int32_t d) {
-    Divisor v{static_cast<uint32_t>(d), 0, 0};
-    while ((1ull << v.shift) < v.d) ++v.shift;
-    v.mul = static_cast<uint32_t>((((1ull << v.shift) - v.d) << 32) / v.d + 1);
-    return v;
-}
-__device__ __forceinline__ uint32_t operator/(uint32_t x, const Divisor& v) { return (__umulhi(x, v.mul) + x) >> v.shift; }
 
 struct RopeArgs {
     RopeSegment seg[3];
