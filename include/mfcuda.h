@@ -479,7 +479,7 @@ typedef struct mf_cache_layout {
  *   starts[r] = sum of new in front of r, starts[n_requests] = their total;
  *   token i = starts[r] + t: positions[i] = lens[r] + t, owner[i] = r,
  *   slots[i] = table[r][positions[i] / P] * P + positions[i] % P, or -1 if r
- *   does not fit; lens_after[r] = lens[r] + new[r] if it fits, else lens[r];
+ *   does not fit (or that entry of the table is negative); lens_after[r] = lens[r] + new[r] if it fits, else lens[r];
  *   pool_after = {pool[0] + taken, pool[1] - taken, total of new, requests
  *   that do not fit}, taken = the largest before + need that fits.
  * pool is {index of the first free page in free_pages, number of free pages};

@@ -21,6 +21,8 @@ namespace {
 constexpr int kAssignThreads = 512;
 constexpr int kAssignItems = 4;                                // requests per thread and tile
 constexpr int kAssignTile = kAssignThreads * kAssignItems;
+constexpr int kAssignRuns = 3;                                 // runs of tokens in flight
+constexpr uint32_t kNone = 0xffffffffu;
 
 struct AssignArgs {
     const int32_t* lens;
@@ -135,15 +137,13 @@ __global__ void __launch_bounds__(kAssignThreads) page_assign_kernel(const Assig
         __syncthreads();  // the tile before is done with the shared arrays
         if (lane == 31) s_warp[warp] = inc;
         __syncthreads();
-        Sums all{0, 0}, before{0, 0};
-#pragma unroll
-        for (int w = 0; w < kAssignThreads / 32; ++w) {
-            if (w == warp) before = all;
-            all.tokens += s_warp[w].tokens;
-            all.pages += s_warp[w].pages;
-        }
-        before.tokens += inc.tokens - mine.tokens;
-        before.pages += inc.pages - mine.pages;
+        // the warps' sums: every warp scans them itself
+        static_assert(kAssignThreads / 32 <= 32, "");
+        const Sums of_warp = lane < kAssignThreads / 32 ? s_warp[lane] : Sums{0, 0};
+        const Sums upto = warp_inclusive(of_warp, lane);
+        const Sums all{__shfl_sync(0xffffffffu, upto.tokens, 31), __shfl_sync(0xffffffffu, upto.pages, 31)};
+        const Sums before{__shfl_sync(0xffffffffu, upto.tokens - of_warp.tokens, warp) + inc.tokens - mine.tokens,
+                          __shfl_sync(0xffffffffu, upto.pages - of_warp.pages, warp) + inc.pages - mine.pages};
 #pragma unroll
         for (int i = 0; i < kAssignItems; ++i) {
             const int32_t k = tid * kAssignItems + i, r = r0 + k;
@@ -169,39 +169,52 @@ __global__ void __launch_bounds__(kAssignThreads) page_assign_kernel(const Assig
         const int64_t end = tok_base + all.tokens, reach = end < 0x7fffffffll ? end : 0x7fffffffll;
         int64_t run = tok_base / kAssignThreads;
         run += (static_cast<int64_t>(blockIdx.x) - run % gridDim.x + gridDim.x) % gridDim.x;
-        for (; run * kAssignThreads < reach; run += gridDim.x) {
-            const int64_t i = run * kAssignThreads + tid;
-            if (i < tok_base || i >= reach) continue;
-            const int32_t in_tokens = static_cast<int32_t>(i - tok_base);
-            int lo = 0, hi = in_tile;  // the last request whose prefix is at or below the token
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (s_tok[mid] <= in_tokens) lo = mid;
-                else hi = mid;
-            }
-            const int32_t r = r0 + lo;
-            const uint32_t l = s_len[lo], f = s_new[lo];
-            bool has_room;
-            const int64_t n = pages_needed(l, f, page, max_pages, has_room);
-            const bool fits = fits_in(has_room, n, s_page[lo], count, tok_base + s_tok[lo], f);
-            const uint32_t pos = l + static_cast<uint32_t>(in_tokens - s_tok[lo]);
-            int64_t slot = -1;
-            if (fits) {
-                const uint32_t col = pos / page, off = pos - col * page.d, held = pages_of(l, page);
-                int32_t* entry = a.table + static_cast<int64_t>(r) * a.table_stride + col;
-                int32_t number;
-                if (col >= held) {
-                    number = a.free_pages[static_cast<int64_t>(head) + s_page[lo] + (col - held)];
-                    if (off == 0) *entry = number;
-                } else {
-                    number = *entry;
+        // a few runs at a time, so that their loads of page numbers travel together
+        for (; run * kAssignThreads < reach; run += static_cast<int64_t>(kAssignRuns) * gridDim.x) {
+            uint32_t at[kAssignRuns], pos[kAssignRuns];  // request of the tile (kNone: no token here), position
+            int32_t number[kAssignRuns];                 // page (-1: none)
+            bool first_of_page[kAssignRuns];
+#pragma unroll
+            for (int b = 0; b < kAssignRuns; ++b) {
+                const int64_t i = (run + static_cast<int64_t>(b) * gridDim.x) * kAssignThreads + tid;
+                at[b] = kNone;
+                if (i < tok_base || i >= reach) continue;
+                const int32_t in_tokens = static_cast<int32_t>(i - tok_base);
+                int lo = 0, hi = in_tile;  // the last request whose prefix is at or below the token
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) >> 1;
+                    if (s_tok[mid] <= in_tokens) lo = mid;
+                    else hi = mid;
                 }
-                slot = static_cast<int64_t>(number) * page.d + off;
+                const uint32_t l = s_len[lo], f = s_new[lo];
+                bool has_room;
+                const int64_t n = pages_needed(l, f, page, max_pages, has_room);
+                at[b] = lo;
+                pos[b] = l + static_cast<uint32_t>(in_tokens - s_tok[lo]);
+                number[b] = -1;
+                first_of_page[b] = false;
+                if (fits_in(has_room, n, s_page[lo], count, tok_base + s_tok[lo], f)) {
+                    const uint32_t col = pos[b] / page, held = pages_of(l, page);
+                    if (col >= held) {
+                        number[b] = __ldg(a.free_pages + static_cast<int64_t>(head) + s_page[lo] + (col - held));
+                        first_of_page[b] = col * page.d == pos[b];
+                    } else {
+                        number[b] = a.table[static_cast<int64_t>(r0 + lo) * a.table_stride + col];
+                    }
+                }
             }
-            if (i < a.tokens) {
-                a.slots[i] = slot;
-                a.positions[i] = clamp_i32(pos);
-                a.owner[i] = r;
+#pragma unroll
+            for (int b = 0; b < kAssignRuns; ++b) {
+                if (at[b] == kNone) continue;
+                const int64_t i = (run + static_cast<int64_t>(b) * gridDim.x) * kAssignThreads + tid;
+                const int32_t r = r0 + static_cast<int32_t>(at[b]);
+                const uint32_t col = pos[b] / page;
+                if (first_of_page[b]) a.table[static_cast<int64_t>(r) * a.table_stride + col] = number[b];
+                if (i < a.tokens) {
+                    a.slots[i] = number[b] < 0 ? -1 : static_cast<int64_t>(number[b]) * page.d + (pos[b] - col * page.d);
+                    a.positions[i] = clamp_i32(pos[b]);
+                    a.owner[i] = r;
+                }
             }
         }
         tok_base = end;
