@@ -263,8 +263,12 @@ def test_rope_refusals(backend):
     for bad in ({"src": 0}, {"dst": 0}, {"positions": 0}, {"freq": 0}):
         with pytest.raises(InvalidArgument):
             run(**bad)
+    with pytest.raises(ShapeInvalid):
+        run(tokens=1 << 31)
     with pytest.raises(LayoutUnsupported):
         run(dst=x, ss=(64, 64), ds=(128, 64))
+    with pytest.raises(LayoutUnsupported):
+        run(ss=(1 << 31, 64))
     with pytest.raises(InvalidArgument):
         paged.Rope(f, BF16, 64, 64, "spiral")
     run(tokens=0)
@@ -697,6 +701,110 @@ def test_attn_handle_serves_any_batch(backend):
         on.attn.run(1, 1, 1, 1, 1, 1, 1)
 
 
+def test_attn_padded_tables_and_caches(backend):
+    """Table rows and pages that are longer than what they hold; the gaps hold NaN codes."""
+    lens, hq, hkv, dim, page = [1, 45, 0, 130], 4, 2, 64, 16
+    s = make_attn(lens, hq, hkv, dim, page, "NHD", BF16, BF16)
+    want = want_attn(s)
+    n, width = s["table"].shape
+    table = np.full((n, width + 5), 1 << 30, np.int32)
+    table[:, :width] = s["table"]
+    rows, heads = page + 3, hkv + 1  # a page of 16 of 19 rows, 2 of 3 heads, 64 of 72 elements
+    kv = []
+    for c in s["kv"]:
+        wide = np.full((s["pages"], rows, heads, dim + 8), 0x7FFF, np.uint16)
+        wide[:, :page, :hkv, :dim] = c
+        kv.append(to_device(wide))
+    layout = paged.CacheLayout(s["pages"], page, hkv, dim, BF16)
+    layout.struct.page_stride, layout.struct.token_stride = rows * heads * (dim + 8), heads * (dim + 8)
+    layout.struct.head_stride = dim + 8
+    bufs = [to_device(x) for x in (s["q"], table, s["lens"])]
+    out, lse = empty(2 * n * hq * dim), empty(4 * n * hq)
+    with paged.PagedAttention(layout, hq, BF16, width, table_stride=width + 5) as attn:
+        attn.run(bufs[0].ptr, kv[0].ptr, kv[1].ptr, bufs[1].ptr, bufs[2].ptr, n, out.ptr, lse.ptr)
+        sync_device()
+    got = fetch(out, out.nbytes, np.uint16).reshape(n, hq, dim), fetch(lse, lse.nbytes, np.float32).reshape(n, hq)
+    assert device_status() == 0
+    check_attn(s, got, want)
+    for b in (*bufs, *kv, out, lse):
+        b.free()
+
+
+@pytest.mark.parametrize("page", [16, 20])
+def test_offsets_past_32_bits(backend, page):
+    """Pages 2^28 bytes apart: the last of 18 lies past 2^32 bytes.  Written by the append, read by the attention."""
+    hkv, hq, dim, pages, tokens = 1, 2, 64, 18, 50
+    stride = 1 << 27  # elements
+    layout = paged.CacheLayout(pages, page, hkv, dim, BF16, "NHD")
+    layout.struct.page_stride = stride
+    row = (hq + 2 * hkv) * dim
+    x = plain.normal(77, (tokens, hq + 2 * hkv, dim), BF16)
+    used = np.array([17, 3, 16, 0][:-(-tokens // page)], np.int32)
+    tok = np.arange(tokens)
+    slots = used[tok // page].astype(np.int64) * page + tok % page
+    nbytes = 2 * ((pages - 1) * stride + page * hkv * dim)
+    assert nbytes > 1 << 32
+    k, v = empty(nbytes, None), empty(nbytes, None)
+    b = [to_device(a) for a in (x, np.zeros(tokens, np.int32), slots, paged.rope_frequencies(dim), used, np.array([tokens], np.int32))]
+    q_out, out, lse = empty(2 * tokens * hq * dim), empty(2 * hq * dim), empty(4 * hq)
+    a = paged.RopeAppend(paged.Rope(b[3].ptr, BF16, dim), layout, hq, token_stride=row)
+    a.run(b[0].ptr, b[0].ptr + 2 * hq * dim, b[0].ptr + 2 * (hq + hkv) * dim, q_out.ptr, k.ptr, v.ptr, b[1].ptr, b[2].ptr, tokens)
+    sync_device()
+    for i, n in enumerate(used):  # nothing turns at position 0: the pages hold the rows as they are
+        have = min(page, tokens - i * page)
+        for c, at in ((k, hq), (v, hq + hkv)):
+            got = fetch(c, 2 * have * dim, np.uint16, offset=2 * int(n) * stride).reshape(have, 1, dim)
+            bits_equal(got, x[i * page:i * page + have, at:at + 1])
+    with paged.PagedAttention(layout, hq, BF16, len(used)) as attn:
+        attn.run(q_out.ptr + 2 * (tokens - 1) * hq * dim, k.ptr, v.ptr, b[4].ptr, b[5].ptr, 1, out.ptr, lse.ptr)
+        sync_device()
+    assert device_status() == 0
+    xv = plain.values(x, BF16)
+    want = plain.attention(xv[-1, :hq], xv[:, hq:hq + 1], xv[:, hq + 1:], None, 0.125, 0.0, 0, hq)
+    check_attn({"dtype": BF16}, (fetch(out, out.nbytes, np.uint16).reshape(1, hq, dim), fetch(lse, lse.nbytes, np.float32).reshape(1, hq)),
+               tuple(w[None] for w in want))
+    for t in (k, v, *b, q_out, out, lse):
+        t.free()
+
+
+@pytest.mark.parametrize("lens", [[1999], [1000] * 8, [50, 900, 2000], [300] * 40, [130] * 90, [2000, 1, 1, 1, 1, 1]])
+@pytest.mark.parametrize("hq,hkv", [(8, 2), (16, 1)])
+def test_attn_ways_to_share_out_the_work(backend, lens, hq, hkv):
+    """CTAs of their own for each item, with few or many tiles, and the even cut: up to 148 items and past them."""
+    run_attn(lens, hq=hq, hkv=hkv, dim=64)
+
+
+def test_attn_handles_made_again(backend):
+    """A new handle may get an earlier one's workspace: other shapes before and after it change nothing."""
+    s = make_attn([3000, 17], 2, 1, 64, 16, "HND", BF16, BF16)
+    first = Running(s)
+    want = first.run()
+    first.close()
+    for hq, dim in ((32, 256), (4, 64), (2, 128)):
+        run_attn([4000, 3], hq=hq, hkv=1, dim=dim)
+    again = Running(s)
+    got = again.run()
+    again.close()
+    bits_equal(got[0], want[0])
+    bits_equal(got[1].view(np.uint32), want[1].view(np.uint32))
+
+
+def test_attn_lengths_that_ask_for_too_much(backend):
+    """More than 2^31 - 1 tiles (65536 requests over one shared table row of the longest reach): reported, not computed."""
+    n, width = 65536, 1 << 20
+    layout = paged.CacheLayout(4, 16, 1, 64, BF16)
+    lens = to_device(np.full(n, 16 << 20, np.int32))
+    b = [empty(4096) for _ in range(3)]
+    out = empty(n * 64 * 2, 0xA5)
+    with paged.PagedAttention(layout, 1, BF16, width, table_stride=width) as attn:
+        attn.run(b[0].ptr, b[1].ptr, b[1].ptr, b[2].ptr, lens.ptr, n, out.ptr)
+        sync_device()
+        assert device_status() == 0x7300
+    assert (fetch(out, out.nbytes) == 0xA5).all()
+    for t in (*b, out, lens):
+        t.free()
+
+
 def test_attn_refusals(backend):
     def make(dtype=BF16, cache=BF16, hq=4, hkv=2, dim=64, page=16, max_pages=4, stride=None, **more):
         paged.PagedAttention(paged.CacheLayout(4, page, hkv, dim, cache), hq, dtype, max_pages, stride, **more).close()
@@ -714,6 +822,11 @@ def test_attn_refusals(backend):
     for bad in ({"q_strides": (256, 63)}, {"out_strides": (258, 64)}):
         with pytest.raises(LayoutUnsupported):
             make(**bad)
+    for stride in (-64, 1 << 31):
+        layout = paged.CacheLayout(4, 16, 2, 64, BF16)
+        layout.struct.page_stride = stride
+        with pytest.raises(LayoutUnsupported):
+            paged.PagedAttention(layout, 4, BF16, 4)
     for bad in ({"window": -1}, {"softcap": -1.0}, {"softcap": float("nan")}):
         with pytest.raises(InvalidArgument):
             make(**bad)
