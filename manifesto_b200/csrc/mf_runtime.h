@@ -50,6 +50,25 @@ inline bool is_decodable(int dt) {
     return dt >= MF_DT_F64 && dt <= MF_DT_U8;
 }
 
+// Launch a kernel that may be set up while the one before it in the stream
+// still runs (programmatic dependent launch).  Such a kernel calls
+// after_previous() (mf_launch.cuh) before it touches memory: that returns when
+// everything before it in the stream is done and visible.
+template <class... Params, class... Args>
+cudaError_t launch_overlapped(void (*kernel)(Params...), dim3 grid, int threads, size_t shared, cudaStream_t s, Args... args) {
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = grid;
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = shared;
+    config.stream = s;
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, kernel, args...);
+}
+
 }  // namespace mf
 
 #define MF_CUDA_CHECK(expr)                                  \

@@ -37,6 +37,7 @@
 
 #include "mf_divisor.cuh"
 #include "mf_internal.h"
+#include "mf_launch.cuh"
 #include "mf_runtime.h"
 #include "mf_vec.cuh"
 
@@ -474,6 +475,8 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
     const int g = lane >> 2, j = lane & 3;  // row and column pair of a product's fragment
     const int32_t items = a.items;
 
+    after_previous();
+    let_next_start();
     // the tiles of thread i's `per` consecutive requests
     const int32_t per = (a.n_requests + K::kThreads - 1) / K::kThreads;
     int64_t sum = 0;
@@ -1423,9 +1426,9 @@ extern "C" int mf_paged_attn_run(mf_paged_attn handle, const void* q, const void
     a.n_requests = n_requests;
     a.out = static_cast<char*>(out);
     a.lse = lse;
-    handle->kernel.fn<<<static_cast<unsigned>(handle->ctas), handle->kernel.threads, handle->kernel.shared,
-                        static_cast<cudaStream_t>(stream)>>>(a);
-    MF_LAUNCH_CHECK("mf_paged_attn_run");
+    const cudaError_t err = launch_overlapped(handle->kernel.fn, dim3(static_cast<unsigned>(handle->ctas)), handle->kernel.threads,
+                                              handle->kernel.shared, static_cast<cudaStream_t>(stream), a);
+    if (err != cudaSuccess) return cuda_fail(err, "mf_paged_attn_run");
     return MF_OK;
 }
 

@@ -13,6 +13,7 @@
 // and one chain of dependent loads for a decoding step; the 16 bytes written
 // per token for a long prompt.
 #include "mf_divisor.cuh"
+#include "mf_launch.cuh"
 #include "mf_runtime.h"
 
 namespace mf {
@@ -96,6 +97,8 @@ __global__ void __launch_bounds__(kAssignThreads) page_assign_kernel(const Assig
     __shared__ long long s_taken;
     __shared__ int s_refused;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    after_previous();
+    let_next_start();
     const Divisor page = a.page;
     const uint32_t max_pages = static_cast<uint32_t>(a.max_pages);
     const int32_t head = a.pool[0] < 0 ? 0 : a.pool[0];
@@ -272,7 +275,8 @@ extern "C" int mf_page_assign(const mf_page_config* config, const int32_t* lens,
                  aligned16(lens) && aligned16(new_tokens)};
     const int64_t work = tokens > n_requests ? tokens : n_requests;
     const int64_t grid = stream_grid(work, kAssignThreads, 1);
-    page_assign_kernel<<<static_cast<unsigned>(grid), kAssignThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
-    MF_LAUNCH_CHECK("mf_page_assign");
+    const cudaError_t err = launch_overlapped(page_assign_kernel, dim3(static_cast<unsigned>(grid)), kAssignThreads, 0,
+                                              static_cast<cudaStream_t>(stream), a);
+    if (err != cudaSuccess) return cuda_fail(err, "mf_page_assign");
     return MF_OK;
 }

@@ -13,6 +13,7 @@
 #include <initializer_list>
 
 #include "mf_divisor.cuh"
+#include "mf_launch.cuh"
 #include "mf_runtime.h"
 #include "mf_vec.cuh"
 
@@ -140,6 +141,8 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a) {
     __shared__ __align__(16) float s_cos[kRopeTableFloats / 2];
     __shared__ __align__(16) float s_sin[kRopeTableFloats / 2];
     const int32_t t0 = static_cast<int32_t>(blockIdx.x * a.tokens_per_cta);
+    after_previous();
+    let_next_start();
     const int n_tok = min(a.tokens_per_cta, a.tokens - t0);
     const int half = a.rot >> 1;
     for (int i = threadIdx.x; i < n_tok * half; i += kRopeThreads) {
@@ -229,10 +232,10 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a) {
 }
 
 template <int IN, int CACHE>
-void launch_rope(const RopeArgs& a, int vec, dim3 grid, cudaStream_t s) {
-    if (vec == 8) rope_kernel<IN, CACHE, 8><<<grid, kRopeThreads, 0, s>>>(a);
-    else if (vec == 4) rope_kernel<IN, CACHE, 4><<<grid, kRopeThreads, 0, s>>>(a);
-    else rope_kernel<IN, CACHE, 1><<<grid, kRopeThreads, 0, s>>>(a);
+cudaError_t launch_rope(const RopeArgs& a, int vec, dim3 grid, cudaStream_t s) {
+    if (vec == 8) return launch_overlapped(rope_kernel<IN, CACHE, 8>, grid, kRopeThreads, 0, s, a);
+    if (vec == 4) return launch_overlapped(rope_kernel<IN, CACHE, 4>, grid, kRopeThreads, 0, s, a);
+    return launch_overlapped(rope_kernel<IN, CACHE, 1>, grid, kRopeThreads, 0, s, a);
 }
 
 // Whether accesses of `vec` elements are aligned: base address, both strides.
@@ -282,26 +285,27 @@ int finish_and_launch(const char* name, RopeArgs& a, const mf_rope_config* c, in
         if (split < 1) split = 1;
     }
     const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(split));
+    cudaError_t err;
     switch (c->dtype) {
     case MF_DT_F32:
-        if (cache_dt == MF_DT_F32) launch_rope<MF_DT_F32, MF_DT_F32>(a, vec, grid, s);
-        else if (cache_dt == MF_DT_F8E4M3) launch_rope<MF_DT_F32, MF_DT_F8E4M3>(a, vec, grid, s);
-        else if (cache_dt == MF_DT_F8E5M2) launch_rope<MF_DT_F32, MF_DT_F8E5M2>(a, vec, grid, s);
-        else launch_rope<MF_DT_F32, MF_DT_INVALID>(a, vec, grid, s);
+        if (cache_dt == MF_DT_F32) err = launch_rope<MF_DT_F32, MF_DT_F32>(a, vec, grid, s);
+        else if (cache_dt == MF_DT_F8E4M3) err = launch_rope<MF_DT_F32, MF_DT_F8E4M3>(a, vec, grid, s);
+        else if (cache_dt == MF_DT_F8E5M2) err = launch_rope<MF_DT_F32, MF_DT_F8E5M2>(a, vec, grid, s);
+        else err = launch_rope<MF_DT_F32, MF_DT_INVALID>(a, vec, grid, s);
         break;
     case MF_DT_BF16:
-        if (cache_dt == MF_DT_BF16) launch_rope<MF_DT_BF16, MF_DT_BF16>(a, vec, grid, s);
-        else if (cache_dt == MF_DT_F8E4M3) launch_rope<MF_DT_BF16, MF_DT_F8E4M3>(a, vec, grid, s);
-        else if (cache_dt == MF_DT_F8E5M2) launch_rope<MF_DT_BF16, MF_DT_F8E5M2>(a, vec, grid, s);
-        else launch_rope<MF_DT_BF16, MF_DT_INVALID>(a, vec, grid, s);
+        if (cache_dt == MF_DT_BF16) err = launch_rope<MF_DT_BF16, MF_DT_BF16>(a, vec, grid, s);
+        else if (cache_dt == MF_DT_F8E4M3) err = launch_rope<MF_DT_BF16, MF_DT_F8E4M3>(a, vec, grid, s);
+        else if (cache_dt == MF_DT_F8E5M2) err = launch_rope<MF_DT_BF16, MF_DT_F8E5M2>(a, vec, grid, s);
+        else err = launch_rope<MF_DT_BF16, MF_DT_INVALID>(a, vec, grid, s);
         break;
     default:
-        if (cache_dt == MF_DT_F16) launch_rope<MF_DT_F16, MF_DT_F16>(a, vec, grid, s);
-        else if (cache_dt == MF_DT_F8E4M3) launch_rope<MF_DT_F16, MF_DT_F8E4M3>(a, vec, grid, s);
-        else if (cache_dt == MF_DT_F8E5M2) launch_rope<MF_DT_F16, MF_DT_F8E5M2>(a, vec, grid, s);
-        else launch_rope<MF_DT_F16, MF_DT_INVALID>(a, vec, grid, s);
+        if (cache_dt == MF_DT_F16) err = launch_rope<MF_DT_F16, MF_DT_F16>(a, vec, grid, s);
+        else if (cache_dt == MF_DT_F8E4M3) err = launch_rope<MF_DT_F16, MF_DT_F8E4M3>(a, vec, grid, s);
+        else if (cache_dt == MF_DT_F8E5M2) err = launch_rope<MF_DT_F16, MF_DT_F8E5M2>(a, vec, grid, s);
+        else err = launch_rope<MF_DT_F16, MF_DT_INVALID>(a, vec, grid, s);
     }
-    MF_LAUNCH_CHECK(name);
+    if (err != cudaSuccess) return cuda_fail(err, name);
     return MF_OK;
 }
 
