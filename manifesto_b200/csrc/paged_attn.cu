@@ -11,27 +11,42 @@
 // key-value head only (4 operations per element and query head: 8 heads on
 // BF16 are 32 operations for 2 bytes), far below what tensor cores need to
 // be the limit, so the design is about keeping loads in flight:
-//   * The work is cut into tiles of 16 tokens of one (request, key-value head,
-//     block of 8 * NT query heads) item, laid end to end over all requests;
-//     every warp of the grid takes an equal run of tiles, whatever the lengths.
-//   * A warp works alone: its own ring of stages in shared memory filled by
-//     16-byte cp.async (rows of masked tokens are zero-filled, not read), no
-//     CTA barrier inside the loop.  Page numbers are read one tile ahead.
+//   * The work is cut into tiles of 16 or 32 tokens (8 KB of keys and values
+//     where a row has up to 256 bytes) of one item: a request, a key-value head
+//     and a block of its query heads.  The tiles of all items in a row are cut
+//     evenly for the teams of the grid, whatever the lengths; a small batch's
+//     items get CTAs of their own.
+//   * A team is a warp, or two that share a ring where more than 8 query heads
+//     share a key-value head.  It works alone: a ring of stages in shared
+//     memory filled by 16-byte cp.async (rows of masked tokens are zero-filled,
+//     not read), no CTA barrier inside the loop, page numbers read one tile
+//     ahead.  Twelve warps per SM; copying warps that feed the others were
+//     slower (108 us with four of them for the 92 below: a copy instruction of
+//     512 bytes needs more issue slots than a few warps have), and so were
+//     bulk copies a row at a time (67 clocks each per issuing warp).
 //   * Products run on mma.m16n8k16 with tokens (then head_dim) on the long side
-//     and query heads on the side of 8: S^T = K Q^T and O^T = V^T P^T, so one
-//     key-value head with up to 8 query heads wastes nothing more; the weights
-//     move from the first product's result layout to the second's operand
-//     layout by movmatrix, in registers.  The wide tensor-core form
-//     (tcgen05) needs 64 or more rows of queries to be fed: there are 1 to 16.
+//     and query heads on the side of 8: S^T = K Q^T and O^T = V^T P^T.  The
+//     weights move from the first product's result layout to the second's
+//     operand layout by movmatrix, in registers.  The wide tensor-core form
+//     (tcgen05) needs 64 or more rows of queries to be fed: there are 1 to 16;
+//     the tensor pipe is 14% (BF16) to 23% (FP8) busy.
 //   * exp(s - m) is rounded to two 16-bit terms (high and low), so the weights
 //     carry 16 bits (BF16) or more and the result's only 16-bit rounding that
-//     counts is the final one.
+//     counts is the final one.  (One f16 term for FP8 caches missed the bound
+//     that two terms give.)
 //   * FP8 codes become f16 in registers (exact); the queries are then f16 too,
 //     scaled by a power of two per head so that none overflows.
-// Where a run of tiles ends inside an item, the warps of a CTA join their
+// Where a run of tiles ends inside an item, the teams of a CTA join their
 // parts in shared memory, CTAs through the workspace: the last of an item's
 // CTAs to arrive (a ticket) joins them in the order of the tokens, so the
 // result does not depend on who was last.
+//
+// Measured (B200, keys and values in the loop come at 7.4 TB/s, the copy rate
+// of the roofline is 6.55): 64 requests of 2048 tokens, 32/8 heads of 128: BF16
+// 92 us (82 at the copy rate), E4M3 55 us (41); 2 of 131071: 162 us (164); the
+// same 64 with 16/8 heads of 256: 171 us (164).  What a call costs besides:
+// about 3 us until the first tile is there and 4 to 6 us for the joins, mostly
+// instruction fetches of code that runs once.
 #include <mutex>
 #include <new>
 
