@@ -75,6 +75,7 @@ struct AttnArgs {
     int64_t head_bytes, table_stride;
     uint32_t n_pages;
     Divisor by_page;
+    Divisor used_heads;   // query heads of an item that has all of its own
     int32_t head_dim;
     const char* q;
     int64_t q_req, q_head;
@@ -197,11 +198,10 @@ __device__ __forceinline__ float rescale(float m_old, float m_new) {
     return m_old == m_new ? 1.0f : exp2_fast(m_old - m_new);
 }
 
-// tanh(x) = 1 - 2 / (1 + exp(2x)): 2^-22 of 1, the limits at both ends.
-__device__ __forceinline__ float tanh_fast(float x) {
+__device__ __forceinline__ float rcp_fast(float x) {
     float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + exp2_fast(2.0f * kLog2e * x)));
-    return __fmaf_rn(-2.0f, r, 1.0f);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
 }
 
 // A request's tokens: [first, len) are seen, in tiles from `base` on (a multiple
@@ -488,7 +488,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int team = warp / TM, member = warp % TM;
     const int g = lane >> 2, j = lane & 3;  // row and column pair of a product's fragment
-    const int32_t items = a.items;
+    const int32_t items = a.items, used_heads = a.used_heads.d;
 
     after_previous();
     let_next_start();
@@ -767,7 +767,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
         const int v_row = K::kFp8 ? k_row : (lane & 7) + (lane >> 4) * 8, v_piece = K::kFp8 ? k_piece : (lane >> 3) & 1;
         const uint32_t k_at = ring + swizzled<K::kChunks>(k_row, k_piece);
         const uint32_t v_at = ring + T * K::kRow + swizzled<K::kChunks>(v_row, v_piece);
-        const bool rules = a.softcap > 0.0f || a.slopes;
+        const float cap = a.softcap * kLog2e;
         int stage = 0, fill = 0;  // the stages of the tile at hand and of the next to be copied
         int32_t done = 0;
         while (done < my_tiles) {
@@ -813,7 +813,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                     const float b = __shfl_sync(0xffffffffu, back, (2 * j + x) * 4);
                     const int hx = member * 8 + 2 * j + x;
                     scale[x] = a.scale * ks * b;
-                    scale[x] = a.softcap > 0.0f ? __fdiv_rn(scale[x], a.softcap) : scale[x] * kLog2e;
+                    scale[x] = a.softcap > 0.0f ? __fdiv_rn(scale[x], a.softcap) * (2.0f * kLog2e) : scale[x] * kLog2e;
                     slope[x] = a.slopes && hx < hd.count ? __ldg(a.slopes + hd.head0 + hx) * kLog2e : 0.0f;
                     m[x] = high[x] = -INFINITY;
                     less[x] = l[x] = 0.0f;
@@ -871,14 +871,17 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                 for (int b = 0; b < K::kBlocks; ++b) {
 #pragma unroll
                     for (int x = 0; x < 4; ++x) p[b][x] = (s[b][0][x] + s[b][1][x]) * scale[x & 1];
-                    if (rules) {
+                    if (a.softcap > 0.0f) {
+                        // cap tanh(y) = cap - 2 cap / (1 + exp(2y)), 2^-22 of the cap, its limits at both ends
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) p[b][x] = __fmaf_rn(-2.0f * cap, rcp_fast(1.0f + exp2_fast(p[b][x])), cap);
+                    }
+                    if (a.slopes) {
                         // distance to the newest token, <= 0
                         const float away = static_cast<float>(at.span.base + t * T + b * kBlock + g - (at.span.len - 1));
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            if (a.softcap > 0.0f) p[b][x] = a.softcap * kLog2e * tanh_fast(p[b][x]);
+                        for (int x = 0; x < 4; ++x)
                             p[b][x] = __fmaf_rn(slope[x & 1], away + (x & 2 ? 8.0f : 0.0f), p[b][x]);
-                        }
                     }
                     if (mask != K::kAll) {
 #pragma unroll
@@ -1013,6 +1016,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
                         const int h = member * 8 + 2 * j + x;
+                        if (h >= used_heads) break;
                         if (g == 0) {
                             sh.m[2 * team][h] = m[x];
                             sh.l[2 * team][h] = l[x];
@@ -1055,6 +1059,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
             const int h = member * 8 + 2 * j + x;
+            if (h >= used_heads) break;
             if (g == 0) {
                 sh.m[2 * team + 1][h] = m[x];
                 sh.l[2 * team + 1][h] = l[x];
@@ -1091,7 +1096,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
     __syncthreads();
 
     // Join the parts of each item inside the CTA.  First the parts' weights: a warp for each head, a lane for each part.
-    for (int h = warp; h < K::kHeads; h += W) {
+    for (int h = warp; h < used_heads; h += W) {
         const bool is = start >= 0;
         const float mine = is ? sh.m[lane][h] : -INFINITY;
         float top = mine;
@@ -1118,29 +1123,26 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
     cp_async_wait<0>();
     __syncthreads();
     const int32_t joined = sh.items;
-    for (int i = tid; i < joined * K::kHeads * K::kFour; i += K::kThreads) {
-        const int which = i / (K::kHeads * K::kFour), h = i / K::kFour % K::kHeads, d = i % K::kFour * 4;
+    for (int i = tid; i < joined * used_heads * K::kFour; i += K::kThreads) {
+        const uint32_t e = static_cast<uint32_t>(i) / K::kFour;
+        const int which = e / a.used_heads, h = e - which * used_heads, d = i % K::kFour * 4;
         const Joined& w = sh.joined[which];
+        if (h >= w.heads) continue;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         for (uint32_t parts = w.parts; parts;) {
             float4 f[4];
-            float by[4];
+            int k[4];
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-                const int k = parts ? __ffs(parts) - 1 : -1;
+                k[x] = parts ? __ffs(parts) - 1 : -1;
                 parts &= parts - 1;
-                by[x] = 0.0f;
-                f[x] = acc;
-                if (k >= 0) {
-                    by[x] = sh.m[k][h];
-                    f[x] = *reinterpret_cast<const float4*>(staged + (k * K::kHeads + h) * K::kLd + d);
-                }
+                if (k[x] >= 0) f[x] = *reinterpret_cast<const float4*>(staged + (k[x] * K::kHeads + h) * K::kLd + d);
             }
 #pragma unroll
-            for (int x = 0; x < 4; ++x) acc = x > 0 && by[x] == 0.0f ? acc : fma4(f[x], by[x], acc);
+            for (int x = 0; x < 4; ++x)
+                if (k[x] >= 0) acc = fma4(f[x], sh.m[k[x]][h], acc);
         }
         const float top = sh.joined_m[which][h], sum_l = sh.joined_l[which][h];
-        if (h >= w.heads) continue;
         if (w.slot < 0) {
             const float vs = a.v_scale ? __ldg(a.v_scale + w.kv) : 1.0f;
             store_out4(a, w.r, w.head0 + h, d, scale4(acc, sum_l == 0.0f ? 0.0f : __fdiv_rn(vs, sum_l)));
@@ -1254,7 +1256,9 @@ namespace mf {
 namespace {
 
 // Workspaces of destroyed handles, for the next ones: allocating one takes
-// from half a millisecond to three.  Their tickets are zero, as every run leaves them.
+// from half a millisecond to three.  Their tickets are zero, as every run
+// leaves them; whoever takes one waits for the device first, so that no run of
+// its earlier handle goes on.
 constexpr int kKept = 8;
 struct Kept {
     void* p;
@@ -1357,7 +1361,14 @@ extern "C" int mf_paged_attn_create(const mf_paged_attn_config* config, mf_paged
     const size_t tickets = (static_cast<size_t>(ctas) * 8 + 255) / 256 * 256;
     h->bytes = bytes;
     h->workspace = take_kept(bytes, state().device, &h->bytes);
-    if (!h->workspace) {
+    if (h->workspace) {
+        const cudaError_t err = cudaDeviceSynchronize();
+        if (err != cudaSuccess) {
+            keep(h->workspace, h->bytes, state().device);
+            delete h;
+            return cuda_fail(err, "mf_paged_attn_create: cudaDeviceSynchronize");
+        }
+    } else {
         cudaError_t err = cudaMalloc(&h->workspace, bytes);
         if (err != cudaSuccess) {
             cudaGetLastError();
@@ -1404,6 +1415,7 @@ extern "C" int mf_paged_attn_create(const mf_paged_attn_config* config, mf_paged
     a.page = k.page_size;
     a.max_pages = c.max_pages;
     a.by_page = divisor(a.page);
+    a.used_heads = divisor(group < (group <= 8 ? 8 : 16) ? group : group <= 8 ? 8 : 16);
     a.window = c.window;
     a.q_f16 = c.q_dtype == MF_DT_F16;
     a.scale = c.scale;
@@ -1450,7 +1462,6 @@ extern "C" int mf_paged_attn_run(mf_paged_attn handle, const void* q, const void
 extern "C" int mf_paged_attn_destroy(mf_paged_attn handle) {
     if (!handle) return MF_OK;
     MF_ENTER();
-    MF_CUDA_CHECK(cudaDeviceSynchronize());  // as freeing it would: no run of the handle goes on
     if (!keep(handle->workspace, handle->bytes, handle->device)) MF_CUDA_CHECK(cudaFree(handle->workspace));
     delete handle;
     return MF_OK;
