@@ -586,7 +586,7 @@ typedef struct mf_paged_attn_config {
     int32_t window;       /* 0: all tokens */
     int64_t table_stride; /* int32 entries */
     float scale;
-    float softcap;            /* 0: none */
+    float softcap;            /* 0: none; finite */
     const float* slopes;      /* [q_heads] on the device, or NULL */
     const float* k_scale_inv; /* [kv_heads] on the device, or NULL */
     const float* v_scale_inv;

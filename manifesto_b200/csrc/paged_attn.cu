@@ -277,6 +277,9 @@ constexpr int kJoin = 16;  // most parts that one step of a join between CTAs ta
 // A maximum is only replaced by one that is this much larger (in powers of two): until then the weights grow up to
 // 2^8, which float32 sums and both terms of a weight hold as well, and what is summed is not rescaled.
 constexpr float kLazy = 8.0f;
+// Up to this cap 2^-22 of it, the error of the short form of its tanh, is 1.5e-5 of a score, no more than what the sum
+// of the products leaves.
+constexpr float kWideCap = 64.0f;
 // MODE: dtype of the cache; DP: head_dim padded to 64, 128 or 256; TM: warps of a team; W: warps; T: tokens of a
 // tile; S: stages of a team's ring.  A team works on one item at a time, each of its warps for 8 query heads.
 template <int MODE, int DP, int TM, int W, int T, int S>
@@ -871,7 +874,11 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                 for (int b = 0; b < K::kBlocks; ++b) {
 #pragma unroll
                     for (int x = 0; x < 4; ++x) p[b][x] = (s[b][0][x] + s[b][1][x]) * scale[x & 1];
-                    if (a.softcap > 0.0f) {
+                    if (a.softcap > kWideCap) {
+                        // p is 2 log2(e) y; relative to the score, which may be far below the cap
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) p[b][x] = cap * tanhf(p[b][x] * (0.5f / kLog2e));
+                    } else if (a.softcap > 0.0f) {
                         // cap tanh(y) = cap - 2 cap / (1 + exp(2y)), 2^-22 of the cap, its limits at both ends
 #pragma unroll
                         for (int x = 0; x < 4; ++x) p[b][x] = __fmaf_rn(-2.0f * cap, rcp_fast(1.0f + exp2_fast(p[b][x])), cap);
@@ -1345,7 +1352,7 @@ extern "C" int mf_paged_attn_create(const mf_paged_attn_config* config, mf_paged
         return fail(MF_ERR_LAYOUT_UNSUPPORTED, "mf_paged_attn_create: cache strides may not be negative, a page is below 2 GB");
     if (c.q_token_stride % 2 || c.q_head_stride % 2 || c.out_token_stride % 4 || c.out_head_stride % 4)
         return fail(MF_ERR_LAYOUT_UNSUPPORTED, "mf_paged_attn_create: query strides must be even, output strides multiples of 4");
-    if (c.window < 0 || !(c.softcap >= 0.0f))
+    if (c.window < 0 || !(c.softcap >= 0.0f && c.softcap < INFINITY))
         return fail(MF_ERR_INVALID_ARGUMENT, "mf_paged_attn_create: window %d, softcap %g", c.window, c.softcap);
     const int group = c.q_heads / k.kv_heads;
     Kernel kernel = pick(k.dtype, group, k.head_dim);

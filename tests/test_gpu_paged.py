@@ -867,3 +867,17 @@ def test_decoding_steps_of_the_example(backend, cache, most):
     spec.loader.exec_module(example)
     worst = example.run(cache_dtype=cache)
     assert len(worst) == 5 and max(worst) <= most
+
+
+@pytest.mark.parametrize("cache", [BF16, E4M3])
+@pytest.mark.parametrize("softcap", [64.0, 65.0, 1000.0, 1e6])
+def test_attn_wide_caps(backend, softcap, cache):
+    """A cap far above the scores leaves them as they are: its tanh has to be good relative to the score, not to the
+    cap.  Up to 64 an error of 2^-22 of the cap is 1.5e-5, inside the usual bound; above, relative errors of 2^-22."""
+    for dim, hq, hkv in ((64, 4, 2), (128, 18, 2), (256, 4, 2)):
+        run_attn([1, 90, 1500, 0], cache=cache, softcap=softcap, dim=dim, hq=hq, hkv=hkv)
+
+
+def test_attn_refuses_an_infinite_cap(backend):
+    with pytest.raises(InvalidArgument):
+        paged.PagedAttention(paged.CacheLayout(4, 16, 2, 64, BF16), 4, BF16, 4, softcap=float("inf"))
