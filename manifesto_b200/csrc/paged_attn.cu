@@ -318,7 +318,8 @@ struct Attn {
         float weight[kJoin][kHeads], top[kHeads], sum[kHeads];
         uint32_t mask[kTeams][S];       // tokens of each stage that are there
         int32_t items;                  // joined items
-        int32_t won[2];                 // whether this CTA joins the item of its slot
+        int32_t won[2];                 // whether this CTA joins its group of the item of its slot
+        int32_t won_groups[2];          // and whether it joins that item's groups
         int32_t first[2], last[2], size[2];  // that item's CTAs, and how many join at a time
     };
     static constexpr int kSharedBytes = kBuffer + static_cast<int>(sizeof(Shared));
@@ -1203,9 +1204,9 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
         for (int level = 0; level < 2; ++level) {
             if (level == 1) {
                 if (groups == 1) break;
-                if (tid == 0) sh.won[slot] = arrive_last(a.tickets + gridDim.x + first, groups);
+                if (tid == 0) sh.won_groups[slot] = arrive_last(a.tickets + gridDim.x + first, groups);
                 __syncthreads();
-                if (!sh.won[slot]) break;
+                if (!sh.won_groups[slot]) break;
                 const int32_t in_last = (last - first) % size + 1;
                 parts = at0 = a.cta_part + first * kCta + 2 * K::kPart;
                 at_end = a.cta_part + (last - in_last + 1) * kCta + (in_last == 1 ? 0 : 2 * K::kPart);
