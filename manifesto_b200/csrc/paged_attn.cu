@@ -44,7 +44,7 @@
 // Measured (B200, keys and values in the loop come at 7.4 TB/s, the copy rate
 // of the roofline is 6.55): 64 requests of 2048 tokens, 32/8 heads of 128: BF16
 // 92 us (82 at the copy rate), E4M3 55 us (41); 2 of 131071: 162 us (164); the
-// same 64 with 16/8 heads of 256: 171 us (164).  What a call costs besides:
+// same 64 with 16/8 heads of 256: 168 us (164).  What a call costs besides:
 // about 3 us until the first tile is there and 4 to 6 us for the joins, mostly
 // instruction fetches of code that runs once.
 #include <mutex>
@@ -278,7 +278,8 @@ constexpr int kJoin = 16;  // most parts that one step of a join between CTAs ta
 // 2^8, which float32 sums and both terms of a weight hold as well, and what is summed is not rescaled.
 constexpr float kLazy = 8.0f;
 // Up to this cap 2^-22 of it, the error of the short form of its tanh, is 1.5e-5 of a score, no more than what the sum
-// of the products leaves.
+// of the products leaves; above it tanhf is exact enough relative to the score.  (Its code alone costs E4M3 caches with a
+// smaller cap 1%: 256 requests ragged to 8192 tokens 390 -> 394 us.)
 constexpr float kWideCap = 64.0f;
 // MODE: dtype of the cache; DP: head_dim padded to 64, 128 or 256; TM: warps of a team; W: warps; T: tokens of a
 // tile; S: stages of a team's ring.  A team works on one item at a time, each of its warps for 8 query heads.
