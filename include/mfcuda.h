@@ -569,8 +569,10 @@ int mf_rope_append(const mf_rope_append_config* config, const void* q, const voi
  * head_dim contiguous; lse (may be NULL): float32 [n_requests, q_heads].  The
  * cache's dtype is q_dtype, F8E4M3 or F8E5M2; head_dim is a multiple of 8 (of
  * 16 for FP8) up to 256; cache buffers and strides are multiples of 16 bytes.
- * Products and sums are float32, the weights exp(s - max) enter the product
- * with the values as two 16-bit terms (their sum has 16 bits or more).
+ * Products and sums are float32.  The weights exp(s - max) enter the product
+ * with the values as two 16-bit terms: for a BF16 cache off by at most 2^-16
+ * of themselves, for an F16 or FP8 cache by 2^-22 of themselves or 2^-37 of
+ * the request's largest weight, whichever is more.
  *
  * One run covers up to 2^31 - 1 tiles (16 tokens of one key-value head, for up
  * to 16 query heads); lengths that ask for more record MF_DEVICE_TOO_LARGE.

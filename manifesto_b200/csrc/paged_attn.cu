@@ -30,10 +30,11 @@
 //     operand layout by movmatrix, in registers.  The wide tensor-core form
 //     (tcgen05) needs 64 or more rows of queries to be fed: there are 1 to 16;
 //     the tensor pipe is 14% (BF16) to 23% (FP8) busy.
-//   * exp(s - m) is rounded to two 16-bit terms (high and low), so the weights
-//     carry 16 bits (BF16) or more and the result's only 16-bit rounding that
-//     counts is the final one.  (One f16 term for FP8 caches missed the bound
-//     that two terms give.)
+//   * exp(s - m) is rounded to two 16-bit terms (high and low).  Two BF16 terms
+//     carry 16 bits of any weight, two f16 terms 22 bits of the large ones and,
+//     since f16 ends at 2^-24, no more than 2^-25 absolutely: the f16 forms put
+//     m below the maximum (see kBelow), so that this is 2^-37 of the largest
+//     weight.  (One f16 term for FP8 caches missed the bound that two give.)
 //   * FP8 codes become f16 in registers (exact); the queries are then f16 too,
 //     scaled by a power of two per head so that none overflows.
 // Where a run of tiles ends inside an item, the teams of a CTA join their
@@ -274,9 +275,6 @@ struct Joined {
 
 constexpr int kFills = 3;  // ways to give each item CTAs of its own
 constexpr int kJoin = 16;  // most parts that one step of a join between CTAs takes
-// A maximum is only replaced by one that is this much larger (in powers of two): until then the weights grow up to
-// 2^8, which float32 sums and both terms of a weight hold as well, and what is summed is not rescaled.
-constexpr float kLazy = 8.0f;
 // Up to this cap 2^-22 of it, the error of the short form of its tanh, is 1.5e-5 of a score, no more than what the sum
 // of the products leaves; above it tanhf is exact enough relative to the score.  (Its code alone costs E4M3 caches with a
 // smaller cap 1%: 256 requests ragged to 8192 tokens 390 -> 394 us.)
@@ -287,6 +285,12 @@ template <int MODE, int DP, int TM, int W, int T, int S>
 struct Attn {
     static constexpr bool kFp8 = MODE == MF_DT_F8E4M3 || MODE == MF_DT_F8E5M2;
     static constexpr bool kBf16 = MODE == MF_DT_BF16;
+    // Weights are exp2(s - m), m a maximum less kBelow.  It is only replaced when a score exceeds it by kAbove: until
+    // then the weights grow up to 2^kAbove and what is summed is not rescaled.  BF16 terms and float32 sums hold any
+    // weight: m is a maximum itself.  f16 terms end at 2^16 and at 2^-24: 2^15 at the top leaves the small ones of
+    // a token that leads by 18 (2^-26) 11 bits, where a maximum as m left none.
+    static constexpr float kBelow = kBf16 ? 0.0f : 12.0f;
+    static constexpr float kAbove = kBf16 ? 8.0f : 15.0f;
     static constexpr int kBytes = kFp8 ? 1 : 2;
     static constexpr int kRow = DP * kBytes;          // bytes of a token's row
     static constexpr int kChunks = kRow / 16;         // 16-byte pieces of it
@@ -777,7 +781,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
         int32_t done = 0;
         while (done < my_tiles) {
             const int32_t ta = at.t, tb = min(at.nt, ta + my_tiles - done);
-            float scale[2], slope[2], less[2], high[2];  // less: m, or 0 while it is -inf; high: what raises the maximum
+            float scale[2], slope[2], less[2], high[2];  // less: m, or 0 while it is -inf; high: what raises m
             {
                 // a new item; its queries were loaded while the one before it ended
                 const Heads<K::kHeads> hd(a, at.item);
@@ -906,11 +910,11 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                         top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 4));
                         top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 8));
                         top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 16));
-                        top[x] = fmaxf(top[x], m[x]);
-                        const float r = rescale(m[x], top[x]);
-                        m[x] = top[x];
-                        high[x] = top[x] + kLazy;
-                        less[x] = top[x] == -INFINITY ? 0.0f : top[x];
+                        const float next = fmaxf(top[x] - K::kBelow, m[x]);
+                        const float r = rescale(m[x], next);
+                        m[x] = next;
+                        high[x] = __fadd_rd(next, K::kAbove);  // down: 2^16 would be past f16
+                        less[x] = next == -INFINITY ? 0.0f : next;
                         l[x] *= r;
 #pragma unroll
                         for (int c = 0; c < K::kSteps; ++c) {
@@ -919,7 +923,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                         }
                     }
                 }
-                // weights; while nothing is seen, the maximum is -inf and so are the scores: weights of 0
+                // weights; while nothing is seen, m is -inf and so are the scores: weights of 0
                 uint32_t ph[K::kBlocks][2], pl[K::kBlocks][2];
 #pragma unroll
                 for (int b = 0; b < K::kBlocks; ++b) {

@@ -881,3 +881,80 @@ def test_attn_wide_caps(backend, softcap, cache):
 def test_attn_refuses_an_infinite_cap(backend):
     with pytest.raises(InvalidArgument):
         paged.PagedAttention(paged.CacheLayout(4, 16, 2, 64, BF16), 4, BF16, 4, softcap=float("inf"))
+
+
+# ------------------------------------------------------------------ a dominant token
+
+# Half the spacing of f16's smallest numbers, 2^-25, over the largest weight that leaves its maximum alone, 2^12.
+FLOOR = 2.0 ** -37
+
+
+def dominant(cache, dtype, lead, n=8192, dim=64, seed=61):
+    """One row of keys and values for every request: token 0 leads by `lead` and has the value zero, as a first token
+    often does, so that the result is what the others' small weights make of it."""
+    rng = np.random.default_rng(seed)
+    k = rng.normal(size=(n, 1, dim)).astype(np.float32)
+    v = rng.uniform(16.0, 48.0, (n, 1, dim)).astype(np.float32)
+    k[0, 0, 0], v[0] = lead, 0.0
+    q = np.zeros((2, dim), np.float32)
+    q[0, 0], q[1, 0] = 8.0, -8.0  # scores of +-k[:, 0] at a scale of 1/8: the second head sees token 0 last of all
+    return plain.codes(q, dtype), plain.codes(k, cache), plain.codes(v, cache)
+
+
+@pytest.mark.parametrize("dtype,cache", [(BF16, BF16), (F16, F16), (F16, E4M3), (F16, E5M2), (BF16, E4M3)])
+@pytest.mark.parametrize("lead", [12.0, 16.0, 20.0])
+def test_attn_small_weights_beside_a_dominant_one(backend, dtype, cache, lead):
+    """2000 requests over the same 8192 tokens: most teams have some thousands of tokens beside the dominant one.
+
+    Beside the usual bound, each f16 weight may be off by FLOOR of the largest (half the spacing of f16's smallest
+    numbers, and what the largest weight is at least): as many times the mean |v| as there are tokens."""
+    requests, n, page = 2000, 8192, 16
+    q, k, v = dominant(cache, dtype, lead, n)
+    dim = q.shape[1]
+    layout = paged.CacheLayout(n // page, page, 1, dim, cache)
+    order = np.random.default_rng(5).permutation(n // page).astype(np.int32)
+    kv = [np.empty_like(x) for x in (k, v)]
+    for x, y in zip(kv, (k, v)):
+        x.reshape(n // page, -1)[order] = y.reshape(n // page, -1)
+    bufs = [to_device(a) for a in (np.repeat(q[None], requests, 0), *kv, np.repeat(order[None], requests, 0),
+                                   np.full(requests, n, np.int32))]
+    out, lse = empty(requests * 2 * dim * 2), empty(requests * 2 * 4)
+    with paged.PagedAttention(layout, 2, dtype, n // page) as attn:
+        attn.run(*(b.ptr for b in bufs), requests, out.ptr, lse.ptr)
+        sync_device()
+    got = plain.values(fetch(out, out.nbytes, np.uint16).reshape(requests, 2, dim), dtype)
+    got_lse = fetch(lse, lse.nbytes, np.float32).reshape(requests, 2)
+    for b in (*bufs, out, lse):
+        b.free()
+    want, want_lse, size = plain.attention(plain.values(q, dtype), plain.values(k, cache), plain.values(v, cache), None,
+                                           0.125, 0.0, 0, 2)
+    floor = 0.0 if cache == BF16 else n * FLOOR * np.abs(plain.values(v, cache)).mean(0)
+    bound = 2e-4 * size + floor + plain.UNIT[dtype] * 1.01 * np.abs(want) + (3.1e-8 if dtype == F16 else 0.0)
+    worst = (np.abs(got - want) / bound).max()
+    assert worst <= 1, f"{worst:.3g} times the bound"
+    assert (np.abs(got_lse - want_lse) <= 1e-4 + 2.0 ** -22 * np.abs(want_lse)).all()
+
+
+@pytest.mark.parametrize("cache", [F16, E4M3])
+def test_attn_weights_stay_inside_f16_at_coarse_scores(backend, cache):
+    """Scores of 2^25 are four apart in float32 (times log2 e): a maximum plus 15 is none of them, and a weight of 2^16,
+    which f16 has not, must not come of it.  All values are 1, so every average is."""
+    n, dim, page = 200, 64, 16
+    k, v, q = np.zeros((n, 1, dim), np.float32), np.ones((n, 1, dim), np.float32), np.zeros((1, 1, dim), np.float32)
+    k[:, 0, 0], k[:, 0, 1] = 128.0, np.arange(n) // 13
+    q[0, 0, :2] = 32768.0, 0.5
+    pages = -(-n // page)
+    layout = paged.CacheLayout(pages, page, 1, dim, cache)
+    kv = [np.zeros((pages * page, 1, dim), cache.storage_numpy) for _ in range(2)]
+    for x, y in zip(kv, (k, v)):
+        x[:n] = plain.codes(y, cache)
+    bufs = [to_device(a) for a in (plain.codes(q, F16), *kv, np.arange(pages, dtype=np.int32), np.array([n], np.int32))]
+    out, lse = empty(2 * dim), empty(4)
+    with paged.PagedAttention(layout, 1, F16, pages, scale=8.0) as attn:
+        attn.run(*(b.ptr for b in bufs), 1, out.ptr, lse.ptr)
+        sync_device()
+    got = plain.values(fetch(out, out.nbytes, np.uint16), F16)
+    assert (np.abs(got - 1.0) <= 2e-4 + 2.0 ** -11).all()
+    assert abs(float(fetch(lse, 4, np.float32)[0]) / 2.0 ** 25 - 1.0) < 1e-5
+    for b in (*bufs, out, lse):
+        b.free()
