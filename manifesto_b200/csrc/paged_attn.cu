@@ -213,7 +213,7 @@ struct Span {
 __device__ __forceinline__ Span span_of(const AttnArgs& a, int32_t r) {
     const int64_t reach = static_cast<int64_t>(a.max_pages) * a.page;
     Span s;
-    s.len = max(__ldg(a.lens + r), 0);
+    s.len = max(a.lens[r], 0);
     if (s.len > reach) s.len = static_cast<int32_t>(reach);
     s.first = a.window > 0 && s.len > a.window ? s.len - a.window : 0;
     s.base = s.first & ~(kBlock - 1);
@@ -456,7 +456,7 @@ __device__ __forceinline__ void join_parts(const AttnArgs& a, typename K::Shared
         }
         __syncthreads();
     }
-    const float vs = a.v_scale ? __ldg(a.v_scale + w.kv) : 1.0f;
+    const float vs = a.v_scale ? a.v_scale[w.kv] : 1.0f;
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
         const int i = tid + e * K::kThreads, h = i / K::kFour, d = i % K::kFour * 4;
@@ -682,7 +682,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                             ++entry[b];
                         }
                 }
-                if (tok < load.span.len) page_no[b] = __ldg(entry[b]);
+                if (tok < load.span.len) page_no[b] = *entry[b];
             }
         };
         uint32_t partial = 0;  // stages that lack some of their tokens: those have a mask
@@ -765,8 +765,8 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
             for (int c = 0; c < K::kSteps; ++c) {
                 const int d0 = K::kFp8 ? c * 16 + 4 * j : c * 16 + 2 * j;
                 const int d1 = K::kFp8 ? d0 + 2 : d0 + 8;
-                qf[c][0] = h < hd.count && d0 < a.head_dim ? __ldg(reinterpret_cast<const uint32_t*>(q + 2 * d0)) : 0u;
-                qf[c][1] = h < hd.count && d1 < a.head_dim ? __ldg(reinterpret_cast<const uint32_t*>(q + 2 * d1)) : 0u;
+                qf[c][0] = h < hd.count && d0 < a.head_dim ? *reinterpret_cast<const uint32_t*>(q + 2 * d0) : 0u;
+                qf[c][1] = h < hd.count && d1 < a.head_dim ? *reinterpret_cast<const uint32_t*>(q + 2 * d1) : 0u;
             }
         };
         load_queries(at);
@@ -815,7 +815,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                             qf[c][x] = pack2<false>(f0 * fit, f1 * fit);
                         }
                 }
-                const float ks = a.k_scale ? __ldg(a.k_scale + hd.kv) : 1.0f;
+                const float ks = a.k_scale ? a.k_scale[hd.kv] : 1.0f;
                 // head 2j + x of this lane's columns: its scale is with the lanes of row 2j + x
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
@@ -823,7 +823,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                     const int hx = member * 8 + 2 * j + x;
                     scale[x] = a.scale * ks * b;
                     scale[x] = a.softcap > 0.0f ? __fdiv_rn(scale[x], a.softcap) * (2.0f * kLog2e) : scale[x] * kLog2e;
-                    slope[x] = a.slopes && hx < hd.count ? __ldg(a.slopes + hd.head0 + hx) * kLog2e : 0.0f;
+                    slope[x] = a.slopes && hx < hd.count ? a.slopes[hd.head0 + hx] * kLog2e : 0.0f;
                     m[x] = high[x] = -INFINITY;
                     less[x] = l[x] = 0.0f;
                 }
@@ -994,7 +994,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                     l[x] += __shfl_xor_sync(0xffffffffu, l[x], 16);
                 }
                 if (all_of_it) {
-                    const float vs = a.v_scale ? __ldg(a.v_scale + hd.kv) : 1.0f;
+                    const float vs = a.v_scale ? a.v_scale[hd.kv] : 1.0f;
                     float f[2];
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
@@ -1157,7 +1157,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
         }
         const float top = sh.joined_m[which][h], sum_l = sh.joined_l[which][h];
         if (w.slot < 0) {
-            const float vs = a.v_scale ? __ldg(a.v_scale + w.kv) : 1.0f;
+            const float vs = a.v_scale ? a.v_scale[w.kv] : 1.0f;
             store_out4(a, w.r, w.head0 + h, d, scale4(acc, sum_l == 0.0f ? 0.0f : __fdiv_rn(vs, sum_l)));
             if (d == 0) store_lse(a, w.r, w.head0 + h, top, sum_l);
         } else {

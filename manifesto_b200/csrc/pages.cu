@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(kAssignThreads) page_assign_kernel(const Assig
                 if (fits_in(has_room, n, s_page[lo], count, tok_base + s_tok[lo], f)) {
                     const uint32_t col = pos[b] / page, held = pages_of(l, page);
                     if (col >= held) {
-                        number[b] = __ldg(a.free_pages + static_cast<int64_t>(head) + s_page[lo] + (col - held));
+                        number[b] = a.free_pages[static_cast<int64_t>(head) + s_page[lo] + (col - held)];
                         first_of_page[b] = col * page.d == pos[b];
                     } else {
                         number[b] = a.table[static_cast<int64_t>(r0 + lo) * a.table_stride + col];

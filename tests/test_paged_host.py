@@ -108,3 +108,15 @@ def test_plain_attention_of_parts():
     assert np.allclose(one, v[8, 0])
     flat, l0, _ = plain.attention(0 * q, k, v, None, 0.3, 0.0, 0, 2)
     assert np.allclose(flat, v[:, 0].mean(0)) and np.allclose(l0, math.log(9))
+
+
+def test_overlapped_kernels_read_with_plain_loads():
+    """A kernel that is set up while the one before it still writes must not use the read-only path, which takes its data
+    to be constant for the kernel's whole life."""
+    from manifesto_b200.build import CSRC
+    overlapped = [f for f in sorted(CSRC.glob("*.cu")) if "launch_overlapped(" in f.read_text()]
+    assert {f.name for f in overlapped} >= {"pages.cu", "rope.cu", "paged_attn.cu"}
+    for f in overlapped:
+        text = f.read_text()
+        for form in ("__ldg(", "ld.global.nc", "ld_stream(", "load4_stream<", "load_raw<", "__restrict__"):
+            assert form not in text, f"{f.name} reads by {form}"
