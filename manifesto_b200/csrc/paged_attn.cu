@@ -655,10 +655,12 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
         const int64_t kv_gap = a.v - a.k;
         const int32_t lane_tok = whole ? 0 : lane & (T - 1);
         // of the blocks of the tile at `load` (or, blocks not being whole, of this lane's row): their pages, the pages'
-        // entries in the table and the blocks' places in the pages
+        // entries in the table and the blocks' places in the pages.  Tokens are unsigned: the last tile of a request of
+        // nearly 2^31 tokens ends past them.
         const char* head_at = nullptr;
         const int32_t* entry[K::kBlocks];
-        int32_t page_no[K::kBlocks], page_off[K::kBlocks], tok0 = 0;
+        int32_t page_no[K::kBlocks];
+        uint32_t page_off[K::kBlocks], tok0 = 0;
         auto look_up = [&](bool new_item) {
             if (new_item) {
                 tok0 = load.span.base + load.t * T;
@@ -668,28 +670,28 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
             }
 #pragma unroll
             for (int b = 0; b < K::kBlocks; ++b) {
-                const int32_t tok = tok0 + lane_tok + (whole ? b * kBlock : 0);
+                const uint32_t tok = tok0 + lane_tok + (whole ? b * kBlock : 0);
                 if (new_item || !whole) {
-                    const int32_t idx = static_cast<uint32_t>(tok) / a.by_page;
+                    const int32_t idx = tok / a.by_page;
                     page_off[b] = tok - idx * a.page;
                     entry[b] = a.table + load.r * a.table_stride + idx;
                 } else {
                     page_off[b] += T;
 #pragma unroll
                     for (int x = 0; x < K::kBlocks; ++x)
-                        if (page_off[b] >= a.page) {
+                        if (page_off[b] >= a.by_page.d) {
                             page_off[b] -= a.page;
                             ++entry[b];
                         }
                 }
-                if (tok < load.span.len) page_no[b] = *entry[b];
+                if (tok < static_cast<uint32_t>(load.span.len)) page_no[b] = *entry[b];
             }
         };
         uint32_t partial = 0;  // stages that lack some of their tokens: those have a mask
         auto issue = [&](int stage) {
             if (to_load > 0) {
-                const uint32_t to = ring + stage * K::kStage;
-                bool ok[K::kBlocks], all = whole && tok0 >= load.span.first && tok0 + T <= load.span.len;
+                const uint32_t to = ring + stage * K::kStage, first = load.span.first, len = load.span.len;
+                bool ok[K::kBlocks], all = whole && tok0 >= first && tok0 + T <= len;
                 int64_t at_block[K::kBlocks];
 #pragma unroll
                 for (int b = 0; b < K::kBlocks; ++b) {
@@ -722,8 +724,8 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                 } else {
                     // the row of this lane: whether it is there, and where
                     const int mine = whole ? (lane & (T - 1)) / kBlock : 0;
-                    const int32_t tok = tok0 + (lane & (T - 1));
-                    const bool seen = tok >= load.span.first && tok < load.span.len;
+                    const uint32_t tok = tok0 + (lane & (T - 1));
+                    const bool seen = tok >= first && tok < len;
                     const bool mine_ok = mine == 0 ? ok[0] : ok[K::kBlocks - 1];
                     if (seen && !mine_ok) atomicExch(a.status, MF_DEVICE_BAD_PAGE);
                     const uint32_t mask = __ballot_sync(0xffffffffu, seen && mine_ok) & K::kAll;
@@ -891,7 +893,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                     }
                     if (a.slopes) {
                         // distance to the newest token, <= 0
-                        const float away = static_cast<float>(at.span.base + t * T + b * kBlock + g - (at.span.len - 1));
+                        const float away = static_cast<float>(at.span.base + t * T - (at.span.len - 1) + b * kBlock + g);
 #pragma unroll
                         for (int x = 0; x < 4; ++x)
                             p[b][x] = __fmaf_rn(slope[x & 1], away + (x & 2 ? 8.0f : 0.0f), p[b][x]);

@@ -5,7 +5,7 @@ import math
 import numpy as np
 import pytest
 
-from manifesto_b200 import Stream, paged, sync_device, synthetic
+from manifesto_b200 import DeviceBuffer, Stream, paged, sync_device, synthetic
 from manifesto_b200._abi import call
 from manifesto_b200.dtype import DType
 from manifesto_b200.errors import (DeviceStickyError, DTypeMismatch, DTypeUnsupported, InvalidArgument,
@@ -957,4 +957,39 @@ def test_attn_weights_stay_inside_f16_at_coarse_scores(backend, cache):
     assert (np.abs(got - 1.0) <= 2e-4 + 2.0 ** -11).all()
     assert abs(float(fetch(lse, 4, np.float32)[0]) / 2.0 ** 25 - 1.0) < 1e-5
     for b in (*bufs, out, lse):
+        b.free()
+
+
+@pytest.mark.parametrize("page", [48, 1000])
+@pytest.mark.parametrize("dim,cache", [(64, BF16), (128, BF16), (128, E4M3)])
+def test_attn_longest_request(backend, page, dim, cache):
+    """2^31 - 1 tokens, of which a window sees the last 40: the tile that ends past 2^31 reads neither a table entry past
+    the row nor the rows past the length, which hold NaN."""
+    n, window, hq, hkv = 2 ** 31 - 1, 40, 4, 2
+    width = -(-n // page)
+    pages = 4
+    tail = np.array([2, 0, 3, 1], np.int32)  # the pages of the row's last entries
+    table = DeviceBuffer(4 * width)
+    table.memset(0xFF)
+    table.upload(tail, offset=4 * (width - len(tail)))
+    first = (width - len(tail)) * page
+    tok = np.arange(n - window, n)
+    kv = [np.full((pages, page, hkv, dim), {BF16: 0x7FFF, E4M3: 0x7F}[cache], cache.storage_numpy) for _ in range(2)]
+    rows = [plain.normal(91 + i, (window, hkv, dim), cache) for i in range(2)]
+    for c, x in zip(kv, rows):
+        c[tail[(tok - first) // page], (tok - first) % page] = x
+    q = plain.normal(93, (1, hq, dim), BF16)
+    slopes = np.array([0.5, 0.25, 0.125, 0.0625], np.float32)
+    bufs = [to_device(a) for a in (q, *kv, np.array([n], np.int32), slopes)]
+    out, lse = empty(2 * hq * dim), empty(4 * hq)
+    layout = paged.CacheLayout(pages, page, hkv, dim, cache, "NHD")
+    with paged.PagedAttention(layout, hq, BF16, width, window=window, slopes=bufs[4].ptr) as attn:
+        attn.run(bufs[0].ptr, bufs[1].ptr, bufs[2].ptr, table.ptr, bufs[3].ptr, 1, out.ptr, lse.ptr)
+        sync_device()
+    assert device_status() == 0
+    want = plain.attention(plain.values(q, BF16)[0], *(plain.values(x, cache) for x in rows), slopes,
+                           float(np.float32(1.0 / math.sqrt(dim))), 0.0, 0, hq // hkv)
+    check_attn({"dtype": BF16}, (fetch(out, out.nbytes, np.uint16).reshape(1, hq, dim), fetch(lse, lse.nbytes, np.float32).reshape(1, hq)),
+               tuple(w[None] for w in want))
+    for b in (*bufs, table, out, lse):
         b.free()
