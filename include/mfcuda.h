@@ -487,7 +487,8 @@ typedef struct mf_cache_layout {
  * and owner have `tokens` entries: those past the total get -1, 0, -1, and
  * tokens past `tokens` have no entry (the table is complete all the same).
  * Inputs are not changed (lens_after and pool_after are other buffers than
- * lens and pool), so a step can be planned again.  One launch. */
+ * lens and pool), so a step can be planned again.  One launch, of up to
+ * 2^31 - 2^16 requests. */
 typedef struct mf_page_config {
     int32_t page_size;
     int32_t max_pages;    /* entries of a request's table row */
@@ -574,8 +575,9 @@ int mf_rope_append(const mf_rope_append_config* config, const void* q, const voi
  * of themselves, for an F16 or FP8 cache by 2^-22 of themselves or 2^-37 of
  * the request's largest weight, whichever is more.
  *
- * One run covers up to 2^31 - 1 tiles (16 tokens of one key-value head, for up
- * to 16 query heads); lengths that ask for more record MF_DEVICE_TOO_LARGE.
+ * One run covers up to 2^31 - 2^16 requests and 2^31 - 1 tiles (16 tokens of
+ * one key-value head, for up to 16 query heads); lengths that ask for more
+ * record MF_DEVICE_TOO_LARGE.
  * A handle holds the description and the workspace of the split (about 10 MB):
  * create it once, run it for every step and layer.  A handle is not shared
  * between streams that run at once.  One launch per run, no host sync; results

@@ -50,6 +50,10 @@ inline bool is_decodable(int dt) {
     return dt >= MF_DT_F64 && dt <= MF_DT_U8;
 }
 
+// Most requests of one call: loops over them in 32 bits may step past the last
+// by a grid or a tile.
+constexpr int32_t kMaxRequests = 0x7fffffff - 0xffff;
+
 // Launch a kernel that may be set up while the one before it in the stream
 // still runs (programmatic dependent launch).  Such a kernel calls
 // after_previous() (mf_launch.cuh) before it touches memory: that returns when

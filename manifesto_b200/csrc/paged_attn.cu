@@ -1451,7 +1451,8 @@ extern "C" int mf_paged_attn_run(mf_paged_attn handle, const void* q, const void
     if (!handle) return fail(MF_ERR_INVALID_ARGUMENT, "mf_paged_attn_run: handle is NULL");
     if (handle->device != state().device)
         return fail(MF_ERR_INVALID_ARGUMENT, "mf_paged_attn_run: the handle belongs to device %d", handle->device);
-    if (n_requests < 0) return fail(MF_ERR_SHAPE_INVALID, "mf_paged_attn_run: %d requests", n_requests);
+    if (n_requests < 0 || n_requests > kMaxRequests)
+        return fail(MF_ERR_SHAPE_INVALID, "mf_paged_attn_run: %d requests (0 to 2^31 - 2^16)", n_requests);
     if (n_requests == 0) return MF_OK;
     if (!q || !k_cache || !v_cache || !table || !lens || !out)
         return fail(MF_ERR_INVALID_ARGUMENT, "mf_paged_attn_run: NULL buffer");

@@ -264,8 +264,9 @@ extern "C" int mf_page_assign(const mf_page_config* config, const int32_t* lens,
     if (config->table_stride < config->max_pages)
         return fail(MF_ERR_SHAPE_MISMATCH, "mf_page_assign: table stride %lld is below the row's %d entries",
                     (long long)config->table_stride, config->max_pages);
-    if (n_requests < 0 || tokens < 0 || tokens > 0x7fffffffll)
-        return fail(MF_ERR_SHAPE_INVALID, "mf_page_assign: %d requests, %lld tokens", n_requests, (long long)tokens);
+    if (n_requests < 0 || n_requests > kMaxRequests || tokens < 0 || tokens > 0x7fffffffll)
+        return fail(MF_ERR_SHAPE_INVALID, "mf_page_assign: %d requests (0 to 2^31 - 2^16), %lld tokens (0 to 2^31 - 1)", n_requests,
+                    (long long)tokens);
     if (!pool || !starts || !pool_after) return fail(MF_ERR_INVALID_ARGUMENT, "mf_page_assign: NULL buffer");
     if (n_requests > 0 && (!lens || !new_tokens || !table || !free_pages || !lens_after))
         return fail(MF_ERR_INVALID_ARGUMENT, "mf_page_assign: NULL buffer");

@@ -993,3 +993,17 @@ def test_attn_longest_request(backend, page, dim, cache):
                tuple(w[None] for w in want))
     for b in (*bufs, table, out, lse):
         b.free()
+
+
+@pytest.mark.parametrize("n", [2 ** 31 - 1, 2 ** 31 - 2 ** 16 + 1])
+def test_request_counts_past_the_loops_are_refused(backend, n):
+    """The loops over requests step past the last in 32 bits: counts that would wrap them do not reach the device."""
+    b = [empty(4096) for _ in range(4)]
+    p = [x.ptr for x in b]
+    with pytest.raises(ShapeInvalid):
+        paged.PageAssigner(16, 1).assign(p[0], p[0], n, p[1], p[1], p[1], 0, 0, 0, 0, p[2], p[2], p[3])
+    with paged.PagedAttention(paged.CacheLayout(4, 16, 1, 16, BF16), 1, BF16, 1) as a:
+        with pytest.raises(ShapeInvalid):
+            a.run(p[0], p[1], p[1], p[2], p[2], n, p[3])
+    for x in b:
+        x.free()
