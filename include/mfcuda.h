@@ -19,9 +19,10 @@
  *   - No entry point synchronises the host with the device except the ones
  *     whose name says so (mf_stream_sync, mf_event_sync, mf_device_sync) and
  *     the set-up calls (mf_init, mf_alloc, mf_free, mf_fused_compile,
- *     mf_comm_init, mf_paged_attn_create). Scalar results such as amax are written to device
- *     memory, never returned to the host (manifesto
- *     scripts/check_banned.sh:28-40 forbids host syncs on the launch path).
+ *     mf_comm_init, mf_paged_attn_create, mf_paged_attn_destroy). Scalar
+ *     results such as amax are written to device memory, never returned to the
+ *     host (manifesto scripts/check_banned.sh:28-40 forbids host syncs on the
+ *     launch path).
  *   - Arithmetic follows manifesto's Go scalar code bit for bit, including
  *     its FP8 rounding quirks (compat = MF_COMPAT_REFERENCE). The file:line
  *     each entry point replaces is given in its comment; paths are inside
@@ -578,7 +579,7 @@ int mf_rope_append(const mf_rope_append_config* config, const void* q, const voi
  * One run covers up to 2^31 - 2^16 requests and 2^31 - 1 tiles (16 tokens of
  * one key-value head, for up to 16 query heads); lengths that ask for more
  * record MF_DEVICE_TOO_LARGE.
- * A handle holds the description and the workspace of the split (about 10 MB):
+ * A handle holds the description and the workspace of the split (5 to 22 MB):
  * create it once, run it for every step and layer.  A handle is not shared
  * between streams that run at once.  One launch per run, no host sync; results
  * do not depend on the order in which the parts finish. */
@@ -601,7 +602,7 @@ int mf_paged_attn_create(const mf_paged_attn_config* config, mf_paged_attn* hand
 int mf_paged_attn_run(mf_paged_attn handle, const void* q, const void* k_cache, const void* v_cache,
                       const int32_t* table, const int32_t* lens, int32_t n_requests, void* out, float* lse,
                       mf_stream stream);
-/* Does not wait for the device: the next create that takes the workspace does. */
+/* Waits for the device, then frees the workspace. */
 int mf_paged_attn_destroy(mf_paged_attn handle);
 
 /* ---------------------------------------------------------------------

@@ -24,8 +24,6 @@ struct AmaxXchg;
 int launch_plan_passes(const mf_chunk_desc* chunks, int32_t n_chunks, int src_dtype, const AmaxXchg* d_xchg,
                        float* d_local_amax, int world, int32_t epoch, int passes, float* d_amax, float* d_scale_inv,
                        int fp8_dtype, int compat, cudaStream_t s);
-// Free the workspaces that destroyed attention handles left (paged_attn.cu).
-void release_attn_workspaces();
 // In-place float32 max all-reduce over the communicator (comm.cu).
 int comm_allreduce_max(mf_comm comm, float* d_vec, int64_t count, cudaStream_t s);
 

@@ -48,7 +48,6 @@
 // same 64 with 16/8 heads of 256: 168 us (164).  What a call costs besides:
 // about 3 us until the first tile is there and 4 to 6 us for the joins, mostly
 // instruction fetches of code that runs once.
-#include <mutex>
 #include <new>
 
 #include "mf_divisor.cuh"
@@ -1267,69 +1266,11 @@ Kernel pick(int cache_dtype, int group, int head_dim) {
 
 using namespace mf;
 
-namespace mf {
-namespace {
-
-// Workspaces of destroyed handles, for the next ones: allocating one takes
-// from half a millisecond to three.  Their tickets are zero, as every run
-// leaves them; whoever takes one waits for the device first, so that no run of
-// its earlier handle goes on.
-constexpr int kKept = 8;
-struct Kept {
-    void* p;
-    size_t bytes;
-    int device;
-};
-Kept g_kept[kKept];
-std::mutex g_kept_mutex;
-
-// The smallest kept workspace of `bytes` to four times that, or NULL.
-void* take_kept(size_t bytes, int device, size_t* got) {
-    std::lock_guard<std::mutex> lock(g_kept_mutex);
-    Kept* best = nullptr;
-    for (Kept& k : g_kept)
-        if (k.p && k.device == device && k.bytes >= bytes && k.bytes <= 4 * bytes && (!best || k.bytes < best->bytes)) best = &k;
-    if (!best) return nullptr;
-    void* p = best->p;
-    *got = best->bytes;
-    best->p = nullptr;
-    // a host that reset the device took it along
-    cudaPointerAttributes at;
-    if (cudaPointerGetAttributes(&at, p) != cudaSuccess || at.type != cudaMemoryTypeDevice || at.device != device) {
-        cudaGetLastError();
-        return nullptr;
-    }
-    return p;
-}
-
-bool keep(void* p, size_t bytes, int device) {
-    std::lock_guard<std::mutex> lock(g_kept_mutex);
-    for (Kept& k : g_kept)
-        if (!k.p) {
-            k = Kept{p, bytes, device};
-            return true;
-        }
-    return false;
-}
-
-}  // namespace
-
-void release_attn_workspaces() {
-    std::lock_guard<std::mutex> lock(g_kept_mutex);
-    for (Kept& k : g_kept) {
-        if (k.p) cudaFree(k.p);
-        k.p = nullptr;
-    }
-}
-
-}  // namespace mf
-
 struct mf_paged_attn_s {
     mf_paged_attn_config config;
     Kernel kernel;
     AttnArgs args;
     void* workspace;
-    size_t bytes;
     int device, ctas;
 };
 
@@ -1369,36 +1310,24 @@ extern "C" int mf_paged_attn_create(const mf_paged_attn_config* config, mf_paged
     const int ctas = state().sm_count;
     const size_t team_part = static_cast<size_t>(ctas) * kernel.teams * kernel.part_floats * 4;
     const size_t cta_part = static_cast<size_t>(ctas) * 3 * kernel.part_floats * 4;
-    const size_t bytes = (static_cast<size_t>(ctas) * 8 + 255) / 256 * 256 + team_part + cta_part;
+    const size_t tickets = (static_cast<size_t>(ctas) * 8 + 255) / 256 * 256;
+    const size_t bytes = tickets + team_part + cta_part;
     mf_paged_attn_s* h = new (std::nothrow) mf_paged_attn_s{};
     if (!h) return fail(MF_ERR_ALLOCATOR_EXHAUSTED, "mf_paged_attn_create: out of host memory");
-    // tickets first: they stay in their place, whatever shape uses the workspace next
-    const size_t tickets = (static_cast<size_t>(ctas) * 8 + 255) / 256 * 256;
-    h->bytes = bytes;
-    h->workspace = take_kept(bytes, state().device, &h->bytes);
-    if (h->workspace) {
-        const cudaError_t err = cudaDeviceSynchronize();
-        if (err != cudaSuccess) {
-            keep(h->workspace, h->bytes, state().device);
-            delete h;
-            return cuda_fail(err, "mf_paged_attn_create: cudaDeviceSynchronize");
-        }
-    } else {
-        cudaError_t err = cudaMalloc(&h->workspace, bytes);
-        if (err != cudaSuccess) {
-            cudaGetLastError();
-            delete h;
-            if (err == cudaErrorMemoryAllocation)
-                return fail(MF_ERR_ALLOCATOR_EXHAUSTED, "mf_paged_attn_create: %zu bytes: out of device memory", bytes);
-            return cuda_fail(err, "mf_paged_attn_create: cudaMalloc");
-        }
-        err = cudaMemset(h->workspace, 0, tickets);
-        if (err == cudaSuccess) err = cudaStreamSynchronize(nullptr);  // streams that do not wait for the default one may run it
-        if (err != cudaSuccess) {
-            cudaFree(h->workspace);
-            delete h;
-            return cuda_fail(err, "mf_paged_attn_create: cudaMemset");
-        }
+    cudaError_t err = cudaMalloc(&h->workspace, bytes);
+    if (err != cudaSuccess) {
+        cudaGetLastError();
+        delete h;
+        if (err == cudaErrorMemoryAllocation)
+            return fail(MF_ERR_ALLOCATOR_EXHAUSTED, "mf_paged_attn_create: %zu bytes: out of device memory", bytes);
+        return cuda_fail(err, "mf_paged_attn_create: cudaMalloc");
+    }
+    err = cudaMemset(h->workspace, 0, tickets);
+    if (err == cudaSuccess) err = cudaStreamSynchronize(nullptr);  // streams that do not wait for the default one may run it
+    if (err != cudaSuccess) {
+        cudaFree(h->workspace);
+        delete h;
+        return cuda_fail(err, "mf_paged_attn_create: cudaMemset");
     }
     char* w = static_cast<char*>(h->workspace);
     h->config = c;
@@ -1478,7 +1407,10 @@ extern "C" int mf_paged_attn_run(mf_paged_attn handle, const void* q, const void
 extern "C" int mf_paged_attn_destroy(mf_paged_attn handle) {
     if (!handle) return MF_OK;
     MF_ENTER();
-    if (!keep(handle->workspace, handle->bytes, handle->device)) MF_CUDA_CHECK(cudaFree(handle->workspace));
+    cudaError_t err = cudaDeviceSynchronize();  // its last run may still use the workspace
+    const cudaError_t freed = cudaFree(handle->workspace);
+    if (err == cudaSuccess) err = freed;
     delete handle;
+    if (err != cudaSuccess) return cuda_fail(err, "mf_paged_attn_destroy");
     return MF_OK;
 }

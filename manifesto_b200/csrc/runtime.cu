@@ -3,7 +3,6 @@
 // tensor.Backend (tensor/backend.go:18-68): Upload/Download become an
 // allocation plus an async copy on a caller stream, Close becomes
 // mf_shutdown, and Tensor.Sync reads the sticky device status.
-#include "mf_internal.h"
 #include "mf_runtime.h"
 
 #include <cstring>
@@ -134,7 +133,6 @@ int mf_shutdown(void) {
     if (!g_state.open) return MF_OK;
     cudaSetDevice(g_state.device);
     cudaError_t err = cudaDeviceSynchronize();
-    release_attn_workspaces();
     g_state.open = false;
     if (err != cudaSuccess) return cuda_fail(err, "mf_shutdown: cudaDeviceSynchronize");
     return MF_OK;

@@ -175,7 +175,7 @@ class PagedAttention:
             _raise("mf_paged_attn_run", rc)
 
     def close(self) -> None:
-        """Free the workspace; the object's last run has to be over."""
+        """Wait for the device and free the workspace."""
         if self._handle is not None:
             handle, self._handle = self._handle, None
             _abi.call("mf_paged_attn_destroy", handle)

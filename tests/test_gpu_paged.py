@@ -1007,3 +1007,26 @@ def test_request_counts_past_the_loops_are_refused(backend, n):
             a.run(p[0], p[1], p[1], p[2], p[2], n, p[3])
     for x in b:
         x.free()
+
+
+# ------------------------------------------------------------------ handles, streams and captured steps
+
+def free_memory() -> int:
+    sync_device()
+    free, total = ctypes.c_size_t(0), ctypes.c_size_t(0)
+    assert ctypes.CDLL("libcuda.so.1").cuMemGetInfo_v2(ctypes.byref(free), ctypes.byref(total)) == 0
+    return free.value
+
+
+def test_attn_destroyed_handles_keep_nothing(backend):
+    """A handle's workspace goes with it: nothing is kept by address for handles to come."""
+    def make():
+        return paged.PagedAttention(paged.CacheLayout(4, 16, 1, 256, BF16), 16, BF16, 4)
+
+    make().close()
+    before = free_memory()
+    handles = [make() for _ in range(6)]
+    assert free_memory() < before - (64 << 20)  # some 22 MB each
+    for h in handles:
+        h.close()
+    assert free_memory() >= before - (4 << 20)
