@@ -602,7 +602,7 @@ int mf_paged_attn_create(const mf_paged_attn_config* config, mf_paged_attn* hand
 int mf_paged_attn_run(mf_paged_attn handle, const void* q, const void* k_cache, const void* v_cache,
                       const int32_t* table, const int32_t* lens, int32_t n_requests, void* out, float* lse,
                       mf_stream stream);
-/* Waits for the device, then frees the workspace. */
+/* Waits for the device, then frees the workspace; after mf_shutdown, too. */
 int mf_paged_attn_destroy(mf_paged_attn handle);
 
 /* ---------------------------------------------------------------------

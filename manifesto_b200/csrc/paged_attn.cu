@@ -1406,10 +1406,16 @@ extern "C" int mf_paged_attn_run(mf_paged_attn handle, const void* q, const void
 
 extern "C" int mf_paged_attn_destroy(mf_paged_attn handle) {
     if (!handle) return MF_OK;
-    MF_ENTER();
-    cudaError_t err = cudaDeviceSynchronize();  // its last run may still use the workspace
-    const cudaError_t freed = cudaFree(handle->workspace);
-    if (err == cudaSuccess) err = freed;
+    // also after mf_shutdown, or with another device in use: what the handle owns has no other way out
+    int current = -1;
+    cudaError_t err = cudaGetDevice(&current);
+    if (err == cudaSuccess && current != handle->device) err = cudaSetDevice(handle->device);
+    if (err == cudaSuccess) {
+        err = cudaDeviceSynchronize();  // its last run may still use the workspace
+        const cudaError_t freed = cudaFree(handle->workspace);
+        if (err == cudaSuccess) err = freed;
+        if (current != handle->device) cudaSetDevice(current);
+    }
     delete handle;
     if (err != cudaSuccess) return cuda_fail(err, "mf_paged_attn_destroy");
     return MF_OK;

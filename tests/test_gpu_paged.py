@@ -1030,3 +1030,20 @@ def test_attn_destroyed_handles_keep_nothing(backend):
     for h in handles:
         h.close()
     assert free_memory() >= before - (4 << 20)
+
+
+def test_attn_handle_closes_after_shutdown(backend):
+    """A handle outlives the library's shutdown: closing it then still frees its workspace."""
+    def make():
+        return paged.PagedAttention(paged.CacheLayout(4, 16, 1, 256, BF16), 16, BF16, 4)
+
+    make().close()
+    before = free_memory()
+    a = make()
+    call("mf_shutdown")
+    try:
+        a.close()
+    finally:
+        call("mf_init", 0)
+    assert free_memory() >= before - (4 << 20)
+    run_attn([1, 90, 0])
