@@ -480,13 +480,18 @@ typedef struct mf_cache_layout {
  *   starts[r] = sum of new in front of r, starts[n_requests] = their total;
  *   token i = starts[r] + t: positions[i] = lens[r] + t, owner[i] = r,
  *   slots[i] = table[r][positions[i] / P] * P + positions[i] % P, or -1 if r
- *   does not fit (or that entry of the table is negative); lens_after[r] = lens[r] + new[r] if it fits, else lens[r];
+ *   does not fit (or that entry of the table is negative);
+ *   lens_after[r] = lens[r] + new[r] if it fits, else lens[r];
  *   pool_after = {pool[0] + taken, pool[1] - taken, total of new, requests
  *   that do not fit}, taken = the largest before + need that fits.
  * pool is {index of the first free page in free_pages, number of free pages};
  * free_pages holds at least pool[0] + pool[1] page numbers.  slots, positions
  * and owner have `tokens` entries: those past the total get -1, 0, -1, and
  * tokens past `tokens` have no entry (the table is complete all the same).
+ * Pages are granted to a prefix of the requests: behind the first that does not
+ * fit for lack of pages nobody gets one in this call, however few it needs
+ * (its need stays in `before`), and what is left stays in the pool.  So put
+ * requests that must go on (a token each) in front of prompts that may wait.
  * Inputs are not changed (lens_after and pool_after are other buffers than
  * lens and pool), so a step can be planned again.  One launch, of up to
  * 2^31 - 2^16 requests. */

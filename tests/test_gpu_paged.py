@@ -1047,3 +1047,19 @@ def test_attn_handle_closes_after_shutdown(backend):
         call("mf_init", 0)
     assert free_memory() >= before - (4 << 20)
     run_attn([1, 90, 0])
+
+
+def test_assign_first_refusal_for_pages_stops_the_rest_of_the_step(backend):
+    """Page grants are a prefix of the step: behind a request whose pages are not there none gets a page, however few it
+    needs; those that need none still fit."""
+    run_assign([16, 0, 16, 3, 32], [1, 32, 1, 1, 1], 16, 8, count=2)
+    lens, new = [to_device(np.array(a, np.int32)) for a in ([16, 0, 16, 3, 32], [1, 32, 1, 1, 1])]
+    table = to_device(np.arange(40, dtype=np.int32).reshape(5, 8))
+    free, pool = to_device(np.array([70, 71], np.int32)), to_device(np.array([0, 2], np.int32))
+    outs = [empty(s) for s in (8 * 36, 4 * 36, 4 * 36, 4 * 6, 4 * 5, 16)]
+    paged.PageAssigner(16, 8).assign(lens.ptr, new.ptr, 5, table.ptr, free.ptr, pool.ptr, 36, *(o.ptr for o in outs))
+    after, left = fetch(outs[4], 20, np.int32), fetch(outs[5], 16, np.int32)
+    assert after.tolist() == [17, 0, 16, 4, 32]
+    assert left.tolist() == [1, 1, 36, 3]
+    for b in (lens, new, table, free, pool, *outs):
+        b.free()
