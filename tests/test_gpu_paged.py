@@ -1063,3 +1063,138 @@ def test_assign_first_refusal_for_pages_stops_the_rest_of_the_step(backend):
     assert left.tolist() == [1, 1, 36, 3]
     for b in (lens, new, table, free, pool, *outs):
         b.free()
+<<<<<<< Updated upstream
+=======
+
+
+def queued(on, times, stream):
+    """`times` runs of the case on a stream, none waited for."""
+    s, p = on.s, [b.ptr for b in on.bufs]
+    for _ in range(times):
+        on.attn.run(p[0], p[1], p[2], p[3], p[4], len(s["lens"]), on.out.ptr, on.lse.ptr, stream=stream)
+
+
+def results(on):
+    return fetch(on.out, on.out.nbytes), fetch(on.lse, on.lse.nbytes)
+
+
+def test_attn_two_handles_on_two_streams(backend):
+    """Each handle has its own workspace: runs that overlap give what each gives alone."""
+    cases = [Running(make_attn([9001, 5, 700], 4, 1, 64, 16, "HND", BF16, BF16)),
+             Running(make_attn([3000] * 40, 8, 2, 128, 16, "NHD", F16, E4M3))]
+    alone = []
+    for on in cases:
+        queued(on, 1, None)
+        alone.append(results(on))
+        on.out.memset(0xA5)
+        on.lse.memset(0xA5)
+    sync_device()
+    streams = [Stream(), Stream()]
+    for _ in range(20):
+        for on, s in zip(cases, streams):
+            queued(on, 2, s)
+    for s in streams:
+        s.sync()
+    for on, want in zip(cases, alone):
+        for x, y in zip(results(on), want):
+            bits_equal(x, y)
+        on.close()
+    for s in streams:
+        s.close()
+
+
+def test_attn_destroyed_while_its_runs_are_queued(backend):
+    """Destroying waits for the handle's runs; the next handle may get their memory."""
+    first = Running(make_attn([30000, 5], 4, 1, 64, 16, "HND", BF16, BF16))
+    queued(first, 1, None)
+    want = results(first)
+    s = Stream()
+    queued(first, 30, s)
+    first.attn.close()
+    second = Running(make_attn([9001, 5, 700], 4, 1, 64, 16, "HND", BF16, BF16, seed=8))
+    queued(second, 1, None)
+    check_attn(second.s, second.run(), want_attn(second.s))
+    for x, y in zip(results(first), want):
+        bits_equal(x, y)
+    first.close()
+    second.close()
+    s.close()
+
+
+@pytest.mark.parametrize("cache", [BF16, E4M3])
+def test_a_captured_step_replays_with_other_lengths(backend, cache):
+    """Page assignment, append and attention captured once; each replay serves the lengths that are there then, as the
+    same calls one by one do."""
+    import torch
+
+    n, hq, hkv, dim, page, width, pages = 5, 4, 2, 64, 16, 32, 200
+    row = (hq + 2 * hkv) * dim
+    layout = paged.CacheLayout(pages, page, hkv, dim, cache)
+    nbytes = pages * page * hkv * dim * cache.size
+    rng = np.random.default_rng(17)
+    freq, free = to_device(paged.rope_frequencies(dim)), to_device(rng.permutation(pages).astype(np.int32))
+    rope, assign = paged.Rope(freq.ptr, BF16, dim), paged.PageAssigner(page, width)
+    append = paged.RopeAppend(rope, layout, hq, token_stride=row)
+    keys, vals = plain.normal(71, (nbytes // cache.size,), cache), plain.normal(72, (nbytes // cache.size,), cache)
+
+    class Step:
+        def __init__(self):
+            self.k, self.v = to_device(keys), to_device(vals)
+            self.table = to_device(np.zeros((n, width), np.int32))
+            self.lens, self.new, self.pool = empty(4 * n), empty(4 * n), empty(8)
+            self.x, self.q, self.out, self.lse = empty(2 * n * row), empty(2 * n * hq * dim), empty(2 * n * hq * dim), empty(4 * n * hq)
+            self.slots, self.pos, self.owner = empty(8 * n), empty(4 * n), empty(4 * n)
+            self.starts, self.after, self.pool_after = empty(4 * (n + 1)), empty(4 * n), empty(16)
+            self.attn = paged.PagedAttention(layout, hq, BF16, width)
+
+        def run(self, stream):
+            assign.assign(self.lens.ptr, self.new.ptr, n, self.table.ptr, free.ptr, self.pool.ptr, n, self.slots.ptr,
+                          self.pos.ptr, self.owner.ptr, self.starts.ptr, self.after.ptr, self.pool_after.ptr, stream)
+            append.run(self.x.ptr, self.x.ptr + 2 * hq * dim, self.x.ptr + 2 * (hq + hkv) * dim, self.q.ptr, self.k.ptr,
+                       self.v.ptr, self.pos.ptr, self.slots.ptr, n, stream)
+            self.attn.run(self.q.ptr, self.k.ptr, self.v.ptr, self.table.ptr, self.after.ptr, n, self.out.ptr, self.lse.ptr,
+                          stream)
+
+        def load(self, lens, x):
+            held = -(-lens // page)
+            table = np.zeros((n, width), np.int32)
+            table[np.arange(width)[None] < held[:, None]] = pages - 1 - np.arange(held.sum())
+            for b, a in ((self.table, table), (self.lens, lens), (self.new, np.ones(n, np.int32)),
+                         (self.pool, np.array([0, 8], np.int32)), (self.x, x)):
+                b.upload(a)
+            sync_device()
+
+        def state(self):
+            return [fetch(b, b.nbytes) for b in (self.table, self.k, self.v, self.q, self.out, self.lse, self.slots, self.pos,
+                                                 self.owner, self.starts, self.after, self.pool_after)]
+
+        def close(self):
+            self.attn.close()
+            for b in vars(self).values():
+                if hasattr(b, "free"):
+                    b.free()
+
+    one, other = Step(), Step()
+    one.load(np.full(n, 3, np.int32), plain.normal(73, (n, row), BF16))
+    stream = torch.cuda.Stream()
+    one.run(stream.cuda_stream)
+    stream.synchronize()
+    one.k.upload(keys)
+    one.v.upload(vals)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        one.run(stream.cuda_stream)
+    for i, lens in enumerate(([3, 0, 15, 16, 31], [200, 1, 64, 0, 499], [0, 0, 0, 0, 0], [496, 497, 1, 95, 96])):
+        lens, x = np.array(lens, np.int32), plain.normal(80 + i, (n, row), BF16)
+        one.load(lens, x)
+        other.load(lens, x)
+        graph.replay()
+        torch.cuda.synchronize()
+        other.run(None)
+        for a, b in zip(one.state(), other.state()):
+            bits_equal(a, b)
+    assert device_status() == 0
+    del graph
+    for b in (one, other, freq, free):
+        getattr(b, "close" if isinstance(b, Step) else "free")()
+>>>>>>> Stashed changes
