@@ -1063,8 +1063,6 @@ def test_assign_first_refusal_for_pages_stops_the_rest_of_the_step(backend):
     assert left.tolist() == [1, 1, 36, 3]
     for b in (lens, new, table, free, pool, *outs):
         b.free()
-<<<<<<< Updated upstream
-=======
 
 
 def queued(on, times, stream):
@@ -1197,4 +1195,3 @@ def test_a_captured_step_replays_with_other_lengths(backend, cache):
     del graph
     for b in (one, other, freq, free):
         getattr(b, "close" if isinstance(b, Step) else "free")()
->>>>>>> Stashed changes
