@@ -44,10 +44,12 @@
 //
 // Measured (B200, keys and values in the loop come at 7.4 TB/s, the copy rate
 // of the roofline is 6.55): 64 requests of 2048 tokens, 32/8 heads of 128: BF16
-// 92 us (82 at the copy rate), E4M3 55 us (41); 2 of 131071: 162 us (164); the
+// 92 us (82 at the copy rate), E4M3 54 us (41); 2 of 131071: 160 us (164); the
 // same 64 with 16/8 heads of 256: 168 us (164).  What a call costs besides:
 // about 3 us until the first tile is there and 4 to 6 us for the joins, mostly
-// instruction fetches of code that runs once.
+// instruction fetches of code that runs once; more where parts are large and
+// few CTAs join them (one request of 30011 tokens, 16/1 heads of 256: 27 us, 5
+// at the copy rate).
 #include <new>
 
 #include "mf_divisor.cuh"
@@ -478,7 +480,7 @@ __device__ __forceinline__ void join_parts(const AttnArgs& a, typename K::Shared
 // CTAs of an item of nt tiles where each item has its own, so that a team has up to kOwnTiles[fill] tiles.  A handful
 // of tiles takes no longer than the join between two CTAs; the first limit whose CTAs are all there is taken, and a
 // request alone gets all there are when it has more than one CTA's.  8 requests of 1000 tokens, 32/8 heads of 128:
-// 16.1 us with the row of tiles cut evenly, 12.7 so; 8 of 2000: 22.8 and 19.5.
+// 16.1 us with the row of tiles cut evenly, 13.4 so; 8 of 2000: 22.2 and 20.8.
 __device__ constexpr int kOwnTiles[kFills] = {3, 6, 12};
 template <class K>
 __device__ __forceinline__ int32_t ctas_of(const AttnArgs& a, int32_t nt, int fill) {

@@ -9,14 +9,14 @@
 // fraction of a turn, then float32 cos/sin of it), and then walks the heads'
 // units of 2 * VEC elements with all threads.
 //
-// Bound: HBM, every element read and written once; issue slots are next (205
+// Bound: HBM, every element read and written once; issue slots are next (212
 // instructions per 16 elements, 65% busy; 275 before divisions became
 // multiplications and the test for NaN one per vector).  Occupancy hides the
 // loads: 40 registers; keeping several heads of a thread in flight in 64 to 80
 // registers was slower (48 to 73 us for the 44 below).  For the few tokens of a
 // decoding step, the launch.  Measured: 16384 tokens of 32 heads of 128 in BF16
-// 43.8 us (0.94 of the copy rate), 32771 tokens of 32/8 heads into an E4M3 cache
-// 123 us (0.92), 48 tokens 2.3 us.
+// 43.7 us (0.94 of the copy rate), 32771 tokens of 32/8 heads into an E4M3 cache
+// 123 us (0.92), 48 tokens 2.1 us.
 #include <cmath>
 #include <initializer_list>
 
@@ -131,7 +131,9 @@ __device__ __forceinline__ void store_n(void* p, int64_t i, const float (&v)[N],
 
 // Cosine and sine of position * frequency, times the magnitude.  The product
 // in turns is off by 2^-52 of itself at most (1e-7 of a turn at 2^31 turns);
-// what is left after whole turns go is exact.
+// what is left after whole turns go is exact, and rounded to float32 there: up
+// to 2^-26 of a turn, 9e-8 of the pair's length, as cosine and sine are
+// themselves (a 16-bit result hides both).
 __device__ __forceinline__ float2 turn_of(int32_t position, float inv_freq, float magnitude, bool inverse) {
     constexpr double kInvTwoPi = 0.15915494309189533577;
     double t = static_cast<double>(position) * (static_cast<double>(inv_freq) * kInvTwoPi);
