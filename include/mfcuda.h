@@ -580,8 +580,7 @@ int mf_rope_append(const mf_rope_append_config* config, const void* q, const voi
  * with the values as two 16-bit terms: for a BF16 cache off by at most 2^-16
  * of themselves, for an F16 or FP8 cache by 2^-22 of themselves or 2^-37 of
  * the request's largest weight, whichever is more.  Exponentials are good to
- * 2^-22; the cap's tanh to 2^-22 of the cap up to a cap of 64, of the score
- * above.  Queries over an FP8 cache are held as f16, scaled by a power of two
+ * 2^-22, capped scores to 2^-20 of themselves.  Queries over an FP8 cache are held as f16, scaled by a power of two
  * to their head's largest: an element is off by 2^-25 of that at most.  An
  * infinity among the values that are seen makes its element of the result
  * infinite or NaN.

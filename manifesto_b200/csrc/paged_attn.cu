@@ -206,6 +206,21 @@ __device__ __forceinline__ float rcp_fast(float x) {
     return r;
 }
 
+// A capped score times log2(e), softcap log2(e) tanh(y), of p = 2 log2(e) y.  With e = exp2(p), tanh(y) = 1 - 2 / (1 + e)
+// takes one exponential and one reciprocal and has its limits at both ends, but is only good to 2^-22 of 1: a score far
+// below the cap would lose bits.  Below y = 0.4 a polynomial in p^2 stands in (tanh(y) / y by minimax of the relative
+// error, 1e-7), above, 2^-22 is 5e-7 of tanh(y).  A warp whose scores are all below takes the polynomial alone: 256
+// requests ragged to 8192 tokens, E4M3, take 399 us with a cap of 30 and without one (401 with the exponential form
+// up to a cap of 64 and tanhf above).
+constexpr float kSmallCapped = 1.15415603f;  // 0.4 * 2 log2(e)
+__device__ __forceinline__ float cap_small(float p, float softcap) {
+    const float v = p * p;
+    return p * softcap * __fmaf_rn(__fmaf_rn(__fmaf_rn(v, -4.1202753e-5f, 9.5731476e-4f), v, -0.020017692f), v, 0.49999995f);
+}
+__device__ __forceinline__ float cap_large(float p, float cap) {
+    return __fmaf_rn(-2.0f * cap, rcp_fast(1.0f + exp2_fast(p)), cap);
+}
+
 // A request's tokens: [first, len) are seen, in tiles from `base` on (a multiple
 // of the block, so that a block never crosses a page of whole blocks).
 struct Span {
@@ -276,10 +291,6 @@ struct Joined {
 
 constexpr int kFills = 3;  // ways to give each item CTAs of its own
 constexpr int kJoin = 16;  // most parts that one step of a join between CTAs takes
-// Up to this cap 2^-22 of it, the error of the short form of its tanh, is 1.5e-5 of a score, no more than what the sum
-// of the products leaves; above it tanhf is exact enough relative to the score.  (Its code alone costs E4M3 caches with a
-// smaller cap 1%: 256 requests ragged to 8192 tokens 390 -> 394 us.)
-constexpr float kWideCap = 64.0f;
 // MODE: dtype of the cache; DP: head_dim padded to 64, 128 or 256; TM: warps of a team; W: warps; T: tokens of a
 // tile; S: stages of a team's ring.  A team works on one item at a time, each of its warps for 8 query heads.
 template <int MODE, int DP, int TM, int W, int T, int S>
@@ -880,18 +891,30 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                 // scores of tokens g and g + 8 of each block, heads 2j and 2j + 1, times log2(e)
                 float p[K::kBlocks][4], top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                for (int b = 0; b < K::kBlocks; ++b) {
+                for (int b = 0; b < K::kBlocks; ++b)
 #pragma unroll
                     for (int x = 0; x < 4; ++x) p[b][x] = (s[b][0][x] + s[b][1][x]) * scale[x & 1];
-                    if (a.softcap > kWideCap) {
-                        // p is 2 log2(e) y; relative to the score, which may be far below the cap
+                if (a.softcap > 0.0f) {
+                    float most = 0.0f;
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) p[b][x] = cap * tanhf(p[b][x] * (0.5f / kLog2e));
-                    } else if (a.softcap > 0.0f) {
-                        // cap tanh(y) = cap - 2 cap / (1 + exp(2y)), 2^-22 of the cap, its limits at both ends
+                    for (int b = 0; b < K::kBlocks; ++b)
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) p[b][x] = __fmaf_rn(-2.0f * cap, rcp_fast(1.0f + exp2_fast(p[b][x])), cap);
+                        for (int x = 0; x < 4; ++x) most = fmaxf(most, fabsf(p[b][x]));
+                    if (__any_sync(0xffffffffu, most >= kSmallCapped)) {
+#pragma unroll
+                        for (int b = 0; b < K::kBlocks; ++b)
+#pragma unroll
+                            for (int x = 0; x < 4; ++x)
+                                p[b][x] = fabsf(p[b][x]) < kSmallCapped ? cap_small(p[b][x], a.softcap) : cap_large(p[b][x], cap);
+                    } else {
+#pragma unroll
+                        for (int b = 0; b < K::kBlocks; ++b)
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) p[b][x] = cap_small(p[b][x], a.softcap);
                     }
+                }
+#pragma unroll
+                for (int b = 0; b < K::kBlocks; ++b) {
                     if (a.slopes) {
                         // distance to the newest token, <= 0
                         const float away = static_cast<float>(at.span.base + t * T - (at.span.len - 1) + b * kBlock + g);

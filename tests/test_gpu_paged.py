@@ -1195,3 +1195,37 @@ def test_a_captured_step_replays_with_other_lengths(backend, cache):
     del graph
     for b in (one, other, freq, free):
         getattr(b, "close" if isinstance(b, Step) else "free")()
+
+
+# ------------------------------------------------------------------ precision of single scores
+
+def single_scores(cache, softcap, n=4096, dim=64):
+    """lse of `n` requests of one token each is its score; q and k have one element each that is not zero, so the score is
+    their product without a rounding.  Returns (lse, the scores in 64 bits)."""
+    rng = np.random.default_rng(21)
+    k = np.zeros((n, 1, 1, dim), np.float32)
+    k[:, 0, 0, 0] = np.exp2(rng.uniform(-4, 4, n)) * rng.choice([-1, 1], n)
+    q = np.zeros((n, 1, dim), np.float32)
+    q[..., 0] = 8.0
+    kc, dtype = plain.codes(k, cache), BF16 if cache == BF16 else F16
+    bufs = [to_device(a) for a in (plain.codes(q, dtype), kc, kc, np.arange(n, dtype=np.int32), np.ones(n, np.int32))]
+    out, lse = empty(2 * n * dim), empty(4 * n)
+    with paged.PagedAttention(paged.CacheLayout(n, 1, 1, dim, cache), 1, dtype, 1, scale=0.125, softcap=softcap) as attn:
+        attn.run(*(b.ptr for b in bufs), n, out.ptr, lse.ptr)
+        sync_device()
+    got = fetch(lse, lse.nbytes, np.float32).astype(np.float64)
+    for b in (*bufs, out, lse):
+        b.free()
+    s = plain.values(kc, cache)[:, 0, 0, 0]
+    return got, softcap * np.tanh(s / softcap) if softcap else s
+
+
+@pytest.mark.parametrize("cache", [BF16, F16, E4M3, E5M2])
+@pytest.mark.parametrize("softcap", [2.0, 20.0, 50.0, 64.0, 1000.0])
+def test_attn_capped_scores_keep_their_bits(backend, cache, softcap):
+    """A capped score is good relative to itself, however far below the cap: the polynomial 1e-7, or at 0.4 of the cap an
+    exponential and a reciprocal of 2^-22 each over tanh(0.4), and some six roundings of 2^-24: 2^-20 together.  The
+    f16 forms hold the maximum less 12 and its distance to it, 2^-21 each, and a logarithm near 12, 2^-21: 2^-20 absolutely
+    after the change of base."""
+    got, want = single_scores(cache, softcap)
+    assert (np.abs(got - want) <= 2.0 ** -20 * np.abs(want) + (0.0 if cache == BF16 else 2.0 ** -20)).all()
