@@ -303,6 +303,7 @@ struct Attn {
     // a token that leads by 18 (2^-26) 11 bits, where a maximum as m left none.
     static constexpr float kBelow = kBf16 ? 0.0f : 12.0f;
     static constexpr float kAbove = kBf16 ? 8.0f : 15.0f;
+    static constexpr float kMost = kBf16 ? 1.0f : 4096.0f;  // 2^kBelow
     static constexpr int kBytes = kFp8 ? 1 : 2;
     static constexpr int kRow = DP * kBytes;          // bytes of a token's row
     static constexpr int kChunks = kRow / 16;         // 16-byte pieces of it
@@ -371,8 +372,12 @@ __device__ __forceinline__ void store_out4(const AttnArgs& a, int32_t r, int32_t
     *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
 }
 
+// l is at least K::kMost, the largest weight of a maximum: its logarithm is taken over that, which leaves it the low bits.
+template <class K>
 __device__ __forceinline__ void store_lse(const AttnArgs& a, int32_t r, int32_t head, float m, float l) {
-    if (a.lse) a.lse[static_cast<int64_t>(r) * a.q_heads + head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+    if (!a.lse) return;
+    a.lse[static_cast<int64_t>(r) * a.q_heads + head] =
+        l == 0.0f ? -INFINITY : (m + K::kBelow + log2f(l * (1.0f / K::kMost))) * kLn2;
 }
 
 __device__ __forceinline__ float4 fma4(float4 f, float r, float4 acc) {
@@ -482,7 +487,7 @@ __device__ __forceinline__ void join_parts(const AttnArgs& a, typename K::Shared
             }
         } else {
             store_out4(a, w.r, w.head0 + h, d, scale4(acc[e], sum == 0.0f ? 0.0f : __fdiv_rn(vs, sum)));
-            if (d == 0) store_lse(a, w.r, w.head0 + h, sh.top[h], sum);
+            if (d == 0) store_lse<K>(a, w.r, w.head0 + h, sh.top[h], sum);
         }
     }
     __syncthreads();
@@ -549,7 +554,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
             if (tiles_of<T>(span_of(a, r)) > 0) continue;
             for (int i = tid; i < a.q_heads * (a.head_dim / 4); i += K::kThreads)
                 store_out4(a, r, i / (a.head_dim / 4), i % (a.head_dim / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f));
-            for (int i = tid; i < a.q_heads; i += K::kThreads) store_lse(a, r, i, 0.0f, 0.0f);
+            for (int i = tid; i < a.q_heads; i += K::kThreads) store_lse<K>(a, r, i, 0.0f, 0.0f);
         }
     }
     // Of W values of warps and the values of their threads, in a row: the thread that place `key` is at, and how far into it.
@@ -1026,7 +1031,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                     for (int x = 0; x < 2; ++x) {
                         const int h = member * 8 + 2 * j + x;
                         f[x] = l[x] == 0.0f ? 0.0f : __fdiv_rn(vs, l[x]);
-                        if (g == 0 && h < hd.count) store_lse(a, at.r, hd.head0 + h, m[x], l[x]);
+                        if (g == 0 && h < hd.count) store_lse<K>(a, at.r, hd.head0 + h, m[x], l[x]);
                     }
                     char* out = a.out + 2 * (at.r * a.out_req + hd.head0 * a.out_head);
 #pragma unroll
@@ -1185,7 +1190,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
         if (w.slot < 0) {
             const float vs = a.v_scale ? a.v_scale[w.kv] : 1.0f;
             store_out4(a, w.r, w.head0 + h, d, scale4(acc, sum_l == 0.0f ? 0.0f : __fdiv_rn(vs, sum_l)));
-            if (d == 0) store_lse(a, w.r, w.head0 + h, top, sum_l);
+            if (d == 0) store_lse<K>(a, w.r, w.head0 + h, top, sum_l);
         } else {
             float* to = a.cta_part + (static_cast<int64_t>(blockIdx.x) * 3 + w.slot) * K::kPart;
             *reinterpret_cast<float4*>(to + h * DP + d) = acc;

@@ -1229,3 +1229,32 @@ def test_attn_capped_scores_keep_their_bits(backend, cache, softcap):
     after the change of base."""
     got, want = single_scores(cache, softcap)
     assert (np.abs(got - want) <= 2.0 ** -20 * np.abs(want) + (0.0 if cache == BF16 else 2.0 ** -20)).all()
+
+
+@pytest.mark.parametrize("cache", [BF16, F16, E4M3, E5M2])
+def test_attn_lse_of_single_tokens(backend, cache):
+    """Without a cap: three roundings of the score, and in the f16 forms those of the maximum less 12 and of its distance
+    to it (2^-21 each at most, times ln 2)."""
+    got, want = single_scores(cache, 0.0)
+    off = np.abs(got - want)
+    assert (off <= 2.0 ** -21 * np.abs(want) + (0.0 if cache == BF16 else 2.0 ** -20 * math.log(2.0))).all()
+    assert math.sqrt((off ** 2).sum() / (want ** 2).sum()) <= 2.0 ** -21
+
+
+@pytest.mark.parametrize("cache", [BF16, F16, E4M3, E5M2])
+def test_attn_lse_of_equal_scores(backend, cache):
+    """Queries of zero: lse = log(n).  What is summed is exact in every form; a float32 log2 (one unit in the last place, up
+    to 0.63 of 2^-22 of the result), a constant and a product: 0.75 of 2^-22 of it, for f16 weights of 2^12 as well."""
+    dim, dtype, most = 64, BF16 if cache == BF16 else F16, 40
+    kv = plain.normal(33, (most, 1, 1, dim), cache)
+    lens = np.arange(1, most + 1, dtype=np.int32)
+    table = np.tile(np.arange(most, dtype=np.int32), (most, 1))
+    bufs = [to_device(a) for a in (np.zeros((most, 1, dim), np.uint16), kv, kv, table, lens)]
+    out, lse = empty(2 * most * dim), empty(4 * most)
+    with paged.PagedAttention(paged.CacheLayout(most, 1, 1, dim, cache), 1, dtype, most) as attn:
+        attn.run(*(b.ptr for b in bufs), most, out.ptr, lse.ptr)
+        sync_device()
+    got = fetch(lse, lse.nbytes, np.float32).astype(np.float64)
+    for b in (*bufs, out, lse):
+        b.free()
+    assert (np.abs(got - np.log(lens)) <= 0.75 * 2.0 ** -22 * np.log(lens)).all()
