@@ -103,6 +103,8 @@ typedef struct mf_fused_kernel_s* mf_fused_kernel;
 typedef struct mf_comm_s* mf_comm;
 typedef struct mf_ckpt_plan_s* mf_ckpt_plan;
 typedef struct mf_paged_attn_s* mf_paged_attn;
+typedef struct mf_beam_select_s* mf_beam_select;
+typedef struct mf_page_book_s* mf_page_book;
 
 /* ---------------------------------------------------------------------
  * Lifecycle and errors
@@ -613,6 +615,126 @@ int mf_paged_attn_run(mf_paged_attn handle, const void* q, const void* k_cache, 
                       mf_stream stream);
 /* Waits for the device, then frees the workspace; after mf_shutdown, too. */
 int mf_paged_attn_destroy(mf_paged_attn handle);
+
+/* ---------------------------------------------------------------------
+ * K11: several continuations of a text over the paged cache of K10 (beam
+ * search, or many samples of a prompt): choosing them, sharing their pages,
+ * attending what they share once.  No counterpart in the reference; the
+ * formulas below are the definition.
+ * ------------------------------------------------------------------- */
+
+/* The best continuations over beams and vocabulary.  Row k = entry * beams +
+ * beam has vocab logits x at logits + k * row_stride (elements; F32, BF16 or
+ * F16, any alignment of the dtype) and the score scores[k] so far:
+ *   s(k, t) = scores[k] + x[t] - log(sum_t exp(x[t])),
+ * but where ended[k] != 0 only t = end_token continues, with scores[k] as it
+ * is and the logits not read.  Of each batch entry the n_out largest, in order
+ * (of equal ones the lowest beam * vocab + t first):
+ *   scores_after = s, tokens = t, parents = k (a row of this call: what
+ *   mf_page_book_fork takes), ended_after = (t == end_token).
+ * A logit of -inf is no candidate, nor is any of a row whose score or sum is
+ * not finite (-inf: a beam not in use; NaN or +inf among the logits).  Where
+ * there are fewer than n_out candidates, the rest is -inf, -1, -1, 0.
+ * Scores are ranked in float64 and rounded once; the sums' terms are float32
+ * (2^-22 of themselves), their partial sums float64.
+ * beams is at most 1024, n_out at most 128, vocab at most 2^30, beams * vocab
+ * below 2^31.  A handle
+ * holds the workspace for batches of up to max_batch; it is not shared between
+ * streams that run at once.  One launch. */
+typedef struct mf_beam_select_config {
+    int32_t dtype;
+    int32_t vocab;
+    int32_t beams;
+    int32_t n_out;
+    int32_t max_batch;
+    int32_t end_token; /* -1: none */
+    int64_t row_stride;
+} mf_beam_select_config;
+int mf_beam_select_create(const mf_beam_select_config* config, mf_beam_select* handle);
+/* ended and ended_after may be NULL. */
+int mf_beam_select_run(mf_beam_select handle, const void* logits, const float* scores, const int32_t* ended,
+                       int32_t batch, float* scores_after, int32_t* tokens, int32_t* parents, int32_t* ended_after,
+                       mf_stream stream);
+/* The destroy calls of K11 wait for the device, then free the workspace; after mf_shutdown, too. */
+int mf_beam_select_destroy(mf_beam_select handle);
+
+/* Page tables of which rows share pages.  Beside lens, table and the pool of
+ * mf_page_assign a cache then has shares[n_pages]: how many rows hold a page
+ * beyond the first.  It is 0 for a page that one row holds, so that what
+ * mf_page_assign grants needs no entry, and 0 for a free page; a row's page
+ * that is not full belongs to it alone (fork sees to that).  A row holds
+ * ceil(lens / page_size) entries of its table, at most max_pages (lens counts as
+ * no more than those hold, negative as 0).  Outputs are other buffers than the
+ * inputs, which stay as they are; free_pages and free_after have n_pages
+ * entries, pool and pool_after are as mf_page_assign's.  What is not named below
+ * is not written.
+ *
+ * fork: row r of n_after continues row p = parents[r] of n_before; any other p
+ * (negative, or past the rows) begins empty: lens_after = 0.
+ *   The first row to continue p has p's pages; every further one shares the full
+ *   ones and, if the last is partly filled, gets a page of its own in its place
+ *   and a move {p's page, its own, lens % page_size, 0} in moves (n_after
+ *   entries, in the order of the rows).
+ *   shares_after[x] = shares[x] + the further rows that share x - the rows that
+ *   hold x and are not continued.  A page that this leaves without a row is
+ *   free, with shares_after 0.
+ *   The list of free pages becomes those, lowest number first, then
+ *   free_pages[pool[0] ...]; new pages are taken from its front in the order of
+ *   the rows, what is left is free_after from entry 0 on.  Where it ends too
+ *   early the later rows that need a page begin empty and share nothing.
+ *   table_after[r] has -1 behind the row's pages, lens_after = lens of p.
+ *   pool_after = {0, pages left, moves, rows that got no page}.
+ * To end rows, leave them out (or give parents of -1) and let the others go on.
+ *
+ * compact: a page is in use if the pool does not list it.  With limit = max(limit,
+ * pages in use), the pages in use from `limit` on move, in ascending order, to the
+ * lowest free ones: numbers[x] is where page x is afterwards (x itself if it
+ * stays or is free), moves (n_pages / 2 entries, at least 1) has {x, numbers[x],
+ * page_size, 0} of those that move, table_after the renamed table (-1 behind a
+ * row's pages), shares_after the moved shares, free_after the free pages, lowest
+ * first, pool_after = {0, free pages, moves, 0}.  limit 0: the pages in use
+ * become 0, 1, 2, ... without a gap.  The tables name every page in use, or
+ * their other holders rename theirs by `numbers`.
+ * After either call run mf_page_copy on the moves before the caches are used.
+ *
+ * A page number outside the cache, a list of free pages past its buffer or with
+ * a page twice record MF_DEVICE_BAD_PAGE: the number stays as it is and holds
+ * nothing, such a list counts as no more pages than there are.
+ * The handle holds the workspace for up to max_requests rows; it is not shared
+ * between streams that run at once.  One launch. */
+typedef struct mf_page_move {
+    int32_t src, dst; /* pages */
+    int32_t tokens;   /* the first so many */
+    int32_t reserved;
+} mf_page_move;
+typedef struct mf_page_book_config {
+    int32_t page_size;
+    int32_t max_pages;    /* entries of a row of the table */
+    int64_t table_stride; /* int32 entries from one row to the next, >= max_pages */
+    int32_t n_pages;
+    int32_t max_requests;
+} mf_page_book_config;
+int mf_page_book_create(const mf_page_book_config* config, mf_page_book* handle);
+int mf_page_book_fork(mf_page_book handle, const int32_t* table, const int32_t* lens, int32_t n_before,
+                      const int32_t* parents, int32_t n_after, const int32_t* shares, const int32_t* free_pages,
+                      const int32_t* pool, int32_t* table_after, int32_t* lens_after, int32_t* shares_after,
+                      int32_t* free_after, int32_t* pool_after, mf_page_move* moves, mf_stream stream);
+int mf_page_book_compact(mf_page_book handle, const int32_t* table, const int32_t* lens, int32_t n_requests,
+                         const int32_t* shares, const int32_t* free_pages, const int32_t* pool, int32_t limit,
+                         int32_t* table_after, int32_t* shares_after, int32_t* free_after, int32_t* pool_after,
+                         int32_t* numbers, mf_page_move* moves, mf_stream stream);
+int mf_page_book_destroy(mf_page_book handle);
+
+/* The first moves[i].tokens tokens of page src copied to page dst, all heads, in
+ * each of n_caches caches of one layout (keys and values of every layer; a host
+ * array of device addresses), for the first min(n_moves, *count) moves (count: on
+ * the device, e.g. pool_after + 2; NULL: n_moves).  No page may be the dst of
+ * two moves, or the src of one and the dst of another.  tokens counts as
+ * 0 to page_size.  A move that names a page outside the cache is left out and records
+ * MF_DEVICE_BAD_PAGE.  Elements of any dtype of a whole number of bytes; any
+ * strides, head_dim contiguous. */
+int mf_page_copy(const mf_cache_layout* layout, void* const* caches, int32_t n_caches, const mf_page_move* moves,
+                 int32_t n_moves, const int32_t* count, mf_stream stream);
 
 /* ---------------------------------------------------------------------
  * Measurement.  No counterpart in the reference (it has no device code).

@@ -119,6 +119,32 @@ class PagedAttnConfig(ctypes.Structure):
     ]
 
 
+class BeamSelectConfig(ctypes.Structure):
+    """mf_beam_select_config."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("vocab", ctypes.c_int32),
+        ("beams", ctypes.c_int32),
+        ("n_out", ctypes.c_int32),
+        ("max_batch", ctypes.c_int32),
+        ("end_token", ctypes.c_int32),
+        ("row_stride", ctypes.c_int64),
+    ]
+
+
+class PageBookConfig(ctypes.Structure):
+    """mf_page_book_config."""
+
+    _fields_ = [
+        ("page_size", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("table_stride", ctypes.c_int64),
+        ("n_pages", ctypes.c_int32),
+        ("max_requests", ctypes.c_int32),
+    ]
+
+
 _vp = ctypes.c_void_p
 _i32 = ctypes.c_int32
 _i64 = ctypes.c_int64
@@ -192,6 +218,14 @@ SIGNATURES: dict[str, list] = {
     "mf_paged_attn_create": [ctypes.POINTER(PagedAttnConfig), ctypes.POINTER(_vp)],
     "mf_paged_attn_run": [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp],
     "mf_paged_attn_destroy": [_vp],
+    "mf_beam_select_create": [ctypes.POINTER(BeamSelectConfig), ctypes.POINTER(_vp)],
+    "mf_beam_select_run": [_vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp],
+    "mf_beam_select_destroy": [_vp],
+    "mf_page_book_create": [ctypes.POINTER(PageBookConfig), ctypes.POINTER(_vp)],
+    "mf_page_book_fork": [_vp, _vp, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    "mf_page_book_compact": [_vp, _vp, _vp, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    "mf_page_book_destroy": [_vp],
+    "mf_page_copy": [ctypes.POINTER(CacheLayout), ctypes.POINTER(_vp), _i32, _vp, _i32, _vp, _vp],
 }
 
 _lib: ctypes.CDLL | None = None

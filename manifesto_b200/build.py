@@ -35,6 +35,8 @@ SOURCES = [
     "pages.cu",
     "rope.cu",
     "paged_attn.cu",
+    "beam.cu",
+    "page_book.cu",
     "comm.cu",
     "probe.cu",
 ]

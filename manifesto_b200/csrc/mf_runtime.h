@@ -46,9 +46,23 @@ inline bool is_float_store_dtype(int dt) {
     return dt == MF_DT_F32 || dt == MF_DT_BF16 || dt == MF_DT_F16;
 }
 inline bool is_fp8(int dt) { return dt == MF_DT_F8E4M3 || dt == MF_DT_F8E5M2; }
+// Bytes of an element, 0 for packed and unknown dtypes.
+inline int element_size(int dt) {
+    switch (dt) {
+    case MF_DT_F64: case MF_DT_I64: case MF_DT_U64: return 8;
+    case MF_DT_F32: case MF_DT_I32: case MF_DT_U32: return 4;
+    case MF_DT_F16: case MF_DT_BF16: case MF_DT_I16: case MF_DT_U16: return 2;
+    case MF_DT_F8E4M3: case MF_DT_F8E5M2: case MF_DT_I8: case MF_DT_U8: return 1;
+    default: return 0;
+    }
+}
 inline bool is_decodable(int dt) {
     return dt >= MF_DT_F64 && dt <= MF_DT_U8;
 }
+
+// Wait for the device that a handle belongs to and free its workspace; also after mf_shutdown, or with another device in
+// use: what a handle owns has no other way out.
+cudaError_t free_workspace(int device, void* workspace);
 
 // Most requests of one call: loops over them in 32 bits may step past the last
 // by a grid or a tile.

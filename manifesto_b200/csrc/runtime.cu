@@ -63,6 +63,18 @@ int64_t stream_grid(int64_t work_items, int threads, int blocks_per_sm) {
     return blocks;
 }
 
+cudaError_t free_workspace(int device, void* workspace) {
+    int current = -1;
+    cudaError_t err = cudaGetDevice(&current);
+    if (err == cudaSuccess && current != device) err = cudaSetDevice(device);
+    if (err != cudaSuccess) return err;
+    err = cudaDeviceSynchronize();  // the handle's last run may still use it
+    const cudaError_t freed = cudaFree(workspace);
+    if (err == cudaSuccess) err = freed;
+    if (current != device) cudaSetDevice(current);
+    return err;
+}
+
 // One thread polls the flag with acquire loads, sleeping between polls; when
 // the poll budget runs out it records MF_DEVICE_TIMEOUT and returns, so the
 // stream moves on and the context stays usable.

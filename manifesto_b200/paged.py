@@ -192,3 +192,89 @@ class PagedAttention:
                 self.close()
             except Exception:
                 pass  # interpreter shutdown, or the library is closed
+
+
+class _Handle:
+    """An object of the library that owns a workspace: created once, closed at the end."""
+
+    _handle = None
+    _destroy = ""
+
+    def _create(self, name: str, *args) -> None:
+        handle = ctypes.c_void_p()
+        _abi.call(name, *args, ctypes.byref(handle))
+        self._handle = handle.value
+
+    def _open(self) -> int:
+        if self._handle is None:
+            raise TensorClosed(f"{type(self).__name__}: closed")
+        return self._handle
+
+    def close(self) -> None:
+        """Wait for the device and free the workspace."""
+        if self._handle is not None:
+            handle, self._handle = self._handle, None
+            _abi.call(self._destroy, handle)
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.close()
+
+    def __del__(self):
+        if getattr(self, "_handle", None) is not None:
+            try:
+                self.close()
+            except Exception:
+                pass  # interpreter shutdown, or the library is closed
+
+
+class PageBook(_Handle):
+    """Page tables whose rows share pages: rows continued by parents, or ended (``fork``), and the pages in use
+    moved together (``compact``); mf_page_book_*.  Both list the pages to copy: run ``PageCopy`` next.
+
+    Holds the workspace for up to ``max_requests`` rows, so one object serves one stream at a time."""
+
+    _destroy = "mf_page_book_destroy"
+
+    def __init__(self, page_size: int, max_pages: int, n_pages: int, max_requests: int, table_stride: int | None = None):
+        self.config = _abi.PageBookConfig(int(page_size), int(max_pages), int(max_pages if table_stride is None else table_stride),
+                                          int(n_pages), int(max_requests))
+        self._create("mf_page_book_create", ctypes.byref(self.config))
+        self._fork, self._compact = _abi.lib().mf_page_book_fork, _abi.lib().mf_page_book_compact
+
+    def fork(self, table: int, lens: int, n_before: int, parents: int, n_after: int, shares: int, free_pages: int, pool: int,
+             table_after: int, lens_after: int, shares_after: int, free_after: int, pool_after: int, moves: int,
+             stream=None) -> None:
+        """Row r of n_after continues row parents[r] of n_before; ``moves`` has room for n_after entries of 16 bytes."""
+        rc = self._fork(self._open(), table, lens, n_before, parents, n_after, shares, free_pages, pool, table_after, lens_after,
+                        shares_after, free_after, pool_after, moves, stream if stream is None else stream_handle(stream))
+        if rc:
+            _raise("mf_page_book_fork", rc)
+
+    def compact(self, table: int, lens: int, n_requests: int, shares: int, free_pages: int, pool: int, limit: int,
+                table_after: int, shares_after: int, free_after: int, pool_after: int, numbers: int, moves: int,
+                stream=None) -> None:
+        """Pages in use from ``limit`` on (0: from their count on) moved below it; ``moves`` has room for n_pages / 2."""
+        rc = self._compact(self._open(), table, lens, n_requests, shares, free_pages, pool, limit, table_after, shares_after,
+                           free_after, pool_after, numbers, moves, stream if stream is None else stream_handle(stream))
+        if rc:
+            _raise("mf_page_book_compact", rc)
+
+
+class PageCopy:
+    """The moves of ``PageBook`` carried out in every cache of a layout: keys and values of all layers (mf_page_copy)."""
+
+    def __init__(self, cache: CacheLayout, caches: list[int]):
+        self._layout = ctypes.byref(cache.struct)
+        self._caches = (ctypes.c_void_p * len(caches))(*caches)
+        self._n = len(caches)
+        self._copy = _abi.lib().mf_page_copy
+
+    def run(self, moves: int, n_moves: int, count: int = 0, stream=None) -> None:
+        """The first n_moves moves, or as many as ``count`` says on the device (``pool_after`` + 8 bytes)."""
+        rc = self._copy(self._layout, self._caches, self._n, moves, n_moves, count or None,
+                        stream if stream is None else stream_handle(stream))
+        if rc:
+            _raise("mf_page_copy", rc)
