@@ -105,6 +105,7 @@ typedef struct mf_ckpt_plan_s* mf_ckpt_plan;
 typedef struct mf_paged_attn_s* mf_paged_attn;
 typedef struct mf_beam_select_s* mf_beam_select;
 typedef struct mf_page_book_s* mf_page_book;
+typedef struct mf_prefix_attn_s* mf_prefix_attn;
 
 /* ---------------------------------------------------------------------
  * Lifecycle and errors
@@ -735,6 +736,28 @@ int mf_page_book_destroy(mf_page_book handle);
  * strides, head_dim contiguous. */
 int mf_page_copy(const mf_cache_layout* layout, void* const* caches, int32_t n_caches, const mf_page_move* moves,
                  int32_t n_moves, const int32_t* count, mf_stream stream);
+
+/* mf_paged_attn_run for groups of requests that share their first tokens.
+ * Requests starts[g] .. starts[g + 1] - 1 (starts: n_groups + 1 ascending
+ * entries on the device) form group g and have the same pages for their first
+ * shared[g] tokens, which are read once for all of them, through the table row
+ * of the group's first request, as products on the tensor cores whose rows are
+ * the group's queries; the tokens behind them are read request by request.
+ * out and lse are those that mf_paged_attn_run defines, for every request, with
+ * the window, cap, slopes and scales of the config; shared[g] may be any number
+ * of tokens (negative: 0), and a member may be shorter than it.  Requests in no
+ *XX * Over the shared tokens the weights exp(s - max) enter the product with the
+ * values as two 16-bit terms, as in mf_paged_attn_run; queries over an FP8 cache
+ * are held as there.  head_dim, dtypes, strides and alignments as there.
+ * The workspace holds float32 parts of max_requests x q_heads x head_dim, three
+ * times, and 20 to 40 MB more; it is not shared between streams that run at
+ * once.  Three launches, no host sync; results do not depend on the order in
+ * which parts finish. */
+int mf_prefix_attn_create(const mf_paged_attn_config* config, int32_t max_requests, mf_prefix_attn* handle);
+int mf_prefix_attn_run(mf_prefix_attn handle, const void* q, const void* k_cache, const void* v_cache,
+                       const int32_t* table, const int32_t* lens, int32_t n_requests, const int32_t* starts,
+                       const int32_t* shared, int32_t n_groups, void* out, float* lse, mf_stream stream);
+int mf_prefix_attn_destroy(mf_prefix_attn handle);
 
 /* ---------------------------------------------------------------------
  * Measurement.  No counterpart in the reference (it has no device code).

@@ -218,6 +218,9 @@ SIGNATURES: dict[str, list] = {
     "mf_paged_attn_create": [ctypes.POINTER(PagedAttnConfig), ctypes.POINTER(_vp)],
     "mf_paged_attn_run": [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp],
     "mf_paged_attn_destroy": [_vp],
+    "mf_prefix_attn_create": [ctypes.POINTER(PagedAttnConfig), _i32, ctypes.POINTER(_vp)],
+    "mf_prefix_attn_run": [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _i32, _vp, _vp, _vp],
+    "mf_prefix_attn_destroy": [_vp],
     "mf_beam_select_create": [ctypes.POINTER(BeamSelectConfig), ctypes.POINTER(_vp)],
     "mf_beam_select_run": [_vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp],
     "mf_beam_select_destroy": [_vp],

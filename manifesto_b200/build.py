@@ -35,6 +35,7 @@ SOURCES = [
     "pages.cu",
     "rope.cu",
     "paged_attn.cu",
+    "prefix_attn.cu",
     "beam.cu",
     "page_book.cu",
     "comm.cu",

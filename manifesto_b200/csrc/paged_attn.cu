@@ -52,6 +52,7 @@
 // at the copy rate).
 #include <new>
 
+#include "mf_attn.cuh"
 #include "mf_divisor.cuh"
 #include "mf_internal.h"
 #include "mf_launch.cuh"
@@ -62,8 +63,6 @@ namespace mf {
 namespace {
 
 constexpr int kBlock = 16;         // tokens of one product; a tile is one or two blocks
-constexpr float kLog2e = 1.44269504088896341f;
-constexpr float kLn2 = 0.693147180559945309f;
 
 // Ordered by first use: the start of a run waits for a line of parameters only once or twice.
 struct AttnArgs {
@@ -93,18 +92,11 @@ struct AttnArgs {
     float* cta_part;      // [CTAs][3][heads * (DP + 2)]: parts that leave the CTA, and joined groups of them
     int32_t* tickets;     // [2][CTAs], zero between runs
     int32_t* status;
+    const int32_t* own_first;  // of a run of parts: each request's first token
 };
 
 // ------------------------------------------------------------------ pieces
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -146,44 +138,11 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-template <bool BF16>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-    uint32_t r;
-    if constexpr (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-template <bool BF16>
-__device__ __forceinline__ void unpack2(uint32_t v, float& lo, float& hi) {
-    if constexpr (BF16) {
-        lo = __uint_as_float(v << 16);
-        hi = __uint_as_float(v & 0xffff0000u);
-    } else {
-        f16x2_to_f32x2(v, lo, hi);
-    }
-}
-__device__ __forceinline__ float exp2_fast(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
 // Barrier of a team's warps.
 template <int TM>
 __device__ __forceinline__ void team_sync(int team) {
     if constexpr (TM == 1) __syncwarp();
     else asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(32 * TM) : "memory");
-}
-// Four FP8 codes -> two f16x2, exact: codes 0, 1 and codes 2, 3.
-template <int DT>
-__device__ __forceinline__ void fp8x4_to_f16(uint32_t four, uint32_t& low, uint32_t& high) {
-    if constexpr (DT == MF_DT_F8E4M3) {
-        asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
-            : "=r"(low), "=r"(high)
-            : "r"(four));
-    } else {
-        low = __byte_perm(four, 0u, 0x1404u);
-        high = __byte_perm(four, 0u, 0x3424u);
-    }
 }
 // The same for codes 0, 2 and codes 1, 3.
 template <int DT>
@@ -195,44 +154,20 @@ __device__ __forceinline__ void fp8x4_to_f16_strided(uint32_t four, uint32_t& ev
         odd = __byte_perm(four, 0u, 0x3414u);
     }
 }
-// exp2(m_old - m_new) for m_old <= m_new, 1 where both are the same infinity.
-__device__ __forceinline__ float rescale(float m_old, float m_new) {
-    return m_old == m_new ? 1.0f : exp2_fast(m_old - m_new);
-}
-
-__device__ __forceinline__ float rcp_fast(float x) {
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-
-// A capped score times log2(e), softcap log2(e) tanh(y), of p = 2 log2(e) y.  With e = exp2(p), tanh(y) = 1 - 2 / (1 + e)
-// takes one exponential and one reciprocal and has its limits at both ends, but is only good to 2^-22 of 1: a score far
-// below the cap would lose bits.  Below y = 0.4 a polynomial in p^2 stands in (tanh(y) / y by minimax of the relative
-// error, 1e-7), above, 2^-22 is 5e-7 of tanh(y).  A warp whose scores are all below takes the polynomial alone: 256
-// requests ragged to 8192 tokens, E4M3, take 399 us with a cap of 30 and without one (401 with the exponential form
-// up to a cap of 64 and tanhf above).
-constexpr float kSmallCapped = 1.15415603f;  // 0.4 * 2 log2(e)
-__device__ __forceinline__ float cap_small(float p, float softcap) {
-    const float v = p * p;
-    return p * softcap * __fmaf_rn(__fmaf_rn(__fmaf_rn(v, -4.1202753e-5f, 9.5731476e-4f), v, -0.020017692f), v, 0.49999995f);
-}
-__device__ __forceinline__ float cap_large(float p, float cap) {
-    return __fmaf_rn(-2.0f * cap, rcp_fast(1.0f + exp2_fast(p)), cap);
-}
-
 // A request's tokens: [first, len) are seen, in tiles from `base` on (a multiple
 // of the block, so that a block never crosses a page of whole blocks).
 struct Span {
     int32_t len, first, base;
 };
+template <bool PART>
 __device__ __forceinline__ Span span_of(const AttnArgs& a, int32_t r) {
     const int64_t reach = static_cast<int64_t>(a.max_pages) * a.page;
     Span s;
     s.len = max(a.lens[r], 0);
     if (s.len > reach) s.len = static_cast<int32_t>(reach);
     s.first = a.window > 0 && s.len > a.window ? s.len - a.window : 0;
-    s.base = s.first & ~(kBlock - 1);
+    if constexpr (PART) s.first = min(max(s.first, a.own_first[r]), s.len);
+    s.base = PART && s.first == s.len ? s.len : s.first & ~(kBlock - 1);
     return s;
 }
 template <int T>
@@ -241,7 +176,7 @@ __device__ __forceinline__ int32_t tiles_of(const Span& s) {
 }
 
 // A place in the row of all tiles: request, item of the request, tile of the item.
-template <int T>
+template <int T, bool PART>
 struct Place {
     int32_t r, item, t, nt;   // nt: tiles of the request's items
     Span span;
@@ -252,25 +187,10 @@ struct Place {
         item = 0;
         nt = 0;
         while (++r < a.n_requests) {
-            span = span_of(a, r);
+            span = span_of<PART>(a, r);
             nt = tiles_of<T>(span);
             if (nt > 0) return;
         }
-    }
-};
-
-// An even cut of `total` into `parts`: part i starts at total * i / parts, in 32 bits (parts are below 2^15).
-struct Cut {
-    int32_t total, parts, q, rem;
-    __device__ __forceinline__ Cut(int32_t total_, int32_t parts_)
-        : total(total_), parts(parts_), q(total_ / parts_), rem(total_ % parts_) {}
-    __device__ __forceinline__ int32_t start(int32_t i) const { return q * i + rem * i / parts; }
-    // the part that x is in, of a cut without empty parts
-    __device__ __forceinline__ int32_t part_of(int32_t x) const {
-        int32_t i = min(parts - 1, static_cast<int32_t>((static_cast<float>(x) + 0.5f) * static_cast<float>(parts) / static_cast<float>(total)));
-        while (start(i) > x) --i;
-        while (i + 1 < parts && start(i + 1) <= x) ++i;
-        return i;
     }
 };
 
@@ -361,9 +281,14 @@ __device__ __forceinline__ uint32_t pieces_on(uint32_t at, int c) {
     else return at ^ static_cast<uint32_t>(c * 16);
 }
 
-// Write `f` (4 floats of head h, elements d..d+3, normalised) to the output.
+// Write `f` (4 floats of head h, elements d..d+3, normalised) to the output; a run of parts has a float32 one.
+template <bool PART>
 __device__ __forceinline__ void store_out4(const AttnArgs& a, int32_t r, int32_t head, int d, float4 f) {
     if (d >= a.head_dim) return;
+    if constexpr (PART) {
+        *reinterpret_cast<float4*>(a.out + 4 * (r * a.out_req + head * a.out_head + d)) = f;
+        return;
+    }
     char* p = a.out + 2 * (r * a.out_req + head * a.out_head + d);
     const float v[4] = {f.x, f.y, f.z, f.w};
     uint32_t w[2];
@@ -412,7 +337,7 @@ __device__ __forceinline__ bool arrive_last(int32_t* ticket, int32_t count) {
 // at at0 and the last at at_end: to the output if `to` is NULL, else to a part
 // there.  All threads of the CTA; the parts pass through shared memory, as many
 // at a time as it holds.
-template <class K, int DP>
+template <class K, int DP, bool PART>
 __device__ __forceinline__ void join_parts(const AttnArgs& a, typename K::Shared& sh, unsigned char* smem, const float* first,
                                            int64_t stride, const float* at0, const float* at_end, int32_t n, const Joined& w,
                                            float* to) {
@@ -486,7 +411,7 @@ __device__ __forceinline__ void join_parts(const AttnArgs& a, typename K::Shared
                 to[kFloats + K::kHeads + h] = sum;
             }
         } else {
-            store_out4(a, w.r, w.head0 + h, d, scale4(acc[e], sum == 0.0f ? 0.0f : __fdiv_rn(vs, sum)));
+            store_out4<PART>(a, w.r, w.head0 + h, d, scale4(acc[e], sum == 0.0f ? 0.0f : __fdiv_rn(vs, sum)));
             if (d == 0) store_lse<K>(a, w.r, w.head0 + h, sh.top[h], sum);
         }
     }
@@ -506,7 +431,8 @@ __device__ __forceinline__ int32_t ctas_of(const AttnArgs& a, int32_t nt, int fi
     return max(min(static_cast<int32_t>(gridDim.x) / a.items, (nt - 1) / K::kTeams + 1), 1);
 }
 
-template <int MODE, int DP, int TM, int W, int T, int S>
+// PART: the requests' tokens from own_first on alone, to a float32 out.
+template <int MODE, int DP, int TM, int W, int T, int S, bool PART>
 __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a) {
     using K = Attn<MODE, DP, TM, W, T, S>;
     extern __shared__ __align__(128) unsigned char smem[];
@@ -526,7 +452,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
     for (int32_t i = 0; i < per; ++i) {
         const int32_t r = tid * per + i;
         if (r >= a.n_requests) break;
-        const int32_t nt = tiles_of<T>(span_of(a, r));
+        const int32_t nt = tiles_of<T>(span_of<PART>(a, r));
         sum += static_cast<int64_t>(nt) * items;
         nt_of = nt;
         empty |= nt == 0 && r % gridDim.x == blockIdx.x;
@@ -551,9 +477,9 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
     if (__syncthreads_or(empty)) {
         // requests that see nothing
         for (int32_t r = blockIdx.x; r < a.n_requests; r += gridDim.x) {
-            if (tiles_of<T>(span_of(a, r)) > 0) continue;
+            if (tiles_of<T>(span_of<PART>(a, r)) > 0) continue;
             for (int i = tid; i < a.q_heads * (a.head_dim / 4); i += K::kThreads)
-                store_out4(a, r, i / (a.head_dim / 4), i % (a.head_dim / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f));
+                store_out4<PART>(a, r, i / (a.head_dim / 4), i % (a.head_dim / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f));
             for (int i = tid; i < a.q_heads; i += K::kThreads) store_lse<K>(a, r, i, 0.0f, 0.0f);
         }
     }
@@ -602,12 +528,12 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
     if (blockIdx.x >= ctas) return;
     const Cut by_cta(total, ctas);
     const int32_t id = blockIdx.x * K::kTeams + team;
-    Place<T> at{};
+    Place<T, PART> at{};
     int32_t x0, my_tiles, own_first = 0, own_last = 0;  // first tile in the row (of the item, if it has its own CTAs), tiles
     if (own) {
         int32_t into;
         at.r = locate(ctas_of_warp, [&](int t) { return ctas_of<K>(a, sh.thread_nt[t], fill) * items; }, blockIdx.x, into);
-        at.span = span_of(a, at.r);
+        at.span = span_of<PART>(a, at.r);
         at.nt = tiles_of<T>(at.span);
         const int32_t each = ctas_of<K>(a, at.nt, fill);
         at.item = into / each;
@@ -629,7 +555,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
             at.r = locate(tiles_of_warp, [&](int t) { return sh.thread_sum[t]; }, x0, into);
             if (per > 1) {
                 for (int32_t r0 = at.r * per;; r0 += 32) {
-                    const int32_t mine = r0 + lane < a.n_requests ? tiles_of<T>(span_of(a, r0 + lane)) * items : 0;
+                    const int32_t mine = r0 + lane < a.n_requests ? tiles_of<T>(span_of<PART>(a, r0 + lane)) * items : 0;
                     int32_t upto = mine;
 #pragma unroll 1
                     for (int d = 1; d < 32; d <<= 1) {
@@ -646,7 +572,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                     into -= __shfl_sync(0xffffffffu, upto, 31);
                 }
             }
-            at.span = span_of(a, at.r);
+            at.span = span_of<PART>(a, at.r);
             at.nt = tiles_of<T>(at.span);
             at.item = into / at.nt;
             at.t = into - at.item * at.nt;
@@ -659,7 +585,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
     if (my_tiles > 0) {
         unsigned char* my_ring = smem + team * (S * K::kStage);
         const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(my_ring));
-        Place<T> load = at;
+        Place<T, PART> load = at;
         int32_t to_load = my_tiles;
         const bool whole = a.page % kBlock == 0;         // a block lies in one page
         const bool dense = a.row_bytes == DP * K::kBytes;  // rows follow one another
@@ -776,7 +702,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
             team_sync<TM>(team);
         }
         // the queries of the item at `p`, as they are
-        auto load_queries = [&](const Place<T>& p) {
+        auto load_queries = [&](const Place<T, PART>& p) {
             const Heads<K::kHeads> hd(a, p.item);
             const int h = member * 8 + g;
             const char* q = a.q + 2 * (p.r * a.q_req + (hd.head0 + h) * a.q_head);
@@ -1008,7 +934,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                 stage = stage + 1 == S ? 0 : stage + 1;
             }
             done += tb - ta;
-            Place<T> following = at;
+            Place<T, PART> following = at;
             following.t = tb - 1;
             const bool ends = tb == at.nt, stops = done == my_tiles;  // the item, this team's run
             if (!stops) {
@@ -1033,10 +959,19 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                         f[x] = l[x] == 0.0f ? 0.0f : __fdiv_rn(vs, l[x]);
                         if (g == 0 && h < hd.count) store_lse<K>(a, at.r, hd.head0 + h, m[x], l[x]);
                     }
-                    char* out = a.out + 2 * (at.r * a.out_req + hd.head0 * a.out_head);
+                    char* out = a.out + (PART ? 4 : 2) * (at.r * a.out_req + hd.head0 * a.out_head);
 #pragma unroll
                     for (int c = 0; c < K::kSteps; ++c) {
-                        if constexpr (!K::kFp8) {
+                        if constexpr (PART) {
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) {
+                                const int h = member * 8 + 2 * j + x;
+                                const int d0 = K::kFp8 ? c * 16 + 2 * g : c * 16 + g, d1 = K::kFp8 ? d0 + 1 : d0 + 8;
+                                float* to = reinterpret_cast<float*>(out) + h * a.out_head;
+                                if (h < hd.count && d0 < a.head_dim) to[d0] = o[c][x] * f[x];
+                                if (h < hd.count && d1 < a.head_dim) to[d1] = o[c][x + 2] * f[x];
+                            }
+                        } else if constexpr (!K::kFp8) {
                             // elements x heads -> heads x elements
                             const uint32_t u = transpose8x8(pack2<K::kBf16>(o[c][0] * f[0], o[c][1] * f[1]));
                             const uint32_t w = transpose8x8(pack2<K::kBf16>(o[c][2] * f[0], o[c][3] * f[1]));
@@ -1189,7 +1124,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
         const float top = sh.joined_m[which][h], sum_l = sh.joined_l[which][h];
         if (w.slot < 0) {
             const float vs = a.v_scale ? a.v_scale[w.kv] : 1.0f;
-            store_out4(a, w.r, w.head0 + h, d, scale4(acc, sum_l == 0.0f ? 0.0f : __fdiv_rn(vs, sum_l)));
+            store_out4<PART>(a, w.r, w.head0 + h, d, scale4(acc, sum_l == 0.0f ? 0.0f : __fdiv_rn(vs, sum_l)));
             if (d == 0) store_lse<K>(a, w.r, w.head0 + h, top, sum_l);
         } else {
             float* to = a.cta_part + (static_cast<int64_t>(blockIdx.x) * 3 + w.slot) * K::kPart;
@@ -1250,7 +1185,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                 n = groups;
                 to = nullptr;
             }
-            if (to == nullptr || n > 1) join_parts<K, DP>(a, sh, smem, parts, stride, at0, at_end, n, w, to);
+            if (to == nullptr || n > 1) join_parts<K, DP, PART>(a, sh, smem, parts, stride, at0, at_end, n, w, to);
         }
     }
 }
@@ -1259,6 +1194,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
 
 struct Kernel {
     void (*fn)(AttnArgs);
+    void (*part_fn)(AttnArgs);
     int threads, shared, part_floats, teams;
 };
 
@@ -1266,7 +1202,7 @@ template <int MODE, int DP, int TM, int W, int T, int S>
 Kernel kernel_of() {
     using K = Attn<MODE, DP, TM, W, T, S>;
     static_assert(K::kSharedBytes <= 232448, "shared memory of one CTA");
-    return Kernel{paged_attn_kernel<MODE, DP, TM, W, T, S>, K::kThreads, K::kSharedBytes, K::kPart, K::kTeams};
+    return Kernel{paged_attn_kernel<MODE, DP, TM, W, T, S, false>, paged_attn_kernel<MODE, DP, TM, W, T, S, true>, K::kThreads, K::kSharedBytes, K::kPart, K::kTeams};
 }
 
 // Warps, tokens of a tile and stages: about 192 KB of ring per SM, the bytes in flight that keep HBM busy.
@@ -1436,17 +1372,38 @@ extern "C" int mf_paged_attn_run(mf_paged_attn handle, const void* q, const void
 
 extern "C" int mf_paged_attn_destroy(mf_paged_attn handle) {
     if (!handle) return MF_OK;
-    // also after mf_shutdown, or with another device in use: what the handle owns has no other way out
-    int current = -1;
-    cudaError_t err = cudaGetDevice(&current);
-    if (err == cudaSuccess && current != handle->device) err = cudaSetDevice(handle->device);
-    if (err == cudaSuccess) {
-        err = cudaDeviceSynchronize();  // its last run may still use the workspace
-        const cudaError_t freed = cudaFree(handle->workspace);
-        if (err == cudaSuccess) err = freed;
-        if (current != handle->device) cudaSetDevice(current);
-    }
+    const cudaError_t err = free_workspace(handle->device, handle->workspace);
     delete handle;
     if (err != cudaSuccess) return cuda_fail(err, "mf_paged_attn_destroy");
     return MF_OK;
 }
+
+namespace mf {
+
+int paged_attn_enable_parts(mf_paged_attn handle) {
+    MF_CUDA_CHECK(cudaFuncSetAttribute(reinterpret_cast<const void*>(handle->kernel.part_fn),
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, handle->kernel.shared));
+    return MF_OK;
+}
+
+int paged_attn_run_parts(mf_paged_attn handle, const void* q, const void* k_cache, const void* v_cache, const int32_t* table,
+                         const int32_t* lens, int32_t n_requests, const int32_t* own_first, float* out, float* lse,
+                         cudaStream_t stream) {
+    AttnArgs a = handle->args;
+    a.q = static_cast<const char*>(q);
+    a.k = static_cast<const char*>(k_cache);
+    a.v = static_cast<const char*>(v_cache);
+    a.table = table;
+    a.lens = lens;
+    a.n_requests = n_requests;
+    a.own_first = own_first;
+    a.out = reinterpret_cast<char*>(out);
+    a.out_head = a.head_dim;
+    a.out_req = static_cast<int64_t>(a.q_heads) * a.head_dim;
+    a.lse = lse;
+    const cudaError_t err = launch_overlapped(handle->kernel.part_fn, dim3(static_cast<unsigned>(handle->ctas)), handle->kernel.threads,
+                                              handle->kernel.shared, stream, a);
+    return err == cudaSuccess ? MF_OK : cuda_fail(err, "mf_prefix_attn_run");
+}
+
+}  // namespace mf

@@ -142,6 +142,18 @@ class RopeAppend:
             _raise("mf_rope_append", rc)
 
 
+def _attn_config(cache: CacheLayout, q_heads, dtype, max_pages, table_stride, scale, softcap, window, slopes, k_scale_inv,
+                 v_scale_inv, q_strides, out_strides) -> _abi.PagedAttnConfig:
+    dim = cache.struct.head_dim
+    qt, qh = q_strides or (q_heads * dim, dim)
+    ot, oh = out_strides or (q_heads * dim, dim)
+    return _abi.PagedAttnConfig(
+        cache.struct, int(dtype), int(q_heads), int(max_pages), int(window),
+        int(max_pages if table_stride is None else table_stride),
+        float(1.0 / math.sqrt(dim) if scale is None and dim > 0 else scale or 0.0), float(softcap), int(slopes) or None,
+        int(k_scale_inv) or None, int(v_scale_inv) or None, qt, qh, ot, oh)
+
+
 class PagedAttention:
     """Attention of one new token per request over a paged cache (mf_paged_attn_*).
 
@@ -152,14 +164,8 @@ class PagedAttention:
                  scale: float | None = None, softcap: float = 0.0, window: int = 0, slopes: int = 0, k_scale_inv: int = 0,
                  v_scale_inv: int = 0, q_strides: tuple[int, int] | None = None,
                  out_strides: tuple[int, int] | None = None):
-        dim = cache.struct.head_dim
-        qt, qh = q_strides or (q_heads * dim, dim)
-        ot, oh = out_strides or (q_heads * dim, dim)
-        self.config = _abi.PagedAttnConfig(
-            cache.struct, int(dtype), int(q_heads), int(max_pages), int(window),
-            int(max_pages if table_stride is None else table_stride),
-            float(1.0 / math.sqrt(dim) if scale is None and dim > 0 else scale or 0.0), float(softcap), int(slopes) or None,
-            int(k_scale_inv) or None, int(v_scale_inv) or None, qt, qh, ot, oh)
+        self.config = _attn_config(cache, q_heads, dtype, max_pages, table_stride, scale, softcap, window, slopes, k_scale_inv,
+                                   v_scale_inv, q_strides, out_strides)
         handle = ctypes.c_void_p()
         _abi.call("mf_paged_attn_create", ctypes.byref(self.config), ctypes.byref(handle))
         self._handle = handle.value
@@ -228,6 +234,33 @@ class _Handle:
                 self.close()
             except Exception:
                 pass  # interpreter shutdown, or the library is closed
+
+
+class PrefixAttention(_Handle):
+    """``PagedAttention`` for groups of requests that share the pages of their first tokens (mf_prefix_attn_*).
+
+    The shared tokens of a group are read once for all its requests: the beams of a prompt, or a batch that begins
+    with the same instructions.  Holds the workspace for up to ``max_requests``, so one object serves one stream at
+    a time; it runs any number of requests, groups, steps and layers of its shape."""
+
+    _destroy = "mf_prefix_attn_destroy"
+
+    def __init__(self, cache: CacheLayout, q_heads: int, dtype: DType, max_pages: int, max_requests: int,
+                 table_stride: int | None = None, scale: float | None = None, softcap: float = 0.0, window: int = 0,
+                 slopes: int = 0, k_scale_inv: int = 0, v_scale_inv: int = 0, q_strides: tuple[int, int] | None = None,
+                 out_strides: tuple[int, int] | None = None):
+        self.config = _attn_config(cache, q_heads, dtype, max_pages, table_stride, scale, softcap, window, slopes, k_scale_inv,
+                                   v_scale_inv, q_strides, out_strides)
+        self._create("mf_prefix_attn_create", ctypes.byref(self.config), int(max_requests))
+        self._attend = _abi.lib().mf_prefix_attn_run
+
+    def run(self, q: int, k_cache: int, v_cache: int, table: int, lens: int, n_requests: int, starts: int, shared: int,
+            n_groups: int, out: int, lse: int = 0, stream=None) -> None:
+        """Requests starts[g] .. starts[g + 1] - 1 have their first shared[g] tokens in the same pages."""
+        rc = self._attend(self._open(), q, k_cache, v_cache, table, lens, n_requests, starts, shared, n_groups, out, lse,
+                          stream if stream is None else stream_handle(stream))
+        if rc:
+            _raise("mf_prefix_attn_run", rc)
 
 
 class PageBook(_Handle):

@@ -1,0 +1,380 @@
+"""Attention over a shared prefix on the GPU against 64-bit attention of every request by itself."""
+import numpy as np
+import pytest
+
+from manifesto_b200 import Stream, paged, sync_device
+from manifesto_b200.dtype import DType
+from manifesto_b200.errors import (DTypeMismatch, DTypeUnsupported, InvalidArgument, LayoutUnsupported, ShapeInvalid, TensorClosed)
+
+from . import paged_ref as plain
+from .gpu_util import bits_equal, empty, fetch, to_device
+from .test_gpu_paged import BAD_PAGE, TYPES, check_attn, device_status, make_attn, want_attn
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32, E4M3, E5M2 = DType.BFLOAT16, DType.FLOAT16, DType.FLOAT32, DType.FLOAT8_E4M3, DType.FLOAT8_E5M2
+
+
+def make_groups(groups, hq, hkv, dim, page, order, dtype, cache, seed, alone=0):
+    """groups: (shared tokens, own tokens of each member; negative: that many tokens less than the shared ones)."""
+    lens, starts, shared = [5 + 3 * i for i in range(alone)], [alone], []
+    for common, own in groups:
+        lens += [common + x for x in own]
+        starts.append(len(lens))
+        shared.append(common)
+    full = [max(n, 0) for n in lens]
+    for g, common in enumerate(shared):  # the first member's row names every shared page
+        if starts[g] < starts[g + 1]:
+            full[starts[g]] = max(full[starts[g]], common)
+    s = make_attn(full, hq, hkv, dim, page, order, dtype, cache, seed)
+    for g, common in enumerate(shared):
+        lead = s["table"][starts[g]] if starts[g] < starts[g + 1] else None
+        for r in range(starts[g] + 1, starts[g + 1]):
+            whole, rest = common // page, common % page
+            n = min(whole, -(-full[r] // page))
+            s["table"][r, :n] = lead[:n]
+            if rest and full[r] > whole * page:  # the page where the members part: equal tokens in pages of their own
+                for c in s["kv"]:
+                    c[s["table"][r, whole], :min(rest, full[r] - whole * page)] = c[lead[whole], :min(rest, full[r] - whole * page)]
+    s["lens"] = np.array(lens, np.int32)
+    s["starts"], s["shared"] = np.array(starts, np.int32), np.array(shared, np.int32)
+    return s
+
+
+class Running:
+    """The case on the device."""
+
+    def __init__(self, s, softcap=0.0, window=0, slopes=None, scale=None, q_pad=0, max_requests=None):
+        self.s = s
+        kv = [c if s["order"] == "NHD" else np.ascontiguousarray(c.transpose(0, 2, 1, 3)) for c in s["kv"]]
+        n, hq, dim = s["q"].shape
+        wide = np.zeros((n, hq, dim + q_pad), s["q"].dtype)
+        wide[..., :dim] = s["q"]
+        self.bufs = [to_device(x) if x.size else empty(16) for x in (wide, kv[0], kv[1], s["table"], s["lens"], s["starts"], s["shared"])]
+        self.extra = [to_device(np.asarray(x, np.float32)) for x in (slopes, s["scales"]) if x is not None]
+        sl = self.extra[0].ptr if slopes is not None else 0
+        ks = self.extra[-1].ptr if s["scales"] is not None else 0
+        self.out_pad = 4 if q_pad else 0
+        width = dim + self.out_pad
+        self.out, self.lse = empty(n * hq * width * 2 + 16), empty(n * hq * 4 + 16)
+        layout = paged.CacheLayout(s["pages"], s["page"], s["hkv"], dim, s["cache"], s["order"])
+        self.attn = paged.PrefixAttention(layout, hq, s["dtype"], s["table"].shape[1], max_requests or n, scale=scale, softcap=softcap,
+                                          window=window, slopes=sl, k_scale_inv=ks, v_scale_inv=ks + 4 * s["hkv"] if ks else 0,
+                                          q_strides=(hq * (dim + q_pad), dim + q_pad), out_strides=(hq * width, width))
+
+    def run(self, stream=None, lse=True, groups=None):
+        s = self.s
+        n, hq, dim, width = len(s["lens"]), s["hq"], s["dim"], s["dim"] + self.out_pad
+        self.out.memset(0xA5)
+        self.lse.memset(0xA5)
+        sync_device()
+        p = [b.ptr for b in self.bufs]
+        self.attn.run(*p[:5], n, p[5], p[6], len(s["shared"]) if groups is None else groups, self.out.ptr, self.lse.ptr if lse else 0,
+                      stream=stream)
+        sync_device()
+        size = n * hq * width * 2
+        raw = fetch(self.out, self.out.nbytes)
+        assert (raw[size:] == 0xA5).all(), "wrote past the output"
+        out = raw[:size].view(np.uint16).reshape(n, hq, width)
+        assert (out[..., dim:] == 0xA5A5).all(), "wrote between the rows"
+        low = fetch(self.lse, self.lse.nbytes)
+        assert (low[(n * hq * 4 if lse else 0):] == 0xA5).all()
+        return out[..., :dim].copy(), low[:n * hq * 4].view(np.float32).reshape(n, hq).copy()
+
+    def close(self):
+        self.attn.close()
+        for b in (*self.bufs, *self.extra, self.out, self.lse):
+            b.free()
+
+
+def run_groups(groups, hq=4, hkv=2, dim=64, page=16, order="HND", dtype=BF16, cache=None, seed=7, alone=0, q_pad=0, stream=None, **rules):
+    """The bounds are those of the attention without sharing: the join adds float32 products of weights that are good to 2^-22."""
+    s = make_groups(groups, hq, hkv, dim, page, order, dtype, dtype if cache is None else cache, seed, alone)
+    on = Running(s, q_pad=q_pad, **rules)
+    device_status()
+    got = on.run(stream)
+    again = on.run(stream)
+    assert device_status() == 0
+    on.close()
+    check_attn(s, got, want_attn(s, **rules))
+    bits_equal(got[0], again[0])
+    bits_equal(got[1].view(np.uint32), again[1].view(np.uint32))
+
+
+def test_prefix_one_tile(backend):
+    run_groups([(128, [1, 2, 3, 4])])
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+@pytest.mark.parametrize("dim", [16, 64, 80, 96, 128, 192, 256])
+def test_prefix_types_and_head_dims(backend, dtype, cache, dim):
+    run_groups([(200, [3, 17, 1]), (35, [2, 40])], dim=dim, dtype=dtype, cache=cache)
+
+
+@pytest.mark.parametrize("dim", [8, 24, 72, 136])
+def test_prefix_head_dims_that_are_not_16s(backend, dim):
+    run_groups([(200, [3, 17, 1])], dim=dim, dtype=F16)
+
+
+@pytest.mark.parametrize("hq,hkv,members", [(1, 1, 2), (8, 1, 3), (5, 1, 30), (16, 1, 8), (16, 1, 9), (40, 1, 7), (14, 2, 19), (32, 32, 130), (32, 8, 70),
+                                            (64, 4, 33), (200, 1, 2)])
+@pytest.mark.parametrize("dim,cache", [(64, BF16), (128, BF16), (128, E4M3), (256, BF16)])
+def test_prefix_rows(backend, hq, hkv, members, dim, cache):
+    """Blocks of one row, of up to 128 (both groups of warps take turns), of up to 256 (each has its own), several blocks."""
+    if members * hq * dim > 200_000:
+        members = max(2, 200_000 // (hq * dim))
+    run_groups([(300, [1 + i % 3 for i in range(members)])], hq=hq, hkv=hkv, dim=dim, cache=cache)
+
+
+@pytest.mark.parametrize("shared", [0, 1, 15, 16, 63, 64, 65, 127, 128, 129, 255, 256, 257, 1000, 4097])
+@pytest.mark.parametrize("dim,cache", [(128, BF16), (64, E4M3), (256, F16)])
+def test_prefix_lengths(backend, shared, dim, cache):
+    run_groups([(shared, [1, 5, 0, 20])], dim=dim, dtype=F16 if cache == F16 else BF16, cache=cache)
+
+
+@pytest.mark.parametrize("page", [1, 2, 7, 16, 20, 48, 128, 300])
+@pytest.mark.parametrize("order", ["HND", "NHD"])
+def test_prefix_pages(backend, page, order):
+    """Shared lengths that end inside a page, too."""
+    run_groups([(page * 5, [1, 3, 9]), (page * 3 + page // 2, [0, 2, page, 3 * page])], page=page, order=order)
+
+
+@pytest.mark.parametrize("n", [1, 7, 60, 700])
+def test_prefix_many_groups(backend, n):
+    run_groups([(20 + 17 * (i % 9), [1 + (i + x) % 5 for x in range(2 + i % 4)]) for i in range(n)], hq=2, hkv=2, dim=32)
+
+
+def test_prefix_groups_of_all_sizes(backend):
+    """None, one member, many; requests in front of the groups; long and short ones side by side."""
+    run_groups([(100, []), (50, [3]), (700, [1] * 9), (0, [4, 5]), (5, [0, 0]), (2000, [1, 300]), (128, [7] * 150)], alone=4)
+
+
+def test_prefix_nothing_is_shared(backend):
+    run_groups([], alone=5)
+    run_groups([(64, [9])], alone=2)
+    run_groups([(0, [9, 8, 7])])
+
+
+def test_prefix_members_shorter_than_the_prefix(backend):
+    """Each sees its own length's part of the shared tokens; an idle one nothing."""
+    run_groups([(300, [5, -1, -171, -172, -173, -300, 0]), (300, [-300, 4, -299]), (40, [-40, -40])])
+
+
+@pytest.mark.parametrize("window", [1, 5, 16, 100, 130, 5000])
+def test_prefix_window(backend, window):
+    run_groups([(300, [1, 20, 90, 140, -30, 0]), (17, [3, 4])], window=window)
+
+
+@pytest.mark.parametrize("cache", [BF16, E4M3])
+@pytest.mark.parametrize("dim", [64, 256])
+def test_prefix_softcap_and_slopes(backend, cache, dim):
+    slopes = [2.0 ** (-x) for x in range(1, 5)]
+    run_groups([(300, [1, 20, -7])], cache=cache, dim=dim, softcap=20.0)
+    run_groups([(300, [1, 20, -7])], cache=cache, dim=dim, slopes=slopes)
+    run_groups([(300, [1, 20, -7])], cache=cache, dim=dim, softcap=3.0, slopes=slopes, window=77)
+
+
+@pytest.mark.parametrize("scale", [-0.1, 0.0, 0.7])
+def test_prefix_scales(backend, scale):
+    run_groups([(300, [1, 20, 2])], scale=scale)
+
+
+def test_prefix_strided_queries_and_outputs(backend):
+    run_groups([(300, [1, 20, 2])], q_pad=8)
+    run_groups([(300, [1, 20, 2])], q_pad=2)
+    run_groups([(300, [1, 20, 2])], q_pad=6, cache=E4M3)
+
+
+def test_prefix_on_another_stream(backend):
+    s = Stream()
+    run_groups([(300, [1, 20, 2])], stream=s)
+    s.close()
+
+
+@pytest.mark.parametrize("dtype,cache", [(BF16, BF16), (F16, E4M3)])
+def test_prefix_long(backend, dtype, cache):
+    """More tiles than CTAs for one item: every CTA has a part, most of them inside it."""
+    run_groups([(30011, [1, 2])], hq=2, hkv=1, dim=128, dtype=dtype, cache=cache)
+    run_groups([(9000, [1] * 70), (40, [1, 2]), (9000, [3, 4])], hq=4, hkv=1, dim=128, dtype=dtype, cache=cache)
+
+
+def test_prefix_nan_stays_with_its_request_and_head(backend):
+    s = make_groups([(300, [1, 20, 2, 9])], 4, 2, 64, 16, "HND", BF16, BF16, 3)
+    want = want_attn(s)
+    s["q"][2, 1, 5] = 0x7fc0
+    on = Running(s)
+    out, lse = on.run()
+    on.close()
+    o = plain.values(out, BF16)
+    assert np.isnan(o[2, 1]).all() and np.isnan(lse[2, 1])
+    o[2, 1], lse[2, 1], want[0][2, 1], want[1][2, 1], want[2][2, 1] = 0, 0, 0, 0, 0
+    keep = np.ones((4, 4), bool)
+    keep[2, 1] = False
+    assert np.isfinite(o).all() and (np.abs(o - want[0])[keep] <= 2e-4 * want[2][keep] + 2.0 ** -8 * 1.01 * np.abs(want[0][keep])).all()
+
+
+@pytest.mark.parametrize("dtype,cache", [(BF16, BF16), (F16, F16), (F16, E4M3)])
+def test_prefix_keys_that_leave_nothing(backend, dtype, cache):
+    """Scores of -inf for every token: nothing is seen."""
+    s = make_groups([(200, [1, 20, 2])], 2, 1, 64, 16, "HND", dtype, dtype, 3)
+    s["kv"][0][:] = plain.normal(1, s["kv"][0].shape, dtype, 0.0)
+    s["kv"][0][..., 0] = 0xff80 if dtype == BF16 else 0xfc00
+    s["q"][..., 0] = 0x3f80 if dtype == BF16 else 0x3c00
+    s["kv"][1][:] = 0
+    on = Running(s)
+    out, lse = on.run()
+    on.close()
+    assert (out == 0).all() and np.isneginf(lse).all()
+
+
+def test_prefix_page_outside_the_cache_is_masked_and_reported(backend):
+    s = make_groups([(300, [5, 20, 2])], 4, 2, 64, 16, "HND", BF16, BF16, 3)
+    for bad in (-1, 1 << 29):
+        s["table"][:, 3] = bad
+        on = Running(s)
+        device_status()
+        got = on.run()
+        assert device_status() == BAD_PAGE
+        on.close()
+        # the same without those 16 tokens
+        t = dict(s)
+        t["table"] = np.delete(s["table"], 3, 1)
+        t["lens"] = s["lens"] - 16
+        check_attn(t, got, want_attn(t))
+
+
+@pytest.mark.parametrize("starts", [[0, 3, 2, 6], [0, 2, 4, 7], [-1, 2, 4, 6], [0, 2 ** 31 - 1, 2, 6]])
+def test_prefix_groups_that_are_none_share_nothing(backend, starts):
+    s = make_groups([(100, [1, 2]), (100, [3, 4]), (100, [5, 6])], 4, 2, 64, 16, "HND", BF16, BF16, 3)
+    s["starts"] = np.array(starts, np.int32)
+    on = Running(s)
+    device_status()
+    got = on.run()
+    assert device_status() == 0x7300
+    on.close()
+    check_attn(s, got, want_attn(s))
+
+
+def test_prefix_shared_past_the_table_or_negative(backend):
+    s = make_groups([(96, [0, 0, -5]), (64, [1, 2])], 4, 2, 64, 16, "HND", BF16, BF16, 3)
+    s["shared"] = np.array([2 ** 31 - 1, -7], np.int32)
+    s["table"] = np.ascontiguousarray(s["table"][:, :6])
+    s["table"][0, 5] = s["table"][1, 5]
+    on = Running(s)
+    device_status()
+    got = on.run()
+    assert device_status() == 0
+    on.close()
+    check_attn(s, got, want_attn(s))
+
+
+@pytest.mark.parametrize("dtype,cache", [(BF16, BF16), (F16, F16), (F16, E4M3), (BF16, E4M3)])
+@pytest.mark.parametrize("lead", [12.0, 16.0, 20.0])
+def test_prefix_small_weights_beside_a_dominant_one(backend, dtype, cache, lead):
+    """A first token of value 0 that leads by `lead`: what the others add up to is all of the result."""
+    s = make_groups([(600, [1, 3])], 2, 1, 64, 16, "HND", dtype, cache, 5)
+    q = np.zeros(s["q"].shape)
+    q[..., 0] = 1.0
+    s["q"] = plain.normal(0, s["q"].shape, dtype, 0.0)
+    one = 0x3f80 if dtype == BF16 else 0x3c00
+    s["q"][..., 0] = one
+    keys, values = s["kv"]
+    if s["scales"] is not None:
+        s["scales"][:] = 1.0
+    page0 = s["table"][0, 0]
+    code = {BF16: lambda x: np.float32(x).view(np.uint32) >> 16, F16: lambda x: np.float16(x).view(np.uint16),
+            E4M3: lambda x: {12.0: 0x54, 16.0: 0x58, 20.0: 0x5a}[x]}[cache](lead)
+    held = sorted({int(x) for row, n in zip(s["table"], s["lens"]) for x in row[:-(-int(n) // 16)]})
+    keys[held] = 0
+    keys[page0, 0, :, 0] = code
+    values[page0, 0] = 0
+    on = Running(s, scale=1.0)
+    got = on.run()
+    on.close()
+    check_attn(s, got, want_attn(s, scale=1.0))
+
+
+def test_prefix_handle_serves_any_batch(backend):
+    """Other requests, groups and lengths on one handle; what the run before left does not show."""
+    h = None
+    for groups in ([(700, [1] * 40)], [(30, [2, 3])], [(200, [1, 2]), (5, [1, 1, 1])], [(700, [1] * 40)]):
+        s = make_groups(groups, 4, 2, 128, 16, "HND", BF16, BF16, 11)
+        on = Running(s, max_requests=64)
+        if h is None:
+            h = on.attn
+        else:
+            on.attn.close()
+            # the same description but for the table's width and the cache's pages: those of the widest case
+        on_attn, on.attn = on.attn, h
+        if on_attn is h:
+            first = s
+        if s["table"].shape[1] <= first["table"].shape[1]:
+            wide = np.full((len(s["lens"]), first["table"].shape[1]), 1 << 30, np.int32)
+            wide[:, :s["table"].shape[1]] = s["table"]
+            on.bufs[3].free()
+            on.bufs[3] = to_device(wide)
+        assert s["pages"] <= first["pages"]
+        check_attn(s, on.run(), want_attn(s))
+        for b in (*on.bufs, *on.extra, on.out, on.lse):
+            b.free()
+    h.close()
+    with pytest.raises(TensorClosed):
+        h.run(*([1] * 5), 1, 1, 1, 1, 1)
+
+
+def test_prefix_without_lse(backend):
+    s = make_groups([(100, [1, 2])], 4, 2, 64, 16, "HND", BF16, BF16, 3)
+    on = Running(s)
+    with_lse, without = on.run(), on.run(lse=False)
+    on.close()
+    bits_equal(with_lse[0], without[0])
+
+
+def test_prefix_two_handles_on_two_streams(backend):
+    cases = [make_groups([(900, [3] * 30)], 8, 2, 128, 16, "HND", BF16, BF16, i) for i in (1, 2)]
+    on, streams = [Running(s) for s in cases], [Stream(), Stream()]
+    for o in on:
+        o.out.memset(0)
+    sync_device()
+    for _ in range(10):
+        for o, st in zip(on, streams):
+            p = [b.ptr for b in o.bufs]
+            o.attn.run(*p[:5], 30, p[5], p[6], 1, o.out.ptr, o.lse.ptr, stream=st)
+    sync_device()
+    for o, s in zip(on, cases):
+        out = fetch(o.out, 30 * 8 * 128 * 2, np.uint16).reshape(30, 8, 128)
+        check_attn(s, (out, fetch(o.lse, 30 * 8 * 4, np.float32).reshape(30, 8)), want_attn(s))
+        o.close()
+    for st in streams:
+        st.close()
+
+
+def test_prefix_refusals(backend):
+    layout = paged.CacheLayout(4, 16, 2, 64, BF16)
+    for kwargs, error in (({"max_requests": 0}, ShapeInvalid), ({"max_requests": -1}, ShapeInvalid), ({"max_requests": 2 ** 31 - 1}, ShapeInvalid),
+                          ({"dtype": F32}, DTypeUnsupported), ({"dtype": F16}, DTypeMismatch), ({"q_heads": 3}, ShapeInvalid),
+                          ({"max_pages": 0}, ShapeInvalid), ({"window": -1}, InvalidArgument), ({"softcap": float("inf")}, InvalidArgument),
+                          ({"q_strides": (257, 65)}, LayoutUnsupported)):
+        with pytest.raises(error):
+            paged.PrefixAttention(**{**dict(cache=layout, q_heads=4, dtype=BF16, max_pages=4, max_requests=4), **kwargs})
+    h = paged.PrefixAttention(layout, 4, BF16, 4, 4)
+    b = [empty(1 << 16) for _ in range(9)]
+    p = [x.ptr for x in b]
+    good = [*p[:5], 4, p[5], p[6], 2, p[7], p[8]]
+
+    def refused(error, at, value):
+        args = list(good)
+        args[at] = value
+        with pytest.raises(error):
+            h.run(*args)
+
+    for at in (0, 1, 2, 3, 4, 6, 7, 9):
+        refused(InvalidArgument, at, 0)
+    for at, value in ((5, 5), (5, -1), (8, -1), (8, 2 ** 31 - 1)):
+        refused(ShapeInvalid, at, value)
+    for at, by in ((0, 2), (1, 8), (2, 8), (9, 4)):
+        refused(LayoutUnsupported, at, p[at if at < 5 else 7] + by)
+    h.run(*p[:5], 0, p[5], p[6], 2, p[7], p[8])  # nothing to do
+    h.close()
+    for x in b:
+        x.free()
