@@ -3,15 +3,20 @@
 // For row k (a beam) of a batch entry with logits x and score s, token t scores
 //   s + x[t] - L,  L = log sum_t exp x[t],
 // and the n largest over all beams and tokens are wanted.  Inside a row the
-// order of the scores is that of the logits, so a row is cut into chunks, and a
-// chunk gives its n largest logits and its part (maximum, sum of exponentials)
-// of L; the last CTA of a batch entry (a ticket) puts the Ls together and
-// merges the chunks' lists.  One launch, every logit read once.
+// order of the scores is that of the logits, so a row is cut into segments, and
+// a segment gives its n largest logits and its part (maximum, sum of
+// exponentials) of L; the last CTA of a batch entry (a ticket) puts the Ls
+// together and merges the segments' lists.  One launch, every logit read once.
 //
-// Bound: HBM, the logits.  A chunk stays in registers (32 logits a thread), so
-// the second look at it is free: the n-th largest of 32 maxima (of 8 threads
-// each) is a bound that n logits reach, only threads whose maximum reaches it
-// look at their logits again, and the few that do are ranked by counting.
+// Bound: HBM, the logits.  A CTA streams its segment once, each thread keeping
+// the maximum of what it met and a sum of exponentials relative to it, without a
+// barrier; the n-th largest of the maxima is a bound that n logits reach, and only
+// what the threads met whose maximum reaches it (n of 1024 parts) is read a second
+// time, out of L2.  The few logits that reach the bound are ranked by counting.
+// 64 x 8 rows of 128256 BF16 logits: 39.5 us (20 at the copy rate; the stream is
+// 20, the bound and the second look 6, the merge 4).  Collecting candidates on the
+// way took 76: the threads of a warp diverge at each, and the bound has to be
+// kept with barriers.  4 rows of 32000: 8.2 us, a chain of twelve dependent steps.
 #include <new>
 
 #include "mf_launch.cuh"
@@ -24,8 +29,10 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMostOut = 128;        // results of a batch entry
 constexpr int kMostBeams = 1024;     // beams of a batch entry
+constexpr int kParts = 4;            // of what a thread meets, with a maximum each
 constexpr int kGroups = 32;          // maxima that bound a list of up to kGroups
-constexpr int kPicked = 1024;        // logits of a chunk that may be ranked by counting
+constexpr int kPicked = 512;         // logits that may be ranked by counting
+constexpr int kCtas = 3;             // CTAs that a batch is cut into for every SM, at least (7: 45 us for the 39.5 below)
 constexpr float kLog2e = 1.44269504088896341f;
 
 struct SelectArgs {
@@ -34,11 +41,11 @@ struct SelectArgs {
     const int32_t* ended;
     int64_t row_stride;   // elements
     int32_t vocab, beams, n_out, end_token;
-    int32_t chunks;       // of a row
-    double* part_sum;     // [rows][chunks]
-    float* part_max;      // [rows][chunks]
-    int32_t* part_n;      // [rows][chunks]: entries of the list
-    float2* lists;        // [rows][chunks][n_out]: logit and token (as bits), the largest first
+    int32_t segments;     // of a row
+    int32_t chunks;       // of a segment
+    double* part_sum;     // [rows][segments]
+    float* part_max;      // [rows][segments]
+    float2* lists;        // [rows][segments][n_out]: logit and token (as bits), the largest first; -inf behind them
     int32_t* tickets;     // [batch], zero between runs
     float* scores_after;
     int32_t* tokens;
@@ -77,19 +84,19 @@ __device__ __forceinline__ void widen(const uint4& v, float* x) {
 
 // The vector of the logits from token t on, one by one; -inf behind the row.
 template <int DT>
-__device__ __noinline__ uint4 some_logits(const char* row, int32_t t, int32_t vocab) {
+__device__ __forceinline__ uint4 some_logits(const char* row, int32_t t, int32_t vocab) {
     uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = DT == MF_DT_F32 ? 0xff800000u : DT == MF_DT_BF16 ? 0xff80ff80u : 0xfc00fc00u;
     if constexpr (DT == MF_DT_F32) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (t + i < vocab) w[i] = reinterpret_cast<const uint32_t*>(row)[t + i];
+        for (int i = 0; i < 4; ++i) w[i] = t + i < vocab ? reinterpret_cast<const uint32_t*>(row)[t + i] : 0xff800000u;
     } else {
+        constexpr uint16_t kNone = DT == MF_DT_BF16 ? 0xff80 : 0xfc00;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (t + i < vocab)
-                w[i / 2] = __byte_perm(w[i / 2], reinterpret_cast<const uint16_t*>(row)[t + i], i & 1 ? 0x5410 : 0x3254);
+        for (int i = 0; i < 4; ++i) {
+            const uint16_t lo = t + 2 * i < vocab ? reinterpret_cast<const uint16_t*>(row)[t + 2 * i] : kNone;
+            const uint16_t hi = t + 2 * i + 1 < vocab ? reinterpret_cast<const uint16_t*>(row)[t + 2 * i + 1] : kNone;
+            w[i] = lo | static_cast<uint32_t>(hi) << 16;
+        }
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
@@ -118,7 +125,47 @@ struct Picked {
     T value[kPicked];
     int32_t index[kPicked];
     int32_t count;
+    // how many of the first n are in front of (v, i)
+    __device__ __forceinline__ int rank(T v, int32_t i, int n) const {
+        int in = 0;
+#pragma unroll 8
+        for (int o = 0; o < n; ++o) in += in_front(value[o], index[o], v, i);
+        return in;
+    }
 };
+template <class T>
+struct Best {
+    T value[kThreads / 32];
+    int32_t index[kThreads / 32];
+};
+// Two float32 at once.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+
+// The largest of a vector's logits; a NaN does not count.
+template <int DT>
+__device__ __forceinline__ float largest(const uint4& v) {
+    if constexpr (DT == MF_DT_F32) {
+        return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+    } else {
+        uint32_t m;
+        if constexpr (DT == MF_DT_BF16)
+            asm("{\n\t.reg .b32 a, b;\n\tmax.bf16x2 a, %1, %2;\n\tmax.bf16x2 b, %3, %4;\n\tmax.bf16x2 %0, a, b;\n\t}"
+                : "=r"(m) : "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w));
+        else
+            asm("{\n\t.reg .b32 a, b;\n\tmax.f16x2 a, %1, %2;\n\tmax.f16x2 b, %3, %4;\n\tmax.f16x2 %0, a, b;\n\t}"
+                : "=r"(m) : "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w));
+        float lo, hi;
+        if constexpr (DT == MF_DT_BF16) {
+            lo = __uint_as_float(m << 16);
+            hi = __uint_as_float(m & 0xffff0000u);
+        } else {
+            f16x2_to_f32x2(m, lo, hi);
+        }
+        return fmaxf(lo, hi);
+    }
+}
+
 struct SelectShared {
     float warp_max[kThreads / 32];
     double warp_sum[kThreads / 32];
@@ -127,10 +174,13 @@ struct SelectShared {
         struct {
             Bound<float> bound;
             Picked<float> picked;
+            Best<float> best;
+            int32_t part[kPicked];
         } chunk;
         struct {
             Bound<double> bound;
             Picked<double> picked;
+            Best<double> best;
         } entry;
     };
 };
@@ -169,7 +219,7 @@ __device__ __forceinline__ T bound_of(T mine, int n, Bound<T>& sh) {
 
 // The first of all threads' (value, index); all threads get it.
 template <class T>
-__device__ __forceinline__ void first_of_all(T& v, int32_t& i, Picked<T>& sh) {
+__device__ __forceinline__ void first_of_all(T& v, int32_t& i, Best<T>& sh) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
     for (int d = 16; d; d >>= 1) {
@@ -194,7 +244,7 @@ __device__ __forceinline__ void first_of_all(T& v, int32_t& i, Picked<T>& sh) {
     }
 }
 
-// What the chunks of batch entry `entry` left, put together by one CTA.
+// What the segments of batch entry `entry` left, put together by one CTA.
 __device__ void merge_lists(const SelectArgs& a, int32_t entry, SelectShared& sh, double* base) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int32_t row0 = entry * a.beams;
@@ -203,15 +253,18 @@ __device__ void merge_lists(const SelectArgs& a, int32_t entry, SelectShared& sh
         double b = static_cast<double>(a.scores[row]);
         if (a.ended == nullptr || a.ended[row] == 0) {
             float top = -INFINITY;
-            for (int32_t c = lane; c < a.chunks; c += 32) top = fmaxf(top, __ldcg(a.part_max + row * a.chunks + c));
-#pragma unroll
-            for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
             double sum = 0.0;
-            for (int32_t c = lane; c < a.chunks; c += 32) {
-                const float m = __ldcg(a.part_max + row * a.chunks + c);
-                const double s = __ldcg(a.part_sum + row * a.chunks + c);
-                // a chunk of -inf alone has a sum of zero; a NaN stays one
-                sum += m == -INFINITY ? s : s * exp(static_cast<double>(m) - static_cast<double>(top));
+            for (int32_t c0 = 0; c0 < a.segments; c0 += 32) {
+                const bool in = c0 + lane < a.segments;
+                const float m = in ? __ldcg(a.part_max + row * a.segments + c0 + lane) : -INFINITY;
+                const double s = in ? __ldcg(a.part_sum + row * a.segments + c0 + lane) : 0.0;
+                float most = fmaxf(m, top);
+#pragma unroll
+                for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+                // a part of -inf alone has a sum of zero; a NaN stays one
+                const double here = m == -INFINITY ? s : s * exp(static_cast<double>(m) - static_cast<double>(most));
+                sum = (top == -INFINITY ? sum : sum * exp(static_cast<double>(top) - static_cast<double>(most))) + here;
+                top = most;
             }
 #pragma unroll
             for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
@@ -221,23 +274,23 @@ __device__ void merge_lists(const SelectArgs& a, int32_t entry, SelectShared& sh
         if (lane == 0) base[k] = b > -INFINITY && b < INFINITY ? b : -INFINITY;
     }
     __syncthreads();
-    const int32_t n_lists = a.beams * a.chunks;
-    // entry e of list l; false behind the list's end
+    const int32_t n_lists = a.beams * a.segments;
+    // entry e of list l, -inf if there is none
     auto get = [&](int32_t l, int32_t e, double& v, int32_t& i) {
-        const int32_t k = l / a.chunks;
+        const int32_t k = l / a.segments;
         const double b = base[k];
-        if (b == -INFINITY) return false;
+        v = -INFINITY;
+        i = 0x7fffffff;
+        if (b == -INFINITY) return;
         if (a.ended != nullptr && a.ended[row0 + k] != 0) {
+            if (e > 0 || l != k * a.segments) return;
             v = b;
             i = k * a.vocab + a.end_token;
-            return e == 0 && l == k * a.chunks;
+            return;
         }
-        const int64_t list = static_cast<int64_t>(row0) * a.chunks + l;
-        if (e >= __ldcg(a.part_n + list)) return false;
-        const float2 x = __ldcg(a.lists + list * a.n_out + e);
+        const float2 x = __ldcg(a.lists + (static_cast<int64_t>(row0) * a.segments + l) * a.n_out + e);
         v = b + static_cast<double>(x.x);
-        i = k * a.vocab + __float_as_int(x.y);
-        return true;
+        if (x.x != -INFINITY) i = k * a.vocab + __float_as_int(x.y);
     };
     auto put = [&](int32_t j, double v, int32_t i) {
         const int64_t to = static_cast<int64_t>(entry) * a.n_out + j;
@@ -248,30 +301,39 @@ __device__ void merge_lists(const SelectArgs& a, int32_t entry, SelectShared& sh
         a.parents[to] = there ? row0 + k : -1;
         if (a.ended_after) a.ended_after[to] = there && token == a.end_token;
     };
+    // every thread's largest entry; entries that follow one another go to different groups of threads
+    const int32_t entries = n_lists * a.n_out, first = tid % (kThreads / kGroups) * kGroups + tid / (kThreads / kGroups);
     double mine = -INFINITY, v;
     int32_t i;
-    for (int32_t l = tid; l < n_lists; l += kThreads)
-        if (get(l, 0, v, i) && v > mine) mine = v;
+#pragma unroll 4
+    for (int32_t x = first; x < entries; x += kThreads) {
+        const int32_t l = x / a.n_out;
+        get(l, x - l * a.n_out, v, i);
+        mine = v > mine ? v : mine;
+    }
     const double bound = bound_of(mine, a.n_out, sh.entry.bound);
     auto& picked = sh.entry.picked;
     if (tid == 0) picked.count = 0;
     __syncthreads();
-    for (int32_t l = tid; l < n_lists; l += kThreads)
-        for (int32_t e = 0; e < a.n_out && get(l, e, v, i) && v >= bound; ++e) {
+#pragma unroll 4
+    for (int32_t x = tid; x < entries; x += kThreads) {
+        const int32_t l = x / a.n_out;
+        get(l, x - l * a.n_out, v, i);
+        if (v >= bound && v > -INFINITY) {
             const int at = atomicAdd(&picked.count, 1);
             if (at < kPicked) {
                 picked.value[at] = v;
                 picked.index[at] = i;
             }
         }
+    }
     __syncthreads();
     const int n = picked.count;
     if (n <= kPicked) {
         for (int x = tid; x < n; x += kThreads) {
             v = picked.value[x];
             i = picked.index[x];
-            int rank = 0;
-            for (int o = 0; o < n; ++o) rank += in_front(picked.value[o], picked.index[o], v, i);
+            const int rank = picked.rank(v, i, n);
             if (rank < a.n_out) put(rank, v, i);
         }
         for (int j = n + tid; j < a.n_out; j += kThreads) put(j, -INFINITY, -1);
@@ -284,84 +346,114 @@ __device__ void merge_lists(const SelectArgs& a, int32_t entry, SelectShared& sh
     for (int j = 0; j < a.n_out; ++j) {
         double best = -INFINITY;
         int32_t best_i = 0x7fffffff;
-        for (int32_t l = tid; l < n_lists; l += kThreads)
-            for (int32_t e = 0; e < a.n_out && get(l, e, v, i); ++e) {
-                if (!in_front(last_v, last_i, v, i)) continue;
-                if (in_front(v, i, best, best_i)) {
-                    best = v;
-                    best_i = i;
-                }
-                break;  // a list is in order
+        for (int32_t x = tid; x < entries; x += kThreads) {
+            const int32_t l = x / a.n_out;
+            get(l, x - l * a.n_out, v, i);
+            if (in_front(last_v, last_i, v, i) && in_front(v, i, best, best_i)) {
+                best = v;
+                best_i = i;
             }
-        first_of_all(best, best_i, picked);
+        }
+        first_of_all(best, best_i, sh.entry.best);
         if (tid == 0) put(j, best, best_i);
         last_v = best;
         last_i = best_i;
     }
 }
 
-// DT: dtype of the logits; V: 16-byte vectors of a thread.
+// The vector of the logits from token t on, wherever in memory the row begins: a thread's tokens do not depend on that, so
+// that equal rows have equal sums, to the bit.
+template <int DT>
+__device__ __forceinline__ uint4 load_vector(const char* row, int32_t t, int32_t vocab) {
+    constexpr int kPer = DT == MF_DT_F32 ? 4 : 8, kBytes = 16 / kPer;  // logits of a vector, bytes of one
+    const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row) & 15u);
+    const int32_t lead = off / kBytes;
+    if (t < lead || t + 2 * kPer > vocab) return some_logits<DT>(row, t, vocab);
+    const uint4* p = reinterpret_cast<const uint4*>(row - off) + t / kPer;
+    return off == 0 ? *p : shifted(p[0], p[1], off);
+}
+
+// A thread's vectors of the chunk from token `first` on.
 template <int DT, int V>
-__global__ void __launch_bounds__(kThreads) beam_select_kernel(const SelectArgs a) {
-    constexpr int kPer = DT == MF_DT_F32 ? 4 : 8;     // logits of a vector
+__device__ __forceinline__ void load_chunk(uint4 (&vec)[V], const char* row, int32_t first, int32_t vocab) {
+    constexpr int kPer = DT == MF_DT_F32 ? 4 : 8, kBytes = 16 / kPer;
+    const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row) & 15u);
+    const int32_t lead = off / kBytes, mine = first + static_cast<int>(threadIdx.x) * kPer;
+    if (first < lead || first + kThreads * V * kPer + kPer > vocab) {  // the row's beginning, where it is not aligned, and its end
+#pragma unroll
+        for (int v = 0; v < V; ++v) vec[v] = load_vector<DT>(row, mine + v * (kThreads * kPer), vocab);
+    } else {
+        const uint4* p = reinterpret_cast<const uint4*>(row - off) + mine / kPer;
+        if (off == 0) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) vec[v] = p[v * kThreads];
+        } else {
+#pragma unroll
+            for (int v = 0; v < V; ++v) vec[v] = shifted(p[v * kThreads], p[v * kThreads + 1], off);
+        }
+    }
+}
+
+// DT: dtype of the logits; V: 16-byte vectors of a thread and chunk.
+template <int DT, int V>
+__global__ void __launch_bounds__(kThreads, 4) beam_select_kernel(const SelectArgs a) {
+    constexpr int kPer = DT == MF_DT_F32 ? 4 : 8;
     constexpr int kBytes = 16 / kPer;
     constexpr int kChunk = kThreads * V * kPer;
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ SelectShared sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int64_t row = blockIdx.x / a.chunks;
-    const int32_t chunk = blockIdx.x - row * a.chunks;
+    const int64_t row = blockIdx.x / a.segments;
+    const int32_t segment = blockIdx.x - row * a.segments;
     const int32_t entry = row / a.beams;
-    const int64_t list = row * a.chunks + chunk;
+    const int64_t list = row * a.segments + segment;
     after_previous();
     let_next_start();
     if (a.ended == nullptr || a.ended[row] == 0) {
-        // A thread's tokens do not depend on where the row begins in memory: equal rows have equal sums, to the bit.
         const char* begin = a.logits + row * a.row_stride * kBytes;
-        const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(begin) & 15u);
-        const int32_t lead = off / kBytes, first = chunk * kChunk;
-        uint4 vec[V];
-        if (off == 0) {
+        const int32_t first0 = segment * a.chunks * kChunk;
+        const int32_t chunks = min(a.chunks, (a.vocab - first0 + kChunk - 1) / kChunk);
+        uint4 vec[V], ahead[V];
+        load_chunk<DT, V>(ahead, begin, first0, a.vocab);
+        // sums relative to the thread's own maximum: differences of near logits are exact
+        float most = -INFINITY, sum = 0.0f, of_part[kParts];
+        const int32_t each = (chunks + kParts - 1) / kParts;  // chunks of a part
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const int32_t t = first + (v * kThreads + tid) * kPer;
-                vec[v] = t + kPer <= a.vocab ? __ldcs(reinterpret_cast<const uint4*>(begin) + t / kPer) : some_logits<DT>(begin, t, a.vocab);
-            }
-        } else {
+        for (int part = 0; part < kParts; ++part) {
+            of_part[part] = -INFINITY;
+#pragma unroll 1
+            for (int32_t c = part * each; c < min(chunks, (part + 1) * each); ++c) {
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const int32_t t = first + (v * kThreads + tid) * kPer;
-                if (t >= lead && t - lead + 2 * kPer <= a.vocab) {
-                    const uint4* p = reinterpret_cast<const uint4*>(begin + static_cast<int64_t>(t - lead) * kBytes);
-                    vec[v] = shifted(p[0], p[1], off);
-                } else {
-                    vec[v] = some_logits<DT>(begin, t, a.vocab);
+                for (int v = 0; v < V; ++v) vec[v] = ahead[v];
+                if (c + 1 < chunks) load_chunk<DT, V>(ahead, begin, first0 + (c + 1) * kChunk, a.vocab);
+                float top = -INFINITY;
+#pragma unroll
+                for (int v = 0; v < V; ++v) top = fmaxf(top, largest<DT>(vec[v]));
+                of_part[part] = fmaxf(of_part[part], top);
+                if (top > most) {
+                    sum *= exp2_fast((most - top) * kLog2e);  // the first time it is 0 times 0
+                    most = top;
                 }
+                const float less = most == -INFINITY ? 0.0f : most;
+                float2 two = make_float2(0.0f, 0.0f);
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    float x[kPer];
+                    widen<DT>(vec[v], x);
+#pragma unroll
+                    for (int i = 0; i < kPer; i += 2) {
+                        const float2 e = mul2(add2(make_float2(x[i], x[i + 1]), make_float2(-less, -less)), make_float2(kLog2e, kLog2e));
+                        two = add2(two, make_float2(exp2_fast(e.x), exp2_fast(e.y)));
+                    }
+                }
+                sum += two.x + two.y;
             }
         }
-        float top = -INFINITY;
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            float x[kPer];
-            widen<DT>(vec[v], x);
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) top = fmaxf(top, x[i]);
-        }
-        // the sum relative to the thread's own maximum: differences of near logits are exact
-        const float less = top == -INFINITY ? 0.0f : top;
-        float sum = 0.0f;
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            float x[kPer];
-            widen<DT>(vec[v], x);
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) sum += exp2_fast((x[i] - less) * kLog2e);
-        }
-        // sums of a warp and of the chunk in float64
-        float all = top;
+        // sums of a warp and of the segment in float64
+        float all = most;
 #pragma unroll
         for (int d = 16; d; d >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, d));
-        double of_warp = top == -INFINITY ? sum : static_cast<double>(sum * exp2_fast((top - all) * kLog2e));
+        double of_warp = most == -INFINITY ? sum : static_cast<double>(sum * exp2_fast((most - all) * kLog2e));
 #pragma unroll
         for (int d = 16; d; d >>= 1) of_warp += __shfl_xor_sync(0xffffffffu, of_warp, d);
         if (lane == 0) {
@@ -370,85 +462,103 @@ __global__ void __launch_bounds__(kThreads) beam_select_kernel(const SelectArgs 
         }
         auto& picked = sh.chunk.picked;
         if (tid == 0) picked.count = 0;
-        const float bound = bound_of(top, a.n_out, sh.chunk.bound);
+        // the threads' parts with the n_out largest maxima, and the least of those; more parts where maxima are equal
+        float bound = bound_of(most, a.n_out, sh.chunk.bound);
         if (warp == 0) {
             const float m = lane < kThreads / 32 ? sh.warp_max[lane] : -INFINITY;
             double s = lane < kThreads / 32 ? sh.warp_sum[lane] : 0.0;
-            float most = m;
+            float top = m;
 #pragma unroll
-            for (int d = 4; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-            if (m != -INFINITY) s *= static_cast<double>(exp2_fast((m - most) * kLog2e));
+            for (int d = 4; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            if (m != -INFINITY) s *= static_cast<double>(exp2_fast((m - top) * kLog2e));
 #pragma unroll
             for (int d = 4; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
             if (lane == 0) {
-                a.part_max[list] = most;
+                a.part_max[list] = top;
                 a.part_sum[list] = s;
             }
         }
-        if (top >= bound && top > -INFINITY) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                float x[kPer];
-                widen<DT>(vec[v], x);
-#pragma unroll
-                for (int i = 0; i < kPer; ++i) {
-                    if (x[i] >= bound && x[i] > -INFINITY) {
-                        const int at = atomicAdd(&picked.count, 1);
-                        if (at < kPicked) {
-                            picked.value[at] = x[i];
-                            picked.index[at] = first + (v * kThreads + tid) * kPer + i;
-                        }
-                    }
-                }
+        auto keep = [&](float x, int32_t i) {
+            const int at = atomicAdd(&picked.count, 1);
+            if (at < kPicked) {
+                picked.value[at] = x;
+                picked.index[at] = i;
             }
-        }
+        };
+#pragma unroll
+        for (int part = 0; part < kParts; ++part)
+            if (of_part[part] >= bound && of_part[part] > -INFINITY) keep(of_part[part], part * kThreads + tid);
         __syncthreads();
-        const int n_picked = picked.count;
-        float2* to = a.lists + list * a.n_out;
-        if (n_picked <= kPicked) {
-            for (int x = tid; x < n_picked; x += kThreads) {
+        const int parts = picked.count;
+        if (parts <= kPicked) {
+            for (int x = tid; x < parts; x += kThreads) {
                 const float v = picked.value[x];
                 const int32_t i = picked.index[x];
-                int rank = 0;
-                for (int o = 0; o < n_picked; ++o) rank += in_front(picked.value[o], picked.index[o], v, i);
+                if (picked.rank(v, i, parts) == a.n_out - 1) sh.chunk.bound.value = v;
+                sh.chunk.part[x] = i;
+            }
+            __syncthreads();
+            if (parts >= a.n_out) bound = sh.chunk.bound.value;
+            if (tid == 0) picked.count = 0;
+            __syncthreads();
+            // their logits again
+            const int32_t vectors = each * V;
+#pragma unroll 2
+            for (int32_t x = tid; x < parts * vectors; x += kThreads) {
+                const int32_t j = x / parts, part = sh.chunk.part[x - j * parts];
+                if (part / kThreads * each * V + j >= chunks * V) continue;
+                const int32_t t = first0 + ((part / kThreads * vectors + j) * kThreads + part % kThreads) * kPer;
+                const uint4 again = load_vector<DT>(begin, t, a.vocab);
+                const float top = largest<DT>(again);
+                if (!(top >= bound && top > -INFINITY)) continue;
+                float v[kPer];
+                widen<DT>(again, v);
+#pragma unroll
+                for (int i = 0; i < kPer; ++i)
+                    if (v[i] >= bound && v[i] > -INFINITY) keep(v[i], t + i);
+            }
+            __syncthreads();
+        }
+        const int n = picked.count;
+        float2* to = a.lists + list * a.n_out;
+        if (n <= kPicked) {
+            for (int x = tid; x < n; x += kThreads) {
+                const float v = picked.value[x];
+                const int32_t i = picked.index[x];
+                const int rank = picked.rank(v, i, n);
                 if (rank < a.n_out) to[rank] = make_float2(v, __int_as_float(i));
             }
-            if (tid == 0) a.part_n[list] = min(n_picked, a.n_out);
+            for (int j = n + tid; j < a.n_out; j += kThreads) to[j] = make_float2(-INFINITY, 0.0f);
         } else {
-            // a chunk of mostly equal logits: one after the other, each the first behind the one before
+            // mostly equal logits: one after the other, each the first behind the one before
             float last_v = INFINITY;
             int32_t last_i = -1;
-            int n = 0;
 #pragma unroll 1
-            for (; n < a.n_out; ++n) {
+            for (int j = 0; j < a.n_out; ++j) {
                 float best = -INFINITY;
                 int32_t best_i = 0x7fffffff;
+                for (int32_t x = 0; x < chunks * V; ++x) {
+                    const int32_t t = first0 + (x * kThreads + tid) * kPer;
+                    float v[kPer];
+                    widen<DT>(load_vector<DT>(begin, t, a.vocab), v);
 #pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    float x[kPer];
-                    widen<DT>(vec[v], x);
-#pragma unroll
-                    for (int i = 0; i < kPer; ++i) {
-                        const int32_t t = first + (v * kThreads + tid) * kPer + i;
-                        if (in_front(last_v, last_i, x[i], t) && in_front(x[i], t, best, best_i)) {
-                            best = x[i];
-                            best_i = t;
+                    for (int i = 0; i < kPer; ++i)
+                        if (in_front(last_v, last_i, v[i], t + i) && in_front(v[i], t + i, best, best_i)) {
+                            best = v[i];
+                            best_i = t + i;
                         }
-                    }
                 }
-                first_of_all(best, best_i, picked);
-                if (best == -INFINITY) break;
+                first_of_all(best, best_i, sh.chunk.best);
                 last_v = best;
                 last_i = best_i;
-                if (tid == 0) to[n] = make_float2(best, __int_as_float(best_i));
+                if (tid == 0) to[j] = make_float2(best, __int_as_float(best_i));
             }
-            if (tid == 0) a.part_n[list] = n;
         }
         __syncthreads();
     }
     if (tid == 0) {
         int32_t old;
-        const int32_t parts = a.beams * a.chunks;
+        const int32_t parts = a.beams * a.segments;
         asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(old) : "l"(a.tickets + entry) : "memory");
         sh.last = old == parts - 1;
         if (sh.last) a.tickets[entry] = 0;
@@ -465,17 +575,33 @@ template <int DT>
 SelectKernel select_kernel(bool small) {
     constexpr int per = DT == MF_DT_F32 ? 4 : 8;
     if (small) return {beam_select_kernel<DT, 8 / per>, kThreads * 8};
-    return {beam_select_kernel<DT, 32 / per>, kThreads * 32};
+    return {beam_select_kernel<DT, 4>, kThreads * 4 * per};
 }
 SelectKernel pick(int dtype, bool small) {
     return dtype == MF_DT_F32 ? select_kernel<MF_DT_F32>(small) : dtype == MF_DT_BF16 ? select_kernel<MF_DT_BF16>(small)
                                                                                      : select_kernel<MF_DT_F16>(small);
 }
 
-int64_t chunks_of(int64_t vocab, int chunk) { return (vocab + chunk - 1) / chunk; }
-
-// Up to how many rows take small chunks: where large ones would not give every SM two.
-int64_t small_rows(int64_t large_chunks, int sms) { return 2 * sms / large_chunks; }
+// How a batch of `rows` rows is cut: the kernel, and the chunks of a segment.
+struct Cuts {
+    SelectKernel kernel;
+    int32_t chunks, segments;
+};
+Cuts cuts_of(int64_t rows, int32_t vocab, int dtype, int sms) {
+    // Small chunks where large ones would not give every SM two; else segments of as many as leave every SM kCtas.
+    Cuts c{pick(dtype, false), 1, 1};
+    int64_t chunks = (vocab + c.kernel.chunk - 1) / c.kernel.chunk;
+    if (rows * chunks <= 2 * sms) {
+        c.kernel = pick(dtype, true);
+        chunks = (vocab + c.kernel.chunk - 1) / c.kernel.chunk;
+    } else {
+        const int64_t want = (kCtas * sms + rows - 1) / rows;  // segments of a row
+        c.chunks = static_cast<int32_t>(want >= chunks ? 1 : (chunks + want - 1) / want);
+    }
+    c.segments = static_cast<int32_t>((chunks + c.chunks - 1) / c.chunks);
+    c.chunks = static_cast<int32_t>((chunks + c.segments - 1) / c.segments);
+    return c;
+}
 
 }  // namespace
 }  // namespace mf
@@ -487,6 +613,7 @@ struct mf_beam_select_s {
     SelectArgs args;
     void* workspace;
     int device, sm_count;
+    int64_t lists;  // that the workspace has room for
 };
 
 extern "C" int mf_beam_select_create(const mf_beam_select_config* config, mf_beam_select* handle) {
@@ -508,16 +635,15 @@ extern "C" int mf_beam_select_create(const mf_beam_select_config* config, mf_bea
                     (long long)c.row_stride, c.vocab);
     if (c.end_token < -1 || c.end_token >= c.vocab)
         return fail(MF_ERR_INVALID_ARGUMENT, "mf_beam_select_create: end token %d of %d", c.end_token, c.vocab);
-    // the workspace holds what the chunks of any batch leave; small chunks are for batches that leave SMs idle
+    // The workspace holds what the segments of any batch leave.  More rows mean fewer segments of each, and no more than
+    // `most` in all until a row is one.
     const int sms = state().sm_count;
-    const int64_t rows = static_cast<int64_t>(c.max_batch) * c.beams;
-    const int64_t large = chunks_of(c.vocab, kThreads * 32), small = chunks_of(c.vocab, kThreads * 8);
-    const int64_t few = rows < small_rows(large, sms) ? rows : small_rows(large, sms);
-    const int64_t lists = rows * large > few * small ? rows * large : few * small;
-    if (lists > 0x7fffffffll)
-        return fail(MF_ERR_SHAPE_INVALID, "mf_beam_select_create: a batch of %d x %d x %d logits", c.max_batch, c.beams, c.vocab);
+    const int64_t rows = static_cast<int64_t>(c.max_batch) * c.beams, least = c.beams;
+    const int64_t large = (c.vocab + kThreads * 16 - 1) / (kThreads * 16);
+    const int64_t most = 64ll * sms + 4 * least * large;
+    const int64_t lists = rows > most ? rows : most < 4 * rows * large ? most : 4 * rows * large;
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-    const size_t at_max = up(static_cast<size_t>(c.max_batch) * 4), at_n = at_max + up(lists * 4), at_sum = at_n + up(lists * 4);
+    const size_t at_max = up(static_cast<size_t>(c.max_batch) * 4), at_sum = at_max + up(lists * 4);
     const size_t at_lists = at_sum + up(lists * 8), bytes = at_lists + static_cast<size_t>(lists) * c.n_out * 8;
     mf_beam_select_s* h = new (std::nothrow) mf_beam_select_s{};
     if (!h) return fail(MF_ERR_ALLOCATOR_EXHAUSTED, "mf_beam_select_create: out of host memory");
@@ -540,6 +666,7 @@ extern "C" int mf_beam_select_create(const mf_beam_select_config* config, mf_bea
     h->config = c;
     h->device = state().device;
     h->sm_count = sms;
+    h->lists = lists;
     SelectArgs& a = h->args;
     a.row_stride = c.row_stride;
     a.vocab = c.vocab;
@@ -548,7 +675,6 @@ extern "C" int mf_beam_select_create(const mf_beam_select_config* config, mf_bea
     a.end_token = c.end_token;
     a.tickets = reinterpret_cast<int32_t*>(w);
     a.part_max = reinterpret_cast<float*>(w + at_max);
-    a.part_n = reinterpret_cast<int32_t*>(w + at_n);
     a.part_sum = reinterpret_cast<double*>(w + at_sum);
     a.lists = reinterpret_cast<float2*>(w + at_lists);
     *handle = h;
@@ -575,18 +701,19 @@ extern "C" int mf_beam_select_run(mf_beam_select handle, const void* logits, con
     if (scores_after == scores || (ended && ended_after == ended))
         return fail(MF_ERR_INVALID_ARGUMENT, "mf_beam_select_run: outputs may not be the inputs (scores_after, ended_after)");
     const int64_t rows = static_cast<int64_t>(batch) * c.beams;
-    const bool small = rows <= small_rows(chunks_of(c.vocab, kThreads * 32), handle->sm_count);
-    const SelectKernel kernel = pick(c.dtype, small);
+    const Cuts cuts = cuts_of(rows, c.vocab, c.dtype, handle->sm_count);
+    if (rows * cuts.segments > handle->lists) return fail(MF_ERR_ALLOCATOR_EXHAUSTED, "mf_beam_select_run: workspace of %lld lists", (long long)handle->lists);
     SelectArgs a = handle->args;
     a.logits = static_cast<const char*>(logits);
     a.scores = scores;
     a.ended = ended;
-    a.chunks = static_cast<int32_t>(chunks_of(c.vocab, kernel.chunk));
+    a.segments = cuts.segments;
+    a.chunks = cuts.chunks;
     a.scores_after = scores_after;
     a.tokens = tokens;
     a.parents = parents;
     a.ended_after = ended_after;
-    const cudaError_t err = launch_overlapped(kernel.fn, dim3(static_cast<unsigned>(rows * a.chunks)), kThreads, c.beams * 8,
+    const cudaError_t err = launch_overlapped(cuts.kernel.fn, dim3(static_cast<unsigned>(rows * a.segments)), kThreads, c.beams * 8,
                                               static_cast<cudaStream_t>(stream), a);
     if (err != cudaSuccess) return cuda_fail(err, "mf_beam_select_run");
     return MF_OK;
