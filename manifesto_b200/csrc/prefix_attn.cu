@@ -51,7 +51,8 @@ struct PrefixArgs {
     int32_t max_pages, page, window, kv_heads;
     const char* k;
     const char* v;
-    int64_t page_bytes, row_bytes, head_bytes, table_stride;
+    int64_t head_bytes, table_stride;
+    uint32_t page_units, row_units, unit;  // a page, a row of it in units of 2^unit bytes
     uint32_t n_pages;
     Divisor by_page;
     Divisor group;        // query heads of a key-value head
@@ -120,6 +121,17 @@ __device__ __forceinline__ void tm_store(uint32_t at, const uint32_t (&r)[32]) {
         MF_I8(r, 0), MF_I8(r, 8), MF_I8(r, 16), MF_I8(r, 24)
         : "memory");
 }
+__device__ __forceinline__ void tm_load16(uint32_t (&r)[16], uint32_t at) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : MF_R8(r, 0), MF_R8(r, 8)
+                 : "r"(at)
+                 : "memory");
+}
+__device__ __forceinline__ void tm_store16(uint32_t at, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at), MF_I8(r, 0),
+                 MF_I8(r, 8)
+                 : "memory");
+}
 // A shared-memory operand in the 128-byte swizzle: where it begins, and the bytes between groups of 8 rows (`stride`) and, of an
 // operand whose rows run along the product's sum, between panels of 64 columns (`lead`).
 __device__ __forceinline__ uint64_t operand(uint32_t at, uint32_t lead, uint32_t stride) {
@@ -132,8 +144,20 @@ __device__ __forceinline__ uint32_t product(bool bf16, int n, bool b_rows) {
     return 1u << 4 | t << 7 | t << 10 | (b_rows ? 1u << 16 : 0u) | static_cast<uint32_t>(n >> 3) << 17 | (128u >> 4) << 24;
 }
 
-constexpr int kProducers = 128;
-constexpr int kMasks = 8;  // tiles whose masks are kept: more than the ring holds
+// Four groups of four warps: softmax, softmax, producers, and single ones (the products' issuer, the pages', the notes').  The
+// registers of the launch (128 each) go where a row of scores is held: 128 x (176 + 176 + 96 + 64) = 512 x 128.
+constexpr int kThreads = 512;
+constexpr int kProducers = 128, kFirstProducer = 256, kIssuer = 12, kPager = 13, kNoter = 14;
+constexpr int kSoftmaxRegs = 176, kProducerRegs = 96, kOtherRegs = 64;
+constexpr int kPlaces = 4;  // tiles whose rows are known in advance
+constexpr int kMasks = 16;  // tiles whose masks are kept: more than the ring and the places hold
+
+// Shared tokens of a group, and its requests; nothing is shared by a request alone.
+struct Group {
+    int32_t start, members, shared;
+    bool bad;
+};
+constexpr uint32_t kMasked = 0xffffffffu;
 
 // MODE: dtype of the cache; DP: head_dim padded to 64, 128 or 256.
 template <int MODE, int DP>
@@ -150,28 +174,25 @@ struct Prefix {
     static constexpr int kPanels = DP / 64;              // of 64 elements (128 bytes) of a row
     static constexpr int kUnit = T * DP * 2;             // bytes of a tile's keys, or values
     static constexpr int kQ = 128 * DP * 2;              // of 128 rows of queries
-    static constexpr int kStages = DP == 64 ? 10 : 5;    // units of the ring
+    static constexpr int kStages = (DP == 64 ? 2 : 1) * (kFp8 ? 3 : 5);  // units of the ring
+    static constexpr int kRaw = kFp8 ? 4 : 0;            // units of FP8 codes on their way
+    static constexpr int kRing = kStages * kUnit + kRaw * (kUnit / 2);
     static constexpr int kRows = 128 * kStreams;         // of a block
-    static constexpr int kSoftmax = 128 * kStreams;      // threads
-    static constexpr int kThreads = kSoftmax + kProducers + 32;
     static constexpr int kO = 2 * T;                     // columns of tensor memory: S of even and odd steps, then O
     struct Shared {
         uint64_t full[kStages], empty[kStages];
         uint64_t s_full[2], p_full[2], o_done[2], q_full[2], drained;
+        uint64_t rows_known[kPlaces], rows_used[kPlaces];
         uint32_t tmem;
         int32_t abandoned;
-        int32_t group, into;        // where this CTA's run begins
+        Group of;                   // where this CTA's run begins
+        int32_t group, into;
         uint32_t mask[kMasks][4];   // tokens of a tile that are there
-        int64_t row[2][T];          // where a tile's rows are, from the head's begin; -1: masked
+        uint32_t row[kPlaces][T];   // where a tile's rows are, from the head's begin, in units of 2^unit bytes; kMasked: nowhere
     };
-    static constexpr int kBytes = kStages * kUnit + kStreams * kQ + static_cast<int>(sizeof(Shared));
+    static constexpr int kBytes = kRing + kStreams * kQ + static_cast<int>(sizeof(Shared));
 };
 
-// Shared tokens of a group, and its requests; nothing is shared by a request alone.
-struct Group {
-    int32_t start, members, shared;
-    bool bad;
-};
 __device__ __forceinline__ Group group_of(const PrefixArgs& a, int32_t g) {
     Group x;
     const int32_t s = a.starts[g], e = a.starts[g + 1];
@@ -179,7 +200,8 @@ __device__ __forceinline__ Group group_of(const PrefixArgs& a, int32_t g) {
     x.start = s;
     x.members = x.bad ? 0 : e - s;
     const int64_t reach = static_cast<int64_t>(a.max_pages) * a.page;
-    x.shared = x.members < 2 ? 0 : max(a.shared[g], 0);
+    const int32_t shared = max(a.shared[g], 0);
+    x.shared = x.members < 2 ? 0 : shared;
     if (x.shared > reach) x.shared = static_cast<int32_t>(reach);
     return x;
 }
@@ -199,8 +221,8 @@ struct Run {
     int32_t g, tiles, items, item, t, left;
     // of the item at hand
     int32_t n, kv, block, rows;  // tiles of the run in it; its key-value head, block of rows, rows
-    __device__ __forceinline__ Run(const PrefixArgs& a, int32_t group, int32_t into, int32_t run) : g(group), left(run) {
-        of = group_of(a, g);
+    __device__ __forceinline__ Run(const PrefixArgs& a, const Group& first, int32_t group, int32_t into, int32_t run)
+        : of(first), g(group), left(run) {
         tiles = tiles_of<K>(of);
         items = static_cast<int32_t>(items_of<K>(a, of));
         item = into / tiles;
@@ -217,6 +239,8 @@ struct Run {
     }
     // whether each softmax group has rows of its own; else they share the rows and take turns at the tiles
     __device__ __forceinline__ bool dual() const { return K::kStreams == 2 && rows > 128; }
+    // among how many warps a row's tokens of a tile are shared out, where there are no rows for four
+    __device__ __forceinline__ int32_t sharers() const { return rows <= 32 && K::T == 128 ? 4 : rows <= 64 ? 2 : 1; }
     __device__ __forceinline__ int32_t steps() const { return dual() ? 2 * n : n; }
     __device__ __forceinline__ bool next(const PrefixArgs& a) {
         left -= n;
@@ -263,9 +287,45 @@ __device__ __forceinline__ uint32_t place(int rows, int row, int c) {
 
 // ------------------------------------------------------------------ roles
 
+// One warp finds the rows of the tiles to come in the page table.
+template <class K>
+__device__ __forceinline__ void find_rows(const PrefixArgs& a, typename K::Shared& sh, Run<K> run) {
+    const int lane = threadIdx.x & 31;
+    uint32_t tile = 0;
+    bool more = true;
+    while (more) {
+        const int64_t at_row = static_cast<int64_t>(run.of.start) * a.table_stride;
+        for (int32_t i = 0; i < run.n; ++i, ++tile) {
+            uint32_t off[K::T / 32];
+            int32_t number[K::T / 32];
+#pragma unroll
+            for (int w = 0; w < K::T / 32; ++w) {
+                const uint32_t tok = static_cast<uint32_t>(run.t + i) * K::T + w * 32 + lane, idx = tok / a.by_page;
+                const bool in = tok < static_cast<uint32_t>(run.of.shared);
+                off[w] = in ? (tok - idx * a.page) * a.row_units : kMasked;
+                number[w] = in ? a.table[at_row + idx] : 0;
+            }
+            const uint32_t at = tile % kPlaces;
+            wait(&sh.abandoned, &sh.rows_used[at], (tile / kPlaces & 1u) ^ 1u);
+            __syncwarp();
+#pragma unroll
+            for (int w = 0; w < K::T / 32; ++w) {
+                const bool in = off[w] != kMasked, ok = in && static_cast<uint32_t>(number[w]) < a.n_pages;
+                if (in && !ok) atomicExch(a.status, MF_DEVICE_BAD_PAGE);
+                sh.row[at][w * 32 + lane] = ok ? static_cast<uint32_t>(number[w]) * a.page_units + off[w] : kMasked;
+                const uint32_t word = __ballot_sync(0xffffffffu, ok);
+                if (lane == 0) sh.mask[tile % kMasks][w] = word;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.rows_known[at]);
+        }
+        more = run.next(a);
+    }
+}
+
 template <class K, int MODE>
 __device__ __forceinline__ void produce(const PrefixArgs& a, typename K::Shared& sh, uint32_t ring, Run<K> run) {
-    const int tid = threadIdx.x - K::kSoftmax, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x - kFirstProducer, lane = tid & 31;
     constexpr int kBytesOf = K::kFp8 ? 1 : 2;
     const int pieces = (a.head_dim * kBytesOf + 15) / 16;  // 16-byte pieces of a row in memory
     constexpr int kMostPieces = K::kPanels * 8 / (K::kFp8 ? 2 : 1);
@@ -273,108 +333,103 @@ __device__ __forceinline__ void produce(const PrefixArgs& a, typename K::Shared&
     constexpr int kStep = kProducers / kMostPieces, kCopies = K::T / kStep;
     const bool mine = piece < pieces;
     const int64_t kv_gap = a.v - a.k;
-    uint32_t unit = 0, told = 0;  // units begun, units of which the consumer knows
-    int32_t tile = 0;             // tiles so far
-    auto tell = [&]() {           // this warp's part of unit `told` is there
+    uint32_t unit = 0, told = 0, tile = 0;  // units begun, units that the consumer has, tiles so far
+    // Unit `told` is there: tell the consumer.  FP8: convert it first; every thread converts the pieces that it copied itself.
+    auto tell = [&]() {
+        if constexpr (K::kFp8) {
+            const uint32_t stage = told % K::kStages, to = ring + stage * K::kUnit;
+            const uint32_t from = ring + K::kStages * K::kUnit + told % K::kRaw * (K::kUnit / 2) + tid * 16;
+            wait(&sh.abandoned, &sh.empty[stage], (told / K::kStages & 1u) ^ 1u);
+            __syncwarp();
+            if (mine) {
+#pragma unroll
+                for (int x = 0; x < kCopies; ++x) {
+                    const int r = row0 + x * kStep;
+                    uint4 code, lo, hi;
+                    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                                 : "=r"(code.x), "=r"(code.y), "=r"(code.z), "=r"(code.w) : "r"(from + x * (kProducers * 16)) : "memory");
+                    fp8x4_to_f16<MODE>(code.x, lo.x, lo.y);
+                    fp8x4_to_f16<MODE>(code.y, lo.z, lo.w);
+                    fp8x4_to_f16<MODE>(code.z, hi.x, hi.y);
+                    fp8x4_to_f16<MODE>(code.w, hi.z, hi.w);
+                    const uint32_t at0 = to + place(K::T, r, 2 * piece), at1 = to + place(K::T, r, 2 * piece + 1);
+                    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at0), "r"(lo.x), "r"(lo.y), "r"(lo.z), "r"(lo.w) : "memory");
+                    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at1), "r"(hi.x), "r"(hi.y), "r"(hi.z), "r"(hi.w) : "memory");
+                }
+            }
+        }
         fence_proxy();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.full[told % K::kStages]);
         ++told;
     };
+    constexpr uint32_t kAhead = K::kFp8 ? K::kRaw - 1 : K::kStages - 2;  // units on their way
     bool more = true;
     while (more) {
-        const int64_t at_row = static_cast<int64_t>(run.of.start) * a.table_stride;
-        const char* head = a.k + run.kv * a.head_bytes;
-        int32_t number = 0;
-        auto look_up = [&](int32_t t) {
-            const uint32_t tok = static_cast<uint32_t>(t) * K::T + tid;
-            if (tid < K::T && tok < static_cast<uint32_t>(run.of.shared)) number = a.table[at_row + tok / a.by_page];
-        };
-        look_up(run.t);
+        const char* keys = a.k + run.kv * a.head_bytes + piece * 16;
         for (int32_t i = 0; i < run.n; ++i, ++tile) {
-            const int buf = tile & 1;
-            if (tid < K::T) {
-                const uint32_t tok = static_cast<uint32_t>(run.t + i) * K::T + tid;
-                const bool in = tok < static_cast<uint32_t>(run.of.shared), ok = in && static_cast<uint32_t>(number) < a.n_pages;
-                if (in && !ok) atomicExch(a.status, MF_DEVICE_BAD_PAGE);
-                sh.row[buf][tid] = ok ? static_cast<int64_t>(number) * a.page_bytes + (tok - tok / a.by_page * a.page) * a.row_bytes : -1;
-                const uint32_t word = __ballot_sync(0xffffffffu, ok);
-                if (lane == 0) sh.mask[tile % kMasks][warp] = word;
-            }
-            asm volatile("bar.sync 1, %0;" ::"n"(kProducers) : "memory");
-            if (i + 1 < run.n) look_up(run.t + i + 1);
+            wait(&sh.abandoned, &sh.rows_known[tile % kPlaces], tile / kPlaces & 1u);
+            __syncwarp();
+            const uint32_t* rows = sh.row[tile % kPlaces];
 #pragma unroll 1
             for (int of = 0; of < 2; ++of) {
                 const uint32_t stage = unit % K::kStages, parity = (unit / K::kStages & 1u) ^ 1u;
-                const uint32_t to = ring + stage * K::kUnit;
-                const char* base = head + (of ? kv_gap : 0) + piece * 16;
-                if constexpr (!K::kFp8) {
-                    if (!__all_sync(0xffffffffu, mbar_try_wait(&sh.empty[stage], parity))) {
-                        // no room: what is on the way may be what the consumer waits for
-                        cp_async_wait<0>();
-                        while (told < unit) tell();
-                        wait(&sh.abandoned, &sh.empty[stage], parity);
-                        __syncwarp();
-                    }
-                    if (mine) {
-#pragma unroll 4
-                        for (int x = 0; x < kCopies; ++x) {
-                            const int r = row0 + x * kStep;
-                            const int64_t off = sh.row[buf][r];
-                            cp_async16(to + place(K::T, r, piece), off >= 0 ? base + off : a.k, off >= 0 ? 16u : 0u);
-                        }
-                    }
-                    cp_async_commit();
-                    ++unit;
-                    if (unit - told > K::kStages - 2) {
-                        cp_async_wait<K::kStages - 2>();
-                        tell();
-                    }
-                } else {
-                    uint4 code[kCopies];
-                    if (mine) {
-#pragma unroll
-                        for (int x = 0; x < kCopies; ++x) {
-                            const int64_t off = sh.row[buf][row0 + x * kStep];
-                            code[x] = off >= 0 ? *reinterpret_cast<const uint4*>(base + off) : make_uint4(0, 0, 0, 0);
-                        }
-                    }
+                const uint32_t to = K::kFp8 ? ring + K::kStages * K::kUnit + unit % K::kRaw * (K::kUnit / 2) + tid * 16 : ring + stage * K::kUnit;
+                const char* base = keys + (of ? kv_gap : 0);
+                if (!K::kFp8 && !__all_sync(0xffffffffu, mbar_try_wait(&sh.empty[stage], parity))) {
+                    // no room: what is on the way may be what the consumer waits for
+                    cp_async_wait<0>();
+                    while (told < unit) tell();
                     wait(&sh.abandoned, &sh.empty[stage], parity);
                     __syncwarp();
-                    if (mine) {
-#pragma unroll
-                        for (int x = 0; x < kCopies; ++x) {
-                            const int r = row0 + x * kStep;
-                            uint4 lo, hi;
-                            fp8x4_to_f16<MODE>(code[x].x, lo.x, lo.y);
-                            fp8x4_to_f16<MODE>(code[x].y, lo.z, lo.w);
-                            fp8x4_to_f16<MODE>(code[x].z, hi.x, hi.y);
-                            fp8x4_to_f16<MODE>(code[x].w, hi.z, hi.w);
-                            const uint32_t at0 = to + place(K::T, r, 2 * piece), at1 = to + place(K::T, r, 2 * piece + 1);
-                            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at0), "r"(lo.x), "r"(lo.y), "r"(lo.z), "r"(lo.w) : "memory");
-                            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at1), "r"(hi.x), "r"(hi.y), "r"(hi.z), "r"(hi.w) : "memory");
-                        }
+                }
+                if (mine) {
+#pragma unroll 8
+                    for (int x = 0; x < kCopies; ++x) {
+                        const int r = row0 + x * kStep;
+                        const uint32_t off = rows[r];
+                        cp_async16(to + (K::kFp8 ? x * (kProducers * 16) : place(K::T, r, piece)),
+                                   off != kMasked ? base + (static_cast<int64_t>(off) << a.unit) : a.k, off != kMasked ? 16u : 0u);
                     }
-                    ++unit;
+                }
+                cp_async_commit();
+                ++unit;
+                if (unit - told > kAhead) {
+                    cp_async_wait<kAhead>();
                     tell();
                 }
             }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.rows_used[tile % kPlaces]);
         }
         more = run.next(a);
     }
-    if constexpr (!K::kFp8) {
-        cp_async_wait<0>();
-        while (told < unit) tell();
-    }
+    cp_async_wait<0>();
+    while (told < unit) tell();
 }
 
-// One thread issues every product.  Step x of an item: group x & 1 at tile x / 2 (dual) or x.
+// Whether weights enter the second product as two terms.  One f16 term is off by up to 2^-11 of a weight, an eighth of what
+// rounding the result to BF16 costs: over an FP8 cache, with BF16 queries, that is enough.  One BF16 term would cost as much as that rounding.
+template <class K>
+__device__ __forceinline__ bool two_terms(const PrefixArgs& a) {
+    return !K::kFp8 || a.q_f16;
+}
+
+__device__ __forceinline__ bool elect_one() {
+    uint32_t is;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(is));
+    return is != 0;
+}
+
+// One warp waits, and one of its threads issues every product.  Step x of an item: group x & 1 at tile x / 2 (dual) or x.
 template <class K>
 __device__ __forceinline__ void multiply(const PrefixArgs& a, typename K::Shared& sh, uint32_t ring, uint32_t queries, uint32_t tmem,
                                          Run<K> run) {
+    const bool leader = elect_one();
     const uint32_t of_s = product(K::kBf16, K::T, false);
     const int wide = (a.head_dim + 15) / 16;  // products of 16 along head_dim, and columns of O in 16s
     const uint32_t of_o = product(K::kBf16, wide * 16, true);
+    const bool two = two_terms<K>(a);
     uint32_t unit = 0;                               // first unit of the item at hand
     uint32_t s_steps[2] = {0, 0}, o_steps[2] = {0, 0}, q_items[2] = {0, 0};
     bool more = true;
@@ -385,272 +440,410 @@ __device__ __forceinline__ void multiply(const PrefixArgs& a, typename K::Shared
         auto scores = [&](int32_t x) {
             const int b = x & 1, s = K::kStreams == 2 ? b : 0;
             if (x < K::kStreams) {  // the group's queries of this item
-                wait(&sh.abandoned, &sh.q_full[s], q_items[s] & 1u);
-                ++q_items[s];
+                wait(&sh.abandoned, &sh.q_full[s], (b ? q_items[1] : q_items[0]) & 1u);
+                if (b) ++q_items[1];
+                else ++q_items[0];
             }
             // its weights of the step before, in S's place, have been used
-            if (o_steps[b] > 0) wait(&sh.abandoned, &sh.o_done[b], (o_steps[b] - 1) & 1u);
+            const uint32_t done = b ? o_steps[1] : o_steps[0];
+            if (done > 0) wait(&sh.abandoned, &sh.o_done[b], (done - 1) & 1u);
             const uint32_t u = unit + 2 * tile_of(x), stage = u % K::kStages;
             wait(&sh.abandoned, &sh.full[stage], u / K::kStages & 1u);
+            __syncwarp();
             tc_fence_after();
-            const uint32_t keys = ring + stage * K::kUnit, q = queries + s * K::kQ;
-            for (int c = 0; c < wide; ++c)
-                mma_ss(tmem + b * K::T, operand(q + (c >> 2) * (128 * 128) + (c & 3) * 32, 16, 1024),
-                       operand(keys + (c >> 2) * (K::T * 128) + (c & 3) * 32, 16, 1024), of_s, c > 0);
-            tc_commit(&sh.s_full[b]);
-            ++s_steps[b];
-            if (!dual || b == 1) tc_commit(&sh.empty[stage]);
+            if (leader) {
+                const uint64_t q = operand(queries + s * K::kQ, 16, 1024), keys = operand(ring + stage * K::kUnit, 16, 1024);
+                const uint32_t to = tmem + b * K::T;
+#pragma unroll
+                for (int c = 0; c < K::kDim / 16; ++c)
+                    if (c < wide) mma_ss(to, q + (c >> 2) * (128 * 8) + (c & 3) * 2, keys + (c >> 2) * (K::T * 8) + (c & 3) * 2, of_s, c > 0);
+                tc_commit(&sh.s_full[b]);
+                if (!dual || b == 1) tc_commit(&sh.empty[stage]);
+            }
+            __syncwarp();
+            if (b) ++s_steps[1];
+            else ++s_steps[0];
         };
-        for (int32_t x = 0; x < 2 && x < steps; ++x)
-            scores(x);
+        for (int32_t x = 0; x < 2 && x < steps; ++x) scores(x);
+#pragma unroll 1
         for (int32_t x = 0; x < steps; ++x) {
             const int b = x & 1, s = K::kStreams == 2 ? b : 0;
-            wait(&sh.abandoned, &sh.p_full[b], (s_steps[b] - 1) & 1u);
             const uint32_t u = unit + 2 * tile_of(x) + 1, stage = u % K::kStages;
             wait(&sh.abandoned, &sh.full[stage], u / K::kStages & 1u);
+            wait(&sh.abandoned, &sh.p_full[b], ((b ? s_steps[1] : s_steps[0]) - 1) & 1u);
+            __syncwarp();
             tc_fence_after();
-            const uint32_t values = ring + stage * K::kUnit, o = tmem + K::kO + s * K::kDim;
-            const bool first = x < K::kStreams;  // of the group's steps in this item
-#pragma unroll 1
-            for (int c = 0; c < K::T / 16; ++c) {
-                const uint64_t rows = operand(values + c * 2048, K::T * 128, 1024);
+            if (leader) {
+                const uint64_t values = operand(ring + stage * K::kUnit, K::T * 128, 1024);
+                const uint32_t o = tmem + K::kO + s * K::kDim, p = tmem + b * K::T;
+                const bool first = x < K::kStreams;  // of the group's steps in this item
                 // 32 tokens' weights: 16 columns of high terms, 16 of low ones
-                const uint32_t p = tmem + b * K::T + (c >> 1) * 32 + (c & 1) * 8;
-                mma_ts(o, p, rows, of_o, !first || c > 0);
-                mma_ts(o, p + 16, rows, of_o, true);
+#pragma unroll
+                for (int c = 0; c < K::T / 16; ++c) {
+                    mma_ts(o, p + (c >> 1) * 32 + (c & 1) * 8, values + c * 128, of_o, !first || c > 0);
+                    if (two) mma_ts(o, p + (c >> 1) * 32 + (c & 1) * 8 + 16, values + c * 128, of_o, true);
+                }
+                tc_commit(&sh.o_done[b]);
+                if (!dual || b == 1) tc_commit(&sh.empty[stage]);
             }
-            tc_commit(&sh.o_done[b]);
-            ++o_steps[b];
-            if (!dual || b == 1) tc_commit(&sh.empty[stage]);
+            __syncwarp();
+            if (b) ++o_steps[1];
+            else ++o_steps[0];
             if (x + 2 < steps) scores(x + 2);
         }
         unit += 2 * run.n;
         more = run.next(a);
     }
+    // the products read shared and tensor memory until here
+    if (leader) tc_commit(&sh.drained);
+    const uint64_t until = global_ns() + kWaitNs;
+    while (!mbar_try_wait(&sh.drained, 0) && global_ns() < until) {
+    }
+}
+
+// A row of a softmax group: what its scores are made of, the tokens that it sees, and its running maximum and sum.
+struct Row {
+    float scale, slope, cap;
+    int32_t len;
+    uint32_t begin, end;
+    float m, less, high, l;  // less: m, or 0 while it is -inf; high: what raises m
+    bool seen;               // whether the row sees any of the shared tokens
+};
+
+// 32 products as scores that count: capped, biased, masked.  `tok`: the first token; `word`: those that are there.
+__device__ __forceinline__ void count_scores(const PrefixArgs& a, const Row& row, uint32_t (&v)[32], uint32_t tok, uint32_t word) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * row.scale);
+    if (a.softcap > 0.0f) {
+        float most = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) most = fmaxf(most, fabsf(__uint_as_float(v[i])));
+        if (__any_sync(0xffffffffu, most >= kSmallCapped)) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                const float p = __uint_as_float(v[i]);
+                v[i] = __float_as_uint(fabsf(p) < kSmallCapped ? cap_small(p, a.softcap) : cap_large(p, row.cap));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(cap_small(__uint_as_float(v[i]), a.softcap));
+        }
+    }
+    if (a.slopes) {
+        // distance to the newest token, <= 0
+        const float away = static_cast<float>(static_cast<int32_t>(tok) - (row.len - 1));
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__fmaf_rn(row.slope, away + static_cast<float>(i), __uint_as_float(v[i])));
+    }
+    if (tok < row.begin) word = row.begin - tok >= 32 ? 0u : word & (0xffffffffu << (row.begin - tok));
+    if (row.end < tok + 32) word = row.end <= tok ? 0u : word & (0xffffffffu >> (32 - (row.end - tok)));
+    if (__any_sync(0xffffffffu, word != 0xffffffffu)) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = word >> i & 1u ? v[i] : 0xff800000u;
+    }
+}
+
+__device__ __forceinline__ float largest(const uint32_t (&v)[32]) {
+    float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int i = 0; i < 32; i += 8)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) t[x] = fmaxf(t[x], fmaxf(__uint_as_float(v[i + 2 * x]), __uint_as_float(v[i + 2 * x + 1])));
+    return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+}
+
+// A new maximum; `before`: whether O holds what earlier steps summed, which is then complete.
+template <class K, class Before>
+__device__ __forceinline__ void raise(const PrefixArgs& a, Row& row, float top, uint32_t o_at, Before&& before) {
+    if (!__any_sync(0xffffffffu, row.seen && top > row.high)) return;
+    const float m = row.m;
+    if (top > row.high) {
+        row.m = fmaxf(top - K::kBelow, m);
+        row.high = __fadd_rd(row.m, K::kAbove);  // down: 2^16 would be past f16
+        row.less = row.m == -INFINITY ? 0.0f : row.m;
+    }
+    const float f = rescale(m, row.m);
+    row.l *= f;
+    if (!before()) return;
+#pragma unroll 1
+    for (int c = 0; c < a.head_dim; c += 16) {
+        uint32_t o[16];
+        tm_load16(o, o_at + c);
+        tc_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+        tm_store16(o_at + c, o);
+    }
+}
+
+// The weights of 32 scores, to where those were: their high terms in 16 columns and their low terms in the 16 behind; their sum.
+template <class K>
+__device__ __forceinline__ float2 weights(const uint32_t (&v)[32], float by, float less, bool two, uint32_t at) {
+    const float2 by2 = make_float2(by, by), less2 = make_float2(-less, -less);
+    float2 sum = make_float2(0.0f, 0.0f);
+    uint32_t high[16], low[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        float2 p = __ffma2_rn(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), by2, less2);
+        p = make_float2(exp2_fast(p.x), exp2_fast(p.y));
+        sum = __fadd2_rn(sum, p);
+        high[i] = pack2<K::kBf16>(p.x, p.y);
+        float2 h;
+        unpack2<K::kBf16>(high[i], h.x, h.y);
+        const float2 rest = __fadd2_rn(p, make_float2(-h.x, -h.y));
+        low[i] = pack2<K::kBf16>(rest.x, rest.y);
+    }
+    tm_store16(at, high);
+    if (two) tm_store16(at + 16, low);
+    return sum;
+}
+
+// The weights of a tile of tokens from `first` on, whose products are at `at`, in their place.
+template <class K, class Before>
+__device__ __forceinline__ void weigh(const PrefixArgs& a, Row& row, uint32_t at, uint32_t first, const uint32_t* words, bool two, uint32_t o_at,
+                                      Before&& before) {
+    constexpr int kChunks = K::T / 32;
+    bool plain = first >= row.begin && first + K::T <= row.end;
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) plain &= words[c] == 0xffffffffu;
+    plain = __all_sync(0xffffffffu, (plain || !row.seen) && row.scale >= 0.0f) && a.softcap == 0.0f && a.slopes == nullptr;
+    uint32_t v[kChunks][32];
+    if (!plain) {
+#pragma unroll 1
+        for (int c = 0; c < kChunks; ++c) {
+            tm_load(v[0], at + c * 32);
+            tc_wait_ld();
+            count_scores(a, row, v[0], first + c * 32, words[c]);
+            tm_store(at + c * 32, v[0]);
+        }
+        tc_wait_st();
+    }
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) tm_load(v[c], at + c * 32);
+    tc_wait_ld();
+    const float by = plain ? row.scale : 1.0f;
+    float top = largest(v[0]);
+#pragma unroll
+    for (int c = 1; c < kChunks; ++c) top = fmaxf(top, largest(v[c]));
+    raise<K>(a, row, top * by, o_at, before);
+    float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) sum = __fadd2_rn(sum, weights<K>(v[c], by, row.less, two, at + c * 32));
+    row.l += sum.x + sum.y;
+}
+
+// The same for `mine` of the tile's chunks of 32 tokens, from c0 on; the others, other warps' with the same rows, weigh nothing here.
+template <class K, class Before>
+__device__ __forceinline__ void weigh_share(const PrefixArgs& a, Row& row, uint32_t at, uint32_t first, const uint32_t* words, int c0, int mine,
+                                            bool two, uint32_t o_at, Before&& before) {
+    uint32_t v[32];
+    float top = -INFINITY;
+#pragma unroll 1
+    for (int c = c0; c < c0 + mine; ++c) {
+        tm_load(v, at + c * 32);
+        tc_wait_ld();
+        count_scores(a, row, v, first + c * 32, words[c]);
+        top = fmaxf(top, largest(v));
+        if (mine > 1) tm_store(at + c * 32, v);
+    }
+    if (mine > 1) tc_wait_st();
+    raise<K>(a, row, top, o_at, before);
+    float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll 1
+    for (int c = c0; c < c0 + mine; ++c) {
+        if (mine > 1) {
+            tm_load(v, at + c * 32);
+            tc_wait_ld();
+        }
+        sum = __fadd2_rn(sum, weights<K>(v, 1.0f, row.less, two, at + c * 32));
+    }
+    row.l += sum.x + sum.y;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = 0u;
+#pragma unroll 1
+    for (int c = 0; c < K::T / 32; ++c)
+        if (c < c0 || c >= c0 + mine) tm_store(at + c * 32, v);
 }
 
 template <class K>
 __device__ __forceinline__ void soften(const PrefixArgs& a, typename K::Shared& sh, unsigned char* queries, uint32_t tmem, Run<K> run) {
     const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) & 3, stream = K::kStreams == 2 ? threadIdx.x >> 7 : 0;
-    const int my_row = threadIdx.x & 127;
+    const int my_lane = threadIdx.x & 127;  // of tensor memory
     const uint32_t lanes = tmem + (static_cast<uint32_t>(warp * 32) << 16);
     unsigned char* my_q = queries + stream * K::kQ;
     const uint32_t o_at = lanes + K::kO + stream * K::kDim;
     uint32_t s_steps[2] = {0, 0}, o_steps[2] = {0, 0};
-    int32_t tile0 = 0;
-    const float cap = a.softcap * kLog2e;
+    uint32_t tile0 = 0;
+    const bool two = two_terms<K>(a);
+    Row row;
+    row.cap = a.softcap * kLog2e;
     bool more = true;
     while (more) {
         const bool dual = run.dual();
-        const int32_t steps = run.steps();
+        const int32_t steps = run.steps(), sharers = dual ? 1 : run.sharers(), apart = 4 / sharers;  // warps of different rows
         const int32_t rows = dual ? min(128, run.rows - 128 * stream) : run.rows;
-        const bool busy = warp * 32 < rows;  // this warp has rows
+        const int set = warp & (apart - 1), my_row = set * 32 + lane, my_share = warp / apart;
+        const bool busy = set * 32 < rows;  // this warp has rows
         const bool valid = my_row < rows;
         // this row: request and query head
         const uint32_t nth = static_cast<uint32_t>(run.block * K::kRows + (dual ? 128 * stream : 0) + (valid ? my_row : 0));
         const int32_t member = nth / a.group, r = run.of.start + member, h = run.kv * a.group.d + (nth - member * a.group.d);
-        float scale = a.scale * (a.k_scale ? a.k_scale[run.kv] : 1.0f);
-        float m = -INFINITY, less = 0.0f, high = -INFINITY, l = 0.0f;
+        row.scale = a.scale * (a.k_scale ? a.k_scale[run.kv] : 1.0f);
+        row.m = row.high = -INFINITY;
+        row.less = row.l = 0.0f;
+        row.len = valid ? a.lens[r] : 0;
         if (stream < steps) {
-            // the queries into shared memory
-            const char* q = a.q + 2 * (r * a.q_req + h * a.q_head);
-            const int pieces = a.head_dim / 8;
-            auto piece = [&](int c) {
-                if (a.q_wide) return *reinterpret_cast<const uint4*>(q + 16 * c);
-                const uint32_t* w = reinterpret_cast<const uint32_t*>(q + 16 * c);
-                return make_uint4(w[0], w[1], w[2], w[3]);
-            };
-            float fit = 1.0f;
-            if constexpr (K::kFp8) {
-                // f16 queries, scaled by a power of two to a largest magnitude in [1, 2)
-                float top = 0.0f;
-                if (valid)
-                    for (int c = 0; c < pieces; ++c) {
-                        const uint4 v = piece(c);
-                        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            // the queries into shared memory: a few rows at a time, the lanes of a row side by side
+            constexpr int kLanes = K::kPanels * 8, kAtOnce = 32 / kLanes;  // 16-byte pieces of a row; rows of an instruction
+            const int64_t q_of = r * a.q_req + h * a.q_head;  // of a row that is not: the first row's
+            const int c = lane % kLanes;
+            const bool has = c < a.head_dim / 8;
+            constexpr int kBatch = 8;
+#pragma unroll 1
+            for (int i0 = 0; i0 < 32 / kAtOnce; i0 += kBatch) {
+                uint4 batch[kBatch];
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            float f0, f1;
-                            if (a.q_f16) unpack2<false>(w[x], f0, f1);
-                            else unpack2<true>(w[x], f0, f1);
-                            top = fmaxf(top, fmaxf(fabsf(f0), fabsf(f1)));
-                        }
+                for (int i = 0; i < kBatch; ++i) {
+                    const char* q = a.q + 2 * (__shfl_sync(0xffffffffu, q_of, (i0 + i) * kAtOnce + lane / kLanes) + (has ? c * 8 : 0));
+                    if (a.q_wide) {
+                        batch[i] = *reinterpret_cast<const uint4*>(q);
+                    } else {
+                        const uint32_t* w = reinterpret_cast<const uint32_t*>(q);
+                        batch[i] = make_uint4(w[0], w[1], w[2], w[3]);
                     }
-                const uint32_t field = __float_as_uint(top) >> 23;  // biased exponent
-                if (field >= 1 && field <= 254) {
-                    const uint32_t e = min(field, 253u);
-                    fit = __uint_as_float((254u - e) << 23);
-                    scale *= __uint_as_float(e << 23);
                 }
-            }
-            for (int c = 0; c < K::kPanels * 8; ++c) {
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (valid && c < pieces) {
-                    v = piece(c);
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) {
+                    const int j = (i0 + i) * kAtOnce + lane / kLanes;
+                    const bool there = __shfl_sync(0xffffffffu, valid, j) && has;
+                    uint32_t w[4] = {there ? batch[i].x : 0u, there ? batch[i].y : 0u, there ? batch[i].z : 0u, there ? batch[i].w : 0u};
                     if constexpr (K::kFp8) {
-                        uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                        // f16 queries, scaled by a power of two to a largest magnitude in [1, 2)
+                        float f[8], top = 0.0f;
 #pragma unroll
                         for (int x = 0; x < 4; ++x) {
-                            float f0, f1;
-                            if (a.q_f16) unpack2<false>(w[x], f0, f1);
-                            else unpack2<true>(w[x], f0, f1);
-                            w[x] = pack2<false>(f0 * fit, f1 * fit);
+                            if (a.q_f16) unpack2<false>(w[x], f[2 * x], f[2 * x + 1]);
+                            else unpack2<true>(w[x], f[2 * x], f[2 * x + 1]);
+                            top = fmaxf(top, fmaxf(fabsf(f[2 * x]), fabsf(f[2 * x + 1])));
                         }
-                        v = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+                        for (int d = 1; d < kLanes; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                        const uint32_t field = __float_as_uint(top) >> 23;  // biased exponent
+                        const bool scales = field >= 1 && field <= 254;
+                        const uint32_t e = min(field, 253u);
+                        const float fit = scales ? __uint_as_float((254u - e) << 23) : 1.0f, back = scales ? __uint_as_float(e << 23) : 1.0f;
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) w[x] = pack2<false>(f[2 * x] * fit, f[2 * x + 1] * fit);
+                        const float mine = __shfl_sync(0xffffffffu, back, lane % kAtOnce * kLanes);
+                        if (lane / kAtOnce == i0 + i) row.scale *= mine;
                     }
+                    *reinterpret_cast<uint4*>(my_q + place(128, warp * 32 + j, c)) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
-                *reinterpret_cast<uint4*>(my_q + place(128, my_row, c)) = v;
             }
             fence_proxy();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.q_full[stream]);
         }
-        scale = a.softcap > 0.0f ? __fdiv_rn(scale, a.softcap) * (2.0f * kLog2e) : scale * kLog2e;
-        const int32_t len = valid ? a.lens[r] : 0;
-        const uint32_t end = max(min(len, run.of.shared), 0), begin = a.window > 0 && len > a.window ? len - a.window : 0;
-        const float slope = a.slopes ? a.slopes[h] * kLog2e : 0.0f;
+        row.scale = a.softcap > 0.0f ? __fdiv_rn(row.scale, a.softcap) * (2.0f * kLog2e) : row.scale * kLog2e;
+        row.end = max(min(row.len, run.of.shared), 0);
+        row.begin = a.window > 0 && row.len > a.window ? row.len - a.window : 0;
+        row.slope = a.slopes ? a.slopes[h] * kLog2e : 0.0f;
+        row.seen = valid && row.begin < row.end;
+#pragma unroll 1
         for (int32_t x = K::kStreams == 2 ? stream : 0; x < steps; x += K::kStreams) {
             const int b = x & 1;
             const int32_t tile = dual ? x >> 1 : x;
-            wait(&sh.abandoned, &sh.s_full[b], s_steps[b] & 1u);
+            wait(&sh.abandoned, &sh.s_full[b], (b ? s_steps[1] : s_steps[0]) & 1u);
             __syncwarp();
-            ++s_steps[b];
-            const uint32_t s_at = lanes + b * K::T;
+            if (b) ++s_steps[1];
+            else ++s_steps[0];
             tc_fence_after();
             if (busy) {
+                const uint32_t s_at = lanes + b * K::T;
                 const uint32_t* words = sh.mask[(tile0 + tile) % kMasks];
                 const uint32_t first = static_cast<uint32_t>(run.t + tile) * K::T;
-                bool whole = first >= begin && first + K::T <= end;
-#pragma unroll
-                for (int c = 0; c < K::T / 32; ++c) whole &= words[c] == 0xffffffffu;
-                const bool plain = __all_sync(0xffffffffu, (whole || !valid) && scale >= 0.0f) && a.softcap == 0.0f && a.slopes == nullptr;
-                float top = -INFINITY;
-                uint32_t v[32];
-                if (plain) {
-#pragma unroll
-                    for (int c = 0; c < K::T / 32; ++c) {
-                        tm_load(v, s_at + c * 32);
-                        tc_wait_ld();
-                        float t0 = -INFINITY, t1 = -INFINITY;
-#pragma unroll
-                        for (int i = 0; i < 32; i += 2) {
-                            t0 = fmaxf(t0, __uint_as_float(v[i]));
-                            t1 = fmaxf(t1, __uint_as_float(v[i + 1]));
-                        }
-                        top = fmaxf(top, fmaxf(t0, t1));
-                    }
-                    top *= scale;
-                } else {
-                    // scores as they count, put back in the place of the products
-#pragma unroll 1
-                    for (int c = 0; c < K::T / 32; ++c) {
-                        tm_load(v, s_at + c * 32);
-                        tc_wait_ld();
-                        const uint32_t word = words[c];
-                        const uint32_t tok = first + c * 32;
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            float p = __uint_as_float(v[i]) * scale;
-                            if (a.softcap > 0.0f) p = fabsf(p) < kSmallCapped ? cap_small(p, a.softcap) : cap_large(p, cap);
-                            if (a.slopes) p = __fmaf_rn(slope, static_cast<float>(static_cast<int32_t>(tok + i) - (len - 1)), p);
-                            const bool seen = (word >> i & 1u) && tok + i >= begin && tok + i < end;
-                            p = seen ? p : -INFINITY;
-                            v[i] = __float_as_uint(p);
-                            top = fmaxf(top, p);
-                        }
-                        tm_store(s_at + c * 32, v);
-                    }
-                    tc_wait_st();
-                }
-                const float by = plain ? scale : 1.0f;
-                if (__any_sync(0xffffffffu, valid && top > high)) {
-                    float less_before = m;
-                    if (top > high) {
-                        m = fmaxf(top - K::kBelow, m);
-                        high = __fadd_rd(m, K::kAbove);  // down: 2^16 would be past f16
-                        less = m == -INFINITY ? 0.0f : m;
-                    }
-                    const float f = rescale(less_before, m);
-                    l *= f;
-                    if (x >= K::kStreams) {
-                        // O of the steps before is complete
-                        const int pb = K::kStreams == 2 ? b : (x - 1) & 1;
-                        wait(&sh.abandoned, &sh.o_done[pb], (o_steps[pb] - 1) & 1u);
-                        __syncwarp();
-                        tc_fence_after();
-#pragma unroll 1
-                        for (int c = 0; c < K::kDim; c += 32) {
-                            if (c >= a.head_dim) break;
-                            tm_load(v, o_at + c);
-                            tc_wait_ld();
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
-                            tm_store(o_at + c, v);
-                        }
-                        tc_wait_st();
-                    }
-                }
-                float sum = 0.0f;
-#pragma unroll 1
-                for (int c = 0; c < K::T / 32; ++c) {
-                    tm_load(v, s_at + c * 32);
-                    tc_wait_ld();
-                    float s0 = 0.0f, s1 = 0.0f;
-                    uint32_t w[32];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float p0 = exp2_fast(__fmaf_rn(__uint_as_float(v[2 * i]), by, -less));
-                        const float p1 = exp2_fast(__fmaf_rn(__uint_as_float(v[2 * i + 1]), by, -less));
-                        s0 += p0;
-                        s1 += p1;
-                        w[i] = pack2<K::kBf16>(p0, p1);
-                        float h0, h1;
-                        unpack2<K::kBf16>(w[i], h0, h1);
-                        w[16 + i] = pack2<K::kBf16>(p0 - h0, p1 - h1);
-                    }
-                    sum += s0 + s1;
-                    tm_store(s_at + c * 32, w);
-                }
-                l += sum;
+                auto before = [&]() {
+                    if (x < K::kStreams) return false;
+                    const int pb = K::kStreams == 2 ? b : (x - 1) & 1;
+                    wait(&sh.abandoned, &sh.o_done[pb], ((pb ? o_steps[1] : o_steps[0]) - 1) & 1u);
+                    __syncwarp();
+                    tc_fence_after();
+                    return true;
+                };
+                const int each = K::T / 32 / sharers;
+                if (sharers == 1) weigh<K>(a, row, s_at, first, words, two, o_at, before);
+                else weigh_share<K>(a, row, s_at, first, words, my_share * each, each, two, o_at, before);
                 tc_wait_st();
             }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.p_full[b]);
-            ++o_steps[b];
+            if (b) ++o_steps[1];
+            else ++o_steps[0];
         }
-        // this CTA's part of the row
-        const bool first = run.t == 0;
-        if (steps > stream) {
-            const int32_t last = steps - 1 - ((steps - 1 - stream) % K::kStreams);
-            const int b = last & 1;
-            wait(&sh.abandoned, &sh.o_done[b], (o_steps[b] - 1) & 1u);
+        // This CTA's part of the rows, through the place of the queries, with which the products are done: rows side by side, and the
+        // warps that share rows joined.
+        const bool has = steps > stream, first = run.t == 0;
+        const int64_t at = first ? (static_cast<int64_t>(dual ? 0 : stream) * a.n_requests + r) * a.q_heads + h
+                                 : (static_cast<int64_t>(blockIdx.x) * 2 + stream) * 128 + my_row;
+        float2* ml_to = (first ? a.part_ml : a.cta_ml) + at;
+        if (!has) {
+            if (valid && my_share == 0) *ml_to = make_float2(-INFINITY, 0.0f);
+        } else {
+            const int b = (steps - 1 - (steps - 1 - stream) % K::kStreams) & 1;
+            wait(&sh.abandoned, &sh.o_done[b], ((b ? o_steps[1] : o_steps[0]) - 1) & 1u);
             __syncwarp();
             tc_fence_after();
-        }
-        const bool has = steps > stream;
-        if (valid && (first || has || !dual)) {
-            const int half = dual ? 0 : stream;
-            const int64_t row = (static_cast<int64_t>(r) + static_cast<int64_t>(half) * a.n_requests) * a.q_heads + h;
-            const int64_t slot = (static_cast<int64_t>(blockIdx.x) * 2 + stream) * 128 + my_row;
-            if (first) a.part_ml[row] = make_float2(m, has ? l : 0.0f);
-            else a.cta_ml[slot] = make_float2(m, has ? l : 0.0f);
-        }
-        if (busy && has) {
-            const int half = dual ? 0 : stream;
-            const int64_t row = (static_cast<int64_t>(r) + static_cast<int64_t>(half) * a.n_requests) * a.q_heads + h;
-            const int64_t slot = (static_cast<int64_t>(blockIdx.x) * 2 + stream) * 128 + my_row;
-            float* to = first ? a.part + row * a.head_dim : a.cta_part + slot * a.head_dim;
+            if (!row.seen) {  // what it has is of nothing
+                row.m = -INFINITY;
+                row.l = 0.0f;
+            }
+            float top = row.m, sum = row.l, weight = 1.0f;
+            if (sharers > 1) {
+                float2* ml = reinterpret_cast<float2*>(my_q);
+                ml[my_lane] = make_float2(row.m, row.l);
+                asm volatile("bar.sync %0, 128;" ::"r"(2 + stream) : "memory");
+                sum = 0.0f;
+                for (int x = 0; x < sharers; ++x) top = fmaxf(top, ml[x * apart * 32 + my_row].x);
+                for (int x = 0; x < sharers; ++x) {
+                    const float2 of = ml[x * apart * 32 + my_row];
+                    if (of.y != 0.0f) sum += of.y * rescale(of.x, top);
+                }
+                weight = rescale(row.m, top);
+                asm volatile("bar.sync %0, 128;" ::"r"(2 + stream) : "memory");
+            }
+            if (valid && my_share == 0) *ml_to = make_float2(top, sum);
+            const float* to = (first ? a.part : a.cta_part) + at * a.head_dim;
+            float4* lines = reinterpret_cast<float4*>(my_q);  // [128][8], pieces exchanged
+            const int piece = lane & 7;
 #pragma unroll 1
             for (int c = 0; c < a.head_dim; c += 32) {
                 uint32_t v[32];
                 tm_load(v, o_at + c);
                 tc_wait_ld();
-                if (valid) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4)
-                        if (c + i < a.head_dim) *reinterpret_cast<uint4*>(to + c + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                for (int i = 0; i < 8; ++i) {
+                    const float4 f = make_float4(__uint_as_float(v[4 * i]) * weight, __uint_as_float(v[4 * i + 1]) * weight,
+                                                 __uint_as_float(v[4 * i + 2]) * weight, __uint_as_float(v[4 * i + 3]) * weight);
+                    lines[my_lane * 8 + (i ^ (lane & 7))] = row.l == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : f;
                 }
+                if (sharers > 1) asm volatile("bar.sync %0, 128;" ::"r"(2 + stream) : "memory");
+                else __syncwarp();
+                // of this warp's set of rows the share of this warp, four rows at a time
+#pragma unroll 2
+                for (int i = 0; i < 8 / sharers; ++i) {
+                    const int j = (my_share * (8 / sharers) + i) * 4 + (lane >> 3);
+                    float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    for (int x = 0; x < sharers; ++x) {
+                        const float4 g = lines[((x * apart + set) * 32 + j) * 8 + (piece ^ (j & 7))];
+                        f = make_float4(f.x + g.x, f.y + g.y, f.z + g.z, f.w + g.w);
+                    }
+                    float* there = const_cast<float*>(reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(to), j)));
+                    const bool is = __shfl_sync(0xffffffffu, valid, j);
+                    if (is && c + piece * 4 < a.head_dim) *reinterpret_cast<float4*>(there + c + piece * 4) = f;
+                }
+                if (sharers > 1) asm volatile("bar.sync %0, 128;" ::"r"(2 + stream) : "memory");
+                else __syncwarp();
             }
             tc_fence_before();
         }
@@ -659,16 +852,53 @@ __device__ __forceinline__ void soften(const PrefixArgs& a, typename K::Shared& 
     }
 }
 
+// One warp tells the other launches each request's first token of its own, and where its shared part's pieces will be.
+template <class K>
+__device__ __forceinline__ void take_notes(const PrefixArgs& a, bool bad) {
+    const int lane = threadIdx.x & 31;
+    const int32_t begin = bad || a.n_groups == 0 ? a.n_requests : a.starts[0], end = bad || a.n_groups == 0 ? a.n_requests : a.starts[a.n_groups];
+    for (int32_t r = blockIdx.x * 32 + lane; r < a.n_requests; r += gridDim.x * 32)
+        if (r < begin || r >= end) {
+            a.own_first[r] = 0;
+            a.info[r] = Shared{0, 0, 0, 0};
+        }
+    if (bad) return;
+    int64_t front = 0;
+    for (int32_t g0 = 0; g0 < a.n_groups; g0 += 32) {
+        const int32_t g = g0 + lane;
+        Group x{0, 0, 0, false};
+        if (g < a.n_groups) x = group_of(a, g);
+        const int64_t of = items_of<K>(a, x) * tiles_of<K>(x);
+        int64_t upto = of;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int64_t y = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += y;
+        }
+        const int32_t base = static_cast<int32_t>(front + upto - of);
+        front += __shfl_sync(0xffffffffu, upto, 31);
+        uint32_t mine = __ballot_sync(0xffffffffu, g < a.n_groups && g % gridDim.x == blockIdx.x);
+        while (mine) {
+            const int src = __ffs(mine) - 1;
+            mine &= mine - 1;
+            const Shared note{__shfl_sync(0xffffffffu, base, src), __shfl_sync(0xffffffffu, tiles_of<K>(x), src), __shfl_sync(0xffffffffu, x.start, src),
+                              __shfl_sync(0xffffffffu, x.members, src)};
+            const int32_t shared = __shfl_sync(0xffffffffu, x.shared, src);
+            for (int32_t i = lane; i < note.members; i += 32) {
+                a.own_first[note.start + i] = shared;
+                a.info[note.start + i] = note;
+            }
+        }
+    }
+}
+
 template <int MODE, int DP>
-__global__ void __launch_bounds__(Prefix<MODE, DP>::kThreads, 1) prefix_kernel(const PrefixArgs a) {
+__global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const PrefixArgs a) {
     using K = Prefix<MODE, DP>;
     extern __shared__ __align__(1024) unsigned char smem[];
-    unsigned char* queries = smem + K::kStages * K::kUnit;
+    unsigned char* queries = smem + K::kRing;
     auto& sh = *reinterpret_cast<typename K::Shared*>(queries + K::kStreams * K::kQ);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    constexpr int kWarps = K::kThreads / 32, kIssuer = kWarps - 1;
-    after_previous();
-    let_next_start();
     if (tid == 0) {
         for (int i = 0; i < K::kStages; ++i) {
             mbar_init(&sh.full[i], kProducers / 32);
@@ -680,42 +910,56 @@ __global__ void __launch_bounds__(Prefix<MODE, DP>::kThreads, 1) prefix_kernel(c
             mbar_init(&sh.o_done[i], 1);
             mbar_init(&sh.q_full[i], 4);
         }
+        for (int i = 0; i < kPlaces; ++i) {
+            mbar_init(&sh.rows_known[i], 1);
+            mbar_init(&sh.rows_used[i], kProducers / 32);
+        }
         mbar_init(&sh.drained, 1);
         fence_barrier_init();
         sh.abandoned = 0;
     }
+    if (warp == kIssuer) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    after_previous();
+    let_next_start();
     // the tiles of thread i's `per` consecutive groups, in a row
-    int64_t* sums = reinterpret_cast<int64_t*>(smem);  // [threads + 1], before the ring is used
-    const int32_t per = (a.n_groups + K::kThreads - 1) / K::kThreads;
+    int64_t* sums = reinterpret_cast<int64_t*>(queries);  // of the warps, before the queries come
+    const int32_t per = (a.n_groups + kThreads - 1) / kThreads;
     int64_t mine = 0;
     bool bad = false;
+    Group last{0, 0, 0, false};
     for (int32_t i = 0; i < per; ++i) {
         const int32_t g = tid * per + i;
         if (g >= a.n_groups) break;
-        const Group x = group_of(a, g);
-        bad |= x.bad;
-        mine += items_of<K>(a, x) * tiles_of<K>(x);
+        last = group_of(a, g);
+        bad |= last.bad;
+        mine += items_of<K>(a, last) * tiles_of<K>(last);
     }
-    bad = __syncthreads_or(bad);
-    sums[tid] = mine;
-    __syncthreads();
-    if (warp == 0) {
-        int64_t front = 0;
-        for (int t0 = 0; t0 < K::kThreads; t0 += 32) {
-            int64_t upto = sums[t0 + lane];
-            const int64_t own = upto;
+    int64_t upto = mine;
 #pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const int64_t x = __shfl_up_sync(0xffffffffu, upto, d);
-                if (lane >= d) upto += x;
-            }
-            sums[t0 + lane] = front + upto - own;
-            front += __shfl_sync(0xffffffffu, upto, 31);
-        }
-        if (lane == 0) sums[K::kThreads] = front;
+    for (int d = 1; d < 32; d <<= 1) {
+        const int64_t x = __shfl_up_sync(0xffffffffu, upto, d);
+        if (lane >= d) upto += x;
     }
-    __syncthreads();
-    int64_t total64 = sums[K::kThreads];
+    if (lane == 31) sums[warp] = upto;
+    // what is past the head in a row is never copied: zeros
+    if (a.head_dim < DP) {
+        for (int i = tid; i < K::kRing / 16; i += kThreads) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+        fence_proxy();
+    }
+    tc_fence_before();
+    bad = __syncthreads_or(bad);
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem, ring = smem_u32(smem);
+    int64_t total64 = 0, front = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+        if (w == warp) front = total64;
+        total64 += sums[w];
+    }
+    front += upto - mine;
     if (bad || total64 > 0x7fffffff) {
         // nothing is shared then: every request reads all of its tokens
         if (tid == 0) atomicExch(a.status, MF_DEVICE_TOO_LARGE);
@@ -723,71 +967,43 @@ __global__ void __launch_bounds__(Prefix<MODE, DP>::kThreads, 1) prefix_kernel(c
         total64 = 0;
     }
     const int32_t total = static_cast<int32_t>(total64), ctas = min(total, static_cast<int32_t>(gridDim.x));
-    // what the other launches need to know
     if (blockIdx.x == 0 && tid == 0) *a.cut = make_int2(total, ctas);
-    const int32_t begin = bad || a.n_groups == 0 ? a.n_requests : a.starts[0], end = bad || a.n_groups == 0 ? a.n_requests : a.starts[a.n_groups];
-    for (int32_t r = blockIdx.x * K::kThreads + tid; r < a.n_requests; r += gridDim.x * K::kThreads)
-        if (r < begin || r >= end) {
-            a.own_first[r] = 0;
-            a.info[r] = Shared{0, 0, 0, 0};
-        }
-    if (!bad)
-        for (int32_t g = blockIdx.x; g < a.n_groups; g += gridDim.x) {
-            const Group x = group_of(a, g);
-            int64_t base = sums[g / max(per, 1)];
-            for (int32_t b = g / per * per; b < g; ++b) {
-                const Group y = group_of(a, b);
-                base += items_of<K>(a, y) * tiles_of<K>(y);
+    if (static_cast<int32_t>(blockIdx.x) < ctas) {
+        const Cut cut(total, ctas);
+        const int32_t x0 = cut.start(blockIdx.x), run_of = cut.start(blockIdx.x + 1) - x0;
+        if (front <= x0 && x0 < front + mine) {
+            int32_t into = x0 - static_cast<int32_t>(front), g = tid * per;
+            if (per > 1) {
+                for (;; ++g) {
+                    last = group_of(a, g);
+                    const int64_t of = items_of<K>(a, last) * tiles_of<K>(last);
+                    if (into < of) break;
+                    into -= static_cast<int32_t>(of);
+                }
             }
-            for (int32_t i = tid; i < x.members; i += K::kThreads) {
-                a.own_first[x.start + i] = x.shared;
-                a.info[x.start + i] = Shared{static_cast<int32_t>(base), tiles_of<K>(x), x.start, x.members};
-            }
+            sh.of = last;
+            sh.group = g;
+            sh.into = into;
         }
-    if (static_cast<int32_t>(blockIdx.x) >= ctas) return;
-    const Cut cut(total, ctas);
-    const int32_t x0 = cut.start(blockIdx.x), run_of = cut.start(blockIdx.x + 1) - x0;
-    const bool here = sums[tid] <= x0 && x0 < sums[tid] + mine;
-    if (here) {
-        int32_t into = x0 - static_cast<int32_t>(sums[tid]);
-        for (int32_t g = tid * per;; ++g) {
-            const Group x = group_of(a, g);
-            const int64_t of = items_of<K>(a, x) * tiles_of<K>(x);
-            if (into < of) {
-                sh.group = g;
-                sh.into = into;
-                break;
-            }
-            into -= static_cast<int32_t>(of);
+        __syncthreads();
+        const Run<K> run(a, sh.of, sh.group, sh.into, run_of);
+        const int role = tid >> 7;
+        if (role < K::kStreams) {
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+            soften<K>(a, sh, queries, tmem, run);
+        } else if (role == kFirstProducer / 128) {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegs));
+            produce<K, MODE>(a, sh, ring, run);
+        } else {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+            if (warp == kIssuer) multiply<K>(a, sh, ring, smem_u32(queries), tmem, run);
+            else if (warp == kPager) find_rows<K>(a, sh, run);
+            else if (warp == kNoter) take_notes<K>(a, bad);
         }
+        __syncwarp();
+    } else if (warp == kNoter) {
+        take_notes<K>(a, bad);
     }
-    if (warp == kIssuer) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem)) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = sh.tmem, ring = smem_u32(smem);
-    // what is past the head in a row is never copied: zeros
-    if (a.head_dim < DP) {
-        for (int i = tid; i < K::kStages * K::kUnit / 16; i += K::kThreads) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
-        fence_proxy();
-    }
-    const Run<K> run(a, sh.group, sh.into, run_of);
-    __syncthreads();
-    if (tid < K::kSoftmax) soften<K>(a, sh, queries, tmem, run);
-    else if (tid < K::kSoftmax + kProducers) produce<K, MODE>(a, sh, ring, run);
-    else if (lane == 0) {
-        multiply<K>(a, sh, ring, smem_u32(queries), tmem, run);
-        // the products read shared and tensor memory until here
-        tc_commit(&sh.drained);
-        const uint64_t until = global_ns() + kWaitNs;
-        while (!mbar_try_wait(&sh.drained, 0) && global_ns() < until) {
-        }
-    }
-    if (warp > K::kSoftmax / 32 - 1 && warp < kIssuer) cp_async_wait<0>();
-    __syncwarp();
     tc_fence_before();
     __syncthreads();
     if (tid == 0 && sh.abandoned) atomicExch(a.status, MF_DEVICE_TIMEOUT);
@@ -801,8 +1017,7 @@ __global__ void __launch_bounds__(Prefix<MODE, DP>::kThreads, 1) prefix_kernel(c
 
 constexpr int kJoinThreads = 256;
 
-// A warp for each query head of a request.  ROWS: of a block; DUAL: whether blocks of more than 128 rows are two; BELOW: what a
-// weight of a maximum is, a power of two.
+// A warp for each query head of a request.  ROWS: of a block; F16: the weights of a maximum are 2^12.
 template <int ROWS, bool F16>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const PrefixArgs a) {
     constexpr float kBelow = F16 ? 12.0f : 0.0f, kMost = F16 ? 4096.0f : 1.0f;
@@ -811,68 +1026,92 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const PrefixArgs a) 
     let_next_start();
     const int64_t n = static_cast<int64_t>(a.n_requests) * a.q_heads;
     const int2 all = *a.cut;
+    const int32_t dim = a.head_dim;
     for (int64_t w = (static_cast<int64_t>(blockIdx.x) * kJoinThreads + threadIdx.x) >> 5; w < n; w += static_cast<int64_t>(gridDim.x) * (kJoinThreads / 32)) {
         const int32_t r = static_cast<int32_t>(w / a.q_heads), h = static_cast<int32_t>(w - static_cast<int64_t>(r) * a.q_heads);
+        const int32_t kv = h / a.group;
+        const float vs = a.v_scale ? a.v_scale[kv] : 1.0f;
         const Shared x = a.info[r];
         // its own tokens as a part whose largest weight is kMost, too
         const float own = a.own_lse[w];
-        float top = own * kLog2e - kBelow;
-        int32_t parts = 0, first = 0, slot = 0;
-        bool dual = false;
-        if (x.tiles > 0) {
-            const int32_t kv = h / a.group.d;
-            const int64_t nth = static_cast<int64_t>(r - x.start) * a.group.d + (h - kv * a.group.d), rows = static_cast<int64_t>(x.members) * a.group.d;
-            const int32_t blocks = static_cast<int32_t>((rows + ROWS - 1) / ROWS), block = static_cast<int32_t>(nth / ROWS);
-            const int32_t row = static_cast<int32_t>(nth - static_cast<int64_t>(block) * ROWS);
-            dual = ROWS == 256 && rows - static_cast<int64_t>(block) * ROWS > 128;
-            const Cut cut(all.x, all.y);
-            const int32_t begin = x.base + (kv * blocks + block) * x.tiles;
-            first = cut.part_of(begin);
-            parts = cut.part_of(begin + x.tiles - 1) - first + 1;
-            slot = row;  // of the 2 x 128 of a CTA: the second half of a dual block, too
+        float4 acc[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int d = 4 * (lane + 32 * i);
+            acc[i] = d < dim ? *reinterpret_cast<const float4*>(a.own + w * dim + d) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
-        const int halves = dual || ROWS == 128 ? 1 : 2;
-        auto ml_of = [&](int32_t p, int half) {
-            return p == 0 ? a.part_ml[(static_cast<int64_t>(half) * a.n_requests + r) * a.q_heads + h]
-                          : a.cta_ml[static_cast<int64_t>(first + p) * 256 + half * 128 + slot];
+        // the parts of its shared tokens, in order: an item's first CTA's, then the other CTAs', each of one half or two
+        int32_t parts = 0, halves = 1;
+        int64_t first_at = 0, first_apart = 0, at = 0;  // rows of part, cta_part
+        if (x.tiles > 0) {
+            const int64_t nth = static_cast<int64_t>(r - x.start) * a.group.d + (h - kv * static_cast<int32_t>(a.group.d)), rows = static_cast<int64_t>(x.members) * a.group.d;
+            const int32_t blocks = static_cast<int32_t>((rows + ROWS - 1) / ROWS), block = static_cast<int32_t>(nth / ROWS);
+            halves = ROWS == 128 || rows - static_cast<int64_t>(block) * ROWS > 128 ? 1 : 2;
+            const Cut cut(all.x, all.y);
+            const int32_t begin = x.base + (kv * blocks + block) * x.tiles, cta = cut.part_of(begin);
+            parts = (cut.part_of(begin + x.tiles - 1) - cta + 1) * halves;
+            first_at = w;
+            first_apart = n;
+            at = static_cast<int64_t>(cta) * 256 + (nth - static_cast<int64_t>(block) * ROWS);
+        }
+        auto row_of = [&](int32_t p) {  // of part p: negative in part (one less than minus its row), else of cta_part
+            const int32_t k = halves == 2 ? p >> 1 : p, half = halves == 2 ? p & 1 : 0;
+            return k == 0 ? -(first_at + half * first_apart) - 1 : at + static_cast<int64_t>(k) * 256 + half * 128;
         };
-        for (int32_t p = 0; p < parts; ++p)
-            for (int half = 0; half < halves; ++half) {
-                const float2 ml = ml_of(p, half);
+        float top = own * kLog2e - kBelow;
+        float2 ml = make_float2(-INFINITY, 0.0f);
+        int64_t row = 0;
+        for (int32_t p0 = 0; p0 < parts; p0 += 32) {
+            if (p0 + lane < parts) {
+                row = row_of(p0 + lane);
+                ml = row < 0 ? a.part_ml[-row - 1] : a.cta_ml[row];
                 if (ml.y != 0.0f) top = fmaxf(top, ml.x);
             }
-        // a NaN anywhere shows in the sum
-        const float vs = a.v_scale ? a.v_scale[h / a.group.d] : 1.0f;
-        const float own_w = own == -INFINITY ? 0.0f : kMost * exp2_fast(own * kLog2e - kBelow - top);
-        float sum = own_w;
-        float acc[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int d = lane + 32 * i;
-            acc[i] = d < a.head_dim && own_w != 0.0f ? a.own[w * a.head_dim + d] * own_w : 0.0f;
         }
-        for (int32_t p = 0; p < parts; ++p)
-            for (int half = 0; half < halves; ++half) {
-                const float2 ml = ml_of(p, half);
-                if (ml.y == 0.0f) continue;
-                const float by = rescale(ml.x, top);
-                sum = __fmaf_rn(ml.y, by, sum);
-                const float* from = p == 0 ? a.part + ((static_cast<int64_t>(half) * a.n_requests + r) * a.q_heads + h) * a.head_dim
-                                           : a.cta_part + (static_cast<int64_t>(first + p) * 256 + half * 128 + slot) * a.head_dim;
-                const float weight = by * vs;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int d = lane + 32 * i;
-                    if (d < a.head_dim) acc[i] = __fmaf_rn(from[d], weight, acc[i]);
+        for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        const float own_w = own == -INFINITY ? 0.0f : kMost * exp2_fast(own * kLog2e - kBelow - top);
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            acc[i] = own_w == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(acc[i].x * own_w, acc[i].y * own_w, acc[i].z * own_w, acc[i].w * own_w);
+        for (int32_t p0 = 0; p0 < parts; p0 += 32) {
+            if (parts > 32 && p0 + lane < parts) {
+                row = row_of(p0 + lane);
+                ml = row < 0 ? a.part_ml[-row - 1] : a.cta_ml[row];
+            }
+            const bool in = p0 + lane < parts && ml.y != 0.0f;
+            const float by = in ? rescale(ml.x, top) : 0.0f;
+            sum += in ? ml.y * by : 0.0f;
+            const int32_t here = min(32, parts - p0);
+#pragma unroll 4
+            for (int32_t p = 0; p < here; ++p) {
+                const float weight = __shfl_sync(0xffffffffu, by, p) * vs;
+                const int64_t of = __shfl_sync(0xffffffffu, row, p);
+                const bool some = __shfl_sync(0xffffffffu, in, p);
+                const float* from = of < 0 ? a.part + (-of - 1) * dim : a.cta_part + of * dim;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int d = 4 * (lane + 32 * i);
+                    if (some && d < dim) {
+                        const float4 f = *reinterpret_cast<const float4*>(from + d);
+                        acc[i] = make_float4(__fmaf_rn(f.x, weight, acc[i].x), __fmaf_rn(f.y, weight, acc[i].y), __fmaf_rn(f.z, weight, acc[i].z),
+                                             __fmaf_rn(f.w, weight, acc[i].w));
+                    }
                 }
             }
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        sum += own_w;
         const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int d = lane + 32 * i;
-            if (d >= a.head_dim) break;
-            const uint32_t two = a.q_f16 ? pack2<false>(acc[i] * inv, 0.0f) : pack2<true>(acc[i] * inv, 0.0f);
-            *reinterpret_cast<uint16_t*>(a.out + 2 * (r * a.out_req + h * a.out_head + d)) = static_cast<uint16_t>(two);
+        for (int i = 0; i < 2; ++i) {
+            const int d = 4 * (lane + 32 * i);
+            if (d >= dim) break;
+            const float4 f = make_float4(acc[i].x * inv, acc[i].y * inv, acc[i].z * inv, acc[i].w * inv);
+            const uint2 two = a.q_f16 ? make_uint2(pack2<false>(f.x, f.y), pack2<false>(f.z, f.w)) : make_uint2(pack2<true>(f.x, f.y), pack2<true>(f.z, f.w));
+            *reinterpret_cast<uint2*>(a.out + 2 * (r * a.out_req + h * a.out_head + d)) = two;
         }
         if (lane == 0 && a.lse) a.lse[w] = sum == 0.0f ? -INFINITY : (top + kBelow + log2f(sum * (1.0f / kMost))) * kLn2;
     }
@@ -889,7 +1128,7 @@ template <int MODE, int DP>
 Kernel kernel_of() {
     using K = Prefix<MODE, DP>;
     static_assert(K::kBytes <= 232448, "shared memory of one CTA");
-    return Kernel{prefix_kernel<MODE, DP>, join_kernel<K::kRows, !K::kBf16>, K::kThreads, K::kBytes};
+    return Kernel{prefix_kernel<MODE, DP>, join_kernel<K::kRows, !K::kBf16>, kThreads, K::kBytes};
 }
 template <int MODE>
 Kernel pick_dim(int head_dim) {
@@ -933,6 +1172,17 @@ extern "C" int mf_prefix_attn_create(const mf_paged_attn_config* config, int32_t
     }
     const mf_paged_attn_config& c = *config;
     const mf_cache_layout& k = c.cache;
+    // places of rows are kept in 32 bits, in the largest unit that strides allow
+    const int code = is_fp8(k.dtype) ? 1 : 2;
+    const int64_t page_bytes = k.page_stride * code, row_bytes = k.token_stride * code;
+    uint32_t unit = 4;
+    while (unit < 30 && ((page_bytes | row_bytes) >> unit & 1) == 0) ++unit;
+    const int64_t n_pages = k.n_pages < 0x7fffffff ? k.n_pages : 0x7fffffff;
+    if (static_cast<double>(n_pages) * page_bytes + static_cast<double>(k.page_size) * row_bytes >= 4294967295.0 * (1ll << unit)) {
+        mf_paged_attn_destroy(own);
+        return fail(MF_ERR_LAYOUT_UNSUPPORTED, "mf_prefix_attn_create: %lld pages of %lld bytes: more than 2^32 - 1 units of %lld bytes",
+                    (long long)n_pages, (long long)page_bytes, 1ll << unit);
+    }
     const Kernel kernel = pick(k.dtype, k.head_dim);
     cudaError_t err = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel.fn), cudaFuncAttributeMaxDynamicSharedMemorySize, kernel.shared);
     const int ctas = state().sm_count;
@@ -962,7 +1212,6 @@ extern "C" int mf_prefix_attn_create(const mf_paged_attn_config* config, int32_t
         return err != cudaSuccess ? cuda_fail(err, "mf_prefix_attn_create: cudaMalloc")
                                   : fail(MF_ERR_CUDA, "mf_prefix_attn_create: sticky status word unavailable");
     }
-    const int code = is_fp8(k.dtype) ? 1 : 2;
     char* w = static_cast<char*>(h->workspace);
     h->own = own;
     h->kernel = kernel;
@@ -973,8 +1222,9 @@ extern "C" int mf_prefix_attn_create(const mf_paged_attn_config* config, int32_t
     a.page = k.page_size;
     a.window = c.window;
     a.kv_heads = k.kv_heads;
-    a.page_bytes = k.page_stride * code;
-    a.row_bytes = k.token_stride * code;
+    a.unit = unit;
+    a.page_units = static_cast<uint32_t>(page_bytes >> unit);
+    a.row_units = static_cast<uint32_t>(row_bytes >> unit);
     a.head_bytes = k.head_stride * code;
     a.table_stride = c.table_stride;
     a.n_pages = static_cast<uint32_t>(k.n_pages < 0x7fffffff ? k.n_pages : 0x7fffffff);

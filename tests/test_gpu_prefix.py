@@ -41,6 +41,17 @@ def make_groups(groups, hq, hkv, dim, page, order, dtype, cache, seed, alone=0):
     return s
 
 
+def check_prefix(s, got, want):
+    """The bounds of the attention without sharing (the join adds float32 products of weights that are good to 2^-22).
+
+    Over an FP8 cache with BF16 queries the shared tokens' weights enter the product as one f16 term, off by half a step,
+    2^-11 of themselves: 2^-11 of the mean |v| more, which check_attn counts as twice `weights`.  lse knows nothing of it."""
+    one_term = s["dtype"] == BF16 and s["cache"] in (E4M3, E5M2)
+    check_attn(s, got, want, 1e-4 + 2.0 ** -12 if one_term else 1e-4)
+    some = np.isfinite(want[1])
+    assert (np.abs(got[1][some] - want[1][some]) <= 1e-4 + 2.0 ** -22 * np.abs(want[1][some])).all()
+
+
 class Running:
     """The case on the device."""
 
@@ -88,7 +99,6 @@ class Running:
 
 
 def run_groups(groups, hq=4, hkv=2, dim=64, page=16, order="HND", dtype=BF16, cache=None, seed=7, alone=0, q_pad=0, stream=None, **rules):
-    """The bounds are those of the attention without sharing: the join adds float32 products of weights that are good to 2^-22."""
     s = make_groups(groups, hq, hkv, dim, page, order, dtype, dtype if cache is None else cache, seed, alone)
     on = Running(s, q_pad=q_pad, **rules)
     device_status()
@@ -96,7 +106,7 @@ def run_groups(groups, hq=4, hkv=2, dim=64, page=16, order="HND", dtype=BF16, ca
     again = on.run(stream)
     assert device_status() == 0
     on.close()
-    check_attn(s, got, want_attn(s, **rules))
+    check_prefix(s, got, want_attn(s, **rules))
     bits_equal(got[0], again[0])
     bits_equal(got[1].view(np.uint32), again[1].view(np.uint32))
 
@@ -240,7 +250,7 @@ def test_prefix_page_outside_the_cache_is_masked_and_reported(backend):
         t = dict(s)
         t["table"] = np.delete(s["table"], 3, 1)
         t["lens"] = s["lens"] - 16
-        check_attn(t, got, want_attn(t))
+        check_prefix(t, got, want_attn(t))
 
 
 @pytest.mark.parametrize("starts", [[0, 3, 2, 6], [0, 2, 4, 7], [-1, 2, 4, 6], [0, 2 ** 31 - 1, 2, 6]])
@@ -252,7 +262,7 @@ def test_prefix_groups_that_are_none_share_nothing(backend, starts):
     got = on.run()
     assert device_status() == 0x7300
     on.close()
-    check_attn(s, got, want_attn(s))
+    check_prefix(s, got, want_attn(s))
 
 
 def test_prefix_shared_past_the_table_or_negative(backend):
@@ -265,7 +275,7 @@ def test_prefix_shared_past_the_table_or_negative(backend):
     got = on.run()
     assert device_status() == 0
     on.close()
-    check_attn(s, got, want_attn(s))
+    check_prefix(s, got, want_attn(s))
 
 
 @pytest.mark.parametrize("dtype,cache", [(BF16, BF16), (F16, F16), (F16, E4M3), (BF16, E4M3)])
@@ -291,7 +301,7 @@ def test_prefix_small_weights_beside_a_dominant_one(backend, dtype, cache, lead)
     on = Running(s, scale=1.0)
     got = on.run()
     on.close()
-    check_attn(s, got, want_attn(s, scale=1.0))
+    check_prefix(s, got, want_attn(s, scale=1.0))
 
 
 def test_prefix_handle_serves_any_batch(backend):
@@ -314,7 +324,7 @@ def test_prefix_handle_serves_any_batch(backend):
             on.bufs[3].free()
             on.bufs[3] = to_device(wide)
         assert s["pages"] <= first["pages"]
-        check_attn(s, on.run(), want_attn(s))
+        check_prefix(s, on.run(), want_attn(s))
         for b in (*on.bufs, *on.extra, on.out, on.lse):
             b.free()
     h.close()
@@ -343,7 +353,7 @@ def test_prefix_two_handles_on_two_streams(backend):
     sync_device()
     for o, s in zip(on, cases):
         out = fetch(o.out, 30 * 8 * 128 * 2, np.uint16).reshape(30, 8, 128)
-        check_attn(s, (out, fetch(o.lse, 30 * 8 * 4, np.float32).reshape(30, 8)), want_attn(s))
+        check_prefix(s, (out, fetch(o.lse, 30 * 8 * 4, np.float32).reshape(30, 8)), want_attn(s))
         o.close()
     for st in streams:
         st.close()
