@@ -36,7 +36,7 @@
 namespace mf {
 namespace {
 
-// What the join needs of a request's group: the place of its first tile, tiles of an item (0: nothing is shared), its first
+// What the join needs of a request's group: the place of its first item, tiles of an item (0: nothing is shared), its first
 // request and its requests.
 struct Shared {
     int32_t base, tiles, start, members;
@@ -67,7 +67,7 @@ struct PrefixArgs {
     // workspace
     int32_t* own_first;   // [requests]
     Shared* info;         // [requests]
-    int2* cut;            // tiles of all items, CTAs that they are cut for
+    int2* cut;            // places of all items, CTAs that they are cut for
     float* part;          // [2][requests][q_heads][head_dim]: an item's first CTA, its two halves
     float2* part_ml;      // [2][requests][q_heads]
     float* cta_part;      // [CTAs][2][128][head_dim]: a CTA that begins inside an item
@@ -174,8 +174,8 @@ struct Prefix {
     static constexpr int kPanels = DP / 64;              // of 64 elements (128 bytes) of a row
     static constexpr int kUnit = T * DP * 2;             // bytes of a tile's keys, or values
     static constexpr int kQ = 128 * DP * 2;              // of 128 rows of queries
-    static constexpr int kStages = (DP == 64 ? 2 : 1) * (kFp8 ? 3 : 5);  // units of the ring
-    static constexpr int kRaw = kFp8 ? 4 : 0;            // units of FP8 codes on their way
+    static constexpr int kStages = (DP == 64 ? 2 : 1) * (kFp8 ? 4 : 5);  // units of the ring
+    static constexpr int kRaw = !kFp8 ? 0 : DP == 64 ? 4 : 2;  // units of FP8 codes on their way
     static constexpr int kRing = kStages * kUnit + kRaw * (kUnit / 2);
     static constexpr int kRows = 128 * kStreams;         // of a block
     static constexpr int kO = 2 * T;                     // columns of tensor memory: S of even and odd steps, then O
@@ -214,48 +214,69 @@ __device__ __forceinline__ int64_t items_of(const PrefixArgs& a, const Group& x)
     return (static_cast<int64_t>(x.members) * a.group.d + K::kRows - 1) / K::kRows * a.kv_heads;
 }
 
+// What an item costs a CTA besides its tiles, in tiles: its queries into shared memory, an empty pipeline, and its part out of
+// tensor memory.  An item is `tiles` + kItemCost places long where the row of all items is cut for the CTAs.
+constexpr int kItemCost = 4;
+
+template <class K>
+__device__ __forceinline__ int32_t places_of(const Group& x) {
+    const int32_t tiles = tiles_of<K>(x);
+    return tiles > 0 ? tiles + kItemCost : 0;
+}
+
 // A run of tiles of one item.  Every role walks the same runs.
 template <class K>
 struct Run {
     Group of;
-    int32_t g, tiles, items, item, t, left;
+    int32_t g, tiles, items, item, at, left;  // at: the run's place in its item; left: places from there on
     // of the item at hand
-    int32_t n, kv, block, rows;  // tiles of the run in it; its key-value head, block of rows, rows
+    int32_t t, n, kv, block, rows;  // first tile of the run and how many; its key-value head, block of rows, rows
     __device__ __forceinline__ Run(const PrefixArgs& a, const Group& first, int32_t group, int32_t into, int32_t run)
         : of(first), g(group), left(run) {
         tiles = tiles_of<K>(of);
         items = static_cast<int32_t>(items_of<K>(a, of));
-        item = into / tiles;
-        t = into - item * tiles;
-        set(a);
+        item = into / (tiles + kItemCost);
+        at = into - item * (tiles + kItemCost);
+        n = 0;
+        if (!set(a)) next(a);
     }
-    __device__ __forceinline__ void set(const PrefixArgs& a) {
+    // false: nothing but places that cost
+    __device__ __forceinline__ bool set(const PrefixArgs& a) {
+        const int32_t places = min(tiles + kItemCost - at, left);
+        t = max(at - kItemCost, 0);
+        n = max(at + places - kItemCost, 0) - t;
         const int32_t blocks = items / a.kv_heads;
         kv = item / blocks;
         block = item - kv * blocks;
         const int64_t after = static_cast<int64_t>(of.members) * a.group.d - static_cast<int64_t>(block) * K::kRows;
         rows = after < K::kRows ? static_cast<int32_t>(after) : K::kRows;
-        n = min(tiles - t, left);
+        at += places;
+        left -= places;
+        return n > 0;
     }
     // whether each softmax group has rows of its own; else they share the rows and take turns at the tiles
     __device__ __forceinline__ bool dual() const { return K::kStreams == 2 && rows > 128; }
     // among how many warps a row's tokens of a tile are shared out, where there are no rows for four
     __device__ __forceinline__ int32_t sharers() const { return rows <= 32 && K::T == 128 ? 4 : rows <= 64 ? 2 : 1; }
     __device__ __forceinline__ int32_t steps() const { return dual() ? 2 * n : n; }
+    // false: the run is over (and n is 0)
     __device__ __forceinline__ bool next(const PrefixArgs& a) {
-        left -= n;
-        if (left <= 0) return false;
-        t = 0;
-        if (++item == items) {
-            item = 0;
-            do {
-                of = group_of(a, ++g);
-                tiles = tiles_of<K>(of);
-            } while (tiles == 0 && g + 1 < a.n_groups);
-            items = static_cast<int32_t>(items_of<K>(a, of));
+        n = 0;
+        while (left > 0) {
+            if (at == tiles + kItemCost) {
+                at = 0;
+                if (++item == items) {
+                    item = 0;
+                    do {
+                        of = group_of(a, ++g);
+                        tiles = tiles_of<K>(of);
+                    } while (tiles == 0 && g + 1 < a.n_groups);
+                    items = static_cast<int32_t>(items_of<K>(a, of));
+                }
+            }
+            if (set(a)) return true;
         }
-        set(a);
-        return true;
+        return false;
     }
 };
 
@@ -292,7 +313,7 @@ template <class K>
 __device__ __forceinline__ void find_rows(const PrefixArgs& a, typename K::Shared& sh, Run<K> run) {
     const int lane = threadIdx.x & 31;
     uint32_t tile = 0;
-    bool more = true;
+    bool more = run.n > 0;
     while (more) {
         const int64_t at_row = static_cast<int64_t>(run.of.start) * a.table_stride;
         for (int32_t i = 0; i < run.n; ++i, ++tile) {
@@ -364,7 +385,7 @@ __device__ __forceinline__ void produce(const PrefixArgs& a, typename K::Shared&
         ++told;
     };
     constexpr uint32_t kAhead = K::kFp8 ? K::kRaw - 1 : K::kStages - 2;  // units on their way
-    bool more = true;
+    bool more = run.n > 0;
     while (more) {
         const char* keys = a.k + run.kv * a.head_bytes + piece * 16;
         for (int32_t i = 0; i < run.n; ++i, ++tile) {
@@ -432,7 +453,7 @@ __device__ __forceinline__ void multiply(const PrefixArgs& a, typename K::Shared
     const bool two = two_terms<K>(a);
     uint32_t unit = 0;                               // first unit of the item at hand
     uint32_t s_steps[2] = {0, 0}, o_steps[2] = {0, 0}, q_items[2] = {0, 0};
-    bool more = true;
+    bool more = run.n > 0;
     while (more) {
         const bool dual = run.dual();
         const int32_t steps = run.steps();
@@ -677,7 +698,7 @@ __device__ __forceinline__ void soften(const PrefixArgs& a, typename K::Shared& 
     const bool two = two_terms<K>(a);
     Row row;
     row.cap = a.softcap * kLog2e;
-    bool more = true;
+    bool more = run.n > 0;
     while (more) {
         const bool dual = run.dual();
         const int32_t steps = run.steps(), sharers = dual ? 1 : run.sharers(), apart = 4 / sharers;  // warps of different rows
@@ -701,44 +722,63 @@ __device__ __forceinline__ void soften(const PrefixArgs& a, typename K::Shared& 
             constexpr int kBatch = 8;
 #pragma unroll 1
             for (int i0 = 0; i0 < 32 / kAtOnce; i0 += kBatch) {
-                uint4 batch[kBatch];
+                uint32_t batch[kBatch][4];
 #pragma unroll
                 for (int i = 0; i < kBatch; ++i) {
                     const char* q = a.q + 2 * (__shfl_sync(0xffffffffu, q_of, (i0 + i) * kAtOnce + lane / kLanes) + (has ? c * 8 : 0));
                     if (a.q_wide) {
-                        batch[i] = *reinterpret_cast<const uint4*>(q);
+                        const uint4 v = *reinterpret_cast<const uint4*>(q);
+                        batch[i][0] = v.x, batch[i][1] = v.y, batch[i][2] = v.z, batch[i][3] = v.w;
                     } else {
-                        const uint32_t* w = reinterpret_cast<const uint32_t*>(q);
-                        batch[i] = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) batch[i][x] = reinterpret_cast<const uint32_t*>(q)[x];
                     }
                 }
 #pragma unroll
                 for (int i = 0; i < kBatch; ++i) {
-                    const int j = (i0 + i) * kAtOnce + lane / kLanes;
-                    const bool there = __shfl_sync(0xffffffffu, valid, j) && has;
-                    uint32_t w[4] = {there ? batch[i].x : 0u, there ? batch[i].y : 0u, there ? batch[i].z : 0u, there ? batch[i].w : 0u};
-                    if constexpr (K::kFp8) {
-                        // f16 queries, scaled by a power of two to a largest magnitude in [1, 2)
-                        float f[8], top = 0.0f;
+                    const bool there = __shfl_sync(0xffffffffu, valid, (i0 + i) * kAtOnce + lane / kLanes) && has;
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) batch[i][x] = there ? batch[i][x] : 0u;
+                }
+                if constexpr (K::kFp8) {
+                    // f16 queries, scaled by a power of two to a largest magnitude in [1, 2)
+                    float top[kBatch];
+#pragma unroll
+                    for (int i = 0; i < kBatch; ++i) {
+                        top[i] = 0.0f;
 #pragma unroll
                         for (int x = 0; x < 4; ++x) {
-                            if (a.q_f16) unpack2<false>(w[x], f[2 * x], f[2 * x + 1]);
-                            else unpack2<true>(w[x], f[2 * x], f[2 * x + 1]);
-                            top = fmaxf(top, fmaxf(fabsf(f[2 * x]), fabsf(f[2 * x + 1])));
+                            float f0, f1;
+                            if (a.q_f16) unpack2<false>(batch[i][x], f0, f1);
+                            else unpack2<true>(batch[i][x], f0, f1);
+                            top[i] = fmaxf(top[i], fmaxf(fabsf(f0), fabsf(f1)));
                         }
+                    }
 #pragma unroll
-                        for (int d = 1; d < kLanes; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                        const uint32_t field = __float_as_uint(top) >> 23;  // biased exponent
+                    for (int d = 1; d < kLanes; d <<= 1)
+#pragma unroll
+                        for (int i = 0; i < kBatch; ++i) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], d));
+#pragma unroll
+                    for (int i = 0; i < kBatch; ++i) {
+                        const uint32_t field = __float_as_uint(top[i]) >> 23;  // biased exponent
                         const bool scales = field >= 1 && field <= 254;
                         const uint32_t e = min(field, 253u);
                         const float fit = scales ? __uint_as_float((254u - e) << 23) : 1.0f, back = scales ? __uint_as_float(e << 23) : 1.0f;
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) w[x] = pack2<false>(f[2 * x] * fit, f[2 * x + 1] * fit);
+                        for (int x = 0; x < 4; ++x) {
+                            float f0, f1;
+                            if (a.q_f16) unpack2<false>(batch[i][x], f0, f1);
+                            else unpack2<true>(batch[i][x], f0, f1);
+                            batch[i][x] = pack2<false>(f0 * fit, f1 * fit);
+                        }
                         const float mine = __shfl_sync(0xffffffffu, back, lane % kAtOnce * kLanes);
                         if (lane / kAtOnce == i0 + i) row.scale *= mine;
                     }
-                    *reinterpret_cast<uint4*>(my_q + place(128, warp * 32 + j, c)) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i)
+                    *reinterpret_cast<uint4*>(my_q + place(128, warp * 32 + (i0 + i) * kAtOnce + lane / kLanes, c)) =
+                        make_uint4(batch[i][0], batch[i][1], batch[i][2], batch[i][3]);
             }
             fence_proxy();
             __syncwarp();
@@ -784,9 +824,10 @@ __device__ __forceinline__ void soften(const PrefixArgs& a, typename K::Shared& 
         // This CTA's part of the rows, through the place of the queries, with which the products are done: rows side by side, and the
         // warps that share rows joined.
         const bool has = steps > stream, first = run.t == 0;
-        const int64_t at = first ? (static_cast<int64_t>(dual ? 0 : stream) * a.n_requests + r) * a.q_heads + h
-                                 : (static_cast<int64_t>(blockIdx.x) * 2 + stream) * 128 + my_row;
-        float2* ml_to = (first ? a.part_ml : a.cta_ml) + at;
+        const int64_t row0 = first ? (static_cast<int64_t>(dual ? 0 : stream) * a.n_requests + run.of.start) * a.q_heads +
+                                         static_cast<int64_t>(run.kv) * run.of.members * a.group.d + run.block * K::kRows + (dual ? 128 * stream : 0)
+                                   : (static_cast<int64_t>(blockIdx.x) * 2 + stream) * 128;
+        float2* ml_to = (first ? a.part_ml : a.cta_ml) + row0 + my_row;
         if (!has) {
             if (valid && my_share == 0) *ml_to = make_float2(-INFINITY, 0.0f);
         } else {
@@ -813,9 +854,10 @@ __device__ __forceinline__ void soften(const PrefixArgs& a, typename K::Shared& 
                 asm volatile("bar.sync %0, 128;" ::"r"(2 + stream) : "memory");
             }
             if (valid && my_share == 0) *ml_to = make_float2(top, sum);
-            const float* to = (first ? a.part : a.cta_part) + at * a.head_dim;
+            // of this warp's set of rows the share of this warp, four rows at a time: a lane's row and elements
+            const int own = my_share * (32 / sharers) + (lane >> 3), piece = lane & 7;
+            float* to = (first ? a.part : a.cta_part) + (row0 + set * 32 + own) * a.head_dim + piece * 4;
             float4* lines = reinterpret_cast<float4*>(my_q);  // [128][8], pieces exchanged
-            const int piece = lane & 7;
 #pragma unroll 1
             for (int c = 0; c < a.head_dim; c += 32) {
                 uint32_t v[32];
@@ -829,18 +871,19 @@ __device__ __forceinline__ void soften(const PrefixArgs& a, typename K::Shared& 
                 }
                 if (sharers > 1) asm volatile("bar.sync %0, 128;" ::"r"(2 + stream) : "memory");
                 else __syncwarp();
-                // of this warp's set of rows the share of this warp, four rows at a time
-#pragma unroll 2
-                for (int i = 0; i < 8 / sharers; ++i) {
-                    const int j = (my_share * (8 / sharers) + i) * 4 + (lane >> 3);
-                    float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    for (int x = 0; x < sharers; ++x) {
-                        const float4 g = lines[((x * apart + set) * 32 + j) * 8 + (piece ^ (j & 7))];
-                        f = make_float4(f.x + g.x, f.y + g.y, f.z + g.z, f.w + g.w);
-                    }
-                    float* there = const_cast<float*>(reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(to), j)));
-                    const bool is = __shfl_sync(0xffffffffu, valid, j);
-                    if (is && c + piece * 4 < a.head_dim) *reinterpret_cast<float4*>(there + c + piece * 4) = f;
+                const bool in = c + piece * 4 < a.head_dim;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    if (i * 4 >= 32 / sharers) break;
+                    const int j = own + i * 4;
+                    float4 f = lines[(set * 32 + j) * 8 + (piece ^ (j & 7))];
+#pragma unroll
+                    for (int x = 1; x < 4; ++x)
+                        if (x < sharers) {
+                            const float4 g = lines[((x * apart + set) * 32 + j) * 8 + (piece ^ (j & 7))];
+                            f = make_float4(f.x + g.x, f.y + g.y, f.z + g.z, f.w + g.w);
+                        }
+                    if (in && set * 32 + j < rows) *reinterpret_cast<float4*>(to + i * 4 * a.head_dim + c) = f;
                 }
                 if (sharers > 1) asm volatile("bar.sync %0, 128;" ::"r"(2 + stream) : "memory");
                 else __syncwarp();
@@ -868,7 +911,7 @@ __device__ __forceinline__ void take_notes(const PrefixArgs& a, bool bad) {
         const int32_t g = g0 + lane;
         Group x{0, 0, 0, false};
         if (g < a.n_groups) x = group_of(a, g);
-        const int64_t of = items_of<K>(a, x) * tiles_of<K>(x);
+        const int64_t of = items_of<K>(a, x) * places_of<K>(x);
         int64_t upto = of;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -935,7 +978,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const PrefixArgs a)
         if (g >= a.n_groups) break;
         last = group_of(a, g);
         bad |= last.bad;
-        mine += items_of<K>(a, last) * tiles_of<K>(last);
+        mine += items_of<K>(a, last) * places_of<K>(last);
     }
     int64_t upto = mine;
 #pragma unroll
@@ -976,7 +1019,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const PrefixArgs a)
             if (per > 1) {
                 for (;; ++g) {
                     last = group_of(a, g);
-                    const int64_t of = items_of<K>(a, last) * tiles_of<K>(last);
+                    const int64_t of = items_of<K>(a, last) * places_of<K>(last);
                     if (into < of) break;
                     into -= static_cast<int32_t>(of);
                 }
@@ -1048,9 +1091,9 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const PrefixArgs a) 
             const int32_t blocks = static_cast<int32_t>((rows + ROWS - 1) / ROWS), block = static_cast<int32_t>(nth / ROWS);
             halves = ROWS == 128 || rows - static_cast<int64_t>(block) * ROWS > 128 ? 1 : 2;
             const Cut cut(all.x, all.y);
-            const int32_t begin = x.base + (kv * blocks + block) * x.tiles, cta = cut.part_of(begin);
+            const int32_t begin = x.base + (kv * blocks + block) * (x.tiles + kItemCost) + kItemCost, cta = cut.part_of(begin);
             parts = (cut.part_of(begin + x.tiles - 1) - cta + 1) * halves;
-            first_at = w;
+            first_at = static_cast<int64_t>(x.start) * a.q_heads + kv * rows + nth;
             first_apart = n;
             at = static_cast<int64_t>(cta) * 256 + (nth - static_cast<int64_t>(block) * ROWS);
         }
