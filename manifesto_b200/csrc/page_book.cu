@@ -23,7 +23,8 @@ namespace {
 
 constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
-constexpr int kCluster = 8;                  // CTAs of a cluster, the portable most
+constexpr int kCluster = 8;                  // CTAs of a cluster, the portable most (16 were no faster)
+constexpr int64_t kClusterShare = 65536;     // entries that a CTA of a cluster has, at most
 constexpr int kMostCtas = 256;               // of a grid
 constexpr uint64_t kBarrierNs = 2000000000;  // after which a barrier in memory gives up
 
@@ -45,13 +46,13 @@ struct BookArgs {
     int32_t n_before, n_after, n_pages, max_pages, limit;
     Divisor page;
     // workspace
-    int32_t* first;      // [max_requests]: the first row that continues a row
+    unsigned long long* first;  // [max_requests]: the first row that continues a row, behind the number of the call
     int32_t* rank;       // [max_requests]: which of the new pages a row gets
     int32_t* list;       // [n_pages]: pages set free, or those that pages move to
     int32_t* list2;      // [n_pages]: pages that move
     uint32_t* bits;      // [n_pages / 32]: free pages
     int2* of_cta;        // [CTAs]: what each has counted
-    uint32_t* barrier;   // arrivals (zero between barriers), barriers passed
+    uint32_t* barrier;   // arrivals (zero between barriers), barriers passed; the number of the call; whether bits are zero
     int32_t* status;
 };
 
@@ -107,19 +108,6 @@ __device__ __forceinline__ int32_t warp_before(int32_t v, int lane) {
     return upto - v;
 }
 
-// The sum of `mine` over the threads in front of this one, and over all.  All threads; `room` is shared, kWarps entries.
-__device__ __forceinline__ int32_t cta_before(int32_t mine, int32_t* room, int32_t& total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int32_t before = warp_before(mine, lane);
-    __syncthreads();
-    if (lane == 31) room[warp] = before + mine;
-    __syncthreads();
-    const int32_t of_warp = room[lane];
-    static_assert(kWarps == 32, "a lane for each warp");
-    total = warp_sum(of_warp);
-    return before + __shfl_sync(0xffffffffu, warp_before(of_warp, lane), warp);
-}
-
 // What the CTAs in front of this one have counted, and all of them.
 __device__ __forceinline__ void ctas_before(const BookArgs& a, int2& before, int2& all) {
     const int lane = threadIdx.x & 31;
@@ -137,9 +125,10 @@ __device__ __forceinline__ void ctas_before(const BookArgs& a, int2& before, int
     all = make_int2(warp_sum(all.x), warp_sum(all.y));
 }
 
-// This CTA's share of n things, a multiple of 32 each.
+// This CTA's share of n things, a multiple of OF each.
+template <int OF>
 __device__ __forceinline__ void share_of(int32_t n, int32_t& begin, int32_t& end) {
-    const int64_t each = (static_cast<int64_t>(n) + 32 * gridDim.x - 1) / (32 * gridDim.x) * 32;
+    const int64_t each = (static_cast<int64_t>(n) + OF * gridDim.x - 1) / (OF * gridDim.x) * OF;
     const int64_t b = each * blockIdx.x, e = b + each;
     begin = static_cast<int32_t>(b < n ? b : n);
     end = static_cast<int32_t>(e < n ? e : n);
@@ -166,58 +155,117 @@ __device__ __forceinline__ uint32_t row_held(const BookArgs& a, uint32_t len) {
     return full + (full * a.page.d != len);
 }
 
+// This warp's share of [begin, end), a multiple of OF each; all warps' together are the CTA's, in order.
+template <int OF>
+__device__ __forceinline__ void warp_share(int32_t begin, int32_t end, int32_t& from, int32_t& to) {
+    const int32_t each = ((end - begin + OF * kWarps - 1) / (OF * kWarps)) * OF, warp = threadIdx.x >> 5;
+    from = min(end, begin + each * warp);
+    to = min(end, from + each);
+}
+
+// The sum of what the warps in front of this one counted (`room`, kWarps entries, filled before a barrier), and of all.
+__device__ __forceinline__ int32_t warps_before(const int32_t* room, int32_t& total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int32_t of_warp = room[lane];
+    static_assert(kWarps == 32, "a lane for each warp");
+    total = warp_sum(of_warp);
+    return __shfl_sync(0xffffffffu, warp_before(of_warp, lane), warp);
+}
+
+constexpr int kEach = 4;  // loads that a thread has on their way
+
 template <bool GRID>
 __global__ void __launch_bounds__(kThreads, 1) fork_kernel(const BookArgs a) {
-    __shared__ int32_t room[kWarps];
+    __shared__ int32_t freed_of[kWarps], needy_of[kWarps];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int32_t step = gridDim.x * kThreads, me = blockIdx.x * kThreads + tid;
     const int32_t warps = gridDim.x * kWarps, my_warp = blockIdx.x * kWarps + warp;
-    constexpr int32_t kNobody = 0x7fffffff;
+    constexpr int32_t kNobody = 0x7fffffff, kWide = 32 * kEach;  // columns of a row that a warp has at a time
+    const int32_t segments = (a.max_pages + kWide - 1) / kWide;
     after_previous();
     let_next_start();
+    const uint32_t call = a.barrier[2];
     int32_t head, count;
     pool_of(a, head, count);
-    for (int32_t i = me; i < a.n_pages; i += step) a.shares_after[i] = a.shares[i];
-    for (int32_t i = me; i < a.n_before; i += step) a.first[i] = kNobody;
-    if (!all_sync<GRID>(a)) return;
+    for (int64_t i0 = me; i0 < a.n_pages; i0 += static_cast<int64_t>(kEach) * step) {
+        int32_t v[kEach];
+#pragma unroll
+        for (int u = 0; u < kEach; ++u) v[u] = i0 + u * static_cast<int64_t>(step) < a.n_pages ? a.shares[i0 + u * static_cast<int64_t>(step)] : 0;
+#pragma unroll
+        for (int u = 0; u < kEach; ++u)
+            if (i0 + u * static_cast<int64_t>(step) < a.n_pages) a.shares_after[i0 + u * static_cast<int64_t>(step)] = v[u];
+    }
     auto parent_of = [&](int32_t r) {
         const int32_t p = a.parents[r];
         return p >= 0 && p < a.n_before ? p : -1;
     };
     for (int32_t r = me; r < a.n_after; r += step) {
         const int32_t p = parent_of(r);
-        if (p >= 0) atomicMin(a.first + p, r);
+        if (p >= 0) atomicMax(a.first + p, static_cast<unsigned long long>(call) << 32 | static_cast<uint32_t>(kNobody - r));
     }
-    if (!all_sync<GRID>(a)) return;
+    const bool met = all_sync<GRID>(a);
+    if (me == 0 || !met) atomicAdd(a.barrier + 2, 1u);  // every CTA knows this call's number: the next one has another
+    if (!met) return;
+    // the first row that continues row p, kNobody if there is none: what earlier calls left does not count
+    auto first_of = [&](int32_t p) {
+        const unsigned long long v = a.first[p];
+        return static_cast<uint32_t>(v >> 32) == call ? kNobody - static_cast<int32_t>(static_cast<uint32_t>(v)) : kNobody;
+    };
     // rows that nobody continues let go of their pages
-    for (int32_t r = my_warp; r < a.n_before; r += warps) {
-        if (a.first[r] != kNobody) continue;
+    for (int64_t w = my_warp; w < static_cast<int64_t>(a.n_before) * segments; w += warps) {
+        const int32_t r = static_cast<int32_t>(w / segments), c0 = static_cast<int32_t>(w - static_cast<int64_t>(r) * segments) * kWide + lane;
+        if (first_of(r) != kNobody) continue;
         const int32_t held = row_held(a, row_len(a, r));
-        for (int32_t c = lane; c < held; c += 32) {
-            const int32_t x = a.table[r * a.table_stride + c];
-            if (x >= 0 && x < a.n_pages) atomicSub(a.shares_after + x, 1);
+        int32_t x[kEach];
+#pragma unroll
+        for (int u = 0; u < kEach; ++u) x[u] = c0 + u * 32 < held ? a.table[r * a.table_stride + c0 + u * 32] : 0;
+#pragma unroll
+        for (int u = 0; u < kEach; ++u) {
+            if (c0 + u * 32 >= held) continue;
+            if (x[u] >= 0 && x[u] < a.n_pages) atomicSub(a.shares_after + x[u], 1);
             else atomicExch(a.status, MF_DEVICE_BAD_PAGE);
         }
     }
-    if (!all_sync<GRID>(a)) return;
-    // count the pages set free and the rows that need one
-    auto needs = [&](int32_t r) {
-        const int32_t p = parent_of(r);
-        if (p < 0 || a.first[p] == r) return false;
-        const uint32_t len = row_len(a, p);
-        return len / a.page * a.page.d != len;
-    };
+    // rows that need a page: marked, and counted
     int32_t page0, page1, row0, row1;
-    share_of(a.n_pages, page0, page1);
-    share_of(a.n_after, row0, row1);
     {
-        int32_t freed = 0, need = 0, total;
-        for (int32_t i = page0 + tid; i < page1; i += kThreads) freed += a.shares_after[i] < 0;
-        for (int32_t r = row0 + tid; r < row1; r += kThreads) need += needs(r);
-        cta_before(freed, room, total);
-        const int32_t all_freed = total;
-        cta_before(need, room, total);
-        if (tid == 0) a.of_cta[blockIdx.x] = make_int2(all_freed, total);
+        int32_t begin, end;
+        share_of<32>(a.n_after, begin, end);
+        warp_share<32>(begin, end, row0, row1);
+        share_of<32>(a.n_pages, begin, end);
+        warp_share<32>(begin, end, page0, page1);
+    }
+    {
+        int32_t needy = 0;
+        for (int32_t r = row0 + lane; r < row1; r += 32) {
+            const int32_t p = parent_of(r);
+            bool is = p >= 0 && first_of(p) != r;
+            if (is) {
+                const uint32_t len = row_len(a, p);
+                is = len / a.page * a.page.d != len;
+            }
+            a.rank[r] = is ? 0 : -1;
+            needy += is;
+        }
+        needy = warp_sum(needy);
+        if (lane == 0) needy_of[warp] = needy;
+    }
+    if (!all_sync<GRID>(a)) return;
+    // pages set free
+    {
+        int32_t freed = 0;
+#pragma unroll 4
+        for (int32_t i = page0 + lane; i < page1; i += 32) freed += a.shares_after[i] < 0;
+        freed = warp_sum(freed);
+        if (lane == 0) freed_of[warp] = freed;
+    }
+    __syncthreads();
+    int32_t my_freed, my_needy;
+    {
+        int32_t all_freed, all_needy;
+        my_freed = warps_before(freed_of, all_freed);
+        my_needy = warps_before(needy_of, all_needy);
+        if (tid == 0) a.of_cta[blockIdx.x] = make_int2(all_freed, all_needy);
     }
     if (!all_sync<GRID>(a)) return;
     int2 before, all;
@@ -229,27 +277,34 @@ __global__ void __launch_bounds__(kThreads, 1) fork_kernel(const BookArgs a) {
     auto put_free = [&](int64_t x, int32_t page) {
         if (x >= taken && x - taken < a.n_pages) a.free_after[x - taken] = page;
     };
-    for (int32_t i0 = page0, base = before.x; i0 < page1; i0 += kThreads) {
-        const int32_t i = i0 + tid;
+#pragma unroll 2
+    for (int32_t i0 = page0, base = before.x + my_freed; i0 < page1; i0 += 32) {
+        const int32_t i = i0 + lane;
         const bool is = i < page1 && a.shares_after[i] < 0;
-        int32_t total;
-        const int32_t x = base + cta_before(is, room, total);
-        base += total;
+        const uint32_t some = __ballot_sync(0xffffffffu, is);
         if (is) {
+            const int32_t x = base + __popc(some & ((1u << lane) - 1u));
             a.shares_after[i] = 0;
             a.list[x] = i;
             put_free(x, i);
         }
+        base += __popc(some);
     }
-    for (int32_t r0 = row0, base = before.y; r0 < row1; r0 += kThreads) {
-        const int32_t r = r0 + tid;
-        const bool is = r < row1 && needs(r);
-        int32_t total;
-        const int32_t x = base + cta_before(is, room, total);
-        base += total;
-        if (r < row1) a.rank[r] = is ? x : -1;
+    for (int32_t r0 = row0, base = before.y + my_needy; r0 < row1; r0 += 32) {
+        const int32_t r = r0 + lane;
+        const bool is = r < row1 && a.rank[r] >= 0;
+        const uint32_t some = __ballot_sync(0xffffffffu, is);
+        if (is) a.rank[r] = base + __popc(some & ((1u << lane) - 1u));
+        base += __popc(some);
     }
-    for (int32_t i = me; i < count; i += step) put_free(static_cast<int64_t>(freed) + i, a.free_pages[head + i]);
+    for (int64_t i0 = me; i0 < count; i0 += static_cast<int64_t>(kEach) * step) {
+        int32_t v[kEach];
+#pragma unroll
+        for (int u = 0; u < kEach; ++u) v[u] = i0 + u * static_cast<int64_t>(step) < count ? a.free_pages[head + i0 + u * static_cast<int64_t>(step)] : 0;
+#pragma unroll
+        for (int u = 0; u < kEach; ++u)
+            if (i0 + u * static_cast<int64_t>(step) < count) put_free(freed + i0 + u * static_cast<int64_t>(step), v[u]);
+    }
     if (me == 0) {
         const int64_t left = there - taken;
         if (left > a.n_pages) atomicExch(a.status, MF_DEVICE_BAD_PAGE);
@@ -260,33 +315,38 @@ __global__ void __launch_bounds__(kThreads, 1) fork_kernel(const BookArgs a) {
     }
     if (!all_sync<GRID>(a)) return;
     // the rows
-    for (int32_t r = my_warp; r < a.n_after; r += warps) {
+    for (int64_t w = my_warp; w < static_cast<int64_t>(a.n_after) * segments; w += warps) {
+        const int32_t r = static_cast<int32_t>(w / segments), segment = static_cast<int32_t>(w - static_cast<int64_t>(r) * segments);
         const int32_t p = parent_of(r), x = a.rank[r];
         const bool lives = p >= 0 && x < taken;
         const uint32_t len = lives ? row_len(a, p) : 0;
-        const int32_t held = row_held(a, len), full = len / a.page;
-        const bool further = lives && a.first[p] != r;
+        const int32_t held = row_held(a, len), full = len / a.page, c0 = segment * kWide + lane;
+        int32_t number[kEach];
+#pragma unroll
+        for (int u = 0; u < kEach; ++u) number[u] = c0 + u * 32 < held ? a.table[p * a.table_stride + c0 + u * 32] : -1;
+        const bool further = lives && first_of(p) != r;
         const int32_t mine = lives && x >= 0 ? (x < freed ? a.list[x] : a.free_pages[head + (x - freed)]) : -1;
-        for (int32_t c = lane; c < a.max_pages; c += 32) {
-            int32_t number = c < held ? a.table[p * a.table_stride + c] : -1;
+#pragma unroll
+        for (int u = 0; u < kEach; ++u) {
+            const int32_t c = c0 + u * 32;
             if (c < held && further) {
                 if (c < full) {
-                    if (number >= 0 && number < a.n_pages) atomicAdd(a.shares_after + number, 1);
+                    if (number[u] >= 0 && number[u] < a.n_pages) atomicAdd(a.shares_after + number[u], 1);
                     else atomicExch(a.status, MF_DEVICE_BAD_PAGE);
                 } else {
-                    a.moves[x] = mf_page_move{number, mine, static_cast<int32_t>(len - full * a.page.d), 0};
-                    number = mine;
+                    a.moves[x] = mf_page_move{number[u], mine, static_cast<int32_t>(len - full * a.page.d), 0};
+                    number[u] = mine;
                 }
             }
-            a.table_after[r * a.table_stride + c] = number;
+            if (c < a.max_pages) a.table_after[r * a.table_stride + c] = number[u];
         }
-        if (lane == 0) a.lens_after[r] = static_cast<int32_t>(len);
+        if (lane == 0 && segment == 0) a.lens_after[r] = static_cast<int32_t>(len);
     }
 }
 
 template <bool GRID>
 __global__ void __launch_bounds__(kThreads, 1) compact_kernel(const BookArgs a) {
-    __shared__ int32_t room[kWarps];
+    __shared__ int32_t free_of[kWarps], below_of[kWarps];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int32_t step = gridDim.x * kThreads, me = blockIdx.x * kThreads + tid;
     const int32_t warps = gridDim.x * kWarps, my_warp = blockIdx.x * kWarps + warp;
@@ -295,63 +355,98 @@ __global__ void __launch_bounds__(kThreads, 1) compact_kernel(const BookArgs a) 
     int32_t head, count;
     pool_of(a, head, count);
     const int32_t words = (a.n_pages + 31) / 32;
-    for (int32_t i = me; i < words; i += step) a.bits[i] = 0;
-    if (!all_sync<GRID>(a)) return;
-    for (int32_t i = me; i < count; i += step) {
-        const int32_t x = a.free_pages[head + i];
-        const bool in = x >= 0 && x < a.n_pages;
-        if (!in || (atomicOr(a.bits + x / 32, 1u << (x & 31)) >> (x & 31) & 1u)) atomicExch(a.status, MF_DEVICE_BAD_PAGE);
+    // bits are zero, but after a call that gave up
+    if (a.barrier[3] == 0) {
+        for (int32_t i = me; i < words; i += step) a.bits[i] = 0;
+        if (!all_sync<GRID>(a)) return;
+    }
+    for (int64_t i0 = me; i0 < count; i0 += static_cast<int64_t>(kEach) * step) {
+        int32_t x[kEach];
+        bool in[kEach];
+#pragma unroll
+        for (int u = 0; u < kEach; ++u) {
+            in[u] = i0 + u * static_cast<int64_t>(step) < count;
+            x[u] = in[u] ? a.free_pages[head + i0 + u * static_cast<int64_t>(step)] : 0;
+        }
+#pragma unroll
+        for (int u = 0; u < kEach; ++u) {
+            if (!in[u]) continue;
+            if (x[u] >= 0 && x[u] < a.n_pages) atomicOr(a.bits + x[u] / 32, 1u << (x[u] & 31));
+            else atomicExch(a.status, MF_DEVICE_BAD_PAGE);
+        }
     }
     if (!all_sync<GRID>(a)) return;
-    int32_t word0, word1;
-    share_of(words, word0, word1);
+    if (me == 0) a.barrier[3] = 0;
+    int32_t begin, end, word0, word1;
+    share_of<1>(words, begin, end);
+    warp_share<1>(begin, end, word0, word1);
     {
-        int32_t mine = 0, total;
-        for (int32_t i = word0 + tid; i < word1; i += kThreads) mine += __popc(a.bits[i]);
-        cta_before(mine, room, total);
-        if (tid == 0) a.of_cta[blockIdx.x] = make_int2(total, 0);
+        int32_t mine = 0;
+#pragma unroll 4
+        for (int32_t i = word0 + lane; i < word1; i += 32) mine += __popc(a.bits[i]);
+        mine = warp_sum(mine);
+        if (lane == 0) free_of[warp] = mine;
     }
+    __syncthreads();
+    int32_t of_all, my_free = warps_before(free_of, of_all);
+    if (tid == 0) a.of_cta[blockIdx.x] = make_int2(of_all, 0);
     if (!all_sync<GRID>(a)) return;
     int2 before, all;
     ctas_before(a, before, all);
     const int32_t n_free = all.x, used = a.n_pages - n_free;
+    if (me == 0 && n_free != count) atomicExch(a.status, MF_DEVICE_BAD_PAGE);  // a page twice, or one outside the cache
     const int32_t limit = min(max(a.limit, used), a.n_pages);
-    // free pages below the limit, and the pages in use from it on: those move
-    int32_t below = 0;
+    // free pages below the limit, and the pages in use from it on: those move.  The CTA at whose words the limit lies counts
+    // again what of them is below; the others count alike.
+    int32_t below;
     {
+        const int64_t each = (static_cast<int64_t>(words) + gridDim.x - 1) / gridDim.x;
+        const int32_t last = limit / 32, at = static_cast<int32_t>(last / each);
         int32_t mine = 0;
-        for (int32_t i = tid; i <= limit / 32 && i < words; i += kThreads)
-            mine += __popc(i < limit / 32 ? a.bits[i] : a.bits[i] & ((1u << (limit & 31)) - 1u));
-        cta_before(mine, room, below);
+        for (int32_t i = static_cast<int32_t>(at * each) + tid; i <= last && i < words; i += kThreads)
+            mine += __popc(i < last ? a.bits[i] : a.bits[i] & ((1u << (limit & 31)) - 1u));
+        for (int c = tid; c < at; c += kThreads) mine += a.of_cta[c].x;
+        mine = warp_sum(mine);
+        if (lane == 0) below_of[warp] = mine;
+        __syncthreads();
+        warps_before(below_of, below);
     }
     const int32_t moving = (a.n_pages - limit) - (n_free - below);
-    for (int32_t w0 = word0, base = before.x; w0 < word1; w0 += kWarps) {
-        // a warp for each word, a lane for each page
-        const int32_t w = w0 + warp;
-        const uint32_t word = w < word1 ? a.bits[w] : 0u;
-        __syncthreads();
-        if (lane == 0) room[warp] = __popc(word);
-        __syncthreads();
-        const int32_t of_warp = room[lane], in_front = warp_before(of_warp, lane);
-        const int32_t free_before = base + __shfl_sync(0xffffffffu, in_front, warp) + __popc(word & ((1u << lane) - 1u));
-        base += warp_sum(of_warp);
-        const int32_t i = w * 32 + lane;
-        if (w >= word1 || i >= a.n_pages) continue;
-        const bool is_free = word >> lane & 1u;
-        if (i >= limit) {
-            a.free_after[below - moving + (i - limit)] = i;
-            a.shares_after[i] = 0;
-            if (is_free) a.numbers[i] = i;
-            else a.list2[(i - limit) - (free_before - below)] = i;
-        } else {
-            a.numbers[i] = i;
-            if (!is_free) {
-                a.shares_after[i] = a.shares[i];
-            } else if (free_before < moving) {
-                a.list[free_before] = i;
-            } else {
-                a.free_after[free_before - moving] = i;
-                a.shares_after[i] = 0;
+    int32_t free_before0 = before.x + my_free;
+    for (int32_t w0 = word0; w0 < word1; w0 += 32) {
+        const uint32_t held = w0 + lane < word1 ? a.bits[w0 + lane] : 0u;
+        const int32_t here = min(32, word1 - w0);
+        for (int k0 = 0; k0 < here; k0 += kEach) {
+            int32_t shares[kEach];
+#pragma unroll
+            for (int u = 0; u < kEach; ++u) {
+                const int32_t i = (w0 + k0 + u) * 32 + lane;
+                shares[u] = k0 + u < here && i < a.n_pages && i < limit ? a.shares[i] : 0;
+            }
+#pragma unroll
+            for (int u = 0; u < kEach; ++u) {
+                const uint32_t word = __shfl_sync(0xffffffffu, held, min(k0 + u, 31));
+                const int32_t i = (w0 + k0 + u) * 32 + lane, free_before = free_before0 + __popc(word & ((1u << lane) - 1u));
+                if (k0 + u >= here) continue;
+                free_before0 += __popc(word);
+                if (i >= a.n_pages) continue;
+                const bool is_free = word >> lane & 1u;
+                if (i >= limit) {
+                    a.free_after[below - moving + (i - limit)] = i;
+                    a.shares_after[i] = 0;
+                    if (is_free) a.numbers[i] = i;
+                    else a.list2[(i - limit) - (free_before - below)] = i;
+                } else {
+                    a.numbers[i] = i;
+                    if (!is_free) {
+                        a.shares_after[i] = shares[u];
+                    } else if (free_before < moving) {
+                        a.list[free_before] = i;
+                    } else {
+                        a.free_after[free_before - moving] = i;
+                        a.shares_after[i] = 0;
+                    }
+                }
             }
         }
     }
@@ -362,6 +457,7 @@ __global__ void __launch_bounds__(kThreads, 1) compact_kernel(const BookArgs a) 
         a.pool_after[3] = 0;
     }
     if (!all_sync<GRID>(a)) return;
+    for (int32_t i = me; i < words; i += step) a.bits[i] = 0;
     for (int32_t j = me; j < moving; j += step) {
         const int32_t src = a.list2[j], dst = a.list[j];
         a.numbers[src] = dst;
@@ -369,16 +465,24 @@ __global__ void __launch_bounds__(kThreads, 1) compact_kernel(const BookArgs a) 
         a.moves[j] = mf_page_move{src, dst, static_cast<int32_t>(a.page.d), 0};
     }
     if (!all_sync<GRID>(a)) return;
-    for (int32_t r = my_warp; r < a.n_before; r += warps) {
+    if (me == 0) a.barrier[3] = 1;
+    constexpr int32_t kWide = 32 * kEach;
+    const int32_t segments = (a.max_pages + kWide - 1) / kWide;
+    for (int64_t w = my_warp; w < static_cast<int64_t>(a.n_before) * segments; w += warps) {
+        const int32_t r = static_cast<int32_t>(w / segments), c0 = static_cast<int32_t>(w - static_cast<int64_t>(r) * segments) * kWide + lane;
         const int32_t held = row_held(a, row_len(a, r));
-        for (int32_t c = lane; c < a.max_pages; c += 32) {
-            int32_t number = c < held ? a.table[r * a.table_stride + c] : -1;
-            if (c < held) {
-                if (number >= 0 && number < a.n_pages) number = a.numbers[number];
-                else atomicExch(a.status, MF_DEVICE_BAD_PAGE);
-            }
-            a.table_after[r * a.table_stride + c] = number;
+        int32_t number[kEach];
+#pragma unroll
+        for (int u = 0; u < kEach; ++u) number[u] = c0 + u * 32 < held ? a.table[r * a.table_stride + c0 + u * 32] : -1;
+#pragma unroll
+        for (int u = 0; u < kEach; ++u) {
+            if (c0 + u * 32 >= held) continue;
+            if (number[u] >= 0 && number[u] < a.n_pages) number[u] = a.numbers[number[u]];
+            else atomicExch(a.status, MF_DEVICE_BAD_PAGE);
         }
+#pragma unroll
+        for (int u = 0; u < kEach; ++u)
+            if (c0 + u * 32 < a.max_pages) a.table_after[r * a.table_stride + c0 + u * 32] = number[u];
     }
 }
 
@@ -469,9 +573,9 @@ namespace {
 template <class Kernel>
 int launch_book(mf_page_book h, Kernel cluster_kernel, Kernel grid_kernel, const BookArgs& a, int64_t entries, cudaStream_t s,
                 const char* name) {
-    // a CTA for each 8 thousand entries; past a cluster's share the grid's slower barriers pay
-    int64_t ctas = (entries + 8191) / 8192;
-    if (ctas <= 4 * kCluster) {
+    // a CTA for each 4 thousand entries; past kClusterShare for each of a cluster the grid's slower barriers pay
+    int64_t ctas = (entries + 4095) / 4096;
+    if (entries <= kClusterShare * kCluster) {
         int n = 1;
         while (n < kCluster && n < ctas) n *= 2;
         cudaLaunchAttribute attr[2]{};
@@ -515,9 +619,9 @@ extern "C" int mf_page_book_create(const mf_page_book_config* config, mf_page_bo
     if (c.n_pages <= 0 || c.n_pages > most || c.max_requests <= 0 || c.max_requests > most)
         return fail(MF_ERR_SHAPE_INVALID, "mf_page_book_create: %d pages, %d requests (1 to %d)", c.n_pages, c.max_requests, most);
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-    const size_t rows = up(static_cast<size_t>(c.max_requests) * 4), pages = up(static_cast<size_t>(c.n_pages) * 4);
+    const size_t firsts = up(static_cast<size_t>(c.max_requests) * 8), rows = up(static_cast<size_t>(c.max_requests) * 4), pages = up(static_cast<size_t>(c.n_pages) * 4);
     const size_t bits = up((static_cast<size_t>(c.n_pages) + 31) / 32 * 4), counted = up(kMostCtas * sizeof(int2));
-    const size_t bytes = 256 + counted + 2 * rows + 2 * pages + bits;
+    const size_t cleared = 256 + firsts, bytes = cleared + counted + rows + 2 * pages + bits;
     mf_page_book_s* h = new (std::nothrow) mf_page_book_s{};
     if (!h) return fail(MF_ERR_ALLOCATOR_EXHAUSTED, "mf_page_book_create: out of host memory");
     cudaError_t err = cudaMalloc(&h->workspace, bytes);
@@ -528,7 +632,7 @@ extern "C" int mf_page_book_create(const mf_page_book_config* config, mf_page_bo
             return fail(MF_ERR_ALLOCATOR_EXHAUSTED, "mf_page_book_create: %zu bytes: out of device memory", bytes);
         return cuda_fail(err, "mf_page_book_create: cudaMalloc");
     }
-    err = cudaMemset(h->workspace, 0, 256);
+    err = cudaMemset(h->workspace, 0, cleared);
     if (err == cudaSuccess) err = cudaStreamSynchronize(nullptr);  // streams that do not wait for the default one may run it
     BookArgs& a = h->args;
     a.status = err == cudaSuccess ? sticky_status_ptr() : nullptr;
@@ -547,9 +651,9 @@ extern "C" int mf_page_book_create(const mf_page_book_config* config, mf_page_bo
     a.max_pages = c.max_pages;
     a.page = divisor(c.page_size);
     a.barrier = reinterpret_cast<uint32_t*>(w);
-    a.of_cta = reinterpret_cast<int2*>(w += 256);
-    a.first = reinterpret_cast<int32_t*>(w += counted);
-    a.rank = reinterpret_cast<int32_t*>(w += rows);
+    a.first = reinterpret_cast<unsigned long long*>(w += 256);
+    a.of_cta = reinterpret_cast<int2*>(w += firsts);
+    a.rank = reinterpret_cast<int32_t*>(w += counted);
     a.list = reinterpret_cast<int32_t*>(w += rows);
     a.list2 = reinterpret_cast<int32_t*>(w += pages);
     a.bits = reinterpret_cast<uint32_t*>(w += pages);
