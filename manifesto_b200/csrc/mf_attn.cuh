@@ -71,6 +71,12 @@ __device__ __forceinline__ float cap_small(float p, float softcap) {
     const float v = p * p;
     return p * softcap * __fmaf_rn(__fmaf_rn(__fmaf_rn(v, -4.1202753e-5f, 9.5731476e-4f), v, -0.020017692f), v, 0.49999995f);
 }
+__device__ __forceinline__ float2 cap_small2(float2 p, float softcap) {
+    const float2 v = __fmul2_rn(p, p);
+    auto both = [](float x) { return make_float2(x, x); };
+    return __fmul2_rn(__fmul2_rn(p, both(softcap)),
+                      __ffma2_rn(__ffma2_rn(__ffma2_rn(v, both(-4.1202753e-5f), both(9.5731476e-4f)), v, both(-0.020017692f)), v, both(0.49999995f)));
+}
 __device__ __forceinline__ float cap_large(float p, float cap) {
     return __fmaf_rn(-2.0f * cap, rcp_fast(1.0f + exp2_fast(p)), cap);
 }

@@ -351,7 +351,7 @@ __device__ __forceinline__ void produce(const PrefixArgs& a, typename K::Shared&
     const int pieces = (a.head_dim * kBytesOf + 15) / 16;  // 16-byte pieces of a row in memory
     constexpr int kMostPieces = K::kPanels * 8 / (K::kFp8 ? 2 : 1);
     const int piece = tid % kMostPieces, row0 = tid / kMostPieces;
-    constexpr int kStep = kProducers / kMostPieces, kCopies = K::T / kStep;
+    constexpr int kStep = kProducers / kMostPieces, kCopies = K::T / kStep, kAtOnce = kCopies < 8 ? kCopies : 8;
     const bool mine = piece < pieces;
     const int64_t kv_gap = a.v - a.k;
     uint32_t unit = 0, told = 0, tile = 0;  // units begun, units that the consumer has, tiles so far
@@ -363,16 +363,19 @@ __device__ __forceinline__ void produce(const PrefixArgs& a, typename K::Shared&
             wait(&sh.abandoned, &sh.empty[stage], (told / K::kStages & 1u) ^ 1u);
             __syncwarp();
             if (mine) {
+                uint4 code[kCopies];
+#pragma unroll
+                for (int x = 0; x < kCopies; ++x)
+                    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                                 : "=r"(code[x].x), "=r"(code[x].y), "=r"(code[x].z), "=r"(code[x].w) : "r"(from + x * (kProducers * 16)) : "memory");
 #pragma unroll
                 for (int x = 0; x < kCopies; ++x) {
                     const int r = row0 + x * kStep;
-                    uint4 code, lo, hi;
-                    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
-                                 : "=r"(code.x), "=r"(code.y), "=r"(code.z), "=r"(code.w) : "r"(from + x * (kProducers * 16)) : "memory");
-                    fp8x4_to_f16<MODE>(code.x, lo.x, lo.y);
-                    fp8x4_to_f16<MODE>(code.y, lo.z, lo.w);
-                    fp8x4_to_f16<MODE>(code.z, hi.x, hi.y);
-                    fp8x4_to_f16<MODE>(code.w, hi.z, hi.w);
+                    uint4 lo, hi;
+                    fp8x4_to_f16<MODE>(code[x].x, lo.x, lo.y);
+                    fp8x4_to_f16<MODE>(code[x].y, lo.z, lo.w);
+                    fp8x4_to_f16<MODE>(code[x].z, hi.x, hi.y);
+                    fp8x4_to_f16<MODE>(code[x].w, hi.z, hi.w);
                     const uint32_t at0 = to + place(K::T, r, 2 * piece), at1 = to + place(K::T, r, 2 * piece + 1);
                     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at0), "r"(lo.x), "r"(lo.y), "r"(lo.z), "r"(lo.w) : "memory");
                     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at1), "r"(hi.x), "r"(hi.y), "r"(hi.z), "r"(hi.w) : "memory");
@@ -405,12 +408,15 @@ __device__ __forceinline__ void produce(const PrefixArgs& a, typename K::Shared&
                     __syncwarp();
                 }
                 if (mine) {
-#pragma unroll 8
-                    for (int x = 0; x < kCopies; ++x) {
-                        const int r = row0 + x * kStep;
-                        const uint32_t off = rows[r];
-                        cp_async16(to + (K::kFp8 ? x * (kProducers * 16) : place(K::T, r, piece)),
-                                   off != kMasked ? base + (static_cast<int64_t>(off) << a.unit) : a.k, off != kMasked ? 16u : 0u);
+#pragma unroll
+                    for (int x0 = 0; x0 < kCopies; x0 += kAtOnce) {
+                        uint32_t off[kAtOnce];
+#pragma unroll
+                        for (int x = 0; x < kAtOnce; ++x) off[x] = rows[row0 + (x0 + x) * kStep];
+#pragma unroll
+                        for (int x = 0; x < kAtOnce; ++x)
+                            cp_async16(to + (K::kFp8 ? (x0 + x) * (kProducers * 16) : place(K::T, row0 + (x0 + x) * kStep, piece)),
+                                       off[x] != kMasked ? base + (static_cast<int64_t>(off[x]) << a.unit) : a.k, off[x] != kMasked ? 16u : 0u);
                     }
                 }
                 cp_async_commit();
@@ -531,10 +537,20 @@ struct Row {
     bool seen;               // whether the row sees any of the shared tokens
 };
 
+// f of 32 numbers, two at a time.
+template <class F>
+__device__ __forceinline__ void each_two(uint32_t (&v)[32], F&& f) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+        const float2 p = f(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])));
+        v[i] = __float_as_uint(p.x);
+        v[i + 1] = __float_as_uint(p.y);
+    }
+}
+
 // 32 products as scores that count: capped, biased, masked.  `tok`: the first token; `word`: those that are there.
 __device__ __forceinline__ void count_scores(const PrefixArgs& a, const Row& row, uint32_t (&v)[32], uint32_t tok, uint32_t word) {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * row.scale);
+    each_two(v, [&](float2 p) { return __fmul2_rn(p, make_float2(row.scale, row.scale)); });
     if (a.softcap > 0.0f) {
         float most = 0.0f;
 #pragma unroll
@@ -546,8 +562,7 @@ __device__ __forceinline__ void count_scores(const PrefixArgs& a, const Row& row
                 v[i] = __float_as_uint(fabsf(p) < kSmallCapped ? cap_small(p, a.softcap) : cap_large(p, row.cap));
             }
         } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(cap_small(__uint_as_float(v[i]), a.softcap));
+            each_two(v, [&](float2 p) { return cap_small2(p, a.softcap); });
         }
     }
     if (a.slopes) {
