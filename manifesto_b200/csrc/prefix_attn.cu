@@ -145,10 +145,10 @@ __device__ __forceinline__ uint32_t product(bool bf16, int n, bool b_rows) {
 }
 
 // Four groups of four warps: softmax, softmax, producers, and single ones (the products' issuer, the pages', the notes').  The
-// registers of the launch (128 each) go where a row of scores is held: 128 x (176 + 176 + 96 + 64) = 512 x 128.
+// registers of the launch (128 each) go where a row of scores is held: 128 x (200 + 200 + 64 + 48) = 512 x 128.
 constexpr int kThreads = 512;
 constexpr int kProducers = 128, kFirstProducer = 256, kIssuer = 12, kPager = 13, kNoter = 14;
-constexpr int kSoftmaxRegs = 176, kProducerRegs = 96, kOtherRegs = 64;
+constexpr int kSoftmaxRegs = 200, kProducerRegs = 64, kOtherRegs = 48;
 constexpr int kPlaces = 4;  // tiles whose rows are known in advance
 constexpr int kMasks = 16;  // tiles whose masks are kept: more than the ring and the places hold
 
@@ -350,7 +350,10 @@ __device__ __forceinline__ void produce(const PrefixArgs& a, typename K::Shared&
     constexpr int kBytesOf = K::kFp8 ? 1 : 2;
     const int pieces = (a.head_dim * kBytesOf + 15) / 16;  // 16-byte pieces of a row in memory
     constexpr int kMostPieces = K::kPanels * 8 / (K::kFp8 ? 2 : 1);
-    const int piece = tid % kMostPieces, row0 = tid / kMostPieces;
+    // FP8: eight lanes have four pieces of two rows, so that what they convert falls on different banks (of one row's eight
+    // pieces the halves of a row would meet)
+    const int piece = K::kFp8 ? (tid & 3) | (tid >> 3 & (kMostPieces / 4 - 1)) << 2 : tid % kMostPieces;
+    const int row0 = K::kFp8 ? (tid >> 2 & 1) | tid / (2 * kMostPieces) << 1 : tid / kMostPieces;
     constexpr int kStep = kProducers / kMostPieces, kCopies = K::T / kStep, kAtOnce = kCopies < 8 ? kCopies : 8;
     const bool mine = piece < pieces;
     const int64_t kv_gap = a.v - a.k;
