@@ -258,6 +258,18 @@ struct Run {
     __device__ __forceinline__ bool dual() const { return K::kStreams == 2 && rows > 128; }
     // among how many warps a row's tokens of a tile are shared out, where there are no rows for four
     __device__ __forceinline__ int32_t sharers() const { return rows <= 32 && K::T == 128 ? 4 : rows <= 64 ? 2 : 1; }
+    // Units of the item's tiles (a tile's keys, or its values) in the order in which products want them.  Dual: keys and values of a
+    // tile by turns.  Else scores run two steps ahead: K0 K1 V0 K2 V1 ... V(n-2) V(n-1).
+    __device__ __forceinline__ uint32_t keys_at(int32_t tile) const { return dual() ? 2 * tile : tile == 0 ? 0 : 2 * tile - 1; }
+    __device__ __forceinline__ uint32_t values_at(int32_t tile) const { return dual() || tile == n - 1 ? 2 * tile + 1 : 2 * tile + 2; }
+    __device__ __forceinline__ int32_t tile_at(int32_t unit, bool& values) const {
+        if (dual() || unit == 0 || unit == 2 * n - 1) {
+            values = unit & 1;
+            return unit >> 1;
+        }
+        values = !(unit & 1);
+        return values ? unit / 2 - 1 : (unit + 1) / 2;
+    }
     __device__ __forceinline__ int32_t steps() const { return dual() ? 2 * n : n; }
     // false: the run is over (and n is 0)
     __device__ __forceinline__ bool next(const PrefixArgs& a) {
@@ -394,44 +406,48 @@ __device__ __forceinline__ void produce(const PrefixArgs& a, typename K::Shared&
     bool more = run.n > 0;
     while (more) {
         const char* keys = a.k + run.kv * a.head_bytes + piece * 16;
-        for (int32_t i = 0; i < run.n; ++i, ++tile) {
-            wait(&sh.abandoned, &sh.rows_known[tile % kPlaces], tile / kPlaces & 1u);
-            __syncwarp();
-            const uint32_t* rows = sh.row[tile % kPlaces];
-#pragma unroll 1
-            for (int of = 0; of < 2; ++of) {
-                const uint32_t stage = unit % K::kStages, parity = (unit / K::kStages & 1u) ^ 1u;
-                const uint32_t to = K::kFp8 ? ring + K::kStages * K::kUnit + unit % K::kRaw * (K::kUnit / 2) + tid * 16 : ring + stage * K::kUnit;
-                const char* base = keys + (of ? kv_gap : 0);
-                if (!K::kFp8 && !__all_sync(0xffffffffu, mbar_try_wait(&sh.empty[stage], parity))) {
-                    // no room: what is on the way may be what the consumer waits for
-                    cp_async_wait<0>();
-                    while (told < unit) tell();
-                    wait(&sh.abandoned, &sh.empty[stage], parity);
-                    __syncwarp();
-                }
-                if (mine) {
+        for (int32_t j = 0; j < 2 * run.n; ++j) {
+            bool of_v;
+            const uint32_t at = tile + run.tile_at(j, of_v);
+            if (!of_v) {
+                wait(&sh.abandoned, &sh.rows_known[at % kPlaces], at / kPlaces & 1u);
+                __syncwarp();
+            }
+            const uint32_t* rows = sh.row[at % kPlaces];
+            const uint32_t stage = unit % K::kStages, parity = (unit / K::kStages & 1u) ^ 1u;
+            const uint32_t to = K::kFp8 ? ring + K::kStages * K::kUnit + unit % K::kRaw * (K::kUnit / 2) + tid * 16 : ring + stage * K::kUnit;
+            const char* base = keys + (of_v ? kv_gap : 0);
+            if (!K::kFp8 && !__all_sync(0xffffffffu, mbar_try_wait(&sh.empty[stage], parity))) {
+                // no room: what is on the way may be what the consumer waits for
+                cp_async_wait<0>();
+                while (told < unit) tell();
+                wait(&sh.abandoned, &sh.empty[stage], parity);
+                __syncwarp();
+            }
+            if (mine) {
 #pragma unroll
-                    for (int x0 = 0; x0 < kCopies; x0 += kAtOnce) {
-                        uint32_t off[kAtOnce];
+                for (int x0 = 0; x0 < kCopies; x0 += kAtOnce) {
+                    uint32_t off[kAtOnce];
 #pragma unroll
-                        for (int x = 0; x < kAtOnce; ++x) off[x] = rows[row0 + (x0 + x) * kStep];
+                    for (int x = 0; x < kAtOnce; ++x) off[x] = rows[row0 + (x0 + x) * kStep];
 #pragma unroll
-                        for (int x = 0; x < kAtOnce; ++x)
-                            cp_async16(to + (K::kFp8 ? (x0 + x) * (kProducers * 16) : place(K::T, row0 + (x0 + x) * kStep, piece)),
-                                       off[x] != kMasked ? base + (static_cast<int64_t>(off[x]) << a.unit) : a.k, off[x] != kMasked ? 16u : 0u);
-                    }
-                }
-                cp_async_commit();
-                ++unit;
-                if (unit - told > kAhead) {
-                    cp_async_wait<kAhead>();
-                    tell();
+                    for (int x = 0; x < kAtOnce; ++x)
+                        cp_async16(to + (K::kFp8 ? (x0 + x) * (kProducers * 16) : place(K::T, row0 + (x0 + x) * kStep, piece)),
+                                   off[x] != kMasked ? base + (static_cast<int64_t>(off[x]) << a.unit) : a.k, off[x] != kMasked ? 16u : 0u);
                 }
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.rows_used[tile % kPlaces]);
+            cp_async_commit();
+            ++unit;
+            if (unit - told > kAhead) {
+                cp_async_wait<kAhead>();
+                tell();
+            }
+            if (of_v) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.rows_used[at % kPlaces]);
+            }
         }
+        tile += run.n;
         more = run.next(a);
     }
     cp_async_wait<0>();
@@ -477,7 +493,7 @@ __device__ __forceinline__ void multiply(const PrefixArgs& a, typename K::Shared
             // its weights of the step before, in S's place, have been used
             const uint32_t done = b ? o_steps[1] : o_steps[0];
             if (done > 0) wait(&sh.abandoned, &sh.o_done[b], (done - 1) & 1u);
-            const uint32_t u = unit + 2 * tile_of(x), stage = u % K::kStages;
+            const uint32_t u = unit + run.keys_at(tile_of(x)), stage = u % K::kStages;
             wait(&sh.abandoned, &sh.full[stage], u / K::kStages & 1u);
             __syncwarp();
             tc_fence_after();
@@ -498,7 +514,7 @@ __device__ __forceinline__ void multiply(const PrefixArgs& a, typename K::Shared
 #pragma unroll 1
         for (int32_t x = 0; x < steps; ++x) {
             const int b = x & 1, s = K::kStreams == 2 ? b : 0;
-            const uint32_t u = unit + 2 * tile_of(x) + 1, stage = u % K::kStages;
+            const uint32_t u = unit + run.values_at(tile_of(x)), stage = u % K::kStages;
             wait(&sh.abandoned, &sh.full[stage], u / K::kStages & 1u);
             wait(&sh.abandoned, &sh.p_full[b], ((b ? s_steps[1] : s_steps[0]) - 1) & 1u);
             __syncwarp();
