@@ -52,7 +52,7 @@ struct PrefixArgs {
     const char* k;
     const char* v;
     int64_t head_bytes, table_stride;
-    uint32_t page_units, row_units, unit;  // a page, a row of it in units of 2^unit bytes
+    uint32_t page_units, row_units, unit;  // a page, a row of it in units of `unit` bytes, a power of two
     uint32_t n_pages;
     Divisor by_page;
     Divisor group;        // query heads of a key-value head
@@ -145,10 +145,10 @@ __device__ __forceinline__ uint32_t product(bool bf16, int n, bool b_rows) {
 }
 
 // Four groups of four warps: softmax, softmax, producers, and single ones (the products' issuer, the pages', the notes').  The
-// registers of the launch (128 each) go where a row of scores is held: 128 x (200 + 200 + 64 + 48) = 512 x 128.
+// registers of the launch (128 each) go where a row of scores is held: 128 x (192 + 192 + 64 + 64) = 512 x 128.
 constexpr int kThreads = 512;
 constexpr int kProducers = 128, kFirstProducer = 256, kIssuer = 12, kPager = 13, kNoter = 14;
-constexpr int kSoftmaxRegs = 200, kProducerRegs = 64, kOtherRegs = 48;
+constexpr int kSoftmaxRegs = 192, kProducerRegs = 64, kOtherRegs = 64;
 constexpr int kPlaces = 4;  // tiles whose rows are known in advance
 constexpr int kMasks = 16;  // tiles whose masks are kept: more than the ring and the places hold
 
@@ -188,7 +188,7 @@ struct Prefix {
         Group of;                   // where this CTA's run begins
         int32_t group, into;
         uint32_t mask[kMasks][4];   // tokens of a tile that are there
-        uint32_t row[kPlaces][T];   // where a tile's rows are, from the head's begin, in units of 2^unit bytes; kMasked: nowhere
+        uint32_t row[kPlaces][T];   // where a tile's rows are, from the head's begin, in units of `unit` bytes; kMasked: nowhere
     };
     static constexpr int kBytes = kRing + kStreams * kQ + static_cast<int>(sizeof(Shared));
 };
@@ -433,7 +433,7 @@ __device__ __forceinline__ void produce(const PrefixArgs& a, typename K::Shared&
 #pragma unroll
                     for (int x = 0; x < kAtOnce; ++x)
                         cp_async16(to + (K::kFp8 ? (x0 + x) * (kProducers * 16) : place(K::T, row0 + (x0 + x) * kStep, piece)),
-                                   off[x] != kMasked ? base + (static_cast<int64_t>(off[x]) << a.unit) : a.k, off[x] != kMasked ? 16u : 0u);
+                                   base + static_cast<uint64_t>(off[x] == kMasked ? 0u : off[x]) * a.unit, off[x] == kMasked ? 0u : 16u);
                 }
             }
             cp_async_commit();
@@ -1299,7 +1299,7 @@ extern "C" int mf_prefix_attn_create(const mf_paged_attn_config* config, int32_t
     a.page = k.page_size;
     a.window = c.window;
     a.kv_heads = k.kv_heads;
-    a.unit = unit;
+    a.unit = 1u << unit;
     a.page_units = static_cast<uint32_t>(page_bytes >> unit);
     a.row_units = static_cast<uint32_t>(row_bytes >> unit);
     a.head_bytes = k.head_stride * code;
