@@ -87,6 +87,7 @@ __device__ __forceinline__ bool all_sync(const BookArgs& a) {
                     if (now == round && global_ns() > until) {
                         late = 1;
                         atomicExch(a.status, MF_DEVICE_TIMEOUT);
+                        atomicExch(a.barrier, 0u);  // the next launch counts from zero
                         break;
                     }
                 }

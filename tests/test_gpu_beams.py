@@ -599,3 +599,145 @@ def test_copy_refusals(backend):
             paged.PageCopy(bad, [buf.ptr]).run(mv.ptr, 1)
     buf.free()
     mv.free()
+
+
+# ------------------------------------------------------------------ together
+
+@pytest.mark.parametrize("cache,most", [("bf16", 0.05), ("f8_e4m3", 0.35), ("f8_e5m2", 0.7)])
+@pytest.mark.parametrize("k", [1, 4])
+def test_beam_search_of_the_example(backend, cache, most, k):
+    """The bounds of an attention over rounded keys and values: as the decoding example's."""
+    from examples import beam_search
+
+    device_status()
+    assert max(beam_search.run(beams=k, cache_dtype=cache)) < most
+    assert device_status() == 0
+
+
+def test_a_captured_step_replays_with_other_beams(backend):
+    """Selection, fork, page copies and compaction captured once; each replay works on the logits and books that are there then,
+    as the same calls one by one do."""
+    import torch
+
+    n, k, vocab, page, width, pages, dim = 3, 4, 3001, 8, 12, 400, 32
+    rows = n * k
+    layout = paged.CacheLayout(pages, page, 2, dim, BF16)
+    data = np.random.default_rng(5).integers(0, 1 << 16, pages * page * 2 * dim).astype(np.uint16)
+
+    class Step:
+        def __init__(self):
+            self.cache = [to_device(data), to_device(data[::-1].copy())]
+            self.x, self.scores, self.out = empty(4 * rows * vocab), empty(4 * rows), empty(4 * rows)
+            self.tokens, self.parents = empty(4 * rows), empty(4 * rows)
+            self.table = [empty(4 * rows * width) for _ in range(3)]
+            self.lens, self.shares = [empty(4 * rows) for _ in range(2)], [empty(4 * pages) for _ in range(3)]
+            self.free, self.pool = [empty(4 * pages) for _ in range(3)], [empty(16) for _ in range(3)]
+            self.moves = [empty(16 * rows, 0), empty(16 * (pages // 2), 0)]
+            self.numbers = empty(4 * pages)
+            self.select, self.book = beams.BeamSelect(F32, vocab, k, k, n), paged.PageBook(page, width, pages, rows)
+            self.copy = paged.PageCopy(layout, [c.ptr for c in self.cache])
+
+        def run(self, stream):
+            self.select.run(self.x.ptr, self.scores.ptr, n, self.out.ptr, self.tokens.ptr, self.parents.ptr, stream=stream)
+            self.book.fork(self.table[0].ptr, self.lens[0].ptr, rows, self.parents.ptr, rows, self.shares[0].ptr, self.free[0].ptr,
+                           self.pool[0].ptr, self.table[1].ptr, self.lens[1].ptr, self.shares[1].ptr, self.free[1].ptr,
+                           self.pool[1].ptr, self.moves[0].ptr, stream)
+            self.copy.run(self.moves[0].ptr, rows, self.pool[1].ptr + 8, stream)
+            self.book.compact(self.table[1].ptr, self.lens[1].ptr, rows, self.shares[1].ptr, self.free[1].ptr, self.pool[1].ptr, 0,
+                              self.table[2].ptr, self.shares[2].ptr, self.free[2].ptr, self.pool[2].ptr, self.numbers.ptr,
+                              self.moves[1].ptr, stream)
+            self.copy.run(self.moves[1].ptr, pages // 2, self.pool[2].ptr + 8, stream)
+
+        def load(self, seed):
+            rng = np.random.default_rng(seed)
+            lens, table, shares, free, pool = family_book(rows, page, width, pages, width * page - 1, seed)
+            for b, a in ((self.x, rng.normal(0, 2, (rows, vocab)).astype(np.float32)), (self.scores, -rng.random(rows, np.float32)),
+                         (self.table[0], table), (self.lens[0], lens), (self.shares[0], shares), (self.free[0], free), (self.pool[0], pool),
+                         (self.cache[0], data), (self.cache[1], data[::-1].copy())):
+                b.upload(np.ascontiguousarray(a))
+            sync_device()
+
+        def bufs(self):
+            return [*self.cache, self.x, self.scores, self.out, self.tokens, self.parents, *self.table, *self.lens, *self.shares,
+                    *self.free, *self.pool, *self.moves, self.numbers]
+
+        def state(self):
+            valid = int(fetch(self.pool[1], 16, np.int32)[1]), int(fetch(self.pool[2], 16, np.int32)[1])
+            return [fetch(b, b.nbytes) for b in (*self.cache, self.out, self.tokens, self.parents, *self.table[1:], self.lens[1],
+                                                 *self.shares[1:], *self.pool[1:], self.numbers)] + \
+                   [fetch(b, 4 * v) for b, v in zip(self.free[1:], valid)]
+
+        def close(self):
+            self.select.close()
+            self.book.close()
+            for b in self.bufs():
+                b.free()
+
+    one, other = Step(), Step()
+    one.load(1)
+    stream = torch.cuda.Stream()
+    one.run(stream.cuda_stream)
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        one.run(stream.cuda_stream)
+    for seed in (2, 3, 4, 5):
+        one.load(seed)
+        other.load(seed)
+        graph.replay()
+        torch.cuda.synchronize()
+        other.run(None)
+        for a, b in zip(one.state(), other.state()):
+            bits_equal(a, b)
+    assert device_status() == 0
+    del graph
+    one.close()
+    other.close()
+
+
+def test_book_two_handles_on_two_streams(backend):
+    """Forks of a grid's size that overlap on two streams give what each gives alone."""
+    made = [family_book(3000, 2, 200, 3000 * 200 + 500, 400, seed) for seed in (1, 2)]
+    parents = [np.random.default_rng(seed).integers(-1, 3000, 3000).astype(np.int32) for seed in (1, 2)]
+    streams = [Stream(), Stream()]
+    handles = [paged.PageBook(2, 200, 3000 * 200 + 500, 3000) for _ in range(2)]
+    ins = [[to_device(a) for a in (m[1], m[0], p, m[2], m[3], m[4])] for m, p in zip(made, parents)]
+    pages = 3000 * 200 + 500
+    outs = [[empty(4 * s) for s in (3000 * 200, 3000, pages, pages, 4, 4 * 3000)] for _ in range(2)]
+    sync_device()
+    for _ in range(10):
+        for h, i, o, s in zip(handles, ins, outs, streams):
+            p = [b.ptr for b in i]
+            h.fork(p[0], p[1], 3000, p[2], 3000, p[3], p[4], p[5], *(b.ptr for b in o), stream=s)
+    for s in streams:
+        s.sync()
+    assert device_status() == 0
+    for m, p, o in zip(made, parents, outs):
+        want = plain.fork(m[1], m[0], p, m[2], m[3], m[4], 2, 200, np.zeros((3000, 4), np.int32), np.zeros(pages, np.int32))
+        bits_equal(fetch(o[0], 4 * 3000 * 200, np.int32).reshape(3000, 200), want[0])
+        bits_equal(fetch(o[2], 4 * pages, np.int32), want[2])
+        bits_equal(fetch(o[4], 16, np.int32), want[4])
+    for h in handles:
+        h.close()
+    for b in (*ins[0], *ins[1], *outs[0], *outs[1]):
+        b.free()
+    for s in streams:
+        s.close()
+
+
+@pytest.mark.parametrize("make", [lambda: beams.BeamSelect(BF16, 128256, 8, 64, 64), lambda: paged.PageBook(16, 64, 4_000_000, 64),
+                                  lambda: paged.PrefixAttention(paged.CacheLayout(4, 16, 1, 256, BF16), 16, BF16, 4, 256)])
+def test_handles_close_after_shutdown_and_keep_nothing(backend, make):
+    import torch
+
+    make().close()
+    before = torch.cuda.mem_get_info()[0]
+    held = [make() for _ in range(4)]
+    assert torch.cuda.mem_get_info()[0] < before - (8 << 20)
+    call("mf_shutdown")
+    try:
+        for h in held:
+            h.close()
+    finally:
+        call("mf_init", 0)
+    assert torch.cuda.mem_get_info()[0] >= before - (4 << 20)

@@ -3,6 +3,7 @@ import numpy as np
 import pytest
 
 from manifesto_b200 import Stream, paged, sync_device
+from manifesto_b200._abi import call
 from manifesto_b200.dtype import DType
 from manifesto_b200.errors import (DTypeMismatch, DTypeUnsupported, InvalidArgument, LayoutUnsupported, ShapeInvalid, TensorClosed)
 
@@ -388,3 +389,115 @@ def test_prefix_refusals(backend):
     h.close()
     for x in b:
         x.free()
+
+
+def test_prefix_longer_than_a_row_of_masks_and_stages(backend):
+    """Runs of one tile between long ones: stages are released in order whatever the steps of an item."""
+    run_groups([(x, [1] * m) for x, m in ((64, 2), (200, 40), (64, 2), (500, 2), (90, 70), (64, 3), (64, 2), (300, 9)) for _ in range(8)], hq=2, hkv=2)
+
+
+@pytest.mark.parametrize("page,cache", [(16, BF16), (20, BF16), (16, E4M3)])
+def test_prefix_offsets_past_32_bits(backend, page, cache):
+    """Pages 2^28 bytes apart or more: the last of 18 lies past 2^32 bytes."""
+    s = make_groups([(page * 3, [1, 2, 5])], 4, 2, 64, page, "NHD", BF16, cache, 9)
+    stride = (1 << 28) // cache.size
+    tight = page * 2 * 64
+    small = s["pages"]
+    number = np.array([17, 3, 16, 0, 9, 15, 2, 12, 5, 7, 11, 14, 1, 4, 6, 8, 10, 13][:small])
+    kv = []
+    for c in s["kv"]:
+        big = empty(cache.size * (17 * stride + tight), None)
+        for i in range(small):
+            call("mf_memcpy_h2d_async", big.ptr + cache.size * int(number[i]) * stride, c[i].ctypes.data, c[i].nbytes, None)
+        sync_device()
+        kv.append(big)
+    table = np.where((s["table"] >= 0) & (s["table"] < small), number[np.clip(s["table"], 0, small - 1)], s["table"]).astype(np.int32)
+    layout = paged.CacheLayout(18, page, 2, 64, cache, "NHD")
+    layout.struct.page_stride = stride
+    b = [to_device(a) for a in (s["q"], table, s["lens"], s["starts"], s["shared"])]
+    sc = to_device(s["scales"]) if s["scales"] is not None else None
+    out, lse = empty(2 * 3 * 4 * 64), empty(4 * 3 * 4)
+    with paged.PrefixAttention(layout, 4, BF16, table.shape[1], 3, k_scale_inv=sc.ptr if sc else 0, v_scale_inv=sc.ptr + 8 if sc else 0) as attn:
+        attn.run(b[0].ptr, kv[0].ptr, kv[1].ptr, b[1].ptr, b[2].ptr, 3, b[3].ptr, b[4].ptr, 1, out.ptr, lse.ptr)
+        sync_device()
+    assert device_status() == 0
+    check_prefix(s, (fetch(out, out.nbytes, np.uint16).reshape(3, 4, 64), fetch(lse, lse.nbytes, np.float32).reshape(3, 4)), want_attn(s))
+    for t in (*kv, *b, out, lse, *([sc] if sc else [])):
+        t.free()
+
+
+def test_prefix_padded_tables_and_caches(backend):
+    """Table rows and pages that are longer than what they hold; the gaps hold NaN codes."""
+    hq, hkv, dim, page = 4, 2, 64, 16
+    s = make_groups([(100, [1, 45, 0]), (30, [3, 4])], hq, hkv, dim, page, "NHD", BF16, BF16, 4)
+    n, width = s["table"].shape
+    table = np.full((n, width + 5), 1 << 30, np.int32)
+    table[:, :width] = s["table"]
+    rows, heads = page + 3, hkv + 1  # a page of 16 of 19 rows, 2 of 3 heads, 64 of 72 elements
+    kv = []
+    for c in s["kv"]:
+        wide = np.full((s["pages"], rows, heads, dim + 8), 0x7FFF, np.uint16)
+        wide[:, :page, :hkv, :dim] = c
+        kv.append(to_device(wide))
+    layout = paged.CacheLayout(s["pages"], page, hkv, dim, BF16)
+    layout.struct.page_stride, layout.struct.token_stride = rows * heads * (dim + 8), heads * (dim + 8)
+    layout.struct.head_stride = dim + 8
+    b = [to_device(x) for x in (s["q"], table, s["lens"], s["starts"], s["shared"])]
+    out, lse = empty(2 * n * hq * dim), empty(4 * n * hq)
+    with paged.PrefixAttention(layout, hq, BF16, width, n, table_stride=width + 5) as attn:
+        attn.run(b[0].ptr, kv[0].ptr, kv[1].ptr, b[1].ptr, b[2].ptr, n, b[3].ptr, b[4].ptr, 2, out.ptr, lse.ptr)
+        sync_device()
+    assert device_status() == 0
+    check_prefix(s, (fetch(out, out.nbytes, np.uint16).reshape(n, hq, dim), fetch(lse, lse.nbytes, np.float32).reshape(n, hq)), want_attn(s))
+    for t in (*b, *kv, out, lse):
+        t.free()
+
+
+@pytest.mark.parametrize("cache", [BF16, E4M3])
+def test_prefix_captured_replays_with_other_groups(backend, cache):
+    """Captured once; each replay serves the lengths, groups and shared tokens that are there then."""
+    import torch
+
+    cases = [make_groups(g, 8, 2, 128, 16, "HND", BF16, cache, 3) for g in
+             ([(200, [1, 2, 3]), (40, [4, 5, 6, 7])], [(0, [9, 8, 7, 1]), (260, [1, 2, 0])], [(64, [1] * 2), (100, [2] * 5)])]
+    most = max(s["pages"] for s in cases), max(s["table"].shape[1] for s in cases)
+    for s in cases:  # one shape for all
+        s["table"] = np.pad(s["table"], ((0, 0), (0, most[1] - s["table"].shape[1])), constant_values=1 << 30)
+        s["kv"] = [np.concatenate([c, np.zeros((most[0] - len(c), *c.shape[1:]), c.dtype)]) for c in s["kv"]]
+        s["pages"], s["scales"] = most[0], cases[0]["scales"]
+    on = Running(cases[0])
+    stream = torch.cuda.Stream()
+    p = [b.ptr for b in on.bufs]
+
+    def launch():
+        on.attn.run(*p[:5], 7, p[5], p[6], 2, on.out.ptr, on.lse.ptr, stream=stream.cuda_stream)
+
+    launch()
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        launch()
+    for s in cases[::-1]:
+        kv = [np.ascontiguousarray(c.transpose(0, 2, 1, 3)) for c in s["kv"]]
+        for b, x in zip(on.bufs, (s["q"], kv[0], kv[1], s["table"], s["lens"], s["starts"], s["shared"])):
+            b.upload(np.ascontiguousarray(x))
+        sync_device()
+        graph.replay()
+        torch.cuda.synchronize()
+        check_prefix(s, (fetch(on.out, 7 * 8 * 128 * 2, np.uint16).reshape(7, 8, 128), fetch(on.lse, 7 * 8 * 4, np.float32).reshape(7, 8)), want_attn(s))
+    assert device_status() == 0
+    del graph
+    on.close()
+
+
+def test_prefix_destroyed_while_its_runs_are_queued(backend):
+    s = make_groups([(3000, [1] * 40)], 8, 2, 128, 16, "HND", BF16, BF16, 3)
+    on, st = Running(s), Stream()
+    p = [b.ptr for b in on.bufs]
+    for _ in range(30):
+        on.attn.run(*p[:5], 40, p[5], p[6], 1, on.out.ptr, on.lse.ptr, stream=st)
+    on.attn.close()
+    got = fetch(on.out, 40 * 8 * 128 * 2, np.uint16).reshape(40, 8, 128), fetch(on.lse, 40 * 8 * 4, np.float32).reshape(40, 8)
+    check_prefix(s, got, want_attn(s))
+    on.close()
+    st.close()
