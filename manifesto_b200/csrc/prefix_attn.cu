@@ -362,22 +362,27 @@ __device__ __forceinline__ void produce(const PrefixArgs& a, typename K::Shared&
     constexpr int kBytesOf = K::kFp8 ? 1 : 2;
     const int pieces = (a.head_dim * kBytesOf + 15) / 16;  // 16-byte pieces of a row in memory
     constexpr int kMostPieces = K::kPanels * 8 / (K::kFp8 ? 2 : 1);
-    // FP8: eight lanes have four pieces of two rows, so that what they convert falls on different banks (of one row's eight
-    // pieces the halves of a row would meet)
-    const int piece = K::kFp8 ? (tid & 3) | (tid >> 3 & (kMostPieces / 4 - 1)) << 2 : tid % kMostPieces;
-    const int row0 = K::kFp8 ? (tid >> 2 & 1) | tid / (2 * kMostPieces) << 1 : tid / kMostPieces;
+    const int piece = tid % kMostPieces, row0 = tid / kMostPieces;
+    // FP8: a warp copies whole rows (as few lines as it can), and converts them with four pieces of two rows for every eight lanes,
+    // so that what they write falls on different banks; odd rows' halves are exchanged on the way, so that what they read does, too.
+    constexpr bool kSwaps = kMostPieces >= 8;
+    const int piece_of = kSwaps ? (lane & 3) | (lane >> 3 & (kMostPieces / 4 - 1)) << 2 : lane % kMostPieces;
+    const int row_in = kSwaps ? (lane >> 2 & 1) | lane / (2 * kMostPieces) << 1 : lane / kMostPieces;
+    const int row_of = tid / 32 * (32 / kMostPieces) + row_in;
+    const int slot_to = (kSwaps ? tid ^ (row0 & 1) << 2 : tid) * 16;
+    const int slot_from = (tid / 32 * 32 + (kSwaps ? (row_in * kMostPieces + piece_of) ^ (row_in & 1) << 2 : lane)) * 16;
     constexpr int kStep = kProducers / kMostPieces, kCopies = K::T / kStep, kAtOnce = kCopies < 8 ? kCopies : 8;
     const bool mine = piece < pieces;
     const int64_t kv_gap = a.v - a.k;
     uint32_t unit = 0, told = 0, tile = 0;  // units begun, units that the consumer has, tiles so far
-    // Unit `told` is there: tell the consumer.  FP8: convert it first; every thread converts the pieces that it copied itself.
+    // Unit `told` is there: tell the consumer.  FP8: convert it first; every warp converts the pieces that it copied itself.
     auto tell = [&]() {
         if constexpr (K::kFp8) {
             const uint32_t stage = told % K::kStages, to = ring + stage * K::kUnit;
-            const uint32_t from = ring + K::kStages * K::kUnit + told % K::kRaw * (K::kUnit / 2) + tid * 16;
+            const uint32_t from = ring + K::kStages * K::kUnit + told % K::kRaw * (K::kUnit / 2) + slot_from;
             wait(&sh.abandoned, &sh.empty[stage], (told / K::kStages & 1u) ^ 1u);
             __syncwarp();
-            if (mine) {
+            if (piece_of < pieces) {
                 uint4 code[kCopies];
 #pragma unroll
                 for (int x = 0; x < kCopies; ++x)
@@ -385,13 +390,13 @@ __device__ __forceinline__ void produce(const PrefixArgs& a, typename K::Shared&
                                  : "=r"(code[x].x), "=r"(code[x].y), "=r"(code[x].z), "=r"(code[x].w) : "r"(from + x * (kProducers * 16)) : "memory");
 #pragma unroll
                 for (int x = 0; x < kCopies; ++x) {
-                    const int r = row0 + x * kStep;
+                    const int r = row_of + x * kStep;
                     uint4 lo, hi;
                     fp8x4_to_f16<MODE>(code[x].x, lo.x, lo.y);
                     fp8x4_to_f16<MODE>(code[x].y, lo.z, lo.w);
                     fp8x4_to_f16<MODE>(code[x].z, hi.x, hi.y);
                     fp8x4_to_f16<MODE>(code[x].w, hi.z, hi.w);
-                    const uint32_t at0 = to + place(K::T, r, 2 * piece), at1 = to + place(K::T, r, 2 * piece + 1);
+                    const uint32_t at0 = to + place(K::T, r, 2 * piece_of), at1 = to + place(K::T, r, 2 * piece_of + 1);
                     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at0), "r"(lo.x), "r"(lo.y), "r"(lo.z), "r"(lo.w) : "memory");
                     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at1), "r"(hi.x), "r"(hi.y), "r"(hi.z), "r"(hi.w) : "memory");
                 }
@@ -415,7 +420,7 @@ __device__ __forceinline__ void produce(const PrefixArgs& a, typename K::Shared&
             }
             const uint32_t* rows = sh.row[at % kPlaces];
             const uint32_t stage = unit % K::kStages, parity = (unit / K::kStages & 1u) ^ 1u;
-            const uint32_t to = K::kFp8 ? ring + K::kStages * K::kUnit + unit % K::kRaw * (K::kUnit / 2) + tid * 16 : ring + stage * K::kUnit;
+            const uint32_t to = K::kFp8 ? ring + K::kStages * K::kUnit + unit % K::kRaw * (K::kUnit / 2) + slot_to : ring + stage * K::kUnit;
             const char* base = keys + (of_v ? kv_gap : 0);
             if (!K::kFp8 && !__all_sync(0xffffffffu, mbar_try_wait(&sh.empty[stage], parity))) {
                 // no room: what is on the way may be what the consumer waits for
