@@ -746,12 +746,17 @@ int mf_page_copy(const mf_cache_layout* layout, void* const* caches, int32_t n_c
  * out and lse are those that mf_paged_attn_run defines, for every request, with
  * the window, cap, slopes and scales of the config; shared[g] may be any number
  * of tokens (negative: 0), and a member may be shorter than it.  Requests in no
- *XX * Over the shared tokens the weights exp(s - max) enter the product with the
+ * group share nothing.  starts that descend or leave the requests, and groups of
+ * more than 2^31 - 1 tiles of tokens together, record MF_DEVICE_TOO_LARGE: nothing
+ * counts as shared then, and the results are the same.  The first request's table
+ * row names all shared pages, even if that request is shorter or idle.
+ * Over the shared tokens the weights exp(s - max) enter the product with the
  * values as two 16-bit terms, as in mf_paged_attn_run, but as one f16 term over an
  * FP8 cache with BF16 queries (off by 2^-11 of a weight at most, an eighth of the
  * result's rounding); queries over an FP8 cache are held as there.  head_dim,
- * dtypes, strides and alignments as there; a cache has at most 2^32 - 1 pieces of
- * the largest power of two of bytes that divides its page and token strides.
+ * dtypes, strides and alignments as there; a cache has less than 2^32 - 1 pieces
+ * of the largest power of two of bytes (2^30 at most) that divides its page and token
+ * strides (else MF_ERR_LAYOUT_UNSUPPORTED).
  * The workspace holds float32 parts of max_requests x q_heads x head_dim, three
  * times, and 15 to 62 MB more; it is not shared between streams that run at
  * once.  Three launches, no host sync; results do not depend on the order in

@@ -11,8 +11,8 @@
 // which atomics arrive, so results are the same in every run; the atomics add
 // to counters (holders) or take a minimum.
 //
-// Bound: latency, the launch and the chain of passes (a cluster's barrier takes a
-// microsecond with the stores before it, the grid's two), then the tables' bytes: 11 us
+// Bound: latency, the launch and the chain of passes (a cluster's barrier takes half
+// a microsecond to one with the stores before it, the grid's two), then the tables' bytes: 11 us
 // for 128 rows of 126 pages, 20 for 2048 rows of 256 over 190 thousand pages (a
 // cluster: 26), 31 for a million pages and 2048 rows of 500 compacted (a cluster: 92;
 // 7 of them are 776 thousand bits set one by one).  Two barriers are saved by not

@@ -26,21 +26,23 @@
 // more than 128 rows each has 128 and sees every tile, else both have the same
 // rows and every second tile.  Up to 64 rows stand in tensor memory two or four
 // times over, and a tile's tokens are shared out among the warps that hold them
-// (24 prompts of 8 beams over E4M3, 32 rows: 326 -> 305 us at that time).  The
+// (24 prompts of 8 beams over E4M3, 32 rows, together with the
+// single f16 term: 404 -> 326 us at that time).  The
 // tiles of all (group, block of rows, key-value head) items in a row are cut evenly
 // for the CTAs, an item counting four tiles more than it has (without them items of
-// two tiles filled a CTA's whole share: 240 -> 146 us); every CTA leaves the part of
+// two tiles filled a CTA's whole share: 240 -> 146 us, with the parts' layout); every CTA leaves the part of
 // its run, and the last launch joins a row's parts in the order of the tokens.
 //
 // Measured (B200): 250 requests behind 8192 shared tokens, 32/8 heads of 128, BF16:
-// this kernel 67 us (the products at the measured rate of the tensor cores: 20 us,
-// 31 with the low terms), tensor pipe 42% of the time busy.  Bound by the chain of a
-// step: scores 0.5 thousand clocks, softmax 2.5, values 1.0, three hand-overs of
-// 0.2; two such chains run at a time, and the issuer, which waits for a step's
-// products before it lets the next scores into their place, takes 2.4 a step
-// itself (no softmax at all: 14 us less).  24 prompts of 8 beams, prefixes ragged to
-// 6000 tokens, E4M3: 97 us (23 to read the codes); copies 20 us of it, softmax 16,
-// parts out of tensor memory 11, conversions nothing that the rest does not hide.
+// this kernel 67 us from cold caches (the products at the measured rate of the tensor cores: 20 us,
+// 31 with the low terms), tensor pipe 41% of the time busy.  Bound by latency: a
+// step's chain is some 5 thousand clocks (scores 0.5, softmax 2.4 to 3, values 1.0,
+// the rest hand-overs; read in an instrumented copy, which is slower itself), two
+// such chains run at a time, and the issuer waits for a step's products before it
+// lets the next scores into their place.  Of 168 us for the whole call, copies that
+// skipped work took: no softmax 154, no parts written 158, no copies 161.  24 prompts of 8 beams, prefixes ragged to
+// 6000 tokens, E4M3: 97 us from cold caches (23 to read the codes).  Of 141 us for the whole
+// call: no copies 121, no softmax 125, no parts written 130, no conversions 147.
 #include <new>
 
 #include "mf_async.cuh"

@@ -10,9 +10,16 @@ operations of a step, in the order in which a step runs them:
 * ``RopeAppend.run``       -- queries and keys rotated, keys and values written to the cache;
 * ``PagedAttention.run``   -- attention of one new token per request over the cache.
 
+For requests that share pages, the continuations of a text (K11; ``beams.BeamSelect`` chooses
+them):
+
+* ``PageBook.fork`` / ``compact`` -- tables continued by parents, and the used pages moved together;
+* ``PageCopy.run``                -- the pages that these move, in every cache;
+* ``PrefixAttention.run``         -- attention that reads a group's shared tokens once for all of it.
+
 Each object holds a description that a program makes once; the calls take device
-addresses (ints, ``DeviceTensor.dispatch_pointer()``) and launch once on a stream,
-without waiting for the device.  ``include/mfcuda.h`` has the formulas (K10).
+addresses (ints, ``DeviceTensor.dispatch_pointer()``) and launch on a stream,
+without waiting for the device.  ``include/mfcuda.h`` has the formulas (K10, K11).
 """
 from __future__ import annotations
 
