@@ -698,9 +698,10 @@ int mf_beam_select_destroy(mf_beam_select handle);
  * their other holders rename theirs by `numbers`.
  * After either call run mf_page_copy on the moves before the caches are used.
  *
- * A page number outside the cache, a list of free pages past its buffer or with
- * a page twice record MF_DEVICE_BAD_PAGE: the number stays as it is and holds
- * nothing, such a list counts as no more pages than there are.
+ * A page number outside the cache (in a table, or in the list of free pages where it
+ * is needed), a list of free pages past its buffer or, in compact, with a page twice
+ * record MF_DEVICE_BAD_PAGE: the number stays as it is and holds nothing, such a
+ * list counts as no more pages than there are.
  * The handle holds the workspace for up to max_requests rows; it is not shared
  * between streams that run at once.  One launch. */
 typedef struct mf_page_move {
@@ -749,7 +750,11 @@ int mf_page_copy(const mf_cache_layout* layout, void* const* caches, int32_t n_c
  * group share nothing.  starts that descend or leave the requests, and groups of
  * more than 2^31 - 1 tiles of tokens together, record MF_DEVICE_TOO_LARGE: nothing
  * counts as shared then, and the results are the same.  The first request's table
- * row names all shared pages, even if that request is shorter or idle.
+ * row names all shared pages, even if that request is shorter or idle, or sees none
+ * of their tokens (a page outside the cache records MF_DEVICE_BAD_PAGE); the others'
+ * rows name those that they see, as in mf_paged_attn_run.  A request in whose shared
+ * tokens an infinity or NaN turns up, seen by it or not, is read request by request,
+ * so that only what it sees counts.
  * Over the shared tokens the weights exp(s - max) enter the product with the
  * values as two 16-bit terms, as in mf_paged_attn_run, but as one f16 term over an
  * FP8 cache with BF16 queries (off by 2^-11 of a weight at most, an eighth of the

@@ -92,7 +92,9 @@ struct AttnArgs {
     float* cta_part;      // [CTAs][3][heads * (DP + 2)]: parts that leave the CTA, and joined groups of them
     int32_t* tickets;     // [2][CTAs], zero between runs
     int32_t* status;
-    const int32_t* own_first;  // of a run of parts: each request's first token
+    const int32_t* own_first;  // of a run of parts: each request's first token; 0 where `alone` has the number of the call
+    const uint32_t* alone;
+    const uint32_t* call;
 };
 
 // ------------------------------------------------------------------ pieces
@@ -166,7 +168,7 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, int32_t r) {
     s.len = max(a.lens[r], 0);
     if (s.len > reach) s.len = static_cast<int32_t>(reach);
     s.first = a.window > 0 && s.len > a.window ? s.len - a.window : 0;
-    if constexpr (PART) s.first = min(max(s.first, a.own_first[r]), s.len);
+    if constexpr (PART) s.first = min(max(s.first, a.alone[r] == *a.call ? 0 : a.own_first[r]), s.len);
     s.base = PART && s.first == s.len ? s.len : s.first & ~(kBlock - 1);
     return s;
 }
@@ -1387,8 +1389,8 @@ int paged_attn_enable_parts(mf_paged_attn handle) {
 }
 
 int paged_attn_run_parts(mf_paged_attn handle, const void* q, const void* k_cache, const void* v_cache, const int32_t* table,
-                         const int32_t* lens, int32_t n_requests, const int32_t* own_first, float* out, float* lse,
-                         cudaStream_t stream) {
+                         const int32_t* lens, int32_t n_requests, const int32_t* own_first, const uint32_t* alone, const uint32_t* call,
+                         float* out, float* lse, cudaStream_t stream) {
     AttnArgs a = handle->args;
     a.q = static_cast<const char*>(q);
     a.k = static_cast<const char*>(k_cache);
@@ -1397,6 +1399,8 @@ int paged_attn_run_parts(mf_paged_attn handle, const void* q, const void* k_cach
     a.lens = lens;
     a.n_requests = n_requests;
     a.own_first = own_first;
+    a.alone = alone;
+    a.call = call;
     a.out = reinterpret_cast<char*>(out);
     a.out_head = a.head_dim;
     a.out_req = static_cast<int64_t>(a.q_heads) * a.head_dim;

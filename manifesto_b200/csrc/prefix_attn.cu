@@ -33,6 +33,11 @@
 // two tiles filled a CTA's whole share: 240 -> 146 us, with the parts' layout); every CTA leaves the part of
 // its run, and the last launch joins a row's parts in the order of the tokens.
 //
+// A masked token's weight is 0, and 0 times a value that is not finite is NaN in the
+// row's sums, though the row does not see it (a shorter request, a token in front of
+// a window).  So a row that ends with such a number marks its request for the call,
+// and the second launch reads all of that request's tokens, masked ones not at all.
+//
 // Measured (B200): 250 requests behind 8192 shared tokens, 32/8 heads of 128, BF16:
 // this kernel 67 us from cold caches (the products at the measured rate of the tensor cores: 20 us,
 // 31 with the low terms), tensor pipe 41% of the time busy.  Bound by latency: a
@@ -67,7 +72,8 @@ struct PrefixArgs {
     const int32_t* starts;
     const int32_t* shared;
     int32_t n_requests, n_groups;
-    int32_t max_pages, page, window, kv_heads;
+    int32_t reach;  // tokens that a row of the table holds, 2^31 - 1 at most
+    int32_t page, window, kv_heads;
     const char* k;
     const char* v;
     int64_t head_bytes, table_stride;
@@ -87,6 +93,8 @@ struct PrefixArgs {
     int32_t* own_first;   // [requests]
     Shared* info;         // [requests]
     int2* cut;            // places of all items, CTAs that they are cut for
+    uint32_t* call;       // the number of the call, for the launches behind the first; of the last call that came to its end
+    uint32_t* alone;      // [requests]: the number of the call that found a number that is not finite, see soften
     float* part;          // [2][requests][q_heads][head_dim]: an item's first CTA, its two halves
     float2* part_ml;      // [2][requests][q_heads]
     float* cta_part;      // [CTAs][2][128][head_dim]: a CTA that begins inside an item
@@ -218,10 +226,7 @@ __device__ __forceinline__ Group group_of(const PrefixArgs& a, int32_t g) {
     x.bad = s < 0 || e < s || e > a.n_requests;
     x.start = s;
     x.members = x.bad ? 0 : e - s;
-    const int64_t reach = static_cast<int64_t>(a.max_pages) * a.page;
-    const int32_t shared = max(a.shared[g], 0);
-    x.shared = x.members < 2 ? 0 : shared;
-    if (x.shared > reach) x.shared = static_cast<int32_t>(reach);
+    x.shared = x.members < 2 ? 0 : min(max(a.shared[g], 0), a.reach);
     return x;
 }
 template <class K>
@@ -770,7 +775,7 @@ __device__ __forceinline__ void soften(const PrefixArgs& a, typename K::Shared& 
         row.scale = a.scale * (a.k_scale ? a.k_scale[run.kv] : 1.0f);
         row.m = row.high = -INFINITY;
         row.less = row.l = 0.0f;
-        row.len = valid ? a.lens[r] : 0;
+        row.len = valid ? min(a.lens[r], a.reach) : 0;
         if (stream < steps) {
             // the queries into shared memory: a few rows at a time, the lanes of a row side by side
             constexpr int kLanes = K::kPanels * 8, kAtOnce = 32 / kLanes;  // 16-byte pieces of a row; rows of an instruction
@@ -886,6 +891,7 @@ __device__ __forceinline__ void soften(const PrefixArgs& a, typename K::Shared& 
                                          static_cast<int64_t>(run.kv) * run.of.members * a.group.d + run.block * K::kRows + (dual ? 128 * stream : 0)
                                    : (static_cast<int64_t>(blockIdx.x) * 2 + stream) * 128;
         float2* ml_to = (first ? a.part_ml : a.cta_ml) + row0 + my_row;
+        float odd = 0.0f;  // NaN once a number is not finite
         if (!has) {
             if (valid && my_share == 0) *ml_to = make_float2(-INFINITY, 0.0f);
         } else {
@@ -922,6 +928,12 @@ __device__ __forceinline__ void soften(const PrefixArgs& a, typename K::Shared& 
                 tm_load(v, o_at + c);
                 tc_wait_ld();
 #pragma unroll
+                for (int i = 0; i < 16; ++i) odd = __fmaf_rn(__uint_as_float(v[i]), 0.0f, odd);
+                if (c + 16 < a.head_dim) {  // no product wrote what is behind
+#pragma unroll
+                    for (int i = 16; i < 32; ++i) odd = __fmaf_rn(__uint_as_float(v[i]), 0.0f, odd);
+                }
+#pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const float4 f = make_float4(__uint_as_float(v[4 * i]) * weight, __uint_as_float(v[4 * i + 1]) * weight,
                                                  __uint_as_float(v[4 * i + 2]) * weight, __uint_as_float(v[4 * i + 3]) * weight);
@@ -946,6 +958,9 @@ __device__ __forceinline__ void soften(const PrefixArgs& a, typename K::Shared& 
                 if (sharers > 1) asm volatile("bar.sync %0, 128;" ::"r"(2 + stream) : "memory");
                 else __syncwarp();
             }
+            // A weight of 0 times a value that is not finite is NaN, and the row may not even see that value's token: then its
+            // request reads all of its tokens in the launch behind this one, where every row has its own.
+            if (busy && row.l != 0.0f && __fmaf_rn(row.l, 0.0f, odd) != 0.0f) a.alone[r] = a.call[1] + 1;
             tc_fence_before();
         }
         tile0 += run.n;
@@ -1068,7 +1083,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const PrefixArgs a)
         total64 = 0;
     }
     const int32_t total = static_cast<int32_t>(total64), ctas = min(total, static_cast<int32_t>(gridDim.x));
-    if (blockIdx.x == 0 && tid == 0) *a.cut = make_int2(total, ctas);
+    if (blockIdx.x == 0 && tid == 0) {
+        *a.cut = make_int2(total, ctas);
+        a.call[0] = a.call[1] + 1;
+    }
     if (static_cast<int32_t>(blockIdx.x) < ctas) {
         const Cut cut(total, ctas);
         const int32_t x0 = cut.start(blockIdx.x), run_of = cut.start(blockIdx.x + 1) - x0;
@@ -1127,6 +1145,8 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const PrefixArgs a) 
     let_next_start();
     const int64_t n = static_cast<int64_t>(a.n_requests) * a.q_heads;
     const int2 all = *a.cut;
+    const uint32_t call = a.call[0];
+    if (blockIdx.x == 0 && threadIdx.x == 0) a.call[1] = call;  // the next call's number is another
     const int32_t dim = a.head_dim;
     for (int64_t w = (static_cast<int64_t>(blockIdx.x) * kJoinThreads + threadIdx.x) >> 5; w < n; w += static_cast<int64_t>(gridDim.x) * (kJoinThreads / 32)) {
         const int32_t r = static_cast<int32_t>(w / a.q_heads), h = static_cast<int32_t>(w - static_cast<int64_t>(r) * a.q_heads);
@@ -1144,7 +1164,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const PrefixArgs a) 
         // the parts of its shared tokens, in order: an item's first CTA's, then the other CTAs', each of one half or two
         int32_t parts = 0, halves = 1;
         int64_t first_at = 0, first_apart = 0, at = 0;  // rows of part, cta_part
-        if (x.tiles > 0) {
+        if (x.tiles > 0 && a.alone[r] != call) {
             const int64_t nth = static_cast<int64_t>(r - x.start) * a.group.d + (h - kv * static_cast<int32_t>(a.group.d)), rows = static_cast<int64_t>(x.members) * a.group.d;
             const int32_t blocks = static_cast<int32_t>((rows + ROWS - 1) / ROWS), block = static_cast<int32_t>(nth / ROWS);
             halves = ROWS == 128 || rows - static_cast<int64_t>(block) * ROWS > 128 ? 1 : 2;
@@ -1288,12 +1308,12 @@ extern "C" int mf_prefix_attn_create(const mf_paged_attn_config* config, int32_t
     cudaError_t err = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel.fn), cudaFuncAttributeMaxDynamicSharedMemorySize, kernel.shared);
     const int ctas = state().sm_count;
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-    const size_t heads = static_cast<size_t>(max_requests) * c.q_heads;
+    const size_t heads = static_cast<size_t>(max_requests) * c.q_heads, alones = up(static_cast<size_t>(max_requests) * 4);
     const size_t firsts = up(static_cast<size_t>(max_requests) * 4), infos = up(static_cast<size_t>(max_requests) * sizeof(Shared));
     const size_t parts = up(2 * heads * k.head_dim * 4), part_mls = up(2 * heads * 8);
     const size_t cta_parts = up(static_cast<size_t>(ctas) * 256 * k.head_dim * 4), cta_mls = up(static_cast<size_t>(ctas) * 256 * 8);
     const size_t owns = up(heads * k.head_dim * 4), lses = up(heads * 4);
-    const size_t bytes = 256 + firsts + infos + parts + part_mls + cta_parts + cta_mls + owns + lses;
+    const size_t cleared = 256 + alones, bytes = cleared + firsts + infos + parts + part_mls + cta_parts + cta_mls + owns + lses;
     mf_prefix_attn_s* h = err == cudaSuccess ? new (std::nothrow) mf_prefix_attn_s{} : nullptr;
     if (!h) {
         mf_paged_attn_destroy(own);
@@ -1301,16 +1321,18 @@ extern "C" int mf_prefix_attn_create(const mf_paged_attn_config* config, int32_t
                                   : fail(MF_ERR_ALLOCATOR_EXHAUSTED, "mf_prefix_attn_create: out of host memory");
     }
     err = cudaMalloc(&h->workspace, bytes);
+    if (err == cudaSuccess) err = cudaMemset(h->workspace, 0, cleared);
+    if (err == cudaSuccess) err = cudaStreamSynchronize(nullptr);  // streams that do not wait for the default one may run it
     PrefixArgs& a = h->args;
     a.status = err == cudaSuccess ? sticky_status_ptr() : nullptr;
     if (!a.status) {
         cudaGetLastError();
-        if (err == cudaSuccess) cudaFree(h->workspace);
+        cudaFree(h->workspace);  // NULL: nothing
         delete h;
         mf_paged_attn_destroy(own);
         if (err == cudaErrorMemoryAllocation)
             return fail(MF_ERR_ALLOCATOR_EXHAUSTED, "mf_prefix_attn_create: %zu bytes: out of device memory", bytes);
-        return err != cudaSuccess ? cuda_fail(err, "mf_prefix_attn_create: cudaMalloc")
+        return err != cudaSuccess ? cuda_fail(err, "mf_prefix_attn_create: workspace")
                                   : fail(MF_ERR_CUDA, "mf_prefix_attn_create: sticky status word unavailable");
     }
     char* w = static_cast<char*>(h->workspace);
@@ -1319,7 +1341,8 @@ extern "C" int mf_prefix_attn_create(const mf_paged_attn_config* config, int32_t
     h->device = state().device;
     h->ctas = ctas;
     h->max_requests = max_requests;
-    a.max_pages = c.max_pages;
+    const int64_t reach = static_cast<int64_t>(c.max_pages) * k.page_size;
+    a.reach = reach < 0x7fffffff ? static_cast<int32_t>(reach) : 0x7fffffff;
     a.page = k.page_size;
     a.window = c.window;
     a.kv_heads = k.kv_heads;
@@ -1344,7 +1367,9 @@ extern "C" int mf_prefix_attn_create(const mf_paged_attn_config* config, int32_t
     a.out_req = c.out_token_stride;
     a.out_head = c.out_head_stride;
     a.cut = reinterpret_cast<int2*>(w);
-    a.own_first = reinterpret_cast<int32_t*>(w += 256);
+    a.call = reinterpret_cast<uint32_t*>(w + 64);
+    a.alone = reinterpret_cast<uint32_t*>(w += 256);
+    a.own_first = reinterpret_cast<int32_t*>(w += alones);
     a.info = reinterpret_cast<Shared*>(w += firsts);
     a.part = reinterpret_cast<float*>(w += infos);
     a.part_ml = reinterpret_cast<float2*>(w += parts);
@@ -1391,7 +1416,8 @@ extern "C" int mf_prefix_attn_run(mf_prefix_attn handle, const void* q, const vo
     cudaError_t err = launch_overlapped(handle->kernel.fn, dim3(static_cast<unsigned>(handle->ctas)), handle->kernel.threads,
                                         handle->kernel.shared, s, a);
     if (err != cudaSuccess) return cuda_fail(err, "mf_prefix_attn_run");
-    const int rc = paged_attn_run_parts(handle->own, q, k_cache, v_cache, table, lens, n_requests, a.own_first, a.own, a.own_lse, s);
+    const int rc = paged_attn_run_parts(handle->own, q, k_cache, v_cache, table, lens, n_requests, a.own_first, a.alone, a.call, a.own,
+                                        a.own_lse, s);
     if (rc != MF_OK) return rc;
     const int64_t grid = stream_grid(static_cast<int64_t>(n_requests) * a.q_heads * 32, kJoinThreads, 8);
     err = launch_overlapped(handle->kernel.join, dim3(static_cast<unsigned>(grid)), kJoinThreads, 0, s, a);

@@ -501,3 +501,86 @@ def test_prefix_destroyed_while_its_runs_are_queued(backend):
     check_prefix(s, got, want_attn(s))
     on.close()
     st.close()
+
+
+NAN = {BF16: 0x7FC0, F16: 0x7E00, E4M3: 0x7F, E5M2: 0x7F}
+INF = {BF16: 0x7F80, F16: 0x7C00, E4M3: 0x7F, E5M2: 0x7C}  # E4M3 has none
+
+
+@pytest.mark.parametrize("hq,hkv,dim", [(4, 2, 64), (16, 1, 72), (16, 2, 128), (32, 1, 128), (4, 2, 256)])
+@pytest.mark.parametrize("dtype,cache", TYPES)
+def test_prefix_values_that_a_member_does_not_see(backend, hq, hkv, dim, dtype, cache):
+    """Infinities and NaN among the shared tokens stay with the members that see them: 4, 2 or 1 warps for a row's tokens,
+    both groups of warps with rows of their own, one group."""
+    if cache in plain.FP8 and dim % 16:
+        dim = 80
+    s = make_groups([(300, [5, -1, -171, -300, 0, 20]), (140, [3, 0])], hq, hkv, dim, 16, "HND", dtype, cache, 5)
+    head, at = hkv - 1, 2
+
+    def put(part, token, number):
+        for r in range(6):  # all of them have the token in the leader's page, or in a copy
+            if s["lens"][r] > token or r == 0:
+                s["kv"][part][s["table"][r, token // 16], token % 16, head, at] = number[cache]
+
+    put(1, 131, INF)
+    put(1, 290, NAN)
+    on = Running(s)
+    device_status()
+    out, lse = on.run()
+    again = on.run()
+    assert device_status() == 0
+    on.close()
+    bits_equal(out, again[0])
+    bits_equal(lse.view(np.uint32), again[1].view(np.uint32))
+    want = [x.copy() for x in want_attn(s)]
+    sees = np.zeros(out.shape, bool)
+    sees[np.ix_([r for r in range(6) if s["lens"][r] > 131], range(head * (hq // hkv), hq), [at])] = True
+    assert not np.isfinite(want[0][sees]).any() and not np.isfinite(plain.values(out, dtype)[sees]).any()
+    out[sees] = 0
+    want[0][sees] = want[2][sees] = 0
+    check_prefix(s, (out, lse), want)
+
+
+@pytest.mark.parametrize("dtype,cache", [(BF16, BF16), (BF16, E4M3), (F16, E5M2)])
+@pytest.mark.parametrize("part", [0, 1])
+def test_prefix_values_that_no_member_sees(backend, dtype, cache, part):
+    """Behind every member's length, and in front of every member's window: whatever is there."""
+    s = make_groups([(300, [-40, -60, -50])], 4, 2, 64, 16, "HND", dtype, cache, 5)
+    for token in (260, 299):
+        s["kv"][part][s["table"][0, token // 16], token % 16] = NAN[cache]
+    for token in (0, 77):
+        s["kv"][part][s["table"][0, token // 16], token % 16] = INF[cache]
+    on = Running(s, window=100)
+    device_status()
+    got = on.run()
+    assert device_status() == 0
+    on.close()
+    check_prefix(s, got, want_attn(s, window=100))
+
+
+def test_prefix_finite_again_after_values_that_were_not(backend):
+    """What one call finds counts for that call alone."""
+    s = make_groups([(300, [5, -171, 0])], 4, 2, 64, 16, "NHD", BF16, BF16, 5)
+    on = Running(s)
+    first = on.run()
+    page, at = s["table"][0, 200 // 16], 200 % 16
+    wild = s["kv"][1].copy()
+    wild[page, at, 0, 7] = NAN[BF16]
+    on.bufs[2].upload(wild)
+    assert np.isnan(plain.values(on.run()[0], BF16)).sum() == 2 * 2  # two members see it, in two heads
+    on.bufs[2].upload(s["kv"][1])
+    last = on.run()
+    on.close()
+    bits_equal(first[0], last[0])
+    bits_equal(first[1].view(np.uint32), last[1].view(np.uint32))
+
+
+@pytest.mark.parametrize("rules", [{}, {"window": 40}, {"slopes": [0.5, 0.25, 0.125, 0.0625]}])
+def test_prefix_lengths_past_the_table(backend, rules):
+    """Lengths count as no more than the table's rows hold, for windows and slopes too."""
+    s = make_groups([(64, [32, 32])], 4, 2, 64, 16, "HND", BF16, BF16, 5)
+    s["table"] = np.ascontiguousarray(s["table"][:, :6])
+    on = Running({**s, "lens": np.array([96, 96 + 500], np.int32)}, **rules)
+    got = on.run()
+    on.close()
+    check_prefix(s, got, want_attn(s, **rules))
