@@ -52,7 +52,7 @@ struct BookArgs {
     int32_t* numbers;
     mf_page_move* moves;
     int64_t table_stride;
-    int32_t n_before, n_after, n_pages, max_pages, limit;
+    int32_t n_before, n_after, n_pages, max_pages, max_requests, limit;
     Divisor page;
     // workspace
     unsigned long long* first;  // [max_requests]: the first row that continues a row, behind the number of the call
@@ -195,6 +195,10 @@ __global__ void __launch_bounds__(kThreads, 1) fork_kernel(const BookArgs a) {
     after_previous();
     let_next_start();
     const uint32_t call = a.barrier[2];
+    if (call == 0) {  // the first call, or 2^32 later: higher numbers would count for more
+        for (int32_t p = me; p < a.max_requests; p += step) a.first[p] = 0;
+        if (!all_sync<GRID>(a)) return;
+    }
     int32_t head, count;
     pool_of(a, head, count);
     for (int64_t i0 = me; i0 < a.n_pages; i0 += static_cast<int64_t>(kEach) * step) {
@@ -344,6 +348,9 @@ __global__ void __launch_bounds__(kThreads, 1) fork_kernel(const BookArgs a) {
                     if (number[u] >= 0 && number[u] < a.n_pages) atomicAdd(a.shares_after + number[u], 1);
                     else atomicExch(a.status, MF_DEVICE_BAD_PAGE);
                 } else {
+                    if (static_cast<uint32_t>(number[u]) >= static_cast<uint32_t>(a.n_pages) ||
+                        static_cast<uint32_t>(mine) >= static_cast<uint32_t>(a.n_pages))
+                        atomicExch(a.status, MF_DEVICE_BAD_PAGE);
                     a.moves[x] = mf_page_move{number[u], mine, static_cast<int32_t>(len - full * a.page.d), 0};
                     number[u] = mine;
                 }
@@ -659,6 +666,7 @@ extern "C" int mf_page_book_create(const mf_page_book_config* config, mf_page_bo
     a.table_stride = c.table_stride;
     a.n_pages = c.n_pages;
     a.max_pages = c.max_pages;
+    a.max_requests = c.max_requests;
     a.page = divisor(c.page_size);
     a.barrier = reinterpret_cast<uint32_t*>(w);
     a.first = reinterpret_cast<unsigned long long*>(w += 256);

@@ -398,6 +398,26 @@ def test_fork_bad_pages_are_reported(backend):
     assert device_status() == BAD_PAGE
 
 
+def test_fork_bad_pages_of_the_list_and_behind_full_ones(backend):
+    """A page that is handed out, or the partly filled one that it is a copy of, outside the cache; one that nobody needs."""
+    lens, shares = np.array([20, 16], np.int32), np.zeros(8, np.int32)
+    table = np.array([[5, 1, -1], [3, -1, -1]], np.int32)
+    device_status()
+    for at, status in ((0, BAD_PAGE), (1, 0)):
+        for wild in (8, 99, -1, -2 ** 31):
+            free, pool = np.array([0, 2, 4, 6, 7, 0, 0, 0], np.int32), np.array([0, 5], np.int32)
+            free[at] = wild
+            run_fork(lens, table, shares, free, pool, np.array([0, 0, 1]), 16)
+            assert device_status() == status
+    free = np.array([0, 2, 4, 6, 7, 0, 0, 0], np.int32)
+    for wild in (8, -1):
+        table[0, 1] = wild
+        run_fork(lens, table, shares, free, np.array([0, 5], np.int32), np.array([0, 0, 1]), 16)
+        assert device_status() == BAD_PAGE
+        run_fork(lens, table, shares, free, np.array([0, 5], np.int32), np.array([0, 1]), 16)
+        assert device_status() == 0
+
+
 def run_compact(lens, table, shares, free, pool, limit, page, stream=None, stride=None):
     n, width = table.shape
     pages = len(shares)
