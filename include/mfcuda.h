@@ -741,20 +741,22 @@ int mf_page_copy(const mf_cache_layout* layout, void* const* caches, int32_t n_c
 /* mf_paged_attn_run for groups of requests that share their first tokens.
  * Requests starts[g] .. starts[g + 1] - 1 (starts: n_groups + 1 ascending
  * entries on the device) form group g and have the same pages for their first
- * shared[g] tokens, which are read once for all of them, through the table row
- * of the group's first request, as products on the tensor cores whose rows are
- * the group's queries; the tokens behind them are read request by request.
+ * shared[g] tokens, which are read once for all of them, as products on the tensor
+ * cores whose rows are the group's queries; the tokens behind them are read request
+ * by request.
  * out and lse are those that mf_paged_attn_run defines, for every request, with
  * the window, cap, slopes and scales of the config; shared[g] may be any number
  * of tokens (negative: 0), and a member may be shorter than it.  Requests in no
  * group share nothing.  starts that descend or leave the requests, and groups of
  * more than 2^31 - 1 tiles of tokens together, record MF_DEVICE_TOO_LARGE: nothing
- * counts as shared then, and the results are the same.  The first request's table
- * row names all shared pages, even if that request is shorter or idle, or sees none
- * of their tokens (a page outside the cache records MF_DEVICE_BAD_PAGE); the others'
- * rows name those that they see, as in mf_paged_attn_run.  A request in whose shared
- * tokens an infinity or NaN turns up, seen by it or not, is read request by request,
- * so that only what it sees counts.
+ * counts as shared then, and the results are the same.
+ * A request's table row names the pages of the tokens that it sees, as in
+ * mf_paged_attn_run.  Shared tokens are read through the row of the first request
+ * that reaches farthest into them; with a window that row names what the shorter
+ * ones see, too.  What no request of the group sees is not read, and idle requests
+ * may stand anywhere in it.  Where an infinity or NaN turns up among what a
+ * request's rows sum, seen by it or not, all its tokens are read for it alone, so
+ * that only what it sees counts.
  * Over the shared tokens the weights exp(s - max) enter the product with the
  * values as two 16-bit terms, as in mf_paged_attn_run, but as one f16 term over an
  * FP8 cache with BF16 queries (off by 2^-11 of a weight at most, an eighth of the

@@ -344,21 +344,57 @@ __device__ __forceinline__ uint32_t place(int rows, int row, int c) {
 
 // ------------------------------------------------------------------ roles
 
+// Of a group's shared tokens those that some request sees, and the first of the requests that reach the last of them: its row
+// of the table is read.  Others (idle, shorter) may name less.
+struct Lead {
+    int32_t row, from, to;
+};
+__device__ __forceinline__ Lead lead_of(const PrefixArgs& a, const Group& of) {
+    constexpr int kEach = 4;  // loads that a lane has on their way
+    const int lane = threadIdx.x & 31;
+    int32_t most = 0, least = 0x7fffffff, who = 0;
+    for (int32_t i0 = 0; i0 < of.members; i0 += 32 * kEach) {
+        int32_t len[kEach];
+#pragma unroll
+        for (int u = 0; u < kEach; ++u) len[u] = of.members - i0 > u * 32 + lane ? min(a.lens[of.start + i0 + u * 32 + lane], a.reach) : 0;
+#pragma unroll
+        for (int u = 0; u < kEach; ++u) {
+            if (len[u] > 0) least = min(least, len[u]);
+            const int32_t sees = min(len[u], of.shared);
+            if (sees > most) {
+                most = sees;
+                who = i0 + u * 32 + lane;
+            }
+        }
+        if (a.window == 0 && __any_sync(0xffffffffu, most == of.shared)) break;
+    }
+    const int32_t to = __reduce_max_sync(0xffffffffu, most);
+    who = __reduce_min_sync(0xffffffffu, most == to ? who : 0x7fffffff);
+    least = __reduce_min_sync(0xffffffffu, least);
+    return Lead{of.start + who, a.window > 0 && to > 0 && least > a.window ? least - a.window : 0, to};
+}
+
 // One warp finds the rows of the tiles to come in the page table.
 template <class K>
 __device__ __forceinline__ void find_rows(const PrefixArgs& a, typename K::Shared& sh, Run<K> run) {
     const int lane = threadIdx.x & 31;
     uint32_t tile = 0;
     bool more = run.n > 0;
+    Lead lead = lead_of(a, run.of);
+    int32_t group = run.g;
     while (more) {
-        const int64_t at_row = static_cast<int64_t>(run.of.start) * a.table_stride;
+        if (run.g != group) {
+            group = run.g;
+            lead = lead_of(a, run.of);
+        }
+        const int64_t at_row = static_cast<int64_t>(lead.row) * a.table_stride;
         for (int32_t i = 0; i < run.n; ++i, ++tile) {
             uint32_t off[K::T / 32];
             int32_t number[K::T / 32];
 #pragma unroll
             for (int w = 0; w < K::T / 32; ++w) {
                 const uint32_t tok = static_cast<uint32_t>(run.t + i) * K::T + w * 32 + lane, idx = tok / a.by_page;
-                const bool in = tok < static_cast<uint32_t>(run.of.shared);
+                const bool in = tok >= static_cast<uint32_t>(lead.from) && tok < static_cast<uint32_t>(lead.to);
                 off[w] = in ? (tok - idx * a.page) * a.row_units : kMasked;
                 number[w] = in ? a.table[at_row + idx] : 0;
             }

@@ -584,3 +584,37 @@ def test_prefix_lengths_past_the_table(backend, rules):
     got = on.run()
     on.close()
     check_prefix(s, got, want_attn(s, **rules))
+
+
+WILD = 1 << 30
+
+
+@pytest.mark.parametrize("own", [[-300, 5, -1, 0], [-170, -300, 9], [-40, -60, -50], [-60, -40, -40], [-299, -300], [-300, -300, -300],
+                                 [-300] * 40 + [3] * 5, [-1] * 150 + [0] * 2])
+@pytest.mark.parametrize("dim,cache", [(64, BF16), (128, E4M3), (256, BF16)])
+def test_prefix_rows_of_the_table_name_what_their_request_has(backend, own, dim, cache):
+    """Idle and shorter requests in front: nothing behind a request's own length is read of its row."""
+    s = make_groups([(300, own), (64, [0, 2])], 4, 2, dim, 16, "HND", BF16, cache, 5)
+    want = want_attn(s)
+    for r, n in enumerate(s["lens"]):
+        s["table"][r, -(-max(n, 0) // 16):] = WILD
+    on = Running(s)
+    device_status()
+    got = on.run()
+    assert device_status() == 0
+    on.close()
+    check_prefix(s, got, want)
+
+
+@pytest.mark.parametrize("window", [1, 100, 250])
+def test_prefix_pages_in_front_of_every_window_are_not_read(backend, window):
+    s = make_groups([(300, [-40, 7, -300, 0, 30])], 4, 2, 64, 16, "HND", BF16, BF16, 5)
+    want = want_attn(s, window=window)
+    s["table"][:, :(260 - window) // 16] = WILD
+    s["table"][2] = WILD
+    on = Running(s, window=window)
+    device_status()
+    got = on.run()
+    assert device_status() == 0
+    on.close()
+    check_prefix(s, got, want)
