@@ -32,7 +32,7 @@ constexpr int kMostBeams = 1024;     // beams of a batch entry
 constexpr int kParts = 4;            // of what a thread meets, with a maximum each
 constexpr int kGroups = 32;          // maxima that bound a list of up to kGroups
 constexpr int kPicked = 512;         // logits that may be ranked by counting
-constexpr int kCtas = 3;             // CTAs that a batch is cut into for every SM, at least (7: 45 us for the 39.5 below)
+constexpr int kCtas = 3;             // CTAs that a batch is cut into for every SM, at least (4 and 6: two segments of a row below, 41 us for 39.5; 7: three, 45)
 constexpr float kLog2e = 1.44269504088896341f;
 
 struct SelectArgs {

@@ -380,8 +380,8 @@ __device__ __forceinline__ void find_rows(const PrefixArgs& a, typename K::Share
     const int lane = threadIdx.x & 31;
     uint32_t tile = 0;
     bool more = run.n > 0;
-    Lead lead = lead_of(a, run.of);
-    int32_t group = run.g;
+    Lead lead{0, 0, 0};
+    int32_t group = -1;
     while (more) {
         if (run.g != group) {
             group = run.g;
