@@ -32,7 +32,9 @@ constexpr int kMostBeams = 1024;     // beams of a batch entry
 constexpr int kParts = 4;            // of what a thread meets, with a maximum each
 constexpr int kGroups = 32;          // maxima that bound a list of up to kGroups
 constexpr int kPicked = 512;         // logits that may be ranked by counting
-constexpr int kCtas = 3;             // CTAs that a batch is cut into for every SM, at least (4 and 6: two segments of a row below, 41 us for 39.5; 7: three, 45)
+// CTAs that a batch is cut into for every SM, at least.  Of the 64 x 8 rows below 3 make one segment each; 4 and 6 two (41 us for
+// 39.5), 7 three (45).
+constexpr int kCtas = 3;
 constexpr float kLog2e = 1.44269504088896341f;
 
 struct SelectArgs {
@@ -301,12 +303,17 @@ __device__ void merge_lists(const SelectArgs& a, int32_t entry, SelectShared& sh
         a.parents[to] = there ? row0 + k : -1;
         if (a.ended_after) a.ended_after[to] = there && token == a.end_token;
     };
-    // every thread's largest entry; entries that follow one another go to different groups of threads
+    // Every thread's largest entry; entries that follow one another go to different groups of threads.  From one round to the next
+    // the threads turn by some 3/8 of a list, an odd number: else a group has entries of one rank where n_out divides kGroups, and
+    // the bound lets too many through (8 beams of 122286 in 480 lists, 16 results: 98 us).
     const int32_t entries = n_lists * a.n_out, first = tid % (kThreads / kGroups) * kGroups + tid / (kThreads / kGroups);
+    const int32_t turn = ((a.n_out * 3 / 8 | 1) + a.n_out - kThreads % a.n_out) % a.n_out;
     double mine = -INFINITY, v;
     int32_t i;
 #pragma unroll 4
-    for (int32_t x = first; x < entries; x += kThreads) {
+    for (int32_t x0 = 0, at = first; x0 < entries; x0 += kThreads, at = (at + turn) & (kThreads - 1)) {
+        const int32_t x = x0 + at;
+        if (x >= entries) continue;
         const int32_t l = x / a.n_out;
         get(l, x - l * a.n_out, v, i);
         mine = v > mine ? v : mine;

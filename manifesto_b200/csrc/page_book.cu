@@ -586,6 +586,10 @@ struct mf_page_book_s {
 
 namespace {
 
+// What a row of the table counts as: a warp takes up to 128 entries of it at a time, and as long for fewer (4 rows of a page
+// continued by 1271, counted as they are, left one CTA with all of it: 38 us).
+int64_t row_entries(int32_t max_pages) { return (static_cast<int64_t>(max_pages) + 127) / 128 * 128; }
+
 // One launch: a cluster where the entries to read and write are few, else a grid of all SMs.
 template <class Kernel>
 int launch_book(mf_page_book h, Kernel cluster_kernel, Kernel grid_kernel, const BookArgs& a, int64_t entries, cudaStream_t s,
@@ -712,7 +716,7 @@ extern "C" int mf_page_book_fork(mf_page_book handle, const int32_t* table, cons
     a.moves = moves;
     a.n_before = n_before;
     a.n_after = n_after;
-    const int64_t entries = (static_cast<int64_t>(n_before) + n_after) * handle->config.max_pages + 3ll * handle->config.n_pages;
+    const int64_t entries = (static_cast<int64_t>(n_before) + n_after) * row_entries(handle->config.max_pages) + 3ll * handle->config.n_pages;
     return launch_book(handle, fork_kernel<false>, fork_kernel<true>, a, entries, static_cast<cudaStream_t>(stream),
                        "mf_page_book_fork");
 }
@@ -748,7 +752,7 @@ extern "C" int mf_page_book_compact(mf_page_book handle, const int32_t* table, c
     a.moves = moves;
     a.n_before = n_requests;
     a.limit = limit;
-    const int64_t entries = 2ll * n_requests * handle->config.max_pages + 4ll * handle->config.n_pages;
+    const int64_t entries = 2ll * n_requests * row_entries(handle->config.max_pages) + 4ll * handle->config.n_pages;
     return launch_book(handle, compact_kernel<false>, compact_kernel<true>, a, entries, static_cast<cudaStream_t>(stream),
                        "mf_page_book_compact");
 }

@@ -108,6 +108,20 @@ def test_select_batches_and_beams(backend, dtype, batch, k, n):
     run_select(logits_of(batch * k, 9001, batch + n), -rng.random(batch * k) * 2 - 30, k, n, dtype)
 
 
+@pytest.mark.parametrize("batch,k,vocab", [(1, 8, 60000), (3, 4, 30011), (1, 1, 120000), (2, 3, 4100)])
+@pytest.mark.parametrize("n", [2, 8, 16, 31, 32, 33, 100, 128])
+def test_select_merges_many_lists(backend, batch, k, vocab, n):
+    """Rows in many segments; beams near one another, one far ahead, one that has ended."""
+    rng = np.random.default_rng(n + k)
+    logits = rng.normal(0, 3, (batch * k, vocab))
+    run_select(logits, rng.normal(-20, 1, batch * k), k, n, F16)
+    scores = rng.normal(-40, 5, batch * k)
+    scores[::k] = -3.0
+    ended = np.zeros(batch * k, np.int32)
+    ended[k - 1::k] = 1
+    run_select(logits, scores, k, n, F16, ended=ended, end=5)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("pad,offset", [(0, 1), (1, 0), (5, 3), (8, 8), (3, 7)])
 def test_select_row_strides_and_alignment(backend, dtype, pad, offset):
