@@ -93,7 +93,8 @@ def run(prompts=(37, 5, 64), beams: int = 4, steps: int = 6, heads: int = 8, kv_
 
     assign = paged.PageAssigner(page, width)
     append = paged.RopeAppend(paged.Rope(freq.ptr, DType.BFLOAT16, dim), layout, heads, compat=COMPAT_OCP, token_stride=per_token, **scales)
-    attend = paged.PrefixAttention(layout, heads, DType.BFLOAT16, width, rows, **scales)
+    # shared always: prompts as short as these would be read beam by beam
+    attend = paged.PrefixAttention(layout, heads, DType.BFLOAT16, width, rows, always=True, **scales)
     select = beam.BeamSelect(DType.FLOAT32, vocab, beams, beams, n)
     book = paged.PageBook(page, width, pages, rows)
     copy = paged.PageCopy(layout, [c.ptr for c in cache])

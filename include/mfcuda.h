@@ -742,8 +742,8 @@ int mf_page_copy(const mf_cache_layout* layout, void* const* caches, int32_t n_c
  * Requests starts[g] .. starts[g + 1] - 1 (starts: n_groups + 1 ascending
  * entries on the device) form group g and have the same pages for their first
  * shared[g] tokens, which are read once for all of them, as products on the tensor
- * cores whose rows are the group's queries; the tokens behind them are read request
- * by request.
+ * cores whose rows are the group's queries; the tokens behind them, and those of
+ * groups that are too small for that to pay, are read request by request.
  * out and lse are those that mf_paged_attn_run defines, for every request, with
  * the window, cap, slopes and scales of the config; shared[g] may be any number
  * of tokens (negative: 0), and a member may be shorter than it.  Requests in no
@@ -772,6 +772,10 @@ int mf_prefix_attn_create(const mf_paged_attn_config* config, int32_t max_reques
 int mf_prefix_attn_run(mf_prefix_attn handle, const void* q, const void* k_cache, const void* v_cache,
                        const int32_t* table, const int32_t* lens, int32_t n_requests, const int32_t* starts,
                        const int32_t* shared, int32_t n_groups, void* out, float* lse, mf_stream stream);
+/* Whether the runs that follow share whatever the groups can (1), or, as they do
+ * from the start (0), where that is quicker than to read the tokens once more
+ * for each request: a rule on the numbers of requests, tokens and heads. */
+int mf_prefix_attn_share(mf_prefix_attn handle, int32_t always);
 int mf_prefix_attn_destroy(mf_prefix_attn handle);
 
 /* ---------------------------------------------------------------------

@@ -89,6 +89,8 @@ struct PrefixArgs {
     const float* slopes;
     const float* k_scale;
     const float* v_scale;
+    int32_t always;       // share whatever can be shared
+    float token_ps;       // of reading a token again, see kItemPs
     // workspace
     int32_t* own_first;   // [requests]
     Shared* info;         // [requests]
@@ -179,11 +181,19 @@ constexpr int kSoftmaxRegs = 192, kProducerRegs = 64, kOtherRegs = 64;
 constexpr int kPlaces = 4;  // tiles whose rows are known in advance
 constexpr int kMasks = 16;  // tiles whose masks are kept: more than the ring and the places hold
 
-// Shared tokens of a group, and its requests; nothing is shared by a request alone.
+// Shared tokens of a group, and its requests; nothing is shared by a request alone, nor where it does not pay.
 struct Group {
     int32_t start, members, shared;
+    float worth;  // what sharing saves, in picoseconds of the whole GPU
     bool bad;
 };
+// Whether a group's tokens are shared, and whether any are.  The requests of a group follow one another, so that its tokens come
+// out of L2 for all but the first of them: reading them again costs 40 ps a token and key-value head of 128 (30 of FP8 codes)
+// with all SMs at work, an item of shared tokens 47 ns (7 us of one CTA), a tile 8 (twice that with more than 128 rows), and the
+// first of them all delays the rest.  32/8 heads of 128, BF16, us with sharing and without: 100 groups of 2 that share 48
+// tokens 84 and 39, 30 groups of 16 with 48 83 and 54, with 800 106 and 180; 6 of 16 with 800 62 and 50, with 3200 77 and 95;
+// one of 4 with 896 32 and 20.
+constexpr float kItemPs = 47e3f, kTilePs = 8e3f, kFirstPs = 25e6f;
 constexpr uint32_t kMasked = 0xffffffffu;
 
 // MODE: dtype of the cache; DP: head_dim padded to 64, 128 or 256.
@@ -220,6 +230,7 @@ struct Prefix {
     static constexpr int kBytes = kRing + kStreams * kQ + static_cast<int>(sizeof(Shared));
 };
 
+template <class K>
 __device__ __forceinline__ Group group_of(const PrefixArgs& a, int32_t g) {
     Group x;
     const int32_t s = a.starts[g], e = a.starts[g + 1];
@@ -227,6 +238,14 @@ __device__ __forceinline__ Group group_of(const PrefixArgs& a, int32_t g) {
     x.start = s;
     x.members = x.bad ? 0 : e - s;
     x.shared = x.members < 2 ? 0 : min(max(a.shared[g], 0), a.reach);
+    const float heads = static_cast<float>(a.kv_heads), rows = static_cast<float>(x.members) * static_cast<float>(a.group.d);
+    const float tiles = ceilf(static_cast<float>(x.shared) * (1.0f / K::T)), items = ceilf(rows * (1.0f / K::kRows));
+    x.worth = heads * (static_cast<float>(x.members - 1) * static_cast<float>(x.shared) * a.token_ps -
+                       items * (kItemPs + tiles * (rows > 128.0f ? 2.0f * kTilePs : kTilePs)));
+    if (x.worth <= 0.0f || x.shared == 0) {
+        x.worth = 0.0f;
+        if (!a.always) x.shared = 0;
+    }
     return x;
 }
 template <class K>
@@ -304,7 +323,7 @@ struct Run {
                 if (++item == items) {
                     item = 0;
                     do {
-                        of = group_of(a, ++g);
+                        of = group_of<K>(a, ++g);
                         tiles = tiles_of<K>(of);
                     } while (tiles == 0 && g + 1 < a.n_groups);
                     items = static_cast<int32_t>(items_of<K>(a, of));
@@ -1006,20 +1025,20 @@ __device__ __forceinline__ void soften(const PrefixArgs& a, typename K::Shared& 
 
 // One warp tells the other launches each request's first token of its own, and where its shared part's pieces will be.
 template <class K>
-__device__ __forceinline__ void take_notes(const PrefixArgs& a, bool bad) {
+__device__ __forceinline__ void take_notes(const PrefixArgs& a, bool none) {
     const int lane = threadIdx.x & 31;
-    const int32_t begin = bad || a.n_groups == 0 ? a.n_requests : a.starts[0], end = bad || a.n_groups == 0 ? a.n_requests : a.starts[a.n_groups];
+    const int32_t begin = none || a.n_groups == 0 ? a.n_requests : a.starts[0], end = none || a.n_groups == 0 ? a.n_requests : a.starts[a.n_groups];
     for (int32_t r = blockIdx.x * 32 + lane; r < a.n_requests; r += gridDim.x * 32)
         if (r < begin || r >= end) {
             a.own_first[r] = 0;
             a.info[r] = Shared{0, 0, 0, 0};
         }
-    if (bad) return;
+    if (none) return;
     int64_t front = 0;
     for (int32_t g0 = 0; g0 < a.n_groups; g0 += 32) {
         const int32_t g = g0 + lane;
-        Group x{0, 0, 0, false};
-        if (g < a.n_groups) x = group_of(a, g);
+        Group x{};
+        if (g < a.n_groups) x = group_of<K>(a, g);
         const int64_t of = items_of<K>(a, x) * places_of<K>(x);
         int64_t upto = of;
 #pragma unroll
@@ -1078,15 +1097,18 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const PrefixArgs a)
     let_next_start();
     // the tiles of thread i's `per` consecutive groups, in a row
     int64_t* sums = reinterpret_cast<int64_t*>(queries);  // of the warps, before the queries come
+    float* worths = reinterpret_cast<float*>(sums + kThreads / 32);
     const int32_t per = (a.n_groups + kThreads - 1) / kThreads;
     int64_t mine = 0;
     bool bad = false;
-    Group last{0, 0, 0, false};
+    Group last{};
+    float worth = 0.0f;
     for (int32_t i = 0; i < per; ++i) {
         const int32_t g = tid * per + i;
         if (g >= a.n_groups) break;
-        last = group_of(a, g);
+        last = group_of<K>(a, g);
         bad |= last.bad;
+        worth += last.worth;
         mine += items_of<K>(a, last) * places_of<K>(last);
     }
     int64_t upto = mine;
@@ -1095,7 +1117,12 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const PrefixArgs a)
         const int64_t x = __shfl_up_sync(0xffffffffu, upto, d);
         if (lane >= d) upto += x;
     }
-    if (lane == 31) sums[warp] = upto;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) worth += __shfl_xor_sync(0xffffffffu, worth, d);
+    if (lane == 31) {
+        sums[warp] = upto;
+        worths[warp] = worth;
+    }
     // what is past the head in a row is never copied: zeros
     if (a.head_dim < DP) {
         for (int i = tid; i < K::kRing / 16; i += kThreads) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
@@ -1106,8 +1133,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const PrefixArgs a)
     tc_fence_after();
     const uint32_t tmem = sh.tmem, ring = smem_u32(smem);
     int64_t total64 = 0, front = 0;
+    worth = 0.0f;
 #pragma unroll
     for (int w = 0; w < kThreads / 32; ++w) {
+        worth += worths[w];
         if (w == warp) front = total64;
         total64 += sums[w];
     }
@@ -1116,8 +1145,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const PrefixArgs a)
         // nothing is shared then: every request reads all of its tokens
         if (tid == 0) atomicExch(a.status, MF_DEVICE_TOO_LARGE);
         bad = true;
-        total64 = 0;
     }
+    const bool none = bad || (!a.always && worth < kFirstPs);
+    if (none) total64 = 0;
     const int32_t total = static_cast<int32_t>(total64), ctas = min(total, static_cast<int32_t>(gridDim.x));
     if (blockIdx.x == 0 && tid == 0) {
         *a.cut = make_int2(total, ctas);
@@ -1130,7 +1160,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const PrefixArgs a)
             int32_t into = x0 - static_cast<int32_t>(front), g = tid * per;
             if (per > 1) {
                 for (;; ++g) {
-                    last = group_of(a, g);
+                    last = group_of<K>(a, g);
                     const int64_t of = items_of<K>(a, last) * places_of<K>(last);
                     if (into < of) break;
                     into -= static_cast<int32_t>(of);
@@ -1153,11 +1183,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const PrefixArgs a)
             asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
             if (warp == kIssuer) multiply<K>(a, sh, ring, smem_u32(queries), tmem, run);
             else if (warp == kPager) find_rows<K>(a, sh, run);
-            else if (warp == kNoter) take_notes<K>(a, bad);
+            else if (warp == kNoter) take_notes<K>(a, none);
         }
         __syncwarp();
     } else if (warp == kNoter) {
-        take_notes<K>(a, bad);
+        take_notes<K>(a, none);
     }
     tc_fence_before();
     __syncthreads();
@@ -1380,6 +1410,8 @@ extern "C" int mf_prefix_attn_create(const mf_paged_attn_config* config, int32_t
     const int64_t reach = static_cast<int64_t>(c.max_pages) * k.page_size;
     a.reach = reach < 0x7fffffff ? static_cast<int32_t>(reach) : 0x7fffffff;
     a.page = k.page_size;
+    a.always = 0;
+    a.token_ps = (10.0f + k.head_dim * (is_fp8(k.dtype) ? 5.0f : 7.5f) / 32.0f) * ((c.q_heads / k.kv_heads + 15) / 16);
     a.window = c.window;
     a.kv_heads = k.kv_heads;
     a.unit = 1u << unit;
@@ -1414,6 +1446,14 @@ extern "C" int mf_prefix_attn_create(const mf_paged_attn_config* config, int32_t
     a.own = reinterpret_cast<float*>(w += cta_mls);
     a.own_lse = reinterpret_cast<float*>(w += owns);
     *handle = h;
+    return MF_OK;
+}
+
+extern "C" int mf_prefix_attn_share(mf_prefix_attn handle, int32_t always) {
+    MF_ENTER();
+    if (!handle) return fail(MF_ERR_INVALID_ARGUMENT, "mf_prefix_attn_share: handle is NULL");
+    if (always != 0 && always != 1) return fail(MF_ERR_INVALID_ARGUMENT, "mf_prefix_attn_share: %d (0 or 1)", always);
+    handle->args.always = always;
     return MF_OK;
 }
 

@@ -247,7 +247,7 @@ class PrefixAttention(_Handle):
     """``PagedAttention`` for groups of requests that share the pages of their first tokens (mf_prefix_attn_*).
 
     The shared tokens of a group are read once for all its requests: the beams of a prompt, or a batch that begins
-    with the same instructions.  Holds the workspace for up to ``max_requests``, so one object serves one stream at
+    with the same instructions; small groups, for which that does not pay, only with ``always``.  Holds the workspace for up to ``max_requests``, so one object serves one stream at
     a time; it runs any number of requests, groups, steps and layers of its shape."""
 
     _destroy = "mf_prefix_attn_destroy"
@@ -255,10 +255,12 @@ class PrefixAttention(_Handle):
     def __init__(self, cache: CacheLayout, q_heads: int, dtype: DType, max_pages: int, max_requests: int,
                  table_stride: int | None = None, scale: float | None = None, softcap: float = 0.0, window: int = 0,
                  slopes: int = 0, k_scale_inv: int = 0, v_scale_inv: int = 0, q_strides: tuple[int, int] | None = None,
-                 out_strides: tuple[int, int] | None = None):
+                 out_strides: tuple[int, int] | None = None, always: bool = False):
         self.config = _attn_config(cache, q_heads, dtype, max_pages, table_stride, scale, softcap, window, slopes, k_scale_inv,
                                    v_scale_inv, q_strides, out_strides)
         self._create("mf_prefix_attn_create", ctypes.byref(self.config), int(max_requests))
+        if always:
+            _abi.call("mf_prefix_attn_share", self._handle, 1)
         self._attend = _abi.lib().mf_prefix_attn_run
 
     def run(self, q: int, k_cache: int, v_cache: int, table: int, lens: int, n_requests: int, starts: int, shared: int,

@@ -56,7 +56,7 @@ def check_prefix(s, got, want):
 class Running:
     """The case on the device."""
 
-    def __init__(self, s, softcap=0.0, window=0, slopes=None, scale=None, q_pad=0, max_requests=None):
+    def __init__(self, s, softcap=0.0, window=0, slopes=None, scale=None, q_pad=0, max_requests=None, always=True):
         self.s = s
         kv = [c if s["order"] == "NHD" else np.ascontiguousarray(c.transpose(0, 2, 1, 3)) for c in s["kv"]]
         n, hq, dim = s["q"].shape
@@ -72,7 +72,7 @@ class Running:
         layout = paged.CacheLayout(s["pages"], s["page"], s["hkv"], dim, s["cache"], s["order"])
         self.attn = paged.PrefixAttention(layout, hq, s["dtype"], s["table"].shape[1], max_requests or n, scale=scale, softcap=softcap,
                                           window=window, slopes=sl, k_scale_inv=ks, v_scale_inv=ks + 4 * s["hkv"] if ks else 0,
-                                          q_strides=(hq * (dim + q_pad), dim + q_pad), out_strides=(hq * width, width))
+                                          q_strides=(hq * (dim + q_pad), dim + q_pad), out_strides=(hq * width, width), always=always)
 
     def run(self, stream=None, lse=True, groups=None):
         s = self.s
@@ -417,7 +417,8 @@ def test_prefix_offsets_past_32_bits(backend, page, cache):
     b = [to_device(a) for a in (s["q"], table, s["lens"], s["starts"], s["shared"])]
     sc = to_device(s["scales"]) if s["scales"] is not None else None
     out, lse = empty(2 * 3 * 4 * 64), empty(4 * 3 * 4)
-    with paged.PrefixAttention(layout, 4, BF16, table.shape[1], 3, k_scale_inv=sc.ptr if sc else 0, v_scale_inv=sc.ptr + 8 if sc else 0) as attn:
+    with paged.PrefixAttention(layout, 4, BF16, table.shape[1], 3, k_scale_inv=sc.ptr if sc else 0, v_scale_inv=sc.ptr + 8 if sc else 0,
+                               always=True) as attn:
         attn.run(b[0].ptr, kv[0].ptr, kv[1].ptr, b[1].ptr, b[2].ptr, 3, b[3].ptr, b[4].ptr, 1, out.ptr, lse.ptr)
         sync_device()
     assert device_status() == 0
@@ -444,7 +445,7 @@ def test_prefix_padded_tables_and_caches(backend):
     layout.struct.head_stride = dim + 8
     b = [to_device(x) for x in (s["q"], table, s["lens"], s["starts"], s["shared"])]
     out, lse = empty(2 * n * hq * dim), empty(4 * n * hq)
-    with paged.PrefixAttention(layout, hq, BF16, width, n, table_stride=width + 5) as attn:
+    with paged.PrefixAttention(layout, hq, BF16, width, n, table_stride=width + 5, always=True) as attn:
         attn.run(b[0].ptr, kv[0].ptr, kv[1].ptr, b[1].ptr, b[2].ptr, n, b[3].ptr, b[4].ptr, 2, out.ptr, lse.ptr)
         sync_device()
     assert device_status() == 0
@@ -618,3 +619,32 @@ def test_prefix_pages_in_front_of_every_window_are_not_read(backend, window):
     assert device_status() == 0
     on.close()
     check_prefix(s, got, want)
+
+
+@pytest.mark.parametrize("dtype,cache", [(BF16, BF16), (F16, E4M3)])
+def test_prefix_shared_where_it_pays(backend, dtype, cache):
+    """Large groups beside small ones; small ones alone; the same where all are shared, or none."""
+    for groups in ([(3000, [2] * 60), (20, [1, 2]), (1900, [3] * 70), (700, [1, 0, 5])], [(48, [1, 2])] * 9):
+        s = make_groups(groups, 8, 4, 128, 16, "HND", dtype, cache, 3, alone=2)
+        want = want_attn(s)
+        for always in (True, False):
+            on = Running(s, always=always)
+            device_status()
+            got, none = on.run(), on.run(groups=0)
+            assert device_status() == 0
+            on.close()
+            check_prefix(s, got, want)
+            check_prefix(s, none, want)
+            if not always and len(groups) == 9:  # too small: as if there were no groups, to the bit
+                bits_equal(got[0], none[0])
+
+
+def test_prefix_share_refusals(backend):
+    s = make_groups([(20, [1, 2])], 4, 2, 64, 16, "HND", BF16, BF16, 3)
+    on = Running(s)
+    for always in (-1, 2):
+        with pytest.raises(InvalidArgument):
+            call("mf_prefix_attn_share", on.attn._handle, always)
+    on.close()
+    with pytest.raises(InvalidArgument):
+        call("mf_prefix_attn_share", None, 1)
