@@ -38,7 +38,8 @@
 // a window).  So a row that ends with such a number marks its request for the call,
 // and the second launch reads all of that request's tokens, masked ones not at all.
 //
-// Measured (B200): 250 requests behind 8192 shared tokens, 32/8 heads of 128, BF16:
+// Measured (B200; the whole calls are 2 to 3 us slower since, for the check of what is
+// not finite and the scan for a group's row): 250 requests behind 8192 shared tokens, 32/8 heads of 128, BF16:
 // this kernel 67 us from cold caches (the products at the measured rate of the tensor cores: 20 us,
 // 31 with the low terms), tensor pipe 41% of the time busy.  Bound by latency: a
 // step's chain is some 5 thousand clocks (scores 0.5, softmax 2.4 to 3, values 1.0,
