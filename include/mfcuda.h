@@ -776,6 +776,11 @@ int mf_prefix_attn_run(mf_prefix_attn handle, const void* q, const void* k_cache
  * from the start (0), where that is quicker than to read the tokens once more
  * for each request: a rule on the numbers of requests, tokens and heads. */
 int mf_prefix_attn_share(mf_prefix_attn handle, int32_t always);
+/* How long, in nanoseconds, the runs that follow may wait for one another's parts inside a CTA: 2 * 10^9 from the start, 0
+ * to 2^32 - 1 (0: not at all, every run that shares tokens is given up).  A run whose wait runs out, as where the GPU is
+ * taken away from it for that long, records MF_DEVICE_TIMEOUT and comes to its end; what it wrote to out and lse counts
+ * for nothing.  The runs behind it are as ever. */
+int mf_prefix_attn_limit(mf_prefix_attn handle, int64_t wait_ns);
 int mf_prefix_attn_destroy(mf_prefix_attn handle);
 
 /* ---------------------------------------------------------------------

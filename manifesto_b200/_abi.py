@@ -221,6 +221,7 @@ SIGNATURES: dict[str, list] = {
     "mf_prefix_attn_create": [ctypes.POINTER(PagedAttnConfig), _i32, ctypes.POINTER(_vp)],
     "mf_prefix_attn_run": [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _i32, _vp, _vp, _vp],
     "mf_prefix_attn_share": [_vp, _i32],
+    "mf_prefix_attn_limit": [_vp, _i64],
     "mf_prefix_attn_destroy": [_vp],
     "mf_beam_select_create": [ctypes.POINTER(BeamSelectConfig), ctypes.POINTER(_vp)],
     "mf_beam_select_run": [_vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp],

@@ -92,6 +92,7 @@ struct PrefixArgs {
     const float* v_scale;
     int32_t always;       // share whatever can be shared
     float token_ps;       // of reading a token again, see kItemPs
+    uint32_t wait_ns;     // that a wait may last
     // workspace
     int32_t* own_first;   // [requests]
     Shared* info;         // [requests]
@@ -182,6 +183,12 @@ constexpr int kSoftmaxRegs = 192, kProducerRegs = 64, kOtherRegs = 64;
 constexpr int kPlaces = 4;  // tiles whose rows are known in advance
 constexpr int kMasks = 16;  // tiles whose masks are kept: more than the ring and the places hold
 
+// How long the waits of a CTA may last, and whether one has run out.
+struct Waits {
+    uint32_t ns;
+    int32_t abandoned;
+};
+
 // Shared tokens of a group, and its requests; nothing is shared by a request alone, nor where it does not pay.
 struct Group {
     int32_t start, members, shared;
@@ -222,7 +229,7 @@ struct Prefix {
         uint64_t s_full[2], p_full[2], o_done[2], q_full[2], drained;
         uint64_t rows_known[kPlaces], rows_used[kPlaces];
         uint32_t tmem;
-        int32_t abandoned;
+        Waits waits;
         Group of;                   // where this CTA's run begins
         int32_t group, into;
         uint32_t mask[kMasks][4];   // tokens of a tile that are there
@@ -343,15 +350,17 @@ __device__ __forceinline__ uint64_t global_ns() {
 }
 
 // Wait for a phase.  Once a wait of the CTA has run out none lasts any more: every role then goes through its remaining steps
-// without waiting (all of its accesses stay in bounds), so that barriers and arrivals still match, and the status says so.
-constexpr uint64_t kWaitNs = 2000000000;
-__device__ __forceinline__ void wait(int32_t* abandoned, uint64_t* bar, uint32_t parity) {
-    if (mbar_try_wait(bar, parity)) return;
-    const uint64_t until = global_ns() + kWaitNs;
+// without waiting, so that barriers and arrivals still match, and the status says so.  All of its accesses stay in bounds: a
+// place whose rows have not been found has kMasked in it, or the rows of an earlier tile, and everything else goes by indexes.
+constexpr uint32_t kWaitNs = 2000000000;
+__device__ __forceinline__ void wait(Waits* waits, uint64_t* bar, uint32_t parity) {
+    volatile int32_t& abandoned = waits->abandoned;
+    if (mbar_try_wait(bar, parity) || abandoned) return;
+    const uint64_t until = global_ns() + waits->ns;
     while (!mbar_try_wait(bar, parity)) {
-        if (*reinterpret_cast<volatile int32_t*>(abandoned)) return;
+        if (abandoned) return;
         if (global_ns() > until) {
-            *reinterpret_cast<volatile int32_t*>(abandoned) = 1;
+            abandoned = 1;
             return;
         }
     }
@@ -419,7 +428,7 @@ __device__ __forceinline__ void find_rows(const PrefixArgs& a, typename K::Share
                 number[w] = in ? a.table[at_row + idx] : 0;
             }
             const uint32_t at = tile % kPlaces;
-            wait(&sh.abandoned, &sh.rows_used[at], (tile / kPlaces & 1u) ^ 1u);
+            wait(&sh.waits, &sh.rows_used[at], (tile / kPlaces & 1u) ^ 1u);
             __syncwarp();
 #pragma unroll
             for (int w = 0; w < K::T / 32; ++w) {
@@ -460,7 +469,7 @@ __device__ __forceinline__ void produce(const PrefixArgs& a, typename K::Shared&
         if constexpr (K::kFp8) {
             const uint32_t stage = told % K::kStages, to = ring + stage * K::kUnit;
             const uint32_t from = ring + K::kStages * K::kUnit + told % K::kRaw * (K::kUnit / 2) + slot_from;
-            wait(&sh.abandoned, &sh.empty[stage], (told / K::kStages & 1u) ^ 1u);
+            wait(&sh.waits, &sh.empty[stage], (told / K::kStages & 1u) ^ 1u);
             __syncwarp();
             if (piece_of < pieces) {
                 uint4 code[kCopies];
@@ -495,7 +504,7 @@ __device__ __forceinline__ void produce(const PrefixArgs& a, typename K::Shared&
             bool of_v;
             const uint32_t at = tile + run.tile_at(j, of_v);
             if (!of_v) {
-                wait(&sh.abandoned, &sh.rows_known[at % kPlaces], at / kPlaces & 1u);
+                wait(&sh.waits, &sh.rows_known[at % kPlaces], at / kPlaces & 1u);
                 __syncwarp();
             }
             const uint32_t* rows = sh.row[at % kPlaces];
@@ -506,7 +515,7 @@ __device__ __forceinline__ void produce(const PrefixArgs& a, typename K::Shared&
                 // no room: what is on the way may be what the consumer waits for
                 cp_async_wait<0>();
                 while (told < unit) tell();
-                wait(&sh.abandoned, &sh.empty[stage], parity);
+                wait(&sh.waits, &sh.empty[stage], parity);
                 __syncwarp();
             }
             if (mine) {
@@ -571,15 +580,15 @@ __device__ __forceinline__ void multiply(const PrefixArgs& a, typename K::Shared
         auto scores = [&](int32_t x) {
             const int b = x & 1, s = K::kStreams == 2 ? b : 0;
             if (x < K::kStreams) {  // the group's queries of this item
-                wait(&sh.abandoned, &sh.q_full[s], (b ? q_items[1] : q_items[0]) & 1u);
+                wait(&sh.waits, &sh.q_full[s], (b ? q_items[1] : q_items[0]) & 1u);
                 if (b) ++q_items[1];
                 else ++q_items[0];
             }
             // its weights of the step before, in S's place, have been used
             const uint32_t done = b ? o_steps[1] : o_steps[0];
-            if (done > 0) wait(&sh.abandoned, &sh.o_done[b], (done - 1) & 1u);
+            if (done > 0) wait(&sh.waits, &sh.o_done[b], (done - 1) & 1u);
             const uint32_t u = unit + run.keys_at(tile_of(x)), stage = u % K::kStages;
-            wait(&sh.abandoned, &sh.full[stage], u / K::kStages & 1u);
+            wait(&sh.waits, &sh.full[stage], u / K::kStages & 1u);
             __syncwarp();
             tc_fence_after();
             if (leader) {
@@ -600,8 +609,8 @@ __device__ __forceinline__ void multiply(const PrefixArgs& a, typename K::Shared
         for (int32_t x = 0; x < steps; ++x) {
             const int b = x & 1, s = K::kStreams == 2 ? b : 0;
             const uint32_t u = unit + run.values_at(tile_of(x)), stage = u % K::kStages;
-            wait(&sh.abandoned, &sh.full[stage], u / K::kStages & 1u);
-            wait(&sh.abandoned, &sh.p_full[b], ((b ? s_steps[1] : s_steps[0]) - 1) & 1u);
+            wait(&sh.waits, &sh.full[stage], u / K::kStages & 1u);
+            wait(&sh.waits, &sh.p_full[b], ((b ? s_steps[1] : s_steps[0]) - 1) & 1u);
             __syncwarp();
             tc_fence_after();
             if (leader) {
@@ -625,11 +634,12 @@ __device__ __forceinline__ void multiply(const PrefixArgs& a, typename K::Shared
         unit += 2 * run.n;
         more = run.next(a);
     }
-    // the products read shared and tensor memory until here
+    // the products read shared and tensor memory until here: waited for whatever has run out
     if (leader) tc_commit(&sh.drained);
     const uint64_t until = global_ns() + kWaitNs;
-    while (!mbar_try_wait(&sh.drained, 0) && global_ns() < until) {
-    }
+    bool drained = mbar_try_wait(&sh.drained, 0);
+    while (!drained && global_ns() < until) drained = mbar_try_wait(&sh.drained, 0);
+    if (!drained) *reinterpret_cast<volatile int32_t*>(&sh.waits.abandoned) = 1;
 }
 
 // A row of a softmax group: what its scores are made of, the tokens that it sees, and its running maximum and sum.
@@ -912,7 +922,7 @@ __device__ __forceinline__ void soften(const PrefixArgs& a, typename K::Shared& 
         for (int32_t x = K::kStreams == 2 ? stream : 0; x < steps; x += K::kStreams) {
             const int b = x & 1;
             const int32_t tile = dual ? x >> 1 : x;
-            wait(&sh.abandoned, &sh.s_full[b], (b ? s_steps[1] : s_steps[0]) & 1u);
+            wait(&sh.waits, &sh.s_full[b], (b ? s_steps[1] : s_steps[0]) & 1u);
             __syncwarp();
             if (b) ++s_steps[1];
             else ++s_steps[0];
@@ -924,7 +934,7 @@ __device__ __forceinline__ void soften(const PrefixArgs& a, typename K::Shared& 
                 auto before = [&]() {
                     if (x < K::kStreams) return false;
                     const int pb = K::kStreams == 2 ? b : (x - 1) & 1;
-                    wait(&sh.abandoned, &sh.o_done[pb], ((pb ? o_steps[1] : o_steps[0]) - 1) & 1u);
+                    wait(&sh.waits, &sh.o_done[pb], ((pb ? o_steps[1] : o_steps[0]) - 1) & 1u);
                     __syncwarp();
                     tc_fence_after();
                     return true;
@@ -952,7 +962,7 @@ __device__ __forceinline__ void soften(const PrefixArgs& a, typename K::Shared& 
             if (valid && my_share == 0) *ml_to = make_float2(-INFINITY, 0.0f);
         } else {
             const int b = (steps - 1 - (steps - 1 - stream) % K::kStreams) & 1;
-            wait(&sh.abandoned, &sh.o_done[b], ((b ? o_steps[1] : o_steps[0]) - 1) & 1u);
+            wait(&sh.waits, &sh.o_done[b], ((b ? o_steps[1] : o_steps[0]) - 1) & 1u);
             __syncwarp();
             tc_fence_after();
             if (!row.seen) {  // what it has is of nothing
@@ -1088,8 +1098,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const PrefixArgs a)
         }
         mbar_init(&sh.drained, 1);
         fence_barrier_init();
-        sh.abandoned = 0;
+        sh.waits = Waits{a.wait_ns, a.wait_ns == 0};
     }
+    // nothing is known of any tile's rows
+    for (int i = tid; i < kPlaces * K::T; i += kThreads) sh.row[i / K::T][i % K::T] = kMasked;
+    for (int i = tid; i < kMasks * 4; i += kThreads) sh.mask[i / 4][i % 4] = 0;
     if (warp == kIssuer) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -1192,7 +1205,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const PrefixArgs a)
     }
     tc_fence_before();
     __syncthreads();
-    if (tid == 0 && sh.abandoned) atomicExch(a.status, MF_DEVICE_TIMEOUT);
+    if (tid == 0 && sh.waits.abandoned) atomicExch(a.status, MF_DEVICE_TIMEOUT);
     if (warp == kIssuer) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
@@ -1412,6 +1425,7 @@ extern "C" int mf_prefix_attn_create(const mf_paged_attn_config* config, int32_t
     a.reach = reach < 0x7fffffff ? static_cast<int32_t>(reach) : 0x7fffffff;
     a.page = k.page_size;
     a.always = 0;
+    a.wait_ns = kWaitNs;
     a.token_ps = (10.0f + k.head_dim * (is_fp8(k.dtype) ? 5.0f : 7.5f) / 32.0f) * ((c.q_heads / k.kv_heads + 15) / 16);
     a.window = c.window;
     a.kv_heads = k.kv_heads;
@@ -1455,6 +1469,15 @@ extern "C" int mf_prefix_attn_share(mf_prefix_attn handle, int32_t always) {
     if (!handle) return fail(MF_ERR_INVALID_ARGUMENT, "mf_prefix_attn_share: handle is NULL");
     if (always != 0 && always != 1) return fail(MF_ERR_INVALID_ARGUMENT, "mf_prefix_attn_share: %d (0 or 1)", always);
     handle->args.always = always;
+    return MF_OK;
+}
+
+extern "C" int mf_prefix_attn_limit(mf_prefix_attn handle, int64_t wait_ns) {
+    MF_ENTER();
+    if (!handle) return fail(MF_ERR_INVALID_ARGUMENT, "mf_prefix_attn_limit: handle is NULL");
+    if (wait_ns < 0 || wait_ns > 0xffffffffll)
+        return fail(MF_ERR_INVALID_ARGUMENT, "mf_prefix_attn_limit: %lld ns (0 to 2^32 - 1)", (long long)wait_ns);
+    handle->args.wait_ns = static_cast<uint32_t>(wait_ns);
     return MF_OK;
 }
 

@@ -588,6 +588,7 @@ def test_prefix_lengths_past_the_table(backend, rules):
 
 
 WILD = 1 << 30
+TIMEOUT = 0x7100
 
 
 @pytest.mark.parametrize("own", [[-300, 5, -1, 0], [-170, -300, 9], [-40, -60, -50], [-60, -40, -40], [-299, -300], [-300, -300, -300],
@@ -648,3 +649,35 @@ def test_prefix_share_refusals(backend):
     on.close()
     with pytest.raises(InvalidArgument):
         call("mf_prefix_attn_share", None, 1)
+
+
+@pytest.mark.parametrize("groups,hq,hkv,dim,dtype,cache",
+                         [([(3000, [2] * 40), (700, [1, 0, 5])], 8, 2, 128, BF16, BF16), ([(900, [1] * 9)], 4, 2, 64, F16, E4M3),
+                          ([(500, [3] * 70), (64, [1, 2])], 8, 1, 128, BF16, E4M3), ([(900, [1, 2])], 4, 1, 256, F16, F16)])
+def test_prefix_waits_that_run_out_are_reported(backend, groups, hq, hkv, dim, dtype, cache):
+    """With no time to wait every role goes on at once, the producers before any row is known.  What they copy then are rows of the
+    cache or nothing; the status tells, and the next run is right."""
+    s = make_groups(groups, hq, hkv, dim, 16, "HND", dtype, cache, 3)
+    want = want_attn(s)
+    on = Running(s)
+    for _ in range(2):
+        device_status()
+        call("mf_prefix_attn_limit", on.attn._handle, 0)
+        on.run()
+        assert device_status() == TIMEOUT
+        call("mf_prefix_attn_limit", on.attn._handle, 2 * 10 ** 9)
+        got = on.run()
+        assert device_status() == 0
+        check_prefix(s, got, want)
+    on.close()
+
+
+def test_prefix_limit_refusals(backend):
+    s = make_groups([(20, [1, 2])], 4, 2, 64, 16, "HND", BF16, BF16, 3)
+    on = Running(s)
+    for ns in (-1, 2 ** 32):
+        with pytest.raises(InvalidArgument):
+            call("mf_prefix_attn_limit", on.attn._handle, ns)
+    on.close()
+    with pytest.raises(InvalidArgument):
+        call("mf_prefix_attn_limit", None, 1)
