@@ -757,10 +757,9 @@ int mf_page_copy(const mf_cache_layout* layout, void* const* caches, int32_t n_c
  * may stand anywhere in it.  Where an infinity or NaN turns up among what a
  * request's rows sum, seen by it or not, all its tokens are read for it alone, so
  * that only what it sees counts.
- * Over the shared tokens the weights exp(s - max) enter the product with the
- * values as two 16-bit terms, as in mf_paged_attn_run, but as one f16 term over an
- * FP8 cache with BF16 queries (off by 2^-11 of a weight at most, an eighth of the
- * result's rounding); queries over an FP8 cache are held as there.  head_dim,
+ * Over the shared tokens, too, the weights exp(s - max) enter the product with the
+ * values as two 16-bit terms, and queries over an FP8 cache are held as in
+ * mf_paged_attn_run: whether a token is shared changes no bound.  head_dim,
  * dtypes, strides and alignments as there; a cache has less than 2^32 - 1 pieces
  * of the largest power of two of bytes (2^30 at most) that divides its page and token
  * strides (else MF_ERR_LAYOUT_UNSUPPORTED).

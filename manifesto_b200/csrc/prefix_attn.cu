@@ -19,15 +19,15 @@
 //   * two groups of four softmax warps, a thread for each row, turn S into P in
 //     place: running maximum and sum in float32, P as two 16-bit terms (high and
 //     low: what the two leave out of a weight is 2^-16 of it in BF16, 2^-22 in
-//     f16; where one f16 term is enough, see two_terms), O rescaled only when a
+//     f16), O rescaled only when a
 //     maximum has grown by more than 2^8 (f16: 2^15);
 //   * one warp writes down for the other launches what each request shares.
 // The groups alternate, so that one's softmax runs beside the other's products: of
 // more than 128 rows each has 128 and sees every tile, else both have the same
 // rows and every second tile.  Up to 64 rows stand in tensor memory two or four
 // times over, and a tile's tokens are shared out among the warps that hold them
-// (24 prompts of 8 beams over E4M3, 32 rows, together with the
-// single f16 term: 404 -> 326 us at that time).  The
+// (24 prompts of 8 beams over E4M3, 32 rows: 404 -> 326 us at that time, when
+// FP8 caches had one term of the weights; now 150, 148 with one).  The
 // tiles of all (group, block of rows, key-value head) items in a row are cut evenly
 // for the CTAs, an item counting four tiles more than it has (without them items of
 // two tiles filled a CTA's whole share: 240 -> 146 us, with the parts' layout); every CTA leaves the part of
@@ -548,13 +548,6 @@ __device__ __forceinline__ void produce(const PrefixArgs& a, typename K::Shared&
     while (told < unit) tell();
 }
 
-// Whether weights enter the second product as two terms.  One f16 term is off by up to 2^-11 of a weight, an eighth of what
-// rounding the result to BF16 costs: over an FP8 cache, with BF16 queries, that is enough.  One BF16 term would cost as much as that rounding.
-template <class K>
-__device__ __forceinline__ bool two_terms(const PrefixArgs& a) {
-    return !K::kFp8 || a.q_f16;
-}
-
 __device__ __forceinline__ bool elect_one() {
     uint32_t is;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(is));
@@ -569,7 +562,6 @@ __device__ __forceinline__ void multiply(const PrefixArgs& a, typename K::Shared
     const uint32_t of_s = product(K::kBf16, K::T, false);
     const int wide = (a.head_dim + 15) / 16;  // products of 16 along head_dim, and columns of O in 16s
     const uint32_t of_o = product(K::kBf16, wide * 16, true);
-    const bool two = two_terms<K>(a);
     uint32_t unit = 0;                               // first unit of the item at hand
     uint32_t s_steps[2] = {0, 0}, o_steps[2] = {0, 0}, q_items[2] = {0, 0};
     bool more = run.n > 0;
@@ -621,7 +613,7 @@ __device__ __forceinline__ void multiply(const PrefixArgs& a, typename K::Shared
 #pragma unroll
                 for (int c = 0; c < K::T / 16; ++c) {
                     mma_ts(o, p + (c >> 1) * 32 + (c & 1) * 8, values + c * 128, of_o, !first || c > 0);
-                    if (two) mma_ts(o, p + (c >> 1) * 32 + (c & 1) * 8 + 16, values + c * 128, of_o, true);
+                    mma_ts(o, p + (c >> 1) * 32 + (c & 1) * 8 + 16, values + c * 128, of_o, true);
                 }
                 tc_commit(&sh.o_done[b]);
                 if (!dual || b == 1) tc_commit(&sh.empty[stage]);
@@ -728,7 +720,7 @@ __device__ __forceinline__ void raise(const PrefixArgs& a, Row& row, float top, 
 
 // The weights of 32 scores, to where those were: their high terms in 16 columns and their low terms in the 16 behind; their sum.
 template <class K>
-__device__ __forceinline__ float2 weights(const uint32_t (&v)[32], float by, float less, bool two, uint32_t at) {
+__device__ __forceinline__ float2 weights(const uint32_t (&v)[32], float by, float less, uint32_t at) {
     const float2 by2 = make_float2(by, by), less2 = make_float2(-less, -less);
     float2 sum = make_float2(0.0f, 0.0f);
     uint32_t high[16], low[16];
@@ -744,13 +736,13 @@ __device__ __forceinline__ float2 weights(const uint32_t (&v)[32], float by, flo
         low[i] = pack2<K::kBf16>(rest.x, rest.y);
     }
     tm_store16(at, high);
-    if (two) tm_store16(at + 16, low);
+    tm_store16(at + 16, low);
     return sum;
 }
 
 // The weights of a tile of tokens from `first` on, whose products are at `at`, in their place.
 template <class K, class Before>
-__device__ __forceinline__ void weigh(const PrefixArgs& a, Row& row, uint32_t at, uint32_t first, const uint32_t* words, bool two, uint32_t o_at,
+__device__ __forceinline__ void weigh(const PrefixArgs& a, Row& row, uint32_t at, uint32_t first, const uint32_t* words, uint32_t o_at,
                                       Before&& before) {
     constexpr int kChunks = K::T / 32;
     bool plain = first >= row.begin && first + K::T <= row.end;
@@ -778,14 +770,14 @@ __device__ __forceinline__ void weigh(const PrefixArgs& a, Row& row, uint32_t at
     raise<K>(a, row, top * by, o_at, before);
     float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) sum = __fadd2_rn(sum, weights<K>(v[c], by, row.less, two, at + c * 32));
+    for (int c = 0; c < kChunks; ++c) sum = __fadd2_rn(sum, weights<K>(v[c], by, row.less, at + c * 32));
     row.l += sum.x + sum.y;
 }
 
 // The same for `mine` of the tile's chunks of 32 tokens, from c0 on; the others, other warps' with the same rows, weigh nothing here.
 template <class K, class Before>
 __device__ __forceinline__ void weigh_share(const PrefixArgs& a, Row& row, uint32_t at, uint32_t first, const uint32_t* words, int c0, int mine,
-                                            bool two, uint32_t o_at, Before&& before) {
+                                            uint32_t o_at, Before&& before) {
     uint32_t v[32];
     float top = -INFINITY;
 #pragma unroll 1
@@ -805,7 +797,7 @@ __device__ __forceinline__ void weigh_share(const PrefixArgs& a, Row& row, uint3
             tm_load(v, at + c * 32);
             tc_wait_ld();
         }
-        sum = __fadd2_rn(sum, weights<K>(v, 1.0f, row.less, two, at + c * 32));
+        sum = __fadd2_rn(sum, weights<K>(v, 1.0f, row.less, at + c * 32));
     }
     row.l += sum.x + sum.y;
 #pragma unroll
@@ -824,7 +816,6 @@ __device__ __forceinline__ void soften(const PrefixArgs& a, typename K::Shared& 
     const uint32_t o_at = lanes + K::kO + stream * K::kDim;
     uint32_t s_steps[2] = {0, 0}, o_steps[2] = {0, 0};
     uint32_t tile0 = 0;
-    const bool two = two_terms<K>(a);
     Row row;
     row.cap = a.softcap * kLog2e;
     bool more = run.n > 0;
@@ -940,8 +931,8 @@ __device__ __forceinline__ void soften(const PrefixArgs& a, typename K::Shared& 
                     return true;
                 };
                 const int each = K::T / 32 / sharers;
-                if (sharers == 1) weigh<K>(a, row, s_at, first, words, two, o_at, before);
-                else weigh_share<K>(a, row, s_at, first, words, my_share * each, each, two, o_at, before);
+                if (sharers == 1) weigh<K>(a, row, s_at, first, words, o_at, before);
+                else weigh_share<K>(a, row, s_at, first, words, my_share * each, each, o_at, before);
                 tc_wait_st();
             }
             tc_fence_before();

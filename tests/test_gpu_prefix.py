@@ -681,3 +681,51 @@ def test_prefix_limit_refusals(backend):
     on.close()
     with pytest.raises(InvalidArgument):
         call("mf_prefix_attn_limit", None, 1)
+
+
+# ------------------------------------------------------------------ precision, and the choice of what is shared
+
+def digits(x, n):
+    """x, multiples of 8^-(n - 1) below 8, as n digits of 3 bits, the largest first."""
+    y = np.round(np.asarray(x) * 8.0 ** (n - 1)).astype(np.int64)
+    assert (y / 8.0 ** (n - 1) == x).all() and (y >= 0).all() and (y < 8 ** n).all()
+    return np.stack([y >> 3 * (n - 1 - j) & 7 for j in range(n)], -1).astype(np.float32)
+
+
+def one_for_all(tokens, values, q, keys, requests, hq, dtype, cache, shared):
+    """Requests of the same tokens, all in the same pages (one key-value head); each token's value is one number."""
+    n, dim = keys.shape
+    s = make_attn([n], hq, 1, dim, 16, "HND", dtype, cache, 5)
+    tok = np.arange(n)
+    s["kv"][0][s["table"][0, tok // 16], tok % 16, 0] = plain.codes(keys, cache)
+    s["kv"][1][s["table"][0, tok // 16], tok % 16, 0] = plain.codes(np.repeat(values[:, None], dim, 1), cache)
+    if s["scales"] is not None:
+        s["scales"][:] = 1.0
+    s["q"] = np.ascontiguousarray(np.broadcast_to(plain.codes(q, dtype), (requests, hq, dim)))
+    s["table"] = np.repeat(s["table"], requests, 0)
+    s["lens"] = np.array(tokens, np.int32)
+    s["starts"], s["shared"] = np.array([0, requests], np.int32), np.array([shared], np.int32)
+    return s
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+@pytest.mark.parametrize("requests", [2, 20, 70])
+def test_prefix_weights_are_good_to_the_bound_without_sharing(backend, dtype, cache, requests):
+    """63 tokens of value 1 and 63 of -1 whose weights lie on either side of the middle between two f16 numbers, a half of the
+    largest: rounded to f16 alone they are 2^-11 off, up and down, and so is the result.  A row's tokens among 4, 2 and 1 warps."""
+    n, dim = 129, 64
+    middle = 1.0 - np.log(2.0) + np.log1p(2.0 ** -11)
+    below, above = np.floor(middle * 2.0 ** 15) / 2.0 ** 15, (np.floor(middle * 2.0 ** 15) + 2) / 2.0 ** 15
+    score, value = np.zeros(n), np.zeros(n, np.float32)
+    score[0] = 1.0
+    score[1:127:2], value[1:127:2] = below, 1.0
+    score[2:127:2], value[2:127:2] = above, -1.0
+    keys, q = np.zeros((n, dim), np.float32), np.zeros(dim, np.float32)
+    keys[:, :6], q[:6] = digits(score, 6), 8.0 ** -np.arange(6)
+    s = one_for_all([n] * requests, value, q, keys, requests, 2, dtype, cache, 128)
+    on = Running(s, scale=1.0)
+    got = on.run()
+    on.close()
+    want = want_attn(s, scale=1.0)
+    assert np.abs(want[0]).max() < 1e-4 and want[2].min() > 0.9
+    check_attn(s, got, want)
