@@ -28,12 +28,13 @@ int launch_plan_passes(const mf_chunk_desc* chunks, int32_t n_chunks, int src_dt
 int comm_allreduce_max(mf_comm comm, float* d_vec, int64_t count, cudaStream_t s);
 
 // The attention of a paged cache restricted to each request's tokens from own_first[r] on (all of them where alone[r] is
-// *call): float32 results [n_requests][q_heads][head_dim], normalised, and their log-sum-exp (paged_attn.cu).  Enabled once
+// *call): float32 results [n_requests][q_heads][head_dim], normalised, and what their weights are: the maximum in base 2 (less
+// 12 where the cache is not BF16; -inf where nothing is seen) and the sum of exp2(score - it) (paged_attn.cu).  Enabled once
 // per handle.
 int paged_attn_enable_parts(mf_paged_attn handle);
 int paged_attn_run_parts(mf_paged_attn handle, const void* q, const void* k_cache, const void* v_cache, const int32_t* table,
                          const int32_t* lens, int32_t n_requests, const int32_t* own_first, const uint32_t* alone, const uint32_t* call,
-                         float* out, float* lse, cudaStream_t stream);
+                         float* out, float2* ml, cudaStream_t stream);
 
 // A validated fused program (postfix) as the CUDA codegen target sees it (fused_jit.cu).
 struct JitSpec {

@@ -299,9 +299,14 @@ __device__ __forceinline__ void store_out4(const AttnArgs& a, int32_t r, int32_t
     *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
 }
 
-// l is at least K::kMost, the largest weight of a maximum: its logarithm is taken over that, which leaves it the low bits.
-template <class K>
+// l is at least K::kMost, the largest weight of a maximum: its logarithm is taken over that, which leaves it the low bits.  A run
+// of parts leaves maximum and sum.
+template <class K, bool PART>
 __device__ __forceinline__ void store_lse(const AttnArgs& a, int32_t r, int32_t head, float m, float l) {
+    if constexpr (PART) {
+        reinterpret_cast<float2*>(a.lse)[static_cast<int64_t>(r) * a.q_heads + head] = make_float2(l == 0.0f ? -INFINITY : m, l);
+        return;
+    }
     if (!a.lse) return;
     a.lse[static_cast<int64_t>(r) * a.q_heads + head] =
         l == 0.0f ? -INFINITY : (m + K::kBelow + log2f(l * (1.0f / K::kMost))) * kLn2;
@@ -414,7 +419,7 @@ __device__ __forceinline__ void join_parts(const AttnArgs& a, typename K::Shared
             }
         } else {
             store_out4<PART>(a, w.r, w.head0 + h, d, scale4(acc[e], sum == 0.0f ? 0.0f : __fdiv_rn(vs, sum)));
-            if (d == 0) store_lse<K>(a, w.r, w.head0 + h, sh.top[h], sum);
+            if (d == 0) store_lse<K, PART>(a, w.r, w.head0 + h, sh.top[h], sum);
         }
     }
     __syncthreads();
@@ -482,7 +487,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
             if (tiles_of<T>(span_of<PART>(a, r)) > 0) continue;
             for (int i = tid; i < a.q_heads * (a.head_dim / 4); i += K::kThreads)
                 store_out4<PART>(a, r, i / (a.head_dim / 4), i % (a.head_dim / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f));
-            for (int i = tid; i < a.q_heads; i += K::kThreads) store_lse<K>(a, r, i, 0.0f, 0.0f);
+            for (int i = tid; i < a.q_heads; i += K::kThreads) store_lse<K, PART>(a, r, i, 0.0f, 0.0f);
         }
     }
     // Of W values of warps and the values of their threads, in a row: the thread that place `key` is at, and how far into it.
@@ -959,7 +964,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
                     for (int x = 0; x < 2; ++x) {
                         const int h = member * 8 + 2 * j + x;
                         f[x] = l[x] == 0.0f ? 0.0f : __fdiv_rn(vs, l[x]);
-                        if (g == 0 && h < hd.count) store_lse<K>(a, at.r, hd.head0 + h, m[x], l[x]);
+                        if (g == 0 && h < hd.count) store_lse<K, PART>(a, at.r, hd.head0 + h, m[x], l[x]);
                     }
                     char* out = a.out + (PART ? 4 : 2) * (at.r * a.out_req + hd.head0 * a.out_head);
 #pragma unroll
@@ -1127,7 +1132,7 @@ __global__ void __launch_bounds__(32 * W, 1) paged_attn_kernel(const AttnArgs a)
         if (w.slot < 0) {
             const float vs = a.v_scale ? a.v_scale[w.kv] : 1.0f;
             store_out4<PART>(a, w.r, w.head0 + h, d, scale4(acc, sum_l == 0.0f ? 0.0f : __fdiv_rn(vs, sum_l)));
-            if (d == 0) store_lse<K>(a, w.r, w.head0 + h, top, sum_l);
+            if (d == 0) store_lse<K, PART>(a, w.r, w.head0 + h, top, sum_l);
         } else {
             float* to = a.cta_part + (static_cast<int64_t>(blockIdx.x) * 3 + w.slot) * K::kPart;
             *reinterpret_cast<float4*>(to + h * DP + d) = acc;
@@ -1390,7 +1395,7 @@ int paged_attn_enable_parts(mf_paged_attn handle) {
 
 int paged_attn_run_parts(mf_paged_attn handle, const void* q, const void* k_cache, const void* v_cache, const int32_t* table,
                          const int32_t* lens, int32_t n_requests, const int32_t* own_first, const uint32_t* alone, const uint32_t* call,
-                         float* out, float* lse, cudaStream_t stream) {
+                         float* out, float2* ml, cudaStream_t stream) {
     AttnArgs a = handle->args;
     a.q = static_cast<const char*>(q);
     a.k = static_cast<const char*>(k_cache);
@@ -1404,7 +1409,7 @@ int paged_attn_run_parts(mf_paged_attn handle, const void* q, const void* k_cach
     a.out = reinterpret_cast<char*>(out);
     a.out_head = a.head_dim;
     a.out_req = static_cast<int64_t>(a.q_heads) * a.head_dim;
-    a.lse = lse;
+    a.lse = reinterpret_cast<float*>(ml);
     const cudaError_t err = launch_overlapped(handle->kernel.part_fn, dim3(static_cast<unsigned>(handle->ctas)), handle->kernel.threads,
                                               handle->kernel.shared, stream, a);
     return err == cudaSuccess ? MF_OK : cuda_fail(err, "mf_prefix_attn_run");

@@ -104,7 +104,7 @@ struct PrefixArgs {
     float* cta_part;      // [CTAs][2][128][head_dim]: a CTA that begins inside an item
     float2* cta_ml;       // [CTAs][2][128]
     float* own;           // [requests][q_heads][head_dim]: the requests' own tokens
-    float* own_lse;       // [requests][q_heads]
+    float2* own_ml;       // [requests][q_heads]: their maximum and sum, as part_ml's
     char* out;
     int64_t out_req, out_head;
     float* lse;
@@ -1224,8 +1224,9 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const PrefixArgs a) 
         const int32_t kv = h / a.group;
         const float vs = a.v_scale ? a.v_scale[kv] : 1.0f;
         const Shared x = a.info[r];
-        // its own tokens as a part whose largest weight is kMost, too
-        const float own = a.own_lse[w];
+        // its own tokens: a part that is normalised already.  Joined by maximum and sum as the others are: in one logarithm the
+        // weight of a part whose scores are large would lose bits (half a step of float32 at 20000 is 2^-10)
+        const float2 own = a.own_ml[w];
         float4 acc[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -1250,7 +1251,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const PrefixArgs a) 
             const int32_t k = halves == 2 ? p >> 1 : p, half = halves == 2 ? p & 1 : 0;
             return k == 0 ? -(first_at + half * first_apart) - 1 : at + static_cast<int64_t>(k) * 256 + half * 128;
         };
-        float top = own * kLog2e - kBelow;
+        float top = own.x;
         float2 ml = make_float2(-INFINITY, 0.0f);
         int64_t row = 0;
         for (int32_t p0 = 0; p0 < parts; p0 += 32) {
@@ -1262,7 +1263,8 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const PrefixArgs a) 
         }
 #pragma unroll
         for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        const float own_w = own == -INFINITY ? 0.0f : kMost * exp2_fast(own * kLog2e - kBelow - top);
+        // alone it stays as it is
+        const float own_l = own.y == 0.0f ? 0.0f : own.y * rescale(own.x, top), own_w = parts == 0 && own.y != 0.0f ? 1.0f : own_l;
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
@@ -1295,8 +1297,8 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const PrefixArgs a) 
         }
 #pragma unroll
         for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        sum += own_w;
-        const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
+        sum += own_l;
+        const float inv = parts == 0 || sum == 0.0f ? 1.0f : __fdiv_rn(1.0f, sum);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int d = 4 * (lane + 32 * i);
@@ -1383,8 +1385,8 @@ extern "C" int mf_prefix_attn_create(const mf_paged_attn_config* config, int32_t
     const size_t firsts = up(static_cast<size_t>(max_requests) * 4), infos = up(static_cast<size_t>(max_requests) * sizeof(Shared));
     const size_t parts = up(2 * heads * k.head_dim * 4), part_mls = up(2 * heads * 8);
     const size_t cta_parts = up(static_cast<size_t>(ctas) * 256 * k.head_dim * 4), cta_mls = up(static_cast<size_t>(ctas) * 256 * 8);
-    const size_t owns = up(heads * k.head_dim * 4), lses = up(heads * 4);
-    const size_t cleared = 256 + alones, bytes = cleared + firsts + infos + parts + part_mls + cta_parts + cta_mls + owns + lses;
+    const size_t owns = up(heads * k.head_dim * 4), own_mls = up(heads * 8);
+    const size_t cleared = 256 + alones, bytes = cleared + firsts + infos + parts + part_mls + cta_parts + cta_mls + owns + own_mls;
     mf_prefix_attn_s* h = err == cudaSuccess ? new (std::nothrow) mf_prefix_attn_s{} : nullptr;
     if (!h) {
         mf_paged_attn_destroy(own);
@@ -1450,7 +1452,7 @@ extern "C" int mf_prefix_attn_create(const mf_paged_attn_config* config, int32_t
     a.cta_part = reinterpret_cast<float*>(w += part_mls);
     a.cta_ml = reinterpret_cast<float2*>(w += cta_parts);
     a.own = reinterpret_cast<float*>(w += cta_mls);
-    a.own_lse = reinterpret_cast<float*>(w += owns);
+    a.own_ml = reinterpret_cast<float2*>(w += owns);
     *handle = h;
     return MF_OK;
 }
@@ -1508,7 +1510,7 @@ extern "C" int mf_prefix_attn_run(mf_prefix_attn handle, const void* q, const vo
                                         handle->kernel.shared, s, a);
     if (err != cudaSuccess) return cuda_fail(err, "mf_prefix_attn_run");
     const int rc = paged_attn_run_parts(handle->own, q, k_cache, v_cache, table, lens, n_requests, a.own_first, a.alone, a.call, a.own,
-                                        a.own_lse, s);
+                                        a.own_ml, s);
     if (rc != MF_OK) return rc;
     const int64_t grid = stream_grid(static_cast<int64_t>(n_requests) * a.q_heads * 32, kJoinThreads, 8);
     err = launch_overlapped(handle->kernel.join, dim3(static_cast<unsigned>(grid)), kJoinThreads, 0, s, a);

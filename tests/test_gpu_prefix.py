@@ -729,3 +729,24 @@ def test_prefix_weights_are_good_to_the_bound_without_sharing(backend, dtype, ca
     want = want_attn(s, scale=1.0)
     assert np.abs(want[0]).max() < 1e-4 and want[2].min() > 0.9
     check_attn(s, got, want)
+
+
+@pytest.mark.parametrize("dtype,cache", [(BF16, BF16), (F16, F16), (F16, E4M3), (BF16, E5M2)])
+def test_prefix_own_tokens_join_at_large_scores(backend, dtype, cache):
+    """Scores of 28672 powers of two and a few: exact products (scale * log2(e) is 1), so that only what the parts are joined by can
+    lose bits.  Shared tokens have value 1, own ones -1."""
+    dim, rng = 64, np.random.default_rng(3)
+    lens = [128 + x for x in (100, 128, 37, 77, 1, 112, 90, 63, 128, 120, 99, 101)]
+    n = max(lens)
+    keys, q = np.zeros((n, dim), np.float32), np.zeros(dim, np.float32)
+    keys[:, 0], q[0] = 224.0, 128.0
+    keys[:, 1:4], q[1:4] = digits(rng.integers(0, 3 * 64, n) / 64.0, 3), 8.0 ** -np.arange(3)
+    value = np.where(np.arange(n) < 128, 1.0, -1.0).astype(np.float32)
+    s = one_for_all(lens, value, q, keys, len(lens), 2, dtype, cache, 128)
+    scale = float(np.float32(np.log(2.0)))
+    on = Running(s, scale=scale)
+    got, alone = on.run(), on.run(groups=0)
+    on.close()
+    want = want_attn(s, scale=scale)
+    check_attn(s, alone, want)  # the bound holds where nothing is joined
+    check_attn(s, got, want)
