@@ -773,7 +773,8 @@ int mf_prefix_attn_run(mf_prefix_attn handle, const void* q, const void* k_cache
                        const int32_t* shared, int32_t n_groups, void* out, float* lse, mf_stream stream);
 /* Whether the runs that follow share whatever the groups can (1), or, as they do
  * from the start (0), where that is quicker than to read the tokens once more
- * for each request: a rule on the numbers of requests, tokens and heads. */
+ * for each request that sees them: a rule on the tokens that requests see (by their
+ * lengths and the window), their numbers and the heads. */
 int mf_prefix_attn_share(mf_prefix_attn handle, int32_t always);
 /* How long, in nanoseconds, the runs that follow may wait for one another's parts inside a CTA: 2 * 10^9 from the start, 0
  * to 2^32 - 1 (0: not at all, every run that shares tokens is given up).  A run whose wait runs out, as where the GPU is

@@ -95,6 +95,7 @@ struct PrefixArgs {
     uint32_t wait_ns;     // that a wait may last
     // workspace
     int32_t* own_first;   // [requests]
+    int32_t* kept;        // [requests], by a group's first: the tokens that it shares; every CTA writes the same, for itself
     Shared* info;         // [requests]
     int2* cut;            // places of all items, CTAs that they are cut for
     uint32_t* call;       // the number of the call, for the launches behind the first; of the last call that came to its end
@@ -192,16 +193,17 @@ struct Waits {
 // Shared tokens of a group, and its requests; nothing is shared by a request alone, nor where it does not pay.
 struct Group {
     int32_t start, members, shared;
-    float worth;  // what sharing saves, in picoseconds of the whole GPU
     bool bad;
 };
 // Whether a group's tokens are shared, and whether any are.  The requests of a group follow one another, so that its tokens come
-// out of L2 for all but the first of them: reading them again costs 40 ps a token and key-value head of 128 (30 of FP8 codes)
-// with all SMs at work, an item of shared tokens 47 ns (7 us of one CTA), a tile 8 (twice that with more than 128 rows), and the
-// first of them all delays the rest.  32/8 heads of 128, BF16, us with sharing and without: 100 groups of 2 that share 48
-// tokens 84 and 39, 30 groups of 16 with 48 83 and 54, with 800 106 and 180; 6 of 16 with 800 62 and 50, with 3200 77 and 95;
-// one of 4 with 896 32 and 20.
-constexpr float kItemPs = 47e3f, kTilePs = 8e3f, kFirstPs = 25e6f;
+// out of L2 for all but one of them: reading them again, as far as each of the others sees them (its length, its window), costs
+// 40 ps a token and key-value head of 128 (30 of FP8 codes) with all SMs at work, an item of shared tokens 47 ns (7 us of one
+// CTA), a tile, seen or not, 8 (32 with more than 128 rows), and the first of them all delays the rest.  32/8 heads of 128, BF16,
+// us with sharing and without: 100 groups of 2 that share 48 tokens 84 and 39, 30 groups of 16 with 48 83 and 54, with 800 106
+// and 180; 6 of 16 with 800 62 and 50, with 3200 77 and 95; one of 4 with 896 32 and 20.  One of 250 with 8192 135 and 643; with
+// a window of 128 136 and 40, of 1024 142 and 106, of 2048 143 and 181; 2 of the 250 not idle 87 and 29, 25 85 and 85, 50 86 and
+// 145.
+constexpr float kItemPs = 47e3f, kTilePs = 8e3f, kWideTilePs = 32e3f, kFirstPs = 25e6f;
 constexpr uint32_t kMasked = 0xffffffffu;
 
 // MODE: dtype of the cache; DP: head_dim padded to 64, 128 or 256.
@@ -238,23 +240,79 @@ struct Prefix {
     static constexpr int kBytes = kRing + kStreams * kQ + static_cast<int>(sizeof(Shared));
 };
 
-template <class K>
-__device__ __forceinline__ Group group_of(const PrefixArgs& a, int32_t g) {
+// A group as the caller has it.
+__device__ __forceinline__ Group asked_group(const PrefixArgs& a, int32_t g) {
     Group x;
     const int32_t s = a.starts[g], e = a.starts[g + 1];
     x.bad = s < 0 || e < s || e > a.n_requests;
     x.start = s;
     x.members = x.bad ? 0 : e - s;
     x.shared = x.members < 2 ? 0 : min(max(a.shared[g], 0), a.reach);
+    return x;
+}
+// As it is shared, once that is decided.
+__device__ __forceinline__ Group group_of(const PrefixArgs& a, int32_t g) {
+    Group x;
+    const int32_t s = a.starts[g], e = a.starts[g + 1];
+    x.bad = false;
+    x.start = s;
+    x.members = e - s;
+    x.shared = x.members < 2 ? 0 : a.kept[s];
+    return x;
+}
+// What sharing saves if its requests would read `again` tokens more than once, in picoseconds of the whole GPU.
+template <class K>
+__device__ __forceinline__ float worth_of(const PrefixArgs& a, const Group& x, float again) {
     const float heads = static_cast<float>(a.kv_heads), rows = static_cast<float>(x.members) * static_cast<float>(a.group.d);
     const float tiles = ceilf(static_cast<float>(x.shared) * (1.0f / K::T)), items = ceilf(rows * (1.0f / K::kRows));
-    x.worth = heads * (static_cast<float>(x.members - 1) * static_cast<float>(x.shared) * a.token_ps -
-                       items * (kItemPs + tiles * (rows > 128.0f ? 2.0f * kTilePs : kTilePs)));
-    if (x.worth <= 0.0f || x.shared == 0) {
-        x.worth = 0.0f;
-        if (!a.always) x.shared = 0;
+    return heads * (again * a.token_ps - items * (kItemPs + tiles * (rows > 128.0f ? kWideTilePs : kTilePs)));
+}
+// The shared tokens that the requests of a group see, and the most of them that one sees.
+struct Seen {
+    int64_t all;
+    int32_t most;
+};
+// EACH requests from `first` on, `apart` from one another, of which those in front of `end` count.
+template <int EACH>
+__device__ __forceinline__ void look(const PrefixArgs& a, int32_t first, int32_t apart, int32_t end, int32_t shared, Seen& seen) {
+    int32_t len[EACH];
+#pragma unroll
+    for (int u = 0; u < EACH; ++u) len[u] = end - first > u * apart ? min(a.lens[first + u * apart], a.reach) : 0;
+#pragma unroll
+    for (int u = 0; u < EACH; ++u) {
+        const int32_t sees = max(min(len[u], shared) - (a.window > 0 && len[u] > a.window ? len[u] - a.window : 0), 0);
+        seen.all += sees;
+        seen.most = max(seen.most, sees);
     }
-    return x;
+}
+// What each lane's group is worth, 0 if it is not shared (whose x.shared is 0 then).  All lanes.
+template <class K>
+__device__ __forceinline__ float decide(const PrefixArgs& a, Group& x) {
+    constexpr int32_t kOfLane = 64;  // requests that a lane looks at itself; a warp together at more
+    constexpr int kEach = 8;
+    const int lane = threadIdx.x & 31;
+    const bool some = x.members > 1 && x.shared > 0;
+    float worth = 0.0f;
+    // not if it would not pay though every request saw all of it
+    const bool may = some && !a.always && worth_of<K>(a, x, static_cast<float>(x.members - 1) * static_cast<float>(x.shared)) > 0.0f;
+    Seen seen{0, 0};
+    if (may && x.members <= kOfLane)
+        for (int32_t i = 0; i < x.members; i += kEach) look<kEach>(a, x.start + i, 1, x.start + x.members, x.shared, seen);
+    for (uint32_t large = __ballot_sync(0xffffffffu, may && x.members > kOfLane); large; large &= large - 1) {
+        const int src = __ffs(large) - 1;
+        const int32_t start = __shfl_sync(0xffffffffu, x.start, src), end = start + __shfl_sync(0xffffffffu, x.members, src);
+        const int32_t shared = __shfl_sync(0xffffffffu, x.shared, src);
+        Seen part{0, 0};
+        for (int32_t i = start; i < end; i += 32 * kEach) look<kEach>(a, min(i + lane, end), 32, end, shared, part);
+#pragma unroll
+        for (int d = 16; d; d >>= 1) part.all += __shfl_xor_sync(0xffffffffu, part.all, d);
+        part.most = __reduce_max_sync(0xffffffffu, part.most);
+        if (lane == src) seen = part;
+    }
+    if (may) worth = fmaxf(worth_of<K>(a, x, static_cast<float>(seen.all - seen.most)), 0.0f);
+    if (worth == 0.0f && !a.always) x.shared = 0;
+    if (x.members > 1) a.kept[x.start] = x.shared;
+    return worth;
 }
 template <class K>
 __device__ __forceinline__ int32_t tiles_of(const Group& x) {
@@ -331,7 +389,7 @@ struct Run {
                 if (++item == items) {
                     item = 0;
                     do {
-                        of = group_of<K>(a, ++g);
+                        of = group_of(a, ++g);
                         tiles = tiles_of<K>(of);
                     } while (tiles == 0 && g + 1 < a.n_groups);
                     items = static_cast<int32_t>(items_of<K>(a, of));
@@ -1040,7 +1098,7 @@ __device__ __forceinline__ void take_notes(const PrefixArgs& a, bool none) {
     for (int32_t g0 = 0; g0 < a.n_groups; g0 += 32) {
         const int32_t g = g0 + lane;
         Group x{};
-        if (g < a.n_groups) x = group_of<K>(a, g);
+        if (g < a.n_groups) x = group_of(a, g);
         const int64_t of = items_of<K>(a, x) * places_of<K>(x);
         int64_t upto = of;
 #pragma unroll
@@ -1110,10 +1168,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const PrefixArgs a)
     float worth = 0.0f;
     for (int32_t i = 0; i < per; ++i) {
         const int32_t g = tid * per + i;
-        if (g >= a.n_groups) break;
-        last = group_of<K>(a, g);
+        last = Group{};
+        if (g < a.n_groups) last = asked_group(a, g);
         bad |= last.bad;
-        worth += last.worth;
+        worth += decide<K>(a, last);
         mine += items_of<K>(a, last) * places_of<K>(last);
     }
     int64_t upto = mine;
@@ -1165,7 +1223,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const PrefixArgs a)
             int32_t into = x0 - static_cast<int32_t>(front), g = tid * per;
             if (per > 1) {
                 for (;; ++g) {
-                    last = group_of<K>(a, g);
+                    last = group_of(a, g);
                     const int64_t of = items_of<K>(a, last) * places_of<K>(last);
                     if (into < of) break;
                     into -= static_cast<int32_t>(of);
@@ -1382,11 +1440,11 @@ extern "C" int mf_prefix_attn_create(const mf_paged_attn_config* config, int32_t
     const int ctas = state().sm_count;
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
     const size_t heads = static_cast<size_t>(max_requests) * c.q_heads, alones = up(static_cast<size_t>(max_requests) * 4);
-    const size_t firsts = up(static_cast<size_t>(max_requests) * 4), infos = up(static_cast<size_t>(max_requests) * sizeof(Shared));
+    const size_t firsts = up(static_cast<size_t>(max_requests) * 4), kepts = firsts, infos = up(static_cast<size_t>(max_requests) * sizeof(Shared));
     const size_t parts = up(2 * heads * k.head_dim * 4), part_mls = up(2 * heads * 8);
     const size_t cta_parts = up(static_cast<size_t>(ctas) * 256 * k.head_dim * 4), cta_mls = up(static_cast<size_t>(ctas) * 256 * 8);
     const size_t owns = up(heads * k.head_dim * 4), own_mls = up(heads * 8);
-    const size_t cleared = 256 + alones, bytes = cleared + firsts + infos + parts + part_mls + cta_parts + cta_mls + owns + own_mls;
+    const size_t cleared = 256 + alones, bytes = cleared + firsts + kepts + infos + parts + part_mls + cta_parts + cta_mls + owns + own_mls;
     mf_prefix_attn_s* h = err == cudaSuccess ? new (std::nothrow) mf_prefix_attn_s{} : nullptr;
     if (!h) {
         mf_paged_attn_destroy(own);
@@ -1446,7 +1504,8 @@ extern "C" int mf_prefix_attn_create(const mf_paged_attn_config* config, int32_t
     a.call = reinterpret_cast<uint32_t*>(w + 64);
     a.alone = reinterpret_cast<uint32_t*>(w += 256);
     a.own_first = reinterpret_cast<int32_t*>(w += alones);
-    a.info = reinterpret_cast<Shared*>(w += firsts);
+    a.kept = reinterpret_cast<int32_t*>(w += firsts);
+    a.info = reinterpret_cast<Shared*>(w += kepts);
     a.part = reinterpret_cast<float*>(w += infos);
     a.part_ml = reinterpret_cast<float2*>(w += parts);
     a.cta_part = reinterpret_cast<float*>(w += part_mls);

@@ -750,3 +750,41 @@ def test_prefix_own_tokens_join_at_large_scores(backend, dtype, cache):
     want = want_attn(s, scale=scale)
     check_attn(s, alone, want)  # the bound holds where nothing is joined
     check_attn(s, got, want)
+
+
+def crowd(lens, shared, cache=BF16):
+    """Requests over one text of 2000 tokens and some; 4 key-value heads of 64."""
+    s = make_attn([2040], 8, 4, 64, 16, "HND", BF16, cache, 9)
+    s["table"] = np.repeat(s["table"], len(lens), 0)
+    s["lens"] = np.array(lens, np.int32)
+    s["q"] = plain.normal(12, (len(lens), 8, 64), BF16)
+    s["starts"], s["shared"] = np.array([0, len(lens)], np.int32), np.array([shared], np.int32)
+    return s
+
+
+CROWDS = {"all see it": ([2001 + i % 30 for i in range(160)], 2000, 0, True),
+          "a window of half of it": ([2001 + i % 30 for i in range(400)], 2000, 1000, True),
+          "a small window": ([2001 + i % 30 for i in range(160)], 2000, 64, False),
+          "a window behind it": ([2040] * 160, 1900, 140, False),
+          "idle rows": ([0] * 70 + [2010, 2003] + [-1] * 88, 2000, 0, False),
+          "ended rows in front": ([40] * 150 + [2010] * 10, 2000, 0, False),
+          "shared past every length": ([30 + i % 9 for i in range(160)], 2000, 0, False)}
+
+
+@pytest.mark.parametrize("which", CROWDS)
+def test_prefix_rule_counts_what_requests_see(backend, which):
+    """Tokens are shared where that saves reading them, not where few of the requests, or of the tokens, are left."""
+    lens, common, window, pays = CROWDS[which]
+    s = crowd(lens, common)
+    want = want_attn(s, window=window)
+    on = Running(s, window=window, always=False)
+    device_status()
+    got, none = on.run(), on.run(groups=0)
+    assert device_status() == 0
+    on.close()
+    check_attn(s, got, want)
+    check_attn(s, none, want)
+    same = (got[1].view(np.uint32) == none[1].view(np.uint32)).all()
+    assert same != pays  # 64-bit sums in another order: some of a thousand log-sums differ in their last bit
+    if not pays:
+        bits_equal(got[0], none[0])
