@@ -636,8 +636,11 @@ int mf_paged_attn_destroy(mf_paged_attn handle);
  * A logit of -inf is no candidate, nor is any of a row whose score or sum is
  * not finite (-inf: a beam not in use; NaN or +inf among the logits).  Where
  * there are fewer than n_out candidates, the rest is -inf, -1, -1, 0.
- * Scores are ranked in float64 and rounded once; the sums' terms are float32
- * (2^-22 of themselves), their partial sums float64.
+ * Scores are ranked in float64 and rounded once.  A term of a sum is a product of
+ * up to three float32 exponentials, each good to 2^-22 of itself and 2^-23 more for
+ * every octave between their arguments (a term of the size of the largest has one);
+ * up to 32 terms are added in float32 (2^-21 of their sum), the rest in float64.
+ * Beams whose scores are nearer to one another than that may change places.
  * beams is at most 1024, n_out at most 128, vocab at most 2^30, beams * vocab
  * below 2^31.  A handle
  * holds the workspace for batches of up to max_batch; it is not shared between

@@ -36,6 +36,7 @@ constexpr int kPicked = 512;         // logits that may be ranked by counting
 // 39.5), 7 three (45).
 constexpr int kCtas = 3;
 constexpr float kLog2e = 1.44269504088896341f;
+constexpr float kReach = 8.0f;       // that logits may exceed what a thread's sum is relative to
 
 struct SelectArgs {
     const char* logits;
@@ -422,8 +423,12 @@ __global__ void __launch_bounds__(kThreads, 4) beam_select_kernel(const SelectAr
         const int32_t chunks = min(a.chunks, (a.vocab - first0 + kChunk - 1) / kChunk);
         uint4 vec[V], ahead[V];
         load_chunk<DT, V>(ahead, begin, first0, a.vocab);
-        // sums relative to the thread's own maximum: differences of near logits are exact
-        float most = -INFINITY, sum = 0.0f, of_part[kParts];
+        // Sums of exp(x - ref), ref a maximum that the thread met: differences of near logits are exact.  It is replaced where a
+        // logit exceeds it by kReach, so that what is left of earlier terms (3e-4) makes the factor's error nothing, however often
+        // the maximum rises.  The terms of a chunk are added in pairs in float32 (five steps), the chunks in float64: one float32 sum
+        // of 256 chunks was 4e-6 off.
+        float ref = -INFINITY, of_part[kParts];
+        double sum = 0.0;
         const int32_t each = (chunks + kParts - 1) / kParts;  // chunks of a part
 #pragma unroll
         for (int part = 0; part < kParts; ++part) {
@@ -437,30 +442,39 @@ __global__ void __launch_bounds__(kThreads, 4) beam_select_kernel(const SelectAr
 #pragma unroll
                 for (int v = 0; v < V; ++v) top = fmaxf(top, largest<DT>(vec[v]));
                 of_part[part] = fmaxf(of_part[part], top);
-                if (top > most) {
-                    sum *= exp2_fast((most - top) * kLog2e);  // the first time it is 0 times 0
-                    most = top;
+                if (top > ref + kReach) {
+                    sum *= static_cast<double>(exp2_fast((ref - top) * kLog2e));  // the first time it is 0 times 0
+                    ref = top;
                 }
-                const float less = most == -INFINITY ? 0.0f : most;
-                float2 two = make_float2(0.0f, 0.0f);
+                const float less = ref == -INFINITY ? 0.0f : ref;
+                float2 of_vec[V];
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
                     float x[kPer];
+                    float2 e[kPer / 2];
                     widen<DT>(vec[v], x);
 #pragma unroll
-                    for (int i = 0; i < kPer; i += 2) {
-                        const float2 e = mul2(add2(make_float2(x[i], x[i + 1]), make_float2(-less, -less)), make_float2(kLog2e, kLog2e));
-                        two = add2(two, make_float2(exp2_fast(e.x), exp2_fast(e.y)));
+                    for (int i = 0; i < kPer / 2; ++i) {
+                        e[i] = mul2(add2(make_float2(x[2 * i], x[2 * i + 1]), make_float2(-less, -less)), make_float2(kLog2e, kLog2e));
+                        e[i] = make_float2(exp2_fast(e[i].x), exp2_fast(e[i].y));
                     }
+                    of_vec[v] = add2(e[0], e[1]);
+                    if constexpr (kPer == 8) of_vec[v] = add2(of_vec[v], add2(e[2], e[3]));
                 }
-                sum += two.x + two.y;
+#pragma unroll
+                for (int d = 1; d < V; d *= 2)
+#pragma unroll
+                    for (int v = 0; v + d < V; v += 2 * d) of_vec[v] = add2(of_vec[v], of_vec[v + d]);
+                sum += static_cast<double>(of_vec[0].x + of_vec[0].y);
             }
         }
         // sums of a warp and of the segment in float64
-        float all = most;
+        float most = of_part[0], all = ref;
+#pragma unroll
+        for (int part = 1; part < kParts; ++part) most = fmaxf(most, of_part[part]);
 #pragma unroll
         for (int d = 16; d; d >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, d));
-        double of_warp = most == -INFINITY ? sum : static_cast<double>(sum * exp2_fast((most - all) * kLog2e));
+        double of_warp = ref == -INFINITY ? sum : sum * static_cast<double>(exp2_fast((ref - all) * kLog2e));
 #pragma unroll
         for (int d = 16; d; d >>= 1) of_warp += __shfl_xor_sync(0xffffffffu, of_warp, d);
         if (lane == 0) {

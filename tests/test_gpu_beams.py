@@ -775,3 +775,57 @@ def test_handles_close_after_shutdown_and_keep_nothing(backend, make):
     finally:
         call("mf_init", 0)
     assert torch.cuda.mem_get_info()[0] >= before - (4 << 20)
+
+
+# ------------------------------------------------------------------ selection of rows of many chunks
+
+def many_chunks(rows, chunks, levels):
+    """Sums over whole rows, a row in one segment (three CTAs for every SM and more): `levels`(row) gives a row's 16-bit logits, a
+    vector for each chunk of 8192 that its other tokens have, and the number of the first token, which leads."""
+    import torch
+
+    vocab = chunks * 8192
+    x = torch.empty((rows, chunks, 8192), dtype=torch.bfloat16, device="cuda")
+    sums = np.empty(rows)
+    for r in range(rows):
+        level, lead = levels(r)
+        x[r] = torch.tensor(level, dtype=torch.bfloat16, device="cuda")[:, None]
+        if lead is not None:  # once for every thread: a token of each 8, of the first 2048
+            x[r, 0, :2048:8] = lead
+        terms = np.exp(np.asarray(level, np.float64))
+        sums[r] = math.log((terms.sum() * 8192) + (0 if lead is None else 256 * (math.exp(lead) - terms[0])))
+    top = np.array([max(levels(r)[0].max(), -np.inf if levels(r)[1] is None else levels(r)[1]) for r in range(rows)])
+    scores = (sums - top).astype(np.float32)  # results near 0, where float32 is fine
+    want = scores.astype(np.float64) + top - sums
+    out = [torch.empty(rows, dtype=t, device="cuda") for t in (torch.float32, torch.int32, torch.int32)]
+    sc = torch.tensor(scores, device="cuda")
+    torch.cuda.synchronize()
+    with beams.BeamSelect(BF16, vocab, 1, 1, rows) as h:
+        h.run(x.data_ptr(), sc.data_ptr(), rows, *[o.data_ptr() for o in out])
+        torch.cuda.synchronize()
+    got = out[0].cpu().numpy().astype(np.float64)
+    assert np.array_equal(out[2].cpu().numpy(), np.arange(rows))
+    return np.abs(got - want) - 2.0 ** -24 * np.abs(want), out[1].cpu().numpy()
+
+
+def test_select_sums_of_many_logits(backend):
+    """448 rows of 2 million logits, all but a few alike: a running float32 sum of a thread's 8192 terms is up to 4e-6 off.
+
+    Bound: an exponential 2^-22, its argument 2^-23 for each octave, 32 terms added in float32 in pairs (5 steps, 2^-24 each);
+    the rest is float64."""
+    steps = np.linspace(0x3d00, 0x3e7f, 448).astype(np.uint32)  # 2^-5 to 2^-2 in BF16
+    below = (steps << 16).view(np.float32).astype(np.float64)
+    off, tokens = many_chunks(448, 256, lambda r: (np.full(256, -below[r]), 0.0))
+    assert (tokens == 0).all()
+    assert (off <= 2.0 ** -22 + 5 * 2.0 ** -24 + 2.0 ** -23 * 0.37).all(), off.max()
+
+
+def test_select_sums_of_rising_logits(backend):
+    """The maximum rises with every chunk, by a step of BF16: what was summed is not rounded each time."""
+    def levels(r):
+        return -2.0 + (np.arange(256) + r % 3) * 2.0 ** -7, None
+    off, tokens = many_chunks(448, 256, levels)
+    # up to 2 nepers (2.9 octaves) from the first maximum
+    assert (off <= 2.0 ** -22 + 5 * 2.0 ** -24 + 2.0 ** -23 * 2.9).all(), off.max()
+    # of a step that BF16 does not tell from the next (2^-7 at 1 to 2) the first token counts
+    assert all(255 * 8192 >= t >= 253 * 8192 and t % 8192 == 0 for t in tokens)
