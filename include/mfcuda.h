@@ -701,10 +701,13 @@ int mf_beam_select_destroy(mf_beam_select handle);
  * their other holders rename theirs by `numbers`.
  * After either call run mf_page_copy on the moves before the caches are used.
  *
- * A page number outside the cache (in a table, or in the list of free pages where it
- * is needed), a list of free pages past its buffer or, in compact, with a page twice
- * record MF_DEVICE_BAD_PAGE: the number stays as it is and holds nothing, such a
- * list counts as no more pages than there are.
+ * A page number outside the cache stays as it is and holds nothing.  It records
+ * MF_DEVICE_BAD_PAGE where a call would change who holds the page or hand it out: in
+ * fork in the tables of rows that nobody continues and of further rows, and among the
+ * free pages that are taken (the pages of a row's first child are carried over as they
+ * are, without a look), in compact in every row and in the whole list.  So does a list
+ * of free pages past its buffer or, in compact, with a page twice; such a list counts
+ * as no more pages than there are.
  * The handle holds the workspace for up to max_requests rows; it is not shared
  * between streams that run at once.  One launch. */
 typedef struct mf_page_move {
@@ -737,7 +740,8 @@ int mf_page_book_destroy(mf_page_book handle);
  * two moves, or the src of one and the dst of another.  tokens counts as
  * 0 to page_size.  A move that names a page outside the cache is left out and records
  * MF_DEVICE_BAD_PAGE.  Elements of any dtype of a whole number of bytes; any
- * strides, head_dim contiguous. */
+ * strides from 0 to 2^40, head_dim contiguous, a page's tokens below 2 GB.  One launch
+ * for every 128 caches. */
 int mf_page_copy(const mf_cache_layout* layout, void* const* caches, int32_t n_caches, const mf_page_move* moves,
                  int32_t n_moves, const int32_t* count, mf_stream stream);
 

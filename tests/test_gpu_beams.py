@@ -829,3 +829,23 @@ def test_select_sums_of_rising_logits(backend):
     assert (off <= 2.0 ** -22 + 5 * 2.0 ** -24 + 2.0 ** -23 * 2.9).all(), off.max()
     # of a step that BF16 does not tell from the next (2^-7 at 1 to 2) the first token counts
     assert all(255 * 8192 >= t >= 253 * 8192 and t % 8192 == 0 for t in tokens)
+
+
+@pytest.mark.parametrize("dtype,vocab,beams_,n,pad,offset", [(BF16, 70001, 8, 16, 0, 0), (F32, 40001, 4, 8, 3, 1), (F16, 70001, 7, 40, 1, 5),
+                                                             (BF16, 131073, 64, 100, 0, 0)])
+def test_select_parts_of_several_chunks(backend, dtype, vocab, beams_, n, pad, offset):
+    """448 rows are cut into one segment each, of 9 to 17 chunks: several for each part that a thread keeps a maximum of.  Masked tails,
+    rows that begin anywhere, ended beams, a best token in every chunk."""
+    rng = np.random.default_rng(vocab + n)
+    logits = rng.normal(0, 2.5, (448, vocab)).astype(np.float32)
+    logits[::3, vocab - 700:] = -np.inf
+    chunk = 4096 if dtype == F32 else 8192
+    for c in range(-(-vocab // chunk)):  # the best of some rows stand in one chunk, or one in each
+        at = np.minimum(c * chunk + rng.integers(0, chunk, 448), vocab - 701)
+        logits[np.arange(448), at] = 12.0 + rng.random(448).astype(np.float32)
+    for r in range(0, 448, 16):
+        first = int(rng.integers(0, vocab - 3000))
+        logits[r, first:first + 2 * n] = 20.0 + rng.random(2 * n).astype(np.float32)
+    ended = np.zeros(448, np.int32)
+    ended[beams_ - 1::beams_] = 1
+    run_select(logits, rng.normal(-30, 1, 448), beams_, n, dtype, ended=ended, end=3, stride=vocab + pad, offset=offset)
