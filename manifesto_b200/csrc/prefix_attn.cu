@@ -197,13 +197,14 @@ struct Group {
 };
 // Whether a group's tokens are shared, and whether any are.  The requests of a group follow one another, so that its tokens come
 // out of L2 for all but one of them: reading them again, as far as each of the others sees them (its length, its window), costs
-// 40 ps a token and key-value head of 128 (30 of FP8 codes) with all SMs at work, an item of shared tokens 47 ns (7 us of one
-// CTA), a tile, seen or not, 8 (32 with more than 128 rows), and the first of them all delays the rest.  32/8 heads of 128, BF16,
-// us with sharing and without: 100 groups of 2 that share 48 tokens 84 and 39, 30 groups of 16 with 48 83 and 54, with 800 106
-// and 180; 6 of 16 with 800 62 and 50, with 3200 77 and 95; one of 4 with 896 32 and 20.  One of 250 with 8192 135 and 643; with
-// a window of 128 136 and 40, of 1024 142 and 106, of 2048 143 and 181; 2 of the 250 not idle 87 and 29, 25 85 and 85, 50 86 and
-// 145.
-constexpr float kItemPs = 47e3f, kTilePs = 8e3f, kWideTilePs = 32e3f, kFirstPs = 25e6f;
+// 8 + 0.32 ps an element of a head a token and key-value head with all SMs at work (of FP8 codes 0.64 of that), an item of shared
+// tokens 90 ns, a tile, seen or not, 3 (8 with more than 128 rows; four times as much where a window takes the way of masked
+// tiles), and the first of them all 28 us.  The prices are fitted to 1176 cases with cold caches, both ways timed: 7 shapes of heads
+// of 64 to 256, BF16 and E4M3, 1 to 100 groups of 2 to 250 requests with 48 to 8192 tokens, windows, idle requests.  Calls by the
+// rule take a tenth and 6 us more than the better way in 79 of them (1.4 times at most).  32/8 heads of 128, BF16, us with sharing and
+// without: 100 groups of 2 that share 48 tokens 84 and 39, 30 of 16 with 48 83 and 54, with 800 106 and 180; one of 4 with 896 32
+// and 20; one of 250 with 8192 135 and 643, with a window of 128 136 and 40, with 2 of the 250 not idle 87 and 29.
+constexpr float kItemPs = 90e3f, kTilePs = 3e3f, kWideTilePs = 8e3f, kWindowed = 4.0f, kFirstPs = 28e6f;
 constexpr uint32_t kMasked = 0xffffffffu;
 
 // MODE: dtype of the cache; DP: head_dim padded to 64, 128 or 256.
@@ -265,7 +266,8 @@ template <class K>
 __device__ __forceinline__ float worth_of(const PrefixArgs& a, const Group& x, float again) {
     const float heads = static_cast<float>(a.kv_heads), rows = static_cast<float>(x.members) * static_cast<float>(a.group.d);
     const float tiles = ceilf(static_cast<float>(x.shared) * (1.0f / K::T)), items = ceilf(rows * (1.0f / K::kRows));
-    return heads * (again * a.token_ps - items * (kItemPs + tiles * (rows > 128.0f ? kWideTilePs : kTilePs)));
+    const float tile = (rows > 128.0f ? kWideTilePs : kTilePs) * (a.window > 0 ? kWindowed : 1.0f);
+    return heads * (again * a.token_ps - items * (kItemPs + tiles * tile));
 }
 // The shared tokens that the requests of a group see, and the most of them that one sees.
 struct Seen {
@@ -1254,7 +1256,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_kernel(const PrefixArgs a)
     }
     tc_fence_before();
     __syncthreads();
-    if (tid == 0 && sh.waits.abandoned) atomicExch(a.status, MF_DEVICE_TIMEOUT);
+    if (tid == 0 && sh.waits.abandoned && static_cast<int32_t>(blockIdx.x) < ctas) atomicExch(a.status, MF_DEVICE_TIMEOUT);
     if (warp == kIssuer) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
@@ -1477,7 +1479,7 @@ extern "C" int mf_prefix_attn_create(const mf_paged_attn_config* config, int32_t
     a.page = k.page_size;
     a.always = 0;
     a.wait_ns = kWaitNs;
-    a.token_ps = (10.0f + k.head_dim * (is_fp8(k.dtype) ? 5.0f : 7.5f) / 32.0f) * ((c.q_heads / k.kv_heads + 15) / 16);
+    a.token_ps = (8.0f + 0.32f * k.head_dim) * (is_fp8(k.dtype) ? 0.64f : 1.0f) * ((c.q_heads / k.kv_heads + 15) / 16);
     a.window = c.window;
     a.kv_heads = k.kv_heads;
     a.unit = 1u << unit;

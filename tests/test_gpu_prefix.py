@@ -672,6 +672,18 @@ def test_prefix_waits_that_run_out_are_reported(backend, groups, hq, hkv, dim, d
     on.close()
 
 
+def test_prefix_without_time_to_wait_what_is_not_shared_is_right(backend):
+    s = make_groups([(90, [1, 2]), (40, [3])], 4, 2, 64, 16, "HND", BF16, BF16, 3, alone=2)
+    for always, groups in ((True, 0), (False, None)):
+        on = Running(s, always=always)
+        call("mf_prefix_attn_limit", on.attn._handle, 0)
+        device_status()
+        got = on.run(groups=groups)
+        assert device_status() == 0
+        on.close()
+        check_prefix(s, got, want_attn(s))
+
+
 def test_prefix_limit_refusals(backend):
     s = make_groups([(20, [1, 2])], 4, 2, 64, 16, "HND", BF16, BF16, 3)
     on = Running(s)
