@@ -13,10 +13,11 @@
 // barrier; the n-th largest of the maxima is a bound that n logits reach, and only
 // what the threads met whose maximum reaches it (n of 1024 parts) is read a second
 // time, out of L2.  The few logits that reach the bound are ranked by counting.
-// 64 x 8 rows of 128256 BF16 logits: 39.5 us (20 at the copy rate; the stream is
-// 20, the bound and the second look 6, the merge 4).  Collecting candidates on the
+// 64 x 8 rows of 128256 BF16 logits: 40.1 us (20 at the copy rate): CTAs end between
+// 23 and 35 us, as SMs hold three or four of them, the last 5 of each on the bound,
+// the second look and the ticket; the merge takes 4.  Collecting candidates on the
 // way took 76: the threads of a warp diverge at each, and the bound has to be
-// kept with barriers.  4 rows of 32000: 8.2 us, a chain of twelve dependent steps.
+// kept with barriers.  4 rows of 32000: 8.4 us, a chain of twelve dependent steps.
 #include <new>
 
 #include "mf_launch.cuh"

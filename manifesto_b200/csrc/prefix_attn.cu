@@ -38,17 +38,17 @@
 // a window).  So a row that ends with such a number marks its request for the call,
 // and the second launch reads all of that request's tokens, masked ones not at all.
 //
-// Measured (B200; the whole calls are 2 to 3 us slower since, for the check of what is
-// not finite and the scan for a group's row): 250 requests behind 8192 shared tokens, 32/8 heads of 128, BF16:
-// this kernel 67 us from cold caches (the products at the measured rate of the tensor cores: 20 us,
-// 31 with the low terms), tensor pipe 41% of the time busy.  Bound by latency: a
+// Measured (B200): 250 requests behind 8192 shared tokens, 32/8 heads of 128, BF16: 170 us for the whole call,
+// this kernel 72 from cold caches (the products at the measured rate of the tensor cores: 20 us,
+// 31 with the low terms), tensor pipe 38% of the time busy.  Bound by latency: a
 // step's chain is some 5 thousand clocks (scores 0.5, softmax 2.4 to 3, values 1.0,
 // the rest hand-overs; read in an instrumented copy, which is slower itself), two
 // such chains run at a time, and the issuer waits for a step's products before it
-// lets the next scores into their place.  Of 168 us for the whole call, copies that
-// skipped work took: no softmax 154, no parts written 158, no copies 161.  24 prompts of 8 beams, prefixes ragged to
-// 6000 tokens, E4M3: 97 us from cold caches (23 to read the codes).  Of 141 us for the whole
-// call: no copies 121, no softmax 125, no parts written 130, no conversions 147.
+// lets the next scores into their place.  24 prompts of 8 beams, prefixes ragged to
+// 6000 tokens, E4M3: 149 us, 107 from cold caches (23 to read the codes), tensor pipe 32%.  Copies of an
+// earlier form that skipped work: of 168 us, no softmax 154, no parts written 158, no
+// copies 161; of 141 us over E4M3, then with one term of the weights, no copies 121, no
+// softmax 125, no parts written 130, no conversions 147.
 #include <new>
 
 #include "mf_async.cuh"

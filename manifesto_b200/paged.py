@@ -247,8 +247,9 @@ class PrefixAttention(_Handle):
     """``PagedAttention`` for groups of requests that share the pages of their first tokens (mf_prefix_attn_*).
 
     The shared tokens of a group are read once for all its requests: the beams of a prompt, or a batch that begins
-    with the same instructions; small groups, for which that does not pay, only with ``always``.  Holds the workspace for up to ``max_requests``, so one object serves one stream at
-    a time; it runs any number of requests, groups, steps and layers of its shape."""
+    with the same instructions; groups for which that does not pay (small ones, few requests that see the tokens) only
+    with ``always``.  Holds the workspace for up to ``max_requests``, so one object serves one stream at a time; it runs
+    any number of requests, groups, steps and layers of its shape."""
 
     _destroy = "mf_prefix_attn_destroy"
 
